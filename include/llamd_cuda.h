@@ -74,6 +74,11 @@ void llamd_fwd_set_pdl(int on);
 void llamd_fwd_set_batch_group(int g);
 /* The library's stream as a cudaStream_t, for callers that time with events. */
 void *llamd_fwd_stream(void);
+/* For callers whose buffers are in use on a stream of their own (a cudaStream_t; NULL: the legacy default stream): what is
+ * enqueued through the library from here on waits for what that stream holds now, or the other way round. Neither waits on the
+ * host. 0 / -1. */
+int llamd_fwd_wait_stream(void *other);
+int llamd_fwd_ready_stream(void *other);
 
 /* Device-time stopwatch: CUDA events on the library stream (the discipline of
  * crates/llamd-rocm/kernels/llamd.hip:1120-1141). stop synchronises. */
@@ -421,6 +426,53 @@ void llamd_fwd_matmul_f32_tokens(const float *w, const float *x, float *out, int
  * not cover fall through to llamd_fwd_attention_tile. */
 void llamd_fwd_attention_prefill(const float *q, const float *kc, const float *vc, float *out, float *scores, int n_head,
                                  int n_head_kv, int hd, const int32_t *meta, int max_kv, int ntok, int n_kv_max);
+
+/* ---- paged K/V caches (no counterpart in the reference, whose caches are one slab per sequence,
+ * crates/llamd-runtime/src/kv.rs:27-170) ----
+ * Many sequences share two pools per layer, K and V: [n_pages][n_head_kv][page_size][hd] in 16 bits; position i of a
+ * sequence is slot i % page_size of page pages[i / page_size] of its table. The caller owns pools and tables; any page may
+ * stand in several tables, so sequences with a common beginning hold it once. Results are at TOLERANCE level (f32 sums in any order,
+ * tensor cores, weights of the softmax rounded to the cache's type), not bit for bit those of the ops above.
+ *
+ * A batch is the shape of one step: how many new tokens each sequence has, how many positions in all, and its pages. It is made on
+ * the host once per step (llamd_cuda_paged_set) and used by every layer. New tokens are the last q_len of a sequence's kv_len
+ * positions; packed, sequence after sequence, they are the rows of q, k, v and out. The library keeps a copy of the tables: the
+ * caller's arrays may change after the call. */
+#define LLAMD_PAGED_F16 0
+#define LLAMD_PAGED_BF16 1
+#define LLAMD_PAGED_F32 2
+/* hd 64 or 128; n_head / n_head_kv a whole number up to 64; page_size a power of two, 16 to 4096; type (of q_out, out and the
+ * pools) LLAMD_PAGED_F16 or _BF16. NULL and a message where refused. */
+void *llamd_cuda_paged_new(int n_head, int n_head_kv, int hd, int page_size, int type);
+/* Waits for the launches that read the batch. */
+void llamd_cuda_paged_free(void *batch);
+/* pages: [n_seq][pages_stride], ids below n_pages (the pools' size), of each sequence the first
+ * ceil(kv_len / page_size) are read. q_len may be 0. n_shared: the first n_shared positions (whole pages, the same ids in every
+ * table) are common to all sequences, no sequence has new tokens among them, and attention reads them once for all. Everything is
+ * checked here, before a launch can use it: 0, or -1 and a message, and the batch is as it was. Enqueues one copy; may allocate where
+ * a batch is larger than any before it; not while a graph is captured. A batch that is set again serves the launches enqueued
+ * after the call. */
+int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int32_t *kv_len, const int32_t *pages, int pages_stride,
+                         int n_pages, int n_shared);
+/* The new tokens' q, k, v rows ([tokens][heads][hd], in_type LLAMD_PAGED_F32 or the batch's type; strides in elements
+ * between tokens): q and k normed per head (x / sqrt(mean x^2 + eps) * w, f32 weights [hd]; wq / wk NULL: not normed),
+ * the first `rot` elements of each head rotated (a multiple of 16, 0: not at all; interleaved 0: element i with i + rot / 2, else
+ * 2i with 2i + 1) by the angles of rope_tab ([rope_rows][rot / 2][2] sines and cosines, a row per position), rounded once; q to q_out
+ * (rows out_stride elements apart), k and v to their slots. q_out, the pools and rope_tab start at 16 bytes. Enqueues, does not
+ * synchronise. 0, or -1 and a message where refused: nothing was launched (so too while an earlier error of the library is unread). */
+int llamd_fwd_paged_append(const void *batch, const void *q, const void *k, const void *v, int in_type, size_t q_stride,
+                           size_t k_stride, size_t v_stride, const float *wq, const float *wk, float eps, const float *rope_tab,
+                           int rope_rows, int rot, int interleaved, void *q_out, size_t out_stride, void *k_pages, void *v_pages);
+/* out[token][head] = softmax(scale * q . k) v over the positions up to the token's own. q and out in the batch's type, or out in f32
+ * (out_f32: the same sums, not rounded); rows start at 16 bytes. Slots behind a sequence's last position may hold
+ * anything, NaN and infinities too. 0 / -1 as above. */
+int llamd_fwd_paged_attention(const void *batch, const void *q, size_t q_stride, const void *k_pages, const void *v_pages, void *out,
+                              size_t out_stride, int out_f32, float scale);
+/* The table of llamd_fwd_paged_append on the host: sine and cosine of r * f_i, f_i = base^(-2i / rot), evaluated in double.
+ * scaling 0: as it is; 1: f / factor (positions stretched); 2: base * factor^(rot / (rot - 2)) in place of base; 3: by frequency,
+ * f / factor for those that turn less than once over `original` positions, f for those that turn 32 times and more, a ramp
+ * between, and all values times 0.1 ln(factor) + 1. */
+int llamd_cuda_rope_table_scaled(float *host_out, int rows, int rot, float freq_base, int scaling, float factor, int original);
 
 #ifdef __cplusplus
 }

@@ -36,6 +36,8 @@ SIGNATURES = {
     "llamd_fwd_last_error": (i32, []),
     "llamd_fwd_stream_init": (i32, []),
     "llamd_fwd_stream": (vp, []),
+    "llamd_fwd_wait_stream": (i32, [vp]),
+    "llamd_fwd_ready_stream": (i32, [vp]),
     "llamd_fwd_launch_count": (C.c_ulonglong, []),
     "llamd_fwd_set_pdl": (None, [i32]),
     "llamd_fwd_set_batch_group": (None, [i32]),
@@ -147,6 +149,12 @@ SIGNATURES = {
     "llamd_fwd_matvec_q8_0_status": (i32, []),
     "llamd_fwd_matmul_f32_tokens": (None, [vp, vp, vp, i32, i32, i32]),
     "llamd_fwd_attention_prefill": (None, [vp, vp, vp, vp, vp, i32, i32, i32, vp, i32, i32, i32]),
+    "llamd_cuda_paged_new": (vp, [i32, i32, i32, i32, i32]),
+    "llamd_cuda_paged_free": (None, [vp]),
+    "llamd_cuda_paged_set": (i32, [vp, i32, vp, vp, vp, i32, i32, i32]),
+    "llamd_fwd_paged_append": (i32, [vp, vp, vp, vp, i32, sz, sz, sz, vp, vp, f32, vp, i32, i32, i32, vp, sz, vp, vp]),
+    "llamd_fwd_paged_attention": (i32, [vp, vp, sz, vp, vp, vp, sz, i32, f32]),
+    "llamd_cuda_rope_table_scaled": (i32, [vp, i32, i32, f32, i32, f32, i32]),
     "llamd_fwd_moe_group": (None, [vp, i32, i32, i32, vp, vp, vp, vp]),
     "llamd_fwd_moe_group_work": (None, [vp, i32, i32, i32, vp, vp, vp, vp, vp, vp]),
 }

@@ -1,0 +1,443 @@
+// Batches over paged K/V caches: the batch itself (lengths, page tables and what the launches need of them, on the host and
+// copied to the device once per step), and the append of new tokens: QK-norm, rotation and the store into the pages in one pass.
+#include <math.h>
+#include <string.h>
+
+#include <algorithm>
+#include <new>
+#include <vector>
+
+#include "paged.cuh"
+
+namespace llamd {
+namespace {
+
+struct Batch {
+    PagedView view = {};
+    int type = 0, n_pages = 0, max_kv = 0;
+    bool ready = false;
+    // the device copy of everything below, and the pinned memory it is made in
+    uint8_t *dev = nullptr, *host = nullptr;
+    size_t dev_bytes = 0, host_bytes = 0;
+    cudaEvent_t copied = nullptr;
+
+    ~Batch() {
+        // (frees wait for the stream: launches that read the batch are done)
+        if (dev || host) cudaStreamSynchronize(stream());
+        if (dev) cudaFree(dev);
+        if (host) cudaFreeHost(host);
+        if (copied) cudaEventDestroy(copied);
+    }
+    // Room for n bytes on both sides; the pinned side is not written before the copy out of it is done.
+    bool reserve(size_t n) {
+        if (!copied && cudaEventCreateWithFlags(&copied, cudaEventDisableTiming) != cudaSuccess) return fail("paged batch: event");
+        if (cudaEventSynchronize(copied) != cudaSuccess) return fail("paged batch: previous copy");
+        if (n > host_bytes) {
+            if (host) cudaFreeHost(host);
+            host = nullptr;
+            host_bytes = 0;
+            if (cudaHostAlloc((void **)&host, 2 * n, cudaHostAllocDefault) != cudaSuccess) return fail("paged batch: pinned memory");
+            host_bytes = 2 * n;
+        }
+        if (n > dev_bytes) {
+            if (dev && cudaStreamSynchronize(stream()) != cudaSuccess) return fail("paged batch: sync");
+            if (dev) cudaFree(dev);
+            dev = nullptr;
+            dev_bytes = 0;
+            if (cudaMalloc((void **)&dev, 2 * n) != cudaSuccess) return fail("paged batch: device memory");
+            dev_bytes = 2 * n;
+        }
+        return true;
+    }
+    bool fail(const char *what) {
+        set_error(cudaGetLastError(), what);
+        return false;
+    }
+};
+
+// One section of the batch's memory: n elements at a 16-byte boundary.
+template <typename T>
+size_t section(size_t &at, size_t n) {
+    const size_t here = at;
+    at += (n * sizeof(T) + 15) & ~(size_t)15;
+    return here;
+}
+
+const char *check_lengths(const Batch &b, int n_seq, const int32_t *q_len, const int32_t *kv_len, const int32_t *pages, int pages_stride, int n_pages,
+                          int n_shared) {
+    const int page = b.view.page;
+    if (n_seq < 0 || n_pages < 1 || n_shared < 0 || (n_seq && (!q_len || !kv_len || !pages))) return "paged batch: sizes";
+    if ((long long)n_pages * b.view.n_head_kv * page > 0x7fffffffLL) return "paged batch: pools of more than 2^31 rows";
+    if (n_shared % page) return "paged batch: the shared prefix is whole pages";
+    long long tokens = 0;
+    for (int s = 0; s < n_seq; s++) {
+        if (q_len[s] < 0 || kv_len[s] < q_len[s]) return "paged batch: a sequence has fewer positions than new tokens";
+        if (kv_len[s] - q_len[s] < n_shared) return "paged batch: new tokens inside the shared prefix";
+        const long long used = ((long long)kv_len[s] + page - 1) / page;
+        if (used > pages_stride) return "paged batch: a table has fewer pages than its sequence";
+        const int32_t *t = pages + (size_t)s * pages_stride;
+        for (long long i = 0; i < used; i++)
+            if (t[i] < 0 || t[i] >= n_pages) return "paged batch: a page id outside the pools";
+        if (s && memcmp(t, pages, (size_t)(n_shared / page) * sizeof(int32_t))) return "paged batch: the shared prefix's pages differ";
+        tokens += q_len[s];
+    }
+    if (tokens * b.view.n_head > 0x7fffffffLL) return "paged batch: too many tokens";
+    return nullptr;
+}
+
+// ---- append --------------------------------------------------------------------------------------------------------------
+//
+//   y = x / sqrt(mean(x^2) + eps) * w        per head of q and k (weights given), in f32
+//   (a, b) -> (a cos - b sin, a sin + b cos) for the pairs among a head's first `rot` elements
+//   q_out <- y; the K and V rows of the token's slot <- y, v, rounded once to the cache's type
+//
+// Bytes bound it: every input is read once, every output written once, and a warp has kAppendVecs loads of 16 bytes a lane in flight
+// before it needs the first. A head takes hd / E lanes, E elements (16 bytes) to a lane, so the norm is a sum over
+// neighbouring lanes and a half-rotation's partner is rot / (2 E) lanes away. A warp stays with one token: its angles are read once.
+constexpr int kAppendVecs = 4;
+
+struct AppendParams {
+    PagedView b;
+    const void *q, *k, *v;
+    size_t q_stride, k_stride, v_stride, out_stride;  // elements between tokens
+    const float *wq, *wk, *rope;
+    float eps;
+    int rot, interleaved, aligned, tasks, chunks;
+    void *q_out, *k_pages, *v_pages;
+};
+
+template <typename T, int E> struct AppendIo;
+template <int E> struct AppendIo<float, E> {
+    static_assert(E == 4, "16 bytes");
+    static __device__ __forceinline__ void load(const float *p, bool aligned, float (&x)[E]) {
+        if (aligned) {
+            const float4 f = __ldcs(reinterpret_cast<const float4 *>(p));
+            x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < E; i++) x[i] = p[i];
+        }
+    }
+};
+template <typename T> struct AppendIo<T, 8> {
+    static __device__ __forceinline__ void load(const T *p, bool aligned, float (&x)[8]) {
+        if (aligned) {
+            const uint4 u = __ldcs(reinterpret_cast<const uint4 *>(p));
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float2 f = Half16<T>::to_f32(w[i]);
+                x[2 * i] = f.x, x[2 * i + 1] = f.y;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = (float)p[i];
+        }
+    }
+};
+
+// TI: the inputs' type, T: the cache's. HD / E lanes to a head.
+template <typename TI, typename T, int HD>
+__global__ void __launch_bounds__(256) paged_append_kernel(const AppendParams p) {
+    constexpr int E = 16 / (int)sizeof(TI), L = HD / E, PER = 32 / L;  // heads side by side in a warp
+    pdl_trigger();
+    pdl_wait();
+    const int warp = (int)((blockIdx.x * blockDim.x + threadIdx.x) >> 5), lane = threadIdx.x & 31;
+    if (warp >= p.tasks) return;
+    const int t = warp / p.chunks, c = warp - t * p.chunks, sub = lane / L, l = lane % L, e0 = l * E;
+    const int H = p.b.n_head, K = p.b.n_head_kv, n_vec = H + 2 * K, v0 = c * (kAppendVecs * PER) + sub;
+    float x[kAppendVecs][E];
+#pragma unroll
+    for (int i = 0; i < kAppendVecs; i++) {
+        const int v = v0 + i * PER;
+        const TI *src = reinterpret_cast<const TI *>(p.q) + (size_t)t * p.q_stride + (size_t)v * HD;
+        if (v >= H) src = reinterpret_cast<const TI *>(p.k) + (size_t)t * p.k_stride + (size_t)(v - H) * HD;
+        if (v >= H + K) src = reinterpret_cast<const TI *>(p.v) + (size_t)t * p.v_stride + (size_t)(v - H - K) * HD;
+        if (v < n_vec) AppendIo<TI, E>::load(src + e0, p.aligned, x[i]);
+        else {
+#pragma unroll
+            for (int j = 0; j < E; j++) x[i][j] = 0.0f;
+        }
+    }
+    const PagedToken tok = p.b.token[t];
+    // the angles of this lane's elements: the pair (a, b) holds x[j] and its partner
+    float sn[E], cs[E];
+    const int half = p.rot >> 1;
+    if (e0 < p.rot) {
+        const float *row = p.rope + (size_t)tok.pos * p.rot;
+        if (p.interleaved) {
+#pragma unroll
+            for (int j = 0; j < E; j += 4) {
+                const float4 f = __ldg(reinterpret_cast<const float4 *>(row + e0 + j));
+                sn[j] = sn[j + 1] = f.x, cs[j] = cs[j + 1] = f.y;
+                sn[j + 2] = sn[j + 3] = f.z, cs[j + 2] = cs[j + 3] = f.w;
+            }
+        } else {
+            const int i0 = e0 < half ? e0 : e0 - half;
+#pragma unroll
+            for (int j = 0; j < E; j += 2) {
+                const float4 f = __ldg(reinterpret_cast<const float4 *>(row + 2 * (i0 + j)));
+                sn[j] = f.x, cs[j] = f.y, sn[j + 1] = f.z, cs[j + 1] = f.w;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < E; j++) sn[j] = 0.0f, cs[j] = 1.0f;
+    }
+    // the sign of the partner's term: the first of a pair loses b sin, the second gains a sin
+#pragma unroll
+    for (int j = 0; j < E; j++)
+        if (p.interleaved ? (j & 1) == 0 : e0 < half) sn[j] = -sn[j];
+    const int hop = half / E, partner = (lane & ~(L - 1)) + (e0 < p.rot ? (l < hop ? l + hop : l - hop) : l);
+    float wq[E], wk[E];
+#pragma unroll
+    for (int j = 0; j < E; j++) wq[j] = p.wq ? __ldg(p.wq + e0 + j) : 1.0f, wk[j] = p.wk ? __ldg(p.wk + e0 + j) : 1.0f;
+#pragma unroll
+    for (int i = 0; i < kAppendVecs; i++) {
+        const int v = v0 + i * PER;
+        const bool is_q = v < H, is_v = v >= H + K;
+        const float *w = is_q ? p.wq : p.wk;
+        // (the shuffles are the whole warp's: heads of other kinds, or beyond the last, come along and drop the result)
+        float ss = 0.0f;
+#pragma unroll
+        for (int j = 0; j < E; j++) ss = fmaf(x[i][j], x[i][j], ss);
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (w && !is_v) {
+            const float r = 1.0f / sqrtf(ss * (1.0f / HD) + p.eps);
+#pragma unroll
+            for (int j = 0; j < E; j++) x[i][j] = x[i][j] * r * (is_q ? wq[j] : wk[j]);
+        }
+        float y[E];
+#pragma unroll
+        for (int j = 0; j < E; j++) {
+            const float far = __shfl_sync(0xffffffffu, x[i][j], partner);
+            const float other = p.interleaved ? x[i][j ^ 1] : far;
+            y[j] = is_v || e0 >= p.rot ? x[i][j] : fmaf(other, sn[j], x[i][j] * cs[j]);
+        }
+        if (v >= n_vec) continue;
+        uint32_t out[E / 2];
+#pragma unroll
+        for (int j = 0; j < E / 2; j++) out[j] = Half16<T>::pack(y[2 * j], y[2 * j + 1]);
+        T *dst;
+        if (is_q) dst = reinterpret_cast<T *>(p.q_out) + (size_t)t * p.out_stride + (size_t)v * HD + e0;
+        else {
+            const size_t row = (size_t)tok.row + (size_t)(is_v ? v - H - K : v - H) * p.b.page;
+            dst = reinterpret_cast<T *>(is_v ? p.v_pages : p.k_pages) + row * HD + e0;
+        }
+        if constexpr (E == 8) *reinterpret_cast<uint4 *>(dst) = make_uint4(out[0], out[1], out[2], out[3]);
+        else *reinterpret_cast<uint2 *>(dst) = make_uint2(out[0], out[1]);
+    }
+}
+
+template <typename TI, typename T>
+void append_launch(AppendParams &p) {
+    const int hd = p.b.hd, per = 32 / (hd * (int)sizeof(TI) / 16);
+    p.chunks = (p.b.n_head + 2 * p.b.n_head_kv + kAppendVecs * per - 1) / (kAppendVecs * per);
+    p.tasks = p.b.tokens * p.chunks;
+    const dim3 grid((unsigned)((p.tasks + 7) / 8));
+    if (hd == 128) launch_k("paged_append", paged_append_kernel<TI, T, 128>, grid, dim3(256), 0, p);
+    else launch_k("paged_append", paged_append_kernel<TI, T, 64>, grid, dim3(256), 0, p);
+}
+
+// ---- attention, one warp per (token, head) -------------------------------------------------------------------------------
+
+struct AttnParams {
+    PagedView b;
+    const void *q, *k_pages, *v_pages;
+    void *out;
+    size_t q_stride, out_stride;
+    int out_f32;
+    float scale;
+};
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(128) paged_attention_kernel(const AttnParams p) {
+    constexpr int E = HD / 32;  // elements to a lane
+    pdl_trigger();
+    pdl_wait();
+    const int warp = (int)((blockIdx.x * blockDim.x + threadIdx.x) >> 5), lane = threadIdx.x & 31;
+    if (warp >= p.b.tokens * p.b.n_head) return;
+    const int t = warp / p.b.n_head, h = warp - t * p.b.n_head, hk = h / p.b.group;
+    const int32_t *table = p.b.table + (size_t)p.b.token_seq[t] * p.b.table_stride;
+    const T *q = reinterpret_cast<const T *>(p.q) + (size_t)t * p.q_stride + (size_t)h * HD + lane * E;
+    float x[E], o[E], m = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < E; j++) x[j] = (float)q[j] * p.scale, o[j] = 0.0f;
+    const int last = p.b.token[t].pos;
+    for (int i = 0; i <= last; i++) {
+        const size_t row = ((size_t)table[i / p.b.page] * p.b.n_head_kv + hk) * p.b.page + i % p.b.page;
+        const T *k = reinterpret_cast<const T *>(p.k_pages) + row * HD + lane * E, *v = reinterpret_cast<const T *>(p.v_pages) + row * HD + lane * E;
+        float s = 0.0f;
+#pragma unroll
+        for (int j = 0; j < E; j++) s = fmaf(x[j], (float)k[j], s);
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+        const float m2 = fmaxf(m, s), a = expf(m - m2), e = expf(s - m2);
+        m = m2;
+        sum = fmaf(sum, a, e);
+#pragma unroll
+        for (int j = 0; j < E; j++) o[j] = fmaf(o[j], a, e * (float)v[j]);
+    }
+    const size_t at = (size_t)t * p.out_stride + (size_t)h * HD + lane * E;
+#pragma unroll
+    for (int j = 0; j < E; j++) {
+        if (p.out_f32) reinterpret_cast<float *>(p.out)[at + j] = o[j] / sum;
+        else reinterpret_cast<T *>(p.out)[at + j] = (T)(o[j] / sum);
+    }
+}
+
+template <typename T>
+void attention_launch(const AttnParams &p) {
+    const dim3 grid((unsigned)(((size_t)p.b.tokens * p.b.n_head + 3) / 4));
+    if (p.b.hd == 128) launch_k("paged_attention", paged_attention_kernel<T, 128>, grid, dim3(128), 0, p);
+    else launch_k("paged_attention", paged_attention_kernel<T, 64>, grid, dim3(128), 0, p);
+}
+
+int refuse(const char *why) {
+    set_error_msg(why);
+    return -1;
+}
+bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+}  // namespace
+}  // namespace llamd
+
+using namespace llamd;
+
+extern "C" {
+
+void *llamd_cuda_paged_new(int n_head, int n_head_kv, int hd, int page_size, int type) {
+    if (n_head < 1 || n_head_kv < 1 || n_head % n_head_kv || n_head / n_head_kv > 64 || (hd != 64 && hd != 128) || page_size < 16 || page_size > 4096 ||
+        (page_size & (page_size - 1)) || (type != kPagedF16 && type != kPagedBf16)) {
+        set_error_msg("paged batch: heads of 64 or 128 elements, up to 64 query heads to a kv head, pages of 16 to 4096 positions (a power of two), f16 or bf16");
+        return nullptr;
+    }
+    if (!stream()) return nullptr;
+    Batch *b = new (std::nothrow) Batch;
+    if (!b) {
+        set_error_msg("paged batch: out of host memory");
+        return nullptr;
+    }
+    b->view.n_head = n_head, b->view.n_head_kv = n_head_kv, b->view.group = n_head / n_head_kv, b->view.hd = hd, b->view.page = page_size;
+    b->type = type;
+    return b;
+}
+
+void llamd_cuda_paged_free(void *batch) { delete (Batch *)batch; }
+
+int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int32_t *kv_len, const int32_t *pages, int pages_stride, int n_pages,
+                         int n_shared) {
+    Batch *b = (Batch *)batch;
+    if (!b) return refuse("paged batch: null");
+    if (const char *why = check_lengths(*b, n_seq, q_len, kv_len, pages, pages_stride, n_pages, n_shared)) return refuse(why);
+    b->ready = false;
+    PagedView &v = b->view;
+    v.n_seq = n_seq, v.n_shared = n_shared, v.tokens = 0, v.table_stride = 1;
+    b->n_pages = n_pages, b->max_kv = 0;
+    for (int s = 0; s < n_seq; s++) {
+        v.tokens += q_len[s];
+        b->max_kv = std::max(b->max_kv, kv_len[s]);
+        v.table_stride = std::max(v.table_stride, (kv_len[s] + v.page - 1) / v.page);
+    }
+    size_t bytes = 0;
+    const size_t o_token = section<PagedToken>(bytes, v.tokens), o_seq = section<int32_t>(bytes, v.tokens),
+                 o_table = section<int32_t>(bytes, (size_t)n_seq * v.table_stride);
+    if (!b->reserve(std::max<size_t>(bytes, 16))) return -1;
+    PagedToken *token = (PagedToken *)(b->host + o_token);
+    int32_t *seq = (int32_t *)(b->host + o_seq), *table = (int32_t *)(b->host + o_table);
+    for (int s = 0, t = 0; s < n_seq; s++) {
+        const int32_t *from = pages + (size_t)s * pages_stride;
+        const int used = (kv_len[s] + v.page - 1) / v.page;
+        for (int i = 0; i < v.table_stride; i++) table[(size_t)s * v.table_stride + i] = i < used ? from[i] : 0;
+        for (int pos = kv_len[s] - q_len[s]; pos < kv_len[s]; pos++, t++) {
+            token[t] = {pos, from[pos / v.page] * v.n_head_kv * v.page + pos % v.page};
+            seq[t] = s;
+        }
+    }
+    v.token = (const PagedToken *)(b->dev + o_token);
+    v.token_seq = (const int32_t *)(b->dev + o_seq);
+    v.table = (const int32_t *)(b->dev + o_table);
+    LLAMD_TRY(cudaMemcpyAsync(b->dev, b->host, bytes, cudaMemcpyHostToDevice, stream()), "paged batch: copy");
+    LLAMD_TRY(cudaEventRecord(b->copied, stream()), "paged batch: event");
+    b->ready = true;
+    return 0;
+}
+
+int llamd_fwd_paged_append(const void *batch, const void *q, const void *k, const void *v, int in_type, size_t q_stride, size_t k_stride, size_t v_stride,
+                            const float *wq, const float *wk, float eps, const float *rope_tab, int rope_rows, int rot, int interleaved, void *q_out,
+                            size_t out_stride, void *k_pages, void *v_pages) {
+    const Batch *b = (const Batch *)batch;
+    if (!b || !b->ready) return refuse("paged append: the batch is not set");
+    if (error_code()) return -1;
+    const PagedView &g = b->view;
+    if (!g.tokens) return 0;
+    if (!q || !k || !v || !q_out || !k_pages || !v_pages) return refuse("paged append: a buffer is missing");
+    if (in_type != kPagedF32 && in_type != b->type) return refuse("paged append: inputs are f32 or of the cache's type");
+    if (rot < 0 || rot > g.hd || rot % 16) return refuse("paged append: the rotated part is a multiple of 16 elements");
+    if (rot && (!rope_tab || rope_rows < b->max_kv || !aligned16(rope_tab))) return refuse("paged append: the angles' table is shorter than the sequences, or not at 16 bytes");
+    const size_t qd = (size_t)g.n_head * g.hd, kvd = (size_t)g.n_head_kv * g.hd;
+    if (q_stride < qd || k_stride < kvd || v_stride < kvd || out_stride < qd) return refuse("paged append: a row overlaps the next");
+    if (!aligned16(q_out) || out_stride % 8 || !aligned16(k_pages) || !aligned16(v_pages)) return refuse("paged append: outputs start at 16 bytes");
+    AppendParams p = {};
+    p.b = g;
+    p.q = q, p.k = k, p.v = v, p.q_stride = q_stride, p.k_stride = k_stride, p.v_stride = v_stride, p.out_stride = out_stride;
+    p.wq = wq, p.wk = wk, p.eps = eps, p.rope = rope_tab, p.rot = rot, p.interleaved = interleaved;
+    p.q_out = q_out, p.k_pages = k_pages, p.v_pages = v_pages;
+    const size_t per16 = in_type == kPagedF32 ? 4 : 8;
+    p.aligned = aligned16(q) && aligned16(k) && aligned16(v) && !(q_stride % per16) && !(k_stride % per16) && !(v_stride % per16);
+    if (b->type == kPagedF16) {
+        if (in_type == kPagedF32) append_launch<float, __half>(p);
+        else append_launch<__half, __half>(p);
+    } else {
+        if (in_type == kPagedF32) append_launch<float, __nv_bfloat16>(p);
+        else append_launch<__nv_bfloat16, __nv_bfloat16>(p);
+    }
+    return error_code() ? -1 : 0;
+}
+
+int llamd_fwd_paged_attention(const void *batch, const void *q, size_t q_stride, const void *k_pages, const void *v_pages, void *out, size_t out_stride,
+                               int out_f32, float scale) {
+    const Batch *b = (const Batch *)batch;
+    if (!b || !b->ready) return refuse("paged attention: the batch is not set");
+    if (error_code()) return -1;
+    const PagedView &g = b->view;
+    if (!g.tokens) return 0;
+    const size_t qd = (size_t)g.n_head * g.hd;
+    if (!q || !k_pages || !v_pages || !out) return refuse("paged attention: a buffer is missing");
+    if (q_stride < qd || out_stride < qd) return refuse("paged attention: a row overlaps the next");
+    if (!aligned16(q) || q_stride % 8 || !aligned16(out) || out_stride % 8 || !aligned16(k_pages) || !aligned16(v_pages))
+        return refuse("paged attention: buffers and rows start at 16 bytes");
+    AttnParams p = {};
+    p.b = g, p.q = q, p.k_pages = k_pages, p.v_pages = v_pages, p.out = out, p.q_stride = q_stride, p.out_stride = out_stride;
+    p.out_f32 = out_f32, p.scale = scale;
+    if (b->type == kPagedF16) attention_launch<__half>(p);
+    else attention_launch<__nv_bfloat16>(p);
+    return error_code() ? -1 : 0;
+}
+
+// The angles' table of llamd_fwd_paged_append, in double and rounded once.
+int llamd_cuda_rope_table_scaled(float *host_out, int rows, int rot, float freq_base, int scaling, float factor, int original) {
+    if (!host_out || rows < 0 || rot < 2 || rot % 2 || !(freq_base > 0.0f) || scaling < 0 || scaling > 3 || (scaling && !(factor >= 1.0f)) ||
+        (scaling == 3 && original < 1)) {
+        return refuse("rope table: sizes");
+    }
+    const int half = rot / 2;
+    const double pi = 3.14159265358979323846, base = scaling == 2 && rot > 2 ? freq_base * pow(factor, rot / (rot - 2.0)) : freq_base;
+    const double magnitude = scaling == 3 ? 0.1 * log(factor) + 1.0 : 1.0;
+    for (int i = 0; i < half; i++) {
+        double f = pow(base, -2.0 * i / rot);
+        if (scaling == 1) f /= factor;
+        if (scaling == 3) {  // frequencies that turn 32 times and more over the trained context stay, below once they are stretched
+            const double turns = original * f / (2.0 * pi), keep = std::min(1.0, std::max(0.0, (turns - 1.0) / 31.0));
+            f = keep * f + (1.0 - keep) * f / factor;
+        }
+        for (int r = 0; r < rows; r++) {
+            host_out[((size_t)r * half + i) * 2] = (float)(magnitude * sin(r * f));
+            host_out[((size_t)r * half + i) * 2 + 1] = (float)(magnitude * cos(r * f));
+        }
+    }
+    return 0;
+}
+
+}  // extern "C"

@@ -384,6 +384,19 @@ void llamd_fwd_set_pdl(int on) { g_pdl = on == 1 ? 7 : on; }
 void llamd_fwd_set_batch_group(int g) { g_batch_group = g < 0 ? 0 : g; }
 void *llamd_fwd_stream(void) { return (void *)stream(); }
 
+// `after` waits for what `first` holds now, through an event that the two need only here.
+static int order_streams(cudaStream_t first, cudaStream_t after) {
+    cudaEvent_t e = nullptr;
+    LLAMD_TRY(cudaEventCreateWithFlags(&e, cudaEventDisableTiming), "event create");
+    cudaError_t rc = cudaEventRecord(e, first);
+    if (rc == cudaSuccess) rc = cudaStreamWaitEvent(after, e, 0);
+    cudaEventDestroy(e);  // (kept by the driver until the wait is over)
+    LLAMD_TRY(rc, "order streams");
+    return 0;
+}
+int llamd_fwd_wait_stream(void *other) { return stream() ? order_streams((cudaStream_t)other, stream()) : -1; }
+int llamd_fwd_ready_stream(void *other) { return stream() ? order_streams(stream(), (cudaStream_t)other) : -1; }
+
 // Device-time stopwatch on the library stream (CUDA events).
 static cudaEvent_t g_t0 = nullptr, g_t1 = nullptr;
 int llamd_fwd_timer_start(void) {

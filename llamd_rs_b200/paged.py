@@ -1,0 +1,237 @@
+"""Many sequences over paged K/V caches: page bookkeeping, the batch of one step, and its two operators.
+
+``Pages`` hands out page ids and counts who holds them; sequences that begin alike hold the beginning's pages together
+(``fork``). ``Batch`` is the shape of one step, set once and used by every layer: ``append`` norms, rotates and stores the new
+tokens, ``attention`` attends them. Buffers are the caller's, on the device: ``DevBuf``, a plain address, or anything with
+``data_ptr()`` (a torch tensor), whose type, shape and strides are then checked. The calls enqueue on the library's stream
+and do not wait; a caller whose buffers are in use on another stream orders the two with ``wait_for`` and ``ready_for``.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+
+import numpy as np
+
+from . import backend
+from ._lib import lib
+from .backend import DevBuf, LlamdError, Malformed, Other, ShapeError, Unsupported
+
+TYPES = {"f16": 0, "bf16": 1, "f32": 2}
+_SIZE = {0: 2, 1: 2, 2: 4}
+_TORCH = {"torch.float16": 0, "torch.bfloat16": 1, "torch.float32": 2}
+_seen = {}  # a tensor's dtype -> its number here, filled as they come
+SCALING = {"none": 0, "linear": 1, "base": 2, "by_frequency": 3}
+
+
+class OutOfPages(LlamdError):
+    pass
+
+
+def _type_of(x):
+    t = _seen.get(x.dtype)
+    if t is None:
+        t = _seen[x.dtype] = _TORCH.get(str(x.dtype), -1)
+    return t
+
+
+def _refuse(what):
+    """The last call's own refusal as an error, read so that the next call starts clean."""
+    why = backend._last_error() or what
+    if lib().llamd_fwd_last_error() > 0:  # not a refusal: the device's own
+        raise Other(why)
+    raise Malformed(why)
+
+
+def rope_table(rows: int, rot: int, freq_base: float, scaling: str = "none", factor: float = 1.0, original: int = 0) -> np.ndarray:
+    """[rows][rot / 2][2] sines and cosines for ``Batch.append`` (llamd_cuda_rope_table_scaled)."""
+    if scaling not in SCALING:
+        raise Unsupported(f"rope scaling {scaling!r}: one of {', '.join(SCALING)}")
+    if rows < 0 or rot < 2 or rot % 2:
+        raise ShapeError(f"rope table of {rows} rows, {rot} elements")
+    out = np.empty((rows, rot // 2, 2), dtype=np.float32)
+    if lib().llamd_cuda_rope_table_scaled(backend._ptr(out), rows, rot, freq_base, SCALING[scaling], factor, original) != 0:
+        _refuse("rope table")
+    return out
+
+
+class Pages:
+    """Which pages of a pool are free, and how many sequences hold each of the others."""
+
+    def __init__(self, n_pages: int, page_size: int):
+        if n_pages < 1 or page_size < 16 or page_size > 4096 or page_size & (page_size - 1):
+            raise ShapeError(f"{n_pages} pages of {page_size} positions")
+        self.n_pages, self.page_size = n_pages, page_size
+        self._free = list(range(n_pages - 1, -1, -1))
+        self._held = [0] * n_pages
+
+    def free(self) -> int:
+        return len(self._free)
+
+    def grow(self, table: list, n_pos: int) -> None:
+        """Adds pages to ``table`` until it holds n_pos positions; all or none."""
+        more = -(-n_pos // self.page_size) - len(table)
+        if more > len(self._free):
+            raise OutOfPages(f"{more} pages wanted, {len(self._free)} free")
+        for _ in range(more):
+            table.append(self._free.pop())
+            self._held[table[-1]] = 1
+
+    def fork(self, table: list, n_pos: int) -> list:
+        """A table of another sequence that begins with the first n_pos positions (whole pages) of this one."""
+        if n_pos % self.page_size or n_pos > len(table) * self.page_size:
+            raise Malformed(f"{n_pos} positions of {len(table)} pages of {self.page_size} cannot be shared")
+        shared = list(table[:n_pos // self.page_size])
+        for p in shared:
+            self._held[p] += 1
+        return shared
+
+    def release(self, table: list) -> None:
+        """The sequence is done: pages that nobody else holds are free again."""
+        for p in table:
+            if self._held[p] < 1:
+                raise Malformed(f"page {p} is released twice")
+            self._held[p] -= 1
+            if not self._held[p]:
+                self._free.append(p)
+        table.clear()
+
+
+class Batch:
+    """One step's sequences over caches of one geometry (llamd_cuda_paged_new)."""
+
+    def __init__(self, n_head: int, n_head_kv: int, head_dim: int, page_size: int, dtype: str = "f16"):
+        self.ptr = None
+        if dtype not in ("f16", "bf16"):
+            raise Unsupported(f"a paged cache holds f16 or bf16, not {dtype}")
+        backend._need_device()
+        self.type = TYPES[dtype]
+        self.n_head, self.n_head_kv, self.head_dim, self.page_size = n_head, n_head_kv, head_dim, page_size
+        self.ptr = lib().llamd_cuda_paged_new(n_head, n_head_kv, head_dim, page_size, self.type)
+        if not self.ptr:
+            _refuse("paged batch")
+        self.tokens, self.n_pages = 0, 0
+        self._pool_bytes = 0
+
+    def set(self, q_lens, kv_lens, pages, n_pages: int, n_shared: int = 0) -> None:
+        """q_lens, kv_lens: new tokens and positions in all of every sequence; pages: their tables, rows of one int32 array or a
+        list of lists; n_pages: the pools' size; n_shared: positions at the beginning that all of them have in common."""
+        q = np.ascontiguousarray(q_lens, dtype=np.int32).ravel()
+        kv = np.ascontiguousarray(kv_lens, dtype=np.int32).ravel()
+        if not isinstance(pages, np.ndarray):
+            rows = [list(r) for r in pages]
+            pages = np.zeros((len(rows), max([len(r) for r in rows] + [1])), dtype=np.int32)
+            for i, r in enumerate(rows):
+                pages[i, :len(r)] = r
+                pages[i, len(r):] = -1  # (refused where a sequence reaches it)
+        pages = np.ascontiguousarray(pages, dtype=np.int32)
+        if q.size != kv.size or pages.ndim != 2 or pages.shape[0] != q.size:
+            raise ShapeError(f"{q.size} new-token counts, {kv.size} lengths, tables {pages.shape}")
+        if lib().llamd_cuda_paged_set(self.ptr, q.size, backend._ptr(q), backend._ptr(kv), backend._ptr(pages), pages.shape[1], n_pages, n_shared) != 0:
+            _refuse("paged batch")
+        self.tokens, self.n_pages = int(q.sum()), n_pages
+        self._pool_bytes = 2 * n_pages * self.n_head_kv * self.page_size * self.head_dim
+
+    def _rows(self, x, heads, type_, what, stride=None):
+        """(address, elements between tokens) of `tokens` rows of `heads` heads."""
+        n = heads * self.head_dim
+        if hasattr(x, "data_ptr"):
+            shape, st = x.shape, x.stride()
+            if _type_of(x) != type_ or not x.is_cuda:
+                raise ShapeError(f"{what}: {x.dtype} on {x.device}")
+            if shape[0] != self.tokens or x.numel() != self.tokens * n or st[-1] != 1 or (len(shape) == 3 and (shape[2] != self.head_dim or (heads > 1 and st[1] != self.head_dim))):
+                raise ShapeError(f"{what}: {tuple(shape)} with strides {st} for {self.tokens} tokens of {heads} heads of {self.head_dim}")
+            return x.data_ptr(), st[0] if shape[0] > 1 else n
+        stride = n if stride is None else stride
+        if isinstance(x, DevBuf):
+            if self.tokens and x.nbytes < ((self.tokens - 1) * stride + n) * _SIZE[type_]:
+                raise ShapeError(f"{what}: {x.nbytes} bytes for {self.tokens} tokens")
+            return x.ptr, stride
+        return x, stride
+
+    def _pool(self, x, what):
+        if hasattr(x, "data_ptr"):
+            if _type_of(x) != self.type or not x.is_cuda or not x.is_contiguous() or x.numel() * 2 < self._pool_bytes:
+                raise ShapeError(f"{what}: {x.dtype}, {tuple(x.shape)} for {self.n_pages} pages")
+            return x.data_ptr()
+        if isinstance(x, DevBuf):
+            if x.nbytes < self._pool_bytes:
+                raise ShapeError(f"{what}: {x.nbytes} bytes for {self.n_pages} pages")
+            return x.ptr
+        return x
+
+    def _f32(self, x, n, what):
+        if x is None:
+            return None
+        if hasattr(x, "data_ptr"):
+            if _type_of(x) != 2 or not x.is_cuda or not x.is_contiguous() or x.numel() < n:
+                raise ShapeError(f"{what}: {x.dtype}, {tuple(x.shape)}")
+            return x.data_ptr()
+        if isinstance(x, DevBuf):
+            if x.nbytes < 4 * n:
+                raise ShapeError(f"{what}: {x.nbytes} bytes for {n} values")
+            return x.ptr
+        return x
+
+    def append(self, q, k, v, q_out, k_pages, v_pages, rope=None, rot: int | None = None, interleaved: bool = False, q_norm=None, k_norm=None,
+               eps: float = 1e-6, inputs: str | None = None, rope_rows: int | None = None, strides=(None, None, None)) -> None:
+        """llamd_fwd_paged_append. ``inputs`` ("f32" or the cache's type) and ``strides`` (elements between tokens of q, k, v)
+        describe buffers that are plain addresses or ``DevBuf``; a tensor says so itself, and its table how many rows it has."""
+        if inputs is None:
+            it = _type_of(q) if hasattr(q, "data_ptr") else 2
+        else:
+            it = TYPES.get(inputs, -1)
+        if it != 2 and it != self.type:
+            raise Unsupported("append takes f32 or the cache's type")
+        rot = (0 if rope is None else self.head_dim) if rot is None else rot
+        if rot and rope is None:
+            raise Malformed("a rotation without its angles")
+        if rope_rows is None:
+            if not rot:
+                rope_rows = 0
+            elif hasattr(rope, "data_ptr"):
+                rope_rows = rope.numel() // rot
+            elif isinstance(rope, DevBuf):
+                rope_rows = rope.nbytes // (4 * rot)
+            else:
+                raise Malformed("rope_rows: how many positions the table has")
+        (qp, qs), (kp, ks), (vp, vs) = (self._rows(x, h, it, w, st) for x, h, w, st in (
+            (q, self.n_head, "q", strides[0]), (k, self.n_head_kv, "k", strides[1]), (v, self.n_head_kv, "v", strides[2])))
+        op, os_ = self._rows(q_out, self.n_head, self.type, "q_out")
+        if lib().llamd_fwd_paged_append(self.ptr, qp, kp, vp, it, qs, ks, vs, self._f32(q_norm, self.head_dim, "q_norm"),
+                                     self._f32(k_norm, self.head_dim, "k_norm"), eps, self._f32(rope, rope_rows * rot, "rope") if rot else None, rope_rows,
+                                     rot, 1 if interleaved else 0, op, os_, self._pool(k_pages, "k_pages"), self._pool(v_pages, "v_pages")) != 0:
+            _refuse("append")
+
+    def attention(self, q, k_pages, v_pages, out, scale: float | None = None, out_f32: bool | None = None) -> None:
+        """llamd_fwd_paged_attention. ``out_f32`` says of an address that it takes f32; a tensor's type says so itself."""
+        if out_f32 is None:
+            out_f32 = hasattr(out, "data_ptr") and _type_of(out) == 2
+        qp, qs = self._rows(q, self.n_head, self.type, "q")
+        op, os_ = self._rows(out, self.n_head, 2 if out_f32 else self.type, "out")
+        if lib().llamd_fwd_paged_attention(self.ptr, qp, qs, self._pool(k_pages, "k_pages"), self._pool(v_pages, "v_pages"), op, os_, 1 if out_f32 else 0,
+                                        1.0 / math.sqrt(self.head_dim) if scale is None else scale) != 0:
+            _refuse("attention")
+
+    def free(self) -> None:
+        if self.ptr:
+            lib().llamd_cuda_paged_free(self.ptr)
+            self.ptr = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+def wait_for(stream: int) -> None:
+    """What is enqueued through the library from here on waits for what ``stream`` (a cudaStream_t) holds now."""
+    if lib().llamd_fwd_wait_stream(C.c_void_p(stream)) != 0:
+        raise Other("wait_for: " + backend._last_error())
+
+
+def ready_for(stream: int) -> None:
+    """What is enqueued on ``stream`` from here on waits for what the library's stream holds now."""
+    if lib().llamd_fwd_ready_stream(C.c_void_p(stream)) != 0:
+        raise Other("ready_for: " + backend._last_error())
