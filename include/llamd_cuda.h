@@ -463,7 +463,7 @@ int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int
 int llamd_fwd_paged_append(const void *batch, const void *q, const void *k, const void *v, int in_type, size_t q_stride,
                            size_t k_stride, size_t v_stride, const float *wq, const float *wk, float eps, const float *rope_tab,
                            int rope_rows, int rot, int interleaved, void *q_out, size_t out_stride, void *k_pages, void *v_pages);
-/* out[token][head] = softmax(scale * q . k) v over the positions up to the token's own. q and out in the batch's type, or out in f32
+/* out[token][head] = softmax(scale * q . k) v over the positions up to the token's own; scale > 0. q and out in the batch's type, or out in f32
  * (out_f32: the same sums, not rounded); rows start at 16 bytes. Slots behind a sequence's last position may hold
  * anything, NaN and infinities too. 0 / -1 as above. */
 int llamd_fwd_paged_attention(const void *batch, const void *q, size_t q_stride, const void *k_pages, const void *v_pages, void *out,

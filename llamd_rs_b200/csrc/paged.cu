@@ -4,6 +4,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <exception>
 #include <new>
 #include <vector>
 
@@ -11,6 +12,11 @@
 
 namespace llamd {
 namespace {
+
+int refuse(const char *why) {
+    set_error_msg(why);
+    return -1;
+}
 
 struct Batch {
     PagedView view = {};
@@ -20,16 +26,35 @@ struct Batch {
     uint8_t *dev = nullptr, *host = nullptr;
     size_t dev_bytes = 0, host_bytes = 0;
     cudaEvent_t copied = nullptr;
+    // attention's pieces (device addresses in `dev`) and the partial results that they leave
+    const PagedItem *item = nullptr;
+    const PagedMerge *merge = nullptr;
+    const PagedPart *part = nullptr;
+    int n_small = 0, small_rows = 0, n_large = 0, n_merge = 0;
+    uint8_t *partial = nullptr;
+    size_t partial_bytes = 0, partial_rows = 0;
 
     ~Batch() {
         // (frees wait for the stream: launches that read the batch are done)
-        if (dev || host) cudaStreamSynchronize(stream());
+        if (dev || host || partial) cudaStreamSynchronize(stream());
         if (dev) cudaFree(dev);
+        if (partial) cudaFree(partial);
         if (host) cudaFreeHost(host);
         if (copied) cudaEventDestroy(copied);
     }
-    // Room for n bytes on both sides; the pinned side is not written before the copy out of it is done.
-    bool reserve(size_t n) {
+    // A device buffer of n bytes at least; what was in it is lost where it grows.
+    bool grow(uint8_t *&p, size_t &have, size_t n) {
+        if (n <= have) return true;
+        if (p && cudaStreamSynchronize(stream()) != cudaSuccess) return fail("paged batch: sync");
+        if (p) cudaFree(p);
+        p = nullptr;
+        have = 0;
+        if (cudaMalloc((void **)&p, n) != cudaSuccess) return fail("paged batch: device memory");
+        have = n;
+        return true;
+    }
+    // Room for n bytes on both sides and for `rows` partial results; the pinned side is not written before the copy out of it is done.
+    bool reserve(size_t n, size_t rows) {
         if (!copied && cudaEventCreateWithFlags(&copied, cudaEventDisableTiming) != cudaSuccess) return fail("paged batch: event");
         if (cudaEventSynchronize(copied) != cudaSuccess) return fail("paged batch: previous copy");
         if (n > host_bytes) {
@@ -39,15 +64,7 @@ struct Batch {
             if (cudaHostAlloc((void **)&host, 2 * n, cudaHostAllocDefault) != cudaSuccess) return fail("paged batch: pinned memory");
             host_bytes = 2 * n;
         }
-        if (n > dev_bytes) {
-            if (dev && cudaStreamSynchronize(stream()) != cudaSuccess) return fail("paged batch: sync");
-            if (dev) cudaFree(dev);
-            dev = nullptr;
-            dev_bytes = 0;
-            if (cudaMalloc((void **)&dev, 2 * n) != cudaSuccess) return fail("paged batch: device memory");
-            dev_bytes = 2 * n;
-        }
-        return true;
+        return (n <= dev_bytes || grow(dev, dev_bytes, 2 * n)) && grow(partial, partial_bytes, rows * (view.hd * sizeof(float) + sizeof(float2)));
     }
     bool fail(const char *what) {
         set_error(cudaGetLastError(), what);
@@ -83,6 +100,70 @@ const char *check_lengths(const Batch &b, int n_seq, const int32_t *q_len, const
     }
     if (tokens * b.view.n_head > 0x7fffffffLL) return "paged batch: too many tokens";
     return nullptr;
+}
+
+// ---- attention's pieces --------------------------------------------------------------------------------------------------
+
+struct Plan {
+    std::vector<PagedItem> small, large;
+    std::vector<PagedMerge> merge;
+    std::vector<PagedPart> part;
+    int small_rows = 0;
+    size_t rows = 0;  // of partial results
+};
+
+// A stretch of positions that some tokens attend to: a sequence's own behind the shared prefix, or the prefix itself.
+struct Stretch {
+    int table, begin, end, token, n_tok, limit, step;
+    bool small(int group) const { return (long long)n_tok * group <= kPagedSmallRows; }
+};
+
+// Positions to a piece of paged_decode.cu. Its CTAs run two to an SM; the longest piece should not outlast an even share of
+// the bytes by much, and a piece costs 8 rows of f32 (4 KB at 128 elements) written and read again where a stretch is cut, which 128 positions
+// (64 KB) repay.
+int decode_piece(long long positions, int n_head_kv, int sms) {
+    const long long share = (positions * n_head_kv + 4LL * sms - 1) / (4LL * sms);
+    return (int)std::max(128LL, (share + 15) / 16 * 16);
+}
+
+void make_plan(Plan &plan, const PagedView &v, const int32_t *q_len, const int32_t *kv_len, int sms) {
+    const int group = v.group;
+    long long small_positions = 0;
+    std::vector<Stretch> own(v.n_seq);
+    const Stretch shared = {0, 0, v.n_shared, 0, v.tokens, v.n_shared, 0};
+    for (int s = 0, t = 0; s < v.n_seq; t += q_len[s], s++) {
+        own[s] = {s * v.table_stride, v.n_shared, kv_len[s], t, q_len[s], kv_len[s] - q_len[s] + 1, 1};
+        if (q_len[s] && own[s].small(group)) small_positions += own[s].end - own[s].begin;
+    }
+    if (v.n_shared && v.tokens && shared.small(group)) small_positions += v.n_shared;
+    const int piece = decode_piece(small_positions, v.n_head_kv, sms);
+    // cuts a stretch into pieces of equal length; where others join their rows, or there are several, they leave partial results
+    auto cut = [&](const Stretch &st, bool joined, std::vector<PagedPart> &parts) {
+        const bool small = st.small(group);
+        const int len = st.end - st.begin, n = small ? (len + piece - 1) / piece : 1, per = ((len + n - 1) / n + 15) / 16 * 16, rows = st.n_tok * group;
+        for (int b = st.begin; b < st.end; b += per) {
+            PagedItem it = {st.table, b, std::min(st.end, b + per), st.token, st.n_tok, st.limit, st.step, -1, 0, 0, {0, 0}};
+            if (joined || len > per) {
+                it.part = (int32_t)plan.rows, it.part_rows = rows;
+                parts.push_back({it.part, rows, st.token});
+                plan.rows += (size_t)rows * v.n_head_kv;
+            }
+            if (small) plan.small_rows = std::max(plan.small_rows, rows);
+            (small ? plan.small : plan.large).push_back(it);
+        }
+    };
+    std::vector<PagedPart> prefix;
+    if (v.n_shared && v.tokens) cut(shared, true, prefix);
+    for (int s = 0; s < v.n_seq; s++) {
+        if (!q_len[s]) continue;
+        const int begin = (int)plan.part.size();
+        plan.part.insert(plan.part.end(), prefix.begin(), prefix.end());
+        cut(own[s], !prefix.empty(), plan.part);
+        const int count = (int)plan.part.size() - begin;
+        for (int i = 0; count && i < q_len[s]; i++) plan.merge.push_back({own[s].token + i, begin, count, 0});
+    }
+    // the longest first: what is left at the end is short
+    std::stable_sort(plan.small.begin(), plan.small.end(), [](const PagedItem &a, const PagedItem &b) { return a.kv_end - a.kv_begin > b.kv_end - b.kv_begin; });
 }
 
 // ---- append --------------------------------------------------------------------------------------------------------------
@@ -168,7 +249,7 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const AppendParams p)
         if (p.interleaved) {
 #pragma unroll
             for (int j = 0; j < E; j += 4) {
-                const float4 f = __ldg(reinterpret_cast<const float4 *>(row + e0 + j));
+                const float4 f = *reinterpret_cast<const float4 *>(row + e0 + j);
                 sn[j] = sn[j + 1] = f.x, cs[j] = cs[j + 1] = f.y;
                 sn[j + 2] = sn[j + 3] = f.z, cs[j + 2] = cs[j + 3] = f.w;
             }
@@ -176,7 +257,7 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const AppendParams p)
             const int i0 = e0 < half ? e0 : e0 - half;
 #pragma unroll
             for (int j = 0; j < E; j += 2) {
-                const float4 f = __ldg(reinterpret_cast<const float4 *>(row + 2 * (i0 + j)));
+                const float4 f = *reinterpret_cast<const float4 *>(row + 2 * (i0 + j));
                 sn[j] = f.x, cs[j] = f.y, sn[j + 1] = f.z, cs[j + 1] = f.w;
             }
         }
@@ -191,7 +272,7 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const AppendParams p)
     const int hop = half / E, partner = (lane & ~(L - 1)) + (e0 < p.rot ? (l < hop ? l + hop : l - hop) : l);
     float wq[E], wk[E];
 #pragma unroll
-    for (int j = 0; j < E; j++) wq[j] = p.wq ? __ldg(p.wq + e0 + j) : 1.0f, wk[j] = p.wk ? __ldg(p.wk + e0 + j) : 1.0f;
+    for (int j = 0; j < E; j++) wq[j] = p.wq ? p.wq[e0 + j] : 1.0f, wk[j] = p.wk ? p.wk[e0 + j] : 1.0f;
 #pragma unroll
     for (int i = 0; i < kAppendVecs; i++) {
         const int v = v0 + i * PER;
@@ -294,10 +375,6 @@ void attention_launch(const AttnParams &p) {
     else launch_k("paged_attention", paged_attention_kernel<T, 64>, grid, dim3(128), 0, p);
 }
 
-int refuse(const char *why) {
-    set_error_msg(why);
-    return -1;
-}
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
 }  // namespace
@@ -331,19 +408,37 @@ int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int
     Batch *b = (Batch *)batch;
     if (!b) return refuse("paged batch: null");
     if (const char *why = check_lengths(*b, n_seq, q_len, kv_len, pages, pages_stride, n_pages, n_shared)) return refuse(why);
-    b->ready = false;
-    PagedView &v = b->view;
+    PagedView v = b->view;
     v.n_seq = n_seq, v.n_shared = n_shared, v.tokens = 0, v.table_stride = 1;
-    b->n_pages = n_pages, b->max_kv = 0;
+    int max_kv = 0;
     for (int s = 0; s < n_seq; s++) {
         v.tokens += q_len[s];
-        b->max_kv = std::max(b->max_kv, kv_len[s]);
+        max_kv = std::max(max_kv, kv_len[s]);
         v.table_stride = std::max(v.table_stride, (kv_len[s] + v.page - 1) / v.page);
     }
+    if ((long long)n_seq * v.table_stride > 0x7fffffffLL) return refuse("paged batch: the tables have more than 2^31 entries");
+    int device = 0, sms = 0;
+    LLAMD_TRY(cudaGetDevice(&device), "paged batch: device");
+    LLAMD_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device), "paged batch: device");
+    Plan plan;
+    try {
+        make_plan(plan, v, q_len, kv_len, sms);
+    } catch (const std::exception &) {
+        return refuse("paged batch: out of host memory");
+    }
+    if (plan.rows > 0x7fffffff) return refuse("paged batch: too many partial results");
     size_t bytes = 0;
     const size_t o_token = section<PagedToken>(bytes, v.tokens), o_seq = section<int32_t>(bytes, v.tokens),
-                 o_table = section<int32_t>(bytes, (size_t)n_seq * v.table_stride);
-    if (!b->reserve(std::max<size_t>(bytes, 16))) return -1;
+                 o_table = section<int32_t>(bytes, (size_t)n_seq * v.table_stride), o_small = section<PagedItem>(bytes, plan.small.size()),
+                 o_merge = section<PagedMerge>(bytes, plan.merge.size()), o_part = section<PagedPart>(bytes, plan.part.size());
+    b->ready = false;  // (from here on what the batch held is being replaced)
+    if (!b->reserve(std::max<size_t>(bytes, 16), plan.rows)) return -1;
+    auto put = [&](size_t at, const void *from, size_t n) {
+        if (n) memcpy(b->host + at, from, n);
+    };
+    put(o_small, plan.small.data(), plan.small.size() * sizeof(PagedItem));
+    put(o_merge, plan.merge.data(), plan.merge.size() * sizeof(PagedMerge));
+    put(o_part, plan.part.data(), plan.part.size() * sizeof(PagedPart));
     PagedToken *token = (PagedToken *)(b->host + o_token);
     int32_t *seq = (int32_t *)(b->host + o_seq), *table = (int32_t *)(b->host + o_table);
     for (int s = 0, t = 0; s < n_seq; s++) {
@@ -355,9 +450,16 @@ int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int
             seq[t] = s;
         }
     }
+    b->item = (const PagedItem *)(b->dev + o_small);
+    b->merge = (const PagedMerge *)(b->dev + o_merge);
+    b->part = (const PagedPart *)(b->dev + o_part);
+    b->n_small = (int)plan.small.size(), b->small_rows = plan.small_rows, b->n_large = (int)plan.large.size(), b->n_merge = (int)plan.merge.size();
+    b->partial_rows = plan.rows;
+    b->n_pages = n_pages, b->max_kv = max_kv;
     v.token = (const PagedToken *)(b->dev + o_token);
     v.token_seq = (const int32_t *)(b->dev + o_seq);
     v.table = (const int32_t *)(b->dev + o_table);
+    b->view = v;
     LLAMD_TRY(cudaMemcpyAsync(b->dev, b->host, bytes, cudaMemcpyHostToDevice, stream()), "paged batch: copy");
     LLAMD_TRY(cudaEventRecord(b->copied, stream()), "paged batch: event");
     b->ready = true;
@@ -405,12 +507,22 @@ int llamd_fwd_paged_attention(const void *batch, const void *q, size_t q_stride,
     if (!g.tokens) return 0;
     const size_t qd = (size_t)g.n_head * g.hd;
     if (!q || !k_pages || !v_pages || !out) return refuse("paged attention: a buffer is missing");
+    if (!(scale > 0.0f) || isinf(scale)) return refuse("paged attention: the scale is a positive number");
     if (q_stride < qd || out_stride < qd) return refuse("paged attention: a row overlaps the next");
     if (!aligned16(q) || q_stride % 8 || !aligned16(out) || out_stride % 8 || !aligned16(k_pages) || !aligned16(v_pages))
         return refuse("paged attention: buffers and rows start at 16 bytes");
     AttnParams p = {};
     p.b = g, p.q = q, p.k_pages = k_pages, p.v_pages = v_pages, p.out = out, p.q_stride = q_stride, p.out_stride = out_stride;
     p.out_f32 = out_f32, p.scale = scale;
+    if (!b->n_large) {
+        PagedAttn a = {};
+        a.b = g, a.item = b->item, a.q = q, a.k_pages = k_pages, a.v_pages = v_pages, a.out = out, a.q_stride = q_stride, a.out_stride = out_stride;
+        a.out_f32 = out_f32, a.scale_log2 = scale * 1.4426950408889634f;
+        a.part_o = (float *)b->partial, a.part_ml = (float2 *)(b->partial + b->partial_rows * g.hd * sizeof(float));
+        paged_decode_launch(a, b->type, b->n_small, b->small_rows);
+        if (b->n_merge) paged_merge_launch(a, b->type, b->merge, b->part, b->n_merge);
+        return error_code() ? -1 : 0;
+    }
     if (b->type == kPagedF16) attention_launch<__half>(p);
     else attention_launch<__nv_bfloat16>(p);
     return error_code() ? -1 : 0;

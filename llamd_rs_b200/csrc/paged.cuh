@@ -24,6 +24,40 @@ struct PagedView {
     const int32_t *table;       // [n_seq][table_stride] page ids
 };
 
+// One piece of attention: n_tok tokens (all their heads that share a kv head; the launch's y is the kv head) over positions [kv_begin, kv_end) of one table.
+// Token i of the piece sees positions below limit + i * step. part < 0: the piece is all its rows need, and writes out;
+// otherwise its rows' sums go to rows part + head_kv * part_rows + part_off + ... of the batch's partial results.
+struct PagedItem {
+    int32_t table, kv_begin, kv_end, token, n_tok, limit, step, part, part_rows, part_off, pad[2];
+};
+static_assert(sizeof(PagedItem) == 48, "three 16-byte words");
+
+// Where a token finds its partial results: entries [begin, begin + count) of the list below.
+struct PagedMerge {
+    int32_t token, begin, count, pad;
+};
+struct PagedPart {
+    int32_t part, part_rows, token;  // row of (token t, head h of kv head k): part + k * part_rows + (t - token) * group + h
+};
+
+// A partial result: sums of 2^(s - m) v over the piece's positions (s: the scores times log2 e), in f32, and beside them m and sum 2^(s - m).
+struct PagedAttn {
+    PagedView b;
+    const PagedItem *item;
+    const void *q, *k_pages, *v_pages;
+    void *out;
+    size_t q_stride, out_stride;
+    int out_f32;
+    float scale_log2;  // scale * log2 e
+    float *part_o;     // [rows][hd]
+    float2 *part_ml;   // [rows] (m, sum)
+};
+
+constexpr int kPagedSmallRows = 32;  // query rows (tokens x heads of a group) of a piece that paged_decode.cu takes
+
+void paged_decode_launch(const PagedAttn &p, int type, int n_items, int max_rows);
+void paged_merge_launch(const PagedAttn &p, int type, const PagedMerge *merge, const PagedPart *parts, int n_tokens);
+
 // 16-bit types of a cache and what the kernels need of them.
 template <typename T> struct Half16;
 template <> struct Half16<__half> {
@@ -40,6 +74,13 @@ template <> struct Half16<__nv_bfloat16> {
         return *reinterpret_cast<const uint32_t *>(&h);
     }
 };
+
+// Four neighbouring elements of an output row.
+template <typename T>
+__device__ __forceinline__ void store_out(void *out, int f32, size_t at, float4 v) {
+    if (f32) *reinterpret_cast<float4 *>(reinterpret_cast<float *>(out) + at) = v;
+    else *reinterpret_cast<uint2 *>(reinterpret_cast<T *>(out) + at) = make_uint2(Half16<T>::pack(v.x, v.y), Half16<T>::pack(v.z, v.w));
+}
 
 }  // namespace llamd
 
