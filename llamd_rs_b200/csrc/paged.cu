@@ -27,7 +27,7 @@ struct Batch {
     size_t dev_bytes = 0, host_bytes = 0;
     cudaEvent_t copied = nullptr;
     // attention's pieces (device addresses in `dev`) and the partial results that they leave
-    const PagedItem *item = nullptr;
+    const PagedItem *small = nullptr, *large = nullptr;  // for paged_decode.cu and paged_prompt.cu
     const PagedMerge *merge = nullptr;
     const PagedPart *part = nullptr;
     int n_small = 0, small_rows = 0, n_large = 0, n_merge = 0;
@@ -126,44 +126,101 @@ int decode_piece(long long positions, int n_head_kv, int sms) {
     return (int)std::max(128LL, (share + 15) / 16 * 16);
 }
 
-void make_plan(Plan &plan, const PagedView &v, const int32_t *q_len, const int32_t *kv_len, int sms) {
-    const int group = v.group;
-    long long small_positions = 0;
-    std::vector<Stretch> own(v.n_seq);
-    const Stretch shared = {0, 0, v.n_shared, 0, v.tokens, v.n_shared, 0};
-    for (int s = 0, t = 0; s < v.n_seq; t += q_len[s], s++) {
-        own[s] = {s * v.table_stride, v.n_shared, kv_len[s], t, q_len[s], kv_len[s] - q_len[s] + 1, 1};
-        if (q_len[s] && own[s].small(group)) small_positions += own[s].end - own[s].begin;
+// Some tokens of a stretch for paged_prompt.cu, and how many blocks of positions they see some of.
+struct Tile {
+    int token, n_tok, end, blocks;
+};
+
+// Blocks to a piece of paged_prompt.cu, one CTA to an SM: the cut of the longest tile that ends soonest. A piece costs about three
+// blocks to begin and end, and a join about four.
+int prompt_piece(const std::vector<Tile> &tiles, int n_head_kv, int sms) {
+    int longest = 1;
+    for (const Tile &t : tiles) longest = std::max(longest, t.blocks);
+    double best = 1e30;
+    int piece = longest;
+    for (int cuts = 1; cuts <= std::min(longest, 64); cuts++) {
+        const int per = (longest + cuts - 1) / cuts;
+        long long n = 0, total = 0;
+        for (const Tile &t : tiles) n += (t.blocks + per - 1) / per, total += t.blocks;
+        n *= n_head_kv, total *= n_head_kv;
+        const double ends = (n <= sms ? per + 3.0 : std::max(per + 3.0, (double)(total + 3 * n) / sms + 0.5 * per)) + (cuts > 1 ? 4.0 : 0.0);
+        if (ends < best) best = ends, piece = per;
+        if ((long long)tiles.size() * n_head_kv * cuts > 16LL * sms) break;
     }
-    if (v.n_shared && v.tokens && shared.small(group)) small_positions += v.n_shared;
-    const int piece = decode_piece(small_positions, v.n_head_kv, sms);
-    // cuts a stretch into pieces of equal length; where others join their rows, or there are several, they leave partial results
-    auto cut = [&](const Stretch &st, bool joined, std::vector<PagedPart> &parts) {
-        const bool small = st.small(group);
-        const int len = st.end - st.begin, n = small ? (len + piece - 1) / piece : 1, per = ((len + n - 1) / n + 15) / 16 * 16, rows = st.n_tok * group;
-        for (int b = st.begin; b < st.end; b += per) {
-            PagedItem it = {st.table, b, std::min(st.end, b + per), st.token, st.n_tok, st.limit, st.step, -1, 0, 0, {0, 0}};
+    return piece;
+}
+
+void make_plan(Plan &plan, const PagedView &v, const int32_t *q_len, const int32_t *kv_len, int sms) {
+    const int group = v.group, tile_tokens = 2 * (kPagedTileRows / group);
+    std::vector<Stretch> stretch;  // the shared one, where there is one, then the sequences' own
+    const bool shared = v.n_shared && v.tokens;
+    if (shared) stretch.push_back({0, 0, v.n_shared, 0, v.tokens, v.n_shared, 0});
+    for (int s = 0, t = 0; s < v.n_seq; t += q_len[s], s++)
+        if (q_len[s]) stretch.push_back({s * v.table_stride, v.n_shared, kv_len[s], t, q_len[s], kv_len[s] - q_len[s] + 1, 1});
+    long long small_positions = 0;
+    std::vector<Tile> tiles;  // of the large stretches, in order
+    for (const Stretch &st : stretch) {
+        if (st.small(group)) {
+            small_positions += st.end - st.begin;
+            continue;
+        }
+        for (int i = 0; i < st.n_tok; i += tile_tokens) {
+            const int n = std::min(tile_tokens, st.n_tok - i), end = std::min(st.end, st.limit + st.step * (i + n - 1));
+            tiles.push_back({st.token + i, n, end, (end - st.begin + kPagedBlock - 1) / kPagedBlock});
+        }
+    }
+    const int small_piece = decode_piece(small_positions, v.n_head_kv, sms), large_piece = prompt_piece(tiles, v.n_head_kv, sms) * kPagedBlock;
+    // The pieces of `tok` tokens from `token` on over [begin, end), cut evenly at multiples of `unit`; where others join their rows, or there are
+    // several, each leaves partial results of its own rows.
+    auto cut = [&](const Stretch &st, int token, int n_tok, int end, bool small, bool joined, std::vector<PagedPart> &parts) {
+        const int unit = small ? 16 : kPagedBlock, most = small ? small_piece : large_piece, len = end - st.begin, n = (len + most - 1) / most;
+        const int per = ((len + n - 1) / n + unit - 1) / unit * unit, rows = n_tok * group;
+        for (int b = st.begin; b < end; b += per) {
+            PagedItem it = {st.table, b, std::min(end, b + per), token, n_tok, st.limit + st.step * (token - st.token), st.step, -1, 0, 0, {0, 0}};
             if (joined || len > per) {
-                it.part = (int32_t)plan.rows, it.part_rows = rows;
-                parts.push_back({it.part, rows, st.token});
+                it.part = (int32_t)std::min<size_t>(plan.rows, 0x7fffffff), it.part_rows = rows;
+                parts.push_back({it.part, rows, token});
                 plan.rows += (size_t)rows * v.n_head_kv;
             }
             if (small) plan.small_rows = std::max(plan.small_rows, rows);
             (small ? plan.small : plan.large).push_back(it);
         }
     };
+    // the shared stretch: its tiles are cut alike, so that all tokens have the same list of parts
     std::vector<PagedPart> prefix;
-    if (v.n_shared && v.tokens) cut(shared, true, prefix);
-    for (int s = 0; s < v.n_seq; s++) {
-        if (!q_len[s]) continue;
-        const int begin = (int)plan.part.size();
-        plan.part.insert(plan.part.end(), prefix.begin(), prefix.end());
-        cut(own[s], !prefix.empty(), plan.part);
-        const int count = (int)plan.part.size() - begin;
-        for (int i = 0; count && i < q_len[s]; i++) plan.merge.push_back({own[s].token + i, begin, count, 0});
+    size_t i = 0, tile = 0;
+    if (shared) {
+        const Stretch &st = stretch[i++];
+        const bool small = st.small(group);
+        const size_t first = plan.large.size();
+        cut(st, st.token, st.n_tok, st.end, small, true, prefix);
+        if (!small) {
+            const std::vector<PagedItem> whole(plan.large.begin() + first, plan.large.end());
+            plan.large.resize(first);
+            for (; tile < tiles.size() && tiles[tile].token < st.n_tok && tile * (size_t)tile_tokens < (size_t)st.n_tok; tile++)
+                for (PagedItem it : whole) {
+                    it.token = tiles[tile].token, it.n_tok = tiles[tile].n_tok, it.part_off = tiles[tile].token * group;
+                    plan.large.push_back(it);
+                }
+        }
+    }
+    for (; i < stretch.size(); i++) {
+        const Stretch &st = stretch[i];
+        const bool small = st.small(group);
+        for (int t = 0; t < st.n_tok;) {
+            const Tile own = small ? Tile{st.token, st.n_tok, st.end, 0} : tiles[tile++];
+            const int begin = (int)plan.part.size();
+            plan.part.insert(plan.part.end(), prefix.begin(), prefix.end());
+            cut(st, own.token, own.n_tok, own.end, small, shared, plan.part);
+            const int count = (int)plan.part.size() - begin;
+            for (int x = 0; count && x < own.n_tok; x++) plan.merge.push_back({own.token + x, begin, count, 0});
+            t += own.n_tok;
+        }
     }
     // the longest first: what is left at the end is short
-    std::stable_sort(plan.small.begin(), plan.small.end(), [](const PagedItem &a, const PagedItem &b) { return a.kv_end - a.kv_begin > b.kv_end - b.kv_begin; });
+    auto longer = [](const PagedItem &a, const PagedItem &b) { return a.kv_end - a.kv_begin > b.kv_end - b.kv_begin; };
+    std::stable_sort(plan.small.begin(), plan.small.end(), longer);
+    std::stable_sort(plan.large.begin(), plan.large.end(), longer);
 }
 
 // ---- append --------------------------------------------------------------------------------------------------------------
@@ -321,60 +378,6 @@ void append_launch(AppendParams &p) {
     else launch_k("paged_append", paged_append_kernel<TI, T, 64>, grid, dim3(256), 0, p);
 }
 
-// ---- attention, one warp per (token, head) -------------------------------------------------------------------------------
-
-struct AttnParams {
-    PagedView b;
-    const void *q, *k_pages, *v_pages;
-    void *out;
-    size_t q_stride, out_stride;
-    int out_f32;
-    float scale;
-};
-
-template <typename T, int HD>
-__global__ void __launch_bounds__(128) paged_attention_kernel(const AttnParams p) {
-    constexpr int E = HD / 32;  // elements to a lane
-    pdl_trigger();
-    pdl_wait();
-    const int warp = (int)((blockIdx.x * blockDim.x + threadIdx.x) >> 5), lane = threadIdx.x & 31;
-    if (warp >= p.b.tokens * p.b.n_head) return;
-    const int t = warp / p.b.n_head, h = warp - t * p.b.n_head, hk = h / p.b.group;
-    const int32_t *table = p.b.table + (size_t)p.b.token_seq[t] * p.b.table_stride;
-    const T *q = reinterpret_cast<const T *>(p.q) + (size_t)t * p.q_stride + (size_t)h * HD + lane * E;
-    float x[E], o[E], m = -INFINITY, sum = 0.0f;
-#pragma unroll
-    for (int j = 0; j < E; j++) x[j] = (float)q[j] * p.scale, o[j] = 0.0f;
-    const int last = p.b.token[t].pos;
-    for (int i = 0; i <= last; i++) {
-        const size_t row = ((size_t)table[i / p.b.page] * p.b.n_head_kv + hk) * p.b.page + i % p.b.page;
-        const T *k = reinterpret_cast<const T *>(p.k_pages) + row * HD + lane * E, *v = reinterpret_cast<const T *>(p.v_pages) + row * HD + lane * E;
-        float s = 0.0f;
-#pragma unroll
-        for (int j = 0; j < E; j++) s = fmaf(x[j], (float)k[j], s);
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-        const float m2 = fmaxf(m, s), a = expf(m - m2), e = expf(s - m2);
-        m = m2;
-        sum = fmaf(sum, a, e);
-#pragma unroll
-        for (int j = 0; j < E; j++) o[j] = fmaf(o[j], a, e * (float)v[j]);
-    }
-    const size_t at = (size_t)t * p.out_stride + (size_t)h * HD + lane * E;
-#pragma unroll
-    for (int j = 0; j < E; j++) {
-        if (p.out_f32) reinterpret_cast<float *>(p.out)[at + j] = o[j] / sum;
-        else reinterpret_cast<T *>(p.out)[at + j] = (T)(o[j] / sum);
-    }
-}
-
-template <typename T>
-void attention_launch(const AttnParams &p) {
-    const dim3 grid((unsigned)(((size_t)p.b.tokens * p.b.n_head + 3) / 4));
-    if (p.b.hd == 128) launch_k("paged_attention", paged_attention_kernel<T, 128>, grid, dim3(128), 0, p);
-    else launch_k("paged_attention", paged_attention_kernel<T, 64>, grid, dim3(128), 0, p);
-}
-
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
 }  // namespace
@@ -430,6 +433,7 @@ int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int
     size_t bytes = 0;
     const size_t o_token = section<PagedToken>(bytes, v.tokens), o_seq = section<int32_t>(bytes, v.tokens),
                  o_table = section<int32_t>(bytes, (size_t)n_seq * v.table_stride), o_small = section<PagedItem>(bytes, plan.small.size()),
+                 o_large = section<PagedItem>(bytes, plan.large.size()),
                  o_merge = section<PagedMerge>(bytes, plan.merge.size()), o_part = section<PagedPart>(bytes, plan.part.size());
     b->ready = false;  // (from here on what the batch held is being replaced)
     if (!b->reserve(std::max<size_t>(bytes, 16), plan.rows)) return -1;
@@ -437,6 +441,7 @@ int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int
         if (n) memcpy(b->host + at, from, n);
     };
     put(o_small, plan.small.data(), plan.small.size() * sizeof(PagedItem));
+    put(o_large, plan.large.data(), plan.large.size() * sizeof(PagedItem));
     put(o_merge, plan.merge.data(), plan.merge.size() * sizeof(PagedMerge));
     put(o_part, plan.part.data(), plan.part.size() * sizeof(PagedPart));
     PagedToken *token = (PagedToken *)(b->host + o_token);
@@ -450,7 +455,8 @@ int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int
             seq[t] = s;
         }
     }
-    b->item = (const PagedItem *)(b->dev + o_small);
+    b->small = (const PagedItem *)(b->dev + o_small);
+    b->large = (const PagedItem *)(b->dev + o_large);
     b->merge = (const PagedMerge *)(b->dev + o_merge);
     b->part = (const PagedPart *)(b->dev + o_part);
     b->n_small = (int)plan.small.size(), b->small_rows = plan.small_rows, b->n_large = (int)plan.large.size(), b->n_merge = (int)plan.merge.size();
@@ -511,20 +517,19 @@ int llamd_fwd_paged_attention(const void *batch, const void *q, size_t q_stride,
     if (q_stride < qd || out_stride < qd) return refuse("paged attention: a row overlaps the next");
     if (!aligned16(q) || q_stride % 8 || !aligned16(out) || out_stride % 8 || !aligned16(k_pages) || !aligned16(v_pages))
         return refuse("paged attention: buffers and rows start at 16 bytes");
-    AttnParams p = {};
-    p.b = g, p.q = q, p.k_pages = k_pages, p.v_pages = v_pages, p.out = out, p.q_stride = q_stride, p.out_stride = out_stride;
-    p.out_f32 = out_f32, p.scale = scale;
-    if (!b->n_large) {
-        PagedAttn a = {};
-        a.b = g, a.item = b->item, a.q = q, a.k_pages = k_pages, a.v_pages = v_pages, a.out = out, a.q_stride = q_stride, a.out_stride = out_stride;
-        a.out_f32 = out_f32, a.scale_log2 = scale * 1.4426950408889634f;
-        a.part_o = (float *)b->partial, a.part_ml = (float2 *)(b->partial + b->partial_rows * g.hd * sizeof(float));
-        paged_decode_launch(a, b->type, b->n_small, b->small_rows);
-        if (b->n_merge) paged_merge_launch(a, b->type, b->merge, b->part, b->n_merge);
-        return error_code() ? -1 : 0;
+    PagedAttn a = {};
+    a.b = g, a.q = q, a.k_pages = k_pages, a.v_pages = v_pages, a.out = out, a.q_stride = q_stride, a.out_stride = out_stride;
+    a.out_f32 = out_f32, a.scale_log2 = scale * 1.4426950408889634f;
+    a.part_o = (float *)b->partial, a.part_ml = (float2 *)(b->partial + b->partial_rows * g.hd * sizeof(float));
+    if (b->n_large) {
+        a.item = b->large;
+        paged_prompt_launch(a, b->type, b->n_pages, b->n_large);
     }
-    if (b->type == kPagedF16) attention_launch<__half>(p);
-    else attention_launch<__nv_bfloat16>(p);
+    if (b->n_small) {
+        a.item = b->small;
+        paged_decode_launch(a, b->type, b->n_small, b->small_rows);
+    }
+    if (b->n_merge) paged_merge_launch(a, b->type, b->merge, b->part, b->n_merge);
     return error_code() ? -1 : 0;
 }
 

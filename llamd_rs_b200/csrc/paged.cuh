@@ -56,6 +56,8 @@ struct PagedAttn {
 constexpr int kPagedSmallRows = 32;  // query rows (tokens x heads of a group) of a piece that paged_decode.cu takes
 
 void paged_decode_launch(const PagedAttn &p, int type, int n_items, int max_rows);
+constexpr int kPagedTileRows = 128, kPagedBlock = 128;  // of paged_prompt.cu: two tiles of query rows to a piece, positions to a block
+void paged_prompt_launch(const PagedAttn &p, int type, int n_pages, int n_items);
 void paged_merge_launch(const PagedAttn &p, int type, const PagedMerge *merge, const PagedPart *parts, int n_tokens);
 
 // 16-bit types of a cache and what the kernels need of them.

@@ -225,6 +225,11 @@ class Batch:
             pass
 
 
+def status() -> int:
+    """0 while every bounded wait inside the attention has been met (llamd_fwd_paged_status; waits for the stream)."""
+    return int(lib().llamd_fwd_paged_status())
+
+
 def wait_for(stream: int) -> None:
     """What is enqueued through the library from here on waits for what ``stream`` (a cudaStream_t) holds now."""
     if lib().llamd_fwd_wait_stream(C.c_void_p(stream)) != 0:
