@@ -5,7 +5,9 @@
 
 #include <algorithm>
 #include <exception>
+#include <functional>
 #include <new>
+#include <utility>
 #include <vector>
 
 #include "paged.cuh"
@@ -30,7 +32,8 @@ struct Batch {
     const PagedItem *small = nullptr, *large = nullptr;  // for paged_decode.cu and paged_prompt.cu
     const PagedMerge *merge = nullptr;
     const PagedPart *part = nullptr;
-    int n_small = 0, small_rows = 0, n_large = 0, n_merge = 0;
+    const int32_t *begin = nullptr;  // large: each CTA's
+    int n_small = 0, small_rows = 0, n_ctas = 0, n_merge = 0;
     uint8_t *partial = nullptr;
     size_t partial_bytes = 0, partial_rows = 0;
 
@@ -106,6 +109,7 @@ const char *check_lengths(const Batch &b, int n_seq, const int32_t *q_len, const
 
 struct Plan {
     std::vector<PagedItem> small, large;
+    std::vector<int32_t> begin;  // large: each CTA's
     std::vector<PagedMerge> merge;
     std::vector<PagedPart> part;
     int small_rows = 0;
@@ -131,21 +135,46 @@ struct Tile {
     int token, n_tok, end, blocks;
 };
 
-// Blocks to a piece of paged_prompt.cu, one CTA to an SM: the cut of the longest tile that ends soonest. A piece costs about three
-// blocks to begin and end, and a join about four.
+// paged_prompt.cu runs one CTA to an SM, each with a list of pieces. In blocks of its loop, a piece costs its blocks and about one more to begin
+// and end, leaving partial results one more again, and the launch that joins them about two.
+constexpr double kPieceCost = 1.0, kPartCost = 1.0, kJoinCost = 2.0;
+
+// Hands the longest of what is left to the CTA with the least so far. costs: in falling order; `to` (may be null) takes each one's CTA. Returns when
+// the last CTA ends.
+double deal(const std::vector<double> &costs, int ctas, std::vector<int> *to) {
+    std::vector<std::pair<double, int>> load(ctas);
+    for (int i = 0; i < ctas; i++) load[i] = {0.0, i};
+    double last = 0.0;
+    const auto later = std::greater<std::pair<double, int>>();
+    for (double c : costs) {
+        std::pop_heap(load.begin(), load.end(), later);
+        load.back().first += c;
+        last = std::max(last, load.back().first);
+        if (to) to->push_back(load.back().second);
+        std::push_heap(load.begin(), load.end(), later);
+    }
+    return last;
+}
+
+// Blocks to a piece: the cut of the longest tile with which the last CTA ends soonest.
 int prompt_piece(const std::vector<Tile> &tiles, int n_head_kv, int sms) {
     int longest = 1;
     for (const Tile &t : tiles) longest = std::max(longest, t.blocks);
     double best = 1e30;
     int piece = longest;
-    for (int cuts = 1; cuts <= std::min(longest, 64); cuts++) {
+    std::vector<double> costs;
+    for (int cuts : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 40, 48, 64, 96, 128}) {
         const int per = (longest + cuts - 1) / cuts;
-        long long n = 0, total = 0;
-        for (const Tile &t : tiles) n += (t.blocks + per - 1) / per, total += t.blocks;
-        n *= n_head_kv, total *= n_head_kv;
-        const double ends = (n <= sms ? per + 3.0 : std::max(per + 3.0, (double)(total + 3 * n) / sms + 0.5 * per)) + (cuts > 1 ? 4.0 : 0.0);
+        if (cuts > longest || (cuts > 1 && (long long)tiles.size() * n_head_kv * cuts > 24LL * sms)) break;
+        costs.clear();
+        for (const Tile &t : tiles) {
+            const int n = (t.blocks + per - 1) / per, each = (t.blocks + n - 1) / n;
+            for (int b = 0; b < t.blocks; b += each)
+                costs.insert(costs.end(), n_head_kv, std::min(each, t.blocks - b) + kPieceCost + (n > 1 ? kPartCost : 0.0));
+        }
+        std::sort(costs.begin(), costs.end(), std::greater<double>());
+        const double ends = deal(costs, sms, nullptr) + (cuts > 1 ? kJoinCost : 0.0);
         if (ends < best) best = ends, piece = per;
-        if ((long long)tiles.size() * n_head_kv * cuts > 16LL * sms) break;
     }
     return piece;
 }
@@ -176,7 +205,7 @@ void make_plan(Plan &plan, const PagedView &v, const int32_t *q_len, const int32
         const int unit = small ? 16 : kPagedBlock, most = small ? small_piece : large_piece, len = end - st.begin, n = (len + most - 1) / most;
         const int per = ((len + n - 1) / n + unit - 1) / unit * unit, rows = n_tok * group;
         for (int b = st.begin; b < end; b += per) {
-            PagedItem it = {st.table, b, std::min(end, b + per), token, n_tok, st.limit + st.step * (token - st.token), st.step, -1, 0, 0, {0, 0}};
+            PagedItem it = {st.table, b, std::min(end, b + per), token, n_tok, st.limit + st.step * (token - st.token), st.step, -1, 0, 0, 0, 0};
             if (joined || len > per) {
                 it.part = (int32_t)std::min<size_t>(plan.rows, 0x7fffffff), it.part_rows = rows;
                 parts.push_back({it.part, rows, token});
@@ -221,6 +250,23 @@ void make_plan(Plan &plan, const PagedView &v, const int32_t *q_len, const int32
     auto longer = [](const PagedItem &a, const PagedItem &b) { return a.kv_end - a.kv_begin > b.kv_end - b.kv_begin; };
     std::stable_sort(plan.small.begin(), plan.small.end(), longer);
     std::stable_sort(plan.large.begin(), plan.large.end(), longer);
+    // the large ones by kv head, dealt out
+    std::vector<PagedItem> dealt;
+    std::vector<double> costs;
+    std::vector<int> to;
+    for (PagedItem it : plan.large)
+        for (it.head = 0; it.head < v.n_head_kv; it.head++) {
+            dealt.push_back(it);
+            costs.push_back((it.kv_end - it.kv_begin + kPagedBlock - 1) / kPagedBlock + kPieceCost + (it.part >= 0 ? kPartCost : 0.0));
+        }
+    const int ctas = (int)std::min<size_t>(sms, dealt.size());
+    deal(costs, ctas, &to);
+    plan.begin.assign(ctas + 1, 0);
+    for (int c : to) plan.begin[c + 1]++;
+    for (int c = 0; c < ctas; c++) plan.begin[c + 1] += plan.begin[c];
+    plan.large.resize(dealt.size());
+    std::vector<int> at(plan.begin.begin(), plan.begin.end() - 1);
+    for (size_t x = 0; x < dealt.size(); x++) plan.large[at[to[x]]++] = dealt[x];
 }
 
 // ---- append --------------------------------------------------------------------------------------------------------------
@@ -433,7 +479,7 @@ int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int
     size_t bytes = 0;
     const size_t o_token = section<PagedToken>(bytes, v.tokens), o_seq = section<int32_t>(bytes, v.tokens),
                  o_table = section<int32_t>(bytes, (size_t)n_seq * v.table_stride), o_small = section<PagedItem>(bytes, plan.small.size()),
-                 o_large = section<PagedItem>(bytes, plan.large.size()),
+                 o_large = section<PagedItem>(bytes, plan.large.size()), o_begin = section<int32_t>(bytes, plan.begin.size()),
                  o_merge = section<PagedMerge>(bytes, plan.merge.size()), o_part = section<PagedPart>(bytes, plan.part.size());
     b->ready = false;  // (from here on what the batch held is being replaced)
     if (!b->reserve(std::max<size_t>(bytes, 16), plan.rows)) return -1;
@@ -442,6 +488,7 @@ int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int
     };
     put(o_small, plan.small.data(), plan.small.size() * sizeof(PagedItem));
     put(o_large, plan.large.data(), plan.large.size() * sizeof(PagedItem));
+    put(o_begin, plan.begin.data(), plan.begin.size() * sizeof(int32_t));
     put(o_merge, plan.merge.data(), plan.merge.size() * sizeof(PagedMerge));
     put(o_part, plan.part.data(), plan.part.size() * sizeof(PagedPart));
     PagedToken *token = (PagedToken *)(b->host + o_token);
@@ -457,9 +504,10 @@ int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int
     }
     b->small = (const PagedItem *)(b->dev + o_small);
     b->large = (const PagedItem *)(b->dev + o_large);
+    b->begin = (const int32_t *)(b->dev + o_begin);
     b->merge = (const PagedMerge *)(b->dev + o_merge);
     b->part = (const PagedPart *)(b->dev + o_part);
-    b->n_small = (int)plan.small.size(), b->small_rows = plan.small_rows, b->n_large = (int)plan.large.size(), b->n_merge = (int)plan.merge.size();
+    b->n_small = (int)plan.small.size(), b->small_rows = plan.small_rows, b->n_ctas = (int)plan.begin.size() - 1, b->n_merge = (int)plan.merge.size();
     b->partial_rows = plan.rows;
     b->n_pages = n_pages, b->max_kv = max_kv;
     v.token = (const PagedToken *)(b->dev + o_token);
@@ -521,9 +569,9 @@ int llamd_fwd_paged_attention(const void *batch, const void *q, size_t q_stride,
     a.b = g, a.q = q, a.k_pages = k_pages, a.v_pages = v_pages, a.out = out, a.q_stride = q_stride, a.out_stride = out_stride;
     a.out_f32 = out_f32, a.scale_log2 = scale * 1.4426950408889634f;
     a.part_o = (float *)b->partial, a.part_ml = (float2 *)(b->partial + b->partial_rows * g.hd * sizeof(float));
-    if (b->n_large) {
+    if (b->n_ctas) {
         a.item = b->large;
-        paged_prompt_launch(a, b->type, b->n_pages, b->n_large);
+        paged_prompt_launch(a, b->type, b->n_pages, b->begin, b->n_ctas);
     }
     if (b->n_small) {
         a.item = b->small;

@@ -24,11 +24,12 @@ struct PagedView {
     const int32_t *table;       // [n_seq][table_stride] page ids
 };
 
-// One piece of attention: n_tok tokens (all their heads that share a kv head; the launch's y is the kv head) over positions [kv_begin, kv_end) of one table.
+// One piece of attention: n_tok tokens (all their heads that share kv head `head`; for paged_decode.cu the launch's y) over positions
+// [kv_begin, kv_end) of one table.
 // Token i of the piece sees positions below limit + i * step. part < 0: the piece is all its rows need, and writes out;
-// otherwise its rows' sums go to rows part + head_kv * part_rows + part_off + ... of the batch's partial results.
+// otherwise its rows' sums go to rows part + head * part_rows + part_off + ... of the batch's partial results.
 struct PagedItem {
-    int32_t table, kv_begin, kv_end, token, n_tok, limit, step, part, part_rows, part_off, pad[2];
+    int32_t table, kv_begin, kv_end, token, n_tok, limit, step, part, part_rows, part_off, head, pad;
 };
 static_assert(sizeof(PagedItem) == 48, "three 16-byte words");
 
@@ -57,7 +58,7 @@ constexpr int kPagedSmallRows = 32;  // query rows (tokens x heads of a group) o
 
 void paged_decode_launch(const PagedAttn &p, int type, int n_items, int max_rows);
 constexpr int kPagedTileRows = 128, kPagedBlock = 128;  // of paged_prompt.cu: two tiles of query rows to a piece, positions to a block
-void paged_prompt_launch(const PagedAttn &p, int type, int n_pages, int n_items);
+void paged_prompt_launch(const PagedAttn &p, int type, int n_pages, const int32_t *begin, int n_ctas);  // begin: each CTA's pieces (n_ctas + 1)
 void paged_merge_launch(const PagedAttn &p, int type, const PagedMerge *merge, const PagedPart *parts, int n_tokens);
 
 // 16-bit types of a cache and what the kernels need of them.

@@ -8,9 +8,11 @@
 // (tcgen05, S and O in TMEM, P written over S in TMEM as the second product's operand), and 16384 exponentials, which take the
 // special function units as long as the products take the tensor cores: while one tile's softmax runs, the other's products do.
 //
-//   warps 0-3, 4-7   softmax of tile 0 / 1, a thread per row: S from TMEM, mask, maximum, exponentials, P to TMEM; at the end O / sum
-//   warp 8           K and V blocks into a ring in shared memory (TMA, a box per page, 128-byte swizzle)
-//   warp 9           the products: S0, S1 of the first block, then per block PV0, S0', PV1, S1'
+//   warps 0-7, 8-15  softmax of tile 0 / 1, two threads to a row, 64 positions each: S from TMEM, mask, maximum, exponentials, P to TMEM;
+//                    at the end O / sum
+//   warp 16          K and V blocks into a ring in shared memory (TMA, a box per page, 128-byte swizzle)
+//   warp 17          the products: S0, S1 of the first block, then per block PV0, S0', PV1, S1'
+//   warps 18, 19     nothing: registers are handed over by whole warpgroups
 //
 // O stays in TMEM over all blocks. It is rescaled only when a row's maximum has grown by more than 2^8 since the last time (P is then at
 // most 2^8, far inside f16's range, and the sums are exact in the same way), which after the first block hardly ever happens.
@@ -20,25 +22,51 @@
 
 #include <type_traits>
 
+#include "packed_f32.cuh"
 #include "paged.cuh"
 
 namespace llamd {
 namespace {
 
 constexpr int kM = kPagedTileRows, kN = kPagedBlock;
-constexpr int kSoftmaxWarps = 8, kThreads = (kSoftmaxWarps + 2) * 32;
+constexpr int kSoftmaxWarps = 16, kThreads = (kSoftmaxWarps + 4) * 32;
+// Registers of a softmax thread (64 scores live in them) and of the others: the launch gives 96 to each of 640, 512 x 104 + 128 x 64 =
+// 640 x 96.
+constexpr int kSoftmaxRegs = 104, kOtherRegs = 64;
+static_assert(kSoftmaxWarps * 32 * kSoftmaxRegs + 128 * kOtherRegs <= kThreads * 96, "no more than the launch's own");
 
 template <int HD> struct Shape {
     static constexpr int kTileBytes = kM * HD * 2;               // a tile of Q, a block of K or V: HD / 64 halves of 128 rows x 128 bytes
     static constexpr int kStages = HD == 128 ? 5 : 8;            // blocks of K or V in flight
-    static constexpr size_t kSmem = (2 + kStages) * (size_t)kTileBytes + 1024;
+    struct Rest {  // what follows the tiles in shared memory
+        uint64_t q_full[2], q_empty[2], s[2], p[2][2], o_full[2], o_empty[2], full[kStages], empty[kStages], drain;
+        float row[2][2][kM];  // what the two threads of a row tell each other
+        uint32_t tmem;
+        volatile int abort;
+    };
+    static constexpr size_t kSmem = (2 + kStages) * (size_t)kTileBytes + sizeof(Rest);
 };
 constexpr int kHalfBytes = kM * 128;
 
 struct PromptParams {
     PagedAttn a;
-    CUtensorMap k, v;
+    const int32_t *begin;  // [CTAs + 1] each CTA's pieces of a.item
+    CUtensorMap q, k, v;
     int *status;
+};
+
+// The tokens of a piece's two tiles, and how many blocks each sees some of.
+struct Tiles {
+    int n_tok[2], n_blk[2], n_all;
+    __device__ __forceinline__ Tiles(const PagedItem &it, int per_tile) {
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            n_tok[t] = min(per_tile, max(0, it.n_tok - t * per_tile));
+            const int end = min(it.kv_end, it.limit + it.step * (t * per_tile + n_tok[t] - 1));
+            n_blk[t] = n_tok[t] && end > it.kv_begin ? (end - it.kv_begin + kN - 1) / kN : 0;
+        }
+        n_all = max(n_blk[0], n_blk[1]);
+    }
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -58,10 +86,10 @@ __device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity, volatil
         uint32_t done;
         asm volatile(
             "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
             "selp.u32 %0, 1, 0, p;\n\t}"
             : "=r"(done)
-            : "r"(a), "r"(parity), "r"(20000u)
+            : "r"(a), "r"(parity)
             : "memory");
         if (done) return true;
         if (*abort) return false;
@@ -77,6 +105,11 @@ __device__ __forceinline__ bool elect_one() {
 __device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap *map, int x, int row, uint64_t *bar) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map), "r"(x), "r"(row),
                  "r"(smem_addr(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void tma_tokens(uint32_t dst, const CUtensorMap *map, int x, int head, int token, uint64_t *bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map), "r"(x), "r"(head),
+                 "r"(token), "r"(smem_addr(bar))
                  : "memory");
 }
 // Matrix descriptors of 128-byte rows with the 128-byte swizzle, 8-row groups 1024 bytes apart (start address, leading and stride offsets
@@ -102,8 +135,6 @@ __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::be
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-#define LLAMD_R32(v, o) \
-    v[o], v[o + 1], v[o + 2], v[o + 3], v[o + 4], v[o + 5], v[o + 6], v[o + 7], v[o + 8], v[o + 9], v[o + 10], v[o + 11], v[o + 12], v[o + 13], v[o + 14], v[o + 15]
 // 32 columns of the warp's 32 lanes; valid after tmem_loaded.
 template <int N>
 __device__ __forceinline__ void tmem_ld(uint32_t addr, float (&v)[N], int o) {
@@ -127,21 +158,37 @@ __device__ __forceinline__ void tmem_loaded(float (&v)[N], int o) {
                           "+f"(v[o + i + 7]), "+f"(v[o + i + 8]), "+f"(v[o + i + 9]), "+f"(v[o + i + 10]), "+f"(v[o + i + 11]), "+f"(v[o + i + 12]),
                           "+f"(v[o + i + 13]), "+f"(v[o + i + 14]), "+f"(v[o + i + 15]));
 }
-template <typename U>
-__device__ __forceinline__ void tmem_st(uint32_t addr, const U (&w)[32]) {
-    uint32_t v[32];
-#pragma unroll
-    for (int i = 0; i < 32; i++) v[i] = *reinterpret_cast<const uint32_t *>(&w[i]);
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&v)[16]) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
-        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]),
-        "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]),
-        "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]),
+          "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+        : "r"(addr)
         : "memory");
+}
+__device__ __forceinline__ void tmem_loaded16(float (&v)[16]) {
+    asm volatile("" : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]),
+                      "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr), "r"(v[0]),
+                 "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]),
+                 "r"(v[14]), "r"(v[15])
+                 : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Whether x holds for any of the 256 softmax threads of a tile, which wait for one another here.
+__device__ __forceinline__ bool tile_any(int barrier, bool x) {
+    uint32_t any;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, %2, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(any) : "r"((uint32_t)x), "r"(barrier) : "memory");
+    return any != 0;
+}
+__device__ __forceinline__ f32x2 sum2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
 __device__ __forceinline__ float exp2_fast(float x) {  // (2 ulp; -inf gives 0)
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -152,247 +199,251 @@ template <typename T, int HD>
 __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_constant__ PromptParams p) {
     using S = Shape<HD>;
     constexpr uint32_t kBf16 = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-    extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t b_q[2], b_s[2], b_p[2], b_o[2], b_full[S::kStages], b_empty[S::kStages], b_drain;
-    __shared__ uint32_t s_tmem;
-    __shared__ volatile int s_abort;
+    constexpr int kLoadWarp = kSoftmaxWarps, kMmaWarp = kSoftmaxWarps + 1;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    typename S::Rest &sh = *reinterpret_cast<typename S::Rest *>(smem + (2 + S::kStages) * S::kTileBytes);
     pdl_trigger();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hk = blockIdx.y, group = p.a.b.group;
-    uint8_t *smem = reinterpret_cast<uint8_t *>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = p.a.b.group, per_tile = kM / group;
     const uint32_t sq = smem_addr(smem), skv = sq + 2 * S::kTileBytes;
-    const PagedItem it = p.a.item[blockIdx.x];
-    // the tiles' tokens, and how many blocks each sees some of
-    const int per_tile = kM / group;
-    int n_tok[2], n_blk[2];
-#pragma unroll
-    for (int t = 0; t < 2; t++) {
-        n_tok[t] = min(per_tile, max(0, it.n_tok - t * per_tile));
-        const int end = min(it.kv_end, it.limit + it.step * (t * per_tile + n_tok[t] - 1));
-        n_blk[t] = n_tok[t] && end > it.kv_begin ? (end - it.kv_begin + kN - 1) / kN : 0;
-    }
-    const int n_all = max(n_blk[0], n_blk[1]);
+    const int first = p.begin[blockIdx.x], last = p.begin[blockIdx.x + 1];
 
     if (threadIdx.x == 0) {
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-            bar_init(&b_q[t], 128);
-            bar_init(&b_s[t], 1);
-            bar_init(&b_p[t], 128);
-            bar_init(&b_o[t], 1);
+            bar_init(&sh.q_full[t], 1);
+            bar_init(&sh.q_empty[t], 1);
+            bar_init(&sh.s[t], 1);
+            bar_init(&sh.p[t][0], 8);
+            bar_init(&sh.p[t][1], 8);
+            bar_init(&sh.o_full[t], 1);
+            bar_init(&sh.o_empty[t], 8);
         }
 #pragma unroll
         for (int i = 0; i < S::kStages; i++) {
-            bar_init(&b_full[i], 1);
-            bar_init(&b_empty[i], 1);
+            bar_init(&sh.full[i], 1);
+            bar_init(&sh.empty[i], 1);
         }
-        bar_init(&b_drain, 1);
-        s_abort = 0;
+        bar_init(&sh.drain, 1);
+        sh.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 9) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)), "r"(512) : "memory");
+    if (warp == kMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&sh.tmem)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     fence_before();
     __syncthreads();
     fence_after();
-    const uint32_t tmem = s_tmem;
+    const uint32_t tmem = sh.tmem;
     pdl_wait();  // (the batch's own tables were complete before the launch in front of this one began)
 
-    if (warp == 8) {
-        // ---- K and V blocks: slot 2 j is K of block j, 2 j + 1 its V ----
-        const int page = p.a.b.page, box = min(page, kN), shift = __ffs(page) - 1, boxes = kN / box;
-        const int32_t *table = p.a.b.table + it.table;
-        constexpr int kHalves = HD / 64;
-        const int my_box = lane / kHalves, my_half = lane % kHalves;
-        auto page_of = [&](int j) {
-            const int pos = it.kv_begin + j * kN + my_box * box;
-            return my_box < boxes && pos < it.kv_end ? table[pos >> shift] : -1;
-        };
-        int id = page_of(0), issued = 0;
-        bool ok = true;
-        for (int j = 0; j < n_all && ok; j++) {
-            const int next = page_of(j + 1), pos = it.kv_begin + j * kN;
-            const int used = (min(kN, it.kv_end - pos) + box - 1) / box;
-            const int row = (id * p.a.b.n_head_kv + hk) * page + ((pos + my_box * box) & (page - 1));
+    if (warp >= kSoftmaxWarps) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        if (warp == kLoadWarp) {
+            // ---- K and V blocks, K of a piece's block j in the ring's slot base + 2 j, V behind it; Q behind the piece's first K ----
+            const int page = p.a.b.page, box = min(page, kN), shift = __ffs(page) - 1, boxes = kN / box;
+            constexpr int kHalves = HD / 64;
+            const int my_box = lane / kHalves, my_half = lane % kHalves;
+            int slot = 0, n_q[2] = {0, 0};
+            bool ok = true;
+            for (int n = first; n < last && ok; n++) {
+                const PagedItem it = p.a.item[n];
+                const Tiles tl(it, per_tile);
+                const int32_t *table = p.a.b.table + it.table;
+                auto page_of = [&](int j) {
+                    const int pos = it.kv_begin + j * kN + my_box * box;
+                    return my_box < boxes && pos < it.kv_end ? table[pos >> shift] : -1;
+                };
+                int id = page_of(0);
+                for (int j = 0; j < tl.n_all && ok; j++) {
+                    const int next = page_of(j + 1), pos = it.kv_begin + j * kN;
+                    const int used = (min(kN, it.kv_end - pos) + box - 1) / box;
+                    const int row = (id * p.a.b.n_head_kv + it.head) * page + ((pos + my_box * box) & (page - 1));
 #pragma unroll
-            for (int kv = 0; kv < 2; kv++) {
-                const int slot = 2 * j + kv, stage = slot % S::kStages, round = slot / S::kStages;
-                if (round) ok = ok && bar_wait(&b_empty[stage], (round - 1) & 1, &s_abort);
-                if (!__all_sync(0xffffffffu, ok)) {
-                    ok = false;
-                    break;
+                    for (int kv = 0; kv < 2; kv++) {
+                        const int stage = slot % S::kStages, round = slot / S::kStages;
+                        if (round) ok = ok && bar_wait(&sh.empty[stage], (round - 1) & 1, &sh.abort);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        if (lane == 0) bar_expect(&sh.full[stage], (uint32_t)(used * box * HD * 2));
+                        __syncwarp();
+                        if (my_box < used)
+                            tma_rows(skv + stage * S::kTileBytes + my_half * kHalfBytes + my_box * box * 128, kv ? &p.v : &p.k, my_half * 64, row, &sh.full[stage]);
+                        slot++;
+                        if (kv || j) continue;
+#pragma unroll
+                        for (int t = 0; t < 2; t++) {  // (heads of a group and tokens come as the tile's rows; what lies behind the piece's tokens is not used)
+                            if (!tl.n_blk[t]) continue;
+                            if (n_q[t]) ok = ok && bar_wait(&sh.q_empty[t], (n_q[t] - 1) & 1, &sh.abort);
+                            ok = __all_sync(0xffffffffu, ok);
+                            if (!ok) break;
+                            if (lane == 0) bar_expect(&sh.q_full[t], (uint32_t)(per_tile * group * HD * 2));
+                            __syncwarp();
+                            if (lane < kHalves)
+                                tma_tokens(sq + t * S::kTileBytes + lane * kHalfBytes, &p.q, lane * 64, it.head * group, it.token + t * per_tile, &sh.q_full[t]);
+                            n_q[t]++;
+                        }
+                    }
+                    id = next;
                 }
-                if (lane == 0) bar_expect(&b_full[stage], (uint32_t)(used * box * HD * 2));
-                __syncwarp();
-                if (my_box < used)
-                    tma_rows(skv + stage * S::kTileBytes + my_half * kHalfBytes + my_box * box * 128, kv ? &p.v : &p.k, my_half * 64, row, &b_full[stage]);
-                issued = slot + 1;
             }
-            id = next;
-        }
-        if (s_abort)  // given up: what is on its way still lands before the block ends
-            for (int slot = max(0, issued - S::kStages); slot < issued; slot++) {
+            if (sh.abort) {  // given up: what is on its way still lands before the block ends
                 volatile int none = 0;
-                bar_wait(&b_full[slot % S::kStages], (slot / S::kStages) & 1, &none);
+                for (int i = max(0, slot - S::kStages); i < slot; i++) bar_wait(&sh.full[i % S::kStages], (i / S::kStages) & 1, &none);
+                for (int t = 0; t < 2; t++)
+                    if (n_q[t]) bar_wait(&sh.q_full[t], (n_q[t] - 1) & 1, &none);
             }
-    } else if (warp == 9) {
-        // ---- the products ----
-        // instruction descriptors: f32 sums (bit 4), operand types (bits 7, 10), N >> 3 at bit 17, M >> 4 at bit 24; V transposed (bit 16)
-        constexpr uint32_t kS = 1u << 4 | kBf16 << 7 | kBf16 << 10 | (uint32_t)(kN >> 3) << 17 | (uint32_t)(kM >> 4) << 24;
-        constexpr uint32_t kO = 1u << 4 | kBf16 << 7 | kBf16 << 10 | 1u << 16 | (uint32_t)(HD >> 3) << 17 | (uint32_t)(kM >> 4) << 24;
-        bool ok = true;
-        auto wait = [&](uint64_t *bar, int parity) {
-            ok = ok && bar_wait(bar, (uint32_t)parity & 1, &s_abort);
-            ok = __all_sync(0xffffffffu, ok);
-            fence_after();
-            return ok;
-        };
-        auto scores = [&](int t, int j) {
-            const int stage = (2 * j) % S::kStages;
-            if (elect_one()) {
-                const uint64_t a = smem_desc(sq + t * S::kTileBytes, 16), b = smem_desc(skv + stage * S::kTileBytes, 16);
+        } else if (warp == kMmaWarp) {
+            // ---- the products ----
+            // instruction descriptors: f32 sums (bit 4), operand types (bits 7, 10), N >> 3 at bit 17, M >> 4 at bit 24; V transposed (bit 16)
+            constexpr uint32_t kS = 1u << 4 | kBf16 << 7 | kBf16 << 10 | (uint32_t)(kN >> 3) << 17 | (uint32_t)(kM >> 4) << 24;
+            constexpr uint32_t kO = 1u << 4 | kBf16 << 7 | kBf16 << 10 | 1u << 16 | (uint32_t)(HD >> 3) << 17 | (uint32_t)(kM >> 4) << 24;
+            bool ok = true;
+            auto wait = [&](uint64_t *bar, int parity) {
+                ok = ok && bar_wait(bar, (uint32_t)parity & 1, &sh.abort);
+                ok = __all_sync(0xffffffffu, ok);
+                fence_after();
+                return ok;
+            };
+            auto commit = [&](uint64_t *bar) {
+                if (elect_one()) mma_commit(bar);
+                __syncwarp();
+            };
+            auto full = [&](int slot) { return wait(&sh.full[slot % S::kStages], slot / S::kStages); };
+            auto scores = [&](int t, int slot) {
+                if (elect_one()) {
+                    const uint64_t a = smem_desc(sq + t * S::kTileBytes, 16), b = smem_desc(skv + (slot % S::kStages) * S::kTileBytes, 16);
 #pragma unroll
-                for (int s = 0; s < HD / 16; s++) {
-                    const uint64_t at = (uint64_t)((s / 4) * (kHalfBytes >> 4) + (s % 4) * 2);
-                    mma_ss(tmem + t * kN, a + at, b + at, kS, s > 0);
+                    for (int s = 0; s < HD / 16; s++) {
+                        const uint64_t at = (uint64_t)((s / 4) * (kHalfBytes >> 4) + (s % 4) * 2);
+                        mma_ss(tmem + t * kN, a + at, b + at, kS, s > 0);
+                    }
+                    mma_commit(&sh.s[t]);
                 }
-                mma_commit(&b_s[t]);
-            }
-            __syncwarp();
-        };
-        auto values = [&](int t, int j) {
-            const int stage = (2 * j + 1) % S::kStages;
-            if (elect_one()) {
-                const uint64_t b = smem_desc(skv + stage * S::kTileBytes, kHalfBytes);
+                __syncwarp();
+            };
+            auto values = [&](int t, int slot, int part, bool more) {  // positions 0-31 and 64-95 of the block, then the others: as the weights come
+                if (elect_one()) {
+                    const uint64_t b = smem_desc(skv + (slot % S::kStages) * S::kTileBytes, kHalfBytes);
 #pragma unroll
-                for (int s = 0; s < kN / 16; s++) mma_ts(tmem + 2 * kN + t * HD, tmem + t * kN + s * 8, b + (uint64_t)(s * (16 * 128 >> 4)), kO, j > 0 || s > 0);
-            }
-            __syncwarp();
-        };
-        auto commit = [&](uint64_t *bar) {
-            if (elect_one()) mma_commit(bar);
-            __syncwarp();
-        };
-        auto full = [&](int slot) { return wait(&b_full[slot % S::kStages], slot / S::kStages); };
-        if (n_all) {
-            full(0);
-            for (int t = 0; t < 2 && ok; t++)
-                if (n_blk[t] && wait(&b_q[t], 0)) scores(t, 0);
-            if (ok) commit(&b_empty[0]);
-        }
-        for (int j = 0; j < n_all && ok; j++) {
-            if (!full(2 * j + 1)) break;
-            const bool more = j + 1 < n_all;
-            bool have_next = false;
-            for (int t = 0; t < 2 && ok; t++) {
-                if (j >= n_blk[t]) continue;
-                if (!wait(&b_p[t], j)) break;
-                values(t, j);
-                if (j + 1 == n_blk[t]) commit(&b_o[t]);
-                if (j + 1 < n_blk[t]) {
-                    if (!have_next && !full(2 * j + 2)) break;
-                    have_next = true;
-                    scores(t, j + 1);
+                    for (int i = 0; i < 4; i++) {
+                        const int half = i >> 1, step = 2 * part + (i & 1);  // 16 positions: 8 columns of P, over the half's own columns of S
+                        mma_ts(tmem + 2 * kN + t * HD, tmem + t * kN + half * 64 + step * 8, b + (uint64_t)((half * 4 + step) * (16 * 128 >> 4)), kO, more || part > 0 || i > 0);
+                    }
                 }
+                __syncwarp();
+            };
+            int base = 0, n_s[2] = {0, 0}, n_q[2] = {0, 0};  // slots of the pieces before; blocks and pieces of each tile
+            for (int n = first; n < last && ok; n++) {
+                const Tiles tl(p.a.item[n], per_tile);
+                if (!tl.n_all) continue;
+                full(base);
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+                    if (ok && tl.n_blk[t] && wait(&sh.q_full[t], n_q[t])) {
+                        scores(t, base);
+                        if (tl.n_blk[t] == 1) commit(&sh.q_empty[t]);
+                    }
+                if (ok) commit(&sh.empty[base % S::kStages]);
+                for (int j = 0; j < tl.n_all && ok; j++) {
+                    const int k_next = base + 2 * j + 2;
+                    if (!full(k_next - 1)) break;
+                    if (j + 1 < tl.n_all && !full(k_next)) break;
+#pragma unroll
+                    for (int t = 0; t < 2; t++) {
+                        if (!ok || j >= tl.n_blk[t]) continue;
+                        if (!j && n_q[t]) wait(&sh.o_empty[t], n_q[t] - 1);  // the piece before has been read out
+                        if (ok && wait(&sh.p[t][0], n_s[t])) values(t, k_next - 1, 0, j > 0);
+                        if (ok && wait(&sh.p[t][1], n_s[t])) values(t, k_next - 1, 1, j > 0);
+                        if (!ok) continue;
+                        n_s[t]++;
+                        if (j + 1 < tl.n_blk[t]) {
+                            scores(t, k_next);
+                            if (j + 2 == tl.n_blk[t]) commit(&sh.q_empty[t]);
+                        } else {
+                            commit(&sh.o_full[t]);
+                        }
+                    }
+                    if (ok) {
+                        commit(&sh.empty[(k_next - 1) % S::kStages]);
+                        if (j + 1 < tl.n_all) commit(&sh.empty[k_next % S::kStages]);
+                    }
+                }
+                base += 2 * tl.n_all;
+#pragma unroll
+                for (int t = 0; t < 2; t++) n_q[t] += tl.n_blk[t] > 0;
             }
-            if (ok) {
-                commit(&b_empty[(2 * j + 1) % S::kStages]);
-                if (more) commit(&b_empty[(2 * j + 2) % S::kStages]);
+            if (sh.abort) {  // given up: products on their way end before TMEM is given back
+                commit(&sh.drain);
+                volatile int none = 0;
+                bar_wait(&sh.drain, 0, &none);
             }
-        }
-        if (s_abort) {  // given up: products on their way end before TMEM is given back
-            commit(&b_drain);
-            volatile int none = 0;
-            bar_wait(&b_drain, 0, &none);
         }
     } else {
-        // ---- softmax of tile t, a thread per row ----
-        const int t = warp >> 2, r = threadIdx.x & 127, rows = n_tok[t] * group;
-        const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), ts = lanes + t * kN, to = lanes + 2 * kN + t * HD;
+        // ---- softmax of tile t ----
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+        const int t = warp >> 3, half = (warp >> 2) & 1, r = threadIdx.x & 127;
+        const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), ts = lanes + t * kN + half * 64, to = lanes + 2 * kN + t * HD;
         const float scale = p.a.scale_log2;
-        float m = -INFINITY, sum = 0.0f;
         bool ok = true;
-        if (n_blk[t]) {
-            // Q's rows, 16 bytes a thread at a time, rows beyond the last as zeros
-            constexpr int kChunks = HD / 8;
-            const T *src = reinterpret_cast<const T *>(p.a.q) + (size_t)(it.token + t * per_tile) * p.a.q_stride + (size_t)hk * group * HD;
-            uint4 q[kChunks];
-#pragma unroll
-            for (int i = 0; i < kChunks; i++) {
-                const int x = r + i * 128, row = x / kChunks, c = x % kChunks, tok = row / group;
-                q[i] = row < rows ? *reinterpret_cast<const uint4 *>(src + (size_t)tok * p.a.q_stride + (size_t)(row - tok * group) * HD + c * 8) : make_uint4(0, 0, 0, 0);
-            }
-#pragma unroll
-            for (int i = 0; i < kChunks; i++) {
-                const int x = r + i * 128, row = x / kChunks, c = x % kChunks;
-                const uint32_t at = sq + t * S::kTileBytes + (c / 8) * kHalfBytes + row * 128 + (((c & 7) ^ (row & 7)) << 4);
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(q[i].x), "r"(q[i].y), "r"(q[i].z), "r"(q[i].w) : "memory");
-            }
-            fence_async();
-            bar_arrive(&b_q[t]);
-        }
-        const int mine = min(it.kv_end, it.limit + it.step * (t * per_tile + min(r, rows - 1) / group)) - it.kv_begin;  // positions of the piece that this row sees
-        for (int j = 0; j < n_blk[t]; j++) {
-            ok = ok && bar_wait(&b_s[t], j & 1, &s_abort);
-            if (!(ok = __all_sync(0xffffffffu, ok))) break;
+        int base = 0, n_s = 0, n_q = 0;  // as the products' warp counts them
+        for (int n = first; n < last; n++) {
+        const PagedItem it = p.a.item[n];
+        const Tiles tl(it, per_tile);
+        const int n_tok = t ? tl.n_tok[1] : tl.n_tok[0], n_blk = t ? tl.n_blk[1] : tl.n_blk[0], rows = n_tok * group;
+        float m = -INFINITY, sum = 0.0f;
+        // positions of the piece that this row sees, counted from the thread's half of a block
+        const int mine = min(it.kv_end, it.limit + it.step * (t * per_tile + min(r, rows - 1) / group)) - it.kv_begin - half * 64;
+        for (int j = 0; j < n_blk; j++, n_s++) {
+            ok = ok && bar_wait(&sh.s[t], n_s & 1, &sh.abort);
+            ok = __all_sync(0xffffffffu, ok);
             fence_after();
-            float s[kN];
-#pragma unroll
-            for (int c = 0; c < kN; c += 32) tmem_ld(ts + c, s, c);
+            float s[64];
+            tmem_ld(ts, s, 0);
+            tmem_ld(ts + 32, s, 32);
             tmem_wait_ld();
-#pragma unroll
-            for (int c = 0; c < kN; c += 32) tmem_loaded(s, c);
+            tmem_loaded(s, 0);
+            tmem_loaded(s, 32);
             const int seen = mine - j * kN;
-            if (__any_sync(0xffffffffu, seen < kN)) {
+            const bool masked = __any_sync(0xffffffffu, seen < 64);
+            if (masked) {
 #pragma unroll
-                for (int c = 0; c < kN; c++) s[c] = c < seen ? s[c] : -INFINITY;
+                for (int c = 0; c < 64; c++) s[c] = c < seen ? s[c] : -INFINITY;
             }
             float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-            for (int c = 4; c < kN; c += 8)
+            for (int c = 4; c < 64; c += 8)
 #pragma unroll
-                for (int x = 0; x < 4; x++) top[x] = c + 4 + x < kN ? fmaxf(fmaxf(top[x], s[c + x]), s[c + 4 + x]) : fmaxf(top[x], s[c + x]);
-            const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-            const bool grew = (high - m) * scale > 8.0f;  // (never where the row has seen nothing: -inf - -inf)
-            if (__any_sync(0xffffffffu, grew)) {
+                for (int x = 0; x < 4; x++) top[x] = c + 4 + x < 64 ? fmaxf(fmaxf(top[x], s[c + x]), s[c + 4 + x]) : fmaxf(top[x], s[c + x]);
+            float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+            // Has any row's maximum grown by more than 2^8 (never where it has seen nothing: -inf - -inf)? Both threads of a row go by the same m.
+            if (tile_any(1 + t, (high - m) * scale > 8.0f)) {
+                sh.row[t][half][r] = high;
+                tile_any(1 + t, false);
+                high = fmaxf(high, sh.row[t][half ^ 1][r]);
+                const bool grew = (high - m) * scale > 8.0f;
                 const float by = grew ? exp2_fast((m - high) * scale) : 1.0f;
                 m = grew ? high : m;
                 sum *= by;
-                if (j) {  // the products of the blocks so far are done: S's commit follows them
-#pragma unroll
-                    for (int c = 0; c < HD; c += 32) {
-                        float o[32];
-                        tmem_ld(to + c, o, 0);
+                if (j && ok) {  // the products of the blocks so far are done: S's commit follows them
+#pragma unroll 1
+                    for (int c = half * (HD / 2); c < (half + 1) * (HD / 2); c += 16) {
+                        float o[16];
+                        tmem_ld16(to + c, o);
                         tmem_wait_ld();
-                        tmem_loaded(o, 0);
+                        tmem_loaded16(o);
 #pragma unroll
-                        for (int i = 0; i < 32; i++) o[i] *= by;
-                        tmem_st(to + c, o);
+                        for (int i = 0; i < 16; i++) o[i] *= by;
+                        tmem_st16(to + c, reinterpret_cast<const uint32_t(&)[16]>(o));
                     }
                 }
+                tile_any(1 + t, false);  // (both have read what the other wrote)
             }
-            const float from = m == -INFINITY ? 0.0f : -m * scale;
-            float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int c = 0; c < kN; c += 64) {
-                uint32_t w[32];
-#pragma unroll
-                for (int i = 0; i < 32; i++) {
-                    const float a = exp2_fast(fmaf(s[c + 2 * i], scale, from)), b = exp2_fast(fmaf(s[c + 2 * i + 1], scale, from));
-                    part[(2 * i) & 3] += a;
-                    part[(2 * i + 1) & 3] += b;
-                    // rounded to the cache's type for the second product: relative 2^-12 (f16) or 2^-9 (bf16), as the output itself will be
-                    w[i] = Half16<T>::pack(a, b);
-                }
-                tmem_st(ts + c / 2, w);
-            }
-            sum += (part[0] + part[1]) + (part[2] + part[3]);
             const int valid = it.kv_end - it.kv_begin - j * kN;
             if (valid < kN) {  // the last block: zeros in V's rows behind the last position (both tiles write the same zeros)
-                const int slot = 2 * j + 1, stage = slot % S::kStages;
-                ok = ok && bar_wait(&b_full[stage], (slot / S::kStages) & 1, &s_abort);
-                for (int x = valid * (HD / 8) + r; x < kN * (HD / 8); x += 128) {
+                const int slot = base + 2 * j + 1, stage = slot % S::kStages;
+                ok = ok && bar_wait(&sh.full[stage], (slot / S::kStages) & 1, &sh.abort);
+                for (int x = valid * (HD / 8) + half * 128 + r; x < kN * (HD / 8); x += 256) {
                     const int row = x / (HD / 8), c = x % (HD / 8);
                     asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(skv + stage * S::kTileBytes + (c / 8) * kHalfBytes + row * 128 + (c & 7) * 16), "r"(0)
                                  : "memory");
@@ -400,57 +451,89 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                 fence_async();
                 __syncwarp();
             }
-            tmem_wait_st();
-            fence_before();
-            bar_arrive(&b_p[t]);
+            const float from = m == -INFINITY ? 0.0f : -m * scale;
+            const f32x2 scale2 = pack2(scale, scale), from2 = pack2(from, from);
+            f32x2 part[2] = {0, 0};
+            // P over the half's own first columns of S, in two parts, so that the second product begins while the rest of the weights are made
+#pragma unroll
+            for (int q = 0; q < 2; q++) {
+                uint32_t w[16];
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const f32x2 x = fma2(pack2(s[q * 32 + 2 * i], s[q * 32 + 2 * i + 1]), scale2, from2);
+                    const float2 xs = unpack2(x), y = make_float2(exp2_fast(xs.x), exp2_fast(xs.y));
+                    part[i & 1] = sum2(part[i & 1], pack2(y.x, y.y));
+                    // rounded to the cache's type for the second product: relative 2^-12 (f16) or 2^-9 (bf16), as the output itself will be
+                    w[i] = Half16<T>::pack(y.x, y.y);
+                }
+                tmem_st16(ts + q * 16, w);
+                tmem_wait_st();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(&sh.p[t][q]);
+            }
+            const float2 total = unpack2(sum2(part[0], part[1]));
+            sum += total.x + total.y;
         }
-        if (n_blk[t]) ok = ok && bar_wait(&b_o[t], 0, &s_abort);
+        base += 2 * tl.n_all;
+        if (!n_tok) continue;
+        if (n_blk) ok = ok && bar_wait(&sh.o_full[t], n_q & 1, &sh.abort);
+        n_q += n_blk > 0;
         ok = __all_sync(0xffffffffu, ok);
         fence_after();
-        const bool live = r < rows;
+        if (n_blk) {  // (the next write there is a block and its barrier away)
+            sh.row[t][half][r] = sum;
+            tile_any(1 + t, false);
+            sum += sh.row[t][half ^ 1][r];
+        }
+        const bool live = ok && r < rows;
         const int tok = t * per_tile + (live ? r / group : 0), g = live ? r % group : 0;
         const bool joined = it.part >= 0;
-        const size_t part_row = (size_t)it.part + (size_t)hk * it.part_rows + it.part_off + (size_t)tok * group + g;
-        const size_t out_at = (size_t)(it.token + tok) * p.a.out_stride + (size_t)(hk * group + g) * HD;
+        const size_t part_row = (size_t)it.part + (size_t)it.head * it.part_rows + it.part_off + (size_t)tok * group + g;
+        const size_t out_at = (size_t)(it.token + tok) * p.a.out_stride + (size_t)(it.head * group + g) * HD;
         const float by = joined ? 1.0f : 1.0f / sum;
-        if (ok && n_tok[t]) {
-#pragma unroll
-            for (int c = 0; c < HD; c += 32) {
-                float o[32];
-                if (n_blk[t]) {
-                    tmem_ld(to + c, o, 0);
-                    tmem_wait_ld();
-                    tmem_loaded(o, 0);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 32; i++) o[i] = 0.0f;
+#pragma unroll 1
+        for (int c = half * (HD / 2); c < (half + 1) * (HD / 2); c += 32) {
+            float o[32];
+            if (n_blk) {
+                tmem_ld(to + c, o, 0);
+                tmem_wait_ld();
+                tmem_loaded(o, 0);
+                if (c + 32 == (half + 1) * (HD / 2)) {  // the last: O may be written again
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(&sh.o_empty[t]);
                 }
+            } else {
 #pragma unroll
-                for (int i = 0; i < 32; i++) o[i] *= by;
-                if (!live) {
-                } else if (joined || p.a.out_f32) {
-                    float *dst = joined ? p.a.part_o + part_row * HD + c : reinterpret_cast<float *>(p.a.out) + out_at + c;
-#pragma unroll
-                    for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4 *>(dst + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-                } else {
-                    T *dst = reinterpret_cast<T *>(p.a.out) + out_at + c;
-#pragma unroll
-                    for (int i = 0; i < 32; i += 8)
-                        *reinterpret_cast<uint4 *>(dst + i) = make_uint4(Half16<T>::pack(o[i], o[i + 1]), Half16<T>::pack(o[i + 2], o[i + 3]),
-                                                                         Half16<T>::pack(o[i + 4], o[i + 5]), Half16<T>::pack(o[i + 6], o[i + 7]));
-                }
-                __syncwarp();  // (the next columns' load is the whole warp's)
+                for (int i = 0; i < 32; i++) o[i] = 0.0f;
             }
-            if (live && joined) p.a.part_ml[part_row] = make_float2(m == -INFINITY ? m : m * scale, sum);
+#pragma unroll
+            for (int i = 0; i < 32; i++) o[i] *= by;
+            if (!live) {
+            } else if (joined || p.a.out_f32) {
+                float *dst = joined ? p.a.part_o + part_row * HD + c : reinterpret_cast<float *>(p.a.out) + out_at + c;
+#pragma unroll
+                for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4 *>(dst + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+            } else {
+                T *dst = reinterpret_cast<T *>(p.a.out) + out_at + c;
+#pragma unroll
+                for (int i = 0; i < 32; i += 8)
+                    *reinterpret_cast<uint4 *>(dst + i) = make_uint4(Half16<T>::pack(o[i], o[i + 1]), Half16<T>::pack(o[i + 2], o[i + 3]),
+                                                                     Half16<T>::pack(o[i + 4], o[i + 5]), Half16<T>::pack(o[i + 6], o[i + 7]));
+            }
+            __syncwarp();  // (the next columns' load is the whole warp's)
+        }
+        if (live && joined && half == 0) p.a.part_ml[part_row] = make_float2(m == -INFINITY ? m : m * scale, sum);
         }
     }
     fence_before();
     __syncthreads();
-    if (warp == 9) {
+    if (warp == kMmaWarp) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
     }
-    if (threadIdx.x == 0 && s_abort) atomicCAS(p.status, 0, 1 + (int)blockIdx.x);
+    if (threadIdx.x == 0 && sh.abort) atomicCAS(p.status, 0, 1 + (int)blockIdx.x);
 }
 
 int *g_status = nullptr;  // device word, made on first use
@@ -477,20 +560,31 @@ bool pool_map(CUtensorMap *map, const void *pool, int type, const PagedView &v, 
                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// q as [tokens][heads][HD]; boxes of 64 elements, a group's heads, a tile's tokens.
+bool query_map(CUtensorMap *map, const PagedAttn &a, int type) {
+    const EncodeTiled encode = encode_tiled();
+    const PagedView &v = a.b;
+    const cuuint64_t dims[3] = {(cuuint64_t)v.hd, (cuuint64_t)v.n_head, (cuuint64_t)v.tokens}, strides[2] = {(cuuint64_t)v.hd * 2, (cuuint64_t)a.q_stride * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)v.group, (cuuint32_t)(kM / v.group)}, step[3] = {1, 1, 1};
+    return encode && encode(map, type == kPagedF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(a.q), dims, strides,
+                            box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, int HD>
-void prompt_launch(const PromptParams &p, int n_items) {
+void prompt_launch(const PromptParams &p, int n_ctas) {
     static bool ready = false;
     if (!ready) {
         const cudaError_t e = cudaFuncSetAttribute(paged_prompt_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<HD>::kSmem);
         if (e != cudaSuccess) return set_error(e, "paged_prompt shared memory");
         ready = true;
     }
-    launch_kc(PDL_PAGED, "paged_prompt", paged_prompt_kernel<T, HD>, dim3(n_items, p.a.b.n_head_kv), dim3(kThreads), Shape<HD>::kSmem, p);
+    launch_kc(PDL_PAGED, "paged_prompt", paged_prompt_kernel<T, HD>, dim3(n_ctas), dim3(kThreads), Shape<HD>::kSmem, p);
 }
 
 }  // namespace
 
-void paged_prompt_launch(const PagedAttn &a, int type, int n_pages, int n_items) {
+void paged_prompt_launch(const PagedAttn &a, int type, int n_pages, const int32_t *begin, int n_ctas) {
     if (!g_status) {
         int *p = nullptr;
         if (cudaMalloc(&p, sizeof(int)) != cudaSuccess || cudaMemsetAsync(p, 0, sizeof(int), stream()) != cudaSuccess)
@@ -499,10 +593,12 @@ void paged_prompt_launch(const PagedAttn &a, int type, int n_pages, int n_items)
     }
     PromptParams p;
     p.a = a;
+    p.begin = begin;
     p.status = g_status;
-    if (!pool_map(&p.k, a.k_pages, type, a.b, n_pages) || !pool_map(&p.v, a.v_pages, type, a.b, n_pages)) return set_error_msg("paged_prompt: a tensor map was refused");
-    if (type == kPagedF16) a.b.hd == 128 ? prompt_launch<__half, 128>(p, n_items) : prompt_launch<__half, 64>(p, n_items);
-    else a.b.hd == 128 ? prompt_launch<__nv_bfloat16, 128>(p, n_items) : prompt_launch<__nv_bfloat16, 64>(p, n_items);
+    if (!query_map(&p.q, a, type) || !pool_map(&p.k, a.k_pages, type, a.b, n_pages) || !pool_map(&p.v, a.v_pages, type, a.b, n_pages)) 
+        return set_error_msg("paged_prompt: a tensor map was refused");
+    if (type == kPagedF16) a.b.hd == 128 ? prompt_launch<__half, 128>(p, n_ctas) : prompt_launch<__half, 64>(p, n_ctas);
+    else a.b.hd == 128 ? prompt_launch<__nv_bfloat16, 128>(p, n_ctas) : prompt_launch<__nv_bfloat16, 64>(p, n_ctas);
 }
 
 }  // namespace llamd
