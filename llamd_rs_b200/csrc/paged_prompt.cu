@@ -79,23 +79,24 @@ __device__ __forceinline__ void bar_arrive(uint64_t *bar) {
 __device__ __forceinline__ void bar_expect(uint64_t *bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes) : "memory");
 }
-// Parks in hardware up to the hinted time per call; gives up after 2^14 of them, or as soon as another warp has.
-__device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity, volatile int *abort) {
-    const uint32_t a = smem_addr(bar);
-    for (int i = 0; i < (1 << 14); i++) {
-        uint32_t done;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(done)
-            : "r"(a), "r"(parity)
-            : "memory");
-        if (done) return true;
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {  // (parks in hardware for a while where the phase is not over)
+    uint32_t done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    return done;
+}
+// Gives up after 2^20 tries (a second and more), or as soon as another warp has.
+__device__ __forceinline__ bool bar_wait_on(uint32_t bar, uint32_t parity, volatile int *abort) {
+    for (int i = 0; i < (1 << 20); i++) {
+        if (bar_try(bar, parity)) return true;
         if (*abort) return false;
     }
     *abort = 1;
     return false;
+}
+__device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity, volatile int *abort) {
+    const uint32_t a = smem_addr(bar);
+    if (__builtin_expect(bar_try(a, parity), 1)) return true;
+    return bar_wait_on(a, parity, abort);
 }
 __device__ __forceinline__ bool elect_one() {
     uint32_t p;
@@ -115,18 +116,21 @@ __device__ __forceinline__ void tma_tokens(uint32_t dst, const CUtensorMap *map,
 // Matrix descriptors of 128-byte rows with the 128-byte swizzle, 8-row groups 1024 bytes apart (start address, leading and stride offsets
 // in 16-byte units, version 1 at bit 46, layout 2 at bits 61-63). For K-major operands the leading offset is unused; for V, which
 // lies position by position (its contraction is along the rows), it is the distance of the next 64 elements.
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t leading) {
-    return (uint64_t)((addr & 0x3FFFF) >> 4) | (uint64_t)(leading >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+constexpr uint32_t kDescHigh = 1024 >> 4 | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t desc_low(uint32_t addr, uint32_t leading) { return addr >> 4 | (leading >> 4) << 16; }  // (shared memory ends below 2^18)
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)accumulate), "r"(kDescHigh)
+        : "memory");
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
-                 "r"(idesc), "r"(accumulate)
-                 : "memory");
-}
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b),
-                 "r"(idesc), "r"(accumulate)
-                 : "memory");
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tmov.b64 b, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)accumulate), "r"(kDescHigh)
+        : "memory");
 }
 __device__ __forceinline__ void mma_commit(uint64_t *bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
@@ -293,88 +297,92 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                 for (int t = 0; t < 2; t++)
                     if (n_q[t]) bar_wait(&sh.q_full[t], (n_q[t] - 1) & 1, &none);
             }
-        } else if (warp == kMmaWarp) {
-            // ---- the products ----
+        } else if (warp == kMmaWarp && elect_one()) {
+            // ---- the products: one thread ----
             // instruction descriptors: f32 sums (bit 4), operand types (bits 7, 10), N >> 3 at bit 17, M >> 4 at bit 24; V transposed (bit 16)
             constexpr uint32_t kS = 1u << 4 | kBf16 << 7 | kBf16 << 10 | (uint32_t)(kN >> 3) << 17 | (uint32_t)(kM >> 4) << 24;
             constexpr uint32_t kO = 1u << 4 | kBf16 << 7 | kBf16 << 10 | 1u << 16 | (uint32_t)(HD >> 3) << 17 | (uint32_t)(kM >> 4) << 24;
-            bool ok = true;
-            auto wait = [&](uint64_t *bar, int parity) {
-                ok = ok && bar_wait(bar, (uint32_t)parity & 1, &sh.abort);
-                ok = __all_sync(0xffffffffu, ok);
+            // (its warp shares a scheduler with four softmax warps, and every instruction between two products is time that the tensor cores
+            // may stand still: with the same steps taken by the whole warp, agreeing on each wait, a block took a tenth longer)
+            auto wait = [&](uint64_t *bar, uint32_t parity) {
+                const bool done = bar_wait(bar, parity, &sh.abort);
                 fence_after();
-                return ok;
+                return done;
             };
-            auto commit = [&](uint64_t *bar) {
-                if (elect_one()) mma_commit(bar);
-                __syncwarp();
-            };
-            auto full = [&](int slot) { return wait(&sh.full[slot % S::kStages], slot / S::kStages); };
-            auto scores = [&](int t, int slot) {
-                if (elect_one()) {
-                    const uint64_t a = smem_desc(sq + t * S::kTileBytes, 16), b = smem_desc(skv + (slot % S::kStages) * S::kTileBytes, 16);
-#pragma unroll
-                    for (int s = 0; s < HD / 16; s++) {
-                        const uint64_t at = (uint64_t)((s / 4) * (kHalfBytes >> 4) + (s % 4) * 2);
-                        mma_ss(tmem + t * kN, a + at, b + at, kS, s > 0);
-                    }
-                    mma_commit(&sh.s[t]);
+            struct Place {  // in the ring
+                int stage = 0;
+                uint32_t phase = 0;
+                __device__ __forceinline__ void on(int n) {
+                    stage += n;
+                    if (stage >= S::kStages) stage -= S::kStages, phase ^= 1;
                 }
-                __syncwarp();
             };
-            auto values = [&](int t, int slot, int part, bool more) {  // positions 0-31 and 64-95 of the block, then the others: as the weights come
-                if (elect_one()) {
-                    const uint64_t b = smem_desc(skv + (slot % S::kStages) * S::kTileBytes, kHalfBytes);
+            const uint32_t q_desc = desc_low(sq, 16), k_desc = desc_low(skv, 16), v_desc = desc_low(skv, kHalfBytes);
+            auto scores = [&](int t, int stage) {
+                const uint32_t a = q_desc + t * (S::kTileBytes >> 4), b = k_desc + stage * (S::kTileBytes >> 4);
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int half = i >> 1, step = 2 * part + (i & 1);  // 16 positions: 8 columns of P, over the half's own columns of S
-                        mma_ts(tmem + 2 * kN + t * HD, tmem + t * kN + half * 64 + step * 8, b + (uint64_t)((half * 4 + step) * (16 * 128 >> 4)), kO, more || part > 0 || i > 0);
-                    }
+                for (int s = 0; s < HD / 16; s++) {
+                    const uint32_t at = (s / 4) * (kHalfBytes >> 4) + (s % 4) * 2;
+                    mma_ss(tmem + t * kN, a + at, b + at, kS, s > 0);
                 }
-                __syncwarp();
+                mma_commit(&sh.s[t]);
             };
-            int base = 0, n_s[2] = {0, 0}, n_q[2] = {0, 0};  // slots of the pieces before; blocks and pieces of each tile
-            for (int n = first; n < last && ok; n++) {
-                const Tiles tl(p.a.item[n], per_tile);
-                if (!tl.n_all) continue;
-                full(base);
+            auto values = [&](int t, int stage, int part, bool more) {  // positions 0-31 and 64-95 of the block, then the others: as the weights come
+                const uint32_t b = v_desc + stage * (S::kTileBytes >> 4);
 #pragma unroll
-                for (int t = 0; t < 2; t++)
-                    if (ok && tl.n_blk[t] && wait(&sh.q_full[t], n_q[t])) {
-                        scores(t, base);
-                        if (tl.n_blk[t] == 1) commit(&sh.q_empty[t]);
-                    }
-                if (ok) commit(&sh.empty[base % S::kStages]);
-                for (int j = 0; j < tl.n_all && ok; j++) {
-                    const int k_next = base + 2 * j + 2;
-                    if (!full(k_next - 1)) break;
-                    if (j + 1 < tl.n_all && !full(k_next)) break;
+                for (int i = 0; i < 4; i++) {
+                    const int half = i >> 1, step = 2 * part + (i & 1);  // 16 positions: 8 columns of P, over the half's own columns of S
+                    mma_ts(tmem + 2 * kN + t * HD, tmem + t * kN + half * 64 + step * 8, b + (half * 4 + step) * (16 * 128 >> 4), kO, more || part > 0 || i > 0);
+                }
+            };
+            auto pieces = [&]() {  // false: a wait ran out
+                Place k, v;
+                v.on(1);
+                uint32_t s_phase[2] = {0, 0}, q_phase[2] = {0, 0};
+                bool read[2] = {false, false};  // O holds an earlier piece
+                for (int n = first; n < last; n++) {
+                    const Tiles tl(p.a.item[n], per_tile);
+                    if (!tl.n_all) continue;
+                    if (!wait(&sh.full[k.stage], k.phase)) return false;
 #pragma unroll
                     for (int t = 0; t < 2; t++) {
-                        if (!ok || j >= tl.n_blk[t]) continue;
-                        if (!j && n_q[t]) wait(&sh.o_empty[t], n_q[t] - 1);  // the piece before has been read out
-                        if (ok && wait(&sh.p[t][0], n_s[t])) values(t, k_next - 1, 0, j > 0);
-                        if (ok && wait(&sh.p[t][1], n_s[t])) values(t, k_next - 1, 1, j > 0);
-                        if (!ok) continue;
-                        n_s[t]++;
-                        if (j + 1 < tl.n_blk[t]) {
-                            scores(t, k_next);
-                            if (j + 2 == tl.n_blk[t]) commit(&sh.q_empty[t]);
-                        } else {
-                            commit(&sh.o_full[t]);
-                        }
+                        if (!tl.n_blk[t]) continue;
+                        if (!wait(&sh.q_full[t], q_phase[t])) return false;
+                        scores(t, k.stage);
+                        if (tl.n_blk[t] == 1) mma_commit(&sh.q_empty[t]);
                     }
-                    if (ok) {
-                        commit(&sh.empty[(k_next - 1) % S::kStages]);
-                        if (j + 1 < tl.n_all) commit(&sh.empty[k_next % S::kStages]);
-                    }
-                }
-                base += 2 * tl.n_all;
+                    mma_commit(&sh.empty[k.stage]);
+                    for (int j = 0; j < tl.n_all; j++) {
+                        k.on(2);
+                        if (!wait(&sh.full[v.stage], v.phase) || (j + 1 < tl.n_all && !wait(&sh.full[k.stage], k.phase))) return false;
 #pragma unroll
-                for (int t = 0; t < 2; t++) n_q[t] += tl.n_blk[t] > 0;
-            }
-            if (sh.abort) {  // given up: products on their way end before TMEM is given back
-                commit(&sh.drain);
+                        for (int t = 0; t < 2; t++) {
+                            if (j >= tl.n_blk[t]) continue;
+                            if (!j && read[t] && !wait(&sh.o_empty[t], q_phase[t] ^ 1)) return false;
+                            if (!wait(&sh.p[t][0], s_phase[t])) return false;
+                            values(t, v.stage, 0, j > 0);
+                            if (!wait(&sh.p[t][1], s_phase[t])) return false;
+                            values(t, v.stage, 1, j > 0);
+                            s_phase[t] ^= 1;
+                            if (j + 1 < tl.n_blk[t]) {
+                                scores(t, k.stage);
+                                if (j + 2 == tl.n_blk[t]) mma_commit(&sh.q_empty[t]);
+                            } else {
+                                mma_commit(&sh.o_full[t]);
+                            }
+                        }
+                        mma_commit(&sh.empty[v.stage]);
+                        if (j + 1 < tl.n_all) mma_commit(&sh.empty[k.stage]);
+                        v.on(2);
+                    }
+#pragma unroll
+                    for (int t = 0; t < 2; t++)
+                        if (tl.n_blk[t]) q_phase[t] ^= 1, read[t] = true;
+                }
+                return true;
+            };
+            if (!pieces()) {  // given up: products on their way end before TMEM is given back
+                mma_commit(&sh.drain);
                 volatile int none = 0;
                 bar_wait(&sh.drain, 0, &none);
             }
