@@ -8,11 +8,11 @@
 // (tcgen05, S and O in TMEM, P written over S in TMEM as the second product's operand), and 16384 exponentials, which take the
 // special function units as long as the products take the tensor cores: while one tile's softmax runs, the other's products do.
 //
-//   warps 0-7, 8-15  softmax of tile 0 / 1, two threads to a row, 64 positions each: S from TMEM, mask, maximum, exponentials, P to TMEM;
-//                    at the end O / sum
-//   warp 16          K and V blocks into a ring in shared memory (TMA, a box per page, 128-byte swizzle)
-//   warp 17          the products: S0, S1 of the first block, then per block PV0, S0', PV1, S1'
-//   warps 18, 19     nothing: registers are handed over by whole warpgroups
+//   warps 0-3, 4-7   softmax of tile 0 / 1, a thread per row: S from TMEM, mask, maximum, exponentials, P to TMEM; at the end O / sum
+//   warp 8           Q, and K and V blocks into a ring in shared memory (TMA, a box per page, 128-byte swizzle)
+//   warp 9           the products, one thread: S0, S1 of the first block, then per block PV0, S0', PV1, S1'
+//   warps 10, 11     nothing: registers are handed over by whole warpgroups
+// A CTA stays on its SM and works off a list of pieces; the next piece's Q and blocks are on their way while the last one ends.
 //
 // O stays in TMEM over all blocks. It is rescaled only when a row's maximum has grown by more than 2^8 since the last time (P is then at
 // most 2^8, far inside f16's range, and the sums are exact in the same way), which after the first block hardly ever happens.
@@ -29,18 +29,17 @@ namespace llamd {
 namespace {
 
 constexpr int kM = kPagedTileRows, kN = kPagedBlock;
-constexpr int kSoftmaxWarps = 16, kThreads = (kSoftmaxWarps + 4) * 32;
-// Registers of a softmax thread (64 scores live in them) and of the others: the launch gives 96 to each of 640, 512 x 104 + 128 x 64 =
-// 640 x 96.
-constexpr int kSoftmaxRegs = 104, kOtherRegs = 64;
-static_assert(kSoftmaxWarps * 32 * kSoftmaxRegs + 128 * kOtherRegs <= kThreads * 96, "no more than the launch's own");
+constexpr int kSoftmaxWarps = 8, kThreads = (kSoftmaxWarps + 4) * 32;
+// Registers of a softmax thread (a row's 128 scores live in them) and of the others: the launch gives 168 to each of 384, 256 x 208 + 128 x 88 =
+// 384 x 168.
+constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
+static_assert(kSoftmaxWarps * 32 * kSoftmaxRegs + 128 * kOtherRegs <= kThreads * 168, "no more than the launch's own");
 
 template <int HD> struct Shape {
     static constexpr int kTileBytes = kM * HD * 2;               // a tile of Q, a block of K or V: HD / 64 halves of 128 rows x 128 bytes
     static constexpr int kStages = HD == 128 ? 5 : 8;            // blocks of K or V in flight
     struct Rest {  // what follows the tiles in shared memory
         uint64_t q_full[2], q_empty[2], s[2], p[2][2], o_full[2], o_empty[2], full[kStages], empty[kStages], drain;
-        float row[2][2][kM];  // what the two threads of a row tell each other
         uint32_t tmem;
         volatile int abort;
     };
@@ -182,12 +181,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&v)[16]
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Whether x holds for any of the 256 softmax threads of a tile, which wait for one another here.
-__device__ __forceinline__ bool tile_any(int barrier, bool x) {
-    uint32_t any;
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, %2, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(any) : "r"((uint32_t)x), "r"(barrier) : "memory");
-    return any != 0;
-}
 __device__ __forceinline__ f32x2 sum2(f32x2 a, f32x2 b) {
     f32x2 r;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
@@ -217,10 +210,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
             bar_init(&sh.q_full[t], 1);
             bar_init(&sh.q_empty[t], 1);
             bar_init(&sh.s[t], 1);
-            bar_init(&sh.p[t][0], 8);
-            bar_init(&sh.p[t][1], 8);
+            bar_init(&sh.p[t][0], 4);
+            bar_init(&sh.p[t][1], 4);
             bar_init(&sh.o_full[t], 1);
-            bar_init(&sh.o_empty[t], 8);
+            bar_init(&sh.o_empty[t], 4);
         }
 #pragma unroll
         for (int i = 0; i < S::kStages; i++) {
@@ -302,7 +295,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
             // instruction descriptors: f32 sums (bit 4), operand types (bits 7, 10), N >> 3 at bit 17, M >> 4 at bit 24; V transposed (bit 16)
             constexpr uint32_t kS = 1u << 4 | kBf16 << 7 | kBf16 << 10 | (uint32_t)(kN >> 3) << 17 | (uint32_t)(kM >> 4) << 24;
             constexpr uint32_t kO = 1u << 4 | kBf16 << 7 | kBf16 << 10 | 1u << 16 | (uint32_t)(HD >> 3) << 17 | (uint32_t)(kM >> 4) << 24;
-            // (its warp shares a scheduler with four softmax warps, and every instruction between two products is time that the tensor cores
+            // (its warp shares a scheduler with two softmax warps, and every instruction between two products is time that the tensor cores
             // may stand still: with the same steps taken by the whole warp, agreeing on each wait, a block took a tenth longer)
             auto wait = [&](uint64_t *bar, uint32_t parity) {
                 const bool done = bar_wait(bar, parity, &sh.abort);
@@ -327,12 +320,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                 }
                 mma_commit(&sh.s[t]);
             };
-            auto values = [&](int t, int stage, int part, bool more) {  // positions 0-31 and 64-95 of the block, then the others: as the weights come
+            auto values = [&](int t, int stage, int part, bool more) {  // over 64 positions of the block
                 const uint32_t b = v_desc + stage * (S::kTileBytes >> 4);
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int half = i >> 1, step = 2 * part + (i & 1);  // 16 positions: 8 columns of P, over the half's own columns of S
-                    mma_ts(tmem + 2 * kN + t * HD, tmem + t * kN + half * 64 + step * 8, b + (half * 4 + step) * (16 * 128 >> 4), kO, more || part > 0 || i > 0);
+                for (int i = 0; i < 4; i++) {  // 16 positions: 8 columns of P, 16 rows of V
+                    const int step = part * 4 + i;
+                    mma_ts(tmem + 2 * kN + t * HD, tmem + t * kN + step * 8, b + step * (16 * 128 >> 4), kO, more || step > 0);
                 }
             };
             auto pieces = [&]() {  // false: a wait ran out
@@ -390,8 +383,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
     } else {
         // ---- softmax of tile t ----
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-        const int t = warp >> 3, half = (warp >> 2) & 1, r = threadIdx.x & 127;
-        const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), ts = lanes + t * kN + half * 64, to = lanes + 2 * kN + t * HD;
+        const int t = warp >> 2, r = threadIdx.x & 127;
+        const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), ts = lanes + t * kN, to = lanes + 2 * kN + t * HD;
         const float scale = p.a.scale_log2;
         bool ok = true;
         int base = 0, n_s = 0, n_q = 0;  // as the products' warp counts them
@@ -400,42 +393,38 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
         const Tiles tl(it, per_tile);
         const int n_tok = t ? tl.n_tok[1] : tl.n_tok[0], n_blk = t ? tl.n_blk[1] : tl.n_blk[0], rows = n_tok * group;
         float m = -INFINITY, sum = 0.0f;
-        // positions of the piece that this row sees, counted from the thread's half of a block
-        const int mine = min(it.kv_end, it.limit + it.step * (t * per_tile + min(r, rows - 1) / group)) - it.kv_begin - half * 64;
+        // positions of the piece that this row sees
+        const int mine = min(it.kv_end, it.limit + it.step * (t * per_tile + min(r, rows - 1) / group)) - it.kv_begin;
         for (int j = 0; j < n_blk; j++, n_s++) {
             ok = ok && bar_wait(&sh.s[t], n_s & 1, &sh.abort);
             ok = __all_sync(0xffffffffu, ok);
             fence_after();
-            float s[64];
-            tmem_ld(ts, s, 0);
-            tmem_ld(ts + 32, s, 32);
-            tmem_wait_ld();
-            tmem_loaded(s, 0);
-            tmem_loaded(s, 32);
-            const int seen = mine - j * kN;
-            const bool masked = __any_sync(0xffffffffu, seen < 64);
-            if (masked) {
+            float s[kN];
 #pragma unroll
-                for (int c = 0; c < 64; c++) s[c] = c < seen ? s[c] : -INFINITY;
+            for (int c = 0; c < kN; c += 32) tmem_ld(ts + c, s, c);
+            tmem_wait_ld();
+#pragma unroll
+            for (int c = 0; c < kN; c += 32) tmem_loaded(s, c);
+            const int seen = mine - j * kN;
+            if (__any_sync(0xffffffffu, seen < kN)) {
+#pragma unroll
+                for (int c = 0; c < kN; c++) s[c] = c < seen ? s[c] : -INFINITY;
             }
             float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-            for (int c = 4; c < 64; c += 8)
+            for (int c = 4; c < kN; c += 8)
 #pragma unroll
-                for (int x = 0; x < 4; x++) top[x] = c + 4 + x < 64 ? fmaxf(fmaxf(top[x], s[c + x]), s[c + 4 + x]) : fmaxf(top[x], s[c + x]);
-            float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-            // Has any row's maximum grown by more than 2^8 (never where it has seen nothing: -inf - -inf)? Both threads of a row go by the same m.
-            if (tile_any(1 + t, (high - m) * scale > 8.0f)) {
-                sh.row[t][half][r] = high;
-                tile_any(1 + t, false);
-                high = fmaxf(high, sh.row[t][half ^ 1][r]);
-                const bool grew = (high - m) * scale > 8.0f;
+                for (int x = 0; x < 4; x++) top[x] = c + 4 + x < kN ? fmaxf(fmaxf(top[x], s[c + x]), s[c + 4 + x]) : fmaxf(top[x], s[c + x]);
+            const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+            // has a row's maximum grown by more than 2^8? (never where it has seen nothing: -inf - -inf)
+            const bool grew = (high - m) * scale > 8.0f;
+            if (__any_sync(0xffffffffu, grew)) {
                 const float by = grew ? exp2_fast((m - high) * scale) : 1.0f;
                 m = grew ? high : m;
                 sum *= by;
                 if (j && ok) {  // the products of the blocks so far are done: S's commit follows them
 #pragma unroll 1
-                    for (int c = half * (HD / 2); c < (half + 1) * (HD / 2); c += 16) {
+                    for (int c = 0; c < HD; c += 16) {
                         float o[16];
                         tmem_ld16(to + c, o);
                         tmem_wait_ld();
@@ -445,13 +434,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                         tmem_st16(to + c, reinterpret_cast<const uint32_t(&)[16]>(o));
                     }
                 }
-                tile_any(1 + t, false);  // (both have read what the other wrote)
             }
             const int valid = it.kv_end - it.kv_begin - j * kN;
             if (valid < kN) {  // the last block: zeros in V's rows behind the last position (both tiles write the same zeros)
                 const int slot = base + 2 * j + 1, stage = slot % S::kStages;
                 ok = ok && bar_wait(&sh.full[stage], (slot / S::kStages) & 1, &sh.abort);
-                for (int x = valid * (HD / 8) + half * 128 + r; x < kN * (HD / 8); x += 256) {
+                for (int x = valid * (HD / 8) + r; x < kN * (HD / 8); x += 128) {
                     const int row = x / (HD / 8), c = x % (HD / 8);
                     asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(skv + stage * S::kTileBytes + (c / 8) * kHalfBytes + row * 128 + (c & 7) * 16), "r"(0)
                                  : "memory");
@@ -462,23 +450,25 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
             const float from = m == -INFINITY ? 0.0f : -m * scale;
             const f32x2 scale2 = pack2(scale, scale), from2 = pack2(from, from);
             f32x2 part[2] = {0, 0};
-            // P over the half's own first columns of S, in two parts, so that the second product begins while the rest of the weights are made
+            // P over S's first columns, in two parts, so that the second product begins while the rest of the weights are made
 #pragma unroll
-            for (int q = 0; q < 2; q++) {
+            for (int q = 0; q < 4; q++) {
                 uint32_t w[16];
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
-                    const f32x2 x = fma2(pack2(s[q * 32 + 2 * i], s[q * 32 + 2 * i + 1]), scale2, from2);
-                    const float2 xs = unpack2(x), y = make_float2(exp2_fast(xs.x), exp2_fast(xs.y));
+                    const float2 x = unpack2(fma2(pack2(s[q * 32 + 2 * i], s[q * 32 + 2 * i + 1]), scale2, from2));
+                    const float2 y = make_float2(exp2_fast(x.x), exp2_fast(x.y));
                     part[i & 1] = sum2(part[i & 1], pack2(y.x, y.y));
                     // rounded to the cache's type for the second product: relative 2^-12 (f16) or 2^-9 (bf16), as the output itself will be
                     w[i] = Half16<T>::pack(y.x, y.y);
                 }
                 tmem_st16(ts + q * 16, w);
-                tmem_wait_st();
-                fence_before();
-                __syncwarp();
-                if (lane == 0) bar_arrive(&sh.p[t][q]);
+                if (q & 1) {
+                    tmem_wait_st();
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(&sh.p[t][q >> 1]);
+                }
             }
             const float2 total = unpack2(sum2(part[0], part[1]));
             sum += total.x + total.y;
@@ -489,11 +479,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
         n_q += n_blk > 0;
         ok = __all_sync(0xffffffffu, ok);
         fence_after();
-        if (n_blk) {  // (the next write there is a block and its barrier away)
-            sh.row[t][half][r] = sum;
-            tile_any(1 + t, false);
-            sum += sh.row[t][half ^ 1][r];
-        }
         const bool live = ok && r < rows;
         const int tok = t * per_tile + (live ? r / group : 0), g = live ? r % group : 0;
         const bool joined = it.part >= 0;
@@ -501,13 +486,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
         const size_t out_at = (size_t)(it.token + tok) * p.a.out_stride + (size_t)(it.head * group + g) * HD;
         const float by = joined ? 1.0f : 1.0f / sum;
 #pragma unroll 1
-        for (int c = half * (HD / 2); c < (half + 1) * (HD / 2); c += 32) {
+        for (int c = 0; c < HD; c += 32) {
             float o[32];
             if (n_blk) {
                 tmem_ld(to + c, o, 0);
                 tmem_wait_ld();
                 tmem_loaded(o, 0);
-                if (c + 32 == (half + 1) * (HD / 2)) {  // the last: O may be written again
+                if (c + 32 == HD) {  // the last: O may be written again
                     fence_before();
                     __syncwarp();
                     if (lane == 0) bar_arrive(&sh.o_empty[t]);
@@ -532,7 +517,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
             }
             __syncwarp();  // (the next columns' load is the whole warp's)
         }
-        if (live && joined && half == 0) p.a.part_ml[part_row] = make_float2(m == -INFINITY ? m : m * scale, sum);
+        if (live && joined) p.a.part_ml[part_row] = make_float2(m == -INFINITY ? m : m * scale, sum);
         }
     }
     fence_before();
