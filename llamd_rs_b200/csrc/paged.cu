@@ -275,9 +275,10 @@ void make_plan(Plan &plan, const PagedView &v, const int32_t *q_len, const int32
 //   (a, b) -> (a cos - b sin, a sin + b cos) for the pairs among a head's first `rot` elements
 //   q_out <- y; the K and V rows of the token's slot <- y, v, rounded once to the cache's type
 //
-// Bytes bound it: every input is read once, every output written once, and a warp has kAppendVecs loads of 16 bytes a lane in flight
-// before it needs the first. A head takes hd / E lanes, E elements (16 bytes) to a lane, so the norm is a sum over
-// neighbouring lanes and a half-rotation's partner is rot / (2 E) lanes away. A warp stays with one token: its angles are read once.
+// Bytes bound it: every input is read once, every output written once. A head takes hd / 8 lanes, 8 elements to a lane: four pairs that
+// rotate together, so that the rotation needs no neighbour (the halves' layout: 4 elements and their 4 partners rot / 2 further on;
+// neighbouring pairs, and what lies behind the rotated part: 8 in a row), and the norm is a sum over the head's lanes. A warp has
+// kAppendVecs heads of one kind (q, k or v) of one token on their way at once, so the token's angles and the weights are read once for them.
 constexpr int kAppendVecs = 4;
 
 struct AppendParams {
@@ -286,142 +287,113 @@ struct AppendParams {
     size_t q_stride, k_stride, v_stride, out_stride;  // elements between tokens
     const float *wq, *wk, *rope;
     float eps;
-    int rot, interleaved, aligned, tasks, chunks;
+    int rot, aligned, tasks, q_tasks, kv_tasks;  // warps to a token, to its q heads, to its k or v heads
     void *q_out, *k_pages, *v_pages;
 };
 
-template <typename T, int E> struct AppendIo;
-template <int E> struct AppendIo<float, E> {
-    static_assert(E == 4, "16 bytes");
-    static __device__ __forceinline__ void load(const float *p, bool aligned, float (&x)[E]) {
-        if (aligned) {
-            const float4 f = __ldcs(reinterpret_cast<const float4 *>(p));
-            x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
-        } else {
+// 4 neighbouring elements in f32
+template <typename T>
+__device__ __forceinline__ void load4(const T *p, bool aligned, float *x) {
+    if (!aligned) {
 #pragma unroll
-            for (int i = 0; i < E; i++) x[i] = p[i];
-        }
-    }
-};
-template <typename T> struct AppendIo<T, 8> {
-    static __device__ __forceinline__ void load(const T *p, bool aligned, float (&x)[8]) {
-        if (aligned) {
-            const uint4 u = __ldcs(reinterpret_cast<const uint4 *>(p));
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float2 f = Half16<T>::to_f32(w[i]);
-                x[2 * i] = f.x, x[2 * i + 1] = f.y;
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = (float)p[i];
-        }
-    }
-};
-
-// TI: the inputs' type, T: the cache's. HD / E lanes to a head.
-template <typename TI, typename T, int HD>
-__global__ void __launch_bounds__(256) paged_append_kernel(const AppendParams p) {
-    constexpr int E = 16 / (int)sizeof(TI), L = HD / E, PER = 32 / L;  // heads side by side in a warp
-    pdl_trigger();
-    pdl_wait();
-    const int warp = (int)((blockIdx.x * blockDim.x + threadIdx.x) >> 5), lane = threadIdx.x & 31;
-    if (warp >= p.tasks) return;
-    const int t = warp / p.chunks, c = warp - t * p.chunks, sub = lane / L, l = lane % L, e0 = l * E;
-    const int H = p.b.n_head, K = p.b.n_head_kv, n_vec = H + 2 * K, v0 = c * (kAppendVecs * PER) + sub;
-    float x[kAppendVecs][E];
-#pragma unroll
-    for (int i = 0; i < kAppendVecs; i++) {
-        const int v = v0 + i * PER;
-        const TI *src = reinterpret_cast<const TI *>(p.q) + (size_t)t * p.q_stride + (size_t)v * HD;
-        if (v >= H) src = reinterpret_cast<const TI *>(p.k) + (size_t)t * p.k_stride + (size_t)(v - H) * HD;
-        if (v >= H + K) src = reinterpret_cast<const TI *>(p.v) + (size_t)t * p.v_stride + (size_t)(v - H - K) * HD;
-        if (v < n_vec) AppendIo<TI, E>::load(src + e0, p.aligned, x[i]);
-        else {
-#pragma unroll
-            for (int j = 0; j < E; j++) x[i][j] = 0.0f;
-        }
-    }
-    const PagedToken tok = p.b.token[t];
-    // the angles of this lane's elements: the pair (a, b) holds x[j] and its partner
-    float sn[E], cs[E];
-    const int half = p.rot >> 1;
-    if (e0 < p.rot) {
-        const float *row = p.rope + (size_t)tok.pos * p.rot;
-        if (p.interleaved) {
-#pragma unroll
-            for (int j = 0; j < E; j += 4) {
-                const float4 f = *reinterpret_cast<const float4 *>(row + e0 + j);
-                sn[j] = sn[j + 1] = f.x, cs[j] = cs[j + 1] = f.y;
-                sn[j + 2] = sn[j + 3] = f.z, cs[j + 2] = cs[j + 3] = f.w;
-            }
-        } else {
-            const int i0 = e0 < half ? e0 : e0 - half;
-#pragma unroll
-            for (int j = 0; j < E; j += 2) {
-                const float4 f = *reinterpret_cast<const float4 *>(row + 2 * (i0 + j));
-                sn[j] = f.x, cs[j] = f.y, sn[j + 1] = f.z, cs[j + 1] = f.w;
-            }
-        }
+        for (int i = 0; i < 4; i++) x[i] = (float)p[i];
+    } else if constexpr (sizeof(T) == 4) {
+        const float4 f = __ldcs(reinterpret_cast<const float4 *>(p));
+        x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
     } else {
-#pragma unroll
-        for (int j = 0; j < E; j++) sn[j] = 0.0f, cs[j] = 1.0f;
-    }
-    // the sign of the partner's term: the first of a pair loses b sin, the second gains a sin
-#pragma unroll
-    for (int j = 0; j < E; j++)
-        if (p.interleaved ? (j & 1) == 0 : e0 < half) sn[j] = -sn[j];
-    const int hop = half / E, partner = (lane & ~(L - 1)) + (e0 < p.rot ? (l < hop ? l + hop : l - hop) : l);
-    float wq[E], wk[E];
-#pragma unroll
-    for (int j = 0; j < E; j++) wq[j] = p.wq ? p.wq[e0 + j] : 1.0f, wk[j] = p.wk ? p.wk[e0 + j] : 1.0f;
-#pragma unroll
-    for (int i = 0; i < kAppendVecs; i++) {
-        const int v = v0 + i * PER;
-        const bool is_q = v < H, is_v = v >= H + K;
-        const float *w = is_q ? p.wq : p.wk;
-        // (the shuffles are the whole warp's: heads of other kinds, or beyond the last, come along and drop the result)
-        float ss = 0.0f;
-#pragma unroll
-        for (int j = 0; j < E; j++) ss = fmaf(x[i][j], x[i][j], ss);
-#pragma unroll
-        for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        if (w && !is_v) {
-            const float r = 1.0f / sqrtf(ss * (1.0f / HD) + p.eps);
-#pragma unroll
-            for (int j = 0; j < E; j++) x[i][j] = x[i][j] * r * (is_q ? wq[j] : wk[j]);
-        }
-        float y[E];
-#pragma unroll
-        for (int j = 0; j < E; j++) {
-            const float far = __shfl_sync(0xffffffffu, x[i][j], partner);
-            const float other = p.interleaved ? x[i][j ^ 1] : far;
-            y[j] = is_v || e0 >= p.rot ? x[i][j] : fmaf(other, sn[j], x[i][j] * cs[j]);
-        }
-        if (v >= n_vec) continue;
-        uint32_t out[E / 2];
-#pragma unroll
-        for (int j = 0; j < E / 2; j++) out[j] = Half16<T>::pack(y[2 * j], y[2 * j + 1]);
-        T *dst;
-        if (is_q) dst = reinterpret_cast<T *>(p.q_out) + (size_t)t * p.out_stride + (size_t)v * HD + e0;
-        else {
-            const size_t row = (size_t)tok.row + (size_t)(is_v ? v - H - K : v - H) * p.b.page;
-            dst = reinterpret_cast<T *>(is_v ? p.v_pages : p.k_pages) + row * HD + e0;
-        }
-        if constexpr (E == 8) *reinterpret_cast<uint4 *>(dst) = make_uint4(out[0], out[1], out[2], out[3]);
-        else *reinterpret_cast<uint2 *>(dst) = make_uint2(out[0], out[1]);
+        const uint2 u = __ldcs(reinterpret_cast<const uint2 *>(p));
+        const float2 f = Half16<T>::to_f32(u.x), g = Half16<T>::to_f32(u.y);
+        x[0] = f.x, x[1] = f.y, x[2] = g.x, x[3] = g.y;
     }
 }
 
-template <typename TI, typename T>
-void append_launch(AppendParams &p) {
-    const int hd = p.b.hd, per = 32 / (hd * (int)sizeof(TI) / 16);
-    p.chunks = (p.b.n_head + 2 * p.b.n_head_kv + kAppendVecs * per - 1) / (kAppendVecs * per);
-    p.tasks = p.b.tokens * p.chunks;
+// TI: the inputs' type, T: the cache's.
+template <typename TI, typename T, int HD, bool INTERLEAVED>
+__global__ void __launch_bounds__(256) paged_append_kernel(const AppendParams p) {
+    constexpr int L = HD / 8, PER = 32 / L;  // lanes to a head, heads side by side
+    pdl_trigger();
+    const int warp = (int)((blockIdx.x * blockDim.x + threadIdx.x) >> 5), lane = threadIdx.x & 31;
+    const int per_token = p.q_tasks + 2 * p.kv_tasks;
+    const bool any = warp < p.tasks;
+    const int t = any ? warp / per_token : 0, c = warp - t * per_token;
+    const PagedToken tok = any ? p.b.token[t] : PagedToken{0, 0};  // (the batch's own: complete before the launch in front of this one began)
+    pdl_wait();
+    if (!any) return;
+    const int kind = c < p.q_tasks ? 0 : c < p.q_tasks + p.kv_tasks ? 1 : 2;  // q, k, v
+    const int heads = kind ? p.b.n_head_kv : p.b.n_head, h0 = (c - (kind ? p.q_tasks + (kind - 1) * p.kv_tasks : 0)) * (kAppendVecs * PER) + lane / L;
+    const int l = lane % L;
+    const bool rotated = kind < 2 && l * 8 < p.rot;
+    const int first = rotated && !INTERLEAVED ? l * 4 : l * 8, second = rotated && !INTERLEAVED ? l * 4 + (p.rot >> 1) : l * 8 + 4;
+    const TI *src = reinterpret_cast<const TI *>(kind == 0 ? p.q : kind == 1 ? p.k : p.v) + (size_t)t * (kind == 0 ? p.q_stride : kind == 1 ? p.k_stride : p.v_stride);
+    float x[kAppendVecs][8];
+#pragma unroll
+    for (int i = 0; i < kAppendVecs; i++) {
+        const int h = h0 + i * PER;
+        if (h < heads) {
+            load4(src + (size_t)h * HD + first, p.aligned, x[i]);
+            load4(src + (size_t)h * HD + second, p.aligned, x[i] + 4);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[i][j] = 0.0f;
+        }
+    }
+    if (kind < 2) {
+        const float *wp = kind ? p.wk : p.wq;
+        float sn[4], cs[4], w[8];
+        if (rotated) {  // pair i's angle: of element first + i, or of the pair's place
+            const float4 *row = reinterpret_cast<const float4 *>(p.rope + (size_t)tok.pos * p.rot + l * 8);
+            const float4 f = row[0], g = row[1];
+            sn[0] = f.x, cs[0] = f.y, sn[1] = f.z, cs[1] = f.w, sn[2] = g.x, cs[2] = g.y, sn[3] = g.z, cs[3] = g.w;
+        }
+        if (wp) load4(wp + first, p.aligned, w), load4(wp + second, p.aligned, w + 4);
+#pragma unroll
+        for (int i = 0; i < kAppendVecs; i++) {
+            if (wp) {
+                float ss = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 8; j++) ss = fmaf(x[i][j], x[i][j], ss);
+#pragma unroll
+                for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                const float r = 1.0f / sqrtf(fmaf(ss, 1.0f / HD, p.eps));
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[i][j] *= r * w[j];
+            }
+            if (rotated) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    float &a = x[i][INTERLEAVED ? 2 * j : j], &b = x[i][INTERLEAVED ? 2 * j + 1 : j + 4];
+                    const float ra = fmaf(-b, sn[j], a * cs[j]), rb = fmaf(a, sn[j], b * cs[j]);
+                    a = ra, b = rb;
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kAppendVecs; i++) {
+        const int h = h0 + i * PER;
+        if (h >= heads) break;
+        T *dst;
+        if (kind == 0) dst = reinterpret_cast<T *>(p.q_out) + (size_t)t * p.out_stride + (size_t)h * HD;
+        else dst = reinterpret_cast<T *>(kind == 1 ? p.k_pages : p.v_pages) + ((size_t)tok.row + (size_t)h * p.b.page) * HD;
+        *reinterpret_cast<uint2 *>(dst + first) = make_uint2(Half16<T>::pack(x[i][0], x[i][1]), Half16<T>::pack(x[i][2], x[i][3]));
+        *reinterpret_cast<uint2 *>(dst + second) = make_uint2(Half16<T>::pack(x[i][4], x[i][5]), Half16<T>::pack(x[i][6], x[i][7]));
+    }
+}
+
+template <typename TI, typename T, int HD>
+void append_launch_hd(AppendParams &p, bool interleaved) {
+    constexpr int kHeads = kAppendVecs * (32 / (HD / 8));  // to a warp
+    p.q_tasks = (p.b.n_head + kHeads - 1) / kHeads;
+    p.kv_tasks = (p.b.n_head_kv + kHeads - 1) / kHeads;
+    p.tasks = p.b.tokens * (p.q_tasks + 2 * p.kv_tasks);
     const dim3 grid((unsigned)((p.tasks + 7) / 8));
-    if (hd == 128) launch_k("paged_append", paged_append_kernel<TI, T, 128>, grid, dim3(256), 0, p);
-    else launch_k("paged_append", paged_append_kernel<TI, T, 64>, grid, dim3(256), 0, p);
+    if (interleaved) launch_kc(PDL_PAGED, "paged_append", paged_append_kernel<TI, T, HD, true>, grid, dim3(256), 0, p);
+    else launch_kc(PDL_PAGED, "paged_append", paged_append_kernel<TI, T, HD, false>, grid, dim3(256), 0, p);
+}
+template <typename TI, typename T>
+void append_launch(AppendParams &p, bool interleaved) {
+    if (p.b.hd == 128) append_launch_hd<TI, T, 128>(p, interleaved);
+    else append_launch_hd<TI, T, 64>(p, interleaved);
 }
 
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
@@ -538,16 +510,16 @@ int llamd_fwd_paged_append(const void *batch, const void *q, const void *k, cons
     AppendParams p = {};
     p.b = g;
     p.q = q, p.k = k, p.v = v, p.q_stride = q_stride, p.k_stride = k_stride, p.v_stride = v_stride, p.out_stride = out_stride;
-    p.wq = wq, p.wk = wk, p.eps = eps, p.rope = rope_tab, p.rot = rot, p.interleaved = interleaved;
+    p.wq = wq, p.wk = wk, p.eps = eps, p.rope = rope_tab, p.rot = rot;
     p.q_out = q_out, p.k_pages = k_pages, p.v_pages = v_pages;
     const size_t per16 = in_type == kPagedF32 ? 4 : 8;
-    p.aligned = aligned16(q) && aligned16(k) && aligned16(v) && !(q_stride % per16) && !(k_stride % per16) && !(v_stride % per16);
+    p.aligned = aligned16(q) && aligned16(k) && aligned16(v) && !(q_stride % per16) && !(k_stride % per16) && !(v_stride % per16) && aligned16(wq) && aligned16(wk);
     if (b->type == kPagedF16) {
-        if (in_type == kPagedF32) append_launch<float, __half>(p);
-        else append_launch<__half, __half>(p);
+        if (in_type == kPagedF32) append_launch<float, __half>(p, interleaved != 0);
+        else append_launch<__half, __half>(p, interleaved != 0);
     } else {
-        if (in_type == kPagedF32) append_launch<float, __nv_bfloat16>(p);
-        else append_launch<__nv_bfloat16, __nv_bfloat16>(p);
+        if (in_type == kPagedF32) append_launch<float, __nv_bfloat16>(p, interleaved != 0);
+        else append_launch<__nv_bfloat16, __nv_bfloat16>(p, interleaved != 0);
     }
     return error_code() ? -1 : 0;
 }

@@ -110,8 +110,9 @@ class Batch:
         self.ptr = lib().llamd_cuda_paged_new(n_head, n_head_kv, head_dim, page_size, self.type)
         if not self.ptr:
             _refuse("paged batch")
-        self.tokens, self.n_pages = 0, 0
-        self._pool_bytes = 0
+        self.tokens, self.n_pages, self.scale = 0, 0, 1.0 / math.sqrt(head_dim)
+        self._append, self._attention = lib().llamd_fwd_paged_append, lib().llamd_fwd_paged_attention
+        self._pool = 0
 
     def set(self, q_lens, kv_lens, pages, n_pages: int, n_shared: int = 0) -> None:
         """q_lens, kv_lens: new tokens and positions in all of every sequence; pages: their tables, rows of one int32 array or a
@@ -130,48 +131,42 @@ class Batch:
         if lib().llamd_cuda_paged_set(self.ptr, q.size, backend._ptr(q), backend._ptr(kv), backend._ptr(pages), pages.shape[1], n_pages, n_shared) != 0:
             _refuse("paged batch")
         self.tokens, self.n_pages = int(q.sum()), n_pages
-        self._pool_bytes = 2 * n_pages * self.n_head_kv * self.page_size * self.head_dim
+        self._pool = n_pages * self.n_head_kv * self.page_size * self.head_dim
 
-    def _rows(self, x, heads, type_, what, stride=None):
-        """(address, elements between tokens) of `tokens` rows of `heads` heads."""
-        n = heads * self.head_dim
-        if hasattr(x, "data_ptr"):
+    def _rows(self, x, n, type_, what, stride=None):
+        """(address, elements between tokens) of `tokens` rows of n elements."""
+        try:
+            ptr = x.data_ptr()
+        except AttributeError:
+            stride = n if stride is None else stride
+            if isinstance(x, DevBuf):
+                if self.tokens and x.nbytes < ((self.tokens - 1) * stride + n) * _SIZE[type_]:
+                    raise ShapeError(f"{what}: {x.nbytes} bytes for {self.tokens} tokens") from None
+                return x.ptr, stride
+            return x, stride
+        if _type_of(x) != type_ or not x.is_cuda:
+            raise ShapeError(f"{what}: {x.dtype} on {x.device}")
+        if x.numel() == self.tokens * n:
+            if x.is_contiguous() and (not self.tokens or x.shape[0] == self.tokens):
+                return ptr, n
             shape, st = x.shape, x.stride()
-            if _type_of(x) != type_ or not x.is_cuda:
-                raise ShapeError(f"{what}: {x.dtype} on {x.device}")
-            if shape[0] != self.tokens or x.numel() != self.tokens * n or st[-1] != 1 or (len(shape) == 3 and (shape[2] != self.head_dim or (heads > 1 and st[1] != self.head_dim))):
-                raise ShapeError(f"{what}: {tuple(shape)} with strides {st} for {self.tokens} tokens of {heads} heads of {self.head_dim}")
-            return x.data_ptr(), st[0] if shape[0] > 1 else n
-        stride = n if stride is None else stride
-        if isinstance(x, DevBuf):
-            if self.tokens and x.nbytes < ((self.tokens - 1) * stride + n) * _SIZE[type_]:
-                raise ShapeError(f"{what}: {x.nbytes} bytes for {self.tokens} tokens")
-            return x.ptr, stride
-        return x, stride
+            if shape[0] == self.tokens and st[-1] == 1 and (len(shape) == 2 or (len(shape) == 3 and shape[2] == self.head_dim and (shape[1] == 1 or st[1] == self.head_dim))):
+                return ptr, st[0] if shape[0] > 1 else n
+        raise ShapeError(f"{what}: {tuple(x.shape)} with strides {x.stride()} for {self.tokens} tokens of {n // self.head_dim} heads of {self.head_dim}")
 
-    def _pool(self, x, what):
-        if hasattr(x, "data_ptr"):
-            if _type_of(x) != self.type or not x.is_cuda or not x.is_contiguous() or x.numel() * 2 < self._pool_bytes:
-                raise ShapeError(f"{what}: {x.dtype}, {tuple(x.shape)} for {self.n_pages} pages")
-            return x.data_ptr()
-        if isinstance(x, DevBuf):
-            if x.nbytes < self._pool_bytes:
-                raise ShapeError(f"{what}: {x.nbytes} bytes for {self.n_pages} pages")
-            return x.ptr
-        return x
-
-    def _f32(self, x, n, what):
-        if x is None:
-            return None
-        if hasattr(x, "data_ptr"):
-            if _type_of(x) != 2 or not x.is_cuda or not x.is_contiguous() or x.numel() < n:
-                raise ShapeError(f"{what}: {x.dtype}, {tuple(x.shape)}")
-            return x.data_ptr()
-        if isinstance(x, DevBuf):
-            if x.nbytes < 4 * n:
-                raise ShapeError(f"{what}: {x.nbytes} bytes for {n} values")
-            return x.ptr
-        return x
+    def _whole(self, x, type_, n, what):
+        """The address of n contiguous values at least."""
+        try:
+            ptr = x.data_ptr()
+        except AttributeError:
+            if isinstance(x, DevBuf):
+                if x.nbytes < n * _SIZE[type_]:
+                    raise ShapeError(f"{what}: {x.nbytes} bytes for {n} values") from None
+                return x.ptr
+            return x
+        if _type_of(x) != type_ or x.numel() < n or not x.is_contiguous() or not x.is_cuda:
+            raise ShapeError(f"{what}: {x.dtype}, {tuple(x.shape)} on {x.device} for {n} values")
+        return ptr
 
     def append(self, q, k, v, q_out, k_pages, v_pages, rope=None, rot: int | None = None, interleaved: bool = False, q_norm=None, k_norm=None,
                eps: float = 1e-6, inputs: str | None = None, rope_rows: int | None = None, strides=(None, None, None)) -> None:
@@ -195,22 +190,27 @@ class Batch:
                 rope_rows = rope.nbytes // (4 * rot)
             else:
                 raise Malformed("rope_rows: how many positions the table has")
-        (qp, qs), (kp, ks), (vp, vs) = (self._rows(x, h, it, w, st) for x, h, w, st in (
-            (q, self.n_head, "q", strides[0]), (k, self.n_head_kv, "k", strides[1]), (v, self.n_head_kv, "v", strides[2])))
-        op, os_ = self._rows(q_out, self.n_head, self.type, "q_out")
-        if lib().llamd_fwd_paged_append(self.ptr, qp, kp, vp, it, qs, ks, vs, self._f32(q_norm, self.head_dim, "q_norm"),
-                                     self._f32(k_norm, self.head_dim, "k_norm"), eps, self._f32(rope, rope_rows * rot, "rope") if rot else None, rope_rows,
-                                     rot, 1 if interleaved else 0, op, os_, self._pool(k_pages, "k_pages"), self._pool(v_pages, "v_pages")) != 0:
+        D = self.head_dim
+        nq, nk = self.n_head * D, self.n_head_kv * D
+        qp, qs = self._rows(q, nq, it, "q", strides[0])
+        kp, ks = self._rows(k, nk, it, "k", strides[1])
+        vp, vs = self._rows(v, nk, it, "v", strides[2])
+        op, os_ = self._rows(q_out, nq, self.type, "q_out")
+        if self._append(self.ptr, qp, kp, vp, it, qs, ks, vs, None if q_norm is None else self._whole(q_norm, 2, D, "q_norm"),
+                        None if k_norm is None else self._whole(k_norm, 2, D, "k_norm"), eps, self._whole(rope, 2, rope_rows * rot, "rope") if rot else None,
+                        rope_rows, rot, interleaved, op, os_, self._whole(k_pages, self.type, self._pool, "k_pages"),
+                        self._whole(v_pages, self.type, self._pool, "v_pages")) != 0:
             _refuse("append")
 
     def attention(self, q, k_pages, v_pages, out, scale: float | None = None, out_f32: bool | None = None) -> None:
         """llamd_fwd_paged_attention. ``out_f32`` says of an address that it takes f32; a tensor's type says so itself."""
         if out_f32 is None:
             out_f32 = hasattr(out, "data_ptr") and _type_of(out) == 2
-        qp, qs = self._rows(q, self.n_head, self.type, "q")
-        op, os_ = self._rows(out, self.n_head, 2 if out_f32 else self.type, "out")
-        if lib().llamd_fwd_paged_attention(self.ptr, qp, qs, self._pool(k_pages, "k_pages"), self._pool(v_pages, "v_pages"), op, os_, 1 if out_f32 else 0,
-                                        1.0 / math.sqrt(self.head_dim) if scale is None else scale) != 0:
+        n = self.n_head * self.head_dim
+        qp, qs = self._rows(q, n, self.type, "q")
+        op, os_ = self._rows(out, n, 2 if out_f32 else self.type, "out")
+        if self._attention(self.ptr, qp, qs, self._whole(k_pages, self.type, self._pool, "k_pages"), self._whole(v_pages, self.type, self._pool, "v_pages"), op, os_,
+                           out_f32, self.scale if scale is None else scale) != 0:
             _refuse("attention")
 
     def free(self) -> None:
