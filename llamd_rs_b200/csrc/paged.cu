@@ -22,7 +22,7 @@ int refuse(const char *why) {
 
 struct Batch {
     PagedView view = {};
-    int type = 0, n_pages = 0, max_kv = 0;
+    int type = 0, n_pages = 0, max_kv = 0, sms = 0;
     bool ready = false;
     // the device copy of everything below, and the pinned memory it is made in
     uint8_t *dev = nullptr, *host = nullptr;
@@ -278,8 +278,11 @@ void make_plan(Plan &plan, const PagedView &v, const int32_t *q_len, const int32
 // Bytes bound it: every input is read once, every output written once. A head takes hd / 8 lanes, 8 elements to a lane: four pairs that
 // rotate together, so that the rotation needs no neighbour (the halves' layout: 4 elements and their 4 partners rot / 2 further on;
 // neighbouring pairs, and what lies behind the rotated part: 8 in a row), and the norm is a sum over the head's lanes. A warp has
-// kAppendVecs heads of one kind (q, k or v) of one token on their way at once, so the token's angles and the weights are read once for them.
-constexpr int kAppendVecs = 4;
+// several heads of one kind (q, k or v) of one token on their way at once, so the token's angles and the weights are read once for them.
+// Heads that a warp has on their way, and CTAs to an SM; 16-bit and f32 inputs measured (2, 4 and 8 heads, 3 to 6 CTAs): 8192 tokens of f32 13.3 us with
+// 2 heads and 4 CTAs, 6279 tokens of f16 31.6 with 4 and 4, the others 13.5 to 18.7 and 34.9 to 55.
+template <typename TI> constexpr int kAppendHeads = sizeof(TI) == 2 ? 4 : 2;
+constexpr int kAppendCtas = 4;
 
 struct AppendParams {
     PagedView b;
@@ -287,106 +290,108 @@ struct AppendParams {
     size_t q_stride, k_stride, v_stride, out_stride;  // elements between tokens
     const float *wq, *wk, *rope;
     float eps;
-    int rot, aligned, tasks, q_tasks, kv_tasks;  // warps to a token, to its q heads, to its k or v heads
+    int rot, aligned, sms, tasks, q_tasks, kv_tasks;  // warps to a token, to its q heads, to its k or v heads
     void *q_out, *k_pages, *v_pages;
 };
 
-// 4 neighbouring elements in f32
-template <typename T>
-__device__ __forceinline__ void load4(const T *p, bool aligned, float *x) {
-    if (!aligned) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) x[i] = (float)p[i];
-    } else if constexpr (sizeof(T) == 4) {
-        const float4 f = __ldcs(reinterpret_cast<const float4 *>(p));
-        x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
-    } else {
-        const uint2 u = __ldcs(reinterpret_cast<const uint2 *>(p));
-        const float2 f = Half16<T>::to_f32(u.x), g = Half16<T>::to_f32(u.y);
+// 4 neighbouring elements as they lie, and in f32
+template <typename T> struct Four {
+    uint2 v;
+    __device__ __forceinline__ void load(const T *p, bool aligned) {
+        if (aligned) {
+            v = __ldcs(reinterpret_cast<const uint2 *>(p));
+        } else {
+            const uint16_t *h = reinterpret_cast<const uint16_t *>(p);
+            v = make_uint2(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16);
+        }
+    }
+    __device__ __forceinline__ void get(float *x) const {
+        const float2 f = Half16<T>::to_f32(v.x), g = Half16<T>::to_f32(v.y);
         x[0] = f.x, x[1] = f.y, x[2] = g.x, x[3] = g.y;
     }
-}
+};
+template <> struct Four<float> {
+    float4 v;
+    __device__ __forceinline__ void load(const float *p, bool aligned) { v = aligned ? __ldcs(reinterpret_cast<const float4 *>(p)) : make_float4(p[0], p[1], p[2], p[3]); }
+    __device__ __forceinline__ void get(float *x) const { x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w; }
+};
 
 // TI: the inputs' type, T: the cache's.
 template <typename TI, typename T, int HD, bool INTERLEAVED>
-__global__ void __launch_bounds__(256) paged_append_kernel(const AppendParams p) {
-    constexpr int L = HD / 8, PER = 32 / L;  // lanes to a head, heads side by side
+__global__ void __launch_bounds__(256, kAppendCtas) paged_append_kernel(const AppendParams p) {
+    constexpr int L = HD / 8, PER = 32 / L, kDeep = kAppendHeads<TI>;  // lanes to a head, heads side by side, heads one behind the other
     pdl_trigger();
-    const int warp = (int)((blockIdx.x * blockDim.x + threadIdx.x) >> 5), lane = threadIdx.x & 31;
-    const int per_token = p.q_tasks + 2 * p.kv_tasks;
-    const bool any = warp < p.tasks;
-    const int t = any ? warp / per_token : 0, c = warp - t * per_token;
-    const PagedToken tok = any ? p.b.token[t] : PagedToken{0, 0};  // (the batch's own: complete before the launch in front of this one began)
+    const int warps = (int)(gridDim.x * (blockDim.x >> 5)), lane = threadIdx.x & 31, per_token = p.q_tasks + 2 * p.kv_tasks;
+    int task = (int)((blockIdx.x * blockDim.x + threadIdx.x) >> 5);
+    // (the batch's own memory: complete before the launch in front of this one began)
+    PagedToken next = task < p.tasks ? p.b.token[task / per_token] : PagedToken{0, 0};
     pdl_wait();
-    if (!any) return;
-    const int kind = c < p.q_tasks ? 0 : c < p.q_tasks + p.kv_tasks ? 1 : 2;  // q, k, v
-    const int heads = kind ? p.b.n_head_kv : p.b.n_head, h0 = (c - (kind ? p.q_tasks + (kind - 1) * p.kv_tasks : 0)) * (kAppendVecs * PER) + lane / L;
-    const int l = lane % L;
-    const bool rotated = kind < 2 && l * 8 < p.rot;
-    const int first = rotated && !INTERLEAVED ? l * 4 : l * 8, second = rotated && !INTERLEAVED ? l * 4 + (p.rot >> 1) : l * 8 + 4;
-    const TI *src = reinterpret_cast<const TI *>(kind == 0 ? p.q : kind == 1 ? p.k : p.v) + (size_t)t * (kind == 0 ? p.q_stride : kind == 1 ? p.k_stride : p.v_stride);
-    float x[kAppendVecs][8];
+    for (; task < p.tasks; task += warps) {
+        const int t = task / per_token, c = task - t * per_token;
+        const PagedToken tok = next;
+        if (task + warps < p.tasks) next = p.b.token[(task + warps) / per_token];  // (a round ahead: the angles' address waits for nothing)
+        const int kind = c < p.q_tasks ? 0 : c < p.q_tasks + p.kv_tasks ? 1 : 2;  // q, k, v
+        const int heads = kind ? p.b.n_head_kv : p.b.n_head, h0 = (c - (kind ? p.q_tasks + (kind - 1) * p.kv_tasks : 0)) * (kDeep * PER) + lane / L;
+        const int l = lane % L;
+        const bool rotated = kind < 2 && l * 8 < p.rot;
+        const int first = rotated && !INTERLEAVED ? l * 4 : l * 8, second = rotated && !INTERLEAVED ? l * 4 + (p.rot >> 1) : l * 8 + 4;
+        const TI *src = reinterpret_cast<const TI *>(kind == 0 ? p.q : kind == 1 ? p.k : p.v) + (size_t)t * (kind == 0 ? p.q_stride : kind == 1 ? p.k_stride : p.v_stride);
+        Four<TI> raw[kDeep][2];
 #pragma unroll
-    for (int i = 0; i < kAppendVecs; i++) {
-        const int h = h0 + i * PER;
-        if (h < heads) {
-            load4(src + (size_t)h * HD + first, p.aligned, x[i]);
-            load4(src + (size_t)h * HD + second, p.aligned, x[i] + 4);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; j++) x[i][j] = 0.0f;
+        for (int i = 0; i < kDeep; i++) {
+            const int h = h0 + i * PER;
+            if (h < heads) raw[i][0].load(src + (size_t)h * HD + first, p.aligned), raw[i][1].load(src + (size_t)h * HD + second, p.aligned);
+            else raw[i][0] = raw[i][1] = Four<TI>{};
         }
-    }
-    if (kind < 2) {
-        const float *wp = kind ? p.wk : p.wq;
-        float sn[4], cs[4], w[8];
+        const float *wp = kind == 0 ? p.wq : kind == 1 ? p.wk : nullptr;
+        float sn[4], cs[4];
+        Four<float> w[2];
         if (rotated) {  // pair i's angle: of element first + i, or of the pair's place
             const float4 *row = reinterpret_cast<const float4 *>(p.rope + (size_t)tok.pos * p.rot + l * 8);
             const float4 f = row[0], g = row[1];
             sn[0] = f.x, cs[0] = f.y, sn[1] = f.z, cs[1] = f.w, sn[2] = g.x, cs[2] = g.y, sn[3] = g.z, cs[3] = g.w;
         }
-        if (wp) load4(wp + first, p.aligned, w), load4(wp + second, p.aligned, w + 4);
+        if (wp) w[0].load(wp + first, p.aligned), w[1].load(wp + second, p.aligned);
+        T *dst = reinterpret_cast<T *>(kind == 0 ? p.q_out : kind == 1 ? p.k_pages : p.v_pages) + (kind ? (size_t)tok.row * HD : (size_t)t * p.out_stride);
+        const size_t dst_step = kind ? (size_t)p.b.page * HD : HD;
 #pragma unroll
-        for (int i = 0; i < kAppendVecs; i++) {
+        for (int i = 0; i < kDeep; i++) {
+            const int h = h0 + i * PER;
+            float x[8];
+            raw[i][0].get(x), raw[i][1].get(x + 4);
             if (wp) {
-                float ss = 0.0f;
+                float ss = 0.0f, wx[8];
 #pragma unroll
-                for (int j = 0; j < 8; j++) ss = fmaf(x[i][j], x[i][j], ss);
+                for (int j = 0; j < 8; j++) ss = fmaf(x[j], x[j], ss);
 #pragma unroll
                 for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-                const float r = 1.0f / sqrtf(fmaf(ss, 1.0f / HD, p.eps));
+                const float r = rsqrtf(fmaf(ss, 1.0f / HD, p.eps));  // (2 ulp)
+                w[0].get(wx), w[1].get(wx + 4);
 #pragma unroll
-                for (int j = 0; j < 8; j++) x[i][j] *= r * w[j];
+                for (int j = 0; j < 8; j++) x[j] *= r * wx[j];
             }
             if (rotated) {
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    float &a = x[i][INTERLEAVED ? 2 * j : j], &b = x[i][INTERLEAVED ? 2 * j + 1 : j + 4];
+                    float &a = x[INTERLEAVED ? 2 * j : j], &b = x[INTERLEAVED ? 2 * j + 1 : j + 4];
                     const float ra = fmaf(-b, sn[j], a * cs[j]), rb = fmaf(a, sn[j], b * cs[j]);
                     a = ra, b = rb;
                 }
             }
+            if (h >= heads) continue;
+            *reinterpret_cast<uint2 *>(dst + h * dst_step + first) = make_uint2(Half16<T>::pack(x[0], x[1]), Half16<T>::pack(x[2], x[3]));
+            *reinterpret_cast<uint2 *>(dst + h * dst_step + second) = make_uint2(Half16<T>::pack(x[4], x[5]), Half16<T>::pack(x[6], x[7]));
         }
-    }
-#pragma unroll
-    for (int i = 0; i < kAppendVecs; i++) {
-        const int h = h0 + i * PER;
-        if (h >= heads) break;
-        T *dst;
-        if (kind == 0) dst = reinterpret_cast<T *>(p.q_out) + (size_t)t * p.out_stride + (size_t)h * HD;
-        else dst = reinterpret_cast<T *>(kind == 1 ? p.k_pages : p.v_pages) + ((size_t)tok.row + (size_t)h * p.b.page) * HD;
-        *reinterpret_cast<uint2 *>(dst + first) = make_uint2(Half16<T>::pack(x[i][0], x[i][1]), Half16<T>::pack(x[i][2], x[i][3]));
-        *reinterpret_cast<uint2 *>(dst + second) = make_uint2(Half16<T>::pack(x[i][4], x[i][5]), Half16<T>::pack(x[i][6], x[i][7]));
     }
 }
 
 template <typename TI, typename T, int HD>
 void append_launch_hd(AppendParams &p, bool interleaved) {
-    constexpr int kHeads = kAppendVecs * (32 / (HD / 8));  // to a warp
+    constexpr int kHeads = kAppendHeads<TI> * (32 / (HD / 8));  // to a warp
     p.q_tasks = (p.b.n_head + kHeads - 1) / kHeads;
     p.kv_tasks = (p.b.n_head_kv + kHeads - 1) / kHeads;
     p.tasks = p.b.tokens * (p.q_tasks + 2 * p.kv_tasks);
-    const dim3 grid((unsigned)((p.tasks + 7) / 8));
+    const dim3 grid((unsigned)std::min((p.tasks + 7) / 8, kAppendCtas * p.sms));
     if (interleaved) launch_kc(PDL_PAGED, "paged_append", paged_append_kernel<TI, T, HD, true>, grid, dim3(256), 0, p);
     else launch_kc(PDL_PAGED, "paged_append", paged_append_kernel<TI, T, HD, false>, grid, dim3(256), 0, p);
 }
@@ -419,6 +424,12 @@ void *llamd_cuda_paged_new(int n_head, int n_head_kv, int hd, int page_size, int
     }
     b->view.n_head = n_head, b->view.n_head_kv = n_head_kv, b->view.group = n_head / n_head_kv, b->view.hd = hd, b->view.page = page_size;
     b->type = type;
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&b->sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) {
+        set_error(cudaGetLastError(), "paged batch: device");
+        delete b;
+        return nullptr;
+    }
     return b;
 }
 
@@ -438,12 +449,9 @@ int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int
         v.table_stride = std::max(v.table_stride, (kv_len[s] + v.page - 1) / v.page);
     }
     if ((long long)n_seq * v.table_stride > 0x7fffffffLL) return refuse("paged batch: the tables have more than 2^31 entries");
-    int device = 0, sms = 0;
-    LLAMD_TRY(cudaGetDevice(&device), "paged batch: device");
-    LLAMD_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device), "paged batch: device");
     Plan plan;
     try {
-        make_plan(plan, v, q_len, kv_len, sms);
+        make_plan(plan, v, q_len, kv_len, b->sms);
     } catch (const std::exception &) {
         return refuse("paged batch: out of host memory");
     }
@@ -508,7 +516,7 @@ int llamd_fwd_paged_append(const void *batch, const void *q, const void *k, cons
     if (q_stride < qd || k_stride < kvd || v_stride < kvd || out_stride < qd) return refuse("paged append: a row overlaps the next");
     if (!aligned16(q_out) || out_stride % 8 || !aligned16(k_pages) || !aligned16(v_pages)) return refuse("paged append: outputs start at 16 bytes");
     AppendParams p = {};
-    p.b = g;
+    p.b = g, p.sms = b->sms;
     p.q = q, p.k = k, p.v = v, p.q_stride = q_stride, p.k_stride = k_stride, p.v_stride = v_stride, p.out_stride = out_stride;
     p.wq = wq, p.wk = wk, p.eps = eps, p.rope = rope_tab, p.rot = rot;
     p.q_out = q_out, p.k_pages = k_pages, p.v_pages = v_pages;
