@@ -33,7 +33,7 @@ struct Batch {
     const PagedMerge *merge = nullptr;
     const PagedPart *part = nullptr;
     const int32_t *begin = nullptr;  // large: each CTA's
-    int n_small = 0, small_rows = 0, n_ctas = 0, n_merge = 0;
+    int n_small = 0, small_rows = 0, n_ctas = 0, n_merge = 0, most = 0;
     uint8_t *partial = nullptr;
     size_t partial_bytes = 0, partial_rows = 0;
 
@@ -112,14 +112,14 @@ struct Plan {
     std::vector<int32_t> begin;  // large: each CTA's
     std::vector<PagedMerge> merge;
     std::vector<PagedPart> part;
-    int small_rows = 0;
+    int small_rows = 0, most = 0;  // rows of a small piece, parts of a token and head
     size_t rows = 0;  // of partial results
 };
 
 // A stretch of positions that some tokens attend to: a sequence's own behind the shared prefix, or the prefix itself.
 struct Stretch {
     int table, begin, end, token, n_tok, limit, step;
-    bool small(int group) const { return (long long)n_tok * group <= kPagedSmallRows; }
+    bool small(int group) const { return group <= kPagedSmallRows && (long long)n_tok * group <= kPagedFewRows; }
 };
 
 // Positions to a piece of paged_decode.cu. Its CTAs run two to an SM; the longest piece should not outlast an even share of
@@ -130,143 +130,177 @@ int decode_piece(long long positions, int n_head_kv, int sms) {
     return (int)std::max(128LL, (share + 15) / 16 * 16);
 }
 
-// Some tokens of a stretch for paged_prompt.cu, and how many blocks of positions they see some of.
-struct Tile {
-    int token, n_tok, end, blocks;
-};
-
 // paged_prompt.cu runs one CTA to an SM, each with a list of pieces. In blocks of its loop, a piece costs its blocks and about one more to begin
 // and end, leaving partial results one more again, and the launch that joins them about two.
-constexpr double kPieceCost = 1.0, kPartCost = 1.0, kJoinCost = 2.0;
+constexpr double kPieceCost = 1.0, kPartCost = 2.5, kJoinCost = 4.0;
 
-// Hands the longest of what is left to the CTA with the least so far. costs: in falling order; `to` (may be null) takes each one's CTA. Returns when
-// the last CTA ends.
-double deal(const std::vector<double> &costs, int ctas, std::vector<int> *to) {
+struct Large {  // a tile of one kv head
+    int tile, head, blocks;
+};
+struct Cut {  // blocks [first, first + n) of a Large, for a CTA
+    int which, first, n, cta;
+};
+
+// Whole tiles, the longest of what is left to the CTA with the least so far. Returns when the last CTA ends; `large`: in falling order of blocks.
+double deal_whole(const std::vector<Large> &large, int ctas, std::vector<Cut> &cuts) {
     std::vector<std::pair<double, int>> load(ctas);
     for (int i = 0; i < ctas; i++) load[i] = {0.0, i};
     double last = 0.0;
     const auto later = std::greater<std::pair<double, int>>();
-    for (double c : costs) {
+    for (size_t i = 0; i < large.size(); i++) {
         std::pop_heap(load.begin(), load.end(), later);
-        load.back().first += c;
+        load.back().first += large[i].blocks + kPieceCost;
         last = std::max(last, load.back().first);
-        if (to) to->push_back(load.back().second);
+        cuts.push_back({(int)i, 0, large[i].blocks, load.back().second});
         std::push_heap(load.begin(), load.end(), later);
     }
     return last;
 }
-
-// Blocks to a piece: the cut of the longest tile with which the last CTA ends soonest.
-int prompt_piece(const std::vector<Tile> &tiles, int n_head_kv, int sms) {
-    int longest = 1;
-    for (const Tile &t : tiles) longest = std::max(longest, t.blocks);
-    double best = 1e30;
-    int piece = longest;
-    std::vector<double> costs;
-    for (int cuts : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 40, 48, 64, 96, 128}) {
-        const int per = (longest + cuts - 1) / cuts;
-        if (cuts > longest || (cuts > 1 && (long long)tiles.size() * n_head_kv * cuts > 24LL * sms)) break;
-        costs.clear();
-        for (const Tile &t : tiles) {
-            const int n = (t.blocks + per - 1) / per, each = (t.blocks + n - 1) / n;
-            for (int b = 0; b < t.blocks; b += each)
-                costs.insert(costs.end(), n_head_kv, std::min(each, t.blocks - b) + kPieceCost + (n > 1 ? kPartCost : 0.0));
+// One tile after the other, each CTA filled up to `most` and the tile cut there. False where `most` is too little.
+bool deal_cut(const std::vector<Large> &large, int ctas, double most, std::vector<Cut> &cuts) {
+    cuts.clear();
+    int cta = 0;
+    double left = most;
+    for (size_t i = 0; i < large.size(); i++)
+        for (int first = 0; first < large[i].blocks;) {
+            const int rest = large[i].blocks - first;
+            int n = rest;
+            if (first || rest + kPieceCost > left) n = std::min(rest, (int)(left - kPieceCost - kPartCost));
+            if (n < std::min(rest, 2)) {  // (not a piece of one block at a CTA's end)
+                if (++cta >= ctas) return false;
+                left = most;
+                if (most < 2 + kPieceCost + kPartCost) return false;
+                continue;
+            }
+            cuts.push_back({(int)i, first, n, cta});
+            left -= n + kPieceCost + (n < large[i].blocks ? kPartCost : 0.0);
+            first += n;
         }
-        std::sort(costs.begin(), costs.end(), std::greater<double>());
-        const double ends = deal(costs, sms, nullptr) + (cuts > 1 ? kJoinCost : 0.0);
-        if (ends < best) best = ends, piece = per;
-    }
-    return piece;
+    return true;
 }
 
 void make_plan(Plan &plan, const PagedView &v, const int32_t *q_len, const int32_t *kv_len, int sms) {
-    const int group = v.group, tile_tokens = 2 * (kPagedTileRows / group);
+    const int group = v.group, few_tokens = std::max(1, kPagedSmallRows / group);
     std::vector<Stretch> stretch;  // the shared one, where there is one, then the sequences' own
     const bool shared = v.n_shared && v.tokens;
     if (shared) stretch.push_back({0, 0, v.n_shared, 0, v.tokens, v.n_shared, 0});
     for (int s = 0, t = 0; s < v.n_seq; t += q_len[s], s++)
         if (q_len[s]) stretch.push_back({s * v.table_stride, v.n_shared, kv_len[s], t, q_len[s], kv_len[s] - q_len[s] + 1, 1});
-    long long small_positions = 0;
-    std::vector<Tile> tiles;  // of the large stretches, in order
-    for (const Stretch &st : stretch) {
-        if (st.small(group)) {
-            small_positions += st.end - st.begin;
-            continue;
-        }
-        for (int i = 0; i < st.n_tok; i += tile_tokens) {
-            const int n = std::min(tile_tokens, st.n_tok - i), end = std::min(st.end, st.limit + st.step * (i + n - 1));
-            tiles.push_back({st.token + i, n, end, (end - st.begin + kPagedBlock - 1) / kPagedBlock});
-        }
-    }
-    const int small_piece = decode_piece(small_positions, v.n_head_kv, sms), large_piece = prompt_piece(tiles, v.n_head_kv, sms) * kPagedBlock;
-    // The pieces of `tok` tokens from `token` on over [begin, end), cut evenly at multiples of `unit`; where others join their rows, or there are
-    // several, each leaves partial results of its own rows.
-    auto cut = [&](const Stretch &st, int token, int n_tok, int end, bool small, bool joined, std::vector<PagedPart> &parts) {
-        const int unit = small ? 16 : kPagedBlock, most = small ? small_piece : large_piece, len = end - st.begin, n = (len + most - 1) / most;
-        const int per = ((len + n - 1) / n + unit - 1) / unit * unit, rows = n_tok * group;
-        for (int b = st.begin; b < end; b += per) {
-            PagedItem it = {st.table, b, std::min(end, b + per), token, n_tok, st.limit + st.step * (token - st.token), st.step, -1, 0, 0, 0, 0};
-            if (joined || len > per) {
-                it.part = (int32_t)std::min<size_t>(plan.rows, 0x7fffffff), it.part_rows = rows;
-                parts.push_back({it.part, rows, token});
-                plan.rows += (size_t)rows * v.n_head_kv;
-            }
-            if (small) plan.small_rows = std::max(plan.small_rows, rows);
-            (small ? plan.small : plan.large).push_back(it);
-        }
+    // a large piece is two tiles of query rows, but one where there are more SMs than such pieces
+    int tile_tokens = 2 * (kPagedTileRows / group);
+    long long pairs = 0;
+    for (const Stretch &st : stretch)
+        if (!st.small(group)) pairs += (st.n_tok + tile_tokens - 1) / tile_tokens;
+    if (2 * pairs * v.n_head_kv <= sms) tile_tokens /= 2;
+
+    // some tokens of a stretch, and where they leave partial results, by kv head
+    struct Tile {
+        int stretch, token, n_tok, end;
+        std::vector<std::vector<PagedPart>> parts;
     };
-    // the shared stretch: its tiles are cut alike, so that all tokens have the same list of parts
-    std::vector<PagedPart> prefix;
-    size_t i = 0, tile = 0;
-    if (shared) {
-        const Stretch &st = stretch[i++];
-        const bool small = st.small(group);
-        const size_t first = plan.large.size();
-        cut(st, st.token, st.n_tok, st.end, small, true, prefix);
-        if (!small) {
-            const std::vector<PagedItem> whole(plan.large.begin() + first, plan.large.end());
-            plan.large.resize(first);
-            for (; tile < tiles.size() && tiles[tile].token < st.n_tok && tile * (size_t)tile_tokens < (size_t)st.n_tok; tile++)
-                for (PagedItem it : whole) {
-                    it.token = tiles[tile].token, it.n_tok = tiles[tile].n_tok, it.part_off = tiles[tile].token * group;
-                    plan.large.push_back(it);
-                }
-        }
-    }
-    for (; i < stretch.size(); i++) {
+    std::vector<Tile> tiles;
+    std::vector<Large> large;
+    long long small_positions = 0;
+    for (size_t i = 0; i < stretch.size(); i++) {
         const Stretch &st = stretch[i];
         const bool small = st.small(group);
-        for (int t = 0; t < st.n_tok;) {
-            const Tile own = small ? Tile{st.token, st.n_tok, st.end, 0} : tiles[tile++];
-            const int begin = (int)plan.part.size();
-            plan.part.insert(plan.part.end(), prefix.begin(), prefix.end());
-            cut(st, own.token, own.n_tok, own.end, small, shared, plan.part);
-            const int count = (int)plan.part.size() - begin;
-            for (int x = 0; count && x < own.n_tok; x++) plan.merge.push_back({own.token + x, begin, count, 0});
-            t += own.n_tok;
+        const int most = small ? few_tokens : tile_tokens, n_tiles = (st.n_tok + most - 1) / most, per = small ? (st.n_tok + n_tiles - 1) / n_tiles : most;
+        for (int x = 0; x < st.n_tok; x += per) {
+            const int n = std::min(per, st.n_tok - x), end = std::min(st.end, st.limit + st.step * (x + n - 1));
+            tiles.push_back({(int)i, st.token + x, n, end, std::vector<std::vector<PagedPart>>(v.n_head_kv)});
+            if (small) small_positions += end - st.begin;
+            else
+                for (int h = 0; h < v.n_head_kv; h++) large.push_back({(int)tiles.size() - 1, h, (end - st.begin + kPagedBlock - 1) / kPagedBlock});
         }
     }
-    // the longest first: what is left at the end is short
-    auto longer = [](const PagedItem &a, const PagedItem &b) { return a.kv_end - a.kv_begin > b.kv_end - b.kv_begin; };
-    std::stable_sort(plan.small.begin(), plan.small.end(), longer);
-    std::stable_sort(plan.large.begin(), plan.large.end(), longer);
-    // the large ones by kv head, dealt out
-    std::vector<PagedItem> dealt;
-    std::vector<double> costs;
-    std::vector<int> to;
-    for (PagedItem it : plan.large)
-        for (it.head = 0; it.head < v.n_head_kv; it.head++) {
-            dealt.push_back(it);
-            costs.push_back((it.kv_end - it.kv_begin + kPagedBlock - 1) / kPagedBlock + kPieceCost + (it.part >= 0 ? kPartCost : 0.0));
+    auto item_of = [&](const Tile &tile, int begin, int end) {
+        const Stretch &st = stretch[tile.stretch];
+        return PagedItem{st.table, begin, end, tile.token, tile.n_tok, st.limit + st.step * (tile.token - st.token), st.step, -1, 0, 0, {0, 0}};
+    };
+    // room for the partial results of a tile's rows, of `heads` kv heads
+    auto room = [&](const Tile &tile, int heads) {
+        const int32_t at = (int32_t)std::min<size_t>(plan.rows, 0x7fffffff);
+        plan.rows += (size_t)tile.n_tok * group * heads;
+        return at;
+    };
+
+    // the small ones: cut evenly, the kv heads alike
+    const int piece = decode_piece(small_positions, v.n_head_kv, sms);
+    for (Tile &tile : tiles) {
+        const Stretch &st = stretch[tile.stretch];
+        if (!st.small(group)) continue;
+        const int len = tile.end - st.begin, n = (len + piece - 1) / piece, per = ((len + n - 1) / n + 15) / 16 * 16, rows = tile.n_tok * group;
+        for (int b = st.begin; b < tile.end; b += per) {
+            PagedItem it = item_of(tile, b, std::min(tile.end, b + per));
+            if (shared || len > per) {
+                it.part = room(tile, v.n_head_kv), it.part_rows = rows;
+                for (int h = 0; h < v.n_head_kv; h++) tile.parts[h].push_back({it.part + h * rows, tile.token});
+            }
+            plan.small_rows = std::max(plan.small_rows, rows);
+            plan.small.push_back(it);
         }
-    const int ctas = (int)std::min<size_t>(sms, dealt.size());
-    deal(costs, ctas, &to);
+    }
+    // (the longest first: what is left at the end is short)
+    std::stable_sort(plan.small.begin(), plan.small.end(), [](const PagedItem &a, const PagedItem &b) { return a.kv_end - a.kv_begin > b.kv_end - b.kv_begin; });
+
+    // the large ones: whole, or cut where that ends sooner
+    std::stable_sort(large.begin(), large.end(), [](const Large &a, const Large &b) { return a.blocks > b.blocks; });
+    std::vector<Cut> cuts, cut;
+    const double whole = deal_whole(large, sms, cuts);
+    double total = 0.0;
+    for (const Large &x : large) total += x.blocks;
+    double low = std::max(total / sms, 2 + kPieceCost + kPartCost), high = whole - kJoinCost;
+    while (high - low > 0.02 * high) {
+        const double most = 0.5 * (low + high);
+        if (deal_cut(large, sms, most, cut)) {
+            cuts = cut;
+            high = most;
+        } else {
+            low = most;
+        }
+    }
+    int ctas = 0;
+    for (const Cut &c : cuts) ctas = std::max(ctas, c.cta + 1);
     plan.begin.assign(ctas + 1, 0);
-    for (int c : to) plan.begin[c + 1]++;
+    for (const Cut &c : cuts) plan.begin[c.cta + 1]++;
     for (int c = 0; c < ctas; c++) plan.begin[c + 1] += plan.begin[c];
-    plan.large.resize(dealt.size());
-    std::vector<int> at(plan.begin.begin(), plan.begin.end() - 1);
-    for (size_t x = 0; x < dealt.size(); x++) plan.large[at[to[x]]++] = dealt[x];
+    plan.large.resize(cuts.size());
+    std::vector<int> at(plan.begin.begin(), plan.begin.end());
+    for (const Cut &c : cuts) {
+        const Large &x = large[c.which];
+        Tile &tile = tiles[x.tile];
+        const int begin = stretch[tile.stretch].begin + c.first * kPagedBlock;
+        PagedItem it = item_of(tile, begin, std::min(tile.end, begin + c.n * kPagedBlock));
+        it.head = x.head;
+        if (shared || c.n < x.blocks) {
+            it.part = room(tile, 1);
+            tile.parts[x.head].push_back({it.part, tile.token});
+        }
+        plan.large[at[c.cta]++] = it;
+    }
+
+    // who joins what: the shared stretch's tiles come first and cover all tokens
+    size_t prefix = 0, own = 0;
+    while (shared && own < tiles.size() && tiles[own].stretch == 0) own++;
+    for (; own < tiles.size(); own++) {
+        const Tile &tile = tiles[own];
+        for (int t = tile.token; t < tile.token + tile.n_tok;) {
+            int end = tile.token + tile.n_tok;
+            if (shared) {
+                while (tiles[prefix].token + tiles[prefix].n_tok <= t) prefix++;
+                end = std::min(end, tiles[prefix].token + tiles[prefix].n_tok);
+            }
+            for (int h = 0; h < v.n_head_kv; h++) {
+                const int begin = (int)plan.part.size();
+                if (shared) plan.part.insert(plan.part.end(), tiles[prefix].parts[h].begin(), tiles[prefix].parts[h].end());
+                plan.part.insert(plan.part.end(), tile.parts[h].begin(), tile.parts[h].end());
+                const int count = (int)plan.part.size() - begin;
+                plan.most = std::max(plan.most, count);
+                for (int x = t; count && x < end; x++) plan.merge.push_back({x, h, begin, count});
+            }
+            t = end;
+        }
+    }
 }
 
 // ---- append --------------------------------------------------------------------------------------------------------------
@@ -455,7 +489,7 @@ int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int
     } catch (const std::exception &) {
         return refuse("paged batch: out of host memory");
     }
-    if (plan.rows > 0x7fffffff) return refuse("paged batch: too many partial results");
+    if (plan.rows > 0x7fffffff || plan.merge.size() * v.group > 0x7fffffff) return refuse("paged batch: too many partial results");
     size_t bytes = 0;
     const size_t o_token = section<PagedToken>(bytes, v.tokens), o_seq = section<int32_t>(bytes, v.tokens),
                  o_table = section<int32_t>(bytes, (size_t)n_seq * v.table_stride), o_small = section<PagedItem>(bytes, plan.small.size()),
@@ -487,7 +521,7 @@ int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int
     b->begin = (const int32_t *)(b->dev + o_begin);
     b->merge = (const PagedMerge *)(b->dev + o_merge);
     b->part = (const PagedPart *)(b->dev + o_part);
-    b->n_small = (int)plan.small.size(), b->small_rows = plan.small_rows, b->n_ctas = (int)plan.begin.size() - 1, b->n_merge = (int)plan.merge.size();
+    b->n_small = (int)plan.small.size(), b->small_rows = plan.small_rows, b->n_ctas = (int)plan.begin.size() - 1, b->n_merge = (int)plan.merge.size(), b->most = plan.most;
     b->partial_rows = plan.rows;
     b->n_pages = n_pages, b->max_kv = max_kv;
     v.token = (const PagedToken *)(b->dev + o_token);
@@ -557,7 +591,7 @@ int llamd_fwd_paged_attention(const void *batch, const void *q, size_t q_stride,
         a.item = b->small;
         paged_decode_launch(a, b->type, b->n_small, b->small_rows);
     }
-    if (b->n_merge) paged_merge_launch(a, b->type, b->merge, b->part, b->n_merge);
+    if (b->n_merge) paged_merge_launch(a, b->type, b->merge, b->part, b->n_merge, b->most, b->sms);
     return error_code() ? -1 : 0;
 }
 

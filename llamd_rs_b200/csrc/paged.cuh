@@ -27,18 +27,18 @@ struct PagedView {
 // One piece of attention: n_tok tokens (all their heads that share kv head `head`; for paged_decode.cu the launch's y) over positions
 // [kv_begin, kv_end) of one table.
 // Token i of the piece sees positions below limit + i * step. part < 0: the piece is all its rows need, and writes out;
-// otherwise its rows' sums go to rows part + head * part_rows + part_off + ... of the batch's partial results.
+// otherwise its rows' sums go to rows part + ... of the batch's partial results (paged_decode.cu: + head * part_rows).
 struct PagedItem {
-    int32_t table, kv_begin, kv_end, token, n_tok, limit, step, part, part_rows, part_off, head, pad;
+    int32_t table, kv_begin, kv_end, token, n_tok, limit, step, part, part_rows, head, pad[2];
 };
 static_assert(sizeof(PagedItem) == 48, "three 16-byte words");
 
-// Where a token finds its partial results: entries [begin, begin + count) of the list below.
+// Where the rows of a token and a kv head find their partial results: entries [begin, begin + count) of the list below.
 struct PagedMerge {
-    int32_t token, begin, count, pad;
+    int32_t token, head, begin, count;
 };
 struct PagedPart {
-    int32_t part, part_rows, token;  // row of (token t, head h of kv head k): part + k * part_rows + (t - token) * group + h
+    int32_t row, token;  // the row of token t and head g of the group: row + (t - token) * group + g
 };
 
 // A partial result: sums of 2^(s - m) v over the piece's positions (s: the scores times log2 e), in f32, and beside them m and sum 2^(s - m).
@@ -54,12 +54,13 @@ struct PagedAttn {
     float2 *part_ml;   // [rows] (m, sum)
 };
 
-constexpr int kPagedSmallRows = 32;  // query rows (tokens x heads of a group) of a piece that paged_decode.cu takes
+// Query rows (tokens x heads of a group) of a piece that paged_decode.cu takes, and of a stretch that goes there in pieces of so many.
+constexpr int kPagedSmallRows = 32, kPagedFewRows = 96;
 
 void paged_decode_launch(const PagedAttn &p, int type, int n_items, int max_rows);
 constexpr int kPagedTileRows = 128, kPagedBlock = 128;  // of paged_prompt.cu: two tiles of query rows to a piece, positions to a block
 void paged_prompt_launch(const PagedAttn &p, int type, int n_pages, const int32_t *begin, int n_ctas);  // begin: each CTA's pieces (n_ctas + 1)
-void paged_merge_launch(const PagedAttn &p, int type, const PagedMerge *merge, const PagedPart *parts, int n_tokens);
+void paged_merge_launch(const PagedAttn &p, int type, const PagedMerge *merge, const PagedPart *parts, int n_merge, int most, int sms);  // most: parts of any of them
 
 // 16-bit types of a cache and what the kernels need of them.
 template <typename T> struct Half16;

@@ -37,13 +37,14 @@ static_assert(kSoftmaxWarps * 32 * kSoftmaxRegs + 128 * kOtherRegs <= kThreads *
 
 template <int HD> struct Shape {
     static constexpr int kTileBytes = kM * HD * 2;               // a tile of Q, a block of K or V: HD / 64 halves of 128 rows x 128 bytes
-    static constexpr int kStages = HD == 128 ? 5 : 8;            // blocks of K or V in flight
+    static constexpr int kQueries = HD == 128 ? 3 : 4;           // tiles of Q: the two at work and the next
+    static constexpr int kStages = HD == 128 ? 4 : 8;            // blocks of K or V in flight
     struct Rest {  // what follows the tiles in shared memory
-        uint64_t q_full[2], q_empty[2], s[2], p[2][2], o_full[2], o_empty[2], full[kStages], empty[kStages], drain;
+        uint64_t q_full[kQueries], q_empty[kQueries], s[2], p[2][2], o_full[2], o_empty[2], full[kStages], empty[kStages], drain;
         uint32_t tmem;
         volatile int abort;
     };
-    static constexpr size_t kSmem = (2 + kStages) * (size_t)kTileBytes + sizeof(Rest);
+    static constexpr size_t kSmem = (kQueries + kStages) * (size_t)kTileBytes + sizeof(Rest);
 };
 constexpr int kHalfBytes = kM * 128;
 
@@ -51,6 +52,7 @@ struct PromptParams {
     PagedAttn a;
     const int32_t *begin;  // [CTAs + 1] each CTA's pieces of a.item
     CUtensorMap q, k, v;
+    int wide;  // out's rows start at 32 bytes
     int *status;
 };
 
@@ -181,6 +183,11 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&v)[16]
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// 32 bytes at once (a whole sector of a row that the thread has to itself)
+__device__ __forceinline__ void store8(void *p, const uint32_t *w) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
 __device__ __forceinline__ f32x2 sum2(f32x2 a, f32x2 b) {
     f32x2 r;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
@@ -198,22 +205,25 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
     constexpr uint32_t kBf16 = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
     constexpr int kLoadWarp = kSoftmaxWarps, kMmaWarp = kSoftmaxWarps + 1;
     extern __shared__ __align__(1024) uint8_t smem[];
-    typename S::Rest &sh = *reinterpret_cast<typename S::Rest *>(smem + (2 + S::kStages) * S::kTileBytes);
+    typename S::Rest &sh = *reinterpret_cast<typename S::Rest *>(smem + (S::kQueries + S::kStages) * S::kTileBytes);
     pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = p.a.b.group, per_tile = kM / group;
-    const uint32_t sq = smem_addr(smem), skv = sq + 2 * S::kTileBytes;
+    const uint32_t sq = smem_addr(smem), skv = sq + S::kQueries * S::kTileBytes;
     const int first = p.begin[blockIdx.x], last = p.begin[blockIdx.x + 1];
 
     if (threadIdx.x == 0) {
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-            bar_init(&sh.q_full[t], 1);
-            bar_init(&sh.q_empty[t], 1);
             bar_init(&sh.s[t], 1);
             bar_init(&sh.p[t][0], 4);
             bar_init(&sh.p[t][1], 4);
             bar_init(&sh.o_full[t], 1);
             bar_init(&sh.o_empty[t], 4);
+        }
+#pragma unroll
+        for (int i = 0; i < S::kQueries; i++) {
+            bar_init(&sh.q_full[i], 1);
+            bar_init(&sh.q_empty[i], 1);
         }
 #pragma unroll
         for (int i = 0; i < S::kStages; i++) {
@@ -241,7 +251,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
             const int page = p.a.b.page, box = min(page, kN), shift = __ffs(page) - 1, boxes = kN / box;
             constexpr int kHalves = HD / 64;
             const int my_box = lane / kHalves, my_half = lane % kHalves;
-            int slot = 0, n_q[2] = {0, 0};
+            int slot = 0, n_q = 0;  // loads so far, tiles of Q so far
             bool ok = true;
             for (int n = first; n < last && ok; n++) {
                 const PagedItem it = p.a.item[n];
@@ -271,14 +281,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
 #pragma unroll
                         for (int t = 0; t < 2; t++) {  // (heads of a group and tokens come as the tile's rows; what lies behind the piece's tokens is not used)
                             if (!tl.n_blk[t]) continue;
-                            if (n_q[t]) ok = ok && bar_wait(&sh.q_empty[t], (n_q[t] - 1) & 1, &sh.abort);
+                            const int buf = n_q % S::kQueries, round = n_q / S::kQueries;
+                            if (round) ok = ok && bar_wait(&sh.q_empty[buf], (round - 1) & 1, &sh.abort);
                             ok = __all_sync(0xffffffffu, ok);
                             if (!ok) break;
-                            if (lane == 0) bar_expect(&sh.q_full[t], (uint32_t)(per_tile * group * HD * 2));
+                            if (lane == 0) bar_expect(&sh.q_full[buf], (uint32_t)(per_tile * group * HD * 2));
                             __syncwarp();
                             if (lane < kHalves)
-                                tma_tokens(sq + t * S::kTileBytes + lane * kHalfBytes, &p.q, lane * 64, it.head * group, it.token + t * per_tile, &sh.q_full[t]);
-                            n_q[t]++;
+                                tma_tokens(sq + buf * S::kTileBytes + lane * kHalfBytes, &p.q, lane * 64, it.head * group, it.token + t * per_tile, &sh.q_full[buf]);
+                            n_q++;
                         }
                     }
                     id = next;
@@ -287,8 +298,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
             if (sh.abort) {  // given up: what is on its way still lands before the block ends
                 volatile int none = 0;
                 for (int i = max(0, slot - S::kStages); i < slot; i++) bar_wait(&sh.full[i % S::kStages], (i / S::kStages) & 1, &none);
-                for (int t = 0; t < 2; t++)
-                    if (n_q[t]) bar_wait(&sh.q_full[t], (n_q[t] - 1) & 1, &none);
+                for (int i = max(0, n_q - S::kQueries); i < n_q; i++) bar_wait(&sh.q_full[i % S::kQueries], (i / S::kQueries) & 1, &none);
             }
         } else if (warp == kMmaWarp && elect_one()) {
             // ---- the products: one thread ----
@@ -302,17 +312,18 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                 fence_after();
                 return done;
             };
-            struct Place {  // in the ring
+            struct Place {  // in a ring
                 int stage = 0;
                 uint32_t phase = 0;
-                __device__ __forceinline__ void on(int n) {
+                __device__ __forceinline__ void on(int n, int of = S::kStages) {
                     stage += n;
-                    if (stage >= S::kStages) stage -= S::kStages, phase ^= 1;
+                    if (stage >= of) stage -= of, phase ^= 1;
                 }
             };
             const uint32_t q_desc = desc_low(sq, 16), k_desc = desc_low(skv, 16), v_desc = desc_low(skv, kHalfBytes);
+            int buf[2] = {0, 0};  // the tiles' Q
             auto scores = [&](int t, int stage) {
-                const uint32_t a = q_desc + t * (S::kTileBytes >> 4), b = k_desc + stage * (S::kTileBytes >> 4);
+                const uint32_t a = q_desc + buf[t] * (S::kTileBytes >> 4), b = k_desc + stage * (S::kTileBytes >> 4);
 #pragma unroll
                 for (int s = 0; s < HD / 16; s++) {
                     const uint32_t at = (s / 4) * (kHalfBytes >> 4) + (s % 4) * 2;
@@ -329,48 +340,69 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                 }
             };
             auto pieces = [&]() {  // false: a wait ran out
-                Place k, v;
+                Place k, v, q;
                 v.on(1);
-                uint32_t s_phase[2] = {0, 0}, q_phase[2] = {0, 0};
+                uint32_t s_phase[2] = {0, 0}, o_phase[2] = {0, 0};
                 bool read[2] = {false, false};  // O holds an earlier piece
-                for (int n = first; n < last; n++) {
+                // the first scores of a tile of a piece whose first K sits at `at`
+                auto begin = [&](int t, int blocks, const Place &at) {
+                    if (!wait(&sh.full[at.stage], at.phase) || !wait(&sh.q_full[q.stage], q.phase)) return false;
+                    buf[t] = q.stage;
+                    q.on(1, S::kQueries);
+                    scores(t, at.stage);
+                    if (blocks == 1) mma_commit(&sh.q_empty[buf[t]]);
+                    return true;
+                };
+                auto piece = [&](int n, int &blocks0, int &blocks1) {  // blocks of the tiles of piece n, 0 behind the last
+                    blocks0 = blocks1 = 0;
+                    if (n >= last) return;
                     const Tiles tl(p.a.item[n], per_tile);
-                    if (!tl.n_all) continue;
-                    if (!wait(&sh.full[k.stage], k.phase)) return false;
+                    blocks0 = tl.n_blk[0], blocks1 = tl.n_blk[1];
+                };
+                int blk[2], next[2];
+                piece(first, blk[0], blk[1]);
 #pragma unroll
-                    for (int t = 0; t < 2; t++) {
-                        if (!tl.n_blk[t]) continue;
-                        if (!wait(&sh.q_full[t], q_phase[t])) return false;
-                        scores(t, k.stage);
-                        if (tl.n_blk[t] == 1) mma_commit(&sh.q_empty[t]);
-                    }
-                    mma_commit(&sh.empty[k.stage]);
-                    for (int j = 0; j < tl.n_all; j++) {
+                for (int t = 0; t < 2; t++)
+                    if (blk[t] && !begin(t, blk[t], k)) return false;
+                if (blk[0] + blk[1]) mma_commit(&sh.empty[k.stage]);
+                for (int n = first; n < last; n++) {
+                    piece(n + 1, next[0], next[1]);
+                    const int n_all = max(blk[0], blk[1]);
+                    bool begun[2] = {false, false};
+                    for (int j = 0; j < n_all; j++) {
                         k.on(2);
-                        if (!wait(&sh.full[v.stage], v.phase) || (j + 1 < tl.n_all && !wait(&sh.full[k.stage], k.phase))) return false;
+                        if (!wait(&sh.full[v.stage], v.phase) || (j + 1 < n_all && !wait(&sh.full[k.stage], k.phase))) return false;
 #pragma unroll
                         for (int t = 0; t < 2; t++) {
-                            if (j >= tl.n_blk[t]) continue;
-                            if (!j && read[t] && !wait(&sh.o_empty[t], q_phase[t] ^ 1)) return false;
+                            if (j >= blk[t]) continue;
+                            if (!j && read[t] && !wait(&sh.o_empty[t], o_phase[t] ^ 1)) return false;
                             if (!wait(&sh.p[t][0], s_phase[t])) return false;
                             values(t, v.stage, 0, j > 0);
                             if (!wait(&sh.p[t][1], s_phase[t])) return false;
                             values(t, v.stage, 1, j > 0);
                             s_phase[t] ^= 1;
-                            if (j + 1 < tl.n_blk[t]) {
+                            if (j + 1 < blk[t]) {
                                 scores(t, k.stage);
-                                if (j + 2 == tl.n_blk[t]) mma_commit(&sh.q_empty[t]);
+                                if (j + 2 == blk[t]) mma_commit(&sh.q_empty[buf[t]]);
                             } else {
                                 mma_commit(&sh.o_full[t]);
+                                o_phase[t] ^= 1, read[t] = true;
+                                // straight on to the next piece (Q's tiles come in order): its softmax finds S when it has written O out
+                                if (next[t] && j + 1 == n_all && (t == 0 || !next[0] || begun[0])) {
+                                    if (!begin(t, next[t], k)) return false;
+                                    begun[t] = true;
+                                }
                             }
                         }
                         mma_commit(&sh.empty[v.stage]);
-                        if (j + 1 < tl.n_all) mma_commit(&sh.empty[k.stage]);
+                        if (j + 1 < n_all) mma_commit(&sh.empty[k.stage]);
                         v.on(2);
                     }
 #pragma unroll
                     for (int t = 0; t < 2; t++)
-                        if (tl.n_blk[t]) q_phase[t] ^= 1, read[t] = true;
+                        if (next[t] && !begun[t] && !begin(t, next[t], k)) return false;
+                    if (next[0] + next[1]) mma_commit(&sh.empty[k.stage]);
+                    blk[0] = next[0], blk[1] = next[1];
                 }
                 return true;
             };
@@ -482,7 +514,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
         const bool live = ok && r < rows;
         const int tok = t * per_tile + (live ? r / group : 0), g = live ? r % group : 0;
         const bool joined = it.part >= 0;
-        const size_t part_row = (size_t)it.part + (size_t)it.head * it.part_rows + it.part_off + (size_t)tok * group + g;
+        const size_t part_row = (size_t)it.part + (size_t)tok * group + g;
         const size_t out_at = (size_t)(it.token + tok) * p.a.out_stride + (size_t)(it.head * group + g) * HD;
         const float by = joined ? 1.0f : 1.0f / sum;
 #pragma unroll 1
@@ -506,8 +538,20 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
             if (!live) {
             } else if (joined || p.a.out_f32) {
                 float *dst = joined ? p.a.part_o + part_row * HD + c : reinterpret_cast<float *>(p.a.out) + out_at + c;
+                if (joined || p.wide) {
 #pragma unroll
-                for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4 *>(dst + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                    for (int i = 0; i < 32; i += 8) store8(dst + i, reinterpret_cast<const uint32_t *>(o + i));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4 *>(dst + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                }
+            } else if (p.wide) {
+                T *dst = reinterpret_cast<T *>(p.a.out) + out_at + c;
+                uint32_t w[16];
+#pragma unroll
+                for (int i = 0; i < 16; i++) w[i] = Half16<T>::pack(o[2 * i], o[2 * i + 1]);
+                store8(dst, w);
+                store8(dst + 16, w + 8);
             } else {
                 T *dst = reinterpret_cast<T *>(p.a.out) + out_at + c;
 #pragma unroll
@@ -587,6 +631,7 @@ void paged_prompt_launch(const PagedAttn &a, int type, int n_pages, const int32_
     PromptParams p;
     p.a = a;
     p.begin = begin;
+    p.wide = ((uintptr_t)a.out & 31) == 0 && a.out_stride * (a.out_f32 ? 4 : 2) % 32 == 0;
     p.status = g_status;
     if (!query_map(&p.q, a, type) || !pool_map(&p.k, a.k_pages, type, a.b, n_pages) || !pool_map(&p.v, a.v_pages, type, a.b, n_pages)) 
         return set_error_msg("paged_prompt: a tensor map was refused");
