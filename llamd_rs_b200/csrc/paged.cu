@@ -130,9 +130,10 @@ int decode_piece(long long positions, int n_head_kv, int sms) {
     return (int)std::max(128LL, (share + 15) / 16 * 16);
 }
 
-// paged_prompt.cu runs one CTA to an SM, each with a list of pieces. In blocks of its loop, a piece costs its blocks and about one more to begin
-// and end, leaving partial results one more again, and the launch that joins them about two.
-constexpr double kPieceCost = 1.0, kPartCost = 2.5, kJoinCost = 4.0;
+// paged_prompt.cu runs one CTA to an SM, each with a list of pieces. In blocks of its loop over two tiles, a block over one tile costs kHalfCost (its
+// softmax waits for its products), a piece kPieceCost to begin and end, leaving partial results kPartCost more, and the launch that joins
+// them kJoinCost (measured with pieces of 1 to 16 blocks, 1 to 4 to a CTA: 1.7 us a block at 64 elements, 2.0 at 128, 3 to 5 us a piece).
+constexpr double kHalfCost = 0.85, kPieceCost = 2.0, kPartCost = 2.0, kJoinCost = 4.0;
 
 struct Large {  // a tile of one kv head
     int tile, head, blocks;
@@ -141,23 +142,38 @@ struct Cut {  // blocks [first, first + n) of a Large, for a CTA
     int which, first, n, cta;
 };
 
-// Whole tiles, the longest of what is left to the CTA with the least so far. Returns when the last CTA ends; `large`: in falling order of blocks.
-double deal_whole(const std::vector<Large> &large, int ctas, std::vector<Cut> &cuts) {
+struct Dealer {
+    int ctas;
+    double block;  // what a block costs
+    double cost(const Large &x, int blocks) const { return block * blocks + kPieceCost + (blocks < x.blocks ? kPartCost : 0.0); }
+    double even(const std::vector<Large> &large, int per, std::vector<Cut> &cuts) const;
+    bool filled(const std::vector<Large> &large, double most, std::vector<Cut> &cuts) const;
+    double best(const std::vector<Large> &large, std::vector<Cut> &cuts) const;
+};
+
+// Tiles in even pieces of up to `per` blocks, the longest of what is left to the CTA with the least so far. Returns when the last CTA ends.
+double Dealer::even(const std::vector<Large> &large, int per, std::vector<Cut> &cuts) const {
+    cuts.clear();
+    for (size_t i = 0; i < large.size(); i++) {
+        const int n = (large[i].blocks + per - 1) / per, each = (large[i].blocks + n - 1) / n;
+        for (int b = 0; b < large[i].blocks; b += each) cuts.push_back({(int)i, b, std::min(each, large[i].blocks - b), 0});
+    }
+    std::stable_sort(cuts.begin(), cuts.end(), [](const Cut &a, const Cut &b) { return a.n > b.n; });
     std::vector<std::pair<double, int>> load(ctas);
     for (int i = 0; i < ctas; i++) load[i] = {0.0, i};
     double last = 0.0;
     const auto later = std::greater<std::pair<double, int>>();
-    for (size_t i = 0; i < large.size(); i++) {
+    for (Cut &c : cuts) {
         std::pop_heap(load.begin(), load.end(), later);
-        load.back().first += large[i].blocks + kPieceCost;
+        load.back().first += cost(large[c.which], c.n);
         last = std::max(last, load.back().first);
-        cuts.push_back({(int)i, 0, large[i].blocks, load.back().second});
+        c.cta = load.back().second;
         std::push_heap(load.begin(), load.end(), later);
     }
     return last;
 }
 // One tile after the other, each CTA filled up to `most` and the tile cut there. False where `most` is too little.
-bool deal_cut(const std::vector<Large> &large, int ctas, double most, std::vector<Cut> &cuts) {
+bool Dealer::filled(const std::vector<Large> &large, double most, std::vector<Cut> &cuts) const {
     cuts.clear();
     int cta = 0;
     double left = most;
@@ -165,18 +181,41 @@ bool deal_cut(const std::vector<Large> &large, int ctas, double most, std::vecto
         for (int first = 0; first < large[i].blocks;) {
             const int rest = large[i].blocks - first;
             int n = rest;
-            if (first || rest + kPieceCost > left) n = std::min(rest, (int)(left - kPieceCost - kPartCost));
+            if (first || cost(large[i], rest) > left) n = std::min(rest, (int)((left - kPieceCost - kPartCost) / block));
             if (n < std::min(rest, 2)) {  // (not a piece of one block at a CTA's end)
-                if (++cta >= ctas) return false;
+                if (++cta >= ctas || most < 2 * block + kPieceCost + kPartCost) return false;
                 left = most;
-                if (most < 2 + kPieceCost + kPartCost) return false;
                 continue;
             }
             cuts.push_back({(int)i, first, n, cta});
-            left -= n + kPieceCost + (n < large[i].blocks ? kPartCost : 0.0);
+            left -= cost(large[i], n);
             first += n;
         }
     return true;
+}
+// The cut and deal with which all is done soonest, and when. `large`: in falling order of blocks.
+double Dealer::best(const std::vector<Large> &large, std::vector<Cut> &cuts) const {
+    if (large.empty()) return 0.0;
+    std::vector<Cut> cut;
+    const int longest = large[0].blocks;
+    double ends = even(large, longest, cuts), total = 0.0;
+    for (int n = 2; n <= longest && (long long)large.size() * n <= 4LL * ctas; n++) {
+        const double e = even(large, (longest + n - 1) / n, cut) + kJoinCost;
+        if (e < ends) ends = e, cuts = cut;
+    }
+    for (const Large &x : large) total += block * x.blocks;
+    double low = total / ctas, high = ends - kJoinCost;
+    while (high - low > 0.02 * high) {
+        const double most = 0.5 * (low + high);
+        if (filled(large, most, cut)) {
+            cuts = cut;
+            high = most;
+            ends = most + kJoinCost;
+        } else {
+            low = most;
+        }
+    }
+    return ends;
 }
 
 void make_plan(Plan &plan, const PagedView &v, const int32_t *q_len, const int32_t *kv_len, int sms) {
@@ -186,33 +225,39 @@ void make_plan(Plan &plan, const PagedView &v, const int32_t *q_len, const int32
     if (shared) stretch.push_back({0, 0, v.n_shared, 0, v.tokens, v.n_shared, 0});
     for (int s = 0, t = 0; s < v.n_seq; t += q_len[s], s++)
         if (q_len[s]) stretch.push_back({s * v.table_stride, v.n_shared, kv_len[s], t, q_len[s], kv_len[s] - q_len[s] + 1, 1});
-    // a large piece is two tiles of query rows, but one where there are more SMs than such pieces
-    int tile_tokens = 2 * (kPagedTileRows / group);
-    long long pairs = 0;
-    for (const Stretch &st : stretch)
-        if (!st.small(group)) pairs += (st.n_tok + tile_tokens - 1) / tile_tokens;
-    if (2 * pairs * v.n_head_kv <= sms) tile_tokens /= 2;
-
     // some tokens of a stretch, and where they leave partial results, by kv head
     struct Tile {
         int stretch, token, n_tok, end;
         std::vector<std::vector<PagedPart>> parts;
     };
+    // the stretches' tiles in order; the large ones of `tile_tokens`
+    auto tiles_of = [&](int tile_tokens, std::vector<Tile> &tiles, std::vector<Large> &large) {
+        for (size_t i = 0; i < stretch.size(); i++) {
+            const Stretch &st = stretch[i];
+            const bool small = st.small(group);
+            const int most = small ? few_tokens : tile_tokens, n_tiles = (st.n_tok + most - 1) / most, per = small ? (st.n_tok + n_tiles - 1) / n_tiles : most;
+            for (int x = 0; x < st.n_tok; x += per) {
+                const int n = std::min(per, st.n_tok - x), end = std::min(st.end, st.limit + st.step * (x + n - 1));
+                tiles.push_back({(int)i, st.token + x, n, end, {}});
+                for (int h = 0; !small && h < v.n_head_kv; h++) large.push_back({(int)tiles.size() - 1, h, (end - st.begin + kPagedBlock - 1) / kPagedBlock});
+            }
+        }
+        std::stable_sort(large.begin(), large.end(), [](const Large &a, const Large &b) { return a.blocks > b.blocks; });
+    };
+    // a large piece is two tiles of query rows, or one where SMs would stand idle
     std::vector<Tile> tiles;
     std::vector<Large> large;
-    long long small_positions = 0;
-    for (size_t i = 0; i < stretch.size(); i++) {
-        const Stretch &st = stretch[i];
-        const bool small = st.small(group);
-        const int most = small ? few_tokens : tile_tokens, n_tiles = (st.n_tok + most - 1) / most, per = small ? (st.n_tok + n_tiles - 1) / n_tiles : most;
-        for (int x = 0; x < st.n_tok; x += per) {
-            const int n = std::min(per, st.n_tok - x), end = std::min(st.end, st.limit + st.step * (x + n - 1));
-            tiles.push_back({(int)i, st.token + x, n, end, std::vector<std::vector<PagedPart>>(v.n_head_kv)});
-            if (small) small_positions += end - st.begin;
-            else
-                for (int h = 0; h < v.n_head_kv; h++) large.push_back({(int)tiles.size() - 1, h, (end - st.begin + kPagedBlock - 1) / kPagedBlock});
-        }
+    std::vector<Cut> cuts;
+    tiles_of(2 * (kPagedTileRows / group), tiles, large);
+    const double ends = Dealer{sms, 1.0}.best(large, cuts);
+    if (!large.empty() && (int)large.size() < sms) {
+        std::vector<Tile> tiles1;
+        std::vector<Large> large1;
+        std::vector<Cut> cuts1;
+        tiles_of(kPagedTileRows / group, tiles1, large1);
+        if (Dealer{sms, kHalfCost}.best(large1, cuts1) < ends) tiles.swap(tiles1), large.swap(large1), cuts.swap(cuts1);
     }
+    for (Tile &tile : tiles) tile.parts.resize(v.n_head_kv);
     auto item_of = [&](const Tile &tile, int begin, int end) {
         const Stretch &st = stretch[tile.stretch];
         return PagedItem{st.table, begin, end, tile.token, tile.n_tok, st.limit + st.step * (tile.token - st.token), st.step, -1, 0, 0, {0, 0}};
@@ -225,6 +270,9 @@ void make_plan(Plan &plan, const PagedView &v, const int32_t *q_len, const int32
     };
 
     // the small ones: cut evenly, the kv heads alike
+    long long small_positions = 0;
+    for (const Tile &tile : tiles)
+        if (stretch[tile.stretch].small(group)) small_positions += tile.end - stretch[tile.stretch].begin;
     const int piece = decode_piece(small_positions, v.n_head_kv, sms);
     for (Tile &tile : tiles) {
         const Stretch &st = stretch[tile.stretch];
@@ -243,22 +291,7 @@ void make_plan(Plan &plan, const PagedView &v, const int32_t *q_len, const int32
     // (the longest first: what is left at the end is short)
     std::stable_sort(plan.small.begin(), plan.small.end(), [](const PagedItem &a, const PagedItem &b) { return a.kv_end - a.kv_begin > b.kv_end - b.kv_begin; });
 
-    // the large ones: whole, or cut where that ends sooner
-    std::stable_sort(large.begin(), large.end(), [](const Large &a, const Large &b) { return a.blocks > b.blocks; });
-    std::vector<Cut> cuts, cut;
-    const double whole = deal_whole(large, sms, cuts);
-    double total = 0.0;
-    for (const Large &x : large) total += x.blocks;
-    double low = std::max(total / sms, 2 + kPieceCost + kPartCost), high = whole - kJoinCost;
-    while (high - low > 0.02 * high) {
-        const double most = 0.5 * (low + high);
-        if (deal_cut(large, sms, most, cut)) {
-            cuts = cut;
-            high = most;
-        } else {
-            low = most;
-        }
-    }
+    // the large ones, by CTA
     int ctas = 0;
     for (const Cut &c : cuts) ctas = std::max(ctas, c.cta + 1);
     plan.begin.assign(ctas + 1, 0);
