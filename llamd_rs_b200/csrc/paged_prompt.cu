@@ -331,13 +331,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                 }
                 mma_commit(&sh.s[t]);
             };
-            auto values = [&](int t, int stage, int part, bool more) {  // over 64 positions of the block
+            auto values = [&](int t, int stage, int part, bool more) {  // over the block's first 96 positions, then its last 32: as the weights come
                 const uint32_t b = v_desc + stage * (S::kTileBytes >> 4);
 #pragma unroll
-                for (int i = 0; i < 4; i++) {  // 16 positions: 8 columns of P, 16 rows of V
-                    const int step = part * 4 + i;
+                for (int step = part ? 6 : 0; step < (part ? 8 : 6); step++)  // 16 positions: 8 columns of P, 16 rows of V
                     mma_ts(tmem + 2 * kN + t * HD, tmem + t * kN + step * 8, b + step * (16 * 128 >> 4), kO, more || step > 0);
-                }
             };
             auto pieces = [&]() {  // false: a wait ran out
                 Place k, v, q;
@@ -427,6 +425,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
         float m = -INFINITY, sum = 0.0f;
         // positions of the piece that this row sees
         const int mine = min(it.kv_end, it.limit + it.step * (t * per_tile + min(r, rows - 1) / group)) - it.kv_begin;
+        const int clear = (int)(__reduce_min_sync(0xffffffffu, (unsigned)max(mine, 0)) / kN);  // blocks that all rows of the warp see whole
         for (int j = 0; j < n_blk; j++, n_s++) {
             ok = ok && bar_wait(&sh.s[t], n_s & 1, &sh.abort);
             ok = __all_sync(0xffffffffu, ok);
@@ -437,8 +436,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
             tmem_wait_ld();
 #pragma unroll
             for (int c = 0; c < kN; c += 32) tmem_loaded(s, c);
-            const int seen = mine - j * kN;
-            if (__any_sync(0xffffffffu, seen < kN)) {
+            if (j >= clear) {
+                const int seen = mine - j * kN;
 #pragma unroll
                 for (int c = 0; c < kN; c++) s[c] = c < seen ? s[c] : -INFINITY;
             }
@@ -448,13 +447,38 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
 #pragma unroll
                 for (int x = 0; x < 4; x++) top[x] = c + 4 + x < kN ? fmaxf(fmaxf(top[x], s[c + x]), s[c + 4 + x]) : fmaxf(top[x], s[c + x]);
             const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+            if (!j) m = high;
+            const f32x2 scale2 = pack2(scale, scale);
+            f32x2 from2, part[2];
+            auto start = [&]() {
+                const float from = m == -INFINITY ? 0.0f : -m * scale;
+                from2 = pack2(from, from);
+                part[0] = part[1] = 0;
+            };
+            auto weights = [&](int q) {  // of 32 positions, to TMEM over S's first columns
+                uint32_t w[16];
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const float2 x = unpack2(fma2(pack2(s[q * 32 + 2 * i], s[q * 32 + 2 * i + 1]), scale2, from2));
+                    const float2 y = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+                    part[i & 1] = sum2(part[i & 1], pack2(y.x, y.y));
+                    // rounded to the cache's type for the second product: relative 2^-12 (f16) or 2^-9 (bf16), as the output itself will be
+                    w[i] = Half16<T>::pack(y.x, y.y);
+                }
+                tmem_st16(ts + q * 16, w);
+            };
+            // P in two parts, so that the second product begins while the rest of the weights are made; the first with the m of the blocks so far,
+            // beside the new maximum rather than behind it, and again where that was too low
+            start();
+#pragma unroll
+            for (int q = 0; q < 3; q++) weights(q);
             // has a row's maximum grown by more than 2^8? (never where it has seen nothing: -inf - -inf)
             const bool grew = (high - m) * scale > 8.0f;
             if (__any_sync(0xffffffffu, grew)) {
                 const float by = grew ? exp2_fast((m - high) * scale) : 1.0f;
                 m = grew ? high : m;
                 sum *= by;
-                if (j && ok) {  // the products of the blocks so far are done: S's commit follows them
+                if (ok) {  // the products of the blocks so far are done: S's commit follows them
 #pragma unroll 1
                     for (int c = 0; c < HD; c += 16) {
                         float o[16];
@@ -466,6 +490,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                         tmem_st16(to + c, reinterpret_cast<const uint32_t(&)[16]>(o));
                     }
                 }
+                start();
+#pragma unroll
+                for (int q = 0; q < 3; q++) weights(q);
             }
             const int valid = it.kv_end - it.kv_begin - j * kN;
             if (valid < kN) {  // the last block: zeros in V's rows behind the last position (both tiles write the same zeros)
@@ -479,29 +506,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                 fence_async();
                 __syncwarp();
             }
-            const float from = m == -INFINITY ? 0.0f : -m * scale;
-            const f32x2 scale2 = pack2(scale, scale), from2 = pack2(from, from);
-            f32x2 part[2] = {0, 0};
-            // P over S's first columns, in two parts, so that the second product begins while the rest of the weights are made
-#pragma unroll
-            for (int q = 0; q < 4; q++) {
-                uint32_t w[16];
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const float2 x = unpack2(fma2(pack2(s[q * 32 + 2 * i], s[q * 32 + 2 * i + 1]), scale2, from2));
-                    const float2 y = make_float2(exp2_fast(x.x), exp2_fast(x.y));
-                    part[i & 1] = sum2(part[i & 1], pack2(y.x, y.y));
-                    // rounded to the cache's type for the second product: relative 2^-12 (f16) or 2^-9 (bf16), as the output itself will be
-                    w[i] = Half16<T>::pack(y.x, y.y);
-                }
-                tmem_st16(ts + q * 16, w);
-                if (q & 1) {
-                    tmem_wait_st();
-                    fence_before();
-                    __syncwarp();
-                    if (lane == 0) bar_arrive(&sh.p[t][q >> 1]);
-                }
-            }
+            tmem_wait_st();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) bar_arrive(&sh.p[t][0]);
+            weights(3);
+            tmem_wait_st();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) bar_arrive(&sh.p[t][1]);
             const float2 total = unpack2(sum2(part[0], part[1]));
             sum += total.x + total.y;
         }
