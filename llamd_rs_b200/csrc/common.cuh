@@ -65,12 +65,12 @@ enum { PDL_MATVEC = 1, PDL_GROUPED = 2, PDL_ROUTER = 4, PDL_OTHER = 8, PDL_NORM 
 constexpr int kPdlDefault = PDL_MATVEC | PDL_GROUPED | PDL_ROUTER | PDL_PAGED;  // measured best
 
 template <typename... KArgs, typename... Args>
-inline void launch_kc(int cls, const char *what, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, Args... args) {
+inline void launch_on(cudaStream_t to, int cls, const char *what, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, Args... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
     cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream();
+    cfg.stream = to;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -79,6 +79,10 @@ inline void launch_kc(int cls, const char *what, void (*kernel)(KArgs...), dim3 
     g_launches++;
     cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
     if (e != cudaSuccess) set_error(e, what);
+}
+template <typename... KArgs, typename... Args>
+inline void launch_kc(int cls, const char *what, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, Args... args) {
+    launch_on(stream(), cls, what, kernel, grid, block, smem, args...);
 }
 template <typename... KArgs, typename... Args>
 inline void launch_k(const char *what, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, Args... args) {

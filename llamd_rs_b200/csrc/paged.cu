@@ -20,6 +20,16 @@ int refuse(const char *why) {
     return -1;
 }
 
+// A second stream for what runs beside the library's own, and the events that order the two; made when a batch first needs them.
+cudaStream_t g_side = nullptr;
+cudaEvent_t g_fork = nullptr, g_join = nullptr;
+bool side_ready() {
+    if (!g_side && cudaStreamCreateWithFlags(&g_side, cudaStreamNonBlocking) != cudaSuccess) g_side = nullptr;
+    if (!g_fork && cudaEventCreateWithFlags(&g_fork, cudaEventDisableTiming) != cudaSuccess) g_fork = nullptr;
+    if (!g_join && cudaEventCreateWithFlags(&g_join, cudaEventDisableTiming) != cudaSuccess) g_join = nullptr;
+    return g_side && g_fork && g_join;
+}
+
 struct Batch {
     PagedView view = {};
     int type = 0, n_pages = 0, max_kv = 0, sms = 0;
@@ -33,6 +43,7 @@ struct Batch {
     const PagedMerge *merge = nullptr;
     const PagedPart *part = nullptr;
     const int32_t *begin = nullptr;  // large: each CTA's
+    bool beside = false;
     int n_small = 0, small_rows = 0, n_ctas = 0, n_merge = 0, most = 0;
     uint8_t *partial = nullptr;
     size_t partial_bytes = 0, partial_rows = 0;
@@ -112,6 +123,7 @@ struct Plan {
     std::vector<int32_t> begin;  // large: each CTA's
     std::vector<PagedMerge> merge;
     std::vector<PagedPart> part;
+    bool beside = false;  // small and large pieces at the same time, each on SMs of its own
     int small_rows = 0, most = 0;  // rows of a small piece, parts of a token and head
     size_t rows = 0;  // of partial results
 };
@@ -134,6 +146,11 @@ int decode_piece(long long positions, int n_head_kv, int sms) {
 // softmax waits for its products), a piece kPieceCost to begin and end, leaving partial results kPartCost more, and the launch that joins
 // them kJoinCost (measured with pieces of 1 to 16 blocks, 1 to 4 to a CTA: 1.7 us a block at 64 elements, 2.0 at 128, 3 to 5 us a piece).
 constexpr double kHalfCost = 0.85, kPieceCost = 2.0, kPartCost = 2.0, kJoinCost = 4.0;
+
+// Small and large pieces of one batch, one launch after the other, leave first HBM and then the tensor cores waiting; at the same time, each on SMs of its
+// own, neither. What they take, in SM-microseconds: an SM draws about 65 GB/s from HBM where all do not draw at once, a block of two tiles
+// takes 2 us. Each has to be worth more than a launch (kBesideLeast us on all SMs).
+constexpr double kSmBytes = 65e3, kBlockMicros = 2.0, kBesideLeast = 6.0;
 
 struct Large {  // a tile of one kv head
     int tile, head, blocks;
@@ -249,13 +266,25 @@ void make_plan(Plan &plan, const PagedView &v, const int32_t *q_len, const int32
     std::vector<Large> large;
     std::vector<Cut> cuts;
     tiles_of(2 * (kPagedTileRows / group), tiles, large);
-    const double ends = Dealer{sms, 1.0}.best(large, cuts);
-    if (!large.empty() && (int)large.size() < sms) {
+    long long small_positions = 0;
+    for (const Tile &tile : tiles)
+        if (stretch[tile.stretch].small(group)) small_positions += tile.end - stretch[tile.stretch].begin;
+    int small_sms = sms, large_sms = sms;
+    double blocks = 0.0;
+    for (const Large &x : large) blocks += x.blocks + kPieceCost;
+    const double small_work = (double)small_positions * v.n_head_kv * v.hd * 4 / kSmBytes, large_work = blocks * kBlockMicros;
+    if (small_work > kBesideLeast * sms && large_work > kBesideLeast * sms) {
+        plan.beside = true;
+        large_sms = std::min(sms - 8, std::max(8, (int)(sms * large_work / (small_work + large_work))));
+        small_sms = sms - large_sms;
+    }
+    const double ends = Dealer{large_sms, 1.0}.best(large, cuts);
+    if (!large.empty() && (int)large.size() < large_sms) {
         std::vector<Tile> tiles1;
         std::vector<Large> large1;
         std::vector<Cut> cuts1;
         tiles_of(kPagedTileRows / group, tiles1, large1);
-        if (Dealer{sms, kHalfCost}.best(large1, cuts1) < ends) tiles.swap(tiles1), large.swap(large1), cuts.swap(cuts1);
+        if (Dealer{large_sms, kHalfCost}.best(large1, cuts1) < ends) tiles.swap(tiles1), large.swap(large1), cuts.swap(cuts1);
     }
     for (Tile &tile : tiles) tile.parts.resize(v.n_head_kv);
     auto item_of = [&](const Tile &tile, int begin, int end) {
@@ -270,10 +299,7 @@ void make_plan(Plan &plan, const PagedView &v, const int32_t *q_len, const int32
     };
 
     // the small ones: cut evenly, the kv heads alike
-    long long small_positions = 0;
-    for (const Tile &tile : tiles)
-        if (stretch[tile.stretch].small(group)) small_positions += tile.end - stretch[tile.stretch].begin;
-    const int piece = decode_piece(small_positions, v.n_head_kv, sms);
+    const int piece = decode_piece(small_positions, v.n_head_kv, small_sms);
     for (Tile &tile : tiles) {
         const Stretch &st = stretch[tile.stretch];
         if (!st.small(group)) continue;
@@ -528,6 +554,10 @@ int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int
                  o_table = section<int32_t>(bytes, (size_t)n_seq * v.table_stride), o_small = section<PagedItem>(bytes, plan.small.size()),
                  o_large = section<PagedItem>(bytes, plan.large.size()), o_begin = section<int32_t>(bytes, plan.begin.size()),
                  o_merge = section<PagedMerge>(bytes, plan.merge.size()), o_part = section<PagedPart>(bytes, plan.part.size());
+    if (plan.beside && !side_ready()) {
+        set_error(cudaGetLastError(), "paged batch: side stream");
+        return -1;
+    }
     b->ready = false;  // (from here on what the batch held is being replaced)
     if (!b->reserve(std::max<size_t>(bytes, 16), plan.rows)) return -1;
     auto put = [&](size_t at, const void *from, size_t n) {
@@ -554,6 +584,7 @@ int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int
     b->begin = (const int32_t *)(b->dev + o_begin);
     b->merge = (const PagedMerge *)(b->dev + o_merge);
     b->part = (const PagedPart *)(b->dev + o_part);
+    b->beside = plan.beside;
     b->n_small = (int)plan.small.size(), b->small_rows = plan.small_rows, b->n_ctas = (int)plan.begin.size() - 1, b->n_merge = (int)plan.merge.size(), b->most = plan.most;
     b->partial_rows = plan.rows;
     b->n_pages = n_pages, b->max_kv = max_kv;
@@ -616,13 +647,19 @@ int llamd_fwd_paged_attention(const void *batch, const void *q, size_t q_stride,
     a.b = g, a.q = q, a.k_pages = k_pages, a.v_pages = v_pages, a.out = out, a.q_stride = q_stride, a.out_stride = out_stride;
     a.out_f32 = out_f32, a.scale_log2 = scale * 1.4426950408889634f;
     a.part_o = (float *)b->partial, a.part_ml = (float2 *)(b->partial + b->partial_rows * g.hd * sizeof(float));
-    if (b->n_ctas) {
+    if (b->beside) LLAMD_TRY(cudaEventRecord(g_fork, stream()), "paged attention: fork");
+    if (b->n_ctas) {  // (first: its CTAs need whole SMs)
         a.item = b->large;
         paged_prompt_launch(a, b->type, b->n_pages, b->begin, b->n_ctas);
     }
     if (b->n_small) {
         a.item = b->small;
-        paged_decode_launch(a, b->type, b->n_small, b->small_rows);
+        if (b->beside) LLAMD_TRY(cudaStreamWaitEvent(g_side, g_fork, 0), "paged attention: fork");
+        paged_decode_launch(a, b->type, b->n_small, b->small_rows, b->beside ? g_side : stream());
+    }
+    if (b->beside) {
+        LLAMD_TRY(cudaEventRecord(g_join, g_side), "paged attention: join");
+        LLAMD_TRY(cudaStreamWaitEvent(stream(), g_join, 0), "paged attention: join");
     }
     if (b->n_merge) paged_merge_launch(a, b->type, b->merge, b->part, b->n_merge, b->most, b->sms);
     return error_code() ? -1 : 0;

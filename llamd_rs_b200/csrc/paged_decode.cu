@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttn p, con
 }
 
 template <typename T, int HD, int NT>
-void launch_nt(const PagedAttn &p, int n_items) {
+void launch_nt(const PagedAttn &p, int n_items, cudaStream_t to) {
     constexpr size_t smem = decode_smem<HD, NT>();
     static bool ready = false;
     if (!ready) {
@@ -336,20 +336,20 @@ void launch_nt(const PagedAttn &p, int n_items) {
         if (e != cudaSuccess) return set_error(e, "paged_decode shared memory");
         ready = true;
     }
-    launch_kc(PDL_PAGED, "paged_decode", paged_decode_kernel<T, HD, NT>, dim3(n_items, p.b.n_head_kv), dim3(kWarps * 32), smem, p);
+    launch_on(to, PDL_PAGED, "paged_decode", paged_decode_kernel<T, HD, NT>, dim3(n_items, p.b.n_head_kv), dim3(kWarps * 32), smem, p);
 }
 template <typename T, int HD>
-void launch_hd(const PagedAttn &p, int n_items, int max_rows) {
-    if (max_rows <= 8) launch_nt<T, HD, 1>(p, n_items);
-    else if (max_rows <= 16) launch_nt<T, HD, 2>(p, n_items);
-    else launch_nt<T, HD, 4>(p, n_items);
+void launch_hd(const PagedAttn &p, int n_items, int max_rows, cudaStream_t to) {
+    if (max_rows <= 8) launch_nt<T, HD, 1>(p, n_items, to);
+    else if (max_rows <= 16) launch_nt<T, HD, 2>(p, n_items, to);
+    else launch_nt<T, HD, 4>(p, n_items, to);
 }
 
 }  // namespace
 
-void paged_decode_launch(const PagedAttn &p, int type, int n_items, int max_rows) {
-    if (type == kPagedF16) p.b.hd == 128 ? launch_hd<__half, 128>(p, n_items, max_rows) : launch_hd<__half, 64>(p, n_items, max_rows);
-    else p.b.hd == 128 ? launch_hd<__nv_bfloat16, 128>(p, n_items, max_rows) : launch_hd<__nv_bfloat16, 64>(p, n_items, max_rows);
+void paged_decode_launch(const PagedAttn &p, int type, int n_items, int max_rows, cudaStream_t to) {
+    if (type == kPagedF16) p.b.hd == 128 ? launch_hd<__half, 128>(p, n_items, max_rows, to) : launch_hd<__half, 64>(p, n_items, max_rows, to);
+    else p.b.hd == 128 ? launch_hd<__nv_bfloat16, 128>(p, n_items, max_rows, to) : launch_hd<__nv_bfloat16, 64>(p, n_items, max_rows, to);
 }
 
 template <typename T, int HD>

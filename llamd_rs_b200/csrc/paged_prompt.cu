@@ -436,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
             tmem_wait_ld();
 #pragma unroll
             for (int c = 0; c < kN; c += 32) tmem_loaded(s, c);
-            if (j >= clear) {
+            if (__builtin_expect(j >= clear, 0)) {
                 const int seen = mine - j * kN;
 #pragma unroll
                 for (int c = 0; c < kN; c++) s[c] = c < seen ? s[c] : -INFINITY;
@@ -474,7 +474,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
             for (int q = 0; q < 3; q++) weights(q);
             // has a row's maximum grown by more than 2^8? (never where it has seen nothing: -inf - -inf)
             const bool grew = (high - m) * scale > 8.0f;
-            if (__any_sync(0xffffffffu, grew)) {
+            if (__builtin_expect(__any_sync(0xffffffffu, grew), 0)) {
                 const float by = grew ? exp2_fast((m - high) * scale) : 1.0f;
                 m = grew ? high : m;
                 sum *= by;
@@ -495,7 +495,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                 for (int q = 0; q < 3; q++) weights(q);
             }
             const int valid = it.kv_end - it.kv_begin - j * kN;
-            if (valid < kN) {  // the last block: zeros in V's rows behind the last position (both tiles write the same zeros)
+            if (__builtin_expect(valid < kN, 0)) {  // the last block: zeros in V's rows behind the last position (both tiles write the same zeros)
                 const int slot = base + 2 * j + 1, stage = slot % S::kStages;
                 ok = ok && bar_wait(&sh.full[stage], (slot / S::kStages) & 1, &sh.abort);
                 for (int x = valid * (HD / 8) + r; x < kN * (HD / 8); x += 128) {
