@@ -449,8 +449,9 @@ void llamd_cuda_paged_free(void *batch);
 /* pages: [n_seq][pages_stride], ids below n_pages (the pools' size), of each sequence the first
  * ceil(kv_len / page_size) are read. q_len may be 0. n_shared: the first n_shared positions (whole pages, the same ids in every
  * table) are common to all sequences, no sequence has new tokens among them, and attention reads them once for all. Everything is
- * checked here, before a launch can use it: 0, or -1 and a message, and the batch is as it was. Enqueues one copy; may allocate where
- * a batch is larger than any before it; not while a graph is captured. A batch that is set again serves the launches enqueued
+ * checked here, before a launch can use it: 0, or -1 and a message, and the batch is as it was (where memory could not be had: not
+ * set). Enqueues one copy; may allocate where a batch is larger than any before it; not while a graph is captured, but what it has set may
+ * be used in one. A batch that is set again serves the launches enqueued
  * after the call. */
 int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int32_t *kv_len, const int32_t *pages, int pages_stride,
                          int n_pages, int n_shared);
@@ -465,7 +466,7 @@ int llamd_fwd_paged_append(const void *batch, const void *q, const void *k, cons
                            int rope_rows, int rot, int interleaved, void *q_out, size_t out_stride, void *k_pages, void *v_pages);
 /* out[token][head] = softmax(scale * q . k) v over the positions up to the token's own; scale > 0. q and out in the batch's type, or out in f32
  * (out_f32: the same sums, not rounded); rows start at 16 bytes. Slots behind a sequence's last position may hold
- * anything, NaN and infinities too. 0 / -1 as above. */
+ * anything, NaN and infinities too. Part of a large batch may run on a second stream of the library's, which the call joins to its own. 0 / -1 as above. */
 int llamd_fwd_paged_attention(const void *batch, const void *q, size_t q_stride, const void *k_pages, const void *v_pages, void *out,
                               size_t out_stride, int out_f32, float scale);
 /* 0 while every wait inside the attention's kernels has been met; otherwise 1 + the first piece whose wait ran out (outputs are

@@ -103,6 +103,7 @@ const char *check_lengths(const Batch &b, int n_seq, const int32_t *q_len, const
     long long tokens = 0;
     for (int s = 0; s < n_seq; s++) {
         if (q_len[s] < 0 || kv_len[s] < q_len[s]) return "paged batch: a sequence has fewer positions than new tokens";
+        if (kv_len[s] > 1 << 30) return "paged batch: a sequence of more than 2^30 positions";
         if (kv_len[s] - q_len[s] < n_shared) return "paged batch: new tokens inside the shared prefix";
         const long long used = ((long long)kv_len[s] + page - 1) / page;
         if (used > pages_stride) return "paged batch: a table has fewer pages than its sequence";
@@ -509,7 +510,7 @@ void *llamd_cuda_paged_new(int n_head, int n_head_kv, int hd, int page_size, int
         set_error_msg("paged batch: heads of 64 or 128 elements, up to 64 query heads to a kv head, pages of 16 to 4096 positions (a power of two), f16 or bf16");
         return nullptr;
     }
-    if (!stream()) return nullptr;
+    if (!stream() || !paged_prompt_ready()) return nullptr;
     Batch *b = new (std::nothrow) Batch;
     if (!b) {
         set_error_msg("paged batch: out of host memory");

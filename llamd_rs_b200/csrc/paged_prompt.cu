@@ -80,14 +80,20 @@ __device__ __forceinline__ void bar_arrive(uint64_t *bar) {
 __device__ __forceinline__ void bar_expect(uint64_t *bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ unsigned long long nanoseconds() {
+    unsigned long long t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
 __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {  // (parks in hardware for a while where the phase is not over)
     uint32_t done;
     asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
     return done;
 }
-// Gives up after 2^20 tries (a second and more), or as soon as another warp has.
+// Gives up after two seconds, or as soon as another warp has.
 __device__ __forceinline__ bool bar_wait_on(uint32_t bar, uint32_t parity, volatile int *abort) {
-    for (int i = 0; i < (1 << 20); i++) {
+    const unsigned long long began = nanoseconds();
+    while (nanoseconds() - began < 2000000000ull) {
         if (bar_try(bar, parity)) return true;
         if (*abort) return false;
     }
@@ -586,7 +592,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
     if (threadIdx.x == 0 && sh.abort) atomicCAS(p.status, 0, 1 + (int)blockIdx.x);
 }
 
-int *g_status = nullptr;  // device word, made on first use
+int *g_status = nullptr;  // device word, made with the first batch
 
 typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
                                 const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -634,13 +640,19 @@ void prompt_launch(const PromptParams &p, int n_ctas) {
 
 }  // namespace
 
-void paged_prompt_launch(const PagedAttn &a, int type, int n_pages, const int32_t *begin, int n_ctas) {
+bool paged_prompt_ready() {
     if (!g_status) {
         int *p = nullptr;
-        if (cudaMalloc(&p, sizeof(int)) != cudaSuccess || cudaMemsetAsync(p, 0, sizeof(int), stream()) != cudaSuccess)
-            return set_error(cudaGetLastError(), "paged_prompt status word");
+        if (cudaMalloc(&p, sizeof(int)) != cudaSuccess || cudaMemsetAsync(p, 0, sizeof(int), stream()) != cudaSuccess) {
+            set_error(cudaGetLastError(), "paged_prompt status word");
+            return false;
+        }
         g_status = p;
     }
+    return true;
+}
+
+void paged_prompt_launch(const PagedAttn &a, int type, int n_pages, const int32_t *begin, int n_ctas) {
     PromptParams p;
     p.a = a;
     p.begin = begin;

@@ -133,6 +133,19 @@ class Batch:
         self.tokens, self.n_pages = int(q.sum()), n_pages
         self._pool = n_pages * self.n_head_kv * self.page_size * self.head_dim
 
+    @staticmethod
+    def _tensors(*wanted):
+        """The addresses of (tensor, type, values at least, rows) that are all as plain as can be, or None: then each is looked at for itself."""
+        found = []
+        try:
+            for x, type_, n, rows in wanted:
+                if _seen.get(x.dtype) != type_ or not x.is_cuda or not x.is_contiguous() or x.numel() < n or (rows is not None and (x.shape[0] != rows or x.numel() != n)):
+                    return None
+                found.append(x.data_ptr())
+        except (AttributeError, IndexError):
+            return None
+        return found
+
     def _rows(self, x, n, type_, what, stride=None):
         """(address, elements between tokens) of `tokens` rows of n elements."""
         try:
@@ -190,8 +203,16 @@ class Batch:
                 rope_rows = rope.nbytes // (4 * rot)
             else:
                 raise Malformed("rope_rows: how many positions the table has")
-        D = self.head_dim
+        D, T, t = self.head_dim, self.tokens, self.type
         nq, nk = self.n_head * D, self.n_head_kv * D
+        if rot and q_norm is not None and k_norm is not None:
+            plain = self._tensors((q, it, T * nq, T), (k, it, T * nk, T), (v, it, T * nk, T), (q_norm, 2, D, None), (k_norm, 2, D, None),
+                                  (rope, 2, rope_rows * rot, None), (q_out, t, T * nq, T), (k_pages, t, self._pool, None), (v_pages, t, self._pool, None))
+            if plain:
+                if self._append(self.ptr, plain[0], plain[1], plain[2], it, nq, nk, nk, plain[3], plain[4], eps, plain[5], rope_rows, rot, interleaved, plain[6],
+                                nq, plain[7], plain[8]) != 0:
+                    _refuse("append")
+                return
         qp, qs = self._rows(q, nq, it, "q", strides[0])
         kp, ks = self._rows(k, nk, it, "k", strides[1])
         vp, vs = self._rows(v, nk, it, "v", strides[2])
@@ -207,10 +228,17 @@ class Batch:
         if out_f32 is None:
             out_f32 = hasattr(out, "data_ptr") and _type_of(out) == 2
         n = self.n_head * self.head_dim
+        scale = self.scale if scale is None else scale
+        plain = self._tensors((q, self.type, self.tokens * n, self.tokens), (k_pages, self.type, self._pool, None), (v_pages, self.type, self._pool, None),
+                              (out, 2 if out_f32 else self.type, self.tokens * n, self.tokens))
+        if plain:
+            if self._attention(self.ptr, plain[0], n, plain[1], plain[2], plain[3], n, out_f32, scale) != 0:
+                _refuse("attention")
+            return
         qp, qs = self._rows(q, n, self.type, "q")
         op, os_ = self._rows(out, n, 2 if out_f32 else self.type, "out")
         if self._attention(self.ptr, qp, qs, self._whole(k_pages, self.type, self._pool, "k_pages"), self._whole(v_pages, self.type, self._pool, "v_pages"), op, os_,
-                           out_f32, self.scale if scale is None else scale) != 0:
+                           out_f32, scale) != 0:
             _refuse("attention")
 
     def free(self) -> None:

@@ -100,7 +100,14 @@ def test_append(paged, H, K, D, page, dtype, inputs, q_len, kv_len, rot, interle
         assert np.array_equal(g, w)
 
 
-def run_attention(paged, H, K, D, page, dtype, q_len, kv_len, n_shared=0, scale=None, out_f32=False, q_scale=1.0, poison=True, seed=0, edit=None):
+def lib():
+    from llamd_rs_b200._lib import lib as load
+
+    return load()
+
+
+def run_attention(paged, H, K, D, page, dtype, q_len, kv_len, n_shared=0, scale=None, out_f32=False, q_scale=1.0, poison=True, seed=0, edit=None,
+                  repeat=1, pad=0, shift=0):
     rng = np.random.default_rng(seed + H * 100 + D + sum(kv_len))
     tables, n_pages = scatter_tables(rng, kv_len, page, n_shared)
     b = paged.Batch(H, K, D, page, dtype)
@@ -119,15 +126,28 @@ def run_attention(paged, H, K, D, page, dtype, q_len, kv_len, n_shared=0, scale=
         dead = np.broadcast_to(~live[:, None, :, None], kp.shape)
         kp[dead], vp[dead] = nan, nan
         vp[..., ::2][dead[..., ::2]] = inf
-    out = dev(np.full((T, H, D), 0xFFFFFFFF if out_f32 else 0xFFFF, np.uint32 if out_f32 else np.uint16))
-    b.attention(dev(q), dev(kp), dev(vp), out, scale=scale, out_f32=out_f32)
     from llamd_rs_b200 import backend
 
+    wide, n = np.uint32 if out_f32 else np.uint16, H * D + pad
+    rows = np.full((T, n), 0x7FFF, np.uint16)
+    rows[:, :H * D] = q.reshape(T, H * D)
+    rows = dev(np.concatenate([np.full(shift, 0x7FFF, np.uint16), rows.ravel()]))
+    out = dev(np.full(shift + T * n, np.iinfo(wide).max, wide))
+    dk, dv = dev(kp), dev(vp)
+    for _ in range(repeat):
+        if pad or shift:
+            assert lib().llamd_fwd_paged_attention(b.ptr, rows.ptr + 2 * shift, n, dk.ptr, dv.ptr, out.ptr + wide().itemsize * shift, n, int(out_f32),
+                                                   D ** -0.5 if scale is None else scale) == 0
+        else:
+            b.attention(rows, dk, dv, out, scale=scale, out_f32=out_f32)
     backend.sync()
-    if out_f32:
-        got = out.download(np.float32, T * H * D).astype(np.float64).reshape(T, H, D)
-    else:
-        got = plain.from_bits(out.download(np.uint16, T * H * D), dtype).reshape(T, H, D)
+    assert paged.status() == 0
+    got = out.download(wide, shift + T * n)
+    assert np.all(got[:shift] == np.iinfo(wide).max)
+    got = got[shift:].reshape(T, n)
+    assert np.all(got[:, H * D:] == np.iinfo(wide).max)  # nothing between the rows is written
+    got = np.ascontiguousarray(got[:, :H * D])
+    got = (got.view(np.float32).astype(np.float64) if out_f32 else plain.from_bits(got, dtype)).reshape(T, H, D)
     want, bound = plain.attention(plain.from_bits(q, dtype), plain.from_bits(kp, dtype), plain.from_bits(vp, dtype), tables, q_len, kv_len,
                                   D ** -0.5 if scale is None else scale, dtype)
     return got, want, bound
@@ -196,6 +216,60 @@ def test_attention_sharp_and_flat(paged, dtype, q_len, kv_len):
     close(*run_attention(paged, 8, 1, 128, 16, dtype, q_len, kv_len, q_scale=0.0))
     close(*run_attention(paged, 8, 1, 128, 16, dtype, q_len, kv_len, scale=0.5))
     close(*run_attention(paged, 8, 1, 128, 16, dtype, q_len, kv_len, out_f32=True))
+
+
+def test_attention_beside(paged):
+    """A batch large enough that the prefix and the sequences' own positions are read at the same time; twice, the second over the first's results."""
+    rng = np.random.default_rng(3)
+    own = [int(x) for x in rng.integers(380, 520, 64)]
+    args = (paged, 32, 4, 128, 64, "bf16", [1] * 64, [7552 + m for m in own], 7552)
+    close(*run_attention(*args, repeat=3))
+
+
+@pytest.mark.parametrize("q_len,kv_len,n_shared", [([1, 2], [300, 90], 0), ([1] * 6, [100 + i for i in range(6)], 96), ([90, 60], [200, 60], 0)])
+def test_attention_rows_apart(paged, q_len, kv_len, n_shared):
+    """Rows of q and out further apart than their values, and starting at 16 bytes but not at 32."""
+    for pad, shift in ((8, 0), (24, 8), (0, 8)):
+        close(*run_attention(paged, 8, 2, 64, 16, "f16", q_len, kv_len, n_shared, pad=pad, shift=shift))
+    close(*run_attention(paged, 8, 2, 64, 16, "f16", q_len, kv_len, n_shared, pad=8, shift=8, out_f32=True))
+
+
+def test_graph(paged):
+    """append and attention of a set batch captured once and replayed over new values."""
+    from llamd_rs_b200 import backend
+
+    H, K, D, page, dtype = 8, 1, 128, 16, "f16"
+    q_len, kv_len = [1, 1, 40], [130, 17, 40]
+    rng = np.random.default_rng(5)
+    tables, n_pages = scatter_tables(rng, kv_len, page)
+    b = paged.Batch(H, K, D, page, dtype)
+    b.set(q_len, kv_len, tables, n_pages)
+    T = b.tokens
+    x = [rng.standard_normal((2, T, n, D)).astype(np.float32) for n in (H, K, K)]
+    bufs = [dev(v[0]) for v in x]
+    cache = [plain.to_bits(rng.standard_normal((n_pages, K, page, D)), dtype) for _ in range(2)]
+    kp, vp, q, out = dev(cache[0]), dev(cache[1]), dev(np.zeros((T, H, D), np.uint16)), dev(np.zeros((T, H, D), np.uint16))
+    backend.sync()
+    assert lib().llamd_fwd_begin_capture() == 0
+    b.append(*bufs, q, kp, vp)
+    b.attention(q, kp, vp, out)
+    assert lib().llamd_fwd_end_capture() == 0
+    try:
+        for i in range(2):
+            for buf, v in zip(bufs, x):
+                buf.upload(v[i])
+            assert lib().llamd_fwd_graph_launch() == 0
+            backend.sync()
+            seq, pos = plain.positions(q_len, kv_len)
+            ids = np.array([tables[s][p // page] for s, p in zip(seq, pos)])
+            for c, v in zip(cache, x[1:]):
+                c[ids, :, pos % page] = plain.to_bits(v[i], dtype)
+            want, bound = plain.attention(plain.from_bits(plain.to_bits(x[0][i], dtype), dtype), plain.from_bits(cache[0], dtype),
+                                          plain.from_bits(cache[1], dtype), tables, q_len, kv_len, D ** -0.5, dtype)
+            close(plain.from_bits(out.download(np.uint16, T * H * D), dtype).reshape(T, H, D), want, bound)
+    finally:
+        lib().llamd_fwd_graph_destroy()
+    assert paged.status() == 0
 
 
 def test_no_tokens(paged):
