@@ -1,0 +1,81 @@
+"""The host side of paged caches, without a device: pages and who holds them, the angles' tables, what is refused before any launch."""
+import numpy as np
+import pytest
+
+
+@pytest.fixture(scope="module")
+def paged():
+    import __graft_entry__ as g
+
+    g.build()
+    from llamd_rs_b200 import paged as p
+
+    return p
+
+
+def test_pages_are_neither_lost_nor_held_twice(paged):
+    """Conversations that begin, fork, grow and end in random order: every page is free or held by exactly the tables that list it."""
+    rng = np.random.default_rng(1)
+    pool, live = paged.Pages(40, 16), []
+    for _ in range(600):
+        what = rng.integers(4)
+        if what == 0 or not live:
+            live.append([[], 0])
+        elif what == 1 and len(live) < 12:
+            table, n = live[rng.integers(len(live))]
+            share = int(rng.integers(0, n // 16 + 1)) * 16
+            live.append([pool.fork(table, share), share])
+        elif what == 2:
+            c = live[rng.integers(len(live))]
+            more = c[1] + int(rng.integers(1, 60))
+            before = list(c[0])
+            try:
+                pool.grow(c[0], more)
+                c[1] = more
+            except paged.OutOfPages:
+                assert c[0] == before
+        else:
+            table, _ = live.pop(rng.integers(len(live)))
+            pool.release(table)
+        held = np.zeros(40, int)
+        for table, n in live:
+            assert len(table) * 16 >= n and len(set(table)) == len(table)
+            for p in table:
+                held[p] += 1
+        assert pool.free() == np.sum(held == 0)
+        assert pool._held == held.tolist()
+
+
+def test_pages_refuse(paged):
+    for n, size in ((0, 16), (4, 8), (4, 24), (4, 8192)):
+        with pytest.raises(paged.ShapeError):
+            paged.Pages(n, size)
+    p = paged.Pages(2, 16)
+    t = []
+    p.grow(t, 20)
+    with pytest.raises(paged.Malformed):
+        p.fork(t, 33)
+    with pytest.raises(paged.Malformed):
+        p.fork(t, 8)
+
+
+@pytest.mark.parametrize("rot,base", [(128, 1e6), (64, 1e4), (2, 1e4)])
+def test_table_of_angles(paged, rot, base):
+    """Rounded once from double: within half a step of f32 of the definition, at far positions too."""
+    rows = 5000
+    got = paged.rope_table(rows, rot, base).astype(np.float64)
+    a = np.arange(rows)[:, None] * float(np.float32(base)) ** (-2.0 * np.arange(rot // 2) / rot)
+    assert np.max(np.abs(got - np.stack([np.sin(a), np.cos(a)], -1))) <= 2.0 ** -25 + 1e-11
+
+
+def test_linear_scaling_stretches_positions(paged):
+    assert np.array_equal(paged.rope_table(64, 32, 1e4, "linear", 4.0)[::4], paged.rope_table(16, 32, 1e4))
+
+
+def test_refused_without_a_device(paged):
+    from llamd_rs_b200 import backend
+
+    if backend.available():
+        pytest.skip("a device is present")
+    with pytest.raises(paged.Unsupported):
+        paged.Batch(8, 2, 64, 16)
