@@ -132,14 +132,14 @@ struct Plan {
 // A stretch of positions that some tokens attend to: a sequence's own behind the shared prefix, or the prefix itself.
 struct Stretch {
     int table, begin, end, token, n_tok, limit, step;
-    bool small(int group) const { return group <= kPagedSmallRows && (long long)n_tok * group <= kPagedFewRows; }
+    bool small = false;  // for paged_decode.cu
 };
 
 // Positions to a piece of paged_decode.cu. Its CTAs run two to an SM; the longest piece should not outlast an even share of
 // the bytes by much, and a piece costs 8 rows of f32 (4 KB at 128 elements) written and read again where a stretch is cut, which 128 positions
 // (64 KB) repay.
 int decode_piece(long long positions, int n_head_kv, int sms) {
-    const long long share = (positions * n_head_kv + 4LL * sms - 1) / (4LL * sms);
+    const long long share = (2 * positions * n_head_kv + 3LL * sms - 1) / (3LL * sms);
     return (int)std::max(128LL, (share + 15) / 16 * 16);
 }
 
@@ -243,6 +243,13 @@ void make_plan(Plan &plan, const PagedView &v, const int32_t *q_len, const int32
     if (shared) stretch.push_back({0, 0, v.n_shared, 0, v.tokens, v.n_shared, 0});
     for (int s = 0, t = 0; s < v.n_seq; t += q_len[s], s++)
         if (q_len[s]) stretch.push_back({s * v.table_stride, v.n_shared, kv_len[s], t, q_len[s], kv_len[s] - q_len[s] + 1, 1});
+    // Which go to paged_decode.cu: those of few query rows, and a shared one that is little work in all, for which a third launch costs more than that
+    // kernel's lower rate (32 tokens of 8 heads behind 512 positions 14.5 us against 20.2, 64 23.6 against 24.7, 100 behind 1024 34.6 against 29.8;
+    // prompts gain nothing: 130 tokens 12.9 against 8.6).
+    for (Stretch &st : stretch) {
+        const long long rows = (long long)st.n_tok * group;
+        st.small = group <= kPagedSmallRows && (rows <= kPagedFewRows || (!st.step && rows * (st.end - st.begin) * v.n_head_kv <= kPagedFewWork));
+    }
     // some tokens of a stretch, and where they leave partial results, by kv head
     struct Tile {
         int stretch, token, n_tok, end;
@@ -252,7 +259,7 @@ void make_plan(Plan &plan, const PagedView &v, const int32_t *q_len, const int32
     auto tiles_of = [&](int tile_tokens, std::vector<Tile> &tiles, std::vector<Large> &large) {
         for (size_t i = 0; i < stretch.size(); i++) {
             const Stretch &st = stretch[i];
-            const bool small = st.small(group);
+            const bool small = st.small;
             const int most = small ? few_tokens : tile_tokens, n_tiles = (st.n_tok + most - 1) / most, per = small ? (st.n_tok + n_tiles - 1) / n_tiles : most;
             for (int x = 0; x < st.n_tok; x += per) {
                 const int n = std::min(per, st.n_tok - x), end = std::min(st.end, st.limit + st.step * (x + n - 1));
@@ -269,7 +276,7 @@ void make_plan(Plan &plan, const PagedView &v, const int32_t *q_len, const int32
     tiles_of(2 * (kPagedTileRows / group), tiles, large);
     long long small_positions = 0;
     for (const Tile &tile : tiles)
-        if (stretch[tile.stretch].small(group)) small_positions += tile.end - stretch[tile.stretch].begin;
+        if (stretch[tile.stretch].small) small_positions += tile.end - stretch[tile.stretch].begin;
     int small_sms = sms, large_sms = sms;
     double blocks = 0.0;
     for (const Large &x : large) blocks += x.blocks + kPieceCost;
@@ -303,7 +310,7 @@ void make_plan(Plan &plan, const PagedView &v, const int32_t *q_len, const int32
     const int piece = decode_piece(small_positions, v.n_head_kv, small_sms);
     for (Tile &tile : tiles) {
         const Stretch &st = stretch[tile.stretch];
-        if (!st.small(group)) continue;
+        if (!st.small) continue;
         const int len = tile.end - st.begin, n = (len + piece - 1) / piece, per = ((len + n - 1) / n + 15) / 16 * 16, rows = tile.n_tok * group;
         for (int b = st.begin; b < tile.end; b += per) {
             PagedItem it = item_of(tile, b, std::min(tile.end, b + per));

@@ -54,8 +54,9 @@ struct PagedAttn {
     float2 *part_ml;   // [rows] (m, sum)
 };
 
-// Query rows (tokens x heads of a group) of a piece that paged_decode.cu takes, and of a stretch that goes there in pieces of so many.
+// Query rows (tokens x heads of a group) of a piece that paged_decode.cu takes, and of a stretch that always goes there, in pieces of so many.
 constexpr int kPagedSmallRows = 32, kPagedFewRows = 96;
+constexpr long long kPagedFewWork = 800000;  // rows x positions x kv heads
 
 void paged_decode_launch(const PagedAttn &p, int type, int n_items, int max_rows, cudaStream_t to);
 constexpr int kPagedTileRows = 128, kPagedBlock = 128;  // of paged_prompt.cu: two tiles of query rows to a piece, positions to a block
