@@ -237,14 +237,14 @@ double Dealer::best(const std::vector<Large> &large, std::vector<Cut> &cuts) con
 }
 
 void make_plan(Plan &plan, const PagedView &v, const int32_t *q_len, const int32_t *kv_len, int sms) {
-    const int group = v.group, few_tokens = std::max(1, kPagedSmallRows / group);
+    const int group = v.group, few_tokens = std::max(1, kPagedPieceRows / group);
     std::vector<Stretch> stretch;  // the shared one, where there is one, then the sequences' own
     const bool shared = v.n_shared && v.tokens;
     if (shared) stretch.push_back({0, 0, v.n_shared, 0, v.tokens, v.n_shared, 0});
     for (int s = 0, t = 0; s < v.n_seq; t += q_len[s], s++)
         if (q_len[s]) stretch.push_back({s * v.table_stride, v.n_shared, kv_len[s], t, q_len[s], kv_len[s] - q_len[s] + 1, 1});
     // Which go to paged_decode.cu: those of few query rows, and a shared one that is little work in all, for which a third launch costs more than that
-    // kernel's lower rate (32 tokens of 8 heads behind 512 positions 14.5 us against 20.2, 64 23.6 against 24.7, 100 behind 1024 34.6 against 29.8;
+    // kernel's lower rate (32 tokens of 8 heads behind 512 positions 11.5 us against 20.2, 64 23.6 against 24.7, 100 behind 1024 34.6 against 29.8;
     // prompts gain nothing: 130 tokens 12.9 against 8.6).
     for (Stretch &st : stretch) {
         const long long rows = (long long)st.n_tok * group;
