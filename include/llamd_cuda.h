@@ -444,7 +444,7 @@ void llamd_fwd_attention_prefill(const float *q, const float *kc, const float *v
 /* hd 64 or 128; n_head / n_head_kv a whole number up to 64; page_size a power of two, 16 to 4096; type (of q_out, out and the
  * pools) LLAMD_PAGED_F16 or _BF16. NULL and a message where refused. */
 void *llamd_cuda_paged_new(int n_head, int n_head_kv, int hd, int page_size, int type);
-/* Waits for the launches that read the batch. */
+/* Launches that read the batch may still be under way. The library keeps some of the batch's memory for the next one. */
 void llamd_cuda_paged_free(void *batch);
 /* pages: [n_seq][pages_stride], ids below n_pages (the pools' size), of each sequence the first
  * ceil(kv_len / page_size) are read. q_len may be 0. n_shared: the first n_shared positions (whole pages, the same ids in every

@@ -30,6 +30,34 @@ bool side_ready() {
     return g_side && g_fork && g_join;
 }
 
+// Memory of batches that are gone, for the next ones: a host that makes a batch for every step would otherwise pin and free for milliseconds each
+// time. Kept device memory needs no wait: whatever still reads it is in front of the next batch's copy on the same stream.
+struct Kept {
+    static constexpr size_t kMost = 6, kLargest = 32 << 20;
+    std::vector<std::pair<uint8_t *, size_t>> blocks;
+    // The smallest that n bytes fit in, or null.
+    uint8_t *take(size_t n, size_t &have) {
+        size_t best = blocks.size();
+        for (size_t i = 0; i < blocks.size(); i++)
+            if (blocks[i].second >= n && (best == blocks.size() || blocks[i].second < blocks[best].second)) best = i;
+        if (best == blocks.size()) return nullptr;
+        uint8_t *p = blocks[best].first;
+        have = blocks[best].second;
+        blocks.erase(blocks.begin() + best);
+        return p;
+    }
+    bool keep(uint8_t *p, size_t n) {
+        if (blocks.size() >= kMost || n > kLargest) return false;
+        try {
+            blocks.push_back({p, n});
+        } catch (const std::exception &) {
+            return false;
+        }
+        return true;
+    }
+};
+Kept g_device, g_pinned;
+
 struct Batch {
     PagedView view = {};
     int type = 0, n_pages = 0, max_kv = 0, sms = 0;
@@ -40,30 +68,42 @@ struct Batch {
     cudaEvent_t copied = nullptr;
     // attention's pieces (device addresses in `dev`) and the partial results that they leave
     const PagedItem *small = nullptr, *large = nullptr;  // for paged_decode.cu and paged_prompt.cu
+    const int32_t *begin = nullptr;                      // large: each CTA's
     const PagedMerge *merge = nullptr;
     const PagedPart *part = nullptr;
-    const int32_t *begin = nullptr;  // large: each CTA's
     bool beside = false;
     int n_small = 0, small_rows = 0, n_ctas = 0, n_merge = 0, most = 0;
     uint8_t *partial = nullptr;
     size_t partial_bytes = 0, partial_rows = 0;
 
     ~Batch() {
-        // (frees wait for the stream: launches that read the batch are done)
-        if (dev || host || partial) cudaStreamSynchronize(stream());
-        if (dev) cudaFree(dev);
-        if (partial) cudaFree(partial);
-        if (host) cudaFreeHost(host);
+        if (copied) cudaEventSynchronize(copied);
+        drop(dev, dev_bytes);
+        drop(partial, partial_bytes);
+        drop_host();
         if (copied) cudaEventDestroy(copied);
+    }
+    void drop(uint8_t *&p, size_t &n) {
+        if (p && !g_device.keep(p, n)) {
+            cudaStreamSynchronize(stream());  // (launches that read it are done)
+            cudaFree(p);
+        }
+        p = nullptr, n = 0;
+    }
+    void drop_host() {  // (not before the copy out of it is done)
+        if (host && !g_pinned.keep(host, host_bytes)) cudaFreeHost(host);
+        host = nullptr, host_bytes = 0;
     }
     // A device buffer of n bytes at least; what was in it is lost where it grows.
     bool grow(uint8_t *&p, size_t &have, size_t n) {
         if (n <= have) return true;
-        if (p && cudaStreamSynchronize(stream()) != cudaSuccess) return fail("paged batch: sync");
-        if (p) cudaFree(p);
-        p = nullptr;
-        have = 0;
-        if (cudaMalloc((void **)&p, n) != cudaSuccess) return fail("paged batch: device memory");
+        drop(p, have);
+        if ((p = g_device.take(n, have))) return true;
+        n = std::max<size_t>(n, 1 << 16);
+        if (cudaMalloc((void **)&p, n) != cudaSuccess) {
+            p = nullptr;
+            return fail("paged batch: device memory");
+        }
         have = n;
         return true;
     }
@@ -72,11 +112,15 @@ struct Batch {
         if (!copied && cudaEventCreateWithFlags(&copied, cudaEventDisableTiming) != cudaSuccess) return fail("paged batch: event");
         if (cudaEventSynchronize(copied) != cudaSuccess) return fail("paged batch: previous copy");
         if (n > host_bytes) {
-            if (host) cudaFreeHost(host);
-            host = nullptr;
-            host_bytes = 0;
-            if (cudaHostAlloc((void **)&host, 2 * n, cudaHostAllocDefault) != cudaSuccess) return fail("paged batch: pinned memory");
-            host_bytes = 2 * n;
+            drop_host();
+            if (!(host = g_pinned.take(n, host_bytes))) {
+                const size_t want = std::max<size_t>(2 * n, 1 << 16);
+                if (cudaHostAlloc((void **)&host, want, cudaHostAllocDefault) != cudaSuccess) {
+                    host = nullptr;
+                    return fail("paged batch: pinned memory");
+                }
+                host_bytes = want;
+            }
         }
         return (n <= dev_bytes || grow(dev, dev_bytes, 2 * n)) && grow(partial, partial_bytes, rows * (view.hd * sizeof(float) + sizeof(float2)));
     }
