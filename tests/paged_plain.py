@@ -58,17 +58,15 @@ def attention(q, k_pages, v_pages, tables, q_len, kv_len, scale, dtype):
         idx = np.arange(m)
         ids = np.asarray(tables[s])[idx // page] if m else np.zeros(0, int)
         k, v = k_pages[ids, :, idx % page], v_pages[ids, :, idx % page]
-        for h in range(n_head):
-            kk, vv = k[:, h // group], v[:, h // group]
-            for i in range(n):
-                e = m - n + i + 1
-                x, row = kk[:e], q[at + i, h]
-                sc = scale * (x @ row)
-                d = 2.0 ** -23 * x.shape[1] * abs(scale) * np.max(np.abs(x) @ np.abs(row))
-                p = np.exp(sc - sc.max())
-                p /= p.sum()
-                o = p @ vv[:e]
-                out[at + i, h] = o
-                bound[at + i, h] = u * np.abs(o) + (u + 2 * d + 2.0 ** -20) * (p @ np.abs(vv[:e])) + tiny * (1 + np.abs(vv[:e]).sum(0))
+        seen = np.arange(m) <= np.arange(m - n, m)[:, None]
+        for h in range(n_head if n else 0):
+            kk, vv, row = k[:, h // group], v[:, h // group], q[at:at + n, h]
+            sc = np.where(seen, scale * (row @ kk.T), -np.inf)
+            d = 2.0 ** -23 * kk.shape[1] * abs(scale) * np.where(seen, np.abs(row) @ np.abs(kk).T, 0).max(1, keepdims=True)
+            p = np.exp(sc - sc.max(1, keepdims=True))
+            p /= p.sum(1, keepdims=True)
+            o = p @ vv
+            out[at:at + n, h] = o
+            bound[at:at + n, h] = u * np.abs(o) + (u + 2 * d + 2.0 ** -20) * (p @ np.abs(vv)) + tiny * (1 + seen @ np.abs(vv))
         at += n
     return out, bound

@@ -226,6 +226,19 @@ def test_attention_beside(paged):
     close(*run_attention(*args, repeat=3))
 
 
+@pytest.mark.parametrize("H,D,dtype", [(8, 128, "f16"), (5, 64, "bf16"), (1, 128, "bf16")])
+def test_attention_many_pieces(paged, H, D, dtype):
+    """Several pieces to every CTA, of one tile and of two, of one block and of several, tails of every length, and short sequences between them."""
+    rng = np.random.default_rng(H)
+    q_len, kv_len = [], []
+    for _ in range(260):
+        n = int(rng.choice([0, 1, 3, rng.integers(13, 17), rng.integers(17, 60), rng.integers(100, 140)], p=[.05, .1, .1, .3, .35, .1])) * (8 if H == 1 else 1)
+        q_len.append(n)
+        kv_len.append(n + int(rng.choice([0, 0, rng.integers(0, 40), rng.integers(0, 400)])))
+    close(*run_attention(paged, H, 1, D, 16, dtype, q_len, kv_len, repeat=2))
+    close(*run_attention(paged, H, 1, D, 32, dtype, q_len, [m + 256 for m in kv_len], 256, repeat=2))
+
+
 @pytest.mark.parametrize("q_len,kv_len,n_shared", [([1, 2], [300, 90], 0), ([1] * 6, [100 + i for i in range(6)], 96), ([90, 60], [200, 60], 0)])
 def test_attention_rows_apart(paged, q_len, kv_len, n_shared):
     """Rows of q and out further apart than their values, and starting at 16 bytes but not at 32."""
