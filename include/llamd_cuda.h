@@ -441,7 +441,7 @@ void llamd_fwd_attention_prefill(const float *q, const float *kc, const float *v
 #define LLAMD_PAGED_F16 0
 #define LLAMD_PAGED_BF16 1
 #define LLAMD_PAGED_F32 2
-/* hd 64 or 128; n_head / n_head_kv a whole number up to 64; page_size a power of two, 16 to 4096; type (of q_out, out and the
+/* hd 64 or 128; n_head up to 4096, n_head / n_head_kv a whole number up to 64; page_size a power of two, 16 to 4096; type (of q_out, out and the
  * pools) LLAMD_PAGED_F16 or _BF16. NULL and a message where refused. */
 void *llamd_cuda_paged_new(int n_head, int n_head_kv, int hd, int page_size, int type);
 /* Launches that read the batch may still be under way. The library keeps some of the batch's memory for the next one. */
@@ -452,7 +452,7 @@ void llamd_cuda_paged_free(void *batch);
  * checked here, before a launch can use it: 0, or -1 and a message, and the batch is as it was (where memory could not be had: not
  * set). Enqueues one copy; may allocate where a batch is larger than any before it; not while a graph is captured, but what it has set may
  * be used in one. A batch that is set again serves the launches enqueued
- * after the call. */
+ * after the call; a graph that was captured with it is not replayed any more. */
 int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int32_t *kv_len, const int32_t *pages, int pages_stride,
                          int n_pages, int n_shared);
 /* The new tokens' q, k, v rows ([tokens][heads][hd], in_type LLAMD_PAGED_F32 or the batch's type; strides in elements
@@ -466,10 +466,11 @@ int llamd_fwd_paged_append(const void *batch, const void *q, const void *k, cons
                            int rope_rows, int rot, int interleaved, void *q_out, size_t out_stride, void *k_pages, void *v_pages);
 /* out[token][head] = softmax(scale * q . k) v over the positions up to the token's own; scale > 0. q and out in the batch's type, or out in f32
  * (out_f32: the same sums, not rounded); rows start at 16 bytes. Slots behind a sequence's last position may hold
- * anything, NaN and infinities too. Part of a large batch may run on a second stream of the library's, which the call joins to its own. 0 / -1 as above. */
+ * anything, NaN and infinities too; values that some of the batch's tokens attend to are finite, or other tokens' outputs may be NaN as well (a weight of
+ * 0 times infinity). Part of a large batch may run on a second stream of the library's, which the call joins to its own. 0 / -1 as above. */
 int llamd_fwd_paged_attention(const void *batch, const void *q, size_t q_stride, const void *k_pages, const void *v_pages, void *out,
                               size_t out_stride, int out_f32, float scale);
-/* 0 while every wait inside the attention's kernels has been met; otherwise 1 + the first piece whose wait ran out (outputs are
+/* 0 while every wait inside the attention's kernels has been met; otherwise 1 + the first block whose wait ran out (outputs are
  * then incomplete). Synchronises the stream. */
 int llamd_fwd_paged_status(void);
 /* The table of llamd_fwd_paged_append on the host: sine and cosine of r * f_i, f_i = base^(-2i / rot), evaluated in double.

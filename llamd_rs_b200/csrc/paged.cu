@@ -193,9 +193,10 @@ int decode_piece(long long positions, int n_head_kv, int sms) {
 constexpr double kHalfCost = 0.85, kPieceCost = 2.0, kPartCost = 2.0, kJoinCost = 4.0;
 
 // Small and large pieces of one batch, one launch after the other, leave first HBM and then the tensor cores waiting; at the same time, each on SMs of its
-// own, neither. What they take, in SM-microseconds: an SM draws about 65 GB/s from HBM where all do not draw at once, a block of two tiles
-// takes 2 us. Each has to be worth more than a launch (kBesideLeast us on all SMs).
-constexpr double kSmBytes = 65e3, kBlockMicros = 2.0, kBesideLeast = 6.0;
+// own, neither. What they take, in SM-microseconds: an SM draws about 85 GB/s from HBM where all do not draw at once, a block of two tiles
+// takes 2 us. Each has to be worth something (kBesideLeast us on all SMs), or the two kernels run in turn (measured: 100 sequences behind 1024 shared
+// positions, 5 query heads to a kv head, 38 us in turn, 33 beside each other; 100 behind 1024, 8 to a kv head, 37 and 28; at worst 200 behind 256, 28 and 29).
+constexpr double kSmBytes = 85e3, kBlockMicros = 2.0, kBesideLeast = 0.5;
 
 struct Large {  // a tile of one kv head
     int tile, head, blocks;
@@ -287,12 +288,18 @@ void make_plan(Plan &plan, const PagedView &v, const int32_t *q_len, const int32
     if (shared) stretch.push_back({0, 0, v.n_shared, 0, v.tokens, v.n_shared, 0});
     for (int s = 0, t = 0; s < v.n_seq; t += q_len[s], s++)
         if (q_len[s]) stretch.push_back({s * v.table_stride, v.n_shared, kv_len[s], t, q_len[s], kv_len[s] - q_len[s] + 1, 1});
-    // Which go to paged_decode.cu: those of few query rows, and a shared one that is little work in all, for which a third launch costs more than that
-    // kernel's lower rate (32 tokens of 8 heads behind 512 positions 11.5 us against 20.2, 64 23.6 against 24.7, 100 behind 1024 34.6 against 29.8;
-    // prompts gain nothing: 130 tokens 12.9 against 8.6).
+    // Which go to paged_decode.cu: those of one of its pieces' rows, and others while they are little work in all (rows x positions x kv heads): a launch
+    // less and no piece to begin weigh more there than reading K and V once for every 16 rows. Measured, that kernel against the other, us: own stretches
+    // of 160 rows and 20 positions 4.0 and 7.1, 240 rows and 130 positions 7.2 and 9.0, 4 times 64 and 508 8.3 and 11.5; 16 times 64 and 1000 to 4000
+    // 43 and 27, 1 of 128 and 8000 14 and 21; 2000 rows and 250 positions 12.9 and 8.6. A shared stretch, which otherwise makes a third launch: 192 rows and
+    // 2048 positions 13.4 and 16.4, 512 and 512 20.5 and 22.9; 1600 and 256 31.8 and 29.3.
+    constexpr long long kFewRows = 256, kFewOwnWork = 800000, kFewSharedWork = 1600000;
+    long long own_work = 0;
+    for (const Stretch &st : stretch)
+        if (st.step && st.n_tok * group > kPagedSmallRows) own_work += (long long)st.n_tok * group * (st.end - st.begin) * v.n_head_kv;
     for (Stretch &st : stretch) {
         const long long rows = (long long)st.n_tok * group;
-        st.small = group <= kPagedSmallRows && (rows <= kPagedFewRows || (!st.step && rows * (st.end - st.begin) * v.n_head_kv <= kPagedFewWork));
+        st.small = group <= kPagedSmallRows && (rows <= kPagedSmallRows || (st.step ? rows <= kFewRows && own_work <= kFewOwnWork : rows * (st.end - st.begin) * v.n_head_kv <= kFewSharedWork));
     }
     // some tokens of a stretch, and where they leave partial results, by kv head
     struct Tile {
@@ -556,9 +563,9 @@ using namespace llamd;
 extern "C" {
 
 void *llamd_cuda_paged_new(int n_head, int n_head_kv, int hd, int page_size, int type) {
-    if (n_head < 1 || n_head_kv < 1 || n_head % n_head_kv || n_head / n_head_kv > 64 || (hd != 64 && hd != 128) || page_size < 16 || page_size > 4096 ||
+    if (n_head < 1 || n_head > 4096 || n_head_kv < 1 || n_head % n_head_kv || n_head / n_head_kv > 64 || (hd != 64 && hd != 128) || page_size < 16 || page_size > 4096 ||
         (page_size & (page_size - 1)) || (type != kPagedF16 && type != kPagedBf16)) {
-        set_error_msg("paged batch: heads of 64 or 128 elements, up to 64 query heads to a kv head, pages of 16 to 4096 positions (a power of two), f16 or bf16");
+        set_error_msg("paged batch: up to 4096 heads of 64 or 128 elements, up to 64 query heads to a kv head, pages of 16 to 4096 positions (a power of two), f16 or bf16");
         return nullptr;
     }
     if (!stream() || !paged_prompt_ready()) return nullptr;
@@ -665,6 +672,8 @@ int llamd_fwd_paged_append(const void *batch, const void *q, const void *k, cons
     const size_t qd = (size_t)g.n_head * g.hd, kvd = (size_t)g.n_head_kv * g.hd;
     if (q_stride < qd || k_stride < kvd || v_stride < kvd || out_stride < qd) return refuse("paged append: a row overlaps the next");
     if (!aligned16(q_out) || out_stride % 8 || !aligned16(k_pages) || !aligned16(v_pages)) return refuse("paged append: outputs start at 16 bytes");
+    const uintptr_t odd = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v, odd_w = (uintptr_t)wq | (uintptr_t)wk;
+    if (odd % (in_type == kPagedF32 ? 4 : 2) || odd_w % 4) return refuse("paged append: an input starts inside an element");
     AppendParams p = {};
     p.b = g, p.sms = b->sms;
     p.q = q, p.k = k, p.v = v, p.q_stride = q_stride, p.k_stride = k_stride, p.v_stride = v_stride, p.out_stride = out_stride;

@@ -54,12 +54,11 @@ struct PagedAttn {
     float2 *part_ml;   // [rows] (m, sum)
 };
 
-// Query rows (tokens x heads of a group) of a piece that paged_decode.cu can take (one token of a wide group), of one that it is given where a
-// stretch has several tokens, and of a stretch that always goes there. Pieces of 16 rows: 32 take four times the registers of 8 and half the
+// Query rows (tokens x heads of a group) of a piece that paged_decode.cu can take (one token of a wide group), and of one that it is given where a
+// stretch has several tokens. Pieces of 16 rows: 32 take four times the registers of 8 and half the
 // CTAs (8 sequences behind 512 shared positions 12.1 us against 6.6, 64 with 3 new tokens behind 3500 102.9 against 90.7), 8 read K and V
 // twice as often (102.9).
-constexpr int kPagedSmallRows = 32, kPagedPieceRows = 16, kPagedFewRows = 96;
-constexpr long long kPagedFewWork = 800000;  // rows x positions x kv heads
+constexpr int kPagedSmallRows = 32, kPagedPieceRows = 16;
 
 void paged_decode_launch(const PagedAttn &p, int type, int n_items, int max_rows, cudaStream_t to);
 constexpr int kPagedTileRows = 128, kPagedBlock = 128;  // of paged_prompt.cu: two tiles of query rows to a piece, positions to a block

@@ -11,13 +11,15 @@
 // A warp owns every fourth slice of 16 positions of the piece, with its own ring of kStages slices (cp.async, 16 bytes a lane), its own running
 // maximum and sums, so nothing in the loop waits for another warp; the four join through shared memory at the end.
 // A page holds a multiple of 16 positions: a slice is 16 neighbouring rows of one page, contiguous in memory.
+//
+// What it measured (32 heads over 4 kv heads of 128): 32 sequences of 150 to 8000 positions, bf16, 42 us, 5.8 TB/s, 0.88 of a copy's rate; one sequence of
+// 4002 positions 6.4 us with the launch that joins its 32 pieces (1.3 us of bytes: two launches and the loads' latency are left).
 #include "paged.cuh"
 
 namespace llamd {
 namespace {
 
 constexpr int kWarps = 4, kStages = 3, kSlice = 16;
-constexpr int kMergeAlone = 8, kMergeAloneFew = 2;  // parts to a row that one warp adds up: of many rows, and of few
 
 __device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, int bytes) {  // (the rest of the 16 is zero)
@@ -257,12 +259,11 @@ __global__ void __launch_bounds__(kWarps * 32, 2) paged_decode_kernel(const Page
 }
 
 // A row (token, head): its parts' m and sums a lane each, then their rows, weighted and added in the parts' order. W warps share a row's
-// parts (every W-th each) and add up through shared memory: the parts of a row are as many loads in a row, and where rows are few
-// nothing else hides them (one token behind 4001 positions, 32 parts to each of 32 rows: the two launches take 12.7 us with W = 1, 7.2 with 8).
+// parts (every W-th each) and add up through shared memory.
 template <typename T, int HD, int W>
 __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttn p, const PagedMerge *merge, const PagedPart *parts, int n_rows) {
     constexpr int V = HD / 32;
-    __shared__ float s_o[W > 1 ? W : 1][HD];
+    __shared__ float s_o[W > 1 ? 8 : 1][HD];
     pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, mine = warp % W, x = (int)blockIdx.x * (8 / W) + warp / W;
     const bool live = x < n_rows;
@@ -309,11 +310,11 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttn p, con
 #pragma unroll
         for (int j = 0; j < V; j++) s_o[warp][lane * V + j] = o[j];
         __syncthreads();
-        if (warp) return;
+        if (mine) return;
 #pragma unroll
         for (int j = 0; j < V; j++)
 #pragma unroll
-            for (int y = 1; y < W; y++) o[j] += s_o[y][lane * V + j];
+            for (int y = 1; y < W; y++) o[j] += s_o[warp + y][lane * V + j];
     }
     if (!live) return;
     const float by = 1.0f / sum;
@@ -355,9 +356,15 @@ void paged_decode_launch(const PagedAttn &p, int type, int n_items, int max_rows
 template <typename T, int HD>
 static void merge_hd(const PagedAttn &p, const PagedMerge *merge, const PagedPart *parts, int n_merge, int most, int sms) {
     const int rows = n_merge * p.b.group;
-    if (most > kMergeAlone || (most > kMergeAloneFew && rows <= 16 * sms))
-        launch_kc(PDL_PAGED, "paged_merge", paged_merge_kernel<T, HD, 8>, dim3(rows), dim3(256), 0, p, merge, parts, rows);
-    else launch_kc(PDL_PAGED, "paged_merge", paged_merge_kernel<T, HD, 1>, dim3((rows + 7) / 8), dim3(256), 0, p, merge, parts, rows);
+    const auto launch = [&](auto kernel, int w) { launch_kc(PDL_PAGED, "paged_merge", kernel, dim3((rows + 8 / w - 1) / (8 / w)), dim3(256), 0, p, merge, parts, rows); };
+    // As many warps to a row as 32 to an SM allow: where rows are few, their parts are loads one behind the other; where they are many, there are warps
+    // enough (32 rows of 32 parts: attention 6.4 us with 8, 14.6 with 1; 768 rows 16.7 and 20.2; 2048 rows 25.7 and 18.3; 8192 rows 76 and 53).
+    int w = most > 2 ? 8 : 1;
+    while (w > 1 && (long long)rows * w > 32LL * sms) w >>= 1;
+    if (w == 8) launch(paged_merge_kernel<T, HD, 8>, 8);
+    else if (w == 4) launch(paged_merge_kernel<T, HD, 4>, 4);
+    else if (w == 2) launch(paged_merge_kernel<T, HD, 2>, 2);
+    else launch(paged_merge_kernel<T, HD, 1>, 1);
 }
 void paged_merge_launch(const PagedAttn &p, int type, const PagedMerge *merge, const PagedPart *parts, int n_merge, int most, int sms) {
     if (type == kPagedF16) p.b.hd == 128 ? merge_hd<__half, 128>(p, merge, parts, n_merge, most, sms) : merge_hd<__half, 64>(p, merge, parts, n_merge, most, sms);

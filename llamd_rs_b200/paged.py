@@ -198,6 +198,8 @@ class Batch:
             if not rot:
                 rope_rows = 0
             elif hasattr(rope, "data_ptr"):
+                if rope.dim() > 1 and rope.shape[0] * rot != rope.numel():
+                    raise ShapeError(f"angles of {tuple(rope.shape)} for {rot} rotated elements")
                 rope_rows = rope.numel() // rot
             elif isinstance(rope, DevBuf):
                 rope_rows = rope.nbytes // (4 * rot)

@@ -352,6 +352,23 @@ def test_refusals(paged):
     backend.sync()
 
 
+def test_refuses_odd_addresses_and_other_tables(paged):
+    torch = pytest.importorskip("torch")
+    from llamd_rs_b200.backend import Malformed, ShapeError
+
+    with pytest.raises(Malformed):
+        paged.Batch(8192, 4096, 64, 16)
+    b = paged.Batch(8, 2, 64, 16, "f16")
+    b.set([2], [20], [[3, 1]], 6)
+    pool, rows = dev(np.zeros(6 * 2 * 16 * 64, np.uint16)), dev(np.zeros(64 * 8 * 64, np.uint16))
+    for i in range(3):  # q, k or v inside an element
+        with pytest.raises(Malformed):
+            b.append(*[rows.ptr + (i == j) for j in range(3)], rows, pool, pool, inputs="f16")
+    x = torch.zeros(2, 12, 64, dtype=torch.float16, device="cuda")
+    with pytest.raises(ShapeError):  # a table of 64 rotated elements read as one of 32
+        b.append(x[:, :8], x[:, 8:10], x[:, 10:], rows, pool, pool, rope=torch.zeros(20, 32, 2, device="cuda"), rot=32)
+
+
 def test_tensors(paged):
     """torch tensors on a stream of their own: strided rows of one projection, types checked, order kept by wait_for / ready_for."""
     torch = pytest.importorskip("torch")
