@@ -431,8 +431,9 @@ void make_plan(Plan &plan, const PagedView &v, const int32_t *q_len, const int32
 // rotate together, so that the rotation needs no neighbour (the halves' layout: 4 elements and their 4 partners rot / 2 further on;
 // neighbouring pairs, and what lies behind the rotated part: 8 in a row), and the norm is a sum over the head's lanes. A warp has
 // several heads of one kind (q, k or v) of one token on their way at once, so the token's angles and the weights are read once for them.
-// Heads that a warp has on their way, and CTAs to an SM; 16-bit and f32 inputs measured (2, 4 and 8 heads, 3 to 6 CTAs): 8192 tokens of f32 13.3 us with
-// 2 heads and 4 CTAs, 6279 tokens of f16 31.6 with 4 and 4, the others 13.5 to 18.7 and 34.9 to 55.
+// Heads that a warp has on their way, and CTAs to an SM; measured with 1 to 8 heads and 3 to 6 CTAs: 6279 tokens of f16, 32 heads over 4 of 128, 28.3 us with 4
+// and 4 (4.6 TB/s), 8192 tokens of f32, 14 over 2 of 64, 11.7 with 2 and 4 (4.9 TB/s), the others 32.8 to 42.7 and 13.0 to 16.9. Instructions and the
+// loads' latency share what is left above the bytes (an issue slot in 7 of 10): 16 elements to a lane or packed arithmetic need registers that cost more warps.
 template <typename TI> constexpr int kAppendHeads = sizeof(TI) == 2 ? 4 : 2;
 constexpr int kAppendCtas = 4;
 
@@ -442,7 +443,7 @@ struct AppendParams {
     size_t q_stride, k_stride, v_stride, out_stride;  // elements between tokens
     const float *wq, *wk, *rope;
     float eps;
-    int rot, aligned, sms, tasks, q_tasks, kv_tasks;  // warps to a token, to its q heads, to its k or v heads
+    int rot, sms, tasks, q_tasks, kv_tasks;  // warps to a token, to its q heads, to its k or v heads
     void *q_out, *k_pages, *v_pages;
 };
 
@@ -469,30 +470,32 @@ template <> struct Four<float> {
 };
 
 // TI: the inputs' type, T: the cache's.
-template <typename TI, typename T, int HD, bool INTERLEAVED>
+template <typename TI, typename T, int HD, bool INTERLEAVED, bool ALIGNED>
 __global__ void __launch_bounds__(256, kAppendCtas) paged_append_kernel(const AppendParams p) {
     constexpr int L = HD / 8, PER = 32 / L, kDeep = kAppendHeads<TI>;  // lanes to a head, heads side by side, heads one behind the other
     pdl_trigger();
     const int warps = (int)(gridDim.x * (blockDim.x >> 5)), lane = threadIdx.x & 31, per_token = p.q_tasks + 2 * p.kv_tasks;
-    int task = (int)((blockIdx.x * blockDim.x + threadIdx.x) >> 5);
+    const int first_task = (int)((blockIdx.x * blockDim.x + threadIdx.x) >> 5), dt = warps / per_token, dc = warps - dt * per_token;
+    int t = first_task / per_token, c = first_task - t * per_token;
     // (the batch's own memory: complete before the launch in front of this one began)
-    PagedToken next = task < p.tasks ? p.b.token[task / per_token] : PagedToken{0, 0};
+    PagedToken next = t < p.b.tokens ? p.b.token[t] : PagedToken{0, 0};
     pdl_wait();
-    for (; task < p.tasks; task += warps) {
-        const int t = task / per_token, c = task - t * per_token;
+    for (int t_next, c_next; t < p.b.tokens; t = t_next, c = c_next) {
         const PagedToken tok = next;
-        if (task + warps < p.tasks) next = p.b.token[(task + warps) / per_token];  // (a round ahead: the angles' address waits for nothing)
+        t_next = t + dt, c_next = c + dc;
+        if (c_next >= per_token) c_next -= per_token, t_next++;
+        if (t_next < p.b.tokens) next = p.b.token[t_next];  // (a round ahead: the angles' address waits for nothing)
         const int kind = c < p.q_tasks ? 0 : c < p.q_tasks + p.kv_tasks ? 1 : 2;  // q, k, v
-        const int heads = kind ? p.b.n_head_kv : p.b.n_head, h0 = (c - (kind ? p.q_tasks + (kind - 1) * p.kv_tasks : 0)) * (kDeep * PER) + lane / L;
-        const int l = lane % L;
+        const int heads = kind ? p.b.n_head_kv : p.b.n_head, h0 = (c - (kind ? p.q_tasks + (kind - 1) * p.kv_tasks : 0)) * (kDeep * PER);
+        const int l = lane % L, mine = h0 + lane / L;
         const bool rotated = kind < 2 && l * 8 < p.rot;
         const int first = rotated && !INTERLEAVED ? l * 4 : l * 8, second = rotated && !INTERLEAVED ? l * 4 + (p.rot >> 1) : l * 8 + 4;
         const TI *src = reinterpret_cast<const TI *>(kind == 0 ? p.q : kind == 1 ? p.k : p.v) + (size_t)t * (kind == 0 ? p.q_stride : kind == 1 ? p.k_stride : p.v_stride);
         Four<TI> raw[kDeep][2];
 #pragma unroll
         for (int i = 0; i < kDeep; i++) {
-            const int h = h0 + i * PER;
-            if (h < heads) raw[i][0].load(src + (size_t)h * HD + first, p.aligned), raw[i][1].load(src + (size_t)h * HD + second, p.aligned);
+            const int h = mine + i * PER;
+            if (h < heads) raw[i][0].load(src + (size_t)h * HD + first, ALIGNED), raw[i][1].load(src + (size_t)h * HD + second, ALIGNED);
             else raw[i][0] = raw[i][1] = Four<TI>{};
         }
         const float *wp = kind == 0 ? p.wq : kind == 1 ? p.wk : nullptr;
@@ -503,12 +506,13 @@ __global__ void __launch_bounds__(256, kAppendCtas) paged_append_kernel(const Ap
             const float4 f = row[0], g = row[1];
             sn[0] = f.x, cs[0] = f.y, sn[1] = f.z, cs[1] = f.w, sn[2] = g.x, cs[2] = g.y, sn[3] = g.z, cs[3] = g.w;
         }
-        if (wp) w[0].load(wp + first, p.aligned), w[1].load(wp + second, p.aligned);
+        if (wp) w[0].load(wp + first, ALIGNED), w[1].load(wp + second, ALIGNED);
         T *dst = reinterpret_cast<T *>(kind == 0 ? p.q_out : kind == 1 ? p.k_pages : p.v_pages) + (kind ? (size_t)tok.row * HD : (size_t)t * p.out_stride);
         const size_t dst_step = kind ? (size_t)p.b.page * HD : HD;
 #pragma unroll
         for (int i = 0; i < kDeep; i++) {
-            const int h = h0 + i * PER;
+            if (h0 + i * PER >= heads) break;  // (the whole warp)
+            const int h = mine + i * PER;
             float x[8];
             raw[i][0].get(x), raw[i][1].get(x + 4);
             if (wp) {
@@ -538,19 +542,20 @@ __global__ void __launch_bounds__(256, kAppendCtas) paged_append_kernel(const Ap
 }
 
 template <typename TI, typename T, int HD>
-void append_launch_hd(AppendParams &p, bool interleaved) {
+void append_launch_hd(AppendParams &p, bool interleaved, bool aligned) {
     constexpr int kHeads = kAppendHeads<TI> * (32 / (HD / 8));  // to a warp
     p.q_tasks = (p.b.n_head + kHeads - 1) / kHeads;
     p.kv_tasks = (p.b.n_head_kv + kHeads - 1) / kHeads;
     p.tasks = p.b.tokens * (p.q_tasks + 2 * p.kv_tasks);
     const dim3 grid((unsigned)std::min((p.tasks + 7) / 8, kAppendCtas * p.sms));
-    if (interleaved) launch_kc(PDL_PAGED, "paged_append", paged_append_kernel<TI, T, HD, true>, grid, dim3(256), 0, p);
-    else launch_kc(PDL_PAGED, "paged_append", paged_append_kernel<TI, T, HD, false>, grid, dim3(256), 0, p);
+    const auto launch = [&](auto kernel) { launch_kc(PDL_PAGED, "paged_append", kernel, grid, dim3(256), 0, p); };
+    if (aligned) launch(interleaved ? paged_append_kernel<TI, T, HD, true, true> : paged_append_kernel<TI, T, HD, false, true>);
+    else launch(interleaved ? paged_append_kernel<TI, T, HD, true, false> : paged_append_kernel<TI, T, HD, false, false>);
 }
 template <typename TI, typename T>
-void append_launch(AppendParams &p, bool interleaved) {
-    if (p.b.hd == 128) append_launch_hd<TI, T, 128>(p, interleaved);
-    else append_launch_hd<TI, T, 64>(p, interleaved);
+void append_launch(AppendParams &p, bool interleaved, bool aligned) {
+    if (p.b.hd == 128) append_launch_hd<TI, T, 128>(p, interleaved, aligned);
+    else append_launch_hd<TI, T, 64>(p, interleaved, aligned);
 }
 
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
@@ -680,13 +685,13 @@ int llamd_fwd_paged_append(const void *batch, const void *q, const void *k, cons
     p.wq = wq, p.wk = wk, p.eps = eps, p.rope = rope_tab, p.rot = rot;
     p.q_out = q_out, p.k_pages = k_pages, p.v_pages = v_pages;
     const size_t per16 = in_type == kPagedF32 ? 4 : 8;
-    p.aligned = aligned16(q) && aligned16(k) && aligned16(v) && !(q_stride % per16) && !(k_stride % per16) && !(v_stride % per16) && aligned16(wq) && aligned16(wk);
+    const bool aligned = aligned16(q) && aligned16(k) && aligned16(v) && !(q_stride % per16) && !(k_stride % per16) && !(v_stride % per16) && aligned16(wq) && aligned16(wk);
     if (b->type == kPagedF16) {
-        if (in_type == kPagedF32) append_launch<float, __half>(p, interleaved != 0);
-        else append_launch<__half, __half>(p, interleaved != 0);
+        if (in_type == kPagedF32) append_launch<float, __half>(p, interleaved != 0, aligned);
+        else append_launch<__half, __half>(p, interleaved != 0, aligned);
     } else {
-        if (in_type == kPagedF32) append_launch<float, __nv_bfloat16>(p, interleaved != 0);
-        else append_launch<__nv_bfloat16, __nv_bfloat16>(p, interleaved != 0);
+        if (in_type == kPagedF32) append_launch<float, __nv_bfloat16>(p, interleaved != 0, aligned);
+        else append_launch<__nv_bfloat16, __nv_bfloat16>(p, interleaved != 0, aligned);
     }
     return error_code() ? -1 : 0;
 }
