@@ -218,6 +218,28 @@ def test_attention_sharp_and_flat(paged, dtype, q_len, kv_len):
     close(*run_attention(paged, 8, 1, 128, 16, dtype, q_len, kv_len, out_f32=True))
 
 
+@pytest.mark.parametrize("H,K,D,page,dtype,q_len,kv_len,n_shared", [c for c in ATTENTION if max(c[5]) > 3 and not c[7]])
+def test_attention_beside_a_long_prompt(paged, H, K, D, page, dtype, q_len, kv_len, n_shared):
+    """Prompts that would be too little work for the tensor cores by themselves, in one batch with another that is not."""
+    long = 300 + 2400 // (H // K)
+    close(*run_attention(paged, H, K, D, page, dtype, q_len + [long], kv_len + [long], n_shared))
+
+
+@pytest.mark.parametrize("n", [9, 24, 41, 90])
+@pytest.mark.parametrize("D,dtype", [(128, "bf16"), (64, "f16")])
+def test_attention_joins(paged, n, D, dtype):
+    """A shared prefix of several parts behind 288 to 2880 rows: they are joined by 8, 4, 2 and 1 warps each."""
+    close(*run_attention(paged, 32, 4, D, 16, dtype, [1] * n, [401 + 5 * i for i in range(n)], 400))
+
+
+@pytest.mark.parametrize("q_len,kv_len", [([9], [300]), ([32], [70]), ([33], [70]), ([20, 1, 31], [20, 400, 131]), ([8] * 5, [600 + i for i in range(5)]),
+                                          ([8] * 24, [500 + i for i in range(24)])])
+def test_attention_few_rows(paged, q_len, kv_len):
+    """Stretches of 64 to 264 query rows, on both sides of the lines between the two kernels."""
+    close(*run_attention(paged, 32, 4, 128, 16, "f16", q_len, kv_len))
+    close(*run_attention(paged, 16, 2, 64, 32, "bf16", q_len, [m + 64 for m in kv_len], 64))
+
+
 def test_attention_beside(paged):
     """A batch large enough that the prefix and the sequences' own positions are read at the same time; twice, the second over the first's results."""
     rng = np.random.default_rng(3)
