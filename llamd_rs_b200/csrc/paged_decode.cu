@@ -14,6 +14,8 @@
 //
 // What it measured (32 heads over 4 kv heads of 128): 32 sequences of 150 to 8000 positions, bf16, 42 us, 5.8 TB/s, 0.88 of a copy's rate; one sequence of
 // 4002 positions 6.4 us with the launch that joins its 32 pieces (1.3 us of bytes: two launches and the loads' latency are left).
+#include <type_traits>
+
 #include "paged.cuh"
 
 namespace llamd {
@@ -65,6 +67,9 @@ template <int HD, int NT> constexpr size_t decode_smem() {
 template <typename T, int HD, int NT>
 __global__ void __launch_bounds__(kWarps * 32, 2) paged_decode_kernel(const PagedAttn p) {
     constexpr int kRow = HD * 2, kTile = kSlice * kRow, kChunks = HD / 8, kSteps = HD / 16;
+    // In f16 the weights are taken 2^15 times as large until the end: at most 2^15 where they would be at most 1, and normal numbers down to 2^-29 of the
+    // largest where they would be down to 2^-14 (131072 positions 15 nats below another, each a weight of 5 subnormal steps, came out 2.6 % too small). bf16 has f32's range.
+    constexpr float kUp = std::is_same<T, __half>::value ? 15.0f : 0.0f;
     extern __shared__ __align__(16) uint8_t ring[];
     __shared__ float2 s_ml[kWarps][NT * 8];
     pdl_trigger();
@@ -186,7 +191,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) paged_decode_kernel(const Page
             float x[4];
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-                const float at = m[n][e] == -INFINITY ? 0.0f : m[n][e];  // (a row that has seen nothing yet: weights 0)
+                const float at = m[n][e] == -INFINITY ? 0.0f : m[n][e] - kUp;  // (a row that has seen nothing yet: weights 0)
                 x[e] = exp2_fast(s[n][e] - at), x[e + 2] = exp2_fast(s[n][e + 2] - at);
                 sum[n][e] += x[e] + x[e + 2];
             }
@@ -223,7 +228,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) paged_decode_kernel(const Page
             float to = -INFINITY;
 #pragma unroll
             for (int x = 0; x < kWarps; x++) to = fmaxf(to, s_ml[x][row].x);
-            const float by = m[n][e] == -INFINITY ? 0.0f : exp2_fast(m[n][e] - to);
+            const float by = m[n][e] == -INFINITY ? 0.0f : exp2_fast(m[n][e] - to - kUp);
 #pragma unroll
             for (int st = 0; st < kSteps; st++) {
                 float *at = join + (size_t)(warp * NT * 8 + row) * kJoin + st * 16 + (lane >> 2);
@@ -241,7 +246,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) paged_decode_kernel(const Page
 #pragma unroll
         for (int y = 0; y < kWarps; y++) {
             const float2 ml = s_ml[y][row];
-            total += ml.x == -INFINITY ? 0.0f : ml.y * exp2_fast(ml.x - to);
+            total += ml.x == -INFINITY ? 0.0f : ml.y * exp2_fast(ml.x - to - kUp);
             const float4 f = *reinterpret_cast<const float4 *>(join + (size_t)(y * NT * 8 + row) * kJoin + d);
             r.x += f.x, r.y += f.y, r.z += f.z, r.w += f.w;
         }

@@ -1,0 +1,55 @@
+"""Paged attention and append at the edges of their use."""
+import numpy as np
+import pytest
+
+import paged_plain as plain
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def paged():
+    from llamd_rs_b200 import backend, paged as p
+
+    backend.stream_init()
+    return p
+
+
+def dev(a):
+    from llamd_rs_b200.backend import DevBuf
+
+    return DevBuf.from_array(a)
+
+
+@pytest.mark.parametrize("n_seq,q_len,more", [(1, 1, 15), (230, 1, 15), (1, 40, 7), (150, 40, 7)])
+@pytest.mark.parametrize("nats", [11, 15, 17])
+@pytest.mark.parametrize("out_f32", [False, True])
+def test_many_small_weights(paged, n_seq, q_len, more, nats, out_f32):
+    """One key far above 131072 alike: each of their weights is small, their sum is not. The sequences hold the same pages; where there are many,
+    each is one piece, with one maximum.
+
+    The scores are exact, so an output is off by its own rounding, by the weights' (u of each, and half a step of f16's subnormals
+    where they end there: 2^-25, of weights scaled by 2^more) and by 2^-20 of f32 arithmetic."""
+    from llamd_rs_b200 import backend
+
+    n, H, D, page = 131072 + q_len, 8, 128, 64
+    n_pages = -(-n // page)
+    k, v = np.zeros((n_pages * page, D)), np.zeros((n_pages * page, D))
+    k[0, 0], v[0, 1::2], v[1:, ::2] = nats, 1, 1
+    q = np.zeros((n_seq, q_len, H, D))
+    q[..., 0] = 1
+    kp, vp = (dev(plain.to_bits(x.reshape(n_pages, 1, page, D), "f16")) for x in (k, v))
+    b = paged.Batch(H, 1, D, page, "f16")
+    b.set([q_len] * n_seq, [n] * n_seq, np.tile(np.arange(n_pages, dtype=np.int32), (n_seq, 1)), n_pages)
+    wide = np.uint32 if out_f32 else np.uint16
+    out = dev(np.zeros(q.shape, wide))
+    b.attention(dev(plain.to_bits(q, "f16")), kp, vp, out, scale=1.0, out_f32=out_f32)
+    backend.sync()
+    got = out.download(wide, q.size)
+    got = (got.view(np.float32).astype(np.float64) if out_f32 else plain.from_bits(got, "f16")).reshape(q.shape)
+    far = np.arange(n - q_len, n)[:, None, None] * np.exp(-float(nats))  # the small weights' sum, token by token
+    want = np.where(np.arange(D) % 2, 1, far) / (1 + far)
+    u, tiny = plain.U["f16"], plain.TINY["f16"]
+    rounded = 0.0 if out_f32 else u * want + tiny
+    bound = rounded + (u + 2.0 ** -20) * want + (n - 1) * tiny * 2.0 ** -more / (1 + far)
+    assert np.all(np.abs(got - want) <= bound), np.max(np.abs(got - want) / bound)
