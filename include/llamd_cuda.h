@@ -76,7 +76,7 @@ void llamd_fwd_set_batch_group(int g);
 void *llamd_fwd_stream(void);
 /* For callers whose buffers are in use on a stream of their own (a cudaStream_t; NULL: the legacy default stream): what is
  * enqueued through the library from here on waits for what that stream holds now, or the other way round. Neither waits on the
- * host. 0 / -1. */
+ * host. Between llamd_fwd_begin_capture and its end both do nothing: order the streams around the graph's launch. 0 / -1. */
 int llamd_fwd_wait_stream(void *other);
 int llamd_fwd_ready_stream(void *other);
 

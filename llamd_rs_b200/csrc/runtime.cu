@@ -23,6 +23,7 @@ static int g_err = 0;
 static std::string g_err_msg;
 static cudaGraph_t g_graph = nullptr;
 static cudaGraphExec_t g_graph_exec = nullptr;
+static bool g_capturing = false;            // between llamd_fwd_begin_capture and its end
 static cudaGraph_t g_kept_graph = nullptr;  // kept beside the current one (graph_swap)
 static cudaGraphExec_t g_kept_exec = nullptr;
 static void *g_scratch[8] = {};
@@ -224,6 +225,7 @@ void graph_swap() {
 int begin_capture_beside() {
     destroy_current_graph();
     LLAMD_TRY(cudaStreamBeginCapture(stream(), cudaStreamCaptureModeThreadLocal), "begin capture");
+    g_capturing = true;
     return 0;
 }
 
@@ -394,8 +396,10 @@ static int order_streams(cudaStream_t first, cudaStream_t after) {
     LLAMD_TRY(rc, "order streams");
     return 0;
 }
-int llamd_fwd_wait_stream(void *other) { return stream() ? order_streams((cudaStream_t)other, stream()) : -1; }
-int llamd_fwd_ready_stream(void *other) { return stream() ? order_streams(stream(), (cudaStream_t)other) : -1; }
+// While the library captures a graph of its own there is nothing to order: an event of another stream would end the capture, and one of the captured
+// stream would draw the other stream into it.
+int llamd_fwd_wait_stream(void *other) { return !stream() ? -1 : g_capturing ? 0 : order_streams((cudaStream_t)other, stream()); }
+int llamd_fwd_ready_stream(void *other) { return !stream() ? -1 : g_capturing ? 0 : order_streams(stream(), (cudaStream_t)other); }
 
 // Device-time stopwatch on the library stream (CUDA events).
 static cudaEvent_t g_t0 = nullptr, g_t1 = nullptr;
@@ -421,6 +425,7 @@ int llamd_fwd_begin_capture(void) {
 }
 int llamd_fwd_end_capture(void) {
     cudaGraph_t g = nullptr;
+    g_capturing = false;
     cudaError_t e = cudaStreamEndCapture(stream(), &g);
     if (e != cudaSuccess || !g) {
         set_error(e, "end capture");

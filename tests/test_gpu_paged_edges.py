@@ -53,3 +53,29 @@ def test_many_small_weights(paged, n_seq, q_len, more, nats, out_f32):
     rounded = 0.0 if out_f32 else u * want + tiny
     bound = rounded + (u + 2.0 ** -20) * want + (n - 1) * tiny * 2.0 ** -more / (1 + far)
     assert np.all(np.abs(got - want) <= bound), np.max(np.abs(got - want) / bound)
+
+
+def test_streams_are_not_ordered_inside_a_capture(paged):
+    """Events of or for another stream would end the capture, or draw that stream into it."""
+    torch = pytest.importorskip("torch")
+    from llamd_rs_b200 import backend
+    from llamd_rs_b200._lib import lib
+
+    side, L = torch.cuda.Stream(), lib()
+    a, c = dev(np.arange(256, dtype=np.float32)), dev(np.zeros(256, np.float32))
+    backend.sync()
+    assert L.llamd_fwd_begin_capture() == 0
+    paged.wait_for(side.cuda_stream)
+    L.llamd_fwd_add(a.ptr, a.ptr, c.ptr, 256)
+    paged.ready_for(side.cuda_stream)
+    assert L.llamd_fwd_end_capture() == 0
+    try:
+        assert not any(c.download_f32(256))
+        assert side.query() and L.llamd_fwd_graph_launch() == 0
+        backend.sync()
+        assert np.array_equal(c.download_f32(256), 2 * np.arange(256, dtype=np.float32))
+        paged.wait_for(side.cuda_stream)  # and they do again afterwards
+        paged.ready_for(side.cuda_stream)
+        side.synchronize()
+    finally:
+        L.llamd_fwd_graph_destroy()
