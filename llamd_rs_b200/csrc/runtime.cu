@@ -386,14 +386,13 @@ void llamd_fwd_set_pdl(int on) { g_pdl = on == 1 ? kPdlDefault : on; }
 void llamd_fwd_set_batch_group(int g) { g_batch_group = g < 0 ? 0 : g; }
 void *llamd_fwd_stream(void) { return (void *)stream(); }
 
-// `after` waits for what `first` holds now, through an event that the two need only here.
+// `after` waits for what `first` holds now. (One event serves all: a wait is for what the event stood for when it was enqueued.)
 static int order_streams(cudaStream_t first, cudaStream_t after) {
-    cudaEvent_t e = nullptr;
-    LLAMD_TRY(cudaEventCreateWithFlags(&e, cudaEventDisableTiming), "event create");
-    cudaError_t rc = cudaEventRecord(e, first);
-    if (rc == cudaSuccess) rc = cudaStreamWaitEvent(after, e, 0);
-    cudaEventDestroy(e);  // (kept by the driver until the wait is over)
-    LLAMD_TRY(rc, "order streams");
+    static cudaEvent_t e = nullptr;
+    if (first == after) return 0;
+    if (!e) LLAMD_TRY(cudaEventCreateWithFlags(&e, cudaEventDisableTiming), "event create");
+    LLAMD_TRY(cudaEventRecord(e, first), "order streams");
+    LLAMD_TRY(cudaStreamWaitEvent(after, e, 0), "order streams");
     return 0;
 }
 // While the library captures a graph of its own there is nothing to order: an event of another stream would end the capture, and one of the captured

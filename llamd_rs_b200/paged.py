@@ -4,12 +4,15 @@
 (``fork``). ``Batch`` is the shape of one step, set once and used by every layer: ``append`` norms, rotates and stores the new
 tokens, ``attention`` attends them. Buffers are the caller's, on the device: ``DevBuf``, a plain address, or anything with
 ``data_ptr()`` (a torch tensor), whose type, shape and strides are then checked. The calls enqueue on the library's stream
-and do not wait; a caller whose buffers are in use on another stream orders the two with ``wait_for`` and ``ready_for``.
+and do not wait. Where a tensor is among their buffers they order that stream with torch's current one, both ways: they read what the current stream
+has written when they are made, and it reads what they have written. A caller whose buffers are in use on any other stream orders the
+two with ``wait_for`` and ``ready_for``.
 """
 from __future__ import annotations
 
 import ctypes as C
 import math
+import sys
 
 import numpy as np
 
@@ -33,6 +36,16 @@ def _type_of(x):
     if t is None:
         t = _seen[x.dtype] = _TORCH.get(str(x.dtype), -1)
     return t
+
+
+def _stream_of(*buffers):
+    """torch's current stream (a cudaStream_t) where one of the buffers is a tensor, else None."""
+    for x in buffers:
+        if hasattr(x, "data_ptr") and x.is_cuda:
+            torch = sys.modules["torch"]
+            raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # (0.1 us; the public way makes an object of it, 2.4 us)
+            return raw(x.get_device()) if raw else torch.cuda.current_stream(x.device).cuda_stream
+    return None
 
 
 def _refuse(what):
@@ -112,6 +125,7 @@ class Batch:
             _refuse("paged batch")
         self.tokens, self.n_pages, self.scale = 0, 0, 1.0 / math.sqrt(head_dim)
         self._append, self._attention = lib().llamd_fwd_paged_append, lib().llamd_fwd_paged_attention
+        self._wait, self._ready = lib().llamd_fwd_wait_stream, lib().llamd_fwd_ready_stream
         self._pool = 0
 
     def set(self, q_lens, kv_lens, pages, n_pages: int, n_shared: int = 0) -> None:
@@ -132,6 +146,15 @@ class Batch:
             _refuse("paged batch")
         self.tokens, self.n_pages = int(q.sum()), n_pages
         self._pool = n_pages * self.n_head_kv * self.page_size * self.head_dim
+
+    def _call(self, what, call, stream, *args):
+        """One of the two calls, between the orders with the caller's stream where there is one."""
+        if stream is not None and self._wait(stream) != 0:
+            _refuse(what)
+        if call(self.ptr, *args) != 0:
+            _refuse(what)
+        if stream is not None and self._ready(stream) != 0:
+            _refuse(what)
 
     @staticmethod
     def _tensors(*wanted):
@@ -211,19 +234,17 @@ class Batch:
             plain = self._tensors((q, it, T * nq, T), (k, it, T * nk, T), (v, it, T * nk, T), (q_norm, 2, D, None), (k_norm, 2, D, None),
                                   (rope, 2, rope_rows * rot, None), (q_out, t, T * nq, T), (k_pages, t, self._pool, None), (v_pages, t, self._pool, None))
             if plain:
-                if self._append(self.ptr, plain[0], plain[1], plain[2], it, nq, nk, nk, plain[3], plain[4], eps, plain[5], rope_rows, rot, interleaved, plain[6],
-                                nq, plain[7], plain[8]) != 0:
-                    _refuse("append")
+                self._call("append", self._append, _stream_of(q), plain[0], plain[1], plain[2], it, nq, nk, nk, plain[3], plain[4], eps, plain[5], rope_rows, rot,
+                           interleaved, plain[6], nq, plain[7], plain[8])
                 return
         qp, qs = self._rows(q, nq, it, "q", strides[0])
         kp, ks = self._rows(k, nk, it, "k", strides[1])
         vp, vs = self._rows(v, nk, it, "v", strides[2])
         op, os_ = self._rows(q_out, nq, self.type, "q_out")
-        if self._append(self.ptr, qp, kp, vp, it, qs, ks, vs, None if q_norm is None else self._whole(q_norm, 2, D, "q_norm"),
-                        None if k_norm is None else self._whole(k_norm, 2, D, "k_norm"), eps, self._whole(rope, 2, rope_rows * rot, "rope") if rot else None,
-                        rope_rows, rot, interleaved, op, os_, self._whole(k_pages, self.type, self._pool, "k_pages"),
-                        self._whole(v_pages, self.type, self._pool, "v_pages")) != 0:
-            _refuse("append")
+        self._call("append", self._append, _stream_of(q, k, v, q_out, k_pages, v_pages, rope, q_norm, k_norm), qp, kp, vp, it, qs, ks, vs,
+                   None if q_norm is None else self._whole(q_norm, 2, D, "q_norm"), None if k_norm is None else self._whole(k_norm, 2, D, "k_norm"), eps,
+                   self._whole(rope, 2, rope_rows * rot, "rope") if rot else None, rope_rows, rot, interleaved, op, os_,
+                   self._whole(k_pages, self.type, self._pool, "k_pages"), self._whole(v_pages, self.type, self._pool, "v_pages"))
 
     def attention(self, q, k_pages, v_pages, out, scale: float | None = None, out_f32: bool | None = None) -> None:
         """llamd_fwd_paged_attention. ``out_f32`` says of an address that it takes f32; a tensor's type says so itself."""
@@ -234,14 +255,12 @@ class Batch:
         plain = self._tensors((q, self.type, self.tokens * n, self.tokens), (k_pages, self.type, self._pool, None), (v_pages, self.type, self._pool, None),
                               (out, 2 if out_f32 else self.type, self.tokens * n, self.tokens))
         if plain:
-            if self._attention(self.ptr, plain[0], n, plain[1], plain[2], plain[3], n, out_f32, scale) != 0:
-                _refuse("attention")
+            self._call("attention", self._attention, _stream_of(q), plain[0], n, plain[1], plain[2], plain[3], n, out_f32, scale)
             return
         qp, qs = self._rows(q, n, self.type, "q")
         op, os_ = self._rows(out, n, 2 if out_f32 else self.type, "out")
-        if self._attention(self.ptr, qp, qs, self._whole(k_pages, self.type, self._pool, "k_pages"), self._whole(v_pages, self.type, self._pool, "v_pages"), op, os_,
-                           out_f32, scale) != 0:
-            _refuse("attention")
+        kp, vp = self._whole(k_pages, self.type, self._pool, "k_pages"), self._whole(v_pages, self.type, self._pool, "v_pages")
+        self._call("attention", self._attention, _stream_of(q, k_pages, v_pages, out), qp, qs, kp, vp, op, os_, out_f32, scale)
 
     def free(self) -> None:
         if self.ptr:
@@ -263,10 +282,10 @@ def status() -> int:
 def wait_for(stream: int) -> None:
     """What is enqueued through the library from here on waits for what ``stream`` (a cudaStream_t) holds now."""
     if lib().llamd_fwd_wait_stream(C.c_void_p(stream)) != 0:
-        raise Other("wait_for: " + backend._last_error())
+        _refuse("wait_for")
 
 
 def ready_for(stream: int) -> None:
     """What is enqueued on ``stream`` from here on waits for what the library's stream holds now."""
     if lib().llamd_fwd_ready_stream(C.c_void_p(stream)) != 0:
-        raise Other("ready_for: " + backend._last_error())
+        _refuse("ready_for")

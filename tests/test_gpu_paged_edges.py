@@ -79,3 +79,32 @@ def test_streams_are_not_ordered_inside_a_capture(paged):
         side.synchronize()
     finally:
         L.llamd_fwd_graph_destroy()
+
+
+def test_tensors_of_another_stream(paged):
+    """Tensors that torch's current stream is still making, outputs that it reads right after the calls: nobody has to say so."""
+    torch = pytest.importorskip("torch")
+
+    H, K, D, page, n = 8, 2, 64, 16, 50
+    b = paged.Batch(H, K, D, page, "bf16")
+    b.set([n], [n], [list(range(4))], 4)
+    side = torch.cuda.Stream()
+    for stream in (side, torch.cuda.default_stream()):
+        with torch.cuda.stream(stream):
+            qkv = torch.randn(n, H + 2 * K, D, device="cuda").bfloat16()
+            source = qkv.clone()
+            kp, vp = (torch.zeros(4, K, page, D, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+            q, out = (torch.zeros(n, H, D, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+            torch.cuda.synchronize()
+            qkv.zero_()
+            torch.cuda._sleep(20_000_000)
+            qkv.copy_(source)  # (in front of this, and of the sleep before it, the calls would read zeros)
+            b.append(qkv[:, :H], qkv[:, H:H + K], qkv[:, H + K:], q, kp, vp)
+            qkv.zero_()        # (this must not come before they have read it)
+            b.attention(q, kp, vp, out)
+            got = [x.clone() for x in (q, kp, vp, out)]
+            torch.cuda.synchronize()
+        assert torch.equal(got[0], source[:, :H]) and torch.equal(got[1].transpose(1, 2).reshape(64, K, D)[:n], source[:, H:H + K])
+        x = source.double().cpu().numpy()
+        want, bound = plain.attention(x[:, :H], *(y.double().cpu().numpy() for y in got[1:3]), [list(range(4))], [n], [n], D ** -0.5, "bf16")
+        assert np.all(np.abs(got[3].double().cpu().numpy() - want) <= bound)
