@@ -714,9 +714,9 @@ int llamd_fwd_paged_attention(const void *batch, const void *q, size_t q_stride,
     a.out_f32 = out_f32, a.scale_log2 = scale * 1.4426950408889634f;
     a.part_o = (float *)b->partial, a.part_ml = (float2 *)(b->partial + b->partial_rows * g.hd * sizeof(float));
     if (b->beside) LLAMD_TRY(cudaEventRecord(g_fork, stream()), "paged attention: fork");
-    if (b->n_ctas) {  // (first: its CTAs need whole SMs)
+    if (b->n_ctas) {  // (first: its CTAs need whole SMs, and what it refuses leaves nothing launched)
         a.item = b->large;
-        paged_prompt_launch(a, b->type, b->n_pages, b->begin, b->n_ctas);
+        if (!paged_prompt_launch(a, b->type, b->n_pages, b->begin, b->n_ctas)) return -1;
     }
     if (b->n_small) {
         a.item = b->small;
@@ -727,6 +727,7 @@ int llamd_fwd_paged_attention(const void *batch, const void *q, size_t q_stride,
         LLAMD_TRY(cudaEventRecord(g_join, g_side), "paged attention: join");
         LLAMD_TRY(cudaStreamWaitEvent(stream(), g_join, 0), "paged attention: join");
     }
+    if (error_code()) return -1;  // (nothing joins what was not made)
     if (b->n_merge) paged_merge_launch(a, b->type, b->merge, b->part, b->n_merge, b->most, b->sms);
     return error_code() ? -1 : 0;
 }

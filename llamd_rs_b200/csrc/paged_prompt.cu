@@ -658,16 +658,19 @@ bool paged_prompt_ready() {
     return true;
 }
 
-void paged_prompt_launch(const PagedAttn &a, int type, int n_pages, const int32_t *begin, int n_ctas) {
+bool paged_prompt_launch(const PagedAttn &a, int type, int n_pages, const int32_t *begin, int n_ctas) {
     PromptParams p;
     p.a = a;
     p.begin = begin;
     p.wide = ((uintptr_t)a.out & 31) == 0 && a.out_stride * (a.out_f32 ? 4 : 2) % 32 == 0;
     p.status = g_status;
-    if (!query_map(&p.q, a, type) || !pool_map(&p.k, a.k_pages, type, a.b, n_pages) || !pool_map(&p.v, a.v_pages, type, a.b, n_pages)) 
-        return set_error_msg("paged_prompt: a tensor map was refused");
+    if (!query_map(&p.q, a, type) || !pool_map(&p.k, a.k_pages, type, a.b, n_pages) || !pool_map(&p.v, a.v_pages, type, a.b, n_pages)) {
+        set_error_msg("paged_prompt: a tensor map was refused");
+        return false;
+    }
     if (type == kPagedF16) a.b.hd == 128 ? prompt_launch<__half, 128>(p, n_ctas) : prompt_launch<__half, 64>(p, n_ctas);
     else a.b.hd == 128 ? prompt_launch<__nv_bfloat16, 128>(p, n_ctas) : prompt_launch<__nv_bfloat16, 64>(p, n_ctas);
+    return !error_code();
 }
 
 }  // namespace llamd

@@ -108,3 +108,25 @@ def test_tensors_of_another_stream(paged):
         x = source.double().cpu().numpy()
         want, bound = plain.attention(x[:, :H], *(y.double().cpu().numpy() for y in got[1:3]), [list(range(4))], [n], [n], D ** -0.5, "bf16")
         assert np.all(np.abs(got[3].double().cpu().numpy() - want) <= bound)
+
+
+def test_refused_attention_launches_nothing(paged):
+    """Rows of q further apart than a tensor map can say, behind a shared prefix, whose parts another launch joins: refused before any of them."""
+    from llamd_rs_b200 import backend
+    from llamd_rs_b200._lib import lib
+
+    L, H, D, n = lib(), 64, 128, 40
+    b = paged.Batch(H, 1, D, 16, "f16")
+    b.set([1], [n], [[0, 1, 2]], 3, 16)
+    rng = np.random.default_rng(0)
+    q, kp, vp = (plain.to_bits(rng.standard_normal(s), "f16") for s in ((1, H, D), (3, 1, 16, D), (3, 1, 16, D)))
+    dq, dk, dv, out = dev(q), dev(kp), dev(vp), dev(np.full((1, H, D), 7, np.uint16))
+    backend.sync()
+    before = L.llamd_fwd_launch_count()
+    assert L.llamd_fwd_paged_attention(b.ptr, dq.ptr, 1 << 40, dk.ptr, dv.ptr, out.ptr, H * D, 0, D ** -0.5) == -1  # (one row: nothing lies that far)
+    assert L.llamd_fwd_launch_count() == before and L.llamd_fwd_last_error() == -1
+    assert np.all(out.download(np.uint16, H * D) == 7)
+    b.attention(dq, dk, dv, out)
+    backend.sync()
+    want, bound = plain.attention(*(plain.from_bits(x, "f16") for x in (q, kp, vp)), [[0, 1, 2]], [1], [n], D ** -0.5, "f16")
+    assert np.all(np.abs(plain.from_bits(out.download(np.uint16, H * D), "f16").reshape(1, H, D) - want) <= bound)
