@@ -169,6 +169,7 @@ unsafe extern "C" {
     pub fn llamd_fwd_paged_append(batch: *const c_void, q: *const c_void, k: *const c_void, v: *const c_void, in_type: c_int, q_stride: usize, k_stride: usize, v_stride: usize, wq: *const f32, wk: *const f32, eps: f32, rope_tab: *const f32, rope_rows: c_int, rot: c_int, interleaved: c_int, q_out: *mut c_void, out_stride: usize, k_pages: *mut c_void, v_pages: *mut c_void) -> c_int;
     pub fn llamd_fwd_paged_attention(batch: *const c_void, q: *const c_void, q_stride: usize, k_pages: *const c_void, v_pages: *const c_void, out: *mut c_void, out_stride: usize, out_f32: c_int, scale: f32) -> c_int;
     pub fn llamd_fwd_paged_status() -> c_int;
+    pub fn llamd_fwd_paged_wait_limit(nanoseconds: c_ulonglong);
     pub fn llamd_cuda_rope_table_scaled(host_out: *mut f32, rows: c_int, rot: c_int, freq_base: f32, scaling: c_int, factor: f32, original: c_int) -> c_int;
 }
 

@@ -470,9 +470,12 @@ int llamd_fwd_paged_append(const void *batch, const void *q, const void *k, cons
  * 0 times infinity). Part of a large batch may run on a second stream of the library's, which the call joins to its own. 0 / -1 as above. */
 int llamd_fwd_paged_attention(const void *batch, const void *q, size_t q_stride, const void *k_pages, const void *v_pages, void *out,
                               size_t out_stride, int out_f32, float scale);
-/* 0 while every wait inside the attention's kernels has been met; otherwise 1 + the first block whose wait ran out (outputs are
- * then incomplete). Synchronises the stream. */
+/* 0 while every wait inside the attention's kernels has been met; otherwise 1 + the first block whose wait ran out, handed out once. Outputs that are
+ * then not complete are NaN, and append and attention refuse (cudaErrorTimeout) until it has been read. Synchronises the stream. */
 int llamd_fwd_paged_status(void);
+/* How long, in wall time, a wait inside the attention's kernels may take before the block gives up: 2 seconds unless it is set, for launches from here on. 0: the
+ * tensor-core kernel begins none and gives up all its pieces, with which a host can try out what it does then. */
+void llamd_fwd_paged_wait_limit(unsigned long long nanoseconds);
 /* The table of llamd_fwd_paged_append on the host: sine and cosine of r * f_i, f_i = base^(-2i / rot), evaluated in double.
  * scaling 0: as it is; 1: f / factor (positions stretched); 2: base * factor^(rot / (rot - 2)) in place of base; 3: by frequency,
  * f / factor for those that turn less than once over `original` positions, f for those that turn 32 times and more, a ramp

@@ -155,6 +155,7 @@ SIGNATURES = {
     "llamd_fwd_paged_append": (i32, [vp, vp, vp, vp, i32, sz, sz, sz, vp, vp, f32, vp, i32, i32, i32, vp, sz, vp, vp]),
     "llamd_fwd_paged_attention": (i32, [vp, vp, sz, vp, vp, vp, sz, i32, f32]),
     "llamd_fwd_paged_status": (i32, []),
+    "llamd_fwd_paged_wait_limit": (None, [C.c_ulonglong]),
     "llamd_cuda_rope_table_scaled": (i32, [vp, i32, i32, f32, i32, f32, i32]),
     "llamd_fwd_moe_group": (None, [vp, i32, i32, i32, vp, vp, vp, vp]),
     "llamd_fwd_moe_group_work": (None, [vp, i32, i32, i32, vp, vp, vp, vp, vp, vp]),

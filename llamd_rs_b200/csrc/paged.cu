@@ -558,6 +558,13 @@ void append_launch(AppendParams &p, bool interleaved, bool aligned) {
     else append_launch_hd<TI, T, 64>(p, interleaved, aligned);
 }
 
+// True and an error where an earlier attention gave up and nobody has read it: what reads its outputs, or works on beside them, has to know.
+bool gave_up() {
+    if (!paged_gave_up()) return false;
+    set_error(cudaErrorTimeout, "paged: a wait inside an earlier attention ran out, its outputs are NaN (llamd_fwd_paged_status reads and clears this)");
+    return true;
+}
+
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
 }  // namespace
@@ -668,6 +675,7 @@ int llamd_fwd_paged_append(const void *batch, const void *q, const void *k, cons
     const Batch *b = (const Batch *)batch;
     if (!b || !b->ready) return refuse("paged append: the batch is not set");
     if (error_code()) return -1;
+    if (gave_up()) return -1;
     const PagedView &g = b->view;
     if (!g.tokens) return 0;
     if (!q || !k || !v || !q_out || !k_pages || !v_pages) return refuse("paged append: a buffer is missing");
@@ -701,6 +709,7 @@ int llamd_fwd_paged_attention(const void *batch, const void *q, size_t q_stride,
     const Batch *b = (const Batch *)batch;
     if (!b || !b->ready) return refuse("paged attention: the batch is not set");
     if (error_code()) return -1;
+    if (gave_up()) return -1;
     const PagedView &g = b->view;
     if (!g.tokens) return 0;
     const size_t qd = (size_t)g.n_head * g.hd;

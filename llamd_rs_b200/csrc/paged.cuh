@@ -62,6 +62,7 @@ constexpr int kPagedSmallRows = 32, kPagedPieceRows = 16;
 
 void paged_decode_launch(const PagedAttn &p, int type, int n_items, int max_rows, cudaStream_t to);
 constexpr int kPagedTileRows = 128, kPagedBlock = 128;  // of paged_prompt.cu: two tiles of query rows to a piece, positions to a block
+bool paged_gave_up();       // a wait of an earlier attention has run out, and the host has not read it yet
 bool paged_prompt_ready();  // what its launches need beside the batch: false and an error where it cannot be had
 bool paged_prompt_launch(const PagedAttn &p, int type, int n_pages, const int32_t *begin, int n_ctas);  // begin: each CTA's pieces (n_ctas + 1); false and an error: not launched
 void paged_merge_launch(const PagedAttn &p, int type, const PagedMerge *merge, const PagedPart *parts, int n_merge, int most, int sms);  // most: parts of any of them

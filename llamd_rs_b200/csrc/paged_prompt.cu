@@ -22,7 +22,7 @@
 // first's 712k cycles: 128 scores out of TMEM, their maximum, exponentials, sums and roundings, to a thread and block, bound it. A piece costs 3 us to
 // begin and end: one prompt of 512 positions takes 12.7 us for 1.4 us of products.
 // Slots of the last block behind the last position are masked in S and set to zero in V's tile before the product reads it.
-// Every wait is bounded; one that runs out raises a flag that the host reads (llamd_fwd_paged_status).
+// Every wait is bounded; one that runs out raises a flag that the host reads (llamd_fwd_paged_status), and outputs that are not complete are NaN.
 #include <cuda.h>
 
 #include <type_traits>
@@ -52,13 +52,15 @@ template <int HD> struct Shape {
     static constexpr size_t kSmem = (kQueries + kStages) * (size_t)kTileBytes + sizeof(Rest);
 };
 constexpr int kHalfBytes = kM * 128;
+constexpr unsigned long long kDrainLimit = 2000000000ull;  // of what a block that has given up waits for, in nanoseconds
 
 struct PromptParams {
     PagedAttn a;
     const int32_t *begin;  // [CTAs + 1] each CTA's pieces of a.item
     CUtensorMap q, k, v;
     int wide;  // out's rows start at 32 bytes
-    int *status;
+    unsigned long long limit;  // nanoseconds that a wait may take; 0: every piece is given up
+    int *status;               // (host memory)
 };
 
 // The tokens of a piece's two tiles, and how many blocks each sees some of.
@@ -95,20 +97,20 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {  // (pa
     asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
     return done;
 }
-// Gives up after two seconds, or as soon as another warp has.
-__device__ __forceinline__ bool bar_wait_on(uint32_t bar, uint32_t parity, volatile int *abort) {
+// Gives up after `limit` nanoseconds, or as soon as another warp has.
+__device__ __forceinline__ bool bar_wait_on(uint32_t bar, uint32_t parity, volatile int *abort, unsigned long long limit) {
     const unsigned long long began = nanoseconds();
-    while (nanoseconds() - began < 2000000000ull) {
+    while (nanoseconds() - began < limit) {
         if (bar_try(bar, parity)) return true;
         if (*abort) return false;
     }
     *abort = 1;
     return false;
 }
-__device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity, volatile int *abort) {
+__device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity, volatile int *abort, unsigned long long limit) {
     const uint32_t a = smem_addr(bar);
     if (__builtin_expect(bar_try(a, parity), 1)) return true;
-    return bar_wait_on(a, parity, abort);
+    return bar_wait_on(a, parity, abort, limit);
 }
 __device__ __forceinline__ bool elect_one() {
     uint32_t p;
@@ -243,7 +245,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
             bar_init(&sh.empty[i], 1);
         }
         bar_init(&sh.drain, 1);
-        sh.abort = 0;
+        sh.abort = p.limit == 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kMmaWarp) {
@@ -255,6 +257,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
     fence_after();
     const uint32_t tmem = sh.tmem;
     pdl_wait();  // (the batch's own tables were complete before the launch in front of this one began)
+    int slot = 0, n_q = 0;  // the loading warp's: loads so far, tiles of Q so far
 
     if (warp >= kSoftmaxWarps) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
@@ -263,8 +266,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
             const int page = p.a.b.page, box = min(page, kN), shift = __ffs(page) - 1, boxes = kN / box;
             constexpr int kHalves = HD / 64;
             const int my_box = lane / kHalves, my_half = lane % kHalves;
-            int slot = 0, n_q = 0;  // loads so far, tiles of Q so far
-            bool ok = true;
+            bool ok = !sh.abort;
             for (int n = first; n < last && ok; n++) {
                 const PagedItem it = p.a.item[n];
                 const Tiles tl(it, per_tile);
@@ -281,7 +283,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
 #pragma unroll
                     for (int kv = 0; kv < 2; kv++) {
                         const int stage = slot % S::kStages, round = slot / S::kStages;
-                        if (round) ok = ok && bar_wait(&sh.empty[stage], (round - 1) & 1, &sh.abort);
+                        if (round) ok = ok && bar_wait(&sh.empty[stage], (round - 1) & 1, &sh.abort, p.limit);
                         ok = __all_sync(0xffffffffu, ok);
                         if (!ok) break;
                         if (lane == 0) bar_expect(&sh.full[stage], (uint32_t)(used * box * HD * 2));
@@ -294,7 +296,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                         for (int t = 0; t < 2; t++) {  // (heads of a group and tokens come as the tile's rows; what lies behind the piece's tokens is not used)
                             if (!tl.n_blk[t]) continue;
                             const int buf = n_q % S::kQueries, round = n_q / S::kQueries;
-                            if (round) ok = ok && bar_wait(&sh.q_empty[buf], (round - 1) & 1, &sh.abort);
+                            if (round) ok = ok && bar_wait(&sh.q_empty[buf], (round - 1) & 1, &sh.abort, p.limit);
                             ok = __all_sync(0xffffffffu, ok);
                             if (!ok) break;
                             if (lane == 0) bar_expect(&sh.q_full[buf], (uint32_t)(per_tile * group * HD * 2));
@@ -307,11 +309,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                     id = next;
                 }
             }
-            if (sh.abort) {  // given up: what is on its way still lands before the block ends
-                volatile int none = 0;
-                for (int i = max(0, slot - S::kStages); i < slot; i++) bar_wait(&sh.full[i % S::kStages], (i / S::kStages) & 1, &none);
-                for (int i = max(0, n_q - S::kQueries); i < n_q; i++) bar_wait(&sh.q_full[i % S::kQueries], (i / S::kQueries) & 1, &none);
-            }
         } else if (warp == kMmaWarp && elect_one()) {
             // ---- the products: one thread ----
             // instruction descriptors: f32 sums (bit 4), operand types (bits 7, 10), N >> 3 at bit 17, M >> 4 at bit 24; V transposed (bit 16)
@@ -320,7 +317,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
             // (its warp shares a scheduler with two softmax warps, and every instruction between two products is time that the tensor cores
             // may stand still: with the same steps taken by the whole warp, agreeing on each wait, a block took a tenth longer)
             auto wait = [&](uint64_t *bar, uint32_t parity) {
-                const bool done = bar_wait(bar, parity, &sh.abort);
+                const bool done = bar_wait(bar, parity, &sh.abort, p.limit);
                 fence_after();
                 return done;
             };
@@ -350,6 +347,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                     mma_ts(tmem + 2 * kN + t * HD, tmem + t * kN + step * 8, b + step * (16 * 128 >> 4), kO, more || step > 0);
             };
             auto pieces = [&]() {  // false: a wait ran out
+                if (sh.abort) return false;
                 Place k, v, q;
                 v.on(1);
                 uint32_t s_phase[2] = {0, 0}, o_phase[2] = {0, 0};
@@ -416,11 +414,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                 }
                 return true;
             };
-            if (!pieces()) {  // given up: products on their way end before TMEM is given back
-                mma_commit(&sh.drain);
-                volatile int none = 0;
-                bar_wait(&sh.drain, 0, &none);
-            }
+            pieces();
+            // (given up or not: every product has ended, and every arrival of its commits is there, before the block's memory is given back)
+            mma_commit(&sh.drain);
+            volatile int none = 0;
+            bar_wait(&sh.drain, 0, &none, kDrainLimit);
         }
     } else {
         // ---- softmax of tile t ----
@@ -428,8 +426,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
         const int t = warp >> 2, r = threadIdx.x & 127;
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), ts = lanes + t * kN, to = lanes + 2 * kN + t * HD;
         const float scale = p.a.scale_log2;
-        bool ok = true;
-        int base = 0, n_s = 0, n_q = 0;  // as the products' warp counts them
+        bool ok = !sh.abort;
+        int base = 0, n_s = 0, n_o = 0;  // as the products' warp counts them
         for (int n = first; n < last; n++) {
             const PagedItem it = p.a.item[n];
             const Tiles tl(it, per_tile);
@@ -439,7 +437,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
             const int mine = min(it.kv_end, it.limit + it.step * (t * per_tile + min(r, rows - 1) / group)) - it.kv_begin;
             const int clear = (int)(__reduce_min_sync(0xffffffffu, (unsigned)max(mine, 0)) / kN);  // blocks that all rows of the warp see whole
             for (int j = 0; j < n_blk; j++, n_s++) {
-                ok = ok && bar_wait(&sh.s[t], n_s & 1, &sh.abort);
+                ok = ok && bar_wait(&sh.s[t], n_s & 1, &sh.abort, p.limit);
                 ok = __all_sync(0xffffffffu, ok);
                 fence_after();
                 float s[kN];
@@ -509,7 +507,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                 const int valid = it.kv_end - it.kv_begin - j * kN;
                 if (__builtin_expect(valid < kN, 0)) {  // the last block: zeros in V's rows behind the last position (both tiles write the same zeros)
                     const int slot = base + 2 * j + 1, stage = slot % S::kStages;
-                    ok = ok && bar_wait(&sh.full[stage], (slot / S::kStages) & 1, &sh.abort);
+                    ok = ok && bar_wait(&sh.full[stage], (slot / S::kStages) & 1, &sh.abort, p.limit);
                     for (int x = valid * (HD / 8) + r; x < kN * (HD / 8); x += 128) {
                         const int row = x / (HD / 8), c = x % (HD / 8);
                         asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(skv + stage * S::kTileBytes + (c / 8) * kHalfBytes + row * 128 + (c & 7) * 16), "r"(0)
@@ -532,16 +530,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
             }
             base += 2 * tl.n_all;
             if (!n_tok) continue;
-            if (n_blk) ok = ok && bar_wait(&sh.o_full[t], n_q & 1, &sh.abort);
-            n_q += n_blk > 0;
+            if (n_blk) ok = ok && bar_wait(&sh.o_full[t], n_o & 1, &sh.abort, p.limit);
+            n_o += n_blk > 0;
             ok = __all_sync(0xffffffffu, ok);
             fence_after();
-            const bool live = ok && r < rows;
+            const bool live = r < rows;
             const int tok = t * per_tile + (live ? r / group : 0), g = live ? r % group : 0;
             const bool joined = it.part >= 0;
             const size_t part_row = (size_t)it.part + (size_t)tok * group + g;
             const size_t out_at = (size_t)(it.token + tok) * p.a.out_stride + (size_t)(it.head * group + g) * HD;
-            const float by = joined ? kDown : 1.0f / sum;
+            const float by = !ok ? NAN : joined ? kDown : 1.0f / sum;  // (a piece that is given up leaves NaN, and so does what it is joined to)
 #pragma unroll 1
             for (int c = 0; c < HD; c += 32) {
                 float o[32];
@@ -586,19 +584,25 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                 }
                 __syncwarp();  // (the next columns' load is the whole warp's)
             }
-            if (live && joined) p.a.part_ml[part_row] = make_float2(m == -INFINITY ? m : m * scale, sum * kDown);
+            if (live && joined) p.a.part_ml[part_row] = make_float2(m == -INFINITY ? m : m * scale, sum * by);
         }
     }
     fence_before();
     __syncthreads();
+    if (warp == kLoadWarp && sh.abort) {  // given up, by whichever warp: what is on its way still lands before the block ends
+        volatile int none = 0;
+        for (int i = max(0, slot - S::kStages); i < slot; i++) bar_wait(&sh.full[i % S::kStages], (i / S::kStages) & 1, &none, kDrainLimit);
+        for (int i = max(0, n_q - S::kQueries); i < n_q; i++) bar_wait(&sh.q_full[i % S::kQueries], (i / S::kQueries) & 1, &none, kDrainLimit);
+    }
     if (warp == kMmaWarp) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
     }
-    if (threadIdx.x == 0 && sh.abort) atomicCAS(p.status, 0, 1 + (int)blockIdx.x);
+    if (threadIdx.x == 0 && sh.abort) atomicCAS_system(p.status, 0, 1 + (int)blockIdx.x);
 }
 
-int *g_status = nullptr;  // device word, made with the first batch
+volatile int *g_status = nullptr;  // pinned host word, made with the first batch: the kernel's 1 + the first block that gave up
+unsigned long long g_limit = 2000000000ull;
 
 typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
                                 const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -646,13 +650,16 @@ void prompt_launch(const PromptParams &p, int n_ctas) {
 
 }  // namespace
 
+bool paged_gave_up() { return g_status && *g_status; }
+
 bool paged_prompt_ready() {
     if (!g_status) {
         int *p = nullptr;
-        if (cudaMalloc(&p, sizeof(int)) != cudaSuccess || cudaMemsetAsync(p, 0, sizeof(int), stream()) != cudaSuccess) {
+        if (cudaHostAlloc((void **)&p, sizeof(int), cudaHostAllocMapped) != cudaSuccess) {
             set_error(cudaGetLastError(), "paged_prompt status word");
             return false;
         }
+        *p = 0;
         g_status = p;
     }
     return true;
@@ -663,7 +670,8 @@ bool paged_prompt_launch(const PagedAttn &a, int type, int n_pages, const int32_
     p.a = a;
     p.begin = begin;
     p.wide = ((uintptr_t)a.out & 31) == 0 && a.out_stride * (a.out_f32 ? 4 : 2) % 32 == 0;
-    p.status = g_status;
+    p.limit = g_limit;
+    p.status = const_cast<int *>(g_status);
     if (!query_map(&p.q, a, type) || !pool_map(&p.k, a.k_pages, type, a.b, n_pages) || !pool_map(&p.v, a.v_pages, type, a.b, n_pages)) {
         set_error_msg("paged_prompt: a tensor map was refused");
         return false;
@@ -675,12 +683,20 @@ bool paged_prompt_launch(const PagedAttn &a, int type, int n_pages, const int32_
 
 }  // namespace llamd
 
-// 0 while every wait inside the prompt attention has completed; otherwise 1 + the first piece whose wait ran out (its outputs were not
-// written). Synchronises the stream.
-extern "C" int llamd_fwd_paged_status(void) {
-    using namespace llamd;
+using namespace llamd;
+
+extern "C" {
+
+// 0 while every wait inside the prompt attention has been met; otherwise 1 + the first block that gave up, and its pieces' outputs, and what they are
+// joined to, are NaN. Synchronises the stream; a value is handed out once.
+int llamd_fwd_paged_status(void) {
     if (!g_status) return 0;
-    int h = 0;
-    if (cudaMemcpyAsync(&h, g_status, sizeof(int), cudaMemcpyDeviceToHost, stream()) != cudaSuccess || cudaStreamSynchronize(stream()) != cudaSuccess) return -1;
+    if (cudaStreamSynchronize(stream()) != cudaSuccess) return -1;
+    const int h = *g_status;
+    *g_status = 0;
     return h;
 }
+
+void llamd_fwd_paged_wait_limit(unsigned long long nanoseconds) { g_limit = nanoseconds; }
+
+}  // extern "C"

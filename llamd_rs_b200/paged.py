@@ -275,8 +275,16 @@ class Batch:
 
 
 def status() -> int:
-    """0 while every bounded wait inside the attention has been met (llamd_fwd_paged_status; waits for the stream)."""
+    """0 while every bounded wait inside the attention has been met; a failure is handed out once, and append and attention refuse until it has been read
+    (llamd_fwd_paged_status; waits for the stream)."""
     return int(lib().llamd_fwd_paged_status())
+
+
+def wait_limit(seconds: float) -> None:
+    """How long a wait inside the attention may take (2 s unless it is set); 0: its tensor-core kernel gives up at once (llamd_fwd_paged_wait_limit)."""
+    if not 0 <= seconds < 1e9:
+        raise Malformed(f"a limit of {seconds} seconds")
+    lib().llamd_fwd_paged_wait_limit(int(round(seconds * 1e9)))
 
 
 def wait_for(stream: int) -> None:

@@ -130,3 +130,73 @@ def test_refused_attention_launches_nothing(paged):
     backend.sync()
     want, bound = plain.attention(*(plain.from_bits(x, "f16") for x in (q, kp, vp)), [[0, 1, 2]], [1], [n], D ** -0.5, "f16")
     assert np.all(np.abs(plain.from_bits(out.download(np.uint16, H * D), "f16").reshape(1, H, D) - want) <= bound)
+
+
+@pytest.mark.parametrize("dtype,out_f32", [("f16", False), ("bf16", True)])
+@pytest.mark.parametrize("q_len,kv_len,n_shared", [([90, 300], [90, 900], 0), ([60, 1, 90], [1728, 1618, 1708], 1600), ([1] * 40, [6001] * 40, 6000)])
+def test_given_up(paged, dtype, out_f32, q_len, kv_len, n_shared):
+    """Waits that may take no time: every row of the tensor-core kernel, or that joins one of its parts, is NaN, the status says so once, calls refuse
+    until it has been read, and then all is as before."""
+    from llamd_rs_b200 import backend
+
+    H, D, page = 8, 128, 16
+    rng = np.random.default_rng(1)
+    first, n_pages, tables = list(range(n_shared // page)), n_shared // page, []
+    for m in kv_len:
+        own = -(-m // page) - n_shared // page
+        tables.append(first + list(range(n_pages, n_pages + own)))
+        n_pages += own
+    b = paged.Batch(H, 1, D, page, dtype)
+    b.set(q_len, kv_len, tables, n_pages, n_shared)
+    T, wide = b.tokens, np.uint32 if out_f32 else np.uint16
+    q, kp, vp = (plain.to_bits(rng.standard_normal(s), dtype) for s in ((T, H, D), (n_pages, 1, page, D), (n_pages, 1, page, D)))
+    dq, dk, dv, out = dev(q), dev(kp), dev(vp), dev(np.zeros((T, H, D), wide))
+
+    def result():
+        got = out.download(wide, T * H * D)
+        return (got.view(np.float32).astype(np.float64) if out_f32 else plain.from_bits(got, dtype)).reshape(T, H, D)
+
+    want, bound = plain.attention(*(plain.from_bits(x, dtype) for x in (q, kp, vp)), tables, q_len, kv_len, D ** -0.5, dtype)
+    b.attention(dq, dk, dv, out, out_f32=out_f32)
+    backend.sync()
+    assert np.all(np.abs(result() - want) <= bound) and paged.status() == 0
+    paged.wait_limit(0)
+    try:
+        b.attention(dq, dk, dv, out, out_f32=out_f32)
+    finally:
+        paged.wait_limit(2)
+    backend.sync()
+    assert np.all(np.isnan(result()))
+    for _ in range(2):
+        with pytest.raises(paged.Other, match="ran out"):
+            b.attention(dq, dk, dv, out, out_f32=out_f32)
+    with pytest.raises(paged.Other, match="ran out"):
+        b.append(dq, dq, dq, dq, dk, dv, inputs=dtype)
+    assert paged.status() > 0 and paged.status() == 0
+    b.attention(dq, dk, dv, out, out_f32=out_f32)
+    backend.sync()
+    assert np.all(np.abs(result() - want) <= bound) and paged.status() == 0
+
+
+def test_given_up_beside_the_decode_kernel(paged):
+    """A batch of which the decode kernel takes some sequences by itself: those are right, the others NaN."""
+    from llamd_rs_b200 import backend
+
+    H, D, page, q_len, kv_len = 8, 128, 16, [1, 400, 2], [20, 400, 33]
+    rng = np.random.default_rng(2)
+    tables = [[0, 1], list(range(2, 27)), [27, 28, 29]]
+    b = paged.Batch(H, 1, D, page, "f16")
+    b.set(q_len, kv_len, tables, 30)
+    q, kp, vp = (plain.to_bits(rng.standard_normal(s), "f16") for s in ((403, H, D), (30, 1, page, D), (30, 1, page, D)))
+    out = dev(np.zeros(q.shape, np.uint16))
+    paged.wait_limit(0)
+    try:
+        b.attention(dev(q), dev(kp), dev(vp), out)
+    finally:
+        paged.wait_limit(2)
+    backend.sync()
+    assert paged.status() > 0 and paged.status() == 0
+    got = plain.from_bits(out.download(np.uint16, q.size), "f16").reshape(q.shape)
+    want, bound = plain.attention(*(plain.from_bits(x, "f16") for x in (q, kp, vp)), tables, q_len, kv_len, D ** -0.5, "f16")
+    assert np.all(np.isnan(got[1:401]))
+    assert np.all(np.abs(got - want)[[0, 401, 402]] <= bound[[0, 401, 402]])
