@@ -450,7 +450,7 @@ void llamd_cuda_paged_free(void *batch);
  * ceil(kv_len / page_size) are read. q_len may be 0. n_shared: the first n_shared positions (whole pages, the same ids in every
  * table) are common to all sequences, no sequence has new tokens among them, and attention reads them once for all. Everything is
  * checked here, before a launch can use it: 0, or -1 and a message, and the batch is as it was (where memory could not be had: not
- * set). Enqueues one copy; may allocate where a batch is larger than any before it; not while a graph is captured, but what it has set may
+ * set). Enqueues one copy; may allocate where a batch is larger than any before it; refused while a graph is captured, but what it has set may
  * be used in one. A batch that is set again serves the launches enqueued
  * after the call; a graph that was captured with it is not replayed any more. */
 int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int32_t *kv_len, const int32_t *pages, int pages_stride,

@@ -12,6 +12,7 @@ namespace llamd {
 // One stream for every device-pointer op, as in the reference's device layer
 // (crates/llamd-rocm/kernels/llamd_forward.hip:701-716).
 cudaStream_t stream();
+bool capturing();  // a graph is being captured from it, by the library or by a stream that it has been ordered behind
 // Sticky error state: the first failure is kept until read.
 void set_error(cudaError_t e, const char *what);
 void set_error_msg(const char *what);

@@ -603,6 +603,7 @@ int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int
                          int n_shared) {
     Batch *b = (Batch *)batch;
     if (!b) return refuse("paged batch: null");
+    if (capturing()) return refuse("paged batch: not set while a graph is captured");
     if (const char *why = check_lengths(*b, n_seq, q_len, kv_len, pages, pages_stride, n_pages, n_shared)) return refuse(why);
     PagedView v = b->view;
     v.n_seq = n_seq, v.n_shared = n_shared, v.tokens = 0, v.table_stride = 1;

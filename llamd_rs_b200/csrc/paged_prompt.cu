@@ -654,6 +654,10 @@ bool paged_gave_up() { return g_status && *g_status; }
 
 bool paged_prompt_ready() {
     if (!g_status) {
+        if (capturing()) {
+            set_error_msg("paged batch: the first is not made while a graph is captured");
+            return false;
+        }
         int *p = nullptr;
         if (cudaHostAlloc((void **)&p, sizeof(int), cudaHostAllocMapped) != cudaSuccess) {
             set_error(cudaGetLastError(), "paged_prompt status word");

@@ -174,6 +174,11 @@ cudaStream_t stream() {
     return g_stream;
 }
 
+bool capturing() {
+    cudaStreamCaptureStatus now = cudaStreamCaptureStatusNone;
+    return g_stream && (cudaStreamIsCapturing(g_stream, &now) != cudaSuccess || now != cudaStreamCaptureStatusNone);
+}
+
 void set_error(cudaError_t e, const char *what) {
     if (g_err == 0) {
         g_err = (int)e;

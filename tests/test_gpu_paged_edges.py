@@ -200,3 +200,30 @@ def test_given_up_beside_the_decode_kernel(paged):
     want, bound = plain.attention(*(plain.from_bits(x, "f16") for x in (q, kp, vp)), tables, q_len, kv_len, D ** -0.5, "f16")
     assert np.all(np.isnan(got[1:401]))
     assert np.all(np.abs(got - want)[[0, 401, 402]] <= bound[[0, 401, 402]])
+
+
+def test_set_inside_a_capture_is_refused(paged):
+    """The batch stays as it was, and the capture goes on."""
+    from llamd_rs_b200 import backend
+    from llamd_rs_b200._lib import lib
+
+    L, H, D = lib(), 8, 64
+    rng = np.random.default_rng(4)
+    q, kp, vp = (plain.to_bits(rng.standard_normal(s), "f16") for s in ((2, H, D), (2, 1, 16, D), (2, 1, 16, D)))
+    dq, dk, dv, out = dev(q), dev(kp), dev(vp), dev(np.zeros((2, H, D), np.uint16))
+    b = paged.Batch(H, 1, D, 16, "f16")
+    b.set([2], [20], [[1, 0]], 2)
+    backend.sync()
+    assert L.llamd_fwd_begin_capture() == 0
+    for tables in ([[0, 1]], [[1, 0]]):
+        with pytest.raises(paged.Malformed, match="captured"):
+            b.set([1], [18], tables, 2)
+    b.attention(dq, dk, dv, out)
+    assert L.llamd_fwd_end_capture() == 0
+    try:
+        assert L.llamd_fwd_graph_launch() == 0
+        backend.sync()
+    finally:
+        L.llamd_fwd_graph_destroy()
+    want, bound = plain.attention(*(plain.from_bits(x, "f16") for x in (q, kp, vp)), [[1, 0]], [2], [20], D ** -0.5, "f16")
+    assert np.all(np.abs(plain.from_bits(out.download(np.uint16, q.size), "f16").reshape(q.shape) - want) <= bound)
