@@ -444,13 +444,14 @@ void llamd_fwd_attention_prefill(const float *q, const float *kc, const float *v
 /* hd 64 or 128; n_head up to 4096, n_head / n_head_kv a whole number up to 64; page_size a power of two, 16 to 4096; type (of q_out, out and the
  * pools) LLAMD_PAGED_F16 or _BF16. NULL and a message where refused. */
 void *llamd_cuda_paged_new(int n_head, int n_head_kv, int hd, int page_size, int type);
-/* Launches that read the batch may still be under way. The library keeps some of the batch's memory for the next one. */
+/* Launches that read the batch may still be under way, a graph may be captured meanwhile: nothing is waited for. The library keeps the batch's memory (up to
+ * 1 GB on the device, 256 MB pinned) for the next ones. Any thread. */
 void llamd_cuda_paged_free(void *batch);
 /* pages: [n_seq][pages_stride], ids below n_pages (the pools' size), of each sequence the first
  * ceil(kv_len / page_size) are read. q_len may be 0. n_shared: the first n_shared positions (whole pages, the same ids in every
  * table) are common to all sequences, no sequence has new tokens among them, and attention reads them once for all. Everything is
  * checked here, before a launch can use it: 0, or -1 and a message, and the batch is as it was (where memory could not be had: not
- * set). Enqueues one copy; may allocate where a batch is larger than any before it; refused while a graph is captured, but what it has set may
+ * set). Enqueues one copy; may allocate, or give memory back, where a batch is more than twice as large as those before it; refused while a graph is captured, but what it has set may
  * be used in one. A batch that is set again serves the launches enqueued
  * after the call; a graph that was captured with it is not replayed any more. */
 int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int32_t *kv_len, const int32_t *pages, int pages_stride,

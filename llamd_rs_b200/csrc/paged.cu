@@ -11,6 +11,7 @@
 #include <vector>
 
 #include "paged.cuh"
+#include "paged_keep.h"
 
 namespace llamd {
 namespace {
@@ -30,42 +31,28 @@ bool side_ready() {
     return g_side && g_fork && g_join;
 }
 
-// Memory of batches that are gone, for the next ones: a host that makes a batch for every step would otherwise pin and free for milliseconds each
-// time. Kept device memory needs no wait: whatever still reads it is in front of the next batch's copy on the same stream.
-struct Kept {
-    static constexpr size_t kMost = 6, kLargest = 32 << 20;
-    std::vector<std::pair<uint8_t *, size_t>> blocks;
-    // The smallest that n bytes fit in, or null.
-    uint8_t *take(size_t n, size_t &have) {
-        size_t best = blocks.size();
-        for (size_t i = 0; i < blocks.size(); i++)
-            if (blocks[i].second >= n && (best == blocks.size() || blocks[i].second < blocks[best].second)) best = i;
-        if (best == blocks.size()) return nullptr;
-        uint8_t *p = blocks[best].first;
-        have = blocks[best].second;
-        blocks.erase(blocks.begin() + best);
-        return p;
+// Device memory needs no event: whatever still reads it is in front of the next batch's copy on the same stream. Pinned memory goes with the event behind
+// the copy out of it.
+Kept g_device(16, (size_t)1 << 30), g_pinned(16, (size_t)256 << 20);
+
+// What the two had no room for goes back to the system. Not where a batch is freed: that may be inside a capture, on any thread, and is not to wait.
+void give_back() {
+    const std::vector<KeptBlock> dev = g_device.gone(), host = g_pinned.gone();
+    if (!dev.empty()) cudaStreamSynchronize(stream());  // (launches that read it are done)
+    for (const KeptBlock &b : dev) cudaFree(b.p);
+    for (const KeptBlock &b : host) {
+        cudaEventSynchronize((cudaEvent_t)b.event);
+        cudaFreeHost(b.p);
+        cudaEventDestroy((cudaEvent_t)b.event);
     }
-    bool keep(uint8_t *p, size_t n) {
-        if (blocks.size() >= kMost || n > kLargest) return false;
-        try {
-            blocks.push_back({p, n});
-        } catch (const std::exception &) {
-            return false;
-        }
-        return true;
-    }
-};
-Kept g_device, g_pinned;
+}
 
 struct Batch {
     PagedView view = {};
     int type = 0, n_pages = 0, max_kv = 0, sms = 0;
     bool ready = false;
-    // the device copy of everything below, and the pinned memory it is made in
-    uint8_t *dev = nullptr, *host = nullptr;
-    size_t dev_bytes = 0, host_bytes = 0;
-    cudaEvent_t copied = nullptr;
+    // the device copy of everything below, and the pinned memory it is made in, with the event behind the copy
+    KeptBlock dev, host;
     // attention's pieces (device addresses in `dev`) and the partial results that they leave
     const PagedItem *small = nullptr, *large = nullptr;  // for paged_decode.cu and paged_prompt.cu
     const int32_t *begin = nullptr;                      // large: each CTA's
@@ -73,56 +60,52 @@ struct Batch {
     const PagedPart *part = nullptr;
     bool beside = false;
     int n_small = 0, small_rows = 0, n_ctas = 0, n_merge = 0, most = 0;
-    uint8_t *partial = nullptr;
-    size_t partial_bytes = 0, partial_rows = 0;
+    KeptBlock partial;
+    size_t partial_rows = 0;
 
     ~Batch() {
-        if (copied) cudaEventSynchronize(copied);
-        drop(dev, dev_bytes);
-        drop(partial, partial_bytes);
-        drop_host();
-        if (copied) cudaEventDestroy(copied);
+        drop(g_device, dev), drop(g_device, partial), drop(g_pinned, host);
     }
-    void drop(uint8_t *&p, size_t &n) {
-        if (p && !g_device.keep(p, n)) {
-            cudaStreamSynchronize(stream());  // (launches that read it are done)
-            cudaFree(p);
-        }
-        p = nullptr, n = 0;
-    }
-    void drop_host() {  // (not before the copy out of it is done)
-        if (host && !g_pinned.keep(host, host_bytes)) cudaFreeHost(host);
-        host = nullptr, host_bytes = 0;
+    static void drop(Kept &to, KeptBlock &b) {
+        if (b.p) to.keep(b);
+        b = {};
     }
     // A device buffer of n bytes at least; what was in it is lost where it grows.
-    bool grow(uint8_t *&p, size_t &have, size_t n) {
-        if (n <= have) return true;
-        drop(p, have);
-        if ((p = g_device.take(n, have))) return true;
-        n = std::max<size_t>(n, 1 << 16);
-        if (cudaMalloc((void **)&p, n) != cudaSuccess) {
-            p = nullptr;
+    bool grow(KeptBlock &b, size_t n) {
+        if (n <= b.n) return true;
+        drop(g_device, b);
+        b = g_device.take(n);
+        if (b.p) return true;
+        n = Kept::rounded(n);
+        if (cudaMalloc((void **)&b.p, n) != cudaSuccess) {
+            b = {};
             return fail("paged batch: device memory");
         }
-        have = n;
+        b.n = n;
+        return true;
+    }
+    bool grow_pinned(size_t n) {
+        if (n <= host.n) return true;
+        drop(g_pinned, host);
+        host = g_pinned.take(n);
+        if (host.p) return true;
+        n = Kept::rounded(n);
+        cudaEvent_t copied;
+        if (cudaEventCreateWithFlags(&copied, cudaEventDisableTiming) != cudaSuccess) return fail("paged batch: event");
+        if (cudaHostAlloc((void **)&host.p, n, cudaHostAllocDefault) != cudaSuccess) {
+            host = {};
+            cudaEventDestroy(copied);
+            return fail("paged batch: pinned memory");
+        }
+        host.n = n, host.event = copied;
         return true;
     }
     // Room for n bytes on both sides and for `rows` partial results; the pinned side is not written before the copy out of it is done.
     bool reserve(size_t n, size_t rows) {
-        if (!copied && cudaEventCreateWithFlags(&copied, cudaEventDisableTiming) != cudaSuccess) return fail("paged batch: event");
-        if (cudaEventSynchronize(copied) != cudaSuccess) return fail("paged batch: previous copy");
-        if (n > host_bytes) {
-            drop_host();
-            if (!(host = g_pinned.take(n, host_bytes))) {
-                const size_t want = std::max<size_t>(2 * n, 1 << 16);
-                if (cudaHostAlloc((void **)&host, want, cudaHostAllocDefault) != cudaSuccess) {
-                    host = nullptr;
-                    return fail("paged batch: pinned memory");
-                }
-                host_bytes = want;
-            }
-        }
-        return (n <= dev_bytes || grow(dev, dev_bytes, 2 * n)) && grow(partial, partial_bytes, rows * (view.hd * sizeof(float) + sizeof(float2)));
+        give_back();
+        if (!grow_pinned(n)) return false;
+        if (cudaEventSynchronize((cudaEvent_t)host.event) != cudaSuccess) return fail("paged batch: previous copy");
+        return grow(dev, n) && grow(partial, rows * (view.hd * sizeof(float) + sizeof(float2)));
     }
     bool fail(const char *what) {
         set_error(cudaGetLastError(), what);
@@ -633,15 +616,15 @@ int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int
     b->ready = false;  // (from here on what the batch held is being replaced)
     if (!b->reserve(std::max<size_t>(bytes, 16), plan.rows)) return -1;
     auto put = [&](size_t at, const void *from, size_t n) {
-        if (n) memcpy(b->host + at, from, n);
+        if (n) memcpy(b->host.p + at, from, n);
     };
     put(o_small, plan.small.data(), plan.small.size() * sizeof(PagedItem));
     put(o_large, plan.large.data(), plan.large.size() * sizeof(PagedItem));
     put(o_begin, plan.begin.data(), plan.begin.size() * sizeof(int32_t));
     put(o_merge, plan.merge.data(), plan.merge.size() * sizeof(PagedMerge));
     put(o_part, plan.part.data(), plan.part.size() * sizeof(PagedPart));
-    PagedToken *token = (PagedToken *)(b->host + o_token);
-    int32_t *seq = (int32_t *)(b->host + o_seq), *table = (int32_t *)(b->host + o_table);
+    PagedToken *token = (PagedToken *)(b->host.p + o_token);
+    int32_t *seq = (int32_t *)(b->host.p + o_seq), *table = (int32_t *)(b->host.p + o_table);
     for (int s = 0, t = 0; s < n_seq; s++) {
         const int32_t *from = pages + (size_t)s * pages_stride;
         const int used = (kv_len[s] + v.page - 1) / v.page;
@@ -651,21 +634,21 @@ int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int
             seq[t] = s;
         }
     }
-    b->small = (const PagedItem *)(b->dev + o_small);
-    b->large = (const PagedItem *)(b->dev + o_large);
-    b->begin = (const int32_t *)(b->dev + o_begin);
-    b->merge = (const PagedMerge *)(b->dev + o_merge);
-    b->part = (const PagedPart *)(b->dev + o_part);
+    b->small = (const PagedItem *)(b->dev.p + o_small);
+    b->large = (const PagedItem *)(b->dev.p + o_large);
+    b->begin = (const int32_t *)(b->dev.p + o_begin);
+    b->merge = (const PagedMerge *)(b->dev.p + o_merge);
+    b->part = (const PagedPart *)(b->dev.p + o_part);
     b->beside = plan.beside;
     b->n_small = (int)plan.small.size(), b->small_rows = plan.small_rows, b->n_ctas = (int)plan.begin.size() - 1, b->n_merge = (int)plan.merge.size(), b->most = plan.most;
     b->partial_rows = plan.rows;
     b->n_pages = n_pages, b->max_kv = max_kv;
-    v.token = (const PagedToken *)(b->dev + o_token);
-    v.token_seq = (const int32_t *)(b->dev + o_seq);
-    v.table = (const int32_t *)(b->dev + o_table);
+    v.token = (const PagedToken *)(b->dev.p + o_token);
+    v.token_seq = (const int32_t *)(b->dev.p + o_seq);
+    v.table = (const int32_t *)(b->dev.p + o_table);
     b->view = v;
-    LLAMD_TRY(cudaMemcpyAsync(b->dev, b->host, bytes, cudaMemcpyHostToDevice, stream()), "paged batch: copy");
-    LLAMD_TRY(cudaEventRecord(b->copied, stream()), "paged batch: event");
+    LLAMD_TRY(cudaMemcpyAsync(b->dev.p, b->host.p, bytes, cudaMemcpyHostToDevice, stream()), "paged batch: copy");
+    LLAMD_TRY(cudaEventRecord((cudaEvent_t)b->host.event, stream()), "paged batch: event");
     b->ready = true;
     return 0;
 }
@@ -722,7 +705,7 @@ int llamd_fwd_paged_attention(const void *batch, const void *q, size_t q_stride,
     PagedAttn a = {};
     a.b = g, a.q = q, a.k_pages = k_pages, a.v_pages = v_pages, a.out = out, a.q_stride = q_stride, a.out_stride = out_stride;
     a.out_f32 = out_f32, a.scale_log2 = scale * 1.4426950408889634f;
-    a.part_o = (float *)b->partial, a.part_ml = (float2 *)(b->partial + b->partial_rows * g.hd * sizeof(float));
+    a.part_o = (float *)b->partial.p, a.part_ml = (float2 *)(b->partial.p + b->partial_rows * g.hd * sizeof(float));
     if (b->beside) LLAMD_TRY(cudaEventRecord(g_fork, stream()), "paged attention: fork");
     if (b->n_ctas) {  // (first: its CTAs need whole SMs, and what it refuses leaves nothing launched)
         a.item = b->large;

@@ -227,3 +227,57 @@ def test_set_inside_a_capture_is_refused(paged):
         L.llamd_fwd_graph_destroy()
     want, bound = plain.attention(*(plain.from_bits(x, "f16") for x in (q, kp, vp)), [[1, 0]], [2], [20], D ** -0.5, "f16")
     assert np.all(np.abs(plain.from_bits(out.download(np.uint16, q.size), "f16").reshape(q.shape) - want) <= bound)
+
+
+def large_batch(paged):
+    """A batch whose partial results are some 40 MB: 1280 sequences behind a shared prefix."""
+    b = paged.Batch(32, 4, 128, 16, "f16")
+    b.set([1] * 1280, [2049] * 1280, np.tile(np.arange(129, dtype=np.int32), (1280, 1)), 129, 2048)
+    return b
+
+
+def test_memory_of_large_batches_is_kept(paged):
+    """A batch made and given back every step: from the second on nothing is allocated or returned."""
+    from llamd_rs_b200 import backend
+
+    large_batch(paged).free()
+    at = []
+    for _ in range(3):
+        b = large_batch(paged)
+        at.append(backend.free_memory())
+        b.free()
+        at.append(backend.free_memory())
+    assert len(set(at)) == 1
+
+
+def test_free_waits_for_nothing_and_may_be_inside_a_capture(paged):
+    torch = pytest.importorskip("torch")
+    import time
+
+    from llamd_rs_b200 import backend
+    from llamd_rs_b200._lib import lib
+
+    L = lib()
+    batches = [large_batch(paged)] + [paged.Batch(8, 2, 64, 16) for _ in range(12)]
+    for b in batches[1:]:
+        b.set([1], [1], [[0]], 1)
+    backend.sync()
+    a, c = dev(np.arange(256, dtype=np.float32)), dev(np.zeros(256, np.float32))
+    with torch.cuda.stream(torch.cuda.ExternalStream(L.llamd_fwd_stream())):
+        torch.cuda._sleep(1_000_000_000)  # half a second
+    t = time.perf_counter()
+    for b in batches[:6]:
+        b.free()
+    assert time.perf_counter() - t < 0.1
+    backend.sync()
+    assert L.llamd_fwd_begin_capture() == 0
+    for b in batches[6:]:
+        b.free()
+    L.llamd_fwd_add(a.ptr, a.ptr, c.ptr, 256)
+    assert L.llamd_fwd_end_capture() == 0
+    try:
+        assert L.llamd_fwd_graph_launch() == 0
+        backend.sync()
+        assert np.array_equal(c.download_f32(256), 2 * np.arange(256, dtype=np.float32))
+    finally:
+        L.llamd_fwd_graph_destroy()
