@@ -453,7 +453,7 @@ void llamd_cuda_paged_free(void *batch);
  * checked here, before a launch can use it: 0, or -1 and a message, and the batch is as it was (where memory could not be had: not
  * set). Enqueues one copy; may allocate, or give memory back, where a batch is more than twice as large as those before it; refused while a graph is captured, but what it has set may
  * be used in one. A batch that is set again serves the launches enqueued
- * after the call; a graph that was captured with it is not replayed any more. */
+ * after the call; llamd_fwd_graph_launch refuses a graph that was captured with it before, and one whose batch has been freed. */
 int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int32_t *kv_len, const int32_t *pages, int pages_stride,
                          int n_pages, int n_shared);
 /* The new tokens' q, k, v rows ([tokens][heads][hd], in_type LLAMD_PAGED_F32 or the batch's type; strides in elements

@@ -5,6 +5,9 @@
 #include <stdint.h>
 #include <stdio.h>
 
+#include <atomic>
+#include <memory>
+
 #include "../../include/llamd_cuda.h"
 
 namespace llamd {
@@ -12,6 +15,12 @@ namespace llamd {
 // One stream for every device-pointer op, as in the reference's device layer
 // (crates/llamd-rocm/kernels/llamd_forward.hip:701-716).
 cudaStream_t stream();
+// What a captured graph and those whose memory its launches read know of each other. Whoever changes or frees that memory says so, and the graph
+// is not launched any more.
+struct GraphUse {
+    std::atomic<bool> broken{false};
+};
+std::shared_ptr<GraphUse> captured_use();  // of the graph that llamd_fwd_begin_capture has begun, or null; may throw std::bad_alloc
 bool capturing();  // a graph is being captured from it, by the library or by a stream that it has been ordered behind
 // Sticky error state: the first failure is kept until read.
 void set_error(cudaError_t e, const char *what);

@@ -62,9 +62,26 @@ struct Batch {
     int n_small = 0, small_rows = 0, n_ctas = 0, n_merge = 0, most = 0;
     KeptBlock partial;
     size_t partial_rows = 0;
+    std::vector<std::shared_ptr<GraphUse>> graphs;  // captured with what is set
 
     ~Batch() {
+        break_graphs();
         drop(g_device, dev), drop(g_device, partial), drop(g_pinned, host);
+    }
+    void break_graphs() {
+        for (const auto &g : graphs) g->broken = true;
+        graphs.clear();
+    }
+    // Its launches go into the graph that is being captured, if one is.
+    bool note_graph() {
+        try {
+            const auto g = captured_use();
+            if (g && (graphs.empty() || graphs.back() != g)) graphs.push_back(g);
+        } catch (const std::exception &) {
+            set_error_msg("paged batch: out of host memory");
+            return false;
+        }
+        return true;
     }
     static void drop(Kept &to, KeptBlock &b) {
         if (b.p) to.keep(b);
@@ -614,6 +631,7 @@ int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int
         return -1;
     }
     b->ready = false;  // (from here on what the batch held is being replaced)
+    b->break_graphs();
     if (!b->reserve(std::max<size_t>(bytes, 16), plan.rows)) return -1;
     auto put = [&](size_t at, const void *from, size_t n) {
         if (n) memcpy(b->host.p + at, from, n);
@@ -656,7 +674,7 @@ int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int
 int llamd_fwd_paged_append(const void *batch, const void *q, const void *k, const void *v, int in_type, size_t q_stride, size_t k_stride, size_t v_stride,
                             const float *wq, const float *wk, float eps, const float *rope_tab, int rope_rows, int rot, int interleaved, void *q_out,
                             size_t out_stride, void *k_pages, void *v_pages) {
-    const Batch *b = (const Batch *)batch;
+    Batch *b = (Batch *)batch;
     if (!b || !b->ready) return refuse("paged append: the batch is not set");
     if (error_code()) return -1;
     if (gave_up()) return -1;
@@ -671,6 +689,7 @@ int llamd_fwd_paged_append(const void *batch, const void *q, const void *k, cons
     if (!aligned16(q_out) || out_stride % 8 || !aligned16(k_pages) || !aligned16(v_pages)) return refuse("paged append: outputs start at 16 bytes");
     const uintptr_t odd = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v, odd_w = (uintptr_t)wq | (uintptr_t)wk;
     if (odd % (in_type == kPagedF32 ? 4 : 2) || odd_w % 4) return refuse("paged append: an input starts inside an element");
+    if (!b->note_graph()) return -1;
     AppendParams p = {};
     p.b = g, p.sms = b->sms;
     p.q = q, p.k = k, p.v = v, p.q_stride = q_stride, p.k_stride = k_stride, p.v_stride = v_stride, p.out_stride = out_stride;
@@ -690,7 +709,7 @@ int llamd_fwd_paged_append(const void *batch, const void *q, const void *k, cons
 
 int llamd_fwd_paged_attention(const void *batch, const void *q, size_t q_stride, const void *k_pages, const void *v_pages, void *out, size_t out_stride,
                                int out_f32, float scale) {
-    const Batch *b = (const Batch *)batch;
+    Batch *b = (Batch *)batch;
     if (!b || !b->ready) return refuse("paged attention: the batch is not set");
     if (error_code()) return -1;
     if (gave_up()) return -1;
@@ -702,6 +721,7 @@ int llamd_fwd_paged_attention(const void *batch, const void *q, size_t q_stride,
     if (q_stride < qd || out_stride < qd) return refuse("paged attention: a row overlaps the next");
     if (!aligned16(q) || q_stride % 8 || !aligned16(out) || out_stride % 8 || !aligned16(k_pages) || !aligned16(v_pages))
         return refuse("paged attention: buffers and rows start at 16 bytes");
+    if (!b->note_graph()) return -1;
     PagedAttn a = {};
     a.b = g, a.q = q, a.k_pages = k_pages, a.v_pages = v_pages, a.out = out, a.q_stride = q_stride, a.out_stride = out_stride;
     a.out_f32 = out_f32, a.scale_log2 = scale * 1.4426950408889634f;

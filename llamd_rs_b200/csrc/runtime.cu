@@ -6,6 +6,7 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include <memory>
 #include <mutex>
 #include <string>
 #include <thread>
@@ -24,6 +25,7 @@ static std::string g_err_msg;
 static cudaGraph_t g_graph = nullptr;
 static cudaGraphExec_t g_graph_exec = nullptr;
 static bool g_capturing = false;            // between llamd_fwd_begin_capture and its end
+static std::shared_ptr<GraphUse> g_use, g_kept_use;  // of the current graph and of the kept one
 static cudaGraph_t g_kept_graph = nullptr;  // kept beside the current one (graph_swap)
 static cudaGraphExec_t g_kept_exec = nullptr;
 static void *g_scratch[8] = {};
@@ -216,6 +218,11 @@ static void destroy_current_graph() {
     if (g_graph) cudaGraphDestroy(g_graph);
     g_graph_exec = nullptr;
     g_graph = nullptr;
+    g_use.reset();
+}
+std::shared_ptr<GraphUse> captured_use() {
+    if (g_capturing && !g_use) g_use = std::make_shared<GraphUse>();
+    return g_capturing ? g_use : nullptr;
 }
 // The current graph and the one kept beside it change places (either may be none).
 void graph_swap() {
@@ -225,6 +232,7 @@ void graph_swap() {
     g_graph_exec = g_kept_exec;
     g_kept_graph = g;
     g_kept_exec = e;
+    g_use.swap(g_kept_use);
 }
 // llamd_fwd_begin_capture that leaves the kept graph alone.
 int begin_capture_beside() {
@@ -449,6 +457,10 @@ int llamd_fwd_end_capture(void) {
 int llamd_fwd_graph_launch(void) {
     if (!g_graph_exec) {
         set_error_msg("graph launch without a captured graph");
+        return -1;
+    }
+    if (g_use && g_use->broken) {
+        set_error_msg("graph launch: a paged batch that the graph was captured with has been set again or freed");
         return -1;
     }
     LLAMD_TRY(cudaGraphLaunch(g_graph_exec, stream()), "graph launch");

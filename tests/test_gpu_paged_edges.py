@@ -281,3 +281,38 @@ def test_free_waits_for_nothing_and_may_be_inside_a_capture(paged):
         assert np.array_equal(c.download_f32(256), 2 * np.arange(256, dtype=np.float32))
     finally:
         L.llamd_fwd_graph_destroy()
+
+
+@pytest.mark.parametrize("how", ["set", "free"])
+def test_graph_whose_batch_is_gone(paged, how):
+    """A graph reads its batch's tables: once they are another's it is not launched any more. A refused set leaves it valid."""
+    from llamd_rs_b200 import backend
+    from llamd_rs_b200._lib import lib
+
+    L, H, D = lib(), 8, 64
+    q, pool, out = (dev(np.zeros(n * 16 * D, np.uint16)) for n in (2 * H, 2, 2 * H))
+    b = paged.Batch(H, 1, D, 16, "f16")
+    b.set([2], [20], [[1, 0]], 2)
+    backend.sync()
+    assert L.llamd_fwd_begin_capture() == 0
+    b.append(q, q, q, q, pool, pool, inputs="f16")
+    b.attention(q, pool, pool, out)
+    assert L.llamd_fwd_end_capture() == 0
+    try:
+        assert L.llamd_fwd_graph_launch() == 0
+        with pytest.raises(paged.Malformed):
+            b.set([2], [20], [[1, 7]], 2)
+        assert L.llamd_fwd_graph_launch() == 0
+        if how == "set":
+            b.set([2], [20], [[1, 0]], 2)
+        else:
+            b.free()
+        assert L.llamd_fwd_graph_launch() == -1 and "freed" in backend._last_error()
+        assert L.llamd_fwd_last_error() == -1
+        backend.sync()
+        assert L.llamd_fwd_begin_capture() == 0  # another graph has nothing to do with it
+        L.llamd_fwd_add(out.ptr, out.ptr, out.ptr, 16)
+        assert L.llamd_fwd_end_capture() == 0 and L.llamd_fwd_graph_launch() == 0
+        backend.sync()
+    finally:
+        L.llamd_fwd_graph_destroy()
