@@ -145,16 +145,19 @@ const char *check_lengths(const Batch &b, int n_seq, const int32_t *q_len, const
     if ((long long)n_pages * b.view.n_head_kv * page > 0x7fffffffLL) return "paged batch: pools of more than 2^31 rows";
     if (n_shared % page) return "paged batch: the shared prefix is whole pages";
     long long tokens = 0;
+    const int32_t *lead = nullptr;  // the table of the first sequence with new tokens
     for (int s = 0; s < n_seq; s++) {
         if (q_len[s] < 0 || kv_len[s] < q_len[s]) return "paged batch: a sequence has fewer positions than new tokens";
         if (kv_len[s] > 1 << 30) return "paged batch: a sequence of more than 2^30 positions";
-        if (kv_len[s] - q_len[s] < n_shared) return "paged batch: new tokens inside the shared prefix";
+        if (q_len[s] && kv_len[s] - q_len[s] < n_shared) return "paged batch: new tokens inside the shared prefix";
         const long long used = ((long long)kv_len[s] + page - 1) / page;
         if (used > pages_stride) return "paged batch: a table has fewer pages than its sequence";
         const int32_t *t = pages + (size_t)s * pages_stride;
         for (long long i = 0; i < used; i++)
             if (t[i] < 0 || t[i] >= n_pages) return "paged batch: a page id outside the pools";
-        if (s && memcmp(t, pages, (size_t)(n_shared / page) * sizeof(int32_t))) return "paged batch: the shared prefix's pages differ";
+        if (!q_len[s]) continue;  // (attends to nothing: an idle slot may have no positions at all)
+        if (!lead) lead = t;
+        if (memcmp(t, lead, (size_t)(n_shared / page) * sizeof(int32_t))) return "paged batch: the shared prefix's pages differ";
         tokens += q_len[s];
     }
     if (tokens * b.view.n_head > 0x7fffffffLL) return "paged batch: too many tokens";
@@ -285,7 +288,11 @@ void make_plan(Plan &plan, const PagedView &v, const int32_t *q_len, const int32
     const int group = v.group, few_tokens = std::max(1, kPagedPieceRows / group);
     std::vector<Stretch> stretch;  // the shared one, where there is one, then the sequences' own
     const bool shared = v.n_shared && v.tokens;
-    if (shared) stretch.push_back({0, 0, v.n_shared, 0, v.tokens, v.n_shared, 0});
+    if (shared) {  // (through the table of the first sequence with new tokens)
+        int lead = 0;
+        while (!q_len[lead]) lead++;
+        stretch.push_back({lead * v.table_stride, 0, v.n_shared, 0, v.tokens, v.n_shared, 0});
+    }
     for (int s = 0, t = 0; s < v.n_seq; t += q_len[s], s++)
         if (q_len[s]) stretch.push_back({s * v.table_stride, v.n_shared, kv_len[s], t, q_len[s], kv_len[s] - q_len[s] + 1, 1});
     // Which go to paged_decode.cu: those of one of its pieces' rows, and others while they are little work in all (rows x positions x kv heads): a launch

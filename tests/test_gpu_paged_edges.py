@@ -316,3 +316,27 @@ def test_graph_whose_batch_is_gone(paged, how):
         backend.sync()
     finally:
         L.llamd_fwd_graph_destroy()
+
+
+@pytest.mark.parametrize("q_len,kv_len,n_shared", [([0, 1, 0, 1], [0, 40, 0, 70], 32), ([0, 0, 2, 1], [50, 16, 34, 33], 32), ([1, 0, 90], [65, 3, 400], 64)])
+def test_idle_slots_behind_a_shared_prefix(paged, q_len, kv_len, n_shared):
+    """Sequences without new tokens need not have the prefix, nor any position, wherever they stand."""
+    from llamd_rs_b200 import backend
+
+    H, K, D, page = 8, 2, 64, 16
+    rng = np.random.default_rng(6)
+    shared = [5, 2, 9, 1][:n_shared // page]
+    tables, at = [], 10
+    for n, m in zip(q_len, kv_len):
+        own = -(-m // page) - (len(shared) if n else 0)
+        tables.append((shared if n else []) + list(range(at, at + own)))
+        at += own
+    b = paged.Batch(H, K, D, page, "f16")
+    b.set(q_len, kv_len, tables, at, n_shared)
+    T = b.tokens
+    q, kp, vp = (plain.to_bits(rng.standard_normal(s), "f16") for s in ((T, H, D), (at, K, page, D), (at, K, page, D)))
+    out = dev(np.zeros(q.shape, np.uint16))
+    b.attention(dev(q), dev(kp), dev(vp), out)
+    backend.sync()
+    want, bound = plain.attention(*(plain.from_bits(x, "f16") for x in (q, kp, vp)), tables, q_len, kv_len, D ** -0.5, "f16")
+    assert np.all(np.abs(plain.from_bits(out.download(np.uint16, q.size), "f16").reshape(q.shape) - want) <= bound)
