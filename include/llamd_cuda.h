@@ -459,7 +459,7 @@ int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int
 /* The new tokens' q, k, v rows ([tokens][heads][hd], in_type LLAMD_PAGED_F32 or the batch's type; strides in elements
  * between tokens): q and k normed per head (x / sqrt(mean x^2 + eps) * w, f32 weights [hd]; wq / wk NULL: not normed),
  * the first `rot` elements of each head rotated (a multiple of 16, 0: not at all; interleaved 0: element i with i + rot / 2, else
- * 2i with 2i + 1) by the angles of rope_tab ([rope_rows][rot / 2][2] sines and cosines, a row per position), rounded once; q to q_out
+ * 2i with 2i + 1) by the angles of rope_tab ([rope_rows][rot / 2][2] sines and cosines, a row per position, for every new token's), rounded once; q to q_out
  * (rows out_stride elements apart), k and v to their slots. q_out, the pools and rope_tab start at 16 bytes. Enqueues, does not
  * synchronise. 0, or -1 and a message where refused: nothing was launched (so too while an earlier error of the library is unread). */
 int llamd_fwd_paged_append(const void *batch, const void *q, const void *k, const void *v, int in_type, size_t q_stride,

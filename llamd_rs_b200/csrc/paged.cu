@@ -49,7 +49,7 @@ void give_back() {
 
 struct Batch {
     PagedView view = {};
-    int type = 0, n_pages = 0, max_kv = 0, sms = 0;
+    int type = 0, n_pages = 0, max_kv = 0, sms = 0;  // max_kv: of sequences with new tokens
     bool ready = false;
     // the device copy of everything below, and the pinned memory it is made in, with the event behind the copy
     KeptBlock dev, host;
@@ -617,7 +617,7 @@ int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int
     int max_kv = 0;
     for (int s = 0; s < n_seq; s++) {
         v.tokens += q_len[s];
-        max_kv = std::max(max_kv, kv_len[s]);
+        if (q_len[s]) max_kv = std::max(max_kv, kv_len[s]);
         v.table_stride = std::max(v.table_stride, (kv_len[s] + v.page - 1) / v.page);
     }
     if ((long long)n_seq * v.table_stride > 0x7fffffffLL) return refuse("paged batch: the tables have more than 2^31 entries");

@@ -340,3 +340,22 @@ def test_idle_slots_behind_a_shared_prefix(paged, q_len, kv_len, n_shared):
     backend.sync()
     want, bound = plain.attention(*(plain.from_bits(x, "f16") for x in (q, kp, vp)), tables, q_len, kv_len, D ** -0.5, "f16")
     assert np.all(np.abs(plain.from_bits(out.download(np.uint16, q.size), "f16").reshape(q.shape) - want) <= bound)
+
+
+def test_angles_need_not_reach_idle_sequences(paged):
+    """A table of angles as long as the sequences with new tokens; one without is longer."""
+    from llamd_rs_b200 import backend
+
+    H, D, page = 2, 64, 16
+    b = paged.Batch(H, 1, D, page, "f16")
+    b.set([1, 0], [20, 90], [[0, 1], list(range(2, 8))], 8)
+    rng = np.random.default_rng(7)
+    x = rng.standard_normal((1, H, D)).astype(np.float32)
+    table, pool, out = paged.rope_table(20, D, 1e4), dev(np.zeros(8 * page * D, np.uint16)), dev(np.zeros(H * D, np.uint16))
+    b.append(dev(x), dev(x[:, :1]), dev(x[:, :1]), out, pool, pool, rope=dev(table))
+    backend.sync()
+    want = plain.norm_rope(x, np.array([19]), None, 0, table, D, False)
+    got = plain.from_bits(out.download(np.uint16, H * D), "f16").reshape(want.shape)
+    assert np.all(np.abs(got - want) <= plain.U["f16"] * np.abs(want) + 2.0 ** -22 * np.abs(want).max() + plain.TINY["f16"])
+    with pytest.raises(paged.Malformed, match="angles"):
+        b.append(dev(x), dev(x[:, :1]), dev(x[:, :1]), out, pool, pool, rope=dev(table), rope_rows=19)
