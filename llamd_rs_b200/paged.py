@@ -92,21 +92,25 @@ class Pages:
 
     def fork(self, table: list, n_pos: int) -> list:
         """A table of another sequence that begins with the first n_pos positions (whole pages) of this one."""
-        if n_pos % self.page_size or n_pos > len(table) * self.page_size:
+        if n_pos < 0 or n_pos % self.page_size or n_pos > len(table) * self.page_size:
             raise Malformed(f"{n_pos} positions of {len(table)} pages of {self.page_size} cannot be shared")
         shared = list(table[:n_pos // self.page_size])
+        for p in shared:
+            if not 0 <= p < self.n_pages or self._held[p] < 1:
+                raise Malformed(f"page {p} is nobody's and cannot be shared")
         for p in shared:
             self._held[p] += 1
         return shared
 
     def release(self, table: list) -> None:
-        """The sequence is done: pages that nobody else holds are free again."""
-        for p in table:
-            if self._held[p] < 1:
+        """The sequence is done: pages that nobody else holds are free again. Where one of them is not held, nothing is released."""
+        for i, p in enumerate(table):
+            if not 0 <= p < self.n_pages or self._held[p] < 1:
+                for x in table[:i]:
+                    self._held[x] += 1
                 raise Malformed(f"page {p} is released twice")
             self._held[p] -= 1
-            if not self._held[p]:
-                self._free.append(p)
+        self._free.extend(p for p in dict.fromkeys(table) if not self._held[p])
         table.clear()
 
 

@@ -79,3 +79,23 @@ def test_refused_without_a_device(paged):
         pytest.skip("a device is present")
     with pytest.raises(paged.Unsupported):
         paged.Batch(8, 2, 64, 16)
+
+
+def test_pages_refuse_what_is_not_held(paged):
+    """A negative length, pages that are free or not there: refused, and nothing has changed."""
+    p = paged.Pages(6, 16)
+    a = []
+    p.grow(a, 60)
+    before = list(p._held)
+    for table, n in ((a, -16), ([5], 16), ([9], 16), ([-1], 16)):
+        with pytest.raises(paged.Malformed):
+            p.fork(table, n)
+        assert p._held == before
+    for table in ([a[0], 5], a[:2] + a[:1], [a[1], 6], [a[1], -1]):
+        kept = list(table)
+        with pytest.raises(paged.Malformed):
+            p.release(table)
+        assert p._held == before and p.free() == 2 and table == kept
+    twice = a + p.fork(a, 32)  # a table may list a page twice, as often as it is held
+    p.release(twice)
+    assert p.free() == 6 and sorted(p._free) == list(range(6)) and not any(p._held)
