@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import operator
 import sys
 
 import numpy as np
@@ -38,6 +39,27 @@ def _type_of(x):
     return t
 
 
+def _int32s(x, what):
+    """x as an int32 array; refused where a conversion would change a value."""
+    a = np.asarray(x)
+    if a.dtype != np.int32:
+        if a.size and (a.dtype.kind not in "iu" or int(a.min()) < -2 ** 31 or int(a.max()) >= 2 ** 31):
+            raise Malformed(f"{what}: {a.dtype}, not whole numbers of 32 bits")
+        a = a.astype(np.int32)
+    return np.ascontiguousarray(a)
+
+
+def _int(x, what, below=2 ** 31):
+    """x as a whole number from 0 on: what the library would else see the low bits of."""
+    try:
+        n = operator.index(x)
+    except TypeError:
+        n = -1
+    if not 0 <= n < below:
+        raise Malformed(f"{what}: {x!r} is not a whole number below {below}")
+    return n
+
+
 def _stream_of(*buffers):
     """torch's current stream (a cudaStream_t) where one of the buffers is a tensor, else None."""
     for x in buffers:
@@ -62,6 +84,7 @@ def rope_table(rows: int, rot: int, freq_base: float, scaling: str = "none", fac
         raise Unsupported(f"rope scaling {scaling!r}: one of {', '.join(SCALING)}")
     if rows < 0 or rot < 2 or rot % 2:
         raise ShapeError(f"rope table of {rows} rows, {rot} elements")
+    rows, rot, original = _int(rows, "rows"), _int(rot, "rotated elements"), _int(original, "trained positions")
     out = np.empty((rows, rot // 2, 2), dtype=np.float32)
     if lib().llamd_cuda_rope_table_scaled(backend._ptr(out), rows, rot, freq_base, SCALING[scaling], factor, original) != 0:
         _refuse("rope table")
@@ -122,6 +145,7 @@ class Batch:
         if dtype not in ("f16", "bf16"):
             raise Unsupported(f"a paged cache holds f16 or bf16, not {dtype}")
         backend._need_device()
+        n_head, n_head_kv, head_dim, page_size = (_int(x, "paged batch") for x in (n_head, n_head_kv, head_dim, page_size))
         self.type = TYPES[dtype]
         self.n_head, self.n_head_kv, self.head_dim, self.page_size = n_head, n_head_kv, head_dim, page_size
         self.ptr = lib().llamd_cuda_paged_new(n_head, n_head_kv, head_dim, page_size, self.type)
@@ -135,15 +159,14 @@ class Batch:
     def set(self, q_lens, kv_lens, pages, n_pages: int, n_shared: int = 0) -> None:
         """q_lens, kv_lens: new tokens and positions in all of every sequence; pages: their tables, rows of one int32 array or a
         list of lists; n_pages: the pools' size; n_shared: positions at the beginning that all of them have in common."""
-        q = np.ascontiguousarray(q_lens, dtype=np.int32).ravel()
-        kv = np.ascontiguousarray(kv_lens, dtype=np.int32).ravel()
+        q, kv = _int32s(q_lens, "new-token counts").ravel(), _int32s(kv_lens, "lengths").ravel()
+        n_pages, n_shared = _int(n_pages, "pages"), _int(n_shared, "shared positions")
         if not isinstance(pages, np.ndarray):
-            rows = [list(r) for r in pages]
-            pages = np.zeros((len(rows), max([len(r) for r in rows] + [1])), dtype=np.int32)
+            rows = [_int32s(r if hasattr(r, "__array__") else list(r), "page ids").ravel() for r in pages]
+            pages = np.full((len(rows), max([len(r) for r in rows] + [1])), -1, dtype=np.int32)  # (-1: refused where a sequence reaches it)
             for i, r in enumerate(rows):
                 pages[i, :len(r)] = r
-                pages[i, len(r):] = -1  # (refused where a sequence reaches it)
-        pages = np.ascontiguousarray(pages, dtype=np.int32)
+        pages = _int32s(pages, "page ids")
         if q.size != kv.size or pages.ndim != 2 or pages.shape[0] != q.size:
             raise ShapeError(f"{q.size} new-token counts, {kv.size} lengths, tables {pages.shape}")
         if lib().llamd_cuda_paged_set(self.ptr, q.size, backend._ptr(q), backend._ptr(kv), backend._ptr(pages), pages.shape[1], n_pages, n_shared) != 0:
@@ -178,7 +201,7 @@ class Batch:
         try:
             ptr = x.data_ptr()
         except AttributeError:
-            stride = n if stride is None else stride
+            stride = n if stride is None else _int(stride, f"{what}: elements between tokens", 2 ** 40)
             if isinstance(x, DevBuf):
                 if self.tokens and x.nbytes < ((self.tokens - 1) * stride + n) * _SIZE[type_]:
                     raise ShapeError(f"{what}: {x.nbytes} bytes for {self.tokens} tokens") from None
@@ -218,7 +241,7 @@ class Batch:
             it = TYPES.get(inputs, -1)
         if it != 2 and it != self.type:
             raise Unsupported("append takes f32 or the cache's type")
-        rot = (0 if rope is None else self.head_dim) if rot is None else rot
+        rot = (0 if rope is None else self.head_dim) if rot is None else _int(rot, "rotated elements")
         if rot and rope is None:
             raise Malformed("a rotation without its angles")
         if rope_rows is None:
@@ -232,6 +255,8 @@ class Batch:
                 rope_rows = rope.nbytes // (4 * rot)
             else:
                 raise Malformed("rope_rows: how many positions the table has")
+        else:
+            rope_rows = _int(rope_rows, "rope_rows")
         D, T, t = self.head_dim, self.tokens, self.type
         nq, nk = self.n_head * D, self.n_head_kv * D
         if rot and q_norm is not None and k_norm is not None:

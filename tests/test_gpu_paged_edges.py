@@ -359,3 +359,20 @@ def test_angles_need_not_reach_idle_sequences(paged):
     assert np.all(np.abs(got - want) <= plain.U["f16"] * np.abs(want) + 2.0 ** -22 * np.abs(want).max() + plain.TINY["f16"])
     with pytest.raises(paged.Malformed, match="angles"):
         b.append(dev(x), dev(x[:, :1]), dev(x[:, :1]), out, pool, pool, rope=dev(table), rope_rows=19)
+
+
+def test_strides_that_point_elsewhere_are_refused(paged):
+    """Negative strides between tokens: before anything is read."""
+    from llamd_rs_b200._lib import lib
+
+    b = paged.Batch(8, 2, 64, 16, "f16")
+    b.set([3], [20], [[3, 1]], 6)
+    pool, rows = dev(np.zeros(6 * 2 * 16 * 64, np.uint16)), dev(np.zeros(64 * 8 * 64, np.uint16))
+    before = lib().llamd_fwd_launch_count()
+    for i in range(3):
+        strides = [None] * 3
+        strides[i] = -1024
+        for q in (rows, rows.ptr):
+            with pytest.raises(paged.Malformed, match="between tokens"):
+                b.append(q, q, q, rows, pool, pool, inputs="f16", strides=strides)
+    assert lib().llamd_fwd_launch_count() == before

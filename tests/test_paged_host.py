@@ -99,3 +99,25 @@ def test_pages_refuse_what_is_not_held(paged):
     twice = a + p.fork(a, 32)  # a table may list a page twice, as often as it is held
     p.release(twice)
     assert p.free() == 6 and sorted(p._free) == list(range(6)) and not any(p._held)
+
+
+def test_numbers_that_would_lose_bits_are_refused(paged):
+    """What int32 cannot hold, and fractions: refused by name, not cut to the low bits (a batch that is never made serves: nothing reaches the library)."""
+    b = paged.Batch.__new__(paged.Batch)
+    b.ptr = None
+    big = np.array([2 ** 32 + 1], np.int64)
+    for q, kv, pages, n_pages, shared, what in (
+            (big, [1], [[0]], 4, 0, "new-token counts"), ([1], big, [[0]], 4, 0, "lengths"), ([1], [1], big[None], 4, 0, "page ids"), ([1], [1], [big], 4, 0, "page ids"),
+            ([1.5], [2], [[0]], 4, 0, "new-token counts"), ([1], [2], [[0.5]], 4, 0, "page ids"), ([1], [1], np.array([[2 ** 31]], np.uint32), 4, 0, "page ids"),
+            ([1], [1], [[0]], 2 ** 32 + 4, 0, "pages"), ([1], [1], [[0]], 4, 2 ** 32, "shared positions"), ([1], [1], [[0]], 4.0, 0, "pages"),
+            ([1], [1], [[0]], 4, -16, "shared positions")):
+        with pytest.raises(paged.Malformed, match=what):
+            b.set(q, kv, pages, n_pages, shared)
+    for rows, rot, original in ((2 ** 32, 2, 0), (4, 2 ** 33, 0), (4, 8, 2 ** 32 + 1), (4, 8, -1)):
+        with pytest.raises(paged.Malformed):
+            paged.rope_table(rows, rot, 1e4, "by_frequency", 2.0, original)
+    b.tokens, b.head_dim = 3, 64
+    for stride in (-64, 2 ** 40, 64.0):
+        with pytest.raises(paged.Malformed, match="elements between tokens"):
+            b._rows(1 << 20, 64, 0, "q", stride)
+    assert b._rows(1 << 20, 64, 0, "q", 72) == (1 << 20, 72) and b._rows(1 << 20, 64, 0, "q") == (1 << 20, 64)
