@@ -6,40 +6,11 @@
 #include <cuda_fp16.h>
 
 #include "common.cuh"
+#include "paged_items.h"
 
 namespace llamd {
 
 enum { kPagedF16 = 0, kPagedBf16 = 1, kPagedF32 = 2 };
-
-// A new token: its position and the row of the pools that head 0 of its K and V goes to (head h: `page` rows further each).
-struct PagedToken {
-    int32_t pos, row;
-};
-
-// The batch as the kernels see it: device memory that the batch owns, every index checked against the pools when it was made.
-struct PagedView {
-    int n_head, n_head_kv, group, hd, page, n_seq, tokens, n_shared, table_stride;
-    const PagedToken *token;    // [tokens]
-    const int32_t *token_seq;   // [tokens]
-    const int32_t *table;       // [n_seq][table_stride] page ids
-};
-
-// One piece of attention: n_tok tokens (all their heads that share kv head `head`; for paged_decode.cu the launch's y) over positions
-// [kv_begin, kv_end) of one table.
-// Token i of the piece sees positions below limit + i * step. part < 0: the piece is all its rows need, and writes out;
-// otherwise its rows' sums go to rows part + ... of the batch's partial results (paged_decode.cu: + head * part_rows).
-struct PagedItem {
-    int32_t table, kv_begin, kv_end, token, n_tok, limit, step, part, part_rows, head, pad[2];
-};
-static_assert(sizeof(PagedItem) == 48, "three 16-byte words");
-
-// Where the rows of a token and a kv head find their partial results: entries [begin, begin + count) of the list below.
-struct PagedMerge {
-    int32_t token, head, begin, count;
-};
-struct PagedPart {
-    int32_t row, token;  // the row of token t and head g of the group: row + (t - token) * group + g
-};
 
 // A partial result: sums of 2^(s - m) v over the piece's positions (s: the scores times log2 e), in f32, and beside them m and sum 2^(s - m).
 struct PagedAttn {
@@ -54,14 +25,7 @@ struct PagedAttn {
     float2 *part_ml;   // [rows] (m, sum)
 };
 
-// Query rows (tokens x heads of a group) of a piece that paged_decode.cu can take (one token of a wide group), and of one that it is given where a
-// stretch has several tokens. Pieces of 16 rows: 32 take four times the registers of 8 and half the
-// CTAs (8 sequences behind 512 shared positions 12.1 us against 6.6, 64 with 3 new tokens behind 3500 102.9 against 90.7), 8 read K and V
-// twice as often (102.9).
-constexpr int kPagedSmallRows = 32, kPagedPieceRows = 16;
-
 void paged_decode_launch(const PagedAttn &p, int type, int n_items, int max_rows, cudaStream_t to);
-constexpr int kPagedTileRows = 128, kPagedBlock = 128;  // of paged_prompt.cu: two tiles of query rows to a piece, positions to a block
 bool paged_gave_up();       // a wait of an earlier attention has run out, and the host has not read it yet
 bool paged_prompt_ready();  // what its launches need beside the batch: false and an error where it cannot be had
 bool paged_prompt_launch(const PagedAttn &p, int type, int n_pages, const int32_t *begin, int n_ctas);  // begin: each CTA's pieces (n_ctas + 1); false and an error: not launched
