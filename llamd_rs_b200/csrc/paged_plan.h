@@ -31,7 +31,7 @@ struct Stretch {
 // (64 KB) repay.
 inline int decode_piece(long long positions, int n_head_kv, int sms) {
     const long long share = (2 * positions * n_head_kv + 3LL * sms - 1) / (3LL * sms);
-    return (int)std::max(128LL, (share + 15) / 16 * 16);
+    return (int)std::min(1LL << 30, std::max(128LL, (share + 15) / 16 * 16));  // (no sequence is longer)
 }
 
 // paged_prompt.cu runs one CTA to an SM, each with a list of pieces. In blocks of its loop over two tiles, a block over one tile costs kHalfCost (its

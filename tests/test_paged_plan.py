@@ -148,6 +148,12 @@ def test_every_position_once_and_every_part_joined(check, seed):
         check(q, kv, group * heads, heads, r.choice([64, 128]), page, shared, r.choice([148, 148, 132, 16]))
 
 
+def test_as_long_as_sequences_may_be(check):
+    """An even share of the positions that is more than 32 bits hold."""
+    check([1] * 500, [1 << 30] * 500, 8, 8, page=4096)
+    check([1, 40], [1 << 30] * 2, 8, 8, page=4096, n_shared=1 << 29)
+
+
 @pytest.mark.parametrize("plant", [1, 2, 3, 4])
 def test_the_checks_find_a_wrong_plan(check, plant):
     check([1] * 30, [3000 + i for i in range(30)], n_shared=2048)
