@@ -449,7 +449,9 @@ void *llamd_cuda_paged_new(int n_head, int n_head_kv, int hd, int page_size, int
 void llamd_cuda_paged_free(void *batch);
 /* pages: [n_seq][pages_stride], ids below n_pages (the pools' size), of each sequence the first
  * ceil(kv_len / page_size) are read. q_len may be 0. n_shared: the first n_shared positions (whole pages, the same ids in every
- * table) are common to all sequences with new tokens, none has new tokens among them, and attention reads them once for all. Everything is
+ * table) are common to all sequences with new tokens, none has new tokens among them, and attention reads them once for all
+ * where that is the quicker: where the sequences have few new tokens each. (The parts that are joined then take 4 hd + 8 bytes for each of
+ * two rows and more per token and head; with n_shared 0 there are fewer.) Everything is
  * checked here, before a launch can use it: 0, or -1 and a message, and the batch is as it was (where memory could not be had: not
  * set). Enqueues one copy; may allocate, or give memory back, where a batch is more than twice as large as those before it; refused while a graph is captured, but what it has set may
  * be used in one. A batch that is set again serves the launches enqueued

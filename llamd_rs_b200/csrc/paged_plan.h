@@ -128,17 +128,31 @@ inline double Dealer::best(const std::vector<Large> &large, std::vector<Cut> &cu
     return ends;
 }
 
+// Is a shared prefix a stretch of its own, read once for all tokens? Every row then leaves two partial results and more (520 bytes each at 128 elements,
+// up to a gigabyte for a few long prompts), which another launch joins. A sequence alone shares with nobody, and sequences of two full tiles of
+// query rows and more read K and V for so many rows at a time that nothing is saved. Measured, apart against whole, us (32 heads over 4 of 128):
+//   behind 256:  64 of 16 tokens (128 rows each) 50.4 / 19.5, 64 of 32 61.8 / 23.2, 256 of 1 22.9 / 21.8, 1 of 2000 behind 1024 102 / 66
+//   behind 1024: 256 of 4 62.0 / 110.5, 64 of 8 40.8 / 38.0, 64 of 32 80.6 / 44.9, 32 of 200 303 / 179, 512 beside 100 of 1 42.4 / 55.7, 2000 beside 30 of 1 119 / 78
+//   behind 4096: 64 of 1 24.5 / 48.0, 64 of 16 107 / 120, 16 of 32 63.0 / 51.9, 64 of 32 160 / 134, 16 of 2048 2866 / 2327
+// From 256 rows a sequence on whole is at worst 1.04 times apart (2 of 512 behind 4096, 8 heads of 64 without groups: 24.5 / 25.5).
+inline bool prefix_apart(const PagedView &v, const int32_t *q_len) {
+    long long active = 0;
+    for (int s = 0; s < v.n_seq; s++) active += q_len[s] > 0;
+    return v.n_shared && active > 1 && (long long)v.tokens * v.group < 2LL * kPagedTileRows * active;
+}
+
 inline void make_plan(Plan &plan, const PagedView &v, const int32_t *q_len, const int32_t *kv_len, int sms) {
     const int group = v.group, few_tokens = std::max(1, kPagedPieceRows / group);
     std::vector<Stretch> stretch;  // the shared one, where there is one, then the sequences' own
-    const bool shared = v.n_shared && v.tokens;
+    const bool shared = prefix_apart(v, q_len);
+    const int from = shared ? v.n_shared : 0;
     if (shared) {  // (through the table of the first sequence with new tokens)
         int lead = 0;
         while (!q_len[lead]) lead++;
         stretch.push_back({lead * v.table_stride, 0, v.n_shared, 0, v.tokens, v.n_shared, 0});
     }
     for (int s = 0, t = 0; s < v.n_seq; t += q_len[s], s++)
-        if (q_len[s]) stretch.push_back({s * v.table_stride, v.n_shared, kv_len[s], t, q_len[s], kv_len[s] - q_len[s] + 1, 1});
+        if (q_len[s]) stretch.push_back({s * v.table_stride, from, kv_len[s], t, q_len[s], kv_len[s] - q_len[s] + 1, 1});
     // Which go to paged_decode.cu: those of one of its pieces' rows, and others while they are little work in all (rows x positions x kv heads): a launch
     // less and no piece to begin weigh more there than reading K and V once for every 16 rows. Measured, that kernel against the other, us: own stretches
     // of 160 rows and 20 positions 4.0 and 7.1, 240 rows and 130 positions 7.2 and 9.0, 4 times 64 and 508 8.3 and 11.5; 16 times 64 and 1000 to 4000

@@ -133,7 +133,7 @@ def test_refused_attention_launches_nothing(paged):
 
 
 @pytest.mark.parametrize("dtype,out_f32", [("f16", False), ("bf16", True)])
-@pytest.mark.parametrize("q_len,kv_len,n_shared", [([90, 300], [90, 900], 0), ([60, 1, 90], [1728, 1618, 1708], 1600), ([1] * 40, [6001] * 40, 6000)])
+@pytest.mark.parametrize("q_len,kv_len,n_shared", [([90, 300], [90, 900], 0), ([20, 1, 20], [6048, 6016, 6040], 6000), ([1] * 40, [6001] * 40, 6000)])
 def test_given_up(paged, dtype, out_f32, q_len, kv_len, n_shared):
     """Waits that may take no time: every row of the tensor-core kernel, or that joins one of its parts, is NaN, the status says so once, calls refuse
     until it has been read, and then all is as before."""
@@ -376,3 +376,28 @@ def test_strides_that_point_elsewhere_are_refused(paged):
             with pytest.raises(paged.Malformed, match="between tokens"):
                 b.append(q, q, q, rows, pool, pool, inputs="f16", strides=strides)
     assert lib().llamd_fwd_launch_count() == before
+
+
+@pytest.mark.parametrize("q_len,n_shared", [([31] * 6, 272), ([33] * 6, 272), ([90] + [1] * 12, 272), ([300] + [1] * 12, 1008), ([40], 512), ([0, 1, 0], 512)])
+@pytest.mark.parametrize("K,D,dtype", [(1, 128, "bf16"), (2, 64, "f16")])
+def test_prefix_apart_and_whole(paged, q_len, n_shared, K, D, dtype):
+    """Prompts and tokens behind a prefix on both sides of the line from which it is read once for all."""
+    from llamd_rs_b200 import backend
+
+    H, page = 8 * K, 16
+    kv_len = [n_shared + n + 5 * i if n else 0 for i, n in enumerate(q_len)]
+    rng, first, tables = np.random.default_rng(len(q_len)), n_shared // page, []
+    ids, at = rng.permutation(sum(-(-m // page) for m in kv_len) + first), first
+    for m in kv_len:
+        own = max(0, -(-m // page) - first)
+        tables.append(np.concatenate([ids[:first] if m else ids[:0], ids[at:at + own]]).astype(np.int32))
+        at += own
+    b = paged.Batch(H, K, D, page, dtype)
+    b.set(q_len, kv_len, tables, len(ids), n_shared)
+    T = b.tokens
+    q, kp, vp = (plain.to_bits(rng.standard_normal(s), dtype) for s in ((T, H, D), (len(ids), K, page, D), (len(ids), K, page, D)))
+    out = dev(np.zeros(q.shape, np.uint16))
+    b.attention(dev(q), dev(kp), dev(vp), out)
+    backend.sync()
+    want, bound = plain.attention(*(plain.from_bits(x, dtype) for x in (q, kp, vp)), tables, q_len, kv_len, D ** -0.5, dtype)
+    assert np.all(np.abs(plain.from_bits(out.download(np.uint16, q.size), dtype).reshape(q.shape) - want) <= bound)

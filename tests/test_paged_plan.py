@@ -148,6 +148,19 @@ def test_every_position_once_and_every_part_joined(check, seed):
         check(q, kv, group * heads, heads, r.choice([64, 128]), page, shared, r.choice([148, 148, 132, 16]))
 
 
+@pytest.mark.parametrize("n,tokens,shared", [(16, 2048, 4096), (32, 200, 1024), (4, 1000, 2048), (1, 2000, 2048), (1, 8192, 16), (8, 1000, 1024), (1, 1, 1024)])
+def test_prompts_behind_a_prefix_need_no_more_room_than_without(check, n, tokens, shared):
+    """Long prompts save nothing by reading the prefix once for all, and one sequence has nobody to share with: planned as if there were no prefix."""
+    q, kv = [tokens] * n, [shared + tokens] * n
+    assert check(q, kv, n_shared=shared) == check(q, kv)
+
+
+def test_few_tokens_read_the_prefix_once(check):
+    for q in ([1] * 64, [31] * 16, [512] + [1] * 100):
+        kv = [4096 + n for n in q]
+        assert check(q, kv, n_shared=4096)[0] >= 2 * 32 * sum(q) and check(q, kv, n_shared=4096) != check(q, kv)
+
+
 def test_as_long_as_sequences_may_be(check):
     """An even share of the positions that is more than 32 bits hold."""
     check([1] * 500, [1 << 30] * 500, 8, 8, page=4096)
