@@ -365,8 +365,7 @@ int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int
     }
     if (plan.rows > 0x7fffffff || plan.merge.size() * v.group > 0x7fffffff) return refuse("paged batch: too many partial results");
     size_t bytes = 0;
-    const size_t o_token = section<PagedToken>(bytes, v.tokens), o_seq = section<int32_t>(bytes, v.tokens),
-                 o_table = section<int32_t>(bytes, (size_t)n_seq * v.table_stride), o_small = section<PagedItem>(bytes, plan.small.size()),
+    const size_t o_token = section<PagedToken>(bytes, v.tokens), o_table = section<int32_t>(bytes, (size_t)n_seq * v.table_stride), o_small = section<PagedItem>(bytes, plan.small.size()),
                  o_large = section<PagedItem>(bytes, plan.large.size()), o_begin = section<int32_t>(bytes, plan.begin.size()),
                  o_merge = section<PagedMerge>(bytes, plan.merge.size()), o_part = section<PagedPart>(bytes, plan.part.size());
     if (plan.beside && !side_ready()) {
@@ -385,15 +384,13 @@ int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int
     put(o_merge, plan.merge.data(), plan.merge.size() * sizeof(PagedMerge));
     put(o_part, plan.part.data(), plan.part.size() * sizeof(PagedPart));
     PagedToken *token = (PagedToken *)(b->host.p + o_token);
-    int32_t *seq = (int32_t *)(b->host.p + o_seq), *table = (int32_t *)(b->host.p + o_table);
+    int32_t *table = (int32_t *)(b->host.p + o_table);
     for (int s = 0, t = 0; s < n_seq; s++) {
         const int32_t *from = pages + (size_t)s * pages_stride;
         const int used = (kv_len[s] + v.page - 1) / v.page;
         for (int i = 0; i < v.table_stride; i++) table[(size_t)s * v.table_stride + i] = i < used ? from[i] : 0;
-        for (int pos = kv_len[s] - q_len[s]; pos < kv_len[s]; pos++, t++) {
+        for (int pos = kv_len[s] - q_len[s]; pos < kv_len[s]; pos++, t++)
             token[t] = {pos, from[pos / v.page] * v.n_head_kv * v.page + pos % v.page};
-            seq[t] = s;
-        }
     }
     b->small = (const PagedItem *)(b->dev.p + o_small);
     b->large = (const PagedItem *)(b->dev.p + o_large);
@@ -405,7 +402,6 @@ int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int
     b->partial_rows = plan.rows;
     b->n_pages = n_pages, b->max_kv = max_kv;
     v.token = (const PagedToken *)(b->dev.p + o_token);
-    v.token_seq = (const int32_t *)(b->dev.p + o_seq);
     v.table = (const int32_t *)(b->dev.p + o_table);
     b->view = v;
     LLAMD_TRY(cudaMemcpyAsync(b->dev.p, b->host.p, bytes, cudaMemcpyHostToDevice, stream()), "paged batch: copy");

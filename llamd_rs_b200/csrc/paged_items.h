@@ -13,7 +13,6 @@ struct PagedToken {
 struct PagedView {
     int n_head, n_head_kv, group, hd, page, n_seq, tokens, n_shared, table_stride;
     const PagedToken *token;    // [tokens]
-    const int32_t *token_seq;   // [tokens]
     const int32_t *table;       // [n_seq][table_stride] page ids
 };
 
