@@ -401,3 +401,74 @@ def test_prefix_apart_and_whole(paged, q_len, n_shared, K, D, dtype):
     backend.sync()
     want, bound = plain.attention(*(plain.from_bits(x, dtype) for x in (q, kp, vp)), tables, q_len, kv_len, D ** -0.5, dtype)
     assert np.all(np.abs(plain.from_bits(out.download(np.uint16, q.size), dtype).reshape(q.shape) - want) <= bound)
+
+
+def test_graph_with_the_side_stream(paged):
+    """A batch whose prefix and own positions are read at the same time, captured and replayed over new queries; a launch before and behind it on the
+    library's stream, so that fork and join are inside."""
+    from llamd_rs_b200 import backend
+    from llamd_rs_b200._lib import lib
+
+    L, H, K, D, page, n_shared = lib(), 32, 4, 128, 64, 7552
+    rng = np.random.default_rng(8)
+    q_len = [1] * 64
+    kv_len = [n_shared + int(x) for x in rng.integers(380, 520, 64)]
+    first, tables, at = n_shared // page, [], n_shared // page
+    for m in kv_len:
+        own = -(-m // page) - first
+        tables.append(list(range(first)) + list(range(at, at + own)))
+        at += own
+    b = paged.Batch(H, K, D, page, "bf16")
+    b.set(q_len, kv_len, tables, at, n_shared)
+    kp, vp = (plain.to_bits(rng.standard_normal((at, K, page, D)), "bf16") for _ in range(2))
+    q = [plain.to_bits(rng.standard_normal((64, H, D)), "bf16") for _ in range(3)]
+    dq, dk, dv, out, x = dev(q[0]), dev(kp), dev(vp), dev(np.zeros((64, H, D), np.float32)), dev(np.ones(64 * H * D, np.float32))
+    total = dev(np.zeros(64 * H * D, np.float32))
+    backend.sync()
+    assert L.llamd_fwd_begin_capture() == 0
+    L.llamd_fwd_add(x.ptr, x.ptr, out.ptr, 64 * H * D)
+    b.attention(dq, dk, dv, out, out_f32=True)
+    L.llamd_fwd_add(out.ptr, x.ptr, total.ptr, 64 * H * D)
+    assert L.llamd_fwd_end_capture() == 0
+    pages = [plain.from_bits(y, "bf16") for y in (kp, vp)]
+    try:
+        for i in range(3):
+            dq.upload(q[i])
+            for _ in range(1 + i):
+                assert L.llamd_fwd_graph_launch() == 0
+            backend.sync()
+            got = total.download_f32(64 * H * D).astype(np.float64).reshape(64, H, D) - 1
+            want, bound = plain.attention(plain.from_bits(q[i], "bf16"), *pages, tables, q_len, kv_len, D ** -0.5, "bf16")
+            assert np.all(np.abs(got - want) <= bound + 2.0 ** -22)  # (the sum with 1 is rounded once)
+    finally:
+        L.llamd_fwd_graph_destroy()
+    assert paged.status() == 0
+
+
+def test_tensors_in_torchs_own_graph(paged):
+    """torch captures its stream: the calls' launches and orders become part of its graph."""
+    torch = pytest.importorskip("torch")
+
+    H, K, D, page, n = 8, 2, 64, 16, 50
+    b = paged.Batch(H, K, D, page, "bf16")
+    b.set([n], [n], [list(range(4))], 4)
+    qkv = torch.randn(n, H + 2 * K, D, device="cuda").bfloat16()
+    kp, vp = (torch.zeros(4, K, page, D, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    q, out = (torch.zeros(n, H, D, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    b.append(qkv[:, :H], qkv[:, H:H + K], qkv[:, H + K:], q, kp, vp)
+    b.attention(q, kp, vp, out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, capture_error_mode="thread_local"):
+        qkv.mul_(0.5)
+        b.append(qkv[:, :H], qkv[:, H:H + K], qkv[:, H + K:], q, kp, vp)
+        b.attention(q, kp, vp, out)
+        doubled = out * 2
+    for _ in range(2):
+        before = qkv.clone()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(qkv, before * 0.5) and torch.equal(q, qkv[:, :H]) and torch.equal(doubled, out * 2)
+        x = qkv.double().cpu().numpy()
+        want, bound = plain.attention(x[:, :H], *(y.double().cpu().numpy() for y in (kp, vp)), [list(range(4))], [n], [n], D ** -0.5, "bf16")
+        assert np.all(np.abs(out.double().cpu().numpy() - want) <= bound)
