@@ -482,7 +482,8 @@ void llamd_fwd_paged_wait_limit(unsigned long long nanoseconds);
 /* The table of llamd_fwd_paged_append on the host: sine and cosine of r * f_i, f_i = base^(-2i / rot), evaluated in double.
  * scaling 0: as it is; 1: f / factor (positions stretched); 2: base * factor^(rot / (rot - 2)) in place of base; 3: by frequency,
  * f / factor for those that turn less than once over `original` positions, f for those that turn 32 times and more, a ramp
- * between, and all values times 0.1 ln(factor) + 1. */
+ * between (in the number of turns), and all values times 0.1 ln(factor) + 1. Checkpoints whose loaders ramp over the pair's index, between the indices where the two
+ * numbers of turns fall, need a table of their own (single frequencies differ by up to a half); append takes any. */
 int llamd_cuda_rope_table_scaled(float *host_out, int rows, int rot, float freq_base, int scaling, float factor, int original);
 
 #ifdef __cplusplus

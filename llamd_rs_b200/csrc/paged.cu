@@ -176,7 +176,7 @@ const char *check_lengths(const Batch &b, int n_seq, const int32_t *q_len, const
 // several heads of one kind (q, k or v) of one token on their way at once, so the token's angles and the weights are read once for them.
 // Heads that a warp has on their way, and CTAs to an SM; measured with 1 to 8 heads and 3 to 6 CTAs: 6279 tokens of f16, 32 heads over 4 of 128, 28.3 us with 4
 // and 4 (4.6 TB/s), 8192 tokens of f32, 14 over 2 of 64, 11.7 with 2 and 4 (4.9 TB/s), the others 32.8 to 42.7 and 13.0 to 16.9. Instructions and the
-// loads' latency share what is left above the bytes (an issue slot in 7 of 10): 16 elements to a lane or packed arithmetic need registers that cost more warps.
+// loads' latency share what is left above the bytes (an issue slot in 6 of 10): 16 elements to a lane or packed arithmetic need registers that cost more warps.
 template <typename TI> constexpr int kAppendHeads = sizeof(TI) == 2 ? 4 : 2;
 constexpr int kAppendCtas = 4;
 

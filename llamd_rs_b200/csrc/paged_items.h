@@ -34,7 +34,7 @@ struct PagedPart {
 };
 
 // Query rows (tokens x heads of a group) of a piece that paged_decode.cu can take (one token of a wide group), and of one that it is given where a
-// stretch has several tokens. Pieces of 16 rows: 32 take four times the registers of 8 and half the
+// stretch has several tokens. Pieces of 16 rows: 32 take 255 registers where 8 take 149 and 16 take 210 (at 128 elements; 203, 93 and 131 at 64) and half the
 // CTAs (8 sequences behind 512 shared positions 12.1 us against 6.6, 64 with 3 new tokens behind 3500 102.9 against 90.7), 8 read K and V
 // twice as often (102.9).
 constexpr int kPagedSmallRows = 32, kPagedPieceRows = 16;

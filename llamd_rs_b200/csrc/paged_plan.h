@@ -41,7 +41,7 @@ constexpr double kHalfCost = 0.85, kPieceCost = 2.0, kPartCost = 2.0, kJoinCost 
 
 // Small and large pieces of one batch, one launch after the other, leave first HBM and then the tensor cores waiting; at the same time, each on SMs of its
 // own, neither. What they take, in SM-microseconds: an SM draws about 85 GB/s from HBM where all do not draw at once, a block of two tiles
-// takes 2 us. Each has to be worth something (kBesideLeast us on all SMs), or the two kernels run in turn (measured: 100 sequences behind 1024 shared
+// takes 2 us (1.7 at 64 elements; 2 stands for both). Each has to be worth something (kBesideLeast us on all SMs), or the two kernels run in turn (measured: 100 sequences behind 1024 shared
 // positions, 5 query heads to a kv head, 38 us in turn, 33 beside each other; 100 behind 1024, 8 to a kv head, 37 and 28; at worst 200 behind 256, 28 and 29).
 constexpr double kSmBytes = 85e3, kBlockMicros = 2.0, kBesideLeast = 0.5;
 

@@ -18,8 +18,9 @@
 // most 2^8, and the sums are exact in the same way), which after the first block hardly ever happens. In f16 P is taken 2^7 times as large until the end,
 // so that it is at most 2^15 and a normal number down to 2^-21 of the maximum's (131072 positions 15 nats below another came out 2.6 % too small without).
 // What it measured (bf16, 32 heads over 4 kv heads of 128): one prompt of 8192 positions 430 us, 1.27 PFLOP/s or 0.78 of the dense rate (0.63 where the
-// power cap has brought the clock down); 9 of 1 to 1999 positions in one batch 120 us. Without any product the softmax warps alone take 645k of the
-// first's 712k cycles: 128 scores out of TMEM, their maximum, exponentials, sums and roundings, to a thread and block, bound it. A piece costs 3 us to
+// power cap has brought the clock down); 9 of 1 to 1999 positions in one batch 120 us. A copy that issues no product took 645k of the
+// first's 712k cycles: the softmax's chain to a thread and block -- 128 scores out of TMEM, their maximum, exponentials, sums, roundings -- bounds it, by its latency:
+// special function units 47 %, tensor pipe 42 %, issue slots 35 % busy. A piece costs 3 us to
 // begin and end: one prompt of 512 positions takes 12.7 us for 1.4 us of products.
 // Slots of the last block behind the last position are masked in S and set to zero in V's tile before the product reads it.
 // Every wait is bounded; one that runs out raises a flag that the host reads (llamd_fwd_paged_status), and outputs that are not complete are NaN.

@@ -79,7 +79,8 @@ def _refuse(what):
 
 
 def rope_table(rows: int, rot: int, freq_base: float, scaling: str = "none", factor: float = 1.0, original: int = 0) -> np.ndarray:
-    """[rows][rot / 2][2] sines and cosines for ``Batch.append`` (llamd_cuda_rope_table_scaled)."""
+    """[rows][rot / 2][2] sines and cosines for ``Batch.append`` (llamd_cuda_rope_table_scaled). "by_frequency" ramps in the number of turns; a checkpoint
+    whose loader ramps over the pair's index needs a table of its own, which append takes as well."""
     if scaling not in SCALING:
         raise Unsupported(f"rope scaling {scaling!r}: one of {', '.join(SCALING)}")
     if rows < 0 or rot < 2 or rot % 2:
