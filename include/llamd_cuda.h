@@ -445,7 +445,7 @@ void llamd_fwd_attention_prefill(const float *q, const float *kc, const float *v
  * pools) LLAMD_PAGED_F16 or _BF16. NULL and a message where refused. */
 void *llamd_cuda_paged_new(int n_head, int n_head_kv, int hd, int page_size, int type);
 /* Launches that read the batch may still be under way, a graph may be captured meanwhile: nothing is waited for. The library keeps the batch's memory (up to
- * 1 GB on the device, 256 MB pinned) for the next ones. Any thread. */
+ * 512 MB on the device, 256 MB pinned) for the next ones. Any thread. */
 void llamd_cuda_paged_free(void *batch);
 /* pages: [n_seq][pages_stride], ids below n_pages (the pools' size), of each sequence the first
  * ceil(kv_len / page_size) are read. q_len may be 0. n_shared: the first n_shared positions (whole pages, the same ids in every
@@ -482,8 +482,8 @@ void llamd_fwd_paged_wait_limit(unsigned long long nanoseconds);
 /* The table of llamd_fwd_paged_append on the host: sine and cosine of r * f_i, f_i = base^(-2i / rot), evaluated in double.
  * scaling 0: as it is; 1: f / factor (positions stretched); 2: base * factor^(rot / (rot - 2)) in place of base; 3: by frequency,
  * f / factor for those that turn less than once over `original` positions, f for those that turn 32 times and more, a ramp
- * between (in the number of turns), and all values times 0.1 ln(factor) + 1. Checkpoints whose loaders ramp over the pair's index, between the indices where the two
- * numbers of turns fall, need a table of their own (single frequencies differ by up to a half); append takes any. */
+ * between (in the number of turns, as the method was published), and all values times 0.1 ln(factor) + 1. Checkpoints whose loaders ramp over the pair's index, between the indices where the two
+ * numbers of turns fall, need a table of their own (single frequencies differ by 40 to 60 %); append takes any. */
 int llamd_cuda_rope_table_scaled(float *host_out, int rows, int rot, float freq_base, int scaling, float factor, int original);
 
 #ifdef __cplusplus

@@ -33,7 +33,7 @@ bool side_ready() {
 
 // Device memory needs no event: whatever still reads it is in front of the next batch's copy on the same stream. Pinned memory goes with the event behind
 // the copy out of it.
-Kept g_device(16, (size_t)1 << 30), g_pinned(16, (size_t)256 << 20);
+Kept g_device(16, (size_t)512 << 20), g_pinned(16, (size_t)256 << 20);
 
 // What the two had no room for goes back to the system. Not where a batch is freed: that may be inside a capture, on any thread, and is not to wait.
 void give_back() {
@@ -94,9 +94,14 @@ struct Batch {
         b = g_device.take(n);
         if (b.p) return true;
         n = Kept::rounded(n);
-        if (cudaMalloc((void **)&b.p, n) != cudaSuccess) {
-            b = {};
-            return fail("paged batch: device memory");
+        if (cudaMalloc((void **)&b.p, n) != cudaSuccess) {  // (what is kept may be what is missing)
+            cudaGetLastError();
+            g_device.let_go();
+            give_back();
+            if (cudaMalloc((void **)&b.p, n) != cudaSuccess) {
+                b = {};
+                return fail("paged batch: device memory");
+            }
         }
         b.n = n;
         return true;

@@ -60,6 +60,16 @@ class Kept {
             drop(least);
         }
     }
+    // Everything kept is to go: memory has run short elsewhere.
+    void let_go() {
+        std::lock_guard<std::mutex> hold(lock_);
+        try {
+            gone_.reserve(gone_.size() + blocks_.size());
+        } catch (const std::exception &) {
+            return;
+        }
+        while (!blocks_.empty()) drop(blocks_.size() - 1);
+    }
     // What keep() had no room for since the last time.
     std::vector<KeptBlock> gone() {
         std::lock_guard<std::mutex> hold(lock_);

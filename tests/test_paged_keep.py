@@ -23,6 +23,7 @@ size_t want(size_t n, size_t *have) {
     *have = b.n;
     return (size_t)b.p;
 }
+void let_go() { k->let_go(); }
 void give(size_t p, size_t n) { KeptBlock b; b.p = (uint8_t *)p, b.n = n; k->keep(b); }
 size_t n_made() { return made; }
 size_t gone(size_t *out, size_t room) {
@@ -124,6 +125,17 @@ def test_a_small_batch_does_not_take_a_large_block(keep):
     big = want(keep, 64 << 20)
     keep.give(*big)
     assert want(keep, 1000)[0] != big[0] and want(keep, 20 << 20)[0] == big[0]
+
+
+def test_all_of_it_can_go(keep):
+    keep.start(6, 1 << 30)
+    blocks = [want(keep, n << 20) for n in (1, 5, 40)]
+    for b in blocks:
+        keep.give(*b)
+    keep.let_go()
+    assert sorted(gone(keep)) == sorted(b[0] for b in blocks) and not gone(keep)
+    made = keep.n_made()
+    assert want(keep, 1 << 20)[0] == made + 1
 
 
 def test_threads(keep):
