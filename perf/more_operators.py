@@ -272,7 +272,7 @@ def _store(y, s, pages, scales):
     held = (last - s["pos"] // BLOCK * BLOCK).clamp(0, BLOCK)                           # rows that the block had
     most = torch.zeros(P * B, K, device="cuda").index_reduce_(0, of, y.abs().amax(-1), "amax")
     fraction, e = torch.frexp(most / high)
-    e = torch.where(fraction == 0.5, e - 1, e).clamp(low_e, high_e)
+    e = torch.where(fraction == 0.5, e - 1, e).masked_fill(most == 0, low_e).clamp(low_e, high_e)
     rows = torch.zeros(P * B, dtype=torch.long, device="cuda").index_put_((of,), held)
     was = sc.permute(0, 2, 1).reshape(P * B, K).int() - 127
     touched = torch.zeros(P * B, dtype=torch.bool, device="cuda").index_fill_(0, of, True)
