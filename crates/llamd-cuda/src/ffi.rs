@@ -164,10 +164,13 @@ unsafe extern "C" {
     pub fn llamd_fwd_matmul_f32_tokens(w: *const f32, x: *const f32, out: *mut f32, k: c_int, rows: c_int, ntok: c_int);
     pub fn llamd_fwd_attention_prefill(q: *const f32, kc: *const f32, vc: *const f32, out: *mut f32, scores: *mut f32, n_head: c_int, n_head_kv: c_int, hd: c_int, meta: *const i32, max_kv: c_int, ntok: c_int, n_kv_max: c_int);
     pub fn llamd_cuda_paged_new(n_head: c_int, n_head_kv: c_int, hd: c_int, page_size: c_int, type_: c_int) -> *mut c_void;
+    pub fn llamd_cuda_paged_new8(n_head: c_int, n_head_kv: c_int, hd: c_int, page_size: c_int, type_: c_int, cache: c_int) -> *mut c_void;
     pub fn llamd_cuda_paged_free(batch: *mut c_void);
     pub fn llamd_cuda_paged_set(batch: *mut c_void, n_seq: c_int, q_len: *const i32, kv_len: *const i32, pages: *const i32, pages_stride: c_int, n_pages: c_int, n_shared: c_int) -> c_int;
     pub fn llamd_fwd_paged_append(batch: *const c_void, q: *const c_void, k: *const c_void, v: *const c_void, in_type: c_int, q_stride: usize, k_stride: usize, v_stride: usize, wq: *const f32, wk: *const f32, eps: f32, rope_tab: *const f32, rope_rows: c_int, rot: c_int, interleaved: c_int, q_out: *mut c_void, out_stride: usize, k_pages: *mut c_void, v_pages: *mut c_void) -> c_int;
+    pub fn llamd_fwd_paged_append8(batch: *const c_void, q: *const c_void, k: *const c_void, v: *const c_void, in_type: c_int, q_stride: usize, k_stride: usize, v_stride: usize, wq: *const f32, wk: *const f32, eps: f32, rope_tab: *const f32, rope_rows: c_int, rot: c_int, interleaved: c_int, q_out: *mut c_void, out_stride: usize, k_pages: *mut c_void, v_pages: *mut c_void, k_scales: *mut u8, v_scales: *mut u8) -> c_int;
     pub fn llamd_fwd_paged_attention(batch: *const c_void, q: *const c_void, q_stride: usize, k_pages: *const c_void, v_pages: *const c_void, out: *mut c_void, out_stride: usize, out_f32: c_int, scale: f32) -> c_int;
+    pub fn llamd_fwd_paged_attention8(batch: *const c_void, q: *const c_void, q_stride: usize, k_pages: *const c_void, v_pages: *const c_void, k_scales: *const u8, v_scales: *const u8, out: *mut c_void, out_stride: usize, out_f32: c_int, scale: f32) -> c_int;
     pub fn llamd_fwd_paged_status() -> c_int;
     pub fn llamd_fwd_paged_wait_limit(nanoseconds: c_ulonglong);
     pub fn llamd_cuda_rope_table_scaled(host_out: *mut f32, rows: c_int, rot: c_int, freq_base: f32, scaling: c_int, factor: f32, original: c_int) -> c_int;

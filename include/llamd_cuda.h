@@ -444,6 +444,14 @@ void llamd_fwd_attention_prefill(const float *q, const float *kc, const float *v
 /* hd 64 or 128; n_head up to 4096, n_head / n_head_kv a whole number up to 64; page_size a power of two, 16 to 4096; type (of q_out, out and the
  * pools) LLAMD_PAGED_F16 or _BF16. NULL and a message where refused. */
 void *llamd_cuda_paged_new(int n_head, int n_head_kv, int hd, int page_size, int type);
+/* ---- the same over caches in 8 bits: half the bytes. Pools [n_pages][n_head_kv][page_size][hd] of codes, and beside each a pool of scales
+ * [n_pages][n_head_kv][page_size / 16]: a byte b for each 16 neighbouring positions of a page and head. A value is its code times 2^(b - 127) (e8m0). Codes are
+ * whole numbers from -127 to 127 (I8) or e4m3 (its two NaN codes count as 480 and -480). */
+#define LLAMD_PAGED_I8 3
+#define LLAMD_PAGED_E4M3 4
+/* As above; type is q_out's and out's, cache one of the two. Set and freed as above; goes with append8 and attention8 only, as a batch of the former with
+ * append and attention only. */
+void *llamd_cuda_paged_new8(int n_head, int n_head_kv, int hd, int page_size, int type, int cache);
 /* Launches that read the batch may still be under way, a graph may be captured meanwhile: nothing is waited for. The library keeps the batch's memory (up to
  * 512 MB on the device, 256 MB pinned) for the next ones. Any thread. */
 void llamd_cuda_paged_free(void *batch);
@@ -467,12 +475,24 @@ int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int
 int llamd_fwd_paged_append(const void *batch, const void *q, const void *k, const void *v, int in_type, size_t q_stride,
                            size_t k_stride, size_t v_stride, const float *wq, const float *wk, float eps, const float *rope_tab,
                            int rope_rows, int rot, int interleaved, void *q_out, size_t out_stride, void *k_pages, void *v_pages);
+/* The same into a cache in 8 bits. A block's scale is the least power of two with which its new values fit (between 2^-24 and 2^9 for I8, 2^-15 and 2^7 for
+ * E4M3: every value is then exact in f16), and no less than it was where the block holds older positions of the sequence: their codes are rounded
+ * again when it grows. Values are rounded to even; larger ones than the largest scale takes (65024, 57344), infinities among them, become the largest; a NaN becomes 0. Rows and scales
+ * without new tokens, and rows behind a sequence's last, stay as they are. A page that new tokens go to belongs to one
+ * sequence: refused where two of the batch's would write to one. */
+int llamd_fwd_paged_append8(const void *batch, const void *q, const void *k, const void *v, int in_type, size_t q_stride,
+                            size_t k_stride, size_t v_stride, const float *wq, const float *wk, float eps, const float *rope_tab,
+                            int rope_rows, int rot, int interleaved, void *q_out, size_t out_stride, void *k_pages, void *v_pages,
+                            uint8_t *k_scales, uint8_t *v_scales);
 /* out[token][head] = softmax(scale * q . k) v over the positions up to the token's own; scale > 0. q and out in the batch's type, or out in f32
  * (out_f32: the same sums, not rounded); rows start at 16 bytes. Slots behind a sequence's last position may hold
  * anything, NaN and infinities too; values that some of the batch's tokens attend to are finite, or other tokens' outputs may be NaN as well (a weight of
  * 0 times infinity). Part of a large batch may run on a second stream of the library's, which the call joins to its own. 0 / -1 as above. */
 int llamd_fwd_paged_attention(const void *batch, const void *q, size_t q_stride, const void *k_pages, const void *v_pages, void *out,
                               size_t out_stride, int out_f32, float scale);
+/* The same over a cache in 8 bits, of which every code of a position that is attended to, and its scale, is read as it stands: scales as append8 makes them. */
+int llamd_fwd_paged_attention8(const void *batch, const void *q, size_t q_stride, const void *k_pages, const void *v_pages,
+                               const uint8_t *k_scales, const uint8_t *v_scales, void *out, size_t out_stride, int out_f32, float scale);
 /* 0 while every wait inside the attention's kernels has been met; otherwise 1 + the first block whose wait ran out, handed out once. Outputs that are
  * then not complete are NaN, and append and attention refuse (cudaErrorTimeout) until it has been read. Synchronises the stream. */
 int llamd_fwd_paged_status(void);

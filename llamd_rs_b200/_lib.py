@@ -150,6 +150,9 @@ SIGNATURES = {
     "llamd_fwd_matmul_f32_tokens": (None, [vp, vp, vp, i32, i32, i32]),
     "llamd_fwd_attention_prefill": (None, [vp, vp, vp, vp, vp, i32, i32, i32, vp, i32, i32, i32]),
     "llamd_cuda_paged_new": (vp, [i32, i32, i32, i32, i32]),
+    "llamd_cuda_paged_new8": (vp, [i32, i32, i32, i32, i32, i32]),
+    "llamd_fwd_paged_append8": (i32, [vp, vp, vp, vp, i32, sz, sz, sz, vp, vp, f32, vp, i32, i32, i32, vp, sz, vp, vp, vp, vp]),
+    "llamd_fwd_paged_attention8": (i32, [vp, vp, sz, vp, vp, vp, vp, vp, sz, i32, f32]),
     "llamd_cuda_paged_free": (None, [vp]),
     "llamd_cuda_paged_set": (i32, [vp, i32, vp, vp, vp, i32, i32, i32]),
     "llamd_fwd_paged_append": (i32, [vp, vp, vp, vp, i32, sz, sz, sz, vp, vp, f32, vp, i32, i32, i32, vp, sz, vp, vp]),

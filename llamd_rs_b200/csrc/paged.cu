@@ -10,6 +10,8 @@
 #include <vector>
 
 #include "paged.cuh"
+#include "paged8.cuh"
+#include "paged_append.cuh"
 #include "paged_keep.h"
 #include "paged_plan.h"
 
@@ -49,7 +51,7 @@ void give_back() {
 
 struct Batch {
     PagedView view = {};
-    int type = 0, n_pages = 0, max_kv = 0, sms = 0;  // max_kv: of sequences with new tokens
+    int type = 0, cache = 0, n_pages = 0, max_kv = 0, sms = 0;  // cache: kPagedI8, kPagedE4m3, or 0 for the type's own; max_kv: of sequences with new tokens
     bool ready = false;
     // the device copy of everything below, and the pinned memory it is made in, with the event behind the copy
     KeptBlock dev, host;
@@ -58,6 +60,9 @@ struct Batch {
     const int32_t *begin = nullptr;                      // large: each CTA's
     const PagedMerge *merge = nullptr;
     const PagedPart *part = nullptr;
+    const PagedBlock *block = nullptr;  // of a cache in 8 bits
+    int n_block = 0;
+    bool shared_write = false;  // two sequences have new tokens in one page
     bool beside = false;
     int n_small = 0, small_rows = 0, n_ctas = 0, n_merge = 0, most = 0;
     KeptBlock partial;
@@ -169,6 +174,25 @@ const char *check_lengths(const Batch &b, int n_seq, const int32_t *q_len, const
     return nullptr;
 }
 
+// What a cache in 8 bits needs of a batch: where its new tokens meet scale blocks.
+void blocks_of(std::vector<PagedBlock> &block, int n_seq, const int32_t *q_len, const int32_t *kv_len) {
+    for (int s = 0, t = 0; s < n_seq; t += q_len[s], s++)
+        for (int pos = kv_len[s] - q_len[s]; pos < kv_len[s];) {
+            const int n = std::min(kScaleBlock - pos % kScaleBlock, kv_len[s] - pos);
+            block.push_back({t + pos - (kv_len[s] - q_len[s]), n});
+            pos += n;
+        }
+}
+// Do two new tokens' places share a page that two sequences list, or one twice?
+bool writes_shared(int page, int n_seq, const int32_t *q_len, const int32_t *kv_len, const int32_t *pages, int pages_stride) {
+    std::vector<int32_t> written;
+    for (int s = 0; s < n_seq; s++)
+        if (q_len[s])
+            for (int i = (kv_len[s] - q_len[s]) / page; i <= (kv_len[s] - 1) / page; i++) written.push_back(pages[(size_t)s * pages_stride + i]);
+    std::sort(written.begin(), written.end());
+    return std::adjacent_find(written.begin(), written.end()) != written.end();
+}
+
 // ---- append --------------------------------------------------------------------------------------------------------------
 //
 //   y = x / sqrt(mean(x^2) + eps) * w        per head of q and k (weights given), in f32
@@ -184,38 +208,6 @@ const char *check_lengths(const Batch &b, int n_seq, const int32_t *q_len, const
 // loads' latency share what is left above the bytes (an issue slot in 6 of 10): 16 elements to a lane or packed arithmetic need registers that cost more warps.
 template <typename TI> constexpr int kAppendHeads = sizeof(TI) == 2 ? 4 : 2;
 constexpr int kAppendCtas = 4;
-
-struct AppendParams {
-    PagedView b;
-    const void *q, *k, *v;
-    size_t q_stride, k_stride, v_stride, out_stride;  // elements between tokens
-    const float *wq, *wk, *rope;
-    float eps;
-    int rot, sms, tasks, q_tasks, kv_tasks;  // warps to a token, to its q heads, to its k or v heads
-    void *q_out, *k_pages, *v_pages;
-};
-
-// 4 neighbouring elements as they lie, and in f32
-template <typename T> struct Four {
-    uint2 v;
-    __device__ __forceinline__ void load(const T *p, bool aligned) {
-        if (aligned) {
-            v = __ldcs(reinterpret_cast<const uint2 *>(p));
-        } else {
-            const uint16_t *h = reinterpret_cast<const uint16_t *>(p);
-            v = make_uint2(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16);
-        }
-    }
-    __device__ __forceinline__ void get(float *x) const {
-        const float2 f = Half16<T>::to_f32(v.x), g = Half16<T>::to_f32(v.y);
-        x[0] = f.x, x[1] = f.y, x[2] = g.x, x[3] = g.y;
-    }
-};
-template <> struct Four<float> {
-    float4 v;
-    __device__ __forceinline__ void load(const float *p, bool aligned) { v = aligned ? __ldcs(reinterpret_cast<const float4 *>(p)) : make_float4(p[0], p[1], p[2], p[3]); }
-    __device__ __forceinline__ void get(float *x) const { x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w; }
-};
 
 // TI: the inputs' type, T: the cache's.
 template <typename TI, typename T, int HD, bool INTERLEAVED, bool ALIGNED>
@@ -322,7 +314,7 @@ using namespace llamd;
 
 extern "C" {
 
-void *llamd_cuda_paged_new(int n_head, int n_head_kv, int hd, int page_size, int type) {
+static void *paged_new(int n_head, int n_head_kv, int hd, int page_size, int type, int cache) {
     if (n_head < 1 || n_head > 4096 || n_head_kv < 1 || n_head % n_head_kv || n_head / n_head_kv > 64 || (hd != 64 && hd != 128) || page_size < 16 || page_size > 4096 ||
         (page_size & (page_size - 1)) || (type != kPagedF16 && type != kPagedBf16)) {
         set_error_msg("paged batch: up to 4096 heads of 64 or 128 elements, up to 64 query heads to a kv head, pages of 16 to 4096 positions (a power of two), f16 or bf16");
@@ -335,7 +327,7 @@ void *llamd_cuda_paged_new(int n_head, int n_head_kv, int hd, int page_size, int
         return nullptr;
     }
     b->view.n_head = n_head, b->view.n_head_kv = n_head_kv, b->view.group = n_head / n_head_kv, b->view.hd = hd, b->view.page = page_size;
-    b->type = type;
+    b->type = type, b->cache = cache;
     int device = 0;
     if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&b->sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) {
         set_error(cudaGetLastError(), "paged batch: device");
@@ -343,6 +335,20 @@ void *llamd_cuda_paged_new(int n_head, int n_head_kv, int hd, int page_size, int
         return nullptr;
     }
     return b;
+}
+
+void *llamd_cuda_paged_new(int n_head, int n_head_kv, int hd, int page_size, int type) { return paged_new(n_head, n_head_kv, hd, page_size, type, 0); }
+
+void *llamd_cuda_paged_new8(int n_head, int n_head_kv, int hd, int page_size, int type, int cache) {
+    if (cache != kPagedI8 && cache != kPagedE4m3) {
+        set_error_msg("paged batch: a cache in 8 bits is i8 or e4m3");
+        return nullptr;
+    }
+    if (n_head_kv > 0 && n_head / n_head_kv > kPagedSmallRows) {
+        set_error_msg("paged batch: up to 32 query heads to a kv head of a cache in 8 bits");
+        return nullptr;
+    }
+    return paged_new(n_head, n_head_kv, hd, page_size, type, cache);
 }
 
 void llamd_cuda_paged_free(void *batch) { delete (Batch *)batch; }
@@ -363,8 +369,14 @@ int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int
     }
     if ((long long)n_seq * v.table_stride > 0x7fffffffLL) return refuse("paged batch: the tables have more than 2^31 entries");
     Plan plan;
+    std::vector<PagedBlock> block;
+    bool shared_write = false;
     try {
-        make_plan(plan, v, q_len, kv_len, b->sms);
+        make_plan(plan, v, q_len, kv_len, b->sms, b->cache != 0);
+        if (b->cache) {
+            blocks_of(block, n_seq, q_len, kv_len);
+            shared_write = writes_shared(v.page, n_seq, q_len, kv_len, pages, pages_stride);
+        }
     } catch (const std::exception &) {
         return refuse("paged batch: out of host memory");
     }
@@ -372,7 +384,7 @@ int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int
     size_t bytes = 0;
     const size_t o_token = section<PagedToken>(bytes, v.tokens), o_table = section<int32_t>(bytes, (size_t)n_seq * v.table_stride), o_small = section<PagedItem>(bytes, plan.small.size()),
                  o_large = section<PagedItem>(bytes, plan.large.size()), o_begin = section<int32_t>(bytes, plan.begin.size()),
-                 o_merge = section<PagedMerge>(bytes, plan.merge.size()), o_part = section<PagedPart>(bytes, plan.part.size());
+                 o_merge = section<PagedMerge>(bytes, plan.merge.size()), o_part = section<PagedPart>(bytes, plan.part.size()), o_block = section<PagedBlock>(bytes, block.size());
     if (plan.beside && !side_ready()) {
         set_error(cudaGetLastError(), "paged batch: side stream");
         return -1;
@@ -388,6 +400,7 @@ int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int
     put(o_begin, plan.begin.data(), plan.begin.size() * sizeof(int32_t));
     put(o_merge, plan.merge.data(), plan.merge.size() * sizeof(PagedMerge));
     put(o_part, plan.part.data(), plan.part.size() * sizeof(PagedPart));
+    put(o_block, block.data(), block.size() * sizeof(PagedBlock));
     PagedToken *token = (PagedToken *)(b->host.p + o_token);
     int32_t *table = (int32_t *)(b->host.p + o_table);
     for (int s = 0, t = 0; s < n_seq; s++) {
@@ -402,6 +415,8 @@ int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int
     b->begin = (const int32_t *)(b->dev.p + o_begin);
     b->merge = (const PagedMerge *)(b->dev.p + o_merge);
     b->part = (const PagedPart *)(b->dev.p + o_part);
+    b->block = (const PagedBlock *)(b->dev.p + o_block);
+    b->n_block = (int)block.size(), b->shared_write = shared_write;
     b->beside = plan.beside;
     b->n_small = (int)plan.small.size(), b->small_rows = plan.small_rows, b->n_ctas = (int)plan.begin.size() - 1, b->n_merge = (int)plan.merge.size(), b->most = plan.most;
     b->partial_rows = plan.rows;
@@ -415,11 +430,9 @@ int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int
     return 0;
 }
 
-int llamd_fwd_paged_append(const void *batch, const void *q, const void *k, const void *v, int in_type, size_t q_stride, size_t k_stride, size_t v_stride,
-                            const float *wq, const float *wk, float eps, const float *rope_tab, int rope_rows, int rot, int interleaved, void *q_out,
-                            size_t out_stride, void *k_pages, void *v_pages) {
-    Batch *b = (Batch *)batch;
-    if (!b || !b->ready) return refuse("paged append: the batch is not set");
+// Both appends' checks and parameters. 1: to be launched, 0: nothing to do, -1: refused.
+static int append_of(Batch *b, AppendParams &p, bool &aligned, const void *q, const void *k, const void *v, int in_type, size_t q_stride, size_t k_stride, size_t v_stride,
+                     const float *wq, const float *wk, float eps, const float *rope_tab, int rope_rows, int rot, void *q_out, size_t out_stride, void *k_pages, void *v_pages) {
     if (error_code()) return -1;
     if (gave_up()) return -1;
     const PagedView &g = b->view;
@@ -433,14 +446,27 @@ int llamd_fwd_paged_append(const void *batch, const void *q, const void *k, cons
     if (!aligned16(q_out) || out_stride % 8 || !aligned16(k_pages) || !aligned16(v_pages)) return refuse("paged append: outputs start at 16 bytes");
     const uintptr_t odd = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v, odd_w = (uintptr_t)wq | (uintptr_t)wk;
     if (odd % (in_type == kPagedF32 ? 4 : 2) || odd_w % 4) return refuse("paged append: an input starts inside an element");
-    if (!b->note_graph()) return -1;
-    AppendParams p = {};
+    p = {};
     p.b = g, p.sms = b->sms;
     p.q = q, p.k = k, p.v = v, p.q_stride = q_stride, p.k_stride = k_stride, p.v_stride = v_stride, p.out_stride = out_stride;
     p.wq = wq, p.wk = wk, p.eps = eps, p.rope = rope_tab, p.rot = rot;
     p.q_out = q_out, p.k_pages = k_pages, p.v_pages = v_pages;
     const size_t per16 = in_type == kPagedF32 ? 4 : 8;
-    const bool aligned = aligned16(q) && aligned16(k) && aligned16(v) && !(q_stride % per16) && !(k_stride % per16) && !(v_stride % per16) && aligned16(wq) && aligned16(wk);
+    aligned = aligned16(q) && aligned16(k) && aligned16(v) && !(q_stride % per16) && !(k_stride % per16) && !(v_stride % per16) && aligned16(wq) && aligned16(wk);
+    return 1;
+}
+
+int llamd_fwd_paged_append(const void *batch, const void *q, const void *k, const void *v, int in_type, size_t q_stride, size_t k_stride, size_t v_stride,
+                            const float *wq, const float *wk, float eps, const float *rope_tab, int rope_rows, int rot, int interleaved, void *q_out,
+                            size_t out_stride, void *k_pages, void *v_pages) {
+    Batch *b = (Batch *)batch;
+    if (!b || !b->ready) return refuse("paged append: the batch is not set");
+    if (b->cache) return refuse("paged append: the batch's cache is in 8 bits");
+    AppendParams p;
+    bool aligned;
+    const int go = append_of(b, p, aligned, q, k, v, in_type, q_stride, k_stride, v_stride, wq, wk, eps, rope_tab, rope_rows, rot, q_out, out_stride, k_pages, v_pages);
+    if (go < 1) return go;
+    if (!b->note_graph()) return -1;
     if (b->type == kPagedF16) {
         if (in_type == kPagedF32) append_launch<float, __half>(p, interleaved != 0, aligned);
         else append_launch<__half, __half>(p, interleaved != 0, aligned);
@@ -451,10 +477,26 @@ int llamd_fwd_paged_append(const void *batch, const void *q, const void *k, cons
     return error_code() ? -1 : 0;
 }
 
-int llamd_fwd_paged_attention(const void *batch, const void *q, size_t q_stride, const void *k_pages, const void *v_pages, void *out, size_t out_stride,
-                               int out_f32, float scale) {
+int llamd_fwd_paged_append8(const void *batch, const void *q, const void *k, const void *v, int in_type, size_t q_stride, size_t k_stride, size_t v_stride,
+                            const float *wq, const float *wk, float eps, const float *rope_tab, int rope_rows, int rot, int interleaved, void *q_out,
+                            size_t out_stride, void *k_pages, void *v_pages, uint8_t *k_scales, uint8_t *v_scales) {
     Batch *b = (Batch *)batch;
-    if (!b || !b->ready) return refuse("paged attention: the batch is not set");
+    if (!b || !b->ready) return refuse("paged append: the batch is not set");
+    if (!b->cache) return refuse("paged append: the batch's cache is not in 8 bits");
+    AppendParams p;
+    bool aligned;
+    const int go = append_of(b, p, aligned, q, k, v, in_type, q_stride, k_stride, v_stride, wq, wk, eps, rope_tab, rope_rows, rot, q_out, out_stride, k_pages, v_pages);
+    if (go < 1) return go;
+    if (!k_scales || !v_scales) return refuse("paged append: a buffer is missing");
+    if (b->shared_write) return refuse("paged append: two new tokens' pages are one, whose scales both would change");
+    if ((long long)b->view.tokens * b->view.n_head + 2LL * b->n_block * b->view.n_head_kv > 1LL << 30) return refuse("paged append: too many tokens");
+    if (!b->note_graph()) return -1;
+    paged_append8_launch(p, Append8{b->block, b->n_block, k_scales, v_scales}, in_type, b->type, b->cache, interleaved != 0, aligned);
+    return error_code() ? -1 : 0;
+}
+
+static int attention_of(Batch *b, const void *q, size_t q_stride, const void *k_pages, const void *v_pages, const uint8_t *k_scales, const uint8_t *v_scales, void *out,
+                        size_t out_stride, int out_f32, float scale) {
     if (error_code()) return -1;
     if (gave_up()) return -1;
     const PagedView &g = b->view;
@@ -469,6 +511,7 @@ int llamd_fwd_paged_attention(const void *batch, const void *q, size_t q_stride,
     PagedAttn a = {};
     a.b = g, a.q = q, a.k_pages = k_pages, a.v_pages = v_pages, a.out = out, a.q_stride = q_stride, a.out_stride = out_stride;
     a.out_f32 = out_f32, a.scale_log2 = scale * 1.4426950408889634f;
+    a.k_scales = k_scales, a.v_scales = v_scales;
     a.part_o = (float *)b->partial.p, a.part_ml = (float2 *)(b->partial.p + b->partial_rows * g.hd * sizeof(float));
     if (b->beside) LLAMD_TRY(cudaEventRecord(g_fork, stream()), "paged attention: fork");
     if (b->n_ctas) {  // (first: its CTAs need whole SMs, and what it refuses leaves nothing launched)
@@ -478,7 +521,9 @@ int llamd_fwd_paged_attention(const void *batch, const void *q, size_t q_stride,
     if (b->n_small) {
         a.item = b->small;
         if (b->beside) LLAMD_TRY(cudaStreamWaitEvent(g_side, g_fork, 0), "paged attention: fork");
-        paged_decode_launch(a, b->type, b->n_small, b->small_rows, b->beside ? g_side : stream());
+        const cudaStream_t to = b->beside ? g_side : stream();
+        if (b->cache) paged_decode8_launch(a, b->type, b->cache, b->n_small, b->small_rows, to);
+        else paged_decode_launch(a, b->type, b->n_small, b->small_rows, to);
     }
     if (b->beside) {
         LLAMD_TRY(cudaEventRecord(g_join, g_side), "paged attention: join");
@@ -487,6 +532,23 @@ int llamd_fwd_paged_attention(const void *batch, const void *q, size_t q_stride,
     if (error_code()) return -1;  // (nothing joins what was not made)
     if (b->n_merge) paged_merge_launch(a, b->type, b->merge, b->part, b->n_merge, b->most, b->sms);
     return error_code() ? -1 : 0;
+}
+
+int llamd_fwd_paged_attention(const void *batch, const void *q, size_t q_stride, const void *k_pages, const void *v_pages, void *out, size_t out_stride,
+                               int out_f32, float scale) {
+    Batch *b = (Batch *)batch;
+    if (!b || !b->ready) return refuse("paged attention: the batch is not set");
+    if (b->cache) return refuse("paged attention: the batch's cache is in 8 bits");
+    return attention_of(b, q, q_stride, k_pages, v_pages, nullptr, nullptr, out, out_stride, out_f32, scale);
+}
+
+int llamd_fwd_paged_attention8(const void *batch, const void *q, size_t q_stride, const void *k_pages, const void *v_pages, const uint8_t *k_scales,
+                               const uint8_t *v_scales, void *out, size_t out_stride, int out_f32, float scale) {
+    Batch *b = (Batch *)batch;
+    if (!b || !b->ready) return refuse("paged attention: the batch is not set");
+    if (!b->cache) return refuse("paged attention: the batch's cache is not in 8 bits");
+    if (b->view.tokens && (!k_scales || !v_scales)) return refuse("paged attention: a buffer is missing");
+    return attention_of(b, q, q_stride, k_pages, v_pages, k_scales, v_scales, out, out_stride, out_f32, scale);
 }
 
 // The angles' table of llamd_fwd_paged_append, in double and rounded once.

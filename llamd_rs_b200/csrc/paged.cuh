@@ -10,7 +10,7 @@
 
 namespace llamd {
 
-enum { kPagedF16 = 0, kPagedBf16 = 1, kPagedF32 = 2 };
+enum { kPagedF16 = 0, kPagedBf16 = 1, kPagedF32 = 2, kPagedI8 = 3, kPagedE4m3 = 4 };
 
 // A partial result: sums of 2^(s - m) v over the piece's positions (s: the scores times log2 e), in f32, and beside them m and sum 2^(s - m).
 struct PagedAttn {
@@ -23,9 +23,11 @@ struct PagedAttn {
     float scale_log2;  // scale * log2 e
     float *part_o;     // [rows][hd]
     float2 *part_ml;   // [rows] (m, sum)
+    const uint8_t *k_scales, *v_scales;  // of a cache in 8 bits (paged8.cuh)
 };
 
 void paged_decode_launch(const PagedAttn &p, int type, int n_items, int max_rows, cudaStream_t to);
+void paged_decode8_launch(const PagedAttn &p, int type, int cache, int n_items, int max_rows, cudaStream_t to);
 bool paged_gave_up();       // a wait of an earlier attention has run out, and the host has not read it yet
 bool paged_prompt_ready();  // what its launches need beside the batch: false and an error where it cannot be had
 bool paged_prompt_launch(const PagedAttn &p, int type, int n_pages, const int32_t *begin, int n_ctas);  // begin: each CTA's pieces (n_ctas + 1); false and an error: not launched

@@ -1,0 +1,38 @@
+// K/V caches in 8 bits: a page's rows are codes, and each 16 neighbouring positions of a page and kv head have one scale 2^e, kept as the byte e + 127
+// ([n_pages][n_head_kv][page / 16]). A value is its code times the scale. With powers of two every value is exact in f16 and bf16, and codes that are
+// taken to a larger scale are rounded once, whatever their history; they cost at most one of an i8 code's 8 bits, and nothing of e4m3's.
+#pragma once
+#include "paged.cuh"
+
+namespace llamd {
+
+constexpr int kScaleBlock = 16;
+
+// The largest code, and the exponents of an append's scales: between them every value is exact in f16, subnormals included.
+template <int C> struct Cache8;
+template <> struct Cache8<kPagedI8> {
+    static constexpr float kMost = 127.0f;
+    static constexpr int kLow = -24, kHigh = 9;
+    // f16x2 of the codes in bytes 0, 1 (half 0) or 2, 3 (half 1) of x, times 2^-kShift. 1024 + 128 + c is a half whose low byte is c with its sign bit flipped.
+    static constexpr int kShift = 0;
+    template <int HALF> static __device__ __forceinline__ uint32_t f16x2(uint32_t x) {
+        const uint32_t y = __byte_perm(x ^ 0x80808080u, 0x64646464u, HALF ? 0x4342 : 0x4140), bias = 0x64806480u;
+        const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&y), *reinterpret_cast<const __half2 *>(&bias));
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+};
+template <> struct Cache8<kPagedE4m3> {
+    static constexpr float kMost = 448.0f;
+    static constexpr int kLow = -15, kHigh = 7;
+    // The code's bits as a half's sign, low exponent bits and high mantissa bits: 2^-8 of its value, subnormals too.
+    static constexpr int kShift = 8;
+    template <int HALF> static __device__ __forceinline__ uint32_t f16x2(uint32_t x) {
+        const uint32_t t = __byte_perm(x, 0, HALF ? 0x3424 : 0x1404);
+        return (t & 0x80008000u) | ((t >> 1) & 0x3F803F80u);
+    }
+};
+
+__device__ __forceinline__ float scale_of(int byte) { return __int_as_float(byte << 23); }             // 2^e of the byte e + 127, 1 to 254
+__device__ __forceinline__ float scale_inverse(int byte) { return __int_as_float((254 - byte) << 23); }  // 2^-e, of 0 to 253
+
+}  // namespace llamd

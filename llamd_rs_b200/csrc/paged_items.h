@@ -9,6 +9,11 @@ struct PagedToken {
     int32_t pos, row;
 };
 
+// A sequence's new tokens that share a scale block of a cache in 8 bits: rows [token, token + n) of the batch, behind the block's older ones.
+struct PagedBlock {
+    int32_t token, n;
+};
+
 // The batch as the kernels see it: device memory that the batch owns, every index checked against the pools when it was made.
 struct PagedView {
     int n_head, n_head_kv, group, hd, page, n_seq, tokens, n_shared, table_stride;

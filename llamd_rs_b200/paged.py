@@ -22,8 +22,11 @@ from ._lib import lib
 from .backend import DevBuf, LlamdError, Malformed, Other, ShapeError, Unsupported
 
 TYPES = {"f16": 0, "bf16": 1, "f32": 2}
-_SIZE = {0: 2, 1: 2, 2: 4}
-_TORCH = {"torch.float16": 0, "torch.bfloat16": 1, "torch.float32": 2}
+CACHES = {"i8": 3, "e4m3": 4}  # in 8 bits
+SCALE_BLOCK = 16  # positions to a scale of theirs
+_SCALES = 5  # (bytes: the exponent plus 127)
+_SIZE = {0: 2, 1: 2, 2: 4, 3: 1, 4: 1, 5: 1}
+_TORCH = {"torch.float16": 0, "torch.bfloat16": 1, "torch.float32": 2, "torch.int8": 3, "torch.float8_e4m3fn": 4, "torch.float8_e8m0fnu": 5, "torch.uint8": 5}
 _seen = {}  # a tensor's dtype -> its number here, filled as they come
 SCALING = {"none": 0, "linear": 1, "base": 2, "by_frequency": 3}
 
@@ -139,21 +142,30 @@ class Pages:
 
 
 class Batch:
-    """One step's sequences over caches of one geometry (llamd_cuda_paged_new)."""
+    """One step's sequences over caches of one geometry (llamd_cuda_paged_new). ``cache``: None, the pools hold ``dtype``, or "i8" or "e4m3", codes in 8 bits
+    beside pools of scales [n_pages][n_head_kv][page_size / 16] (llamd_cuda_paged_new8), which ``append`` and ``attention`` then take as well."""
 
-    def __init__(self, n_head: int, n_head_kv: int, head_dim: int, page_size: int, dtype: str = "f16"):
+    def __init__(self, n_head: int, n_head_kv: int, head_dim: int, page_size: int, dtype: str = "f16", cache: str | None = None):
         self.ptr = None
         if dtype not in ("f16", "bf16"):
             raise Unsupported(f"a paged cache holds f16 or bf16, not {dtype}")
+        if cache is not None and cache not in CACHES:
+            raise Unsupported(f"a paged cache in 8 bits holds {' or '.join(CACHES)}, not {cache}")
         backend._need_device()
         n_head, n_head_kv, head_dim, page_size = (_int(x, "paged batch") for x in (n_head, n_head_kv, head_dim, page_size))
         self.type = TYPES[dtype]
         self.n_head, self.n_head_kv, self.head_dim, self.page_size = n_head, n_head_kv, head_dim, page_size
-        self.ptr = lib().llamd_cuda_paged_new(n_head, n_head_kv, head_dim, page_size, self.type)
+        self.cache = self.type if cache is None else CACHES[cache]
+        if cache is None:
+            self.ptr = lib().llamd_cuda_paged_new(n_head, n_head_kv, head_dim, page_size, self.type)
+        else:
+            self.ptr = lib().llamd_cuda_paged_new8(n_head, n_head_kv, head_dim, page_size, self.type, self.cache)
         if not self.ptr:
             _refuse("paged batch")
         self.tokens, self.n_pages, self.scale = 0, 0, 1.0 / math.sqrt(head_dim)
         self._append, self._attention = lib().llamd_fwd_paged_append, lib().llamd_fwd_paged_attention
+        if cache is not None:
+            self._append, self._attention = lib().llamd_fwd_paged_append8, lib().llamd_fwd_paged_attention8
         self._wait, self._ready = lib().llamd_fwd_wait_stream, lib().llamd_fwd_ready_stream
         self._pool = 0
 
@@ -233,8 +245,8 @@ class Batch:
         return ptr
 
     def append(self, q, k, v, q_out, k_pages, v_pages, rope=None, rot: int | None = None, interleaved: bool = False, q_norm=None, k_norm=None,
-               eps: float = 1e-6, inputs: str | None = None, rope_rows: int | None = None, strides=(None, None, None)) -> None:
-        """llamd_fwd_paged_append. ``inputs`` ("f32" or the cache's type) and ``strides`` (elements between tokens of q, k, v)
+               eps: float = 1e-6, inputs: str | None = None, rope_rows: int | None = None, strides=(None, None, None), k_scales=None, v_scales=None) -> None:
+        """llamd_fwd_paged_append, or _append8 with the scales of a cache in 8 bits. ``inputs`` ("f32" or the cache's type) and ``strides`` (elements between tokens of q, k, v)
         describe buffers that are plain addresses or ``DevBuf``; a tensor says so itself, and its table how many rows it has."""
         if inputs is None:
             it = _type_of(q) if hasattr(q, "data_ptr") else 2
@@ -258,39 +270,53 @@ class Batch:
                 raise Malformed("rope_rows: how many positions the table has")
         else:
             rope_rows = _int(rope_rows, "rope_rows")
-        D, T, t = self.head_dim, self.tokens, self.type
+        D, T, t, c = self.head_dim, self.tokens, self.type, self.cache
         nq, nk = self.n_head * D, self.n_head_kv * D
+        scales = () if c == t and k_scales is None and v_scales is None else self._scales_of(k_scales, v_scales)
         if rot and q_norm is not None and k_norm is not None:
             plain = self._tensors((q, it, T * nq, T), (k, it, T * nk, T), (v, it, T * nk, T), (q_norm, 2, D, None), (k_norm, 2, D, None),
-                                  (rope, 2, rope_rows * rot, None), (q_out, t, T * nq, T), (k_pages, t, self._pool, None), (v_pages, t, self._pool, None))
+                                  (rope, 2, rope_rows * rot, None), (q_out, t, T * nq, T), (k_pages, c, self._pool, None), (v_pages, c, self._pool, None))
             if plain:
                 self._call("append", self._append, _stream_of(q), plain[0], plain[1], plain[2], it, nq, nk, nk, plain[3], plain[4], eps, plain[5], rope_rows, rot,
-                           interleaved, plain[6], nq, plain[7], plain[8])
+                           interleaved, plain[6], nq, plain[7], plain[8], *scales)
                 return
         qp, qs = self._rows(q, nq, it, "q", strides[0])
         kp, ks = self._rows(k, nk, it, "k", strides[1])
         vp, vs = self._rows(v, nk, it, "v", strides[2])
         op, os_ = self._rows(q_out, nq, self.type, "q_out")
-        self._call("append", self._append, _stream_of(q, k, v, q_out, k_pages, v_pages, rope, q_norm, k_norm), qp, kp, vp, it, qs, ks, vs,
+        self._call("append", self._append, _stream_of(q, k, v, q_out, k_pages, v_pages, rope, q_norm, k_norm, k_scales, v_scales), qp, kp, vp, it, qs, ks, vs,
                    None if q_norm is None else self._whole(q_norm, 2, D, "q_norm"), None if k_norm is None else self._whole(k_norm, 2, D, "k_norm"), eps,
                    self._whole(rope, 2, rope_rows * rot, "rope") if rot else None, rope_rows, rot, interleaved, op, os_,
-                   self._whole(k_pages, self.type, self._pool, "k_pages"), self._whole(v_pages, self.type, self._pool, "v_pages"))
+                   self._whole(k_pages, c, self._pool, "k_pages"), self._whole(v_pages, c, self._pool, "v_pages"), *scales)
 
-    def attention(self, q, k_pages, v_pages, out, scale: float | None = None, out_f32: bool | None = None) -> None:
-        """llamd_fwd_paged_attention. ``out_f32`` says of an address that it takes f32; a tensor's type says so itself."""
+    def _scales_of(self, k_scales, v_scales):
+        """The addresses of a cache's scales where it is in 8 bits."""
+        if self.cache == self.type:
+            if k_scales is not None or v_scales is not None:
+                raise Malformed("scales of a cache that is not in 8 bits")
+            return ()
+        if k_scales is None or v_scales is None:
+            raise Malformed("a cache in 8 bits without its scales")
+        n = self._pool // (SCALE_BLOCK * self.head_dim)
+        return self._tensors((k_scales, _SCALES, n, None), (v_scales, _SCALES, n, None)) or (self._whole(k_scales, _SCALES, n, "k_scales"), self._whole(v_scales, _SCALES, n, "v_scales"))
+
+    def attention(self, q, k_pages, v_pages, out, scale: float | None = None, out_f32: bool | None = None, k_scales=None, v_scales=None) -> None:
+        """llamd_fwd_paged_attention, or _attention8 with the scales of a cache in 8 bits. ``out_f32`` says of an address that it takes f32; a tensor's type says so itself."""
         if out_f32 is None:
             out_f32 = hasattr(out, "data_ptr") and _type_of(out) == 2
         n = self.n_head * self.head_dim
         scale = self.scale if scale is None else scale
-        plain = self._tensors((q, self.type, self.tokens * n, self.tokens), (k_pages, self.type, self._pool, None), (v_pages, self.type, self._pool, None),
+        c = self.cache
+        scales = () if c == self.type and k_scales is None and v_scales is None else self._scales_of(k_scales, v_scales)
+        plain = self._tensors((q, self.type, self.tokens * n, self.tokens), (k_pages, c, self._pool, None), (v_pages, c, self._pool, None),
                               (out, 2 if out_f32 else self.type, self.tokens * n, self.tokens))
         if plain:
-            self._call("attention", self._attention, _stream_of(q), plain[0], n, plain[1], plain[2], plain[3], n, out_f32, scale)
+            self._call("attention", self._attention, _stream_of(q), plain[0], n, plain[1], plain[2], *scales, plain[3], n, out_f32, scale)
             return
         qp, qs = self._rows(q, n, self.type, "q")
         op, os_ = self._rows(out, n, 2 if out_f32 else self.type, "out")
-        kp, vp = self._whole(k_pages, self.type, self._pool, "k_pages"), self._whole(v_pages, self.type, self._pool, "v_pages")
-        self._call("attention", self._attention, _stream_of(q, k_pages, v_pages, out), qp, qs, kp, vp, op, os_, out_f32, scale)
+        kp, vp = self._whole(k_pages, c, self._pool, "k_pages"), self._whole(v_pages, c, self._pool, "v_pages")
+        self._call("attention", self._attention, _stream_of(q, k_pages, v_pages, out, k_scales, v_scales), qp, qs, kp, vp, *scales, op, os_, out_f32, scale)
 
     def free(self) -> None:
         if self.ptr:
