@@ -344,10 +344,6 @@ void *llamd_cuda_paged_new8(int n_head, int n_head_kv, int hd, int page_size, in
         set_error_msg("paged batch: a cache in 8 bits is i8 or e4m3");
         return nullptr;
     }
-    if (n_head_kv > 0 && n_head / n_head_kv > kPagedSmallRows) {
-        set_error_msg("paged batch: up to 32 query heads to a kv head of a cache in 8 bits");
-        return nullptr;
-    }
     return paged_new(n_head, n_head_kv, hd, page_size, type, cache);
 }
 
@@ -372,7 +368,7 @@ int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int
     std::vector<PagedBlock> block;
     bool shared_write = false;
     try {
-        make_plan(plan, v, q_len, kv_len, b->sms, b->cache != 0);
+        make_plan(plan, v, q_len, kv_len, b->sms);
         if (b->cache) {
             blocks_of(block, n_seq, q_len, kv_len);
             shared_write = writes_shared(v.page, n_seq, q_len, kv_len, pages, pages_stride);
@@ -516,7 +512,7 @@ static int attention_of(Batch *b, const void *q, size_t q_stride, const void *k_
     if (b->beside) LLAMD_TRY(cudaEventRecord(g_fork, stream()), "paged attention: fork");
     if (b->n_ctas) {  // (first: its CTAs need whole SMs, and what it refuses leaves nothing launched)
         a.item = b->large;
-        if (!paged_prompt_launch(a, b->type, b->n_pages, b->begin, b->n_ctas)) return -1;
+        if (!paged_prompt_launch(a, b->type, b->cache, b->n_pages, b->begin, b->n_ctas)) return -1;
     }
     if (b->n_small) {
         a.item = b->small;

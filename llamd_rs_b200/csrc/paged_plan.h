@@ -141,7 +141,7 @@ inline bool prefix_apart(const PagedView &v, const int32_t *q_len) {
     return v.n_shared && active > 1 && (long long)v.tokens * v.group < 2LL * kPagedTileRows * active;
 }
 
-inline void make_plan(Plan &plan, const PagedView &v, const int32_t *q_len, const int32_t *kv_len, int sms, bool all_small = false) {
+inline void make_plan(Plan &plan, const PagedView &v, const int32_t *q_len, const int32_t *kv_len, int sms) {
     const int group = v.group, few_tokens = std::max(1, kPagedPieceRows / group);
     std::vector<Stretch> stretch;  // the shared one, where there is one, then the sequences' own
     const bool shared = prefix_apart(v, q_len);
@@ -164,7 +164,7 @@ inline void make_plan(Plan &plan, const PagedView &v, const int32_t *q_len, cons
         if (st.step && st.n_tok * group > kPagedSmallRows) own_work += (long long)st.n_tok * group * (st.end - st.begin) * v.n_head_kv;
     for (Stretch &st : stretch) {
         const long long rows = (long long)st.n_tok * group;
-        st.small = group <= kPagedSmallRows && (all_small || rows <= kPagedSmallRows || (st.step ? rows <= kFewRows && own_work <= kFewOwnWork : rows * (st.end - st.begin) * v.n_head_kv <= kFewSharedWork));
+        st.small = group <= kPagedSmallRows && (rows <= kPagedSmallRows || (st.step ? rows <= kFewRows && own_work <= kFewOwnWork : rows * (st.end - st.begin) * v.n_head_kv <= kFewSharedWork));
     }
     // some tokens of a stretch, and where they leave partial results, by kv head
     struct Tile {

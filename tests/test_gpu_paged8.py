@@ -194,7 +194,7 @@ def run_attention8(paged, cache, H, K, D, page, dtype, q_len, kv_len, n_shared=0
 
 
 @pytest.mark.parametrize("cache", CACHES)
-@pytest.mark.parametrize("H,K,D,page,dtype,q_len,kv_len,n_shared", [c for c in ATTENTION if c[0] // c[1] <= 32])
+@pytest.mark.parametrize("H,K,D,page,dtype,q_len,kv_len,n_shared", ATTENTION)
 def test_attention(paged, cache, H, K, D, page, dtype, q_len, kv_len, n_shared):
     close(*run_attention8(paged, cache, H, K, D, page, dtype, q_len, kv_len, n_shared))
 
@@ -230,6 +230,75 @@ def test_queries_of_any_size(paged, cache, size):
 @pytest.mark.parametrize("D,dtype", [(128, "bf16"), (64, "f16")])
 def test_attention_joins(paged, cache, n, D, dtype):
     close(*run_attention8(paged, cache, 32, 4, D, 16, dtype, [1] * n, [401 + 5 * i for i in range(n)], 400))
+
+
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("H,K,D,page,dtype,q_len,kv_len,n_shared", [c for c in ATTENTION if max(c[5]) > 3 and not c[7]])
+def test_attention_beside_a_long_prompt(paged, cache, H, K, D, page, dtype, q_len, kv_len, n_shared):
+    """Prompts that would be too little work for the tensor cores by themselves, in one batch with another that is not."""
+    long = 300 + 2400 // (H // K)
+    close(*run_attention8(paged, cache, H, K, D, page, dtype, q_len + [long], kv_len + [long], n_shared))
+
+
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("H,D,dtype", [(8, 128, "f16"), (5, 64, "bf16"), (1, 128, "bf16"), (2, 64, "f16")])
+def test_attention_many_pieces(paged, cache, H, D, dtype):
+    """Several pieces to every CTA, of one tile and of two, of one block and of several, tails of every length, and short sequences between them."""
+    rng = np.random.default_rng(H)
+    q_len, kv_len = [], []
+    for _ in range(260):
+        n = int(rng.choice([0, 1, 3, rng.integers(13, 17), rng.integers(17, 60), rng.integers(100, 140)], p=[.05, .1, .1, .3, .35, .1])) * (8 if H == 1 else 1)
+        q_len.append(n)
+        kv_len.append(n + int(rng.choice([0, 0, rng.integers(0, 40), rng.integers(0, 400)])))
+    close(*run_attention8(paged, cache, H, 1, D, 16, dtype, q_len, kv_len, repeat=2))
+    close(*run_attention8(paged, cache, H, 1, D, 32, dtype, q_len, [m + 256 for m in kv_len], 256, repeat=2))
+
+
+@pytest.mark.parametrize("cache", CACHES)
+def test_attention_beside(paged, cache):
+    """A batch large enough that the prefix and the sequences' own positions are read at the same time; three times."""
+    rng = np.random.default_rng(3)
+    own = [int(x) for x in rng.integers(900, 1100, 64)]
+    close(*run_attention8(paged, cache, 32, 4, 128, 64, "bf16", [1] * 64, [7552 + m for m in own], 7552, repeat=3))
+
+
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("prompt", [True, False])
+def test_every_code_and_scale(paged, cache, dtype, D, prompt):
+    """V holds all codes (-128 is none of i8's: with the largest scale it is beyond f16) with all of an append's scales, and each query's weight is 1 at one
+    position and below 2^-700 at all others: out is that value. One prompt for the tensor cores' kernel, as many sequences of one token for the other.
+
+    The weight itself is 2^d, |d| <= 2^-12 (a score of 2560 log2 e has a rounding of half a step of 2^-12), and is rounded by u for the product, not for the
+    sum that the product is divided by: u and 2^-22 of the quotient's own arithmetic. Neighbouring codes are 2^-7 apart at least."""
+    from llamd_rs_b200 import backend
+
+    _, low, high = plain8.FORMATS[cache]
+    n_blocks = high - low + 1
+    n = 16 * n_blocks
+    codes = np.tile(np.arange(256, dtype=np.uint8), n * D // 256 + 1)[:n * D].reshape(n_blocks, 1, 16, D)
+    if cache == "i8":
+        codes[codes == 0x80] = 0x81
+    scales = np.arange(127 + low, 128 + high, dtype=np.uint8).reshape(n_blocks, 1, 1)
+    # position i's key is its number in base 2, 16 and -16 by bit: a token scores 2560 at its own, 2048 at most at those before it
+    kv = np.zeros((n, D))
+    kv[:, :10] = np.where((np.arange(n)[:, None] >> np.arange(10)) & 1, 16.0, -16.0)
+    k_codes = np.searchsorted(plain8.TABLE[cache][:127], np.abs(kv)).astype(np.uint8)
+    k_codes = np.where(kv < 0, (k_codes | 128) if cache == "e4m3" else (-k_codes.view(np.int8)).view(np.uint8), k_codes).astype(np.uint8)
+    assert np.array_equal(plain8.TABLE[cache][k_codes], kv)
+    b = paged.Batch(1, 1, D, 16, dtype, cache=cache)
+    table = list(range(n_blocks))
+    if prompt:
+        b.set([n], [n], [table], n_blocks)
+    else:
+        b.set([1] * n, np.arange(1, n + 1), [table] * n, n_blocks)
+    q, out = dev(plain.to_bits(kv.reshape(n, 1, D), dtype)), dev(np.zeros((n, 1, D), np.uint32))
+    b.attention(q, dev(k_codes.reshape(n_blocks, 1, 16, D)), dev(codes), out, scale=1.0, out_f32=True, k_scales=dev(np.full((n_blocks, 1, 1), 127, np.uint8)), v_scales=dev(scales))
+    backend.sync()
+    got = out.download(np.uint32, n * D).view(np.float32).astype(np.float64).reshape(n, D)
+    want = plain8.values(codes, scales, cache).reshape(n, D)
+    assert np.all(np.abs(got - want) <= (plain.U[dtype if prompt else "f16"] + 2.0 ** -22) * np.abs(want))
 
 
 @pytest.mark.parametrize("cache", CACHES)
