@@ -60,8 +60,11 @@ struct Batch {
     const int32_t *begin = nullptr;                      // large: each CTA's
     const PagedMerge *merge = nullptr;
     const PagedPart *part = nullptr;
-    const PagedBlock *block = nullptr;  // of a cache in 8 bits
-    int n_block = 0;
+    // of a cache in 8 bits: where new tokens meet scale blocks, and the pages that the large pieces read, in 16 bits (K's, then V's)
+    const PagedBlock *block = nullptr;
+    const PagedWide *wide = nullptr;
+    int n_block = 0, n_wide = 0;
+    KeptBlock widened;
     bool shared_write = false;  // two sequences have new tokens in one page
     bool beside = false;
     int n_small = 0, small_rows = 0, n_ctas = 0, n_merge = 0, most = 0;
@@ -71,7 +74,7 @@ struct Batch {
 
     ~Batch() {
         break_graphs();
-        drop(g_device, dev), drop(g_device, partial), drop(g_pinned, host);
+        drop(g_device, dev), drop(g_device, partial), drop(g_device, widened), drop(g_pinned, host);
     }
     void break_graphs() {
         for (const auto &g : graphs) g->broken = true;
@@ -127,12 +130,14 @@ struct Batch {
         host.n = n, host.event = copied;
         return true;
     }
-    // Room for n bytes on both sides and for `rows` partial results; the pinned side is not written before the copy out of it is done.
-    bool reserve(size_t n, size_t rows) {
+    // Bytes of K or of V of a page in 16 bits.
+    size_t wide_bytes() const { return (size_t)view.n_head_kv * view.page * view.hd * 2; }
+    // Room for n bytes on both sides, for `rows` partial results and `pages` in 16 bits; the pinned side is not written before the copy out of it is done.
+    bool reserve(size_t n, size_t rows, size_t pages) {
         give_back();
         if (!grow_pinned(n)) return false;
         if (cudaEventSynchronize((cudaEvent_t)host.event) != cudaSuccess) return fail("paged batch: previous copy");
-        return grow(dev, n) && grow(partial, rows * (view.hd * sizeof(float) + sizeof(float2)));
+        return grow(dev, n) && grow(partial, rows * (view.hd * sizeof(float) + sizeof(float2))) && grow(widened, 2 * pages * wide_bytes());
     }
     bool fail(const char *what) {
         set_error(cudaGetLastError(), what);
@@ -182,6 +187,36 @@ void blocks_of(std::vector<PagedBlock> &block, int n_seq, const int32_t *q_len, 
             block.push_back({t + pos - (kv_len[s] - q_len[s]), n});
             pos += n;
         }
+}
+// The pages that the plan's large pieces read: each once, a shared prefix's for all; and a table of their places in that list beside the batch's own (a
+// second [n_seq][table_stride] behind it), which the pieces are pointed to.
+void wide_pages(std::vector<PagedWide> &wide, std::vector<int32_t> &table, Plan &plan, const PagedView &v, const int32_t *pages, int pages_stride) {
+    if (plan.large.empty()) return;
+    const int stride = v.table_stride, common = v.n_shared / v.page;
+    std::vector<std::pair<int, int>> range(v.n_seq, {0x7fffffff, 0});  // positions that a sequence's pieces read: one stretch, or the prefix and its own behind it
+    for (const PagedItem &it : plan.large) {
+        auto &r = range[it.table / stride];
+        r = {std::min(r.first, it.kv_begin), std::max(r.second, it.kv_end)};
+    }
+    table.assign((size_t)v.n_seq * stride, 0);
+    int prefix = -1;  // where the common pages begin in the list
+    for (int s = 0; s < v.n_seq; s++) {
+        const int end = range[s].second, n = (end + v.page - 1) / v.page;
+        if (!end) continue;
+        int i = range[s].first / v.page;
+        if (i < common) {  // (a stretch that begins in front of its own positions begins with the prefix)
+            if (prefix < 0) {
+                prefix = (int)wide.size();
+                for (int x = 0; x < common; x++) wide.push_back({pages[(size_t)s * pages_stride + x], v.page});
+            }
+            for (; i < std::min(n, common); i++) table[(size_t)s * stride + i] = prefix + i;
+        }
+        for (; i < n; i++) {
+            table[(size_t)s * stride + i] = (int32_t)wide.size();
+            wide.push_back({pages[(size_t)s * pages_stride + i], std::min(v.page, end - i * v.page)});
+        }
+    }
+    for (PagedItem &it : plan.large) it.table += v.n_seq * stride;
 }
 // Do two new tokens' places share a page that two sequences list, or one twice?
 bool writes_shared(int page, int n_seq, const int32_t *q_len, const int32_t *kv_len, const int32_t *pages, int pages_stride) {
@@ -363,31 +398,36 @@ int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int
         if (q_len[s]) max_kv = std::max(max_kv, kv_len[s]);
         v.table_stride = std::max(v.table_stride, (kv_len[s] + v.page - 1) / v.page);
     }
-    if ((long long)n_seq * v.table_stride > 0x7fffffffLL) return refuse("paged batch: the tables have more than 2^31 entries");
+    if ((long long)n_seq * v.table_stride * (b->cache ? 2 : 1) > 0x7fffffffLL) return refuse("paged batch: the tables have more than 2^31 entries");
     Plan plan;
     std::vector<PagedBlock> block;
+    std::vector<PagedWide> wide;
+    std::vector<int32_t> wide_table;
     bool shared_write = false;
     try {
         make_plan(plan, v, q_len, kv_len, b->sms);
         if (b->cache) {
             blocks_of(block, n_seq, q_len, kv_len);
+            wide_pages(wide, wide_table, plan, v, pages, pages_stride);
             shared_write = writes_shared(v.page, n_seq, q_len, kv_len, pages, pages_stride);
         }
     } catch (const std::exception &) {
         return refuse("paged batch: out of host memory");
     }
+    if ((long long)wide.size() * v.n_head_kv * v.page * v.hd > 1LL << 34) return refuse("paged batch: more than 2^34 values in 16 bits");
     if (plan.rows > 0x7fffffff || plan.merge.size() * v.group > 0x7fffffff) return refuse("paged batch: too many partial results");
     size_t bytes = 0;
-    const size_t o_token = section<PagedToken>(bytes, v.tokens), o_table = section<int32_t>(bytes, (size_t)n_seq * v.table_stride), o_small = section<PagedItem>(bytes, plan.small.size()),
+    const size_t o_token = section<PagedToken>(bytes, v.tokens), o_table = section<int32_t>(bytes, (size_t)n_seq * v.table_stride + wide_table.size()), o_small = section<PagedItem>(bytes, plan.small.size()),
                  o_large = section<PagedItem>(bytes, plan.large.size()), o_begin = section<int32_t>(bytes, plan.begin.size()),
-                 o_merge = section<PagedMerge>(bytes, plan.merge.size()), o_part = section<PagedPart>(bytes, plan.part.size()), o_block = section<PagedBlock>(bytes, block.size());
+                 o_merge = section<PagedMerge>(bytes, plan.merge.size()), o_part = section<PagedPart>(bytes, plan.part.size()), o_block = section<PagedBlock>(bytes, block.size()),
+                 o_wide = section<PagedWide>(bytes, wide.size());
     if (plan.beside && !side_ready()) {
         set_error(cudaGetLastError(), "paged batch: side stream");
         return -1;
     }
     b->ready = false;  // (from here on what the batch held is being replaced)
     b->break_graphs();
-    if (!b->reserve(std::max<size_t>(bytes, 16), plan.rows)) return -1;
+    if (!b->reserve(std::max<size_t>(bytes, 16), plan.rows, wide.size())) return -1;
     auto put = [&](size_t at, const void *from, size_t n) {
         if (n) memcpy(b->host.p + at, from, n);
     };
@@ -397,6 +437,8 @@ int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int
     put(o_merge, plan.merge.data(), plan.merge.size() * sizeof(PagedMerge));
     put(o_part, plan.part.data(), plan.part.size() * sizeof(PagedPart));
     put(o_block, block.data(), block.size() * sizeof(PagedBlock));
+    put(o_wide, wide.data(), wide.size() * sizeof(PagedWide));
+    put(o_table + (size_t)n_seq * v.table_stride * sizeof(int32_t), wide_table.data(), wide_table.size() * sizeof(int32_t));
     PagedToken *token = (PagedToken *)(b->host.p + o_token);
     int32_t *table = (int32_t *)(b->host.p + o_table);
     for (int s = 0, t = 0; s < n_seq; s++) {
@@ -412,7 +454,8 @@ int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int
     b->merge = (const PagedMerge *)(b->dev.p + o_merge);
     b->part = (const PagedPart *)(b->dev.p + o_part);
     b->block = (const PagedBlock *)(b->dev.p + o_block);
-    b->n_block = (int)block.size(), b->shared_write = shared_write;
+    b->wide = (const PagedWide *)(b->dev.p + o_wide);
+    b->n_block = (int)block.size(), b->n_wide = (int)wide.size(), b->shared_write = shared_write;
     b->beside = plan.beside;
     b->n_small = (int)plan.small.size(), b->small_rows = plan.small_rows, b->n_ctas = (int)plan.begin.size() - 1, b->n_merge = (int)plan.merge.size(), b->most = plan.most;
     b->partial_rows = plan.rows;
@@ -511,8 +554,15 @@ static int attention_of(Batch *b, const void *q, size_t q_stride, const void *k_
     a.part_o = (float *)b->partial.p, a.part_ml = (float2 *)(b->partial.p + b->partial_rows * g.hd * sizeof(float));
     if (b->beside) LLAMD_TRY(cudaEventRecord(g_fork, stream()), "paged attention: fork");
     if (b->n_ctas) {  // (first: its CTAs need whole SMs, and what it refuses leaves nothing launched)
-        a.item = b->large;
-        if (!paged_prompt_launch(a, b->type, b->cache, b->n_pages, b->begin, b->n_ctas)) return -1;
+        PagedAttn l = a;
+        l.item = b->large;
+        PagedWiden w = {};
+        if (b->cache) {
+            uint8_t *const k = b->widened.p, *const v = k + (size_t)b->n_wide * b->wide_bytes();
+            w = {b->wide, b->n_wide, g.page, g.n_head_kv * g.page, g.hd / 16, k_pages, v_pages, k_scales, v_scales, k, v, b->cache, b->sms};
+            l.k_pages = k, l.v_pages = v;
+        }
+        if (!paged_prompt_launch(l, b->type, b->cache ? b->n_wide : b->n_pages, b->begin, b->n_ctas, b->cache ? &w : nullptr)) return -1;
     }
     if (b->n_small) {
         a.item = b->small;

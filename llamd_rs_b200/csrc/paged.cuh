@@ -30,7 +30,18 @@ void paged_decode_launch(const PagedAttn &p, int type, int n_items, int max_rows
 void paged_decode8_launch(const PagedAttn &p, int type, int cache, int n_items, int max_rows, cudaStream_t to);
 bool paged_gave_up();       // a wait of an earlier attention has run out, and the host has not read it yet
 bool paged_prompt_ready();  // what its launches need beside the batch: false and an error where it cannot be had
-bool paged_prompt_launch(const PagedAttn &p, int type, int cache, int n_pages, const int32_t *begin, int n_ctas);  // begin: each CTA's pieces (n_ctas + 1); false and an error: not launched
+// The pages of a cache in 8 bits that paged_prompt.cu reads, and where their 16-bit values go: page i of the list is page i of k_out and v_out.
+struct PagedWiden {
+    const PagedWide *page;
+    int n_pages, page_size, rows, chunks;  // rows (heads x positions) of a page, 16-byte pieces of a row of codes
+    const void *k_pages, *v_pages;
+    const uint8_t *k_scales, *v_scales;
+    void *k_out, *v_out;
+    int cache, sms;
+};
+void paged_widen_launch(const PagedWiden &w, int type);
+// widen: launched in front where it is not null
+bool paged_prompt_launch(const PagedAttn &p, int type, int n_pages, const int32_t *begin, int n_ctas, const PagedWiden *widen);  // begin: each CTA's pieces (n_ctas + 1); false and an error: not launched
 void paged_merge_launch(const PagedAttn &p, int type, const PagedMerge *merge, const PagedPart *parts, int n_merge, int most, int sms);  // most: parts of any of them
 
 // 16-bit types of a cache and what the kernels need of them.

@@ -14,6 +14,11 @@ struct PagedBlock {
     int32_t token, n;
 };
 
+// A page of a cache in 8 bits whose first `valid` positions are wanted in 16 (paged_widen.cu).
+struct PagedWide {
+    int32_t page, valid;
+};
+
 // The batch as the kernels see it: device memory that the batch owns, every index checked against the pools when it was made.
 struct PagedView {
     int n_head, n_head_kv, group, hd, page, n_seq, tokens, n_shared, table_stride;

@@ -11,7 +11,7 @@
 //   warps 0-3, 4-7   softmax of tile 0 / 1, a thread per row: S from TMEM, mask, maximum, exponentials, P to TMEM; at the end O / sum
 //   warp 8           Q, and K and V blocks into a ring in shared memory (TMA, a box per page, 128-byte swizzle)
 //   warp 9           the products, one thread: S0, S1 of the first block, then per block PV0, S0', PV1, S1'
-//   warps 10, 11     nothing: registers are handed over by whole warpgroups; of a cache in 8 bits, the blocks' codes to 16-bit values
+//   warps 10, 11     nothing: registers are handed over by whole warpgroups
 // A CTA stays on its SM and works off a list of pieces; the next piece's Q and blocks are on their way while the last one ends.
 //
 // O stays in TMEM over all blocks. It is rescaled only when a row's maximum has grown by more than 2^8 since the last time (P is then at
@@ -23,16 +23,13 @@
 // special function units 47 %, tensor pipe 42 %, issue slots 35 % busy. A piece costs 3 us to
 // begin and end: one prompt of 512 positions takes 12.7 us for 1.4 us of products.
 // Slots of the last block behind the last position are masked in S and set to zero in V's tile before the product reads it.
-// A cache in 8 bits (paged8.cuh) comes as codes, into the part of a ring slot that its 16-bit block fills last; warps 10 and 11 write the block, every value
-// exact, with zeros behind the last position, and the products read it as any other. At 128 elements the codes lie where the block's second half goes, the first is
-// written first, and then each row over its own codes. Half the bytes come from HBM and nothing else changes: no other copy of the cache, no other softmax.
 // Every wait is bounded; one that runs out raises a flag that the host reads (llamd_fwd_paged_status), and outputs that are not complete are NaN.
 #include <cuda.h>
 
 #include <type_traits>
 
 #include "packed_f32.cuh"
-#include "paged8.cuh"
+#include "paged.cuh"
 
 namespace llamd {
 namespace {
@@ -44,20 +41,16 @@ constexpr int kSoftmaxWarps = 8, kThreads = (kSoftmaxWarps + 4) * 32;
 constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
 static_assert(kSoftmaxWarps * 32 * kSoftmaxRegs + 128 * kOtherRegs <= kThreads * 168, "no more than the launch's own");
 
-// C: kPagedI8 or kPagedE4m3, or 0 for a cache of 16 bits.
-template <int HD, int C> struct Shape {
+template <int HD> struct Shape {
     static constexpr int kTileBytes = kM * HD * 2;               // a tile of Q, a block of K or V: HD / 64 halves of 128 rows x 128 bytes
     static constexpr int kQueries = HD == 128 ? 3 : 4;           // tiles of Q: the two at work and the next
-    static constexpr int kStages = HD == 128 ? 4 : C ? 6 : 8;    // blocks of K or V in flight
-    static constexpr int kRawAt = 16384;                         // of a slot: its codes, 128 rows of HD bytes
-    static constexpr int kSlotBytes = C && HD == 64 ? kRawAt + kN * HD : kTileBytes;
+    static constexpr int kStages = HD == 128 ? 4 : 8;            // blocks of K or V in flight
     struct Rest {  // what follows the tiles in shared memory
-        uint64_t q_full[kQueries], q_empty[kQueries], s[2], p[2][2], o_full[2], o_empty[2], full[kStages], empty[kStages], raw[C ? kStages : 1], drain;
+        uint64_t q_full[kQueries], q_empty[kQueries], s[2], p[2][2], o_full[2], o_empty[2], full[kStages], empty[kStages], drain;
         uint32_t tmem;
         volatile int abort;
     };
-    static constexpr size_t kRing = kQueries * (size_t)kTileBytes, kRestAt = kRing + kStages * (size_t)kSlotBytes, kSmem = kRestAt + sizeof(Rest);
-    static_assert(kSmem <= 227 * 1024, "one CTA to an SM");
+    static constexpr size_t kSmem = (kQueries + kStages) * (size_t)kTileBytes + sizeof(Rest);
 };
 constexpr int kHalfBytes = kM * 128;
 constexpr unsigned long long kDrainLimit = 2000000000ull;  // of what a block that has given up waits for, in nanoseconds
@@ -204,82 +197,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&v)[16]
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// 16 codes as 16-bit values, exactly: f16 or bf16 pairs times `by`, which holds the scale and what the pairs are short of.
-template <int C, typename T> struct Widen;
-template <int C> struct Widen<C, __half> {
-    static __device__ __forceinline__ uint32_t factor(int byte) { return __half_as_ushort(__float2half_rn(scale_of(byte) * (float)(1 << Cache8<C>::kShift))) * 0x10001u; }
-    template <int HALF> static __device__ __forceinline__ uint32_t pair(uint32_t x, uint32_t by) {
-        const uint32_t y = Cache8<C>::template f16x2<HALF>(x);
-        const __half2 h = __hmul2(*reinterpret_cast<const __half2 *>(&y), *reinterpret_cast<const __half2 *>(&by));
-        return *reinterpret_cast<const uint32_t *>(&h);
-    }
-};
-__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
-    const __nv_bfloat162 h = __hmul2(*reinterpret_cast<const __nv_bfloat162 *>(&a), *reinterpret_cast<const __nv_bfloat162 *>(&b));
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-template <> struct Widen<kPagedI8, __nv_bfloat16> {
-    static __device__ __forceinline__ uint32_t factor(int byte) { return (uint32_t)byte << 7 | (uint32_t)byte << 23; }
-    // 128 + the code's low 7 bits, less 128, or 256 where its sign bit is set
-    template <int HALF> static __device__ __forceinline__ uint32_t pair(uint32_t x, uint32_t by) {
-        const uint32_t t = __byte_perm(x, 0x43434343u, HALF ? 0x4342 : 0x4140), a = t & 0xFF7FFF7Fu, b = t & 0xFF80FF80u;
-        const __nv_bfloat162 h = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&a), *reinterpret_cast<const __nv_bfloat162 *>(&b));
-        return mul_bf16x2(*reinterpret_cast<const uint32_t *>(&h), by);
-    }
-};
-template <> struct Widen<kPagedE4m3, __nv_bfloat16> {
-    static __device__ __forceinline__ uint32_t factor(int byte) { return (uint32_t)min(byte + 120, 255) * 0x800080u; }
-    // the code's bits as a bf16's sign, low exponent bits and high mantissa bits: 2^-120 of its value
-    template <int HALF> static __device__ __forceinline__ uint32_t pair(uint32_t x, uint32_t by) {
-        const uint32_t t = __byte_perm(x, 0, HALF ? 0x3424 : 0x1404);
-        return mul_bf16x2((t & 0x80008000u) | ((t >> 4) & 0x07F007F0u), by);
-    }
-};
-__device__ __forceinline__ uint4 shared_load(uint32_t addr) {
-    uint4 v;
-    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
-    return v;
-}
-__device__ __forceinline__ void shared_store(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
-}
-
-// Half the rows of a block, by a warp: codes of the slot at `slot` (rows of HD bytes at kRawAt; of 128 bytes with the 128-byte swizzle) to values in the products' layout.
-// `bytes`: lane i's is the scale of the block's 16 positions from 16 i on, for i < 8. Rows from `valid` on become zeros. A lane takes 16 codes: at 128 elements lanes of 8 that
-// go to shared memory together have rows 4 apart, whose swizzles differ in the high bit, and those of one write their two halves in the other order: no
-// bank is met twice. Four steps at a time, so that loads are under way beside one another.
-template <int C, typename T, int HD>
-__device__ __forceinline__ void widen_rows(uint32_t slot, int first_row, int bytes, int valid) {
-    using W = Widen<C, T>;
-    const int lane = threadIdx.x & 31, c = lane & 3, in = HD == 128 ? ((lane >> 2) & 1) * 4 + (lane >> 3) : lane >> 2;
-    const bool swap = HD == 128 && (lane & 4);
-#pragma unroll
-    for (int h = 0; h < HD / 64; h++) {
-#pragma unroll
-        for (int i = 0; i < 8; i += 4) {
-            uint4 x[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int r = first_row + (i + j) * 8 + in;
-                x[j] = shared_load(slot + 16384 + r * HD + (HD == 128 ? ((h * 4 + c) ^ (r & 7)) << 4 : c << 4));
-            }
-            if (h) __syncwarp();  // (a row's codes are read before they are written over)
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int r = first_row + (i + j) * 8 + in;
-                const uint32_t by = W::factor(__shfl_sync(0xffffffffu, bytes, (first_row + (i + j) * 8) >> 4));
-                uint32_t w[8] = {W::template pair<0>(x[j].x, by), W::template pair<1>(x[j].x, by), W::template pair<0>(x[j].y, by), W::template pair<1>(x[j].y, by),
-                                 W::template pair<0>(x[j].z, by), W::template pair<1>(x[j].z, by), W::template pair<0>(x[j].w, by), W::template pair<1>(x[j].w, by)};
-#pragma unroll
-                for (int e = 0; e < 8; e++) w[e] = r < valid ? w[e] : 0u;
-                const uint32_t to = slot + h * kHalfBytes + r * 128, a0 = to + ((2 * c ^ (r & 7)) << 4), a1 = to + (((2 * c + 1) ^ (r & 7)) << 4);
-                shared_store(swap ? a1 : a0, swap ? w[4] : w[0], swap ? w[5] : w[1], swap ? w[6] : w[2], swap ? w[7] : w[3]);
-                shared_store(swap ? a0 : a1, swap ? w[0] : w[4], swap ? w[1] : w[5], swap ? w[2] : w[6], swap ? w[3] : w[7]);
-            }
-        }
-    }
-}
-
 // 32 bytes at once (a whole sector of a row that the thread has to itself)
 __device__ __forceinline__ void store8(void *p, const uint32_t *w) {
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
@@ -296,17 +213,17 @@ __device__ __forceinline__ float exp2_fast(float x) {  // (2 ulp; -inf gives 0)
     return y;
 }
 
-template <typename T, int HD, int C>
+template <typename T, int HD>
 __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_constant__ PromptParams p) {
-    using S = Shape<HD, C>;
+    using S = Shape<HD>;
     constexpr uint32_t kBf16 = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
     constexpr float kUp = std::is_same<T, __half>::value ? 7.0f : 0.0f, kDown = std::is_same<T, __half>::value ? 1.0f / 128 : 1.0f;
     constexpr int kLoadWarp = kSoftmaxWarps, kMmaWarp = kSoftmaxWarps + 1;
     extern __shared__ __align__(1024) uint8_t smem[];
-    typename S::Rest &sh = *reinterpret_cast<typename S::Rest *>(smem + S::kRestAt);
+    typename S::Rest &sh = *reinterpret_cast<typename S::Rest *>(smem + (S::kQueries + S::kStages) * S::kTileBytes);
     pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = p.a.b.group, per_tile = kM / group;
-    const uint32_t sq = smem_addr(smem), skv = sq + (uint32_t)S::kRing;
+    const uint32_t sq = smem_addr(smem), skv = sq + S::kQueries * S::kTileBytes;
     const int first = p.begin[blockIdx.x], last = p.begin[blockIdx.x + 1];
 
     if (threadIdx.x == 0) {
@@ -325,9 +242,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
         }
 #pragma unroll
         for (int i = 0; i < S::kStages; i++) {
-            bar_init(&sh.full[i], C ? 2 : 1);
+            bar_init(&sh.full[i], 1);
             bar_init(&sh.empty[i], 1);
-            if constexpr (C != 0) bar_init(&sh.raw[i], 1);
         }
         bar_init(&sh.drain, 1);
         sh.abort = p.limit == 0;
@@ -349,8 +265,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
         if (warp == kLoadWarp) {
             // ---- K and V blocks, K of a piece's block j in the ring's slot base + 2 j, V behind it; Q behind the piece's first K ----
             const int page = p.a.b.page, box = min(page, kN), shift = __ffs(page) - 1, boxes = kN / box;
-            constexpr int kHalves = HD / 64, kCopies = C ? 1 : kHalves;  // copies to a box of K or V
-            const int my_box = lane / kCopies, my_half = lane % kCopies;
+            constexpr int kHalves = HD / 64;
+            const int my_box = lane / kHalves, my_half = lane % kHalves;
             bool ok = !sh.abort;
             for (int n = first; n < last && ok; n++) {
                 const PagedItem it = p.a.item[n];
@@ -371,12 +287,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                         if (round) ok = ok && bar_wait(&sh.empty[stage], (round - 1) & 1, &sh.abort, p.limit);
                         ok = __all_sync(0xffffffffu, ok);
                         if (!ok) break;
-                        uint64_t *const landed = C ? &sh.raw[C ? stage : 0] : &sh.full[stage];
-                        if (lane == 0) bar_expect(landed, (uint32_t)(used * box * HD * (C ? 1 : 2)));
+                        if (lane == 0) bar_expect(&sh.full[stage], (uint32_t)(used * box * HD * 2));
                         __syncwarp();
                         if (my_box < used)
-                            tma_rows(skv + stage * S::kSlotBytes + (C ? S::kRawAt + my_box * box * HD : my_half * kHalfBytes + my_box * box * 128), kv ? &p.v : &p.k,
-                                     my_half * 64, row, landed);
+                            tma_rows(skv + stage * S::kTileBytes + my_half * kHalfBytes + my_box * box * 128, kv ? &p.v : &p.k, my_half * 64, row, &sh.full[stage]);
                         slot++;
                         if (kv || j) continue;
 #pragma unroll
@@ -394,39 +308,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                         }
                     }
                     id = next;
-                }
-            }
-        } else if (C != 0 && warp > kMmaWarp) {
-            // ---- codes to values: half of a block's rows each ----
-            const int shift = __ffs(p.a.b.page) - 1, half = warp - kMmaWarp - 1;
-            int at = 0;  // blocks of K and V so far
-            bool ok = !sh.abort;
-            for (int n = first; n < last && ok; n++) {
-                const PagedItem it = p.a.item[n];
-                const Tiles tl(it, per_tile);
-                const int32_t *table = p.a.b.table + it.table;
-                auto scale_at = [&](int j) {  // lanes 0-7 K's scales of block j, 8-15 V's
-                    const int pos = it.kv_begin + j * kN + (lane & 7) * kScaleBlock;
-                    if (lane >= 16 || pos >= it.kv_end) return 0;
-                    const size_t to = (((size_t)table[pos >> shift] * p.a.b.n_head_kv + it.head) << (shift - 4)) + ((pos & (p.a.b.page - 1)) >> 4);
-                    return (int)(lane < 8 ? p.a.k_scales : p.a.v_scales)[to];
-                };
-                int next = scale_at(0);
-                for (int j = 0; j < tl.n_all && ok; j++) {
-                    const int now = next;
-                    next = scale_at(j + 1);
-#pragma unroll
-                    for (int kv = 0; kv < 2; kv++, at++) {
-                        const int stage = at % S::kStages;
-                        ok = ok && bar_wait(&sh.raw[C ? stage : 0], (at / S::kStages) & 1, &sh.abort, p.limit);
-                        ok = __all_sync(0xffffffffu, ok);
-                        if (!ok) break;
-                        const int bytes = kv ? __shfl_down_sync(0xffffffffu, now, 8) : now;
-                        if constexpr (C != 0) widen_rows<C, T, HD>(skv + stage * S::kSlotBytes, half * (kN / 2), bytes, it.kv_end - it.kv_begin - j * kN);
-                        fence_async();
-                        __syncwarp();
-                        if (lane == 0) bar_arrive(&sh.full[stage]);
-                    }
                 }
             }
         } else if (warp == kMmaWarp && elect_one()) {
@@ -452,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
             const uint32_t q_desc = desc_low(sq, 16), k_desc = desc_low(skv, 16), v_desc = desc_low(skv, kHalfBytes);
             int buf[2] = {0, 0};  // the tiles' Q
             auto scores = [&](int t, int stage) {
-                const uint32_t a = q_desc + buf[t] * (S::kTileBytes >> 4), b = k_desc + stage * (S::kSlotBytes >> 4);
+                const uint32_t a = q_desc + buf[t] * (S::kTileBytes >> 4), b = k_desc + stage * (S::kTileBytes >> 4);
 #pragma unroll
                 for (int s = 0; s < HD / 16; s++) {
                     const uint32_t at = (s / 4) * (kHalfBytes >> 4) + (s % 4) * 2;
@@ -461,7 +342,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                 mma_commit(&sh.s[t]);
             };
             auto values = [&](int t, int stage, int part, bool more) {  // over the block's first 96 positions, then its last 32: as the weights come
-                const uint32_t b = v_desc + stage * (S::kSlotBytes >> 4);
+                const uint32_t b = v_desc + stage * (S::kTileBytes >> 4);
 #pragma unroll
                 for (int step = part ? 6 : 0; step < (part ? 8 : 6); step++)  // 16 positions: 8 columns of P, 16 rows of V
                     mma_ts(tmem + 2 * kN + t * HD, tmem + t * kN + step * 8, b + step * (16 * 128 >> 4), kO, more || step > 0);
@@ -625,7 +506,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
                     for (int q = 0; q < 3; q++) weights(q);
                 }
                 const int valid = it.kv_end - it.kv_begin - j * kN;
-                if (C == 0 && __builtin_expect(valid < kN, 0)) {  // the last block: zeros in V's rows behind the last position (both tiles write the same zeros)
+                if (__builtin_expect(valid < kN, 0)) {  // the last block: zeros in V's rows behind the last position (both tiles write the same zeros)
                     const int slot = base + 2 * j + 1, stage = slot % S::kStages;
                     ok = ok && bar_wait(&sh.full[stage], (slot / S::kStages) & 1, &sh.abort, p.limit);
                     for (int x = valid * (HD / 8) + r; x < kN * (HD / 8); x += 128) {
@@ -711,7 +592,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prompt_kernel(const __grid_
     __syncthreads();
     if (warp == kLoadWarp && sh.abort) {  // given up, by whichever warp: what is on its way still lands before the block ends
         volatile int none = 0;
-        for (int i = max(0, slot - S::kStages); i < slot; i++) bar_wait(C ? &sh.raw[C ? i % S::kStages : 0] : &sh.full[i % S::kStages], (i / S::kStages) & 1, &none, kDrainLimit);
+        for (int i = max(0, slot - S::kStages); i < slot; i++) bar_wait(&sh.full[i % S::kStages], (i / S::kStages) & 1, &none, kDrainLimit);
         for (int i = max(0, n_q - S::kQueries); i < n_q; i++) bar_wait(&sh.q_full[i % S::kQueries], (i / S::kQueries) & 1, &none, kDrainLimit);
     }
     if (warp == kMmaWarp) {
@@ -737,15 +618,8 @@ EncodeTiled encode_tiled() {
     return fn;
 }
 // A pool as rows of HD elements; boxes of 64 elements (128 bytes) and a page's rows, 128 at most.
-bool pool_map(CUtensorMap *map, const void *pool, int type, int cache, const PagedView &v, int n_pages) {
+bool pool_map(CUtensorMap *map, const void *pool, int type, const PagedView &v, int n_pages) {
     const EncodeTiled encode = encode_tiled();
-    if (cache) {  // codes: whole rows
-        const cuuint64_t dims[2] = {(cuuint64_t)v.hd, (cuuint64_t)n_pages * v.n_head_kv * v.page}, strides[1] = {(cuuint64_t)v.hd};
-        const cuuint32_t box[2] = {(cuuint32_t)v.hd, (cuuint32_t)(v.page < kN ? v.page : kN)}, step[2] = {1, 1};
-        return encode && encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(pool), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                v.hd == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-    }
     const cuuint64_t dims[2] = {(cuuint64_t)v.hd, (cuuint64_t)n_pages * v.n_head_kv * v.page}, strides[1] = {(cuuint64_t)v.hd * 2};
     const cuuint32_t box[2] = {64, (cuuint32_t)(v.page < kN ? v.page : kN)}, step[2] = {1, 1};
     return encode && encode(map, type == kPagedF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(pool), dims, strides,
@@ -764,26 +638,15 @@ bool query_map(CUtensorMap *map, const PagedAttn &a, int type) {
                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int HD, int C>
+template <typename T, int HD>
 void prompt_launch(const PromptParams &p, int n_ctas) {
     static bool ready = false;
     if (!ready) {
-        const cudaError_t e = cudaFuncSetAttribute(paged_prompt_kernel<T, HD, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<HD, C>::kSmem);
+        const cudaError_t e = cudaFuncSetAttribute(paged_prompt_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<HD>::kSmem);
         if (e != cudaSuccess) return set_error(e, "paged_prompt shared memory");
         ready = true;
     }
-    launch_kc(PDL_PAGED, "paged_prompt", paged_prompt_kernel<T, HD, C>, dim3(n_ctas), dim3(kThreads), Shape<HD, C>::kSmem, p);
-}
-template <typename T, int C>
-void prompt_launch(const PromptParams &p, int n_ctas) {
-    if (p.a.b.hd == 128) prompt_launch<T, 128, C>(p, n_ctas);
-    else prompt_launch<T, 64, C>(p, n_ctas);
-}
-template <typename T>
-void prompt_launch(const PromptParams &p, int cache, int n_ctas) {
-    if (cache == kPagedI8) prompt_launch<T, kPagedI8>(p, n_ctas);
-    else if (cache == kPagedE4m3) prompt_launch<T, kPagedE4m3>(p, n_ctas);
-    else prompt_launch<T, 0>(p, n_ctas);
+    launch_kc(PDL_PAGED, "paged_prompt", paged_prompt_kernel<T, HD>, dim3(n_ctas), dim3(kThreads), Shape<HD>::kSmem, p);
 }
 
 }  // namespace
@@ -807,19 +670,20 @@ bool paged_prompt_ready() {
     return true;
 }
 
-bool paged_prompt_launch(const PagedAttn &a, int type, int cache, int n_pages, const int32_t *begin, int n_ctas) {
+bool paged_prompt_launch(const PagedAttn &a, int type, int n_pages, const int32_t *begin, int n_ctas, const PagedWiden *widen) {
     PromptParams p;
     p.a = a;
     p.begin = begin;
     p.wide = ((uintptr_t)a.out & 31) == 0 && a.out_stride * (a.out_f32 ? 4 : 2) % 32 == 0;
     p.limit = g_limit;
     p.status = const_cast<int *>(g_status);
-    if (!query_map(&p.q, a, type) || !pool_map(&p.k, a.k_pages, type, cache, a.b, n_pages) || !pool_map(&p.v, a.v_pages, type, cache, a.b, n_pages)) {
+    if (!query_map(&p.q, a, type) || !pool_map(&p.k, a.k_pages, type, a.b, n_pages) || !pool_map(&p.v, a.v_pages, type, a.b, n_pages)) {
         set_error_msg("paged_prompt: a tensor map was refused");
         return false;
     }
-    if (type == kPagedF16) prompt_launch<__half>(p, cache, n_ctas);
-    else prompt_launch<__nv_bfloat16>(p, cache, n_ctas);
+    if (widen) paged_widen_launch(*widen, type);
+    if (type == kPagedF16) a.b.hd == 128 ? prompt_launch<__half, 128>(p, n_ctas) : prompt_launch<__half, 64>(p, n_ctas);
+    else a.b.hd == 128 ? prompt_launch<__nv_bfloat16, 128>(p, n_ctas) : prompt_launch<__nv_bfloat16, 64>(p, n_ctas);
     return !error_code();
 }
 

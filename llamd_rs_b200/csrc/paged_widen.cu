@@ -1,0 +1,104 @@
+// The pages of a cache in 8 bits that the tensor-core kernel is to read, as 16-bit values: K and V of the stretches that it takes, each page once, into the batch's own
+// memory and in the pools' layout, under page ids of their own.
+//
+//   value = code 2^e, exact in f16 and bf16
+//
+// Bytes bound it: 1 read and 2 written per value, and 2 read by the kernel that follows, of which L2 holds the latest. It is that or making the values
+// beside the products, of every block again for each 256 query rows: by two warps inside the tensor-core kernel, through shared memory, a block of 128 positions took
+// 5.3 us where its products take 2.0 (one prompt of 8192 positions 1320 us; one of 512 26.6).
+#include <algorithm>
+
+#include "paged8.cuh"
+
+namespace llamd {
+namespace {
+
+// 16 codes as 16-bit values, exactly: f16 or bf16 pairs times `by`, which holds the scale and what the pairs are short of.
+template <int C, typename T> struct Widen;
+template <int C> struct Widen<C, __half> {
+    static __device__ __forceinline__ uint32_t factor(int byte) { return __half_as_ushort(__float2half_rn(scale_of(byte) * (float)(1 << Cache8<C>::kShift))) * 0x10001u; }
+    template <int HALF> static __device__ __forceinline__ uint32_t pair(uint32_t x, uint32_t by) {
+        const uint32_t y = Cache8<C>::template f16x2<HALF>(x);
+        const __half2 h = __hmul2(*reinterpret_cast<const __half2 *>(&y), *reinterpret_cast<const __half2 *>(&by));
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+};
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 h = __hmul2(*reinterpret_cast<const __nv_bfloat162 *>(&a), *reinterpret_cast<const __nv_bfloat162 *>(&b));
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <> struct Widen<kPagedI8, __nv_bfloat16> {
+    static __device__ __forceinline__ uint32_t factor(int byte) { return (uint32_t)byte << 7 | (uint32_t)byte << 23; }
+    // 128 + the code's low 7 bits, less 128, or 256 where its sign bit is set
+    template <int HALF> static __device__ __forceinline__ uint32_t pair(uint32_t x, uint32_t by) {
+        const uint32_t t = __byte_perm(x, 0x43434343u, HALF ? 0x4342 : 0x4140), a = t & 0xFF7FFF7Fu, b = t & 0xFF80FF80u;
+        const __nv_bfloat162 h = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&a), *reinterpret_cast<const __nv_bfloat162 *>(&b));
+        return mul_bf16x2(*reinterpret_cast<const uint32_t *>(&h), by);
+    }
+};
+template <> struct Widen<kPagedE4m3, __nv_bfloat16> {
+    static __device__ __forceinline__ uint32_t factor(int byte) { return (uint32_t)min(byte + 120, 255) * 0x800080u; }
+    // the code's bits as a bf16's sign, low exponent bits and high mantissa bits: 2^-120 of its value
+    template <int HALF> static __device__ __forceinline__ uint32_t pair(uint32_t x, uint32_t by) {
+        const uint32_t t = __byte_perm(x, 0, HALF ? 0x3424 : 0x1404);
+        return mul_bf16x2((t & 0x80008000u) | ((t >> 4) & 0x07F007F0u), by);
+    }
+};
+
+constexpr int kUnits = 4;  // of 16 codes that a thread has on their way
+
+// blockIdx.y: K or V. Units of 16 codes, page by page; `per_page` of them to a page.
+template <int C, typename T, int CHUNKS>
+__global__ void __launch_bounds__(256) paged_widen_kernel(const PagedWiden w, int units, int per_page) {
+    using W = Widen<C, T>;
+    pdl_trigger();
+    const uint8_t *const codes = reinterpret_cast<const uint8_t *>(blockIdx.y ? w.v_pages : w.k_pages), *const scales = blockIdx.y ? w.v_scales : w.k_scales;
+    uint4 *const out = reinterpret_cast<uint4 *>(blockIdx.y ? w.v_out : w.k_out);
+    const int step = (int)(gridDim.x * blockDim.x);
+    pdl_wait();
+    for (int first = (int)(blockIdx.x * blockDim.x + threadIdx.x); first < units; first += kUnits * step) {
+        // (each kind of load for all of them at once: three that wait for one another, not twelve)
+        uint4 x[kUnits];
+        PagedWide p[kUnits];
+        int in[kUnits], byte[kUnits];
+#pragma unroll
+        for (int i = 0; i < kUnits; i++) {
+            const int u = min(first + i * step, units - 1), page = u / per_page;
+            in[i] = u - page * per_page;
+            p[i] = w.page[page];
+        }
+#pragma unroll
+        for (int i = 0; i < kUnits; i++) {
+            const int row = in[i] / CHUNKS;  // of the page's heads and positions
+            const bool live = first + i * step < units && (row & (w.page_size - 1)) < p[i].valid;  // (whatever lies behind the last position stays)
+            const size_t at = live ? (size_t)p[i].page * per_page + in[i] : 0;
+            x[i] = __ldcs(reinterpret_cast<const uint4 *>(codes) + at);
+            const int scale = scales[at / (kScaleBlock * CHUNKS)];
+            byte[i] = live ? scale : -1;
+        }
+#pragma unroll
+        for (int i = 0; i < kUnits; i++) {
+            if (byte[i] < 0) continue;
+            const size_t to = 2 * (size_t)(first + i * step);
+            const uint32_t by = W::factor(byte[i]);
+            out[to] = make_uint4(W::template pair<0>(x[i].x, by), W::template pair<1>(x[i].x, by), W::template pair<0>(x[i].y, by), W::template pair<1>(x[i].y, by));
+            out[to + 1] = make_uint4(W::template pair<0>(x[i].z, by), W::template pair<1>(x[i].z, by), W::template pair<0>(x[i].w, by), W::template pair<1>(x[i].w, by));
+        }
+    }
+}
+
+template <int C, typename T>
+void launch(const PagedWiden &w) {
+    const int per_page = w.rows * w.chunks, units = w.n_pages * per_page;
+    const dim3 grid((unsigned)std::min((units + 256 * kUnits - 1) / (256 * kUnits), 4 * w.sms), 2);
+    launch_kc(PDL_PAGED, "paged_widen", w.chunks == 8 ? paged_widen_kernel<C, T, 8> : paged_widen_kernel<C, T, 4>, grid, dim3(256), 0, w, units, per_page);
+}
+
+}  // namespace
+
+void paged_widen_launch(const PagedWiden &w, int type) {
+    if (w.cache == kPagedI8) type == kPagedF16 ? launch<kPagedI8, __half>(w) : launch<kPagedI8, __nv_bfloat16>(w);
+    else type == kPagedF16 ? launch<kPagedE4m3, __half>(w) : launch<kPagedE4m3, __nv_bfloat16>(w);
+}
+
+}  // namespace llamd
