@@ -446,7 +446,7 @@ void llamd_fwd_attention_prefill(const float *q, const float *kc, const float *v
 void *llamd_cuda_paged_new(int n_head, int n_head_kv, int hd, int page_size, int type);
 /* ---- the same over caches in 8 bits: half the bytes. Pools [n_pages][n_head_kv][page_size][hd] of codes, and beside each a pool of scales
  * [n_pages][n_head_kv][page_size / 16]: a byte b for each 16 neighbouring positions of a page and head. A value is its code times 2^(b - 127) (e8m0). Codes are
- * whole numbers from -127 to 127 (I8) or e4m3 (its two NaN codes count as 480 and -480). */
+ * whole numbers from -127 to 127 (I8) or e4m3. */
 #define LLAMD_PAGED_I8 3
 #define LLAMD_PAGED_E4M3 4
 /* As above; type is q_out's and out's, cache one of the two. Set and freed as above; goes with append8 and attention8 only, as a batch of the former with
@@ -477,7 +477,8 @@ int llamd_fwd_paged_append(const void *batch, const void *q, const void *k, cons
                            int rope_rows, int rot, int interleaved, void *q_out, size_t out_stride, void *k_pages, void *v_pages);
 /* The same into a cache in 8 bits. A block's scale is the least power of two with which its new values fit (between 2^-24 and 2^9 for I8, 2^-15 and 2^7 for
  * E4M3: every value is then exact in f16), and no less than it was where the block holds older positions of the sequence: their codes are rounded
- * again when it grows. Values are rounded to even; larger ones than the largest scale takes (65024, 57344), infinities among them, become the largest; a NaN becomes 0. Rows and scales
+ * again when it grows. Values are rounded to even; larger ones than the largest scale takes (65024, 57344), infinities among them, become the largest; a NaN
+ * counts for nothing in a scale, and becomes 0 in I8. Rows and scales
  * without new tokens, and rows behind a sequence's last, stay as they are. A page that new tokens go to belongs to one
  * sequence: refused where two of the batch's would write to one. */
 int llamd_fwd_paged_append8(const void *batch, const void *q, const void *k, const void *v, int in_type, size_t q_stride,

@@ -60,10 +60,11 @@ struct Batch {
     const int32_t *begin = nullptr;                      // large: each CTA's
     const PagedMerge *merge = nullptr;
     const PagedPart *part = nullptr;
-    // of a cache in 8 bits: where new tokens meet scale blocks, and the pages that the large pieces read, in 16 bits (K's, then V's)
+    // of a cache in 8 bits: where new tokens meet scale blocks, each CTA's small pieces, and the pages that the large pieces read, in 16 bits (K's, then V's)
     const PagedBlock *block = nullptr;
     const PagedWide *wide = nullptr;
-    int n_block = 0, n_wide = 0;
+    const int32_t *small_begin = nullptr;
+    int n_block = 0, n_wide = 0, small_ctas = 0;
     KeptBlock widened;
     bool shared_write = false;  // two sequences have new tokens in one page
     bool beside = false;
@@ -405,7 +406,7 @@ int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int
     std::vector<int32_t> wide_table;
     bool shared_write = false;
     try {
-        make_plan(plan, v, q_len, kv_len, b->sms);
+        make_plan(plan, v, q_len, kv_len, b->sms, b->cache != 0);
         if (b->cache) {
             blocks_of(block, n_seq, q_len, kv_len);
             wide_pages(wide, wide_table, plan, v, pages, pages_stride);
@@ -420,7 +421,7 @@ int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int
     const size_t o_token = section<PagedToken>(bytes, v.tokens), o_table = section<int32_t>(bytes, (size_t)n_seq * v.table_stride + wide_table.size()), o_small = section<PagedItem>(bytes, plan.small.size()),
                  o_large = section<PagedItem>(bytes, plan.large.size()), o_begin = section<int32_t>(bytes, plan.begin.size()),
                  o_merge = section<PagedMerge>(bytes, plan.merge.size()), o_part = section<PagedPart>(bytes, plan.part.size()), o_block = section<PagedBlock>(bytes, block.size()),
-                 o_wide = section<PagedWide>(bytes, wide.size());
+                 o_wide = section<PagedWide>(bytes, wide.size()), o_small_begin = section<int32_t>(bytes, plan.small_begin.size());
     if (plan.beside && !side_ready()) {
         set_error(cudaGetLastError(), "paged batch: side stream");
         return -1;
@@ -437,6 +438,7 @@ int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int
     put(o_merge, plan.merge.data(), plan.merge.size() * sizeof(PagedMerge));
     put(o_part, plan.part.data(), plan.part.size() * sizeof(PagedPart));
     put(o_block, block.data(), block.size() * sizeof(PagedBlock));
+    put(o_small_begin, plan.small_begin.data(), plan.small_begin.size() * sizeof(int32_t));
     put(o_wide, wide.data(), wide.size() * sizeof(PagedWide));
     put(o_table + (size_t)n_seq * v.table_stride * sizeof(int32_t), wide_table.data(), wide_table.size() * sizeof(int32_t));
     PagedToken *token = (PagedToken *)(b->host.p + o_token);
@@ -455,6 +457,8 @@ int llamd_cuda_paged_set(void *batch, int n_seq, const int32_t *q_len, const int
     b->part = (const PagedPart *)(b->dev.p + o_part);
     b->block = (const PagedBlock *)(b->dev.p + o_block);
     b->wide = (const PagedWide *)(b->dev.p + o_wide);
+    b->small_begin = (const int32_t *)(b->dev.p + o_small_begin);
+    b->small_ctas = std::max(1, (int)plan.small_begin.size()) - 1;
     b->n_block = (int)block.size(), b->n_wide = (int)wide.size(), b->shared_write = shared_write;
     b->beside = plan.beside;
     b->n_small = (int)plan.small.size(), b->small_rows = plan.small_rows, b->n_ctas = (int)plan.begin.size() - 1, b->n_merge = (int)plan.merge.size(), b->most = plan.most;
@@ -568,7 +572,7 @@ static int attention_of(Batch *b, const void *q, size_t q_stride, const void *k_
         a.item = b->small;
         if (b->beside) LLAMD_TRY(cudaStreamWaitEvent(g_side, g_fork, 0), "paged attention: fork");
         const cudaStream_t to = b->beside ? g_side : stream();
-        if (b->cache) paged_decode8_launch(a, b->type, b->cache, b->n_small, b->small_rows, to);
+        if (b->cache) paged_decode8_launch(a, b->type, b->cache, b->small_begin, b->small_ctas, b->small_rows, to);
         else paged_decode_launch(a, b->type, b->n_small, b->small_rows, to);
     }
     if (b->beside) {

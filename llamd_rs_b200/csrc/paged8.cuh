@@ -13,8 +13,7 @@ template <int C> struct Cache8;
 template <> struct Cache8<kPagedI8> {
     static constexpr float kMost = 127.0f;
     static constexpr int kLow = -24, kHigh = 9;
-    // f16x2 of the codes in bytes 0, 1 (half 0) or 2, 3 (half 1) of x, times 2^-kShift. 1024 + 128 + c is a half whose low byte is c with its sign bit flipped.
-    static constexpr int kShift = 0;
+    // f16x2 of the codes in bytes 0, 1 (half 0) or 2, 3 (half 1) of x. 1024 + 128 + c is a half whose low byte is c with its sign bit flipped.
     template <int HALF> static __device__ __forceinline__ uint32_t f16x2(uint32_t x) {
         const uint32_t y = __byte_perm(x ^ 0x80808080u, 0x64646464u, HALF ? 0x4342 : 0x4140), bias = 0x64806480u;
         const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&y), *reinterpret_cast<const __half2 *>(&bias));
@@ -24,11 +23,12 @@ template <> struct Cache8<kPagedI8> {
 template <> struct Cache8<kPagedE4m3> {
     static constexpr float kMost = 448.0f;
     static constexpr int kLow = -15, kHigh = 7;
-    // The code's bits as a half's sign, low exponent bits and high mantissa bits: 2^-8 of its value, subnormals too.
-    static constexpr int kShift = 8;
+    // (33 pairs a clock and SM measured, where a permutation, a shift and two logical operations, which give 2^-8 of a pair, go at 64 a clock each)
     template <int HALF> static __device__ __forceinline__ uint32_t f16x2(uint32_t x) {
-        const uint32_t t = __byte_perm(x, 0, HALF ? 0x3424 : 0x1404);
-        return (t & 0x80008000u) | ((t >> 1) & 0x3F803F80u);
+        uint32_t y;
+        if constexpr (HALF) asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, b;\n\t}" : "=r"(y) : "r"(x));
+        else asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\t}" : "=r"(y) : "r"(x));
+        return y;
     }
 };
 

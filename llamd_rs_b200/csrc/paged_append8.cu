@@ -3,7 +3,7 @@
 //   y = rotate(x / sqrt(mean(x^2) + eps) * w)         as there, in f32
 //   e = the least exponent with max |y| <= most 2^e   over the block's new rows of one head, most the largest code; between the format's kLow and kHigh
 //   e = max(e, the block's own)                       where it holds older rows, whose codes c become round(c 2^(own - e))
-//   code = round(y 2^-e), to even; beyond the largest code: the largest; of a NaN: 0
+//   code = round(y 2^-e), to even; beyond the largest code: the largest; a NaN stays one in e4m3, and is 0 in i8
 //
 // A warp has a block of one head: up to 16 rows, hd / 8 lanes to a row and 8 elements of it to a lane (four pairs that rotate together), so that y stays in registers
 // from the maximum to the codes and every input is read once. A block belongs to one warp alone: no atomics, and the same
@@ -25,7 +25,6 @@ constexpr int kAppend8Ctas = 2;  // (a block's 64 values to a lane)
 // four codes
 template <int C> __device__ __forceinline__ uint32_t codes(float a, float b, float c, float d);
 template <> __device__ __forceinline__ uint32_t codes<kPagedE4m3>(float a, float b, float c, float d) {
-    a = a != a ? 0.0f : a, b = b != b ? 0.0f : b, c = c != c ? 0.0f : c, d = d != d ? 0.0f : d;
     const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3), hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
     return lo | hi << 16;
 }
@@ -38,9 +37,8 @@ template <> __device__ __forceinline__ uint32_t codes<kPagedI8>(float a, float b
 template <int C>
 __device__ __forceinline__ uint32_t again(uint32_t x, float by) {
     using Cv = Cache8<C>;
-    const float up = by * (float)(1 << Cv::kShift);
     const float2 lo = Half16<__half>::to_f32(Cv::template f16x2<0>(x)), hi = Half16<__half>::to_f32(Cv::template f16x2<1>(x));
-    return codes<C>(lo.x * up, lo.y * up, hi.x * up, hi.y * up);
+    return codes<C>(lo.x * by, lo.y * by, hi.x * by, hi.y * by);
 }
 // the byte of the least scale that takes values up to `top`
 template <int C>

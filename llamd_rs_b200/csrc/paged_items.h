@@ -49,6 +49,9 @@ struct PagedPart {
 // twice as often (102.9).
 constexpr int kPagedSmallRows = 32, kPagedPieceRows = 16;
 
+// paged_decode8.cu: CTAs to an SM.
+constexpr int kDecode8Ctas = 2;
+
 // paged_prompt.cu: two tiles of so many query rows to a piece, positions to a block.
 constexpr int kPagedTileRows = 128, kPagedBlock = 128;
 

