@@ -125,6 +125,7 @@ unsafe extern "C" {
     pub fn llamd_fwd_moe_combine(down: *const f32, weights: *const f32, out: *mut f32, n_used: c_int, n_embd: c_int);
     pub fn llamd_fwd_moe_combine_add(down: *const f32, weights: *const f32, residual: *const f32, out: *mut f32, n_used: c_int, n_embd: c_int, nseq: c_int);
     pub fn llamd_fwd_argmax(x: *const f32, n: c_int, scratch_v: *mut f32, scratch_i: *mut i32, out: *mut i32, nblocks: c_int, nseq: c_int);
+    pub fn llamd_fwd_sample(logits: *const c_void, type_: c_int, stride: usize, rows: c_int, n_vocab: c_int, temperature: *const f32, top_k: *const i32, top_p: *const f32, min_p: *const f32, uniform: *const f32, token: *mut i32, prob: *mut f32) -> c_int;
     pub fn llamd_fwd_moe_group(ids: *const i32, n_expert: c_int, n_used: c_int, nseq: c_int, gstart: *mut i32, gcount: *mut i32, ptoken: *mut i32, pslot: *mut i32);
     pub fn llamd_fwd_moe_group_work(ids: *const i32, n_expert: c_int, n_used: c_int, nseq: c_int, gstart: *mut i32, gcount: *mut i32, ptoken: *mut i32, pslot: *mut i32, work: *mut i32, n_work: *mut i32);
     pub fn llamd_fwd_matvec_tokens(w0: *const c_void, w1: *const c_void, w2: *const c_void, aq: *const i8, ad: *const f32, o0: *mut f32, o1: *mut f32, o2: *mut f32, blocks: c_int, rows0: c_int, rows1: c_int, rows2: c_int, ntok: c_int);
@@ -210,6 +211,7 @@ unsafe extern "C" {
     pub fn llamd_model_launches_per_pass(m: *mut llamd_model) -> c_ulonglong;
     pub fn llamd_model_profile_pass(m: *mut llamd_model, token: i32, pos: i32, ms_out: *mut f32) -> c_int;
     pub fn llamd_model_logits(m: *mut llamd_model, host_out: *mut f32, nseq: c_int) -> c_int;
+    pub fn llamd_model_sample(m: *mut llamd_model, nseq: c_int, temperature: *const f32, top_k: *const i32, top_p: *const f32, min_p: *const f32, uniform: *const f32, out_tokens: *mut i32, out_probs: *mut f32) -> c_int;
     pub fn llamd_model_read_trace(m: *mut llamd_model, x_out: *mut f32, ids_out: *mut i32) -> c_int;
     pub fn llamd_model_read_kv(m: *mut llamd_model, layer: c_int, seq: c_int, n_pos: c_int, k_out: *mut f32, v_out: *mut f32) -> c_int;
 }

@@ -271,6 +271,16 @@ void llamd_fwd_moe_combine_add(const float *down, const float *weights, const fl
                                float *out, int n_used, int n_embd, int nseq);           /* :586 */
 void llamd_fwd_argmax(const float *x, int n, float *scratch_v, int32_t *scratch_i, int32_t *out,
                       int nblocks, int nseq);                                           /* :332 */
+/* A token for each row by other rules than the largest logit (no counterpart in the reference, which decodes greedily). Row r: n_vocab logits from r * stride on
+ * (elements; type LLAMD_PAGED_F32, _F16 or _BF16); its settings and its uniform number in [0, 1) are element r of device arrays, of which temperature, top_k, top_p
+ * and min_p may be NULL (1, and no limits). Weights exp((x - max) / temperature); tokens in order of falling logit, equal ones of rising index; kept are the
+ * first top_k (0 and less: all), of those the ones whose predecessors weigh less than top_p times the k's together (1 and more: all; the first always is), of those the ones
+ * that weigh min_p of the first's or more. token[r]: by rising index the first at which the kept weights up to it are more than uniform times all of
+ * them; prob[r] (may be NULL): its share of them. A temperature that is not above 0: the first token, share 1. NaN logits count as -inf; a row with nothing else: -1
+ * and 0. Weights are taken in whole multiples of 2^-40 of the first's and summed exactly: the same token every time. n_vocab up to 393216. Numbers outside their range are
+ * brought to its ends (a NaN limits nothing, and as a uniform number is 0). Enqueues; 0, or -1 and a message where refused, and nothing was launched. */
+int llamd_fwd_sample(const void *logits, int type, size_t stride, int rows, int n_vocab, const float *temperature, const int32_t *top_k,
+                     const float *top_p, const float *min_p, const float *uniform, int32_t *token, float *prob);
 
 /* Expert scatter plan (crates/llamd-vulkan/shaders/moe_group.comp:40-82):
  * counting sort of the nseq*n_used (token, slot) pairs by expert. Within an

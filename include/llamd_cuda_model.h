@@ -219,6 +219,11 @@ enum {
 int llamd_model_profile_pass(llamd_model *m, int32_t token, int32_t pos, float *ms_out);
 /* Logits of the last pass, [nseq][n_vocab], to host memory (device.rs:966). */
 int llamd_model_logits(llamd_model *m, float *host_out, int nseq);
+/* The next tokens of the last pass's nseq rows of logits by llamd_fwd_sample's rules (no counterpart in the reference). Host arrays of nseq: settings (NULL: 1, and no
+ * limits), uniform numbers in [0, 1), tokens and their shares of the kept weights (probs may be NULL). Synchronises. -1 and a message where a setting is out of range: a
+ * temperature below 0, top_p or min_p outside [0, 1]. */
+int llamd_model_sample(llamd_model *m, int nseq, const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
+                       const float *uniform, int32_t *out_tokens, float *out_probs);
 /* With "trace" on: x after every layer [n_layer][max_seq][n_embd] and the
  * routed expert ids [n_layer][max_seq][n_expert_used] of the last pass. */
 int llamd_model_read_trace(llamd_model *m, float *x_out, int32_t *ids_out);

@@ -124,6 +124,7 @@ SIGNATURES = {
     "llamd_fwd_moe_combine": (None, [vp, vp, vp, i32, i32]),
     "llamd_fwd_moe_combine_add": (None, [vp, vp, vp, vp, i32, i32, i32]),
     "llamd_fwd_argmax": (None, [vp, i32, vp, vp, vp, i32, i32]),
+    "llamd_fwd_sample": (i32, [vp, i32, sz, i32, i32, vp, vp, vp, vp, vp, vp, vp]),
     "llamd_fwd_matvec_tokens": (None, [vp, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32]),
     "llamd_fwd_expert_major": (None, [vp, vp, vp, vp, i32, vp, vp, vp, vp, vp, vp, i32, i32, i32]),
     "llamd_fwd_q8k_residue_major": (None, [vp, vp, sz]),

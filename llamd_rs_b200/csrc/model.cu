@@ -148,7 +148,7 @@ struct Model {
     Buf head_rm, aq2_rm;     // a batch's activations in the GEMM's operand order, and its experts' (decode pass)
     Buf plan;                // ... and its scatter plan: gstart, gcount [n_expert], ptoken, pslot [max_seq * n_expert_used]
     Buf slot_order;          // [max_seq * n_expert_used] a batch's (sequence, slot) pairs sorted by expert (decode pass, 8 sequences and more)
-    Buf e_gate, e_up, e_down, logits, amax_v, amax_i, out_token, meta;
+    Buf e_gate, e_up, e_down, logits, amax_v, amax_i, out_token, meta, sample;
     Buf trace_x, trace_ids;  // [n_layer][max_seq][n_embd], [n_layer][max_seq][n_used]
     Buf scores;              // [max_seq][n_head][max_kv] scaled attention logits
     Buf router_counter;      // the router kernel's arrival counters, one per sequence
@@ -992,7 +992,7 @@ void llamd_model_free(llamd_model *h) {
             b->release();
     for (Buf *b : {&m->tok_embd, &m->output_norm, &m->output, &m->rope_tab, &m->x, &m->xb, &m->xb2, &m->q, &m->k, &m->v, &m->attn,
                    &m->aq, &m->ad, &m->aq2, &m->ad2, &m->router_logits, &m->router_probs, &m->expert_ids, &m->slot_order, &m->dense_fold, &m->head_rm, &m->aq2_rm, &m->plan, &m->expert_w, &m->e_gate,
-                   &m->e_up, &m->e_down, &m->logits, &m->amax_v, &m->amax_i, &m->out_token, &m->meta, &m->trace_x, &m->trace_ids,
+                   &m->e_up, &m->e_down, &m->logits, &m->amax_v, &m->amax_i, &m->out_token, &m->meta, &m->sample, &m->trace_x, &m->trace_ids,
                    &m->tok_log, &m->tok_count, &m->router_counter, &m->tail_counter, &m->scores, &m->ids_all, &m->ad_all, &m->aq_all, &m->gate_all,
                    &m->up_all, &m->aq2_all, &m->ad2_all, &m->down_all, &m->recv_all, &m->ep_arrive, &m->ep_status, &m->ep_out_tab,
                    &m->ep_arrive_tab, &m->ep_disp, &m->ep_epoch, &m->ep_ids_tab, &m->ep_ad_tab, &m->ep_aq_tab, &m->ep_disp_tab, &m->mega_layers, &m->mega_bar, &m->mega_status, &m->mega_prof,
@@ -2116,6 +2116,36 @@ int llamd_model_logits(llamd_model *h, float *host_out, int nseq) {
     Model *m = (Model *)h;
     if (!m || !host_out || nseq < 1 || nseq > m->max_seq) return -1;
     return llamd_fwd_download(host_out, m->logits.p, (size_t)nseq * m->hp.n_vocab * sizeof(float));
+}
+
+int llamd_model_sample(llamd_model *h, int nseq, const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p, const float *uniform,
+                       int32_t *out_tokens, float *out_probs) {
+    Model *m = (Model *)h;
+    if (!m || nseq < 1 || nseq > m->max_seq || !uniform || !out_tokens) return -1;
+    m->err.clear();
+    for (int s = 0; s < nseq; s++) {
+        const bool good = (!temperature || temperature[s] >= 0.0f) && (!top_p || (top_p[s] >= 0.0f && top_p[s] <= 1.0f)) && (!min_p || (min_p[s] >= 0.0f && min_p[s] <= 1.0f)) &&
+                          uniform[s] >= 0.0f && uniform[s] < 1.0f;
+        if (!good) {
+            m->err = "sample: row " + std::to_string(s) + ": temperature from 0, top_p and min_p from 0 to 1, the uniform number from 0 and below 1";
+            return -1;
+        }
+    }
+    // [7][max_seq] words: the settings, the numbers, tokens and shares
+    const size_t S = (size_t)m->max_seq;
+    if (!m->sample.p && !m->sample.alloc(7 * S * 4)) return -1;
+    const void *from[5] = {temperature, top_k, top_p, min_p, uniform};
+    uint8_t *at[7];
+    for (int i = 0; i < 7; i++) at[i] = (uint8_t *)m->sample.p + i * S * 4;
+    for (int i = 0; i < 5; i++)
+        if (from[i] && llamd_fwd_upload(at[i], from[i], (size_t)nseq * 4) != 0) return -1;
+    if (llamd_fwd_sample(m->logits.p, LLAMD_PAGED_F32, (size_t)m->hp.n_vocab, nseq, m->hp.n_vocab, temperature ? (float *)at[0] : nullptr, top_k ? (int32_t *)at[1] : nullptr,
+                         top_p ? (float *)at[2] : nullptr, min_p ? (float *)at[3] : nullptr, (float *)at[4], (int32_t *)at[5], (float *)at[6]) != 0) {
+        m->err = llamd_cuda_last_error_string();
+        return -1;
+    }
+    if (out_probs && llamd_fwd_download(out_probs, at[6], (size_t)nseq * 4) != 0) return -1;
+    return llamd_fwd_download(out_tokens, at[5], (size_t)nseq * 4);
 }
 
 int llamd_model_read_trace(llamd_model *h, float *x_out, int32_t *ids_out) {

@@ -55,6 +55,8 @@ def _bind():
     L.llamd_model_forward_batch.argtypes = [vp, vp, vp, i32, vp]
     L.llamd_model_logits.restype = i32
     L.llamd_model_logits.argtypes = [vp, vp, i32]
+    L.llamd_model_sample.restype = i32
+    L.llamd_model_sample.argtypes = [vp, i32, vp, vp, vp, vp, vp, vp, vp]
     L.llamd_model_read_trace.restype = i32
     L.llamd_model_read_trace.argtypes = [vp, vp, vp]
     L.llamd_model_read_kv.restype = i32
@@ -435,6 +437,40 @@ class CudaModel:
         if self._L.llamd_model_logits(self._h, out.ctypes.data, nseq) != 0:
             raise backend.Other("logits: " + self._err())
         return out
+
+    def sample(self, uniform, temperature=None, top_k=None, top_p=None, min_p=None):
+        """The next tokens of the last pass's rows of logits (llamd_model_sample): one uniform number in [0, 1) for each row, settings for each row or one for all,
+        None for no limit. -> (tokens int32, their shares of the kept weights)"""
+        u = np.ascontiguousarray(np.atleast_1d(np.asarray(uniform, dtype=np.float32)))
+        if u.ndim != 1 or not 1 <= u.size <= self.max_seq:
+            raise backend.ShapeError(f"sample: {u.shape} uniform numbers for up to {self.max_seq} rows")
+        settings = []
+        for what, x, t in (("temperature", temperature, np.float32), ("top_k", top_k, np.int32), ("top_p", top_p, np.float32), ("min_p", min_p, np.float32)):
+            if x is not None:
+                a = np.asarray(x)
+                if a.ndim > 1 or (a.ndim == 1 and a.size != u.size) or (t == np.int32 and a.dtype.kind not in "iu"):
+                    raise backend.Malformed(f"sample: {what} for {u.size} rows: {a.dtype}, {a.shape}")
+                if t == np.int32 and (a.size and (int(a.min()) < -2 ** 31 or int(a.max()) >= 2 ** 31)):
+                    raise backend.Malformed(f"sample: {what} beyond 32 bits")
+                x = np.ascontiguousarray(np.broadcast_to(a.astype(t), u.shape))
+            settings.append(x)
+        tokens, probs = np.zeros(u.size, dtype=np.int32), np.zeros(u.size, dtype=np.float32)
+        at = [None if a is None else a.ctypes.data for a in (*settings, u, tokens, probs)]
+        if self._L.llamd_model_sample(self._h, u.size, *at) != 0:
+            raise backend.Malformed("sample: " + (self._err() or backend._last_error()))
+        return tokens, probs
+
+    def sample_decode(self, first_token: int, start_pos: int, uniforms, **settings):
+        """Tokens after `first_token` at `start_pos`, one for each uniform number, each drawn by `sample`'s rules from the pass before and fed to the next.
+        -> (tokens int32, shares)"""
+        out, probs, token = [], [], int(first_token)
+        for i, u in enumerate(np.asarray(uniforms, dtype=np.float32).ravel()):
+            self.forward(token, start_pos + i)
+            t, s = self.sample([u], **settings)
+            token = int(t[0])
+            out.append(token)
+            probs.append(s[0])
+        return np.array(out, dtype=np.int32), np.array(probs, dtype=np.float32)
 
     def read_trace(self):
         """-> (x [n_layer][max_seq][n_embd], ids [n_layer][max_seq][n_used]) of the last traced pass"""

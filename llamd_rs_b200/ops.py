@@ -256,6 +256,21 @@ def argmax(x, nblocks: int = 512):
     return do.download_i32(nseq)
 
 
+def sample(x, uniform, temperature=None, top_k=None, top_p=None, min_p=None):
+    """x f32 [rows][n_vocab], uniform numbers and settings for each row -> (tokens, their shares of the kept weights) (llamd_fwd_sample)."""
+    from . import sampling
+
+    x = _f32(x)
+    x2 = x.reshape(-1, x.shape[-1])
+    rows, n = x2.shape
+    per_row = lambda a, t: None if a is None else DevBuf.from_array(np.ascontiguousarray(np.broadcast_to(np.asarray(a, dtype=t), (rows,))))  # noqa: E731
+    dx, token, prob = DevBuf.from_array(x2), DevBuf(4 * rows), DevBuf(4 * rows)
+    du, dt, dk, dp, dm = (per_row(a, t) for a, t in ((uniform, np.float32), (temperature, np.float32), (top_k, np.int32), (top_p, np.float32), (min_p, np.float32)))
+    sampling.sample(dx, du, token, dt, dk, dp, dm, prob, rows=rows, n_vocab=n)
+    backend.sync()
+    return token.download_i32(rows), prob.download_f32(rows)
+
+
 def moe_group(ids, n_expert: int, n_used: int):
     """ids int32 [nseq][n_used] -> dict(gstart, gcount, ptoken, pslot, work [n_work][3])."""
     ids = np.ascontiguousarray(ids, dtype=np.int32)
