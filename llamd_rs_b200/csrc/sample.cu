@@ -7,13 +7,15 @@
 // Every weight is a whole multiple of 2^-40 (from an exponential in 64 bits, off by 2^-43), so that sums are exact and the same in whatever order they are made, and a
 // token is another than in exact arithmetic only where u falls within some 2^-40 of a border.
 //
-// A row belongs to a cluster of up to 8 CTAs, each with a part of it in shared memory: read once from memory, looked at as often as need be. A histogram of the logits
-// (kBins over their range: tokens, and where a share of the weights is asked for the weights themselves, exactly, as three 14-bit digits) finds the bin in which the kept ones
-// end. Are there at most kList tokens up to it, one CTA sorts them and settles everything: all rows with a small k, and those whose nucleus is small. Otherwise that bin is
-// cut in bins again, of (logit, index) compared as one number, until kList or fewer are in it, which are sorted; then every thread adds up the kept weights of a stretch of
-// neighbours, and the one that u falls on looks through its own.
-// What it costs: the row's bytes; three to eight joins of the cluster one behind the other; and for rows without a k an exponential in 64 bits for each
-// token, some 16 operations at 64 a clock and SM, once for the histogram and once for the stretches.
+// A row belongs to a cluster of 1 to 8 CTAs. The first look at it finds its top, and every thread's largest logit: what is at least the j-th largest of those is at least
+// j tokens, and little more. With j = k, or some hundreds where only a share of the weights is asked for, these few are gathered in a second look, in which the weights
+// of all are summed where a share of them is wanted, and one CTA sorts them and settles the row. Where they are too many, or their weights too little (a large k, a flat
+// row), a histogram of all logits (kBins over their range: tokens, and weights exactly, as three 14-bit digits) finds the bin in which the kept ones end; that bin is cut in
+// bins again, of (logit, index) compared as one number, until kList or fewer are in it, which are sorted. What is kept then, or where min-p is the only limit, is weighed tile by tile
+// of 128 neighbours, and the tile that u falls on looked through.
+// Few rows are kept in shared memory, each looked at there; of many, parts are read again, from L2.
+// What it costs: the row's bytes; five joins of the cluster one behind the other, some ten in the long way; and for rows without a k an exponential in 64 bits for each
+// token, some 16 operations at 64 a clock and SM, once for the sum and once or twice for the rest.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -27,8 +29,10 @@ namespace {
 namespace cg = cooperative_groups;
 typedef unsigned long long u64;
 
-constexpr int kThreads = 512, kWarpsN = kThreads / 32, kBins = 1024, kList = 1024, kMostCtas = 8;
-constexpr int kMostTokens = kMostCtas * 49152;  // what a cluster's shared memory holds
+constexpr int kThreads = 512, kWarpsN = kThreads / 32, kBins = 1024, kList = 1024, kMostCtas = 8, kTile = 128;
+static_assert(kBins % 2 == 0, "bins are read two at a time");
+constexpr int kMostTokens = 393216, kMostPart = 262144;  // of a row; of a CTA (the digits' sums have 32 bits, the tiles' sums room)
+constexpr int kShare = 512;  // tokens that are gathered where a share of the weights is asked for
 
 struct SampleParams {
     const void *x;
@@ -53,12 +57,13 @@ struct Shared {
     // of the row (CTA 0)
     u64 total, before, cut;
     int bin, n_range, n_list;
-    uint32_t hist[kBins];
+    alignas(16) uint32_t hist[kBins];
     union {
-        uint32_t digit[3][kBins];  // of the bins' weights: bits 0 to 13, 14 to 27, 28 to 40 of each, summed (a part has fewer than 2^18 tokens)
-        struct {                   // (CTA 0, when the histogram has been read)
+        alignas(16) uint32_t digit[3][kBins];  // of the bins' weights: bits 0 to 13, 14 to 27, 28 to 40 of each, summed
+        struct {                   // (when the histogram has been read) some tokens' places, CTA 0's the whole row's in the end, and their weights
             u64 list[kList], weight[kList];
         };
+        u64 tile[kMostPart / kTile];  // (last of all)
     };
 };
 
@@ -162,8 +167,9 @@ __device__ __forceinline__ void sort_list(u64 *list, int size) {
     __syncthreads();
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) {
+// CACHED: the CTA's part is kept in shared memory.
+template <typename T, bool CACHED>
+__global__ void __launch_bounds__(kThreads, CACHED ? 1 : 2) sample_kernel(const SampleParams p) {
     extern __shared__ __align__(16) uint8_t raw[];
     Shared &sh = *reinterpret_cast<Shared *>(raw);
     float *const x = reinterpret_cast<float *>(raw + sizeof(Shared));
@@ -172,34 +178,45 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, at = rank * p.part, mine = max(0, min(p.part, p.n - at));
     Shared &lead = *cluster.map_shared_rank(&sh, 0);
     auto of = [&](int r) { return cluster.map_shared_rank(&sh, r); };
+    const T *const src = reinterpret_cast<const T *>(p.x) + (size_t)row * p.stride + at;
+    auto clean = [](float v) { return v == v ? v + 0.0f : -INFINITY; };  // (NaN is no token; -0 is 0)
+    constexpr int kWide = 16 / sizeof(T);
+    const int wide = ((uintptr_t)src & 15) == 0 ? mine / kWide : 0;
+    // f(i, logit) for the part's tokens, of one thread in rising order
+    auto from_memory = [&](auto f) {
+#pragma unroll 4
+        for (int i = threadIdx.x; i < wide; i += kThreads) {
+            const uint4 v = reinterpret_cast<const uint4 *>(src)[i];
+            const T *e = reinterpret_cast<const T *>(&v);
+#pragma unroll
+            for (int j = 0; j < kWide; j++) f(i * kWide + j, clean(to_float(e[j])));
+        }
+#pragma unroll 4
+        for (int i = wide * kWide + threadIdx.x; i < mine; i += kThreads) f(i, clean(to_float(src[i])));
+    };
+    auto each = [&](auto f) {
+        if constexpr (CACHED) {
+#pragma unroll 4
+            for (int i = threadIdx.x; i < mine; i += kThreads) f(i, x[i]);
+        } else {
+            from_memory(f);
+        }
+    };
+    auto value = [&](int i) { return CACHED ? x[i] : clean(to_float(src[i])); };
     pdl_trigger();
+    for (int i = threadIdx.x; i < kBins; i += kThreads) sh.hist[i] = 0;
     if (threadIdx.x == 0) sh.n_list = 0;
     pdl_wait();
 
-    // ---- this CTA's part of the row, its first token in order, its least logit above -inf, how many are ----
-    const T *const src = reinterpret_cast<const T *>(p.x) + (size_t)row * p.stride + at;
-    u64 first = ~0ull;
-    float least = INFINITY;
-    int live = 0;
-    auto take = [&](int i, float v) {
-        v = v == v ? v + 0.0f : -INFINITY;  // (NaN is no token; -0 is 0)
-        x[i] = v;
-        const u64 o = order_of(v, at + i);
-        first = o < first ? o : first;
+    // ---- the first look: the thread's largest logit, the row's top, its least above -inf, how many are ----
+    float best = -INFINITY, least = INFINITY;
+    int best_at = 0, live = 0;
+    from_memory([&](int i, float v) {
+        if (CACHED) x[i] = v;
+        if (v > best) best = v, best_at = i;
         if (v > -INFINITY) least = fminf(least, v), live++;
-    };
-    constexpr int kWide = 16 / sizeof(T);
-    const int wide = ((uintptr_t)src & 15) == 0 ? mine / kWide : 0;
-#pragma unroll 4
-    for (int i = threadIdx.x; i < wide; i += kThreads) {
-        const uint4 v = __ldcs(reinterpret_cast<const uint4 *>(src) + i);
-        const T *e = reinterpret_cast<const T *>(&v);
-#pragma unroll
-        for (int j = 0; j < kWide; j++) take(i * kWide + j, to_float(e[j]));
-    }
-#pragma unroll 4
-    for (int i = wide * kWide + threadIdx.x; i < mine; i += kThreads) take(i, to_float(src[i]));
-    first = warp_least(first);
+    });
+    u64 first = warp_least(best > -INFINITY ? order_of(best, at + best_at) : ~0ull);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
@@ -207,22 +224,27 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) 
     }
     if (lane == 0) sh.low[warp] = first, sh.least[warp] = least, sh.count[warp] = live;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < kWarpsN; w++) first = sh.low[w] < first ? sh.low[w] : first, least = fminf(least, sh.least[w]), live += sh.count[w];
-        sh.first = first, sh.part_least = least, sh.part_count = live;
+    if (warp == 0) {
+        first = warp_least(lane < kWarpsN ? sh.low[lane] : ~0ull);
+        least = lane < kWarpsN ? sh.least[lane] : INFINITY, live = lane < kWarpsN ? sh.count[lane] : 0;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
+        live = __reduce_add_sync(0xffffffffu, live);
+        if (lane == 0) sh.first = first, sh.part_least = least, sh.part_count = live;
     }
     cluster.sync();
-    live = 0;
-    for (int r = 0; r < ctas; r++) {
-        const Shared &o = *of(r);
-        first = r == 0 || o.first < first ? o.first : first;
-        least = r == 0 ? o.part_least : fminf(least, o.part_least);
-        live += o.part_count;
+    {  // (a lane to a CTA; each warp for itself)
+        const Shared &o = *of(lane < ctas ? lane : 0);
+        first = warp_least(o.first), least = o.part_least, live = lane < ctas ? o.part_count : 0;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) least = fminf(least, __shfl_xor_sync(0xffffffffu, least, d));
+        live = __reduce_add_sync(0xffffffffu, live);
     }
     const float top = logit_of(first);
     const float temperature = p.temperature ? p.temperature[row] : 1.0f;
     const int32_t k_in = p.top_k ? p.top_k[row] : 0;
-    const float p_in = p.top_p ? p.top_p[row] : 1.0f, m_in = p.min_p ? p.min_p[row] : 0.0f, u = p.u[row];
+    const float p_in = p.top_p ? p.top_p[row] : 1.0f, u = p.u[row];
+    const double least_weight = p.min_p && p.min_p[row] > 0.0f ? fminf(p.min_p[row], 1.0f) : 0.0f;
     const int k = k_in > 0 && k_in < live ? k_in : 0;
     const bool by_mass = p_in < 1.0f;
     if (!live || !(temperature > 0.0f)) {  // nothing to choose from; or the first token
@@ -266,34 +288,37 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) 
             if (d1) atomicAdd(&sh.digit[1][bin], d1);
             if (d2) atomicAdd(&sh.digit[2][bin], d2);
         };
-        // CTA 0: the first bin up to which there are k tokens, or a share of `whole` (of all that is in the bins, where that is 0)
-        auto find = [&]() {
+        // CTA 0: the first bin up to which there are `wanted` tokens, or a share of `whole` (of all that is in the bins, where that is 0)
+        auto find = [&](u64 wanted) {
             cluster.sync();
             if (rank == 0) {
                 constexpr int kPer = kBins / kThreads;
-                uint32_t c[kPer] = {};
-                u64 w[kPer] = {}, n_all, w_all = 0, n = 0, m = 0;
-                for (int r = 0; r < ctas; r++) {
-                    const Shared &o = *of(r);
+                static_assert(kPer == 2, "pairs of bins");
+                uint2 c = {0, 0};
+                u64 w[kPer] = {}, n_all, w_all = 0, n, m;
 #pragma unroll
-                    for (int j = 0; j < kPer; j++) {
-                        const int b = threadIdx.x * kPer + j;
-                        c[j] += o.hist[b];
-                        if (!counting) w[j] += o.digit[0][b] + ((u64)o.digit[1][b] << 14) + ((u64)o.digit[2][b] << 28);
+                for (int r = 0; r < kMostCtas; r++) {
+                    if (r >= ctas) break;
+                    const Shared &o = *of(r);
+                    const uint2 h = reinterpret_cast<const uint2 *>(o.hist)[threadIdx.x];
+                    c.x += h.x, c.y += h.y;
+                    if (!wanted) {
+                        const uint2 d0 = reinterpret_cast<const uint2 *>(o.digit[0])[threadIdx.x], d1 = reinterpret_cast<const uint2 *>(o.digit[1])[threadIdx.x],
+                                    d2 = reinterpret_cast<const uint2 *>(o.digit[2])[threadIdx.x];
+                        w[0] += d0.x + ((u64)d1.x << 14) + ((u64)d2.x << 28), w[1] += d0.y + ((u64)d1.y << 14) + ((u64)d2.y << 28);
                     }
                 }
-#pragma unroll
-                for (int j = 0; j < kPer; j++) n += c[j], m += w[j];
-                n = block_prefix(n, sh.scratch, n_all);
-                m = block_prefix(m, sh.scratch, w_all);
+                n = block_prefix((u64)c.x + c.y, sh.scratch, n_all);
+                m = block_prefix(w[0] + w[1], sh.scratch, w_all);
                 if (threadIdx.x == 0 && !whole) sh.total = w_all;
                 const double want = (double)p_in * (double)(whole ? whole : w_all);
 #pragma unroll
                 for (int j = 0; j < kPer; j++) {
-                    const bool here = counting ? ahead + n < (u64)k && ahead + n + c[j] >= (u64)k
-                                               : c[j] && ((double)(ahead + m) < want || (!ahead && !m)) && (double)(ahead + m + w[j]) >= want;
-                    if (here) sh.bin = threadIdx.x * kPer + j, sh.n_range = (int)n + c[j], sh.before = ahead + (counting ? n : m);
-                    n += c[j], m += w[j];
+                    const uint32_t cj = j ? c.y : c.x;
+                    const bool here = wanted ? ahead + n < wanted && ahead + n + cj >= wanted
+                                             : cj && ((double)(ahead + m) < want || (!ahead && !m)) && (double)(ahead + m + w[j]) >= want;
+                    if (here) sh.bin = threadIdx.x * kPer + j, sh.before = ahead + (wanted ? n : m);
+                    n += cj, m += w[j];
                 }
             }
             cluster.sync();
@@ -305,50 +330,91 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) 
             __syncthreads();
             if (lane == 0) sh.low[warp] = low, sh.high[warp] = high, sh.scratch[warp] = sum, sh.count[warp] = c;
             __syncthreads();
-            if (threadIdx.x == 0) {
-                u64 l = ~0ull, h = 0, s = 0;
-                int n = 0;
-                for (int w = 0; w < kWarpsN; w++) l = sh.low[w] < l ? sh.low[w] : l, h = sh.high[w] > h ? sh.high[w] : h, s += sh.scratch[w], n += sh.count[w];
-                sh.part_low = l, sh.part_high = h, sh.mass = s, sh.part_count = n;
+            if (warp == 0) {
+                const bool in = lane < kWarpsN;
+                const u64 l = warp_least(in ? sh.low[lane] : ~0ull), h = warp_most(in ? sh.high[lane] : 0), s = warp_sum(in ? sh.scratch[lane] : 0);
+                const int n = __reduce_add_sync(0xffffffffu, in ? sh.count[lane] : 0);
+                if (lane == 0) sh.part_low = l, sh.part_high = h, sh.mass = s, sh.part_count = n;
             }
             cluster.sync();
-            low = ~0ull, high = 0, sum = 0, count = 0;
-            for (int r = 0; r < ctas; r++) {
-                const Shared &o = *of(r);
-                low = o.part_low < low ? o.part_low : low, high = o.part_high > high ? o.part_high : high, sum += o.mass, count += o.part_count;
-            }
+            const bool in = lane < ctas;
+            const Shared &o = *of(in ? lane : 0);
+            low = warp_least(o.part_low), high = warp_most(o.part_high), sum = warp_sum(in ? o.mass : 0);
+            count = __reduce_add_sync(0xffffffffu, in ? o.part_count : 0);
             cluster.sync();  // (all have read it)
         };
-        auto append = [&](bool yes, u64 o) {  // to CTA 0's list, in any order
-            const unsigned ballot = __ballot_sync(__activemask(), yes);
-            if (!yes) return;
-            const int leader = __ffs(ballot) - 1;
-            int to = 0;
-            if (lane == leader) to = atomicAdd(&lead.n_list, __popc(ballot));
-            to = __shfl_sync(ballot, to, leader) + __popc(ballot & ((1u << lane) - 1));
-            if (to < kList) lead.list[to] = o;
+        // Into this CTA's own list, in any order; all lists then into CTA 0's, where they are no more than kList in all. Between the two the cluster is joined.
+        auto append = [&](u64 o) {
+            const int to = atomicAdd(&sh.n_list, 1);
+            if (to < kList) sh.list[to] = o;
         };
-        // CTA 0's list sorted, padded to a power of two behind its n
-        auto sorted = [&](int &n, int &size) {
-            n = min(sh.n_list, kList), size = 2;
+        auto in_all_lists = [&]() {
+            const int n = lane < ctas ? of(lane < ctas ? lane : 0)->n_list : 0;
+            return __reduce_add_sync(0xffffffffu, n);
+        };
+        auto pull = [&]() {  // (CTA 0)
+            int to = sh.n_list;
+            for (int r = 1; r < ctas; r++) {
+                const Shared &o = *of(r);
+                const int n = o.n_list;
+                for (int i = threadIdx.x; i < n; i += kThreads) sh.list[to + i] = o.list[i];
+                to += n;
+            }
+            __syncthreads();
+        };
+        auto padded = [&](int n) {  // the list's n to a power of two
+            int size = 2;
             while (size < n) size <<= 1;
             for (int i = n + threadIdx.x; i < size; i += kThreads) sh.list[i] = ~0ull;
-            sort_list(sh.list, size);
+            return size;
         };
 
-        clear();
-        for (int i = threadIdx.x; i < mine; i += kThreads)
-            if (x[i] > -INFINITY) enter(bin_of(x[i]), x[i]);
-        find();
-        const int bin = lead.bin;
-        if (!k) whole = lead.total;
-        if (lead.n_range <= kList) {
-            // ---- few: one CTA settles the row ----
-            for (int i = threadIdx.x; i < mine; i += kThreads) append(x[i] > -INFINITY && bin_of(x[i]) <= bin, order_of(x[i], at + i));
+        // ---- the second look: the few that may be kept ----
+        const int groups = ctas * kThreads, wanted = k ? k : min(min(kShare, groups / 2), live);
+        bool few = wanted < groups * 3 / 4 && wanted <= kList * 3 / 4;
+        if (few) {
+            if (best > -INFINITY) atomicAdd(&sh.hist[bin_of(best)], 1u);
+            // (fewer threads than `wanted` may have a token: all of them, then)
+            if (rank == 0 && threadIdx.x == 0) sh.bin = kBins - 1;
+            find((u64)wanted);
+            const int bin = lead.bin;
+            sum = 0;
+            const bool all_mass = !k;
+            each([&](int i, float v) {
+                if (v == -INFINITY) return;
+                if (bin_of(v) <= bin) append(order_of(v, at + i));
+                if (all_mass) sum += weigh(v);
+            });
+            sum = warp_sum(sum);
+            if (lane == 0) sh.scratch[warp] = sum;
+            __syncthreads();
+            if (warp == 0) {
+                sum = warp_sum(lane < kWarpsN ? sh.scratch[lane] : 0);
+                if (lane == 0) sh.mass = sum;
+            }
             cluster.sync();
-            if (rank == 0) {
-                int n, size;
-                sorted(n, size);
+            const int n = in_all_lists();
+            few = n <= kList;
+            if (all_mass && few) {  // do they have the share?
+                whole = warp_sum(lane < ctas ? of(lane < ctas ? lane : 0)->mass : 0);
+                u64 part = 0, all;
+                if (rank == 0) {
+                    pull();
+                    for (int i = threadIdx.x; i < n; i += kThreads) part += weigh(logit_of(sh.list[i]));
+                    block_prefix(part, sh.scratch, all);
+                    if (threadIdx.x == 0) sh.part_count = n == live || (double)all >= (double)p_in * (double)whole;
+                }
+                cluster.sync();
+                few = lead.part_count;
+                cluster.sync();
+            } else if (few) {
+                if (rank == 0) pull();
+                cluster.sync();  // (the other CTAs are done)
+            }
+            if (few && rank != 0) return;
+            if (few) {
+                const int size = padded(n);
+                sort_list(sh.list, size);
                 // each thread has `per` neighbours
                 const int per = (size + kThreads - 1) / kThreads, begin = min(n, (int)threadIdx.x * per), end = min(n, begin + per), kept_k = k ? min(k, n) : n;
                 u64 part = 0, all;
@@ -362,21 +428,25 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) 
                 part = 0;
                 for (int i = begin; i < end; i++) {
                     const u64 w = sh.weight[i];
-                    const bool keep = i < kept_k && (!i || !by_mass || (double)before < limit) && weigh.exact(logit_of(sh.list[i])) >= (double)m_in;
+                    const bool keep = i < kept_k && (!i || !by_mass || (double)before < limit) && weigh.exact(logit_of(sh.list[i])) >= least_weight;
                     before += w;
                     if (!keep) sh.weight[i] = 0;
-                    part += keep ? w : 0;
+                    part += keep ? w + (1ull << 52) : 0;  // (in the top bits: how many; weights are 2^50 at most in all)
                 }
                 u64 kept;
                 block_prefix(part, sh.scratch, kept);
-                // by rising index: (index, place in order) sorted
-                for (int i = threadIdx.x; i < size; i += kThreads) sh.list[i] = i < n ? (sh.list[i] & 0xFFFFFFFFull) << 32 | (uint32_t)i : ~0ull;
-                sort_list(sh.list, size);
+                // the kept ones are the first of the list: by rising index, (index, place in order) sorted
+                const int n_kept = (int)(kept >> 52), size_kept = padded(n_kept);
+                kept &= (1ull << 52) - 1;
+                __syncthreads();
+                for (int i = threadIdx.x; i < size_kept; i += kThreads) sh.list[i] = i < n_kept ? (sh.list[i] & 0xFFFFFFFFull) << 32 | (uint32_t)i : ~0ull;
+                sort_list(sh.list, size_kept);
                 part = 0;
-                for (int i = begin; i < end; i++) part += sh.weight[(uint32_t)sh.list[i]];
+                const int last = min(end, n_kept);
+                for (int i = begin; i < last; i++) part += sh.weight[(uint32_t)sh.list[i]];
                 u64 run = block_prefix(part, sh.scratch, all);
                 const u64 want = target(kept);
-                for (int i = begin; i < end; i++) {
+                for (int i = begin; i < last; i++) {
                     const u64 w = sh.weight[(uint32_t)sh.list[i]];
                     if (run <= want && want < run + w) {
                         p.token[row] = (int32_t)(sh.list[i] >> 32);
@@ -384,20 +454,27 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) 
                     }
                     run += w;
                 }
+                return;
             }
-            cluster.sync();
-            return;
+            whole = 0;
         }
 
         // ---- many: where they end ----
+        clear();
+        each([&](int, float v) {
+            if (v > -INFINITY) enter(bin_of(v), v);
+        });
+        find((u64)k);
+        const int bin = lead.bin;
+        if (!k) whole = lead.total;
         ahead = lead.before;
-        low = ~0ull, high = 0;
-        for (int i = threadIdx.x; i < mine; i += kThreads) {
-            if (!(x[i] > -INFINITY) || bin_of(x[i]) != bin) continue;
-            const u64 o = order_of(x[i], at + i);
+        low = ~0ull, high = 0, sum = 0;
+        each([&](int i, float v) {
+            if (!(v > -INFINITY) || bin_of(v) != bin) return;
+            const u64 o = order_of(v, at + i);
             low = o < low ? o : low, high = o > high ? o : high;
             count++;
-        }
+        });
         joined();
         for (;;) {
             // (every round leaves one bin of 1024, and places are numbers of 64 bits that all differ: at most seven)
@@ -405,32 +482,34 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) 
                 int shift = 0;
                 while ((high - low) >> shift >= (u64)kBins) shift++;
                 clear();
-                for (int i = threadIdx.x; i < mine; i += kThreads) {
-                    const u64 o = order_of(x[i], at + i);
-                    if (x[i] > -INFINITY && o >= low && o <= high) enter((int)((o - low) >> shift), x[i]);
-                }
-                find();
+                each([&](int i, float v) {
+                    const u64 o = order_of(v, at + i);
+                    if (v > -INFINITY && o >= low && o <= high) enter((int)((o - low) >> shift), v);
+                });
+                find(counting ? (u64)k : 0);
                 ahead = lead.before;
                 const u64 from = low + ((u64)lead.bin << shift), to = min(high, from + ((1ull << shift) - 1));
                 low = ~0ull, high = 0, count = 0, sum = 0;
-                for (int i = threadIdx.x; i < mine; i += kThreads) {
-                    const u64 o = order_of(x[i], at + i);
-                    if (!(x[i] > -INFINITY) || o < from || o > to) continue;
+                each([&](int i, float v) {
+                    const u64 o = order_of(v, at + i);
+                    if (!(v > -INFINITY) || o < from || o > to) return;
                     low = o < low ? o : low, high = o > high ? o : high;
                     count++;
-                }
+                });
                 joined();
             }
-            if (rank == 0 && threadIdx.x == 0) sh.n_list = 0;
+            if (threadIdx.x == 0) sh.n_list = 0;
+            __syncthreads();
+            each([&](int i, float v) {
+                const u64 o = order_of(v, at + i);
+                if (v > -INFINITY && o >= low && o <= high) append(o);
+            });
             cluster.sync();
-            for (int i = threadIdx.x; i < mine; i += kThreads) {
-                const u64 o = order_of(x[i], at + i);
-                append(x[i] > -INFINITY && o >= low && o <= high, o);
-            }
-            cluster.sync();
+            const int n = min(in_all_lists(), kList);
             if (rank == 0) {
-                int n, size;
-                sorted(n, size);
+                pull();
+                const int size = padded(n);
+                sort_list(sh.list, size);
                 if (counting) {
                     if (threadIdx.x == 0) sh.cut = sh.list[max(0, min(n, k - (int)ahead) - 1)];
                 } else {
@@ -454,56 +533,83 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) 
             // a share of the k's: their weights, and all of them in doubt
             counting = false;
             low = ~0ull, high = 0, sum = 0, count = 0;
-            for (int i = threadIdx.x; i < mine; i += kThreads) {
-                const u64 o = order_of(x[i], at + i);
-                if (!(x[i] > -INFINITY) || o > cut) continue;
-                sum += weigh(x[i]);
+            each([&](int i, float v) {
+                const u64 o = order_of(v, at + i);
+                if (!(v > -INFINITY) || o > cut) return;
+                sum += weigh(v);
                 low = o < low ? o : low, high = o > high ? o : high;
                 count++;
-            }
+            });
             joined();
             whole = sum, ahead = 0;
         }
     }
 
-    // ---- the kept tokens' weights by stretches of neighbours, a stretch to a thread (an odd number: no bank is met twice) ----
-    const int per = ((mine + kThreads - 1) / kThreads) | 1, begin = min(mine, (int)threadIdx.x * per), end = min(mine, begin + per);
-    auto kept_weight = [&](int i) -> u64 {
-        const float v = x[i];
+    // ---- the kept tokens' weights by tiles of neighbours, a warp to a tile, four tokens to a lane ----
+    auto kept_weight = [&](int i, float v) -> u64 {
         if (v == -INFINITY || order_of(v, at + i) > cut) return 0;
         const double w = weigh.exact(v);
-        return w >= (double)m_in ? Weigher::units(w) : 0;
+        return w >= least_weight ? Weigher::units(w) : 0;
     };
-    u64 sum = 0, mine_all;
-    for (int i = begin; i < end; i++) sum += kept_weight(i);
-    u64 run = block_prefix(sum, sh.scratch, mine_all);
-    if (threadIdx.x == 0) sh.mass = mine_all;
-    cluster.sync();
-    u64 kept = 0;
-    for (int r = 0; r < ctas; r++) {
-        const u64 m = of(r)->mass;
-        run += r < rank ? m : 0;
-        kept += m;
-    }
-    const u64 want = target(kept);
-    if (run <= want && want < run + sum)
-        for (int i = begin; i < end; i++) {
-            const u64 w = kept_weight(i);
-            if (run <= want && want < run + w) {
-                p.token[row] = at + i;
-                if (p.prob) p.prob[row] = (float)((double)w / (double)kept);
-            }
-            run += w;
+    const int tiles = (mine + kTile - 1) / kTile;
+    auto tile_weights = [&](int t, u64 (&w)[4]) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int i = t * kTile + j * 32 + lane;
+            w[j] = i < mine ? kept_weight(i, value(i)) : 0;
         }
-    cluster.sync();  // (nobody leaves while its memory is read)
+    };
+    __syncthreads();
+#pragma unroll 2
+    for (int t = warp; t < tiles; t += kWarpsN) {
+        u64 w[4];
+        tile_weights(t, w);
+        const u64 s = warp_sum(w[0] + w[1] + w[2] + w[3]);
+        if (lane == 0) sh.tile[t] = s;
+    }
+    __syncthreads();
+    const int per = (tiles + kThreads - 1) / kThreads, begin = min(tiles, (int)threadIdx.x * per), end = min(tiles, begin + per);
+    u64 part = 0, mine_all;
+    for (int t = begin; t < end; t++) part += sh.tile[t];
+    u64 run = block_prefix(part, sh.scratch, mine_all);
+    if (threadIdx.x == 0) sh.mass = mine_all, sh.bin = -1;
+    cluster.sync();
+    const u64 of_cta = lane < ctas ? of(lane < ctas ? lane : 0)->mass : 0, kept = warp_sum(of_cta);
+    run += warp_sum(lane < rank ? of_cta : 0);
+    const u64 want = target(kept);
+    cluster.sync();  // (all have read it: from here on each for itself)
+    for (int t = begin; t < end; t++) {
+        const u64 w = sh.tile[t];
+        if (run <= want && want < run + w) sh.bin = t, sh.before = run;
+        run += w;
+    }
+    __syncthreads();
+    if (warp == 0 && sh.bin >= 0) {
+        u64 w[4], from = sh.before;
+        tile_weights(sh.bin, w);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            u64 up_to = w[j];
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const u64 v = __shfl_up_sync(0xffffffffu, up_to, o);
+                if (lane >= o) up_to += v;
+            }
+            if (from + up_to - w[j] <= want && want < from + up_to) {
+                p.token[row] = at + sh.bin * kTile + j * 32 + lane;
+                if (p.prob) p.prob[row] = (float)((double)w[j] / (double)kept);
+            }
+            from += __shfl_sync(0xffffffffu, up_to, 31);
+        }
+    }
 }
 
-template <typename T>
+template <typename T, bool CACHED>
 bool launch(const SampleParams &p, int rows, int ctas) {
-    const size_t smem = sizeof(Shared) + (size_t)p.part * sizeof(float);
+    const size_t smem = sizeof(Shared) + (CACHED ? (size_t)p.part * sizeof(float) : 0);
     static size_t ready = 0;
     if (smem > ready) {
-        const cudaError_t e = cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        const cudaError_t e = cudaFuncSetAttribute(sample_kernel<T, CACHED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) {
             set_error(e, "sample shared memory");
             return false;
@@ -523,9 +629,13 @@ bool launch(const SampleParams &p, int rows, int ctas) {
     cfg.attrs = attr;
     cfg.numAttrs = g_pdl & PDL_PAGED ? 2 : 1;
     g_launches++;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, sample_kernel<T>, p);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, sample_kernel<T, CACHED>, p);
     if (e != cudaSuccess) set_error(e, "sample");
     return e == cudaSuccess;
+}
+template <typename T>
+bool launch(const SampleParams &p, int rows, int ctas, bool cached) {
+    return cached ? launch<T, true>(p, rows, ctas) : launch<T, false>(p, rows, ctas);
 }
 
 int refuse(const char *why) {
@@ -547,10 +657,17 @@ extern "C" int llamd_fwd_sample(const void *logits, int type, size_t stride, int
     if (!logits || !uniform || !token) return refuse("sample: a buffer is missing");
     const uintptr_t words = (uintptr_t)temperature | (uintptr_t)top_k | (uintptr_t)top_p | (uintptr_t)min_p | (uintptr_t)uniform | (uintptr_t)token | (uintptr_t)prob;
     if (words & 3 || (uintptr_t)logits & (type == LLAMD_PAGED_F32 ? 3 : 1)) return refuse("sample: a buffer starts inside an element");
-    // a CTA for every 8192 tokens, up to 8
+    int device = 0, sms = 0;
+    LLAMD_TRY(cudaGetDevice(&device), "sample: device");
+    LLAMD_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device), "sample: device");
+    // CTAs to a row: one for every 8192 tokens up to 8, fewer where that is more than two to an SM in all
     int ctas = 1;
-    while (ctas < kMostCtas && n_vocab > 8192 * ctas) ctas *= 2;
+    while (ctas < kMostCtas && (n_vocab > kMostPart * ctas || (n_vocab > 8192 * ctas && 2LL * rows * ctas <= 2LL * sms))) ctas *= 2;
     SampleParams p = {logits, stride, n_vocab, ((n_vocab + ctas - 1) / ctas + 7) / 8 * 8, temperature, top_p, min_p, uniform, top_k, token, prob};
-    const bool ok = type == LLAMD_PAGED_F32 ? launch<float>(p, rows, ctas) : type == LLAMD_PAGED_F16 ? launch<__half>(p, rows, ctas) : launch<__nv_bfloat16>(p, rows, ctas);
+    // kept in shared memory where every CTA has an SM to itself
+    const bool cached = (long long)rows * ctas <= sms && p.part <= 49152;
+    const bool ok = type == LLAMD_PAGED_F32   ? launch<float>(p, rows, ctas, cached)
+                    : type == LLAMD_PAGED_F16 ? launch<__half>(p, rows, ctas, cached)
+                                              : launch<__nv_bfloat16>(p, rows, ctas, cached);
     return ok && !error_code() ? 0 : -1;
 }

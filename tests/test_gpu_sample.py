@@ -138,6 +138,24 @@ def test_numbers_at_the_ends(sampling, u):
     assert np.array_equal(run(sampling, x, [u] * 3)[0], run(sampling, x, [0.0 if not u > 0 else min(u, 1 - 2.0 ** -24)] * 3)[0])
 
 
+def test_settings_beyond_their_ranges(sampling):
+    rng = np.random.default_rng(12)
+    x, u = logits(rng, 6, 5000), rng.random(6)
+    for got, as_if in ((dict(min_p=7.0), dict(min_p=1.0)), (dict(min_p=np.nan), dict()), (dict(top_p=np.nan), dict()), (dict(top_p=9.0), dict()), (dict(top_p=-2.0), dict(top_p=0.0)),
+                       (dict(temperature=np.nan), dict(temperature=0.0)), (dict(temperature=-3.0), dict(temperature=0.0)), (dict(top_k=-5), dict()), (dict(min_p=-1.0), dict())):
+        assert np.array_equal(run(sampling, x, u, **got)[0], run(sampling, x, u, **as_if)[0])
+
+
+@pytest.mark.parametrize("rows", [1, 2, 18, 19, 37, 75, 149, 300])
+@pytest.mark.parametrize("n", [3000, 40001])
+def test_rows(sampling, rows, n):
+    """Clusters of every size, rows kept in shared memory and read again."""
+    rng = np.random.default_rng(rows + n)
+    x = logits(rng, rows, n, spread=1.0)
+    for rule in (RULES[1], RULES[2], RULES[3], RULES[5], RULES[10]):
+        check(sampling, x, rng.random(rows), **rule)
+
+
 @pytest.mark.parametrize("temperature", [1e-45, 1e-30, 1e-4, 50.0, 1e30, np.inf])
 def test_temperatures(sampling, temperature):
     rng = np.random.default_rng(4)
