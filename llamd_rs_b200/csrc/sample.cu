@@ -4,18 +4,17 @@
 //   kept: the first k; of those the ones whose predecessors weigh less than p times the k's; of those the ones with w_i >= m
 //   token: by rising index the first at which the kept weights up to it are more than u times all of them
 //
-// Every weight is a whole multiple of 2^-40 (from an exponential in 64 bits, off by 2^-43), so that sums are exact and the same in whatever order they are made, and a
+// Every weight is a whole multiple of 2^-40 (from an exponential in 64 bits, off by 2^-37 of itself), so that sums are exact and the same in whatever order they are made, and a
 // token is another than in exact arithmetic only where u falls within some 2^-40 of a border.
 //
-// A row belongs to a cluster of 1 to 8 CTAs. The first look at it finds its top, and every thread's largest logit: what is at least the j-th largest of those is at least
-// j tokens, and little more. With j = k, or some hundreds where only a share of the weights is asked for, these few are gathered in a second look, in which the weights
-// of all are summed where a share of them is wanted, and one CTA sorts them and settles the row. Where they are too many, or their weights too little (a large k, a flat
-// row), a histogram of all logits (kBins over their range: tokens, and weights exactly, as three 14-bit digits) finds the bin in which the kept ones end; that bin is cut in
-// bins again, of (logit, index) compared as one number, until kList or fewer are in it, which are sorted. What is kept then, or where min-p is the only limit, is weighed tile by tile
-// of 128 neighbours, and the tile that u falls on looked through.
+// A row belongs to a cluster of 1 to 8 CTAs. The first look at it finds its top, and every thread's largest logit. With a small k: what is at least the k-th largest of those is
+// k tokens and little more; they are gathered in a second look, and one CTA sorts them and settles the row. Else, or where they are too many, a histogram of all logits (kBins
+// over their range: tokens, or weights, exactly) finds the bin in which the kept ones end; a CTA whose part has few tokens up to it keeps those in a list. The bin
+// is cut in bins again, of (logit, index) compared as one number, until kList or fewer are in it, which are sorted. What is kept then, or where min-p is the only limit, is
+// weighed tile by tile of 128 neighbours, and the tile that u falls on looked through.
 // Few rows are kept in shared memory, each looked at there; of many, parts are read again, from L2.
-// What it costs: the row's bytes; five joins of the cluster one behind the other, some ten in the long way; and for rows without a k an exponential in 64 bits for each
-// token, some 16 operations at 64 a clock and SM, once for the sum and once or twice for the rest.
+// What it costs: the row's bytes; four joins of the cluster one behind the other, some eight in the long way; and for rows without a k an exponential in 64 bits for each
+// token, some 20 operations at 64 a clock and SM, for the histogram and, where more than the lists' are kept, for the tiles.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -29,10 +28,10 @@ namespace {
 namespace cg = cooperative_groups;
 typedef unsigned long long u64;
 
-constexpr int kThreads = 512, kWarpsN = kThreads / 32, kBins = 1024, kList = 1024, kMostCtas = 8, kTile = 128;
+constexpr int kThreads = 256, kWarpsN = kThreads / 32, kBins = 1024, kList = 1024, kMostCtas = 8, kTile = 128;
 static_assert(kBins % 2 == 0, "bins are read two at a time");
-constexpr int kMostTokens = 393216, kMostPart = 262144;  // of a row; of a CTA (the digits' sums have 32 bits, the tiles' sums room)
-constexpr int kShare = 512;  // tokens that are gathered where a share of the weights is asked for
+constexpr int kMostTokens = 393216, kMostPart = 262144;  // of a row; of a CTA (the tiles' sums have room)
+constexpr int kFew = 2560;   // tokens of a CTA's part that may be in its list
 
 struct SampleParams {
     const void *x;
@@ -56,10 +55,10 @@ struct Shared {
     int part_count;
     // of the row (CTA 0)
     u64 total, before, cut;
-    int bin, n_range, n_list;
+    int bin, n_list;
     alignas(16) uint32_t hist[kBins];
     union {
-        alignas(16) uint32_t digit[3][kBins];  // of the bins' weights: bits 0 to 13, 14 to 27, 28 to 40 of each, summed
+        alignas(16) uint32_t digit[2][kBins];  // the bins' weights: the sums' low 32 bits, and what is above them
         struct {                   // (when the histogram has been read) some tokens' places, CTA 0's the whole row's in the end, and their weights
             u64 list[kList], weight[kList];
         };
@@ -73,7 +72,7 @@ __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162f
 
 // Falling logits, then rising indexes, as one rising number.
 __device__ __forceinline__ u64 order_of(float x, int i) {
-    const uint32_t b = __float_as_uint(x);
+    const uint32_t b = __float_as_uint(x + 0.0f);  // (-0 is 0)
     return (u64)(b & 0x80000000u ? b : ~b & 0x7FFFFFFFu) << 32 | (uint32_t)i;
 }
 __device__ __forceinline__ float logit_of(u64 order) {
@@ -81,19 +80,16 @@ __device__ __forceinline__ float logit_of(u64 order) {
     return __uint_as_float(b & 0x80000000u ? b : ~b & 0x7FFFFFFFu);
 }
 
-// 2^y for y <= 0 in units of 2^-40, rounded, and as it is: y = n + f, |f| <= 1/2, the exponential's series up to f^11 (the next term is below 2^-47)
+// 2^y for y <= 0 in units of 2^-40, rounded, and as it is: y = n + f, |f| <= 1/2, the exponential's series up to f^9 (the next term is below 2^-37)
 struct Weigher {
     double max, per;  // log2 e / T
-    float top;
+    float top, per32;
     __device__ __forceinline__ double exact(float x) const {
-        if (x == top) return 1.0;  // (an infinite one too)
-        if (x == -INFINITY) return 0.0;
-        const double y = fmax(((double)x - max) * per, -1000.0), magic = 6755399441055744.0;  // 1.5 * 2^52
+        const bool far = !((x - top) * per32 >= -100.0f);  // (also where x or T is infinite: weight 0)
+        const double y = far ? 0.0 : ((double)x - max) * per, magic = 6755399441055744.0;  // 1.5 * 2^52
         const double t = y + magic, f = y - (t - magic);
         const int n = (int)(uint32_t)__double2loint(t);
-        double p = 4.44553827187081162e-10;  // ln 2^k / k! for k = 11 to 0
-        p = fma(p, f, 7.05491162080112336e-09);
-        p = fma(p, f, 1.01780860092396999e-07);
+        double p = 1.01780860092396999e-07;  // ln 2^k / k! for k = 9 to 0
         p = fma(p, f, 1.32154867901443095e-06);
         p = fma(p, f, 1.52527338040598411e-05);
         p = fma(p, f, 1.54035303933816088e-04);
@@ -103,7 +99,8 @@ struct Weigher {
         p = fma(p, f, 2.40226506959100722e-01);
         p = fma(p, f, 6.93147180559945286e-01);
         p = fma(p, f, 1.0);
-        return __hiloint2double(__double2hiint(p) + (n << 20), __double2loint(p));
+        const double w = __hiloint2double(__double2hiint(p) + (n << 20), __double2loint(p));
+        return x == top ? 1.0 : far ? 0.0 : w;  // (also where both are infinite)
     }
     static __device__ __forceinline__ u64 units(double w) {
         return (u64)__double_as_longlong(fma(w, 1099511627776.0, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;  // (+ 2^52: the whole number is the low bits)
@@ -169,35 +166,68 @@ __device__ __forceinline__ void sort_list(u64 *list, int size) {
 
 // CACHED: the CTA's part is kept in shared memory.
 template <typename T, bool CACHED>
-__global__ void __launch_bounds__(kThreads, CACHED ? 1 : 2) sample_kernel(const SampleParams p) {
+__global__ void __launch_bounds__(kThreads, CACHED ? 1 : 4) sample_kernel(const SampleParams p) {
     extern __shared__ __align__(16) uint8_t raw[];
     Shared &sh = *reinterpret_cast<Shared *>(raw);
-    float *const x = reinterpret_cast<float *>(raw + sizeof(Shared));
+    u64 *const few_places = reinterpret_cast<u64 *>(raw + sizeof(Shared));
+    float *const x = reinterpret_cast<float *>(raw + sizeof(Shared) + kFew * sizeof(u64));
     cg::cluster_group cluster = cg::this_cluster();
     const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), row = (int)(blockIdx.x / ctas);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, at = rank * p.part, mine = max(0, min(p.part, p.n - at));
     Shared &lead = *cluster.map_shared_rank(&sh, 0);
     auto of = [&](int r) { return cluster.map_shared_rank(&sh, r); };
     const T *const src = reinterpret_cast<const T *>(p.x) + (size_t)row * p.stride + at;
-    auto clean = [](float v) { return v == v ? v + 0.0f : -INFINITY; };  // (NaN is no token; -0 is 0)
+    auto clean = [](float v) { return fmaxf(v, -INFINITY); };  // (NaN is no token)
     constexpr int kWide = 16 / sizeof(T);
     const int wide = ((uintptr_t)src & 15) == 0 ? mine / kWide : 0;
     // f(i, logit) for the part's tokens, of one thread in rising order
+    // (loads first, kBatch of them at a time: what f does keeps the compiler from moving them)
+    constexpr int kBatch = sizeof(T) == 4 ? 4 : 2;
     auto from_memory = [&](auto f) {
-#pragma unroll 4
-        for (int i = threadIdx.x; i < wide; i += kThreads) {
-            const uint4 v = reinterpret_cast<const uint4 *>(src)[i];
+        const uint4 *const from = reinterpret_cast<const uint4 *>(src);
+        int i = threadIdx.x;
+        for (; i + (kBatch - 1) * kThreads < wide; i += kBatch * kThreads) {
+            uint4 v[kBatch];
+#pragma unroll
+            for (int b = 0; b < kBatch; b++) v[b] = from[i + b * kThreads];
+#pragma unroll
+            for (int b = 0; b < kBatch; b++) {
+                const T *e = reinterpret_cast<const T *>(&v[b]);
+#pragma unroll
+                for (int j = 0; j < kWide; j++) f((i + b * kThreads) * kWide + j, clean(to_float(e[j])));
+            }
+        }
+        for (; i < wide; i += kThreads) {
+            const uint4 v = from[i];
             const T *e = reinterpret_cast<const T *>(&v);
 #pragma unroll
             for (int j = 0; j < kWide; j++) f(i * kWide + j, clean(to_float(e[j])));
         }
-#pragma unroll 4
-        for (int i = wide * kWide + threadIdx.x; i < mine; i += kThreads) f(i, clean(to_float(src[i])));
+        i = wide * kWide + threadIdx.x;
+        for (; i + 7 * kThreads < mine; i += 8 * kThreads) {  // (rows that do not start at 16 bytes)
+            T v[8];
+#pragma unroll
+            for (int b = 0; b < 8; b++) v[b] = src[i + b * kThreads];
+#pragma unroll
+            for (int b = 0; b < 8; b++) f(i + b * kThreads, clean(to_float(v[b])));
+        }
+        for (; i < mine; i += kThreads) f(i, clean(to_float(src[i])));
     };
+    // Once a CTA's part has few tokens that still matter, they are in a list of their own, and each() goes through that.
+    int n_few = -1;
     auto each = [&](auto f) {
-        if constexpr (CACHED) {
-#pragma unroll 4
-            for (int i = threadIdx.x; i < mine; i += kThreads) f(i, x[i]);
+        if (n_few >= 0) {
+            for (int i = threadIdx.x; i < n_few; i += kThreads) f((int)(uint32_t)few_places[i] - at, logit_of(few_places[i]));
+        } else if constexpr (CACHED) {
+            int i = threadIdx.x;
+            for (; i + 3 * kThreads < mine; i += 4 * kThreads) {
+                float v[4];
+#pragma unroll
+                for (int b = 0; b < 4; b++) v[b] = x[i + b * kThreads];
+#pragma unroll
+                for (int b = 0; b < 4; b++) f(i + b * kThreads, v[b]);
+            }
+            for (; i < mine; i += kThreads) f(i, x[i]);
         } else {
             from_memory(f);
         }
@@ -255,7 +285,8 @@ __global__ void __launch_bounds__(kThreads, CACHED ? 1 : 2) sample_kernel(const 
         cluster.sync();  // (nobody leaves while its memory is read)
         return;
     }
-    const Weigher weigh = {(double)top, 1.4426950408889634 / (double)temperature, top};
+    const double per_logit = 1.4426950408889634 / (double)temperature;
+    const Weigher weigh = {(double)top, per_logit, top, (float)fmin(per_logit, 1e38)};
 
     // the whole part of u times `total`, exactly
     auto target = [&](u64 total) -> u64 {
@@ -267,8 +298,11 @@ __global__ void __launch_bounds__(kThreads, CACHED ? 1 : 2) sample_kernel(const 
 
     u64 cut = ~0ull;  // the last kept token's place in order
     if (k || by_mass) {
-        const float range = top - least, per_bin = range > 0.0f && range < INFINITY ? (kBins - 1) / range : 0.0f;
-        auto bin_of = [&](float v) { return per_bin > 0.0f ? min(kBins - 1, (int)((top - v) * per_bin)) : 0; };  // (rises with falling v)
+        // bins by distance from the top (0 where that has no end: all in one bin), numbers that rise with falling logits; and whether a logit's is at most `bin`
+        const float range = top - least, per_bin = range > 0.0f && range < INFINITY ? fminf((kBins - 1) / range, 1e30f) : 0.0f;
+        auto distance = [&](float v) { return per_bin > 0.0f ? (top - v) * per_bin : 0.0f; };
+        auto bin_of = [&](float v) { return min(kBins - 1, (int)distance(v)); };
+        auto up_to_bin = [&](float v, int bin) { return v > -INFINITY && (bin == kBins - 1 || distance(v) < (float)(bin + 1)); };
         // In doubt are tokens of places [low, high], `count` of them; in front of them are `ahead` tokens or weights that are kept for certain. First the k's end is
         // looked for, where there is a k, then that of a share of the weights, all or the k's.
         bool counting = k > 0;
@@ -276,49 +310,61 @@ __global__ void __launch_bounds__(kThreads, CACHED ? 1 : 2) sample_kernel(const 
         int count = 0;
         auto clear = [&]() {
             __syncthreads();
-            for (int i = threadIdx.x; i < kBins; i += kThreads) sh.hist[i] = sh.digit[0][i] = sh.digit[1][i] = sh.digit[2][i] = 0;
+            for (int i = threadIdx.x; i < kBins; i += kThreads) sh.hist[i] = sh.digit[0][i] = sh.digit[1][i] = 0;
             __syncthreads();
         };
-        auto enter = [&](int bin, float v) {
-            atomicAdd(&sh.hist[bin], 1u);
-            if (counting) return;
-            const u64 w = weigh(v);
-            const uint32_t d0 = w & 0x3FFF, d1 = w >> 14 & 0x3FFF, d2 = (uint32_t)(w >> 28);
-            if (d0) atomicAdd(&sh.digit[0][bin], d0);
-            if (d1) atomicAdd(&sh.digit[1][bin], d1);
-            if (d2) atomicAdd(&sh.digit[2][bin], d2);
+        // (two loops: in one, an exponential would be made for each token and thrown away where only tokens are counted)
+        auto fill = [&](auto bin) {  // bin(i, v): below 0 for those that are not to be in any
+            if (counting) {
+                each([&](int i, float v) {
+                    const int b = bin(i, v);
+                    if (b >= 0) atomicAdd(&sh.hist[b], 1u);
+                });
+            } else {
+                each([&](int i, float v) {
+                    const int b = bin(i, v);
+                    if (b < 0) return;
+                    const u64 w = weigh(v);
+                    // (64 bits in two: what the low ones carry goes with the high ones, which few weights have)
+                    const uint32_t lo = (uint32_t)w, was = atomicAdd(&sh.digit[0][b], lo), up = (uint32_t)(w >> 32) + (was > ~lo);
+                    if (up) atomicAdd(&sh.digit[1][b], up);
+                });
+            }
         };
         // CTA 0: the first bin up to which there are `wanted` tokens, or a share of `whole` (of all that is in the bins, where that is 0)
         auto find = [&](u64 wanted) {
             cluster.sync();
             if (rank == 0) {
                 constexpr int kPer = kBins / kThreads;
-                static_assert(kPer == 2, "pairs of bins");
-                uint2 c = {0, 0};
-                u64 w[kPer] = {}, n_all, w_all = 0, n, m;
+                static_assert(kPer == 4, "four bins to a thread");
+                uint32_t c[kPer] = {};
+                u64 w[kPer] = {}, n_all, w_all = 0, n, m = 0;
+                auto add = [&](const uint32_t *bins, int shift) {  // (all CTAs' at once)
+                    uint4 h[kMostCtas];
 #pragma unroll
-                for (int r = 0; r < kMostCtas; r++) {
-                    if (r >= ctas) break;
-                    const Shared &o = *of(r);
-                    const uint2 h = reinterpret_cast<const uint2 *>(o.hist)[threadIdx.x];
-                    c.x += h.x, c.y += h.y;
-                    if (!wanted) {
-                        const uint2 d0 = reinterpret_cast<const uint2 *>(o.digit[0])[threadIdx.x], d1 = reinterpret_cast<const uint2 *>(o.digit[1])[threadIdx.x],
-                                    d2 = reinterpret_cast<const uint2 *>(o.digit[2])[threadIdx.x];
-                        w[0] += d0.x + ((u64)d1.x << 14) + ((u64)d2.x << 28), w[1] += d0.y + ((u64)d1.y << 14) + ((u64)d2.y << 28);
+                    for (int r = 0; r < kMostCtas; r++) h[r] = r < ctas ? reinterpret_cast<const uint4 *>(cluster.map_shared_rank(bins, r < ctas ? r : 0))[threadIdx.x] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                    for (int r = 0; r < kMostCtas; r++) {
+                        if (shift < 0) c[0] += h[r].x, c[1] += h[r].y, c[2] += h[r].z, c[3] += h[r].w;
+                        else w[0] += (u64)h[r].x << shift, w[1] += (u64)h[r].y << shift, w[2] += (u64)h[r].z << shift, w[3] += (u64)h[r].w << shift;
                     }
+                };
+                if (wanted) {
+                    add(sh.hist, -1);
+                } else {
+                    add(sh.digit[0], 0);
+                    add(sh.digit[1], 32);
                 }
-                n = block_prefix((u64)c.x + c.y, sh.scratch, n_all);
-                m = block_prefix(w[0] + w[1], sh.scratch, w_all);
+                n = block_prefix((u64)c[0] + c[1] + c[2] + c[3], sh.scratch, n_all);
+                if (!wanted) m = block_prefix(w[0] + w[1] + w[2] + w[3], sh.scratch, w_all);
                 if (threadIdx.x == 0 && !whole) sh.total = w_all;
                 const double want = (double)p_in * (double)(whole ? whole : w_all);
 #pragma unroll
                 for (int j = 0; j < kPer; j++) {
-                    const uint32_t cj = j ? c.y : c.x;
-                    const bool here = wanted ? ahead + n < wanted && ahead + n + cj >= wanted
-                                             : cj && ((double)(ahead + m) < want || (!ahead && !m)) && (double)(ahead + m + w[j]) >= want;
+                    const bool here = wanted ? ahead + n < wanted && ahead + n + c[j] >= wanted
+                                             : w[j] && ((double)(ahead + m) < want || (!ahead && !m)) && (double)(ahead + m + w[j]) >= want;
                     if (here) sh.bin = threadIdx.x * kPer + j, sh.before = ahead + (wanted ? n : m);
-                    n += cj, m += w[j];
+                    n += c[j], m += w[j];
                 }
             }
             cluster.sync();
@@ -352,14 +398,12 @@ __global__ void __launch_bounds__(kThreads, CACHED ? 1 : 2) sample_kernel(const 
             const int n = lane < ctas ? of(lane < ctas ? lane : 0)->n_list : 0;
             return __reduce_add_sync(0xffffffffu, n);
         };
-        auto pull = [&]() {  // (CTA 0)
-            int to = sh.n_list;
-            for (int r = 1; r < ctas; r++) {
-                const Shared &o = *of(r);
-                const int n = o.n_list;
-                for (int i = threadIdx.x; i < n; i += kThreads) sh.list[to + i] = o.list[i];
-                to += n;
-            }
+        auto pull = [&]() {  // (CTA 0: a warp to a CTA; together they have room)
+            static_assert(kWarpsN >= kMostCtas, "a warp to a CTA");
+            const int n = lane < ctas ? of(lane < ctas ? lane : 0)->n_list : 0, theirs = __shfl_sync(0xffffffffu, n, warp);
+            const int to = __reduce_add_sync(0xffffffffu, lane < warp ? n : 0);
+            if (warp > 0 && warp < ctas)
+                for (int i = lane; i < theirs; i += 32) sh.list[to + i] = of(warp)->list[i];
             __syncthreads();
         };
         auto padded = [&](int n) {  // the list's n to a power of two
@@ -369,54 +413,28 @@ __global__ void __launch_bounds__(kThreads, CACHED ? 1 : 2) sample_kernel(const 
             return size;
         };
 
-        // ---- the second look: the few that may be kept ----
-        const int groups = ctas * kThreads, wanted = k ? k : min(min(kShare, groups / 2), live);
-        bool few = wanted < groups * 3 / 4 && wanted <= kList * 3 / 4;
+        // ---- the second look: the few that may be kept of a small k ----
+        bool few = k && k < ctas * kThreads * 3 / 4 && k <= kList * 3 / 4;
         if (few) {
             if (best > -INFINITY) atomicAdd(&sh.hist[bin_of(best)], 1u);
-            // (fewer threads than `wanted` may have a token: all of them, then)
+            // (fewer than k threads may have a token: all of them, then)
             if (rank == 0 && threadIdx.x == 0) sh.bin = kBins - 1;
-            find((u64)wanted);
+            find((u64)k);
             const int bin = lead.bin;
-            sum = 0;
-            const bool all_mass = !k;
             each([&](int i, float v) {
-                if (v == -INFINITY) return;
-                if (bin_of(v) <= bin) append(order_of(v, at + i));
-                if (all_mass) sum += weigh(v);
+                if (up_to_bin(v, bin)) append(order_of(v, at + i));
             });
-            sum = warp_sum(sum);
-            if (lane == 0) sh.scratch[warp] = sum;
-            __syncthreads();
-            if (warp == 0) {
-                sum = warp_sum(lane < kWarpsN ? sh.scratch[lane] : 0);
-                if (lane == 0) sh.mass = sum;
-            }
             cluster.sync();
             const int n = in_all_lists();
             few = n <= kList;
-            if (all_mass && few) {  // do they have the share?
-                whole = warp_sum(lane < ctas ? of(lane < ctas ? lane : 0)->mass : 0);
-                u64 part = 0, all;
-                if (rank == 0) {
-                    pull();
-                    for (int i = threadIdx.x; i < n; i += kThreads) part += weigh(logit_of(sh.list[i]));
-                    block_prefix(part, sh.scratch, all);
-                    if (threadIdx.x == 0) sh.part_count = n == live || (double)all >= (double)p_in * (double)whole;
-                }
-                cluster.sync();
-                few = lead.part_count;
-                cluster.sync();
-            } else if (few) {
-                if (rank == 0) pull();
-                cluster.sync();  // (the other CTAs are done)
-            }
+            if (few && rank == 0) pull();
+            cluster.sync();  // (the other CTAs are done)
             if (few && rank != 0) return;
             if (few) {
                 const int size = padded(n);
                 sort_list(sh.list, size);
                 // each thread has `per` neighbours
-                const int per = (size + kThreads - 1) / kThreads, begin = min(n, (int)threadIdx.x * per), end = min(n, begin + per), kept_k = k ? min(k, n) : n;
+                const int per = (size + kThreads - 1) / kThreads, begin = min(n, (int)threadIdx.x * per), end = min(n, begin + per), kept_k = min(k, n);
                 u64 part = 0, all;
                 for (int i = begin; i < end; i++) {
                     const u64 w = i < kept_k ? weigh(logit_of(sh.list[i])) : 0;
@@ -424,7 +442,7 @@ __global__ void __launch_bounds__(kThreads, CACHED ? 1 : 2) sample_kernel(const 
                     part += w;
                 }
                 u64 before = block_prefix(part, sh.scratch, all);
-                const double limit = (double)p_in * (double)(k ? all : whole);
+                const double limit = (double)p_in * (double)all;
                 part = 0;
                 for (int i = begin; i < end; i++) {
                     const u64 w = sh.weight[i];
@@ -456,35 +474,41 @@ __global__ void __launch_bounds__(kThreads, CACHED ? 1 : 2) sample_kernel(const 
                 }
                 return;
             }
-            whole = 0;
         }
 
         // ---- many: where they end ----
         clear();
-        each([&](int, float v) {
-            if (v > -INFINITY) enter(bin_of(v), v);
-        });
+        fill([&](int, float v) { return v > -INFINITY ? bin_of(v) : -1; });
         find((u64)k);
         const int bin = lead.bin;
         if (!k) whole = lead.total;
         ahead = lead.before;
         low = ~0ull, high = 0, sum = 0;
+        if (threadIdx.x == 0) sh.n_list = 0;
+        __syncthreads();
         each([&](int i, float v) {
-            if (!(v > -INFINITY) || bin_of(v) != bin) return;
+            if (!up_to_bin(v, bin)) return;
             const u64 o = order_of(v, at + i);
+            if (*(volatile int *)&sh.n_list <= kFew) {
+                const int to = atomicAdd(&sh.n_list, 1);
+                if (to < kFew) few_places[to] = o;
+            }
+            if (bin_of(v) != bin) return;
             low = o < low ? o : low, high = o > high ? o : high;
             count++;
         });
         joined();
+        if (sh.n_list <= kFew) n_few = sh.n_list;  // (what is not in it is not kept)
+        __syncthreads();
         for (;;) {
             // (every round leaves one bin of 1024, and places are numbers of 64 bits that all differ: at most seven)
             while (count > kList) {
                 int shift = 0;
                 while ((high - low) >> shift >= (u64)kBins) shift++;
                 clear();
-                each([&](int i, float v) {
+                fill([&](int i, float v) {
                     const u64 o = order_of(v, at + i);
-                    if (v > -INFINITY && o >= low && o <= high) enter((int)((o - low) >> shift), v);
+                    return v > -INFINITY && o >= low && o <= high ? (int)((o - low) >> shift) : -1;
                 });
                 find(counting ? (u64)k : 0);
                 ahead = lead.before;
@@ -553,19 +577,28 @@ __global__ void __launch_bounds__(kThreads, CACHED ? 1 : 2) sample_kernel(const 
     };
     const int tiles = (mine + kTile - 1) / kTile;
     auto tile_weights = [&](int t, u64 (&w)[4]) {
+        float v[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int i = t * kTile + j * 32 + lane;
-            w[j] = i < mine ? kept_weight(i, value(i)) : 0;
-        }
+        for (int j = 0; j < 4; j++) v[j] = t * kTile + j * 32 + lane < mine ? value(t * kTile + j * 32 + lane) : -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 4; j++) w[j] = kept_weight(t * kTile + j * 32 + lane, v[j]);
     };
     __syncthreads();
+    if (n_few >= 0) {
+        for (int t = threadIdx.x; t < tiles; t += kThreads) sh.tile[t] = 0;
+        __syncthreads();
+        each([&](int i, float v) {
+            const u64 w = kept_weight(i, v);
+            if (w) atomicAdd(&sh.tile[i / kTile], w);  // (whole numbers: the same sums in any order)
+        });
+    } else {
 #pragma unroll 2
-    for (int t = warp; t < tiles; t += kWarpsN) {
-        u64 w[4];
-        tile_weights(t, w);
-        const u64 s = warp_sum(w[0] + w[1] + w[2] + w[3]);
-        if (lane == 0) sh.tile[t] = s;
+        for (int t = warp; t < tiles; t += kWarpsN) {
+            u64 w[4];
+            tile_weights(t, w);
+            const u64 s = warp_sum(w[0] + w[1] + w[2] + w[3]);
+            if (lane == 0) sh.tile[t] = s;
+        }
     }
     __syncthreads();
     const int per = (tiles + kThreads - 1) / kThreads, begin = min(tiles, (int)threadIdx.x * per), end = min(tiles, begin + per);
@@ -606,7 +639,7 @@ __global__ void __launch_bounds__(kThreads, CACHED ? 1 : 2) sample_kernel(const 
 
 template <typename T, bool CACHED>
 bool launch(const SampleParams &p, int rows, int ctas) {
-    const size_t smem = sizeof(Shared) + (CACHED ? (size_t)p.part * sizeof(float) : 0);
+    const size_t smem = sizeof(Shared) + kFew * sizeof(u64) + (CACHED ? (size_t)p.part * sizeof(float) : 0);
     static size_t ready = 0;
     if (smem > ready) {
         const cudaError_t e = cudaFuncSetAttribute(sample_kernel<T, CACHED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
@@ -660,12 +693,12 @@ extern "C" int llamd_fwd_sample(const void *logits, int type, size_t stride, int
     int device = 0, sms = 0;
     LLAMD_TRY(cudaGetDevice(&device), "sample: device");
     LLAMD_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device), "sample: device");
-    // CTAs to a row: one for every 8192 tokens up to 8, fewer where that is more than two to an SM in all
+    // CTAs to a row: one for every 8192 tokens up to 8, fewer where that is more than seven to an SM in all
     int ctas = 1;
-    while (ctas < kMostCtas && (n_vocab > kMostPart * ctas || (n_vocab > 8192 * ctas && 2LL * rows * ctas <= 2LL * sms))) ctas *= 2;
+    while (ctas < kMostCtas && (n_vocab > kMostPart * ctas || (n_vocab > 8192 * ctas && 2LL * rows * ctas <= 7LL * sms))) ctas *= 2;
     SampleParams p = {logits, stride, n_vocab, ((n_vocab + ctas - 1) / ctas + 7) / 8 * 8, temperature, top_p, min_p, uniform, top_k, token, prob};
     // kept in shared memory where every CTA has an SM to itself
-    const bool cached = (long long)rows * ctas <= sms && p.part <= 49152;
+    const bool cached = (long long)rows * ctas <= sms && p.part <= 40960;
     const bool ok = type == LLAMD_PAGED_F32   ? launch<float>(p, rows, ctas, cached)
                     : type == LLAMD_PAGED_F16 ? launch<__half>(p, rows, ctas, cached)
                                               : launch<__nv_bfloat16>(p, rows, ctas, cached);
