@@ -28,7 +28,9 @@ namespace {
 namespace cg = cooperative_groups;
 typedef unsigned long long u64;
 
-constexpr int kThreads = 256, kWarpsN = kThreads / 32, kBins = 1024, kList = 1024, kMostCtas = 8, kTile = 128;
+// threads of a CTA: of one of four to an SM, and of one that has its SM to itself (and its part of the row in shared memory)
+constexpr int kManyThreads = 256, kOneThreads = 1024, kMostWarps = kOneThreads / 32;
+constexpr int kBins = 1024, kList = 1024, kRanked = 256, kMostCtas = 8, kTile = 128;  // kRanked: lists that are put in order by counting, not sorted
 static_assert(kBins % 2 == 0, "bins are read two at a time");
 constexpr int kMostTokens = 393216, kMostPart = 262144;  // of a row; of a CTA (the tiles' sums have room)
 constexpr int kFew = 2560;   // tokens of a CTA's part that may be in its list
@@ -45,17 +47,17 @@ struct SampleParams {
 
 // What the cluster's CTAs tell one another; what is the row's own is read from CTA 0.
 struct Shared {
-    u64 scratch[kWarpsN];
-    u64 low[kWarpsN], high[kWarpsN];
-    int count[kWarpsN];
-    float least[kWarpsN];
+    u64 scratch[kMostWarps];
+    u64 low[kMostWarps], high[kMostWarps];
+    int count[kMostWarps];
+    float least[kMostWarps];
     // of this CTA
     u64 first, mass, part_low, part_high;
     float part_least;
     int part_count;
     // of the row (CTA 0)
     u64 total, before, cut;
-    int bin, n_list;
+    int bin, n_list, n_few;
     alignas(16) uint32_t hist[kBins];
     union {
         alignas(16) uint32_t digit[2][kBins];  // the bins' weights: the sums' low 32 bits, and what is above them
@@ -130,6 +132,7 @@ __device__ __forceinline__ u64 warp_most(u64 v) {
     return v;
 }
 // The sum of all threads' values up to this one's, exclusive; `total` gets all of them. One value a thread; the scratch may be used again at once.
+template <int N>
 __device__ __forceinline__ u64 block_prefix(u64 v, u64 *scratch, u64 &total) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     u64 in = v;
@@ -141,21 +144,17 @@ __device__ __forceinline__ u64 block_prefix(u64 v, u64 *scratch, u64 &total) {
     __syncthreads();
     if (lane == 31) scratch[warp] = in;
     __syncthreads();
-    u64 before = 0;
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < kWarpsN; w++) {
-        before += w < warp ? scratch[w] : 0;
-        total += scratch[w];
-    }
-    return before + in - v;
+    const u64 of_warp = lane < N / 32 ? scratch[lane] : 0;
+    total = warp_sum(of_warp);
+    return warp_sum(lane < warp ? of_warp : 0) + in - v;
 }
 // list[0 .. size) in rising order; size a power of two.
+template <int N>
 __device__ __forceinline__ void sort_list(u64 *list, int size) {
     for (int k = 2; k <= size; k <<= 1)
         for (int j = k >> 1; j > 0; j >>= 1) {
             __syncthreads();
-            for (int i = threadIdx.x; i < size / 2; i += kThreads) {
+            for (int i = threadIdx.x; i < size / 2; i += N) {
                 const int a = 2 * i - (i & (j - 1)), b = a + j;
                 const u64 x = list[a], y = list[b];
                 if ((x > y) == ((a & k) == 0)) list[a] = y, list[b] = x;
@@ -166,7 +165,8 @@ __device__ __forceinline__ void sort_list(u64 *list, int size) {
 
 // CACHED: the CTA's part is kept in shared memory.
 template <typename T, bool CACHED>
-__global__ void __launch_bounds__(kThreads, CACHED ? 1 : 4) sample_kernel(const SampleParams p) {
+__global__ void __launch_bounds__(CACHED ? kOneThreads : kManyThreads, CACHED ? 1 : 4) sample_kernel(const SampleParams p) {
+    constexpr int kThreads = CACHED ? kOneThreads : kManyThreads, kWarpsN = kThreads / 32;
     extern __shared__ __align__(16) uint8_t raw[];
     Shared &sh = *reinterpret_cast<Shared *>(raw);
     u64 *const few_places = reinterpret_cast<u64 *>(raw + sizeof(Shared));
@@ -303,11 +303,10 @@ __global__ void __launch_bounds__(kThreads, CACHED ? 1 : 4) sample_kernel(const 
         auto distance = [&](float v) { return per_bin > 0.0f ? (top - v) * per_bin : 0.0f; };
         auto bin_of = [&](float v) { return min(kBins - 1, (int)distance(v)); };
         auto up_to_bin = [&](float v, int bin) { return v > -INFINITY && (bin == kBins - 1 || distance(v) < (float)(bin + 1)); };
-        // In doubt are tokens of places [low, high], `count` of them; in front of them are `ahead` tokens or weights that are kept for certain. First the k's end is
+        // In doubt are tokens of places [low, high]; in front of them are `ahead` tokens or weights that are kept for certain. First the k's end is
         // looked for, where there is a k, then that of a share of the weights, all or the k's.
         bool counting = k > 0;
-        u64 low = 0, high = ~0ull, ahead = 0, sum = 0, whole = 0;
-        int count = 0;
+        u64 low = 0, high = ~0ull, ahead = 0, whole = 0;
         auto clear = [&]() {
             __syncthreads();
             for (int i = threadIdx.x; i < kBins; i += kThreads) sh.hist[i] = sh.digit[0][i] = sh.digit[1][i] = 0;
@@ -335,14 +334,14 @@ __global__ void __launch_bounds__(kThreads, CACHED ? 1 : 4) sample_kernel(const 
         auto find = [&](u64 wanted) {
             cluster.sync();
             if (rank == 0) {
-                constexpr int kPer = kBins / kThreads;
-                static_assert(kPer == 4, "four bins to a thread");
+                constexpr int kPer = 4;  // bins to a thread of the first
+                const bool has = threadIdx.x < kBins / kPer;
                 uint32_t c[kPer] = {};
                 u64 w[kPer] = {}, n_all, w_all = 0, n, m = 0;
                 auto add = [&](const uint32_t *bins, int shift) {  // (all CTAs' at once)
                     uint4 h[kMostCtas];
 #pragma unroll
-                    for (int r = 0; r < kMostCtas; r++) h[r] = r < ctas ? reinterpret_cast<const uint4 *>(cluster.map_shared_rank(bins, r < ctas ? r : 0))[threadIdx.x] : make_uint4(0, 0, 0, 0);
+                    for (int r = 0; r < kMostCtas; r++) h[r] = has && r < ctas ? reinterpret_cast<const uint4 *>(cluster.map_shared_rank(bins, r < ctas ? r : 0))[threadIdx.x] : make_uint4(0, 0, 0, 0);
 #pragma unroll
                     for (int r = 0; r < kMostCtas; r++) {
                         if (shift < 0) c[0] += h[r].x, c[1] += h[r].y, c[2] += h[r].z, c[3] += h[r].w;
@@ -355,8 +354,8 @@ __global__ void __launch_bounds__(kThreads, CACHED ? 1 : 4) sample_kernel(const 
                     add(sh.digit[0], 0);
                     add(sh.digit[1], 32);
                 }
-                n = block_prefix((u64)c[0] + c[1] + c[2] + c[3], sh.scratch, n_all);
-                if (!wanted) m = block_prefix(w[0] + w[1] + w[2] + w[3], sh.scratch, w_all);
+                n = block_prefix<kThreads>((u64)c[0] + c[1] + c[2] + c[3], sh.scratch, n_all);
+                if (!wanted) m = block_prefix<kThreads>(w[0] + w[1] + w[2] + w[3], sh.scratch, w_all);
                 if (threadIdx.x == 0 && !whole) sh.total = w_all;
                 const double want = (double)p_in * (double)(whole ? whole : w_all);
 #pragma unroll
@@ -369,28 +368,25 @@ __global__ void __launch_bounds__(kThreads, CACHED ? 1 : 4) sample_kernel(const 
             }
             cluster.sync();
         };
-        // the CTAs' own low, high, sum and count as the row's
+        // the CTAs' own low and high as the row's
         auto joined = [&]() {
-            low = warp_least(low), high = warp_most(high), sum = warp_sum(sum);
-            const int c = __reduce_add_sync(0xffffffffu, count);
+            low = warp_least(low), high = warp_most(high);
             __syncthreads();
-            if (lane == 0) sh.low[warp] = low, sh.high[warp] = high, sh.scratch[warp] = sum, sh.count[warp] = c;
+            if (lane == 0) sh.low[warp] = low, sh.high[warp] = high;
             __syncthreads();
             if (warp == 0) {
-                const bool in = lane < kWarpsN;
-                const u64 l = warp_least(in ? sh.low[lane] : ~0ull), h = warp_most(in ? sh.high[lane] : 0), s = warp_sum(in ? sh.scratch[lane] : 0);
-                const int n = __reduce_add_sync(0xffffffffu, in ? sh.count[lane] : 0);
-                if (lane == 0) sh.part_low = l, sh.part_high = h, sh.mass = s, sh.part_count = n;
+                const u64 l = warp_least(lane < kWarpsN ? sh.low[lane] : ~0ull), h = warp_most(lane < kWarpsN ? sh.high[lane] : 0);
+                if (lane == 0) sh.part_low = l, sh.part_high = h;
             }
             cluster.sync();
-            const bool in = lane < ctas;
-            const Shared &o = *of(in ? lane : 0);
-            low = warp_least(o.part_low), high = warp_most(o.part_high), sum = warp_sum(in ? o.mass : 0);
-            count = __reduce_add_sync(0xffffffffu, in ? o.part_count : 0);
+            const Shared &o = *of(lane < ctas ? lane : 0);
+            low = warp_least(o.part_low), high = warp_most(o.part_high);
             cluster.sync();  // (all have read it)
         };
-        // Into this CTA's own list, in any order; all lists then into CTA 0's, where they are no more than kList in all. Between the two the cluster is joined.
+        // Into this CTA's own list, in any order (up to kList, counted beyond); all lists then into CTA 0's, where they are no more than kList in all. Between the
+        // two the cluster is joined.
         auto append = [&](u64 o) {
+            if (*(volatile int *)&sh.n_list > kList) return;
             const int to = atomicAdd(&sh.n_list, 1);
             if (to < kList) sh.list[to] = o;
         };
@@ -400,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, CACHED ? 1 : 4) sample_kernel(const 
         };
         auto pull = [&]() {  // (CTA 0: a warp to a CTA; together they have room)
             static_assert(kWarpsN >= kMostCtas, "a warp to a CTA");
-            const int n = lane < ctas ? of(lane < ctas ? lane : 0)->n_list : 0, theirs = __shfl_sync(0xffffffffu, n, warp);
+            const int n = lane < ctas ? of(lane < ctas ? lane : 0)->n_list : 0, theirs = __shfl_sync(0xffffffffu, n, min(warp, ctas - 1));
             const int to = __reduce_add_sync(0xffffffffu, lane < warp ? n : 0);
             if (warp > 0 && warp < ctas)
                 for (int i = lane; i < theirs; i += 32) sh.list[to + i] = of(warp)->list[i];
@@ -411,6 +407,17 @@ __global__ void __launch_bounds__(kThreads, CACHED ? 1 : 4) sample_kernel(const 
             while (size < n) size <<= 1;
             for (int i = n + threadIdx.x; i < size; i += kThreads) sh.list[i] = ~0ull;
             return size;
+        };
+        // of list[i]: how many are in front of it, and what they weigh
+        auto in_front = [&](int n, u64 o, u64 &weight) {
+            int rank = 0;
+            weight = 0;
+#pragma unroll 4
+            for (int j = 0; j < n; j++) {
+                const bool yes = sh.list[j] < o;
+                rank += yes, weight += yes ? sh.weight[j] : 0;
+            }
+            return rank;
         };
 
         // ---- the second look: the few that may be kept of a small k ----
@@ -430,9 +437,35 @@ __global__ void __launch_bounds__(kThreads, CACHED ? 1 : 4) sample_kernel(const 
             if (few && rank == 0) pull();
             cluster.sync();  // (the other CTAs are done)
             if (few && rank != 0) return;
+            if (few && n <= kRanked) {
+                // a thread to a token: its weight, its rank, what is in front of it; then the same by index among the kept
+                const int i = threadIdx.x;
+                const u64 o = i < n ? sh.list[i] : 0;
+                const double exact = i < n ? weigh.exact(logit_of(o)) : 0.0;
+                const u64 w = Weigher::units(exact);
+                if (i < n) sh.weight[i] = w;
+                __syncthreads();
+                u64 before = 0, all, kept;
+                const int place = i < n ? in_front(n, o, before) : n;
+                block_prefix<kThreads>(place < k ? w : 0, sh.scratch, all);
+                const bool keep = place < k && (!place || !by_mass || (double)before < (double)p_in * (double)all) && exact >= least_weight;
+                const u64 mine_kept = keep ? w : 0;
+                block_prefix<kThreads>(mine_kept, sh.scratch, kept);
+                if (i < n) sh.list[i] = (uint32_t)o, sh.weight[i] = mine_kept;
+                __syncthreads();
+                if (keep) {
+                    in_front(n, (uint32_t)o, before);
+                    const u64 want = target(kept);
+                    if (before <= want && want < before + w) {
+                        p.token[row] = (int32_t)(uint32_t)o;
+                        if (p.prob) p.prob[row] = (float)((double)w / (double)kept);
+                    }
+                }
+                return;
+            }
             if (few) {
                 const int size = padded(n);
-                sort_list(sh.list, size);
+                sort_list<kThreads>(sh.list, size);
                 // each thread has `per` neighbours
                 const int per = (size + kThreads - 1) / kThreads, begin = min(n, (int)threadIdx.x * per), end = min(n, begin + per), kept_k = min(k, n);
                 u64 part = 0, all;
@@ -441,7 +474,7 @@ __global__ void __launch_bounds__(kThreads, CACHED ? 1 : 4) sample_kernel(const 
                     sh.weight[i] = w;
                     part += w;
                 }
-                u64 before = block_prefix(part, sh.scratch, all);
+                u64 before = block_prefix<kThreads>(part, sh.scratch, all);
                 const double limit = (double)p_in * (double)all;
                 part = 0;
                 for (int i = begin; i < end; i++) {
@@ -452,17 +485,17 @@ __global__ void __launch_bounds__(kThreads, CACHED ? 1 : 4) sample_kernel(const 
                     part += keep ? w + (1ull << 52) : 0;  // (in the top bits: how many; weights are 2^50 at most in all)
                 }
                 u64 kept;
-                block_prefix(part, sh.scratch, kept);
+                block_prefix<kThreads>(part, sh.scratch, kept);
                 // the kept ones are the first of the list: by rising index, (index, place in order) sorted
                 const int n_kept = (int)(kept >> 52), size_kept = padded(n_kept);
                 kept &= (1ull << 52) - 1;
                 __syncthreads();
                 for (int i = threadIdx.x; i < size_kept; i += kThreads) sh.list[i] = i < n_kept ? (sh.list[i] & 0xFFFFFFFFull) << 32 | (uint32_t)i : ~0ull;
-                sort_list(sh.list, size_kept);
+                sort_list<kThreads>(sh.list, size_kept);
                 part = 0;
                 const int last = min(end, n_kept);
                 for (int i = begin; i < last; i++) part += sh.weight[(uint32_t)sh.list[i]];
-                u64 run = block_prefix(part, sh.scratch, all);
+                u64 run = block_prefix<kThreads>(part, sh.scratch, all);
                 const u64 want = target(kept);
                 for (int i = begin; i < last; i++) {
                     const u64 w = sh.weight[(uint32_t)sh.list[i]];
@@ -483,26 +516,29 @@ __global__ void __launch_bounds__(kThreads, CACHED ? 1 : 4) sample_kernel(const 
         const int bin = lead.bin;
         if (!k) whole = lead.total;
         ahead = lead.before;
-        low = ~0ull, high = 0, sum = 0;
-        if (threadIdx.x == 0) sh.n_list = 0;
+        // what is in doubt into the lists, and its first and last place; what comes in front of it as well into the CTA's own list
+        low = ~0ull, high = 0;
+        if (threadIdx.x == 0) sh.n_list = sh.n_few = 0;
         __syncthreads();
         each([&](int i, float v) {
             if (!up_to_bin(v, bin)) return;
             const u64 o = order_of(v, at + i);
-            if (*(volatile int *)&sh.n_list <= kFew) {
-                const int to = atomicAdd(&sh.n_list, 1);
+            if (*(volatile int *)&sh.n_few <= kFew) {
+                const int to = atomicAdd(&sh.n_few, 1);
                 if (to < kFew) few_places[to] = o;
             }
             if (bin_of(v) != bin) return;
             low = o < low ? o : low, high = o > high ? o : high;
-            count++;
+            append(o);
         });
-        joined();
-        if (sh.n_list <= kFew) n_few = sh.n_list;  // (what is not in it is not kept)
-        __syncthreads();
+        cluster.sync();
+        if (sh.n_few <= kFew) n_few = sh.n_few;  // (what is not in it is not kept)
+        int n = in_all_lists();
+        bool bounds = false;  // low and high are the row's, not the CTA's
         for (;;) {
             // (every round leaves one bin of 1024, and places are numbers of 64 bits that all differ: at most seven)
-            while (count > kList) {
+            while (n > kList) {
+                if (!bounds) joined();
                 int shift = 0;
                 while ((high - low) >> shift >= (u64)kBins) shift++;
                 clear();
@@ -511,62 +547,62 @@ __global__ void __launch_bounds__(kThreads, CACHED ? 1 : 4) sample_kernel(const 
                     return v > -INFINITY && o >= low && o <= high ? (int)((o - low) >> shift) : -1;
                 });
                 find(counting ? (u64)k : 0);
+                if (!counting && !whole) whole = lead.total;
                 ahead = lead.before;
                 const u64 from = low + ((u64)lead.bin << shift), to = min(high, from + ((1ull << shift) - 1));
-                low = ~0ull, high = 0, count = 0, sum = 0;
+                low = ~0ull, high = 0, bounds = false;
+                if (threadIdx.x == 0) sh.n_list = 0;
+                __syncthreads();
                 each([&](int i, float v) {
                     const u64 o = order_of(v, at + i);
                     if (!(v > -INFINITY) || o < from || o > to) return;
                     low = o < low ? o : low, high = o > high ? o : high;
-                    count++;
+                    append(o);
                 });
-                joined();
+                cluster.sync();
+                n = in_all_lists();
             }
-            if (threadIdx.x == 0) sh.n_list = 0;
-            __syncthreads();
-            each([&](int i, float v) {
-                const u64 o = order_of(v, at + i);
-                if (v > -INFINITY && o >= low && o <= high) append(o);
-            });
-            cluster.sync();
-            const int n = min(in_all_lists(), kList);
             if (rank == 0) {
                 pull();
-                const int size = padded(n);
-                sort_list(sh.list, size);
-                if (counting) {
-                    if (threadIdx.x == 0) sh.cut = sh.list[max(0, min(n, k - (int)ahead) - 1)];
+                const double limit = (double)p_in * (double)whole;
+                if (!counting)
+                    for (int i = threadIdx.x; i < n; i += kThreads) sh.weight[i] = weigh(logit_of(sh.list[i]));
+                if (threadIdx.x == 0) sh.cut = 0;
+                __syncthreads();
+                if (n <= kRanked) {
+                    const int i = threadIdx.x;
+                    u64 before = 0;
+                    if (i < n) {
+                        const u64 o = sh.list[i];
+                        const int place = in_front(n, o, before);
+                        // the k-th; or the last that is kept, and the row's first is always
+                        if (counting ? (u64)place == (u64)k - ahead - 1 : !place || (double)(ahead + before) < limit) atomicMax(&sh.cut, o);
+                    }
                 } else {
-                    const int per = (size + kThreads - 1) / kThreads, begin = min(n, (int)threadIdx.x * per), end = min(n, begin + per);
-                    u64 part = 0, all;
-                    for (int i = begin; i < end; i++) part += sh.weight[i] = weigh(logit_of(sh.list[i]));
-                    u64 before = ahead + block_prefix(part, sh.scratch, all);
-                    const double limit = (double)p_in * (double)whole;
-                    if (threadIdx.x == 0) sh.cut = sh.list[0];
-                    __syncthreads();
-                    for (int i = begin; i < end; i++) {  // (the last that is kept; the row's first always is)
-                        if ((double)before < limit) atomicMax(&sh.cut, sh.list[i]);
-                        before += sh.weight[i];
+                    const int size = padded(n);
+                    sort_list<kThreads>(sh.list, size);
+                    if (counting) {
+                        if (threadIdx.x == 0) sh.cut = sh.list[max(0, min(n, k - (int)ahead) - 1)];
+                    } else {
+                        const int per = (size + kThreads - 1) / kThreads, begin = min(n, (int)threadIdx.x * per), end = min(n, begin + per);
+                        u64 part = 0, all;
+                        for (int i = begin; i < end; i++) part += weigh(logit_of(sh.list[i]));
+                        u64 before = ahead + block_prefix<kThreads>(part, sh.scratch, all);
+                        for (int i = begin; i < end; i++) {
+                            if (!i || (double)before < limit) atomicMax(&sh.cut, sh.list[i]);
+                            before += weigh(logit_of(sh.list[i]));
+                        }
                     }
                 }
             }
             cluster.sync();
             cut = lead.cut;
-            cluster.sync();
             if (!counting || !by_mass) break;
-            // a share of the k's: their weights, and all of them in doubt
-            counting = false;
-            low = ~0ull, high = 0, sum = 0, count = 0;
-            each([&](int i, float v) {
-                const u64 o = order_of(v, at + i);
-                if (!(v > -INFINITY) || o > cut) return;
-                sum += weigh(v);
-                low = o < low ? o : low, high = o > high ? o : high;
-                count++;
-            });
-            joined();
-            whole = sum, ahead = 0;
+            // a share of the k's: all of them in doubt
+            counting = false, bounds = true;
+            low = first, high = cut, ahead = 0, n = kList + 1;
         }
+        cluster.sync();  // (all have read it)
     }
 
     // ---- the kept tokens' weights by tiles of neighbours, a warp to a tile, four tokens to a lane ----
@@ -604,7 +640,7 @@ __global__ void __launch_bounds__(kThreads, CACHED ? 1 : 4) sample_kernel(const 
     const int per = (tiles + kThreads - 1) / kThreads, begin = min(tiles, (int)threadIdx.x * per), end = min(tiles, begin + per);
     u64 part = 0, mine_all;
     for (int t = begin; t < end; t++) part += sh.tile[t];
-    u64 run = block_prefix(part, sh.scratch, mine_all);
+    u64 run = block_prefix<kThreads>(part, sh.scratch, mine_all);
     if (threadIdx.x == 0) sh.mass = mine_all, sh.bin = -1;
     cluster.sync();
     const u64 of_cta = lane < ctas ? of(lane < ctas ? lane : 0)->mass : 0, kept = warp_sum(of_cta);
@@ -651,7 +687,7 @@ bool launch(const SampleParams &p, int rows, int ctas) {
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)rows * ctas);
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(CACHED ? kOneThreads : kManyThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream();
     cudaLaunchAttribute attr[2];
