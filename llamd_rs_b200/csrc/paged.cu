@@ -317,11 +317,12 @@ __global__ void __launch_bounds__(256, kAppendCtas) paged_append_kernel(const Ap
     }
 }
 
+// queries: the keys and values go elsewhere (paged_append8.cu)
 template <typename TI, typename T, int HD>
-void append_launch_hd(AppendParams &p, bool interleaved, bool aligned) {
+void append_launch_hd(AppendParams &p, bool interleaved, bool aligned, bool queries) {
     constexpr int kHeads = kAppendHeads<TI> * (32 / (HD / 8));  // to a warp
     p.q_tasks = (p.b.n_head + kHeads - 1) / kHeads;
-    p.kv_tasks = (p.b.n_head_kv + kHeads - 1) / kHeads;
+    p.kv_tasks = queries ? 0 : (p.b.n_head_kv + kHeads - 1) / kHeads;
     p.tasks = p.b.tokens * (p.q_tasks + 2 * p.kv_tasks);
     const dim3 grid((unsigned)std::min((p.tasks + 7) / 8, kAppendCtas * p.sms));
     const auto launch = [&](auto kernel) { launch_kc(PDL_PAGED, "paged_append", kernel, grid, dim3(256), 0, p); };
@@ -329,9 +330,18 @@ void append_launch_hd(AppendParams &p, bool interleaved, bool aligned) {
     else launch(interleaved ? paged_append_kernel<TI, T, HD, true, false> : paged_append_kernel<TI, T, HD, false, false>);
 }
 template <typename TI, typename T>
-void append_launch(AppendParams &p, bool interleaved, bool aligned) {
-    if (p.b.hd == 128) append_launch_hd<TI, T, 128>(p, interleaved, aligned);
-    else append_launch_hd<TI, T, 64>(p, interleaved, aligned);
+void append_launch(AppendParams &p, bool interleaved, bool aligned, bool queries) {
+    if (p.b.hd == 128) append_launch_hd<TI, T, 128>(p, interleaved, aligned, queries);
+    else append_launch_hd<TI, T, 64>(p, interleaved, aligned, queries);
+}
+void append_launch(AppendParams &p, int in_type, int type, bool interleaved, bool aligned, bool queries) {
+    if (type == kPagedF16) {
+        if (in_type == kPagedF32) append_launch<float, __half>(p, interleaved, aligned, queries);
+        else append_launch<__half, __half>(p, interleaved, aligned, queries);
+    } else {
+        if (in_type == kPagedF32) append_launch<float, __nv_bfloat16>(p, interleaved, aligned, queries);
+        else append_launch<__nv_bfloat16, __nv_bfloat16>(p, interleaved, aligned, queries);
+    }
 }
 
 // True and an error where an earlier attention gave up and nobody has read it: what reads its outputs, or works on beside them, has to know.
@@ -510,13 +520,7 @@ int llamd_fwd_paged_append(const void *batch, const void *q, const void *k, cons
     const int go = append_of(b, p, aligned, q, k, v, in_type, q_stride, k_stride, v_stride, wq, wk, eps, rope_tab, rope_rows, rot, q_out, out_stride, k_pages, v_pages);
     if (go < 1) return go;
     if (!b->note_graph()) return -1;
-    if (b->type == kPagedF16) {
-        if (in_type == kPagedF32) append_launch<float, __half>(p, interleaved != 0, aligned);
-        else append_launch<__half, __half>(p, interleaved != 0, aligned);
-    } else {
-        if (in_type == kPagedF32) append_launch<float, __nv_bfloat16>(p, interleaved != 0, aligned);
-        else append_launch<__nv_bfloat16, __nv_bfloat16>(p, interleaved != 0, aligned);
-    }
+    append_launch(p, in_type, b->type, interleaved != 0, aligned, false);
     return error_code() ? -1 : 0;
 }
 
@@ -534,7 +538,10 @@ int llamd_fwd_paged_append8(const void *batch, const void *q, const void *k, con
     if (b->shared_write) return refuse("paged append: two new tokens' pages are one, whose scales both would change");
     if ((long long)b->view.tokens * b->view.n_head + 2LL * b->n_block * b->view.n_head_kv > 1LL << 30) return refuse("paged append: too many tokens");
     if (!b->note_graph()) return -1;
-    paged_append8_launch(p, Append8{b->block, b->n_block, k_scales, v_scales}, in_type, b->type, b->cache, interleaved != 0, aligned);
+    const Append8 a = {b->block, b->n_block, k_scales, v_scales};
+    const bool apart = paged_append8_apart(p, a);
+    if (apart) append_launch(p, in_type, b->type, interleaved != 0, aligned, true);
+    paged_append8_launch(p, a, in_type, b->type, b->cache, interleaved != 0, aligned, !apart);
     return error_code() ? -1 : 0;
 }
 

@@ -20,7 +20,8 @@ struct Append8 {
     int n_blocks;
     uint8_t *k_scales, *v_scales;
 };
-void paged_append8_launch(AppendParams &p, const Append8 &a, int in_type, int type, int cache, bool interleaved, bool aligned);
+bool paged_append8_apart(const AppendParams &p, const Append8 &a);  // the queries are worth a launch of their own, by the append of 16 bits
+void paged_append8_launch(AppendParams &p, const Append8 &a, int in_type, int type, int cache, bool interleaved, bool aligned, bool queries);
 
 // 4 neighbouring elements as they lie, and in f32
 template <typename T> struct Four {

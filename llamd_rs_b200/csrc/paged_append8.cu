@@ -20,7 +20,7 @@ namespace llamd {
 namespace {
 
 template <typename TI> constexpr int kQueryHeads = sizeof(TI) == 2 ? 4 : 2;  // that a warp has on their way, as in paged.cu
-constexpr int kAppend8Ctas = 2;  // (a block's 64 values to a lane)
+constexpr int kAppend8Ctas = 2;  // (a block's 64 values to a lane; half a block to a warp and three CTAs were no quicker: 43 us for 42)
 
 // four codes
 template <int C> __device__ __forceinline__ uint32_t codes(float a, float b, float c, float d);
@@ -144,14 +144,21 @@ __global__ void __launch_bounds__(256, kAppend8Ctas) paged_append8_kernel(const 
             if (r < blk.n) raw[0].load(src + r * stride + first, ALIGNED), raw[1].load(src + r * stride + second, ALIGNED);
             raw[0].get(y[i]), raw[1].get(y[i] + 4);
         }
-#pragma unroll
-        for (int i = 0; i < kRounds; i++) {
-            if (i * PER >= blk.n) break;  // (the whole warp)
-            const int r = i * PER + side;
-            if (rotated && r < blk.n) angles(tok.pos + r, sn, cs);
-            norm_rotate<HD, INTERLEAVED>(y[i], wp != nullptr, w, p.eps, rotated && r < blk.n, sn, cs);
+        auto round = [&](int i, bool live) {
+            if (rotated && live) angles(tok.pos + i * PER + side, sn, cs);
+            norm_rotate<HD, INTERLEAVED>(y[i], wp != nullptr, w, p.eps, rotated && live, sn, cs);
 #pragma unroll
             for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(y[i][j]));  // (a NaN counts for nothing)
+        };
+        if (blk.n == kScaleBlock) {  // (nothing to decide: the rounds go side by side)
+#pragma unroll
+            for (int i = 0; i < kRounds; i++) round(i, true);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kRounds; i++) {
+                if (i * PER >= blk.n) break;  // (the whole warp)
+                round(i, i * PER + side < blk.n);
+            }
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -179,9 +186,9 @@ __global__ void __launch_bounds__(256, kAppend8Ctas) paged_append8_kernel(const 
 }
 
 template <typename TI, typename T, int C, int HD>
-void launch_hd(AppendParams &p, const Append8 &a, bool interleaved, bool aligned) {
+void launch_hd(AppendParams &p, const Append8 &a, bool interleaved, bool aligned, bool queries) {
     constexpr int kHeads = kQueryHeads<TI> * (32 / (HD / 8));  // to a warp
-    p.q_tasks = (p.b.n_head + kHeads - 1) / kHeads;
+    p.q_tasks = queries ? (p.b.n_head + kHeads - 1) / kHeads : 0;
     p.tasks = p.b.tokens * p.q_tasks + a.n_blocks * 2 * p.b.n_head_kv;
     const dim3 grid((unsigned)std::min((p.tasks + 7) / 8, kAppend8Ctas * p.sms));
     const auto launch = [&](auto kernel) { launch_kc(PDL_PAGED, "paged_append8", kernel, grid, dim3(256), 0, p, a); };
@@ -189,20 +196,26 @@ void launch_hd(AppendParams &p, const Append8 &a, bool interleaved, bool aligned
     else launch(interleaved ? paged_append8_kernel<TI, T, C, HD, true, false> : paged_append8_kernel<TI, T, C, HD, false, false>);
 }
 template <typename TI, typename T>
-void launch_types(AppendParams &p, const Append8 &a, int cache, bool interleaved, bool aligned) {
-    if (cache == kPagedI8) p.b.hd == 128 ? launch_hd<TI, T, kPagedI8, 128>(p, a, interleaved, aligned) : launch_hd<TI, T, kPagedI8, 64>(p, a, interleaved, aligned);
-    else p.b.hd == 128 ? launch_hd<TI, T, kPagedE4m3, 128>(p, a, interleaved, aligned) : launch_hd<TI, T, kPagedE4m3, 64>(p, a, interleaved, aligned);
+void launch_types(AppendParams &p, const Append8 &a, int cache, bool interleaved, bool aligned, bool queries) {
+    if (cache == kPagedI8) p.b.hd == 128 ? launch_hd<TI, T, kPagedI8, 128>(p, a, interleaved, aligned, queries) : launch_hd<TI, T, kPagedI8, 64>(p, a, interleaved, aligned, queries);
+    else p.b.hd == 128 ? launch_hd<TI, T, kPagedE4m3, 128>(p, a, interleaved, aligned, queries) : launch_hd<TI, T, kPagedE4m3, 64>(p, a, interleaved, aligned, queries);
 }
 
 }  // namespace
 
-void paged_append8_launch(AppendParams &p, const Append8 &a, int in_type, int type, int cache, bool interleaved, bool aligned) {
+// One launch while its warps run all at once; beyond that the queries, which need half the registers, by themselves: 8511 tokens of f16, 32 heads over 4 of
+// 128, 42 us in two launches (the queries 28), 52 in one, 45 in one with twice as many heads to a warp, 45 in two at the same time on two streams.
+bool paged_append8_apart(const AppendParams &p, const Append8 &a) {
+    return (long long)p.b.tokens * p.b.n_head / 8 + 2LL * a.n_blocks * p.b.n_head_kv > 16LL * kAppend8Ctas * p.sms;
+}
+
+void paged_append8_launch(AppendParams &p, const Append8 &a, int in_type, int type, int cache, bool interleaved, bool aligned, bool queries) {
     if (type == kPagedF16) {
-        if (in_type == kPagedF32) launch_types<float, __half>(p, a, cache, interleaved, aligned);
-        else launch_types<__half, __half>(p, a, cache, interleaved, aligned);
+        if (in_type == kPagedF32) launch_types<float, __half>(p, a, cache, interleaved, aligned, queries);
+        else launch_types<__half, __half>(p, a, cache, interleaved, aligned, queries);
     } else {
-        if (in_type == kPagedF32) launch_types<float, __nv_bfloat16>(p, a, cache, interleaved, aligned);
-        else launch_types<__nv_bfloat16, __nv_bfloat16>(p, a, cache, interleaved, aligned);
+        if (in_type == kPagedF32) launch_types<float, __nv_bfloat16>(p, a, cache, interleaved, aligned, queries);
+        else launch_types<__nv_bfloat16, __nv_bfloat16>(p, a, cache, interleaved, aligned, queries);
     }
 }
 
