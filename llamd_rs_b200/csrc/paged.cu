@@ -180,55 +180,6 @@ const char *check_lengths(const Batch &b, int n_seq, const int32_t *q_len, const
     return nullptr;
 }
 
-// What a cache in 8 bits needs of a batch: where its new tokens meet scale blocks.
-void blocks_of(std::vector<PagedBlock> &block, int n_seq, const int32_t *q_len, const int32_t *kv_len) {
-    for (int s = 0, t = 0; s < n_seq; t += q_len[s], s++)
-        for (int pos = kv_len[s] - q_len[s]; pos < kv_len[s];) {
-            const int n = std::min(kScaleBlock - pos % kScaleBlock, kv_len[s] - pos);
-            block.push_back({t + pos - (kv_len[s] - q_len[s]), n});
-            pos += n;
-        }
-}
-// The pages that the plan's large pieces read: each once, a shared prefix's for all; and a table of their places in that list beside the batch's own (a
-// second [n_seq][table_stride] behind it), which the pieces are pointed to.
-void wide_pages(std::vector<PagedWide> &wide, std::vector<int32_t> &table, Plan &plan, const PagedView &v, const int32_t *pages, int pages_stride) {
-    if (plan.large.empty()) return;
-    const int stride = v.table_stride, common = v.n_shared / v.page;
-    std::vector<std::pair<int, int>> range(v.n_seq, {0x7fffffff, 0});  // positions that a sequence's pieces read: one stretch, or the prefix and its own behind it
-    for (const PagedItem &it : plan.large) {
-        auto &r = range[it.table / stride];
-        r = {std::min(r.first, it.kv_begin), std::max(r.second, it.kv_end)};
-    }
-    table.assign((size_t)v.n_seq * stride, 0);
-    int prefix = -1;  // where the common pages begin in the list
-    for (int s = 0; s < v.n_seq; s++) {
-        const int end = range[s].second, n = (end + v.page - 1) / v.page;
-        if (!end) continue;
-        int i = range[s].first / v.page;
-        if (i < common) {  // (a stretch that begins in front of its own positions begins with the prefix)
-            if (prefix < 0) {
-                prefix = (int)wide.size();
-                for (int x = 0; x < common; x++) wide.push_back({pages[(size_t)s * pages_stride + x], v.page});
-            }
-            for (; i < std::min(n, common); i++) table[(size_t)s * stride + i] = prefix + i;
-        }
-        for (; i < n; i++) {
-            table[(size_t)s * stride + i] = (int32_t)wide.size();
-            wide.push_back({pages[(size_t)s * pages_stride + i], std::min(v.page, end - i * v.page)});
-        }
-    }
-    for (PagedItem &it : plan.large) it.table += v.n_seq * stride;
-}
-// Do two new tokens' places share a page that two sequences list, or one twice?
-bool writes_shared(int page, int n_seq, const int32_t *q_len, const int32_t *kv_len, const int32_t *pages, int pages_stride) {
-    std::vector<int32_t> written;
-    for (int s = 0; s < n_seq; s++)
-        if (q_len[s])
-            for (int i = (kv_len[s] - q_len[s]) / page; i <= (kv_len[s] - 1) / page; i++) written.push_back(pages[(size_t)s * pages_stride + i]);
-    std::sort(written.begin(), written.end());
-    return std::adjacent_find(written.begin(), written.end()) != written.end();
-}
-
 // ---- append --------------------------------------------------------------------------------------------------------------
 //
 //   y = x / sqrt(mean(x^2) + eps) * w        per head of q and k (weights given), in f32

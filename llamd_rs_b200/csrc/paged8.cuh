@@ -6,8 +6,6 @@
 
 namespace llamd {
 
-constexpr int kScaleBlock = 16;
-
 // The largest code, and the exponents of an append's scales: between them every value is exact in f16, subnormals included.
 template <int C> struct Cache8;
 template <> struct Cache8<kPagedI8> {

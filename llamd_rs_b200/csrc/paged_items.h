@@ -9,6 +9,9 @@ struct PagedToken {
     int32_t pos, row;
 };
 
+// Positions of a page that share a scale in a cache in 8 bits.
+constexpr int kScaleBlock = 16;
+
 // A sequence's new tokens that share a scale block of a cache in 8 bits: rows [token, token + n) of the batch, behind the block's older ones.
 struct PagedBlock {
     int32_t token, n;
