@@ -29,18 +29,24 @@ __global__ void __launch_bounds__(256) paged_widen_kernel(const PagedWiden w, in
     const uint8_t *const codes = reinterpret_cast<const uint8_t *>(blockIdx.y ? w.v_pages : w.k_pages), *const scales = blockIdx.y ? w.v_scales : w.k_scales;
     uint4 *const out = reinterpret_cast<uint4 *>(blockIdx.y ? w.v_out : w.k_out);
     const int step = (int)(gridDim.x * blockDim.x);
-    pdl_wait();
-    for (int first = (int)(blockIdx.x * blockDim.x + threadIdx.x); first < units; first += kUnits * step) {
-        // (each kind of load for all of them at once: three that wait for one another, not twelve)
-        uint4 x[kUnits];
-        PagedWide p[kUnits];
-        int in[kUnits], byte[kUnits];
+    // (each kind of load for all of them at once; the list is the batch's own, complete before the launch in front of this one began)
+    PagedWide p[kUnits];
+    int in[kUnits];
+    auto find = [&](int first) {
 #pragma unroll
         for (int i = 0; i < kUnits; i++) {
             const int u = min(first + i * step, units - 1), page = u / per_page;
             in[i] = u - page * per_page;
             p[i] = w.page[page];
         }
+    };
+    const int begin = (int)(blockIdx.x * blockDim.x + threadIdx.x);
+    find(begin);
+    pdl_wait();
+    for (int first = begin; first < units; first += kUnits * step) {
+        if (first != begin) find(first);
+        uint4 x[kUnits];
+        int byte[kUnits];
 #pragma unroll
         for (int i = 0; i < kUnits; i++) {
             const int row = in[i] / CHUNKS;  // of the page's heads and positions
