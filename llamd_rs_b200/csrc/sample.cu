@@ -30,7 +30,7 @@ typedef unsigned long long u64;
 
 // threads of a CTA: of one of four to an SM, and of one that has its SM to itself (and its part of the row in shared memory)
 constexpr int kManyThreads = 256, kOneThreads = 1024, kMostWarps = kOneThreads / 32;
-constexpr int kBins = 1024, kList = 1024, kRanked = 256, kMostCtas = 8, kTile = 128;  // kRanked: lists that are put in order by counting, not sorted
+constexpr int kBins = 1024, kList = 1024, kMostCtas = 8, kTile = 128;
 static_assert(kBins % 2 == 0, "bins are read two at a time");
 constexpr int kMostTokens = 393216, kMostPart = 262144;  // of a row; of a CTA (the tiles' sums have room)
 constexpr int kFew = 2560;   // tokens of a CTA's part that may be in its list
@@ -167,6 +167,7 @@ __device__ __forceinline__ void sort_list(u64 *list, int size) {
 template <typename T, bool CACHED>
 __global__ void __launch_bounds__(CACHED ? kOneThreads : kManyThreads, CACHED ? 1 : 4) sample_kernel(const SampleParams p) {
     constexpr int kThreads = CACHED ? kOneThreads : kManyThreads, kWarpsN = kThreads / 32;
+    constexpr int kRanked = kThreads;  // lists up to so many are put in order by counting, not sorted
     extern __shared__ __align__(16) uint8_t raw[];
     Shared &sh = *reinterpret_cast<Shared *>(raw);
     u64 *const few_places = reinterpret_cast<u64 *>(raw + sizeof(Shared));
@@ -180,9 +181,21 @@ __global__ void __launch_bounds__(CACHED ? kOneThreads : kManyThreads, CACHED ? 
     auto clean = [](float v) { return fmaxf(v, -INFINITY); };  // (NaN is no token)
     constexpr int kWide = 16 / sizeof(T);
     const int wide = ((uintptr_t)src & 15) == 0 ? mine / kWide : 0;
-    // f(i, logit) for the part's tokens, of one thread in rising order
-    // (loads first, kBatch of them at a time: what f does keeps the compiler from moving them)
+    // f(i, logits) for the part's tokens, four at a time (i: the place of each, logits -inf where there is none), of one thread in rising order. Loads first, several
+    // fours of them: what f does keeps the compiler from moving them.
     constexpr int kBatch = sizeof(T) == 4 ? 4 : 2;
+    typedef int Places[4];
+    typedef float Logits[4];
+    auto wide_four = [&](int i, uint4 v, auto f) {
+        const T *e = reinterpret_cast<const T *>(&v);
+#pragma unroll
+        for (int h = 0; h < kWide; h += 4) {
+            const int at0 = i * kWide + h;
+            const Places places = {at0, at0 + 1, at0 + 2, at0 + 3};
+            const Logits logits = {clean(to_float(e[h])), clean(to_float(e[h + 1])), clean(to_float(e[h + 2])), clean(to_float(e[h + 3]))};
+            f(places, logits);
+        }
+    };
     auto from_memory = [&](auto f) {
         const uint4 *const from = reinterpret_cast<const uint4 *>(src);
         int i = threadIdx.x;
@@ -191,43 +204,40 @@ __global__ void __launch_bounds__(CACHED ? kOneThreads : kManyThreads, CACHED ? 
 #pragma unroll
             for (int b = 0; b < kBatch; b++) v[b] = from[i + b * kThreads];
 #pragma unroll
-            for (int b = 0; b < kBatch; b++) {
-                const T *e = reinterpret_cast<const T *>(&v[b]);
-#pragma unroll
-                for (int j = 0; j < kWide; j++) f((i + b * kThreads) * kWide + j, clean(to_float(e[j])));
-            }
+            for (int b = 0; b < kBatch; b++) wide_four(i + b * kThreads, v[b], f);
         }
-        for (; i < wide; i += kThreads) {
-            const uint4 v = from[i];
-            const T *e = reinterpret_cast<const T *>(&v);
+        for (; i < wide; i += kThreads) wide_four(i, from[i], f);
+        for (i = wide * kWide + threadIdx.x; i < mine; i += 4 * kThreads) {  // (rows that do not start at 16 bytes)
+            Places places;
+            Logits logits;
 #pragma unroll
-            for (int j = 0; j < kWide; j++) f(i * kWide + j, clean(to_float(e[j])));
+            for (int b = 0; b < 4; b++) places[b] = i + b * kThreads, logits[b] = places[b] < mine ? clean(to_float(src[places[b]])) : -INFINITY;
+            f(places, logits);
         }
-        i = wide * kWide + threadIdx.x;
-        for (; i + 7 * kThreads < mine; i += 8 * kThreads) {  // (rows that do not start at 16 bytes)
-            T v[8];
-#pragma unroll
-            for (int b = 0; b < 8; b++) v[b] = src[i + b * kThreads];
-#pragma unroll
-            for (int b = 0; b < 8; b++) f(i + b * kThreads, clean(to_float(v[b])));
-        }
-        for (; i < mine; i += kThreads) f(i, clean(to_float(src[i])));
     };
     // Once a CTA's part has few tokens that still matter, they are in a list of their own, and each() goes through that.
     int n_few = -1;
     auto each = [&](auto f) {
         if (n_few >= 0) {
-            for (int i = threadIdx.x; i < n_few; i += kThreads) f((int)(uint32_t)few_places[i] - at, logit_of(few_places[i]));
-        } else if constexpr (CACHED) {
-            int i = threadIdx.x;
-            for (; i + 3 * kThreads < mine; i += 4 * kThreads) {
-                float v[4];
+            for (int i = threadIdx.x; i < n_few; i += 4 * kThreads) {
+                Places places;
+                Logits logits;
 #pragma unroll
-                for (int b = 0; b < 4; b++) v[b] = x[i + b * kThreads];
-#pragma unroll
-                for (int b = 0; b < 4; b++) f(i + b * kThreads, v[b]);
+                for (int b = 0; b < 4; b++) {
+                    const bool in = i + b * kThreads < n_few;
+                    const u64 o = few_places[in ? i + b * kThreads : 0];
+                    places[b] = (int)(uint32_t)o - at, logits[b] = in ? logit_of(o) : -INFINITY;
+                }
+                f(places, logits);
             }
-            for (; i < mine; i += kThreads) f(i, x[i]);
+        } else if constexpr (CACHED) {
+            for (int i = threadIdx.x; i < mine; i += 4 * kThreads) {
+                Places places;
+                Logits logits;
+#pragma unroll
+                for (int b = 0; b < 4; b++) places[b] = i + b * kThreads, logits[b] = places[b] < mine ? x[places[b]] : -INFINITY;
+                f(places, logits);
+            }
         } else {
             from_memory(f);
         }
@@ -241,10 +251,14 @@ __global__ void __launch_bounds__(CACHED ? kOneThreads : kManyThreads, CACHED ? 
     // ---- the first look: the thread's largest logit, the row's top, its least above -inf, how many are ----
     float best = -INFINITY, least = INFINITY;
     int best_at = 0, live = 0;
-    from_memory([&](int i, float v) {
-        if (CACHED) x[i] = v;
-        if (v > best) best = v, best_at = i;
-        if (v > -INFINITY) least = fminf(least, v), live++;
+    from_memory([&](const Places &i, const Logits &v) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if (CACHED && i[j] < mine) x[i[j]] = v[j];
+            if (v[j] > best) best = v[j], best_at = i[j];
+            least = v[j] > -INFINITY ? fminf(least, v[j]) : least;
+            live += v[j] > -INFINITY;
+        }
     });
     u64 first = warp_least(best > -INFINITY ? order_of(best, at + best_at) : ~0ull);
 #pragma unroll
@@ -302,7 +316,7 @@ __global__ void __launch_bounds__(CACHED ? kOneThreads : kManyThreads, CACHED ? 
         const float range = top - least, per_bin = range > 0.0f && range < INFINITY ? fminf((kBins - 1) / range, 1e30f) : 0.0f;
         auto distance = [&](float v) { return per_bin > 0.0f ? (top - v) * per_bin : 0.0f; };
         auto bin_of = [&](float v) { return min(kBins - 1, (int)distance(v)); };
-        auto up_to_bin = [&](float v, int bin) { return v > -INFINITY && (bin == kBins - 1 || distance(v) < (float)(bin + 1)); };
+        auto bin_end = [&](int bin) { return bin == kBins - 1 ? INFINITY : (float)(bin + 1); };  // the first distance behind it
         // In doubt are tokens of places [low, high]; in front of them are `ahead` tokens or weights that are kept for certain. First the k's end is
         // looked for, where there is a k, then that of a share of the weights, all or the k's.
         bool counting = k > 0;
@@ -315,18 +329,30 @@ __global__ void __launch_bounds__(CACHED ? kOneThreads : kManyThreads, CACHED ? 
         // (two loops: in one, an exponential would be made for each token and thrown away where only tokens are counted)
         auto fill = [&](auto bin) {  // bin(i, v): below 0 for those that are not to be in any
             if (counting) {
-                each([&](int i, float v) {
-                    const int b = bin(i, v);
-                    if (b >= 0) atomicAdd(&sh.hist[b], 1u);
+                each([&](const Places &i, const Logits &v) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const int b = bin(i[j], v[j]);
+                        if (b >= 0) atomicAdd(&sh.hist[b], 1u);
+                    }
                 });
             } else {
-                each([&](int i, float v) {
-                    const int b = bin(i, v);
-                    if (b < 0) return;
-                    const u64 w = weigh(v);
-                    // (64 bits in two: what the low ones carry goes with the high ones, which few weights have)
-                    const uint32_t lo = (uint32_t)w, was = atomicAdd(&sh.digit[0][b], lo), up = (uint32_t)(w >> 32) + (was > ~lo);
-                    if (up) atomicAdd(&sh.digit[1][b], up);
+                // 64 bits in two: what the low ones carry goes with the high ones, which few weights have
+                each([&](const Places &i, const Logits &v) {
+                    int b[4];
+                    uint32_t up[4], any = 0;
+                    u64 w[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) b[j] = bin(i[j], v[j]), w[j] = weigh(v[j]);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const uint32_t lo = (uint32_t)w[j], was = b[j] >= 0 ? atomicAdd(&sh.digit[0][b[j]], lo) : 0;
+                        up[j] = b[j] >= 0 ? (uint32_t)(w[j] >> 32) + (was > ~lo) : 0, any |= up[j];
+                    }
+                    if (any)
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            if (up[j]) atomicAdd(&sh.digit[1][b[j]], up[j]);
                 });
             }
         };
@@ -383,13 +409,26 @@ __global__ void __launch_bounds__(CACHED ? kOneThreads : kManyThreads, CACHED ? 
             low = warp_least(o.part_low), high = warp_most(o.part_high);
             cluster.sync();  // (all have read it)
         };
-        // Into this CTA's own list, in any order (up to kList, counted beyond); all lists then into CTA 0's, where they are no more than kList in all. Between the
-        // two the cluster is joined.
-        auto append = [&](u64 o) {
-            if (*(volatile int *)&sh.n_list > kList) return;
-            const int to = atomicAdd(&sh.n_list, 1);
-            if (to < kList) sh.list[to] = o;
+        // Four tokens' places of each lane, those that are wanted, behind the others in a list of up to `most`, in any order: one atomic for the warp. Counted beyond.
+        auto append = [&](const bool (&yes)[4], const Logits &v, const Places &i, u64 *list, int most, int *count) {
+            const unsigned here = __activemask(), below = (1u << lane) - 1;
+            int before[4], all = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const unsigned b = __ballot_sync(here, yes[j]);
+                before[j] = all + __popc(b & below), all += __popc(b);
+            }
+            if (!all) return false;
+            const int leader = __ffs(here) - 1;
+            int from = 0;
+            if (lane == leader) from = atomicAdd(count, all);
+            from = __shfl_sync(here, from, leader);
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (yes[j] && from + before[j] < most) list[from + before[j]] = order_of(v[j], at + i[j]);
+            return from + all > most;
         };
+        // This CTA's own list; all lists then go into CTA 0's, where they are no more than kList in all. Between the two the cluster is joined.
         auto in_all_lists = [&]() {
             const int n = lane < ctas ? of(lane < ctas ? lane : 0)->n_list : 0;
             return __reduce_add_sync(0xffffffffu, n);
@@ -414,22 +453,46 @@ __global__ void __launch_bounds__(CACHED ? kOneThreads : kManyThreads, CACHED ? 
             weight = 0;
 #pragma unroll 4
             for (int j = 0; j < n; j++) {
-                const bool yes = sh.list[j] < o;
-                rank += yes, weight += yes ? sh.weight[j] : 0;
+                const u64 other = sh.list[j], w = sh.weight[j];
+                rank += other < o, weight += other < o ? w : 0;
             }
             return rank;
         };
 
         // ---- the second look: the few that may be kept of a small k ----
+        // Every CTA by its own threads' largest where all their lists together are no more than a thread to a token; by all of the row's for a larger k.
         bool few = k && k < ctas * kThreads * 3 / 4 && k <= kList * 3 / 4;
         if (few) {
+            const bool alone = ctas * (k + k / 8 + 4) <= kRanked && k < kThreads / 2;
             if (best > -INFINITY) atomicAdd(&sh.hist[bin_of(best)], 1u);
-            // (fewer than k threads may have a token: all of them, then)
-            if (rank == 0 && threadIdx.x == 0) sh.bin = kBins - 1;
-            find((u64)k);
-            const int bin = lead.bin;
-            each([&](int i, float v) {
-                if (up_to_bin(v, bin)) append(order_of(v, at + i));
+            int bin;
+            if (alone) {
+                __syncthreads();
+                constexpr int kPer = 4;
+                uint4 c = {0, 0, 0, 0};
+                if (threadIdx.x < kBins / kPer) c = reinterpret_cast<const uint4 *>(sh.hist)[threadIdx.x];
+                u64 all, n = block_prefix<kThreads>((u64)c.x + c.y + c.z + c.w, sh.scratch, all);
+                if (threadIdx.x == 0) sh.n_few = kBins - 1;  // (fewer than k threads may have a token: all of them, then)
+                __syncthreads();
+                const uint32_t counts[kPer] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+                for (int j = 0; j < kPer; j++) {
+                    if (n < (u64)k && n + counts[j] >= (u64)k) sh.n_few = threadIdx.x * kPer + j;
+                    n += counts[j];
+                }
+                __syncthreads();
+                bin = sh.n_few;
+            } else {
+                if (rank == 0 && threadIdx.x == 0) sh.bin = kBins - 1;
+                find((u64)k);
+                bin = lead.bin;
+            }
+            const float end = bin_end(bin);
+            each([&](const Places &i, const Logits &v) {
+                bool in[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) in[j] = v[j] > -INFINITY && distance(v[j]) < end;
+                append(in, v, i, sh.list, kList, &sh.n_list);
             });
             cluster.sync();
             const int n = in_all_lists();
@@ -438,23 +501,28 @@ __global__ void __launch_bounds__(CACHED ? kOneThreads : kManyThreads, CACHED ? 
             cluster.sync();  // (the other CTAs are done)
             if (few && rank != 0) return;
             if (few && n <= kRanked) {
-                // a thread to a token: its weight, its rank, what is in front of it; then the same by index among the kept
+                // a thread to a token: its rank by counting puts it in its place; the kept ones are the first of these; among them by index once more
                 const int i = threadIdx.x;
-                const u64 o = i < n ? sh.list[i] : 0;
-                const double exact = i < n ? weigh.exact(logit_of(o)) : 0.0;
+                if (i < n) {
+                    const u64 o = sh.list[i];
+                    int place = 0;
+#pragma unroll 8
+                    for (int j = 0; j < n; j++) place += sh.list[j] < o;
+                    sh.weight[place] = o;
+                }
+                __syncthreads();
+                const bool of_k = i < min(k, n);
+                const u64 o = of_k ? sh.weight[i] : 0;
+                const double exact = of_k ? weigh.exact(logit_of(o)) : 0.0;
                 const u64 w = Weigher::units(exact);
-                if (i < n) sh.weight[i] = w;
-                __syncthreads();
-                u64 before = 0, all, kept;
-                const int place = i < n ? in_front(n, o, before) : n;
-                block_prefix<kThreads>(place < k ? w : 0, sh.scratch, all);
-                const bool keep = place < k && (!place || !by_mass || (double)before < (double)p_in * (double)all) && exact >= least_weight;
-                const u64 mine_kept = keep ? w : 0;
-                block_prefix<kThreads>(mine_kept, sh.scratch, kept);
-                if (i < n) sh.list[i] = (uint32_t)o, sh.weight[i] = mine_kept;
-                __syncthreads();
+                u64 all, kept;
+                u64 before = block_prefix<kThreads>(w, sh.scratch, all);
+                const bool keep = of_k && (!i || !by_mass || (double)before < (double)p_in * (double)all) && exact >= least_weight;
+                block_prefix<kThreads>(keep ? w : 0, sh.scratch, kept);
+                if (keep) sh.list[i] = (uint32_t)o, sh.weight[i] = w;
+                const int n_kept = __syncthreads_count(keep);
                 if (keep) {
-                    in_front(n, (uint32_t)o, before);
+                    in_front(n_kept, (uint32_t)o, before);
                     const u64 want = target(kept);
                     if (before <= want && want < before + w) {
                         p.token[row] = (int32_t)(uint32_t)o;
@@ -520,16 +588,24 @@ __global__ void __launch_bounds__(CACHED ? kOneThreads : kManyThreads, CACHED ? 
         low = ~0ull, high = 0;
         if (threadIdx.x == 0) sh.n_list = sh.n_few = 0;
         __syncthreads();
-        each([&](int i, float v) {
-            if (!up_to_bin(v, bin)) return;
-            const u64 o = order_of(v, at + i);
-            if (*(volatile int *)&sh.n_few <= kFew) {
-                const int to = atomicAdd(&sh.n_few, 1);
-                if (to < kFew) few_places[to] = o;
+        const float first_of_bin = (float)bin, end_of_bin = bin_end(bin);
+        bool room = true;  // in the CTA's own list
+        each([&](const Places &i, const Logits &v) {
+            bool front[4], in[4], any = false;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float d = distance(v[j]);
+                front[j] = v[j] > -INFINITY && d < end_of_bin, in[j] = front[j] && d >= first_of_bin;
+                any |= in[j];
             }
-            if (bin_of(v) != bin) return;
-            low = o < low ? o : low, high = o > high ? o : high;
-            append(o);
+            if (room) room = !append(front, v, i, few_places, kFew, &sh.n_few);
+            if (any)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const u64 o = order_of(v[j], at + i[j]);
+                    low = in[j] && o < low ? o : low, high = in[j] && o > high ? o : high;
+                }
+            append(in, v, i, sh.list, kList, &sh.n_list);
         });
         cluster.sync();
         if (sh.n_few <= kFew) n_few = sh.n_few;  // (what is not in it is not kept)
@@ -553,11 +629,15 @@ __global__ void __launch_bounds__(CACHED ? kOneThreads : kManyThreads, CACHED ? 
                 low = ~0ull, high = 0, bounds = false;
                 if (threadIdx.x == 0) sh.n_list = 0;
                 __syncthreads();
-                each([&](int i, float v) {
-                    const u64 o = order_of(v, at + i);
-                    if (!(v > -INFINITY) || o < from || o > to) return;
-                    low = o < low ? o : low, high = o > high ? o : high;
-                    append(o);
+                each([&](const Places &i, const Logits &v) {
+                    bool in[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const u64 o = order_of(v[j], at + i[j]);
+                        in[j] = v[j] > -INFINITY && o >= from && o <= to;
+                        low = in[j] && o < low ? o : low, high = in[j] && o > high ? o : high;
+                    }
+                    append(in, v, i, sh.list, kList, &sh.n_list);
                 });
                 cluster.sync();
                 n = in_all_lists();
@@ -565,34 +645,71 @@ __global__ void __launch_bounds__(CACHED ? kOneThreads : kManyThreads, CACHED ? 
             if (rank == 0) {
                 pull();
                 const double limit = (double)p_in * (double)whole;
+                // what is left of it where it is long, by bins once more: this CTA's own, its places spread between the first and the last
+                u64 ahead_here = ahead;
+                while (n > kRanked) {
+                    constexpr int kEach = kList / kThreads, kPer = 4;
+                    u64 o[kEach], lo = ~0ull, hi = 0;
+#pragma unroll
+                    for (int j = 0; j < kEach; j++) {
+                        const int i = threadIdx.x + j * kThreads;
+                        o[j] = i < n ? sh.list[i] : ~0ull;
+                        if (i < n) lo = o[j] < lo ? o[j] : lo, hi = o[j] > hi ? o[j] : hi;
+                    }
+                    lo = warp_least(lo), hi = warp_most(hi);
+                    if (lane == 0) sh.low[warp] = lo, sh.high[warp] = hi;
+                    uint32_t *const low_words = reinterpret_cast<uint32_t *>(sh.weight), *const high_words = low_words + kBins;
+                    for (int i = threadIdx.x; i < kBins; i += kThreads) sh.hist[i] = low_words[i] = high_words[i] = 0;
+                    __syncthreads();
+                    lo = warp_least(lane < kWarpsN ? sh.low[lane] : ~0ull), hi = warp_most(lane < kWarpsN ? sh.high[lane] : 0);
+                    int shift = 0;
+                    while ((hi - lo) >> shift >= (u64)kBins) shift++;
+#pragma unroll
+                    for (int j = 0; j < kEach; j++) {
+                        if (threadIdx.x + j * kThreads >= n) break;
+                        const int b = (int)((o[j] - lo) >> shift);
+                        atomicAdd(&sh.hist[b], 1u);
+                        if (counting) continue;
+                        const u64 w = weigh(logit_of(o[j]));
+                        const uint32_t was = atomicAdd(&low_words[b], (uint32_t)w), up = (uint32_t)(w >> 32) + (was > ~(uint32_t)w);
+                        if (up) atomicAdd(&high_words[b], up);
+                    }
+                    __syncthreads();
+                    uint32_t c[kPer] = {};
+                    u64 w[kPer] = {}, all, m = 0;
+#pragma unroll
+                    for (int j = 0; j < kPer; j++)
+                        if (threadIdx.x < kBins / kPer) c[j] = sh.hist[threadIdx.x * kPer + j], w[j] = counting ? c[j] : low_words[threadIdx.x * kPer + j] | (u64)high_words[threadIdx.x * kPer + j] << 32, m += w[j];
+                    m = block_prefix<kThreads>(m, sh.scratch, all);
+                    if (threadIdx.x == 0) sh.n_list = 0;
+#pragma unroll
+                    for (int j = 0; j < kPer; j++) {
+                        const bool here = counting ? ahead_here + m < (u64)k && ahead_here + m + c[j] >= (u64)k
+                                                   : w[j] && ((double)(ahead_here + m) < limit || (!ahead_here && !m)) && (double)(ahead_here + m + w[j]) >= limit;
+                        if (here) sh.bin = threadIdx.x * kPer + j, sh.before = ahead_here + m;
+                        m += w[j];
+                    }
+                    __syncthreads();
+                    const int b = sh.bin;
+                    ahead_here = sh.before;
+#pragma unroll
+                    for (int j = 0; j < kEach; j++)
+                        if (threadIdx.x + j * kThreads < n && (int)((o[j] - lo) >> shift) == b) sh.list[atomicAdd(&sh.n_list, 1)] = o[j];
+                    __syncthreads();
+                    n = sh.n_list;
+                    __syncthreads();
+                }
                 if (!counting)
                     for (int i = threadIdx.x; i < n; i += kThreads) sh.weight[i] = weigh(logit_of(sh.list[i]));
                 if (threadIdx.x == 0) sh.cut = 0;
                 __syncthreads();
-                if (n <= kRanked) {
-                    const int i = threadIdx.x;
+                const int i = threadIdx.x;
+                if (i < n) {
                     u64 before = 0;
-                    if (i < n) {
-                        const u64 o = sh.list[i];
-                        const int place = in_front(n, o, before);
-                        // the k-th; or the last that is kept, and the row's first is always
-                        if (counting ? (u64)place == (u64)k - ahead - 1 : !place || (double)(ahead + before) < limit) atomicMax(&sh.cut, o);
-                    }
-                } else {
-                    const int size = padded(n);
-                    sort_list<kThreads>(sh.list, size);
-                    if (counting) {
-                        if (threadIdx.x == 0) sh.cut = sh.list[max(0, min(n, k - (int)ahead) - 1)];
-                    } else {
-                        const int per = (size + kThreads - 1) / kThreads, begin = min(n, (int)threadIdx.x * per), end = min(n, begin + per);
-                        u64 part = 0, all;
-                        for (int i = begin; i < end; i++) part += weigh(logit_of(sh.list[i]));
-                        u64 before = ahead + block_prefix<kThreads>(part, sh.scratch, all);
-                        for (int i = begin; i < end; i++) {
-                            if (!i || (double)before < limit) atomicMax(&sh.cut, sh.list[i]);
-                            before += weigh(logit_of(sh.list[i]));
-                        }
-                    }
+                    const u64 o = sh.list[i];
+                    const int place = in_front(n, o, before);
+                    // the k-th; or the last that is kept, and the row's first is always
+                    if (counting ? (u64)place == (u64)k - ahead_here - 1 : !place || (double)(ahead_here + before) < limit) atomicMax(&sh.cut, o);
                 }
             }
             cluster.sync();
@@ -607,9 +724,8 @@ __global__ void __launch_bounds__(CACHED ? kOneThreads : kManyThreads, CACHED ? 
 
     // ---- the kept tokens' weights by tiles of neighbours, a warp to a tile, four tokens to a lane ----
     auto kept_weight = [&](int i, float v) -> u64 {
-        if (v == -INFINITY || order_of(v, at + i) > cut) return 0;
         const double w = weigh.exact(v);
-        return w >= least_weight ? Weigher::units(w) : 0;
+        return v > -INFINITY && order_of(v, at + i) <= cut && w >= least_weight ? Weigher::units(w) : 0;
     };
     const int tiles = (mine + kTile - 1) / kTile;
     auto tile_weights = [&](int t, u64 (&w)[4]) {
@@ -623,9 +739,12 @@ __global__ void __launch_bounds__(CACHED ? kOneThreads : kManyThreads, CACHED ? 
     if (n_few >= 0) {
         for (int t = threadIdx.x; t < tiles; t += kThreads) sh.tile[t] = 0;
         __syncthreads();
-        each([&](int i, float v) {
-            const u64 w = kept_weight(i, v);
-            if (w) atomicAdd(&sh.tile[i / kTile], w);  // (whole numbers: the same sums in any order)
+        each([&](const Places &i, const Logits &v) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const u64 w = kept_weight(i[j], v[j]);
+                if (w) atomicAdd(&sh.tile[i[j] / kTile], w);  // (whole numbers: the same sums in any order)
+            }
         });
     } else {
 #pragma unroll 2
