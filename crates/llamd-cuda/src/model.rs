@@ -296,6 +296,35 @@ impl CudaModelHandle {
         }
     }
 
+    /// The next tokens of the last pass's rows of logits, one for each uniform number in [0, 1), and their shares of the kept weights
+    /// (`llamd_model_sample`; the reference decodes greedily). Settings: one for each row, or `None` for no limit.
+    pub fn sample(&self, uniform: &[f32], temperature: Option<&[f32]>, top_k: Option<&[i32]>, top_p: Option<&[f32]>, min_p: Option<&[f32]>) -> Result<(Vec<i32>, Vec<f32>)> {
+        let n = uniform.len();
+        let short = [temperature.map(<[f32]>::len), top_k.map(<[i32]>::len), top_p.map(<[f32]>::len), min_p.map(<[f32]>::len)];
+        if n == 0 || n > self.max_seq || short.iter().flatten().any(|&len| len != n) {
+            return Err(Error::malformed("sample", format!("{n} rows of {}", self.max_seq)));
+        }
+        #[cfg(not(cuda))]
+        {
+            not_built()
+        }
+        #[cfg(cuda)]
+        {
+            let (mut tokens, mut shares) = (vec![0i32; n], vec![0f32; n]);
+            let f = |x: Option<&[f32]>| x.map_or(std::ptr::null(), <[f32]>::as_ptr);
+            let k = top_k.map_or(std::ptr::null(), <[i32]>::as_ptr);
+            // SAFETY: every slice holds n elements, what the callee reads and writes.
+            #[allow(unsafe_code)]
+            let rc = unsafe {
+                ffi::llamd_model_sample(self.h, n as i32, f(temperature), k, f(top_p), f(min_p), uniform.as_ptr(), tokens.as_mut_ptr(), shares.as_mut_ptr())
+            };
+            if rc != 0 {
+                return Err(Error::other(format!("sample: {}", self.error_text())));
+            }
+            Ok((tokens, shares))
+        }
+    }
+
     /// The logits of the last pass, `nseq` rows of `n_vocab`.
     pub fn logits(&self, nseq: usize) -> Result<Vec<f32>> {
         if nseq == 0 || nseq > self.max_seq {

@@ -13,8 +13,12 @@
 // is cut in bins again, of (logit, index) compared as one number, until kList or fewer are in it, which are sorted. What is kept then, or where min-p is the only limit, is
 // weighed tile by tile of 128 neighbours, and the tile that u falls on looked through.
 // Few rows are kept in shared memory, each looked at there; of many, parts are read again, from L2.
-// What it costs: the row's bytes; four joins of the cluster one behind the other, some eight in the long way; and for rows without a k an exponential in 64 bits for each
-// token, some 20 operations at 64 a clock and SM, for the histogram and, where more than the lists' are kept, for the tiles.
+// What bounds it: one row, the joins of the cluster one behind the other, three with a small k (151936 tokens, k 20: 13.6 us, 31k cycles: the first look 5k, the top 5k, the second look
+// 10k, CTA 0 for itself 11k), some ten in the long way. Many rows without a k, an exponential in 64 bits for each token, some 20 operations at 64 a clock and SM and a conversion at 16, for
+// the histogram and, where more than the lists' are kept, for the tiles: 64 rows of 16 bits with tens of thousands kept 116 us, of whose 175k cycles the histogram takes 50k and the
+// tiles 40k. 128 rows of 151936 f32, each with its own limits, a fifth with k 5000 and a fifth without: 107 us; those with a small k alone are the least of it.
+// CTAs of 256 threads, four to an SM: a batch's rows wait for one another's joins less than with 512 and two (163 us where 246 were). Counting instead of sorting up to a thread to
+// a token, and lists in place of the row once few matter, took 130 to 107.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -31,9 +35,9 @@ typedef unsigned long long u64;
 // threads of a CTA: of one of four to an SM, and of one that has its SM to itself (and its part of the row in shared memory)
 constexpr int kManyThreads = 256, kOneThreads = 1024, kMostWarps = kOneThreads / 32;
 constexpr int kBins = 1024, kList = 1024, kMostCtas = 8, kTile = 128;
-static_assert(kBins % 2 == 0, "bins are read two at a time");
 constexpr int kMostTokens = 393216, kMostPart = 262144;  // of a row; of a CTA (the tiles' sums have room)
 constexpr int kFew = 2560;   // tokens of a CTA's part that may be in its list
+constexpr float kMasked = -9999.0f;  // logits up to it are taken for a mask's, finite ones too: the bins' range does not reach to them, the last bin holds them
 
 struct SampleParams {
     const void *x;
@@ -248,7 +252,7 @@ __global__ void __launch_bounds__(CACHED ? kOneThreads : kManyThreads, CACHED ? 
     if (threadIdx.x == 0) sh.n_list = 0;
     pdl_wait();
 
-    // ---- the first look: the thread's largest logit, the row's top, its least above -inf, how many are ----
+    // ---- the first look: the thread's largest logit, the row's top, its least above a mask's, how many are above -inf ----
     float best = -INFINITY, least = INFINITY;
     int best_at = 0, live = 0;
     from_memory([&](const Places &i, const Logits &v) {
@@ -256,7 +260,7 @@ __global__ void __launch_bounds__(CACHED ? kOneThreads : kManyThreads, CACHED ? 
         for (int j = 0; j < 4; j++) {
             if (CACHED && i[j] < mine) x[i[j]] = v[j];
             if (v[j] > best) best = v[j], best_at = i[j];
-            least = v[j] > -INFINITY ? fminf(least, v[j]) : least;
+            least = v[j] > kMasked ? fminf(least, v[j]) : least;
             live += v[j] > -INFINITY;
         }
     });
@@ -292,11 +296,11 @@ __global__ void __launch_bounds__(CACHED ? kOneThreads : kManyThreads, CACHED ? 
     const int k = k_in > 0 && k_in < live ? k_in : 0;
     const bool by_mass = p_in < 1.0f;
     if (!live || !(temperature > 0.0f)) {  // nothing to choose from; or the first token
+        cluster.sync();  // (nobody leaves while its memory is read, and the settings, which may be where the answers go, have been read by all)
         if (rank == 0 && threadIdx.x == 0) {
             p.token[row] = live ? (int32_t)(uint32_t)first : -1;
             if (p.prob) p.prob[row] = live ? 1.0f : 0.0f;
         }
-        cluster.sync();  // (nobody leaves while its memory is read)
         return;
     }
     const double per_logit = 1.4426950408889634 / (double)temperature;
@@ -314,7 +318,7 @@ __global__ void __launch_bounds__(CACHED ? kOneThreads : kManyThreads, CACHED ? 
     if (k || by_mass) {
         // bins by distance from the top (0 where that has no end: all in one bin), numbers that rise with falling logits; and whether a logit's is at most `bin`
         const float range = top - least, per_bin = range > 0.0f && range < INFINITY ? fminf((kBins - 1) / range, 1e30f) : 0.0f;
-        auto distance = [&](float v) { return per_bin > 0.0f ? (top - v) * per_bin : 0.0f; };
+        auto distance = [&](float v) { return per_bin > 0.0f ? fminf((top - v) * per_bin, 1e30f) : 0.0f; };  // (finite: a mask's too)
         auto bin_of = [&](float v) { return min(kBins - 1, (int)distance(v)); };
         auto bin_end = [&](int bin) { return bin == kBins - 1 ? INFINITY : (float)(bin + 1); };  // the first distance behind it
         // In doubt are tokens of places [low, high]; in front of them are `ahead` tokens or weights that are kept for certain. First the k's end is

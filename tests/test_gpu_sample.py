@@ -138,6 +138,36 @@ def test_numbers_at_the_ends(sampling, u):
     assert np.array_equal(run(sampling, x, [u] * 3)[0], run(sampling, x, [0.0 if not u > 0 else min(u, 1 - 2.0 ** -24)] * 3)[0])
 
 
+def test_finite_masks(sampling):
+    """Masks that are numbers: most of a row far below the rest, all of it, and rows whose own logits are that low."""
+    rng = np.random.default_rng(13)
+    n = 40000
+    for mask in (-1e4, -65504.0, -1e9, -3e38):
+        x = logits(rng, 5, n)
+        x[:, rng.random(n) < 0.9] = mask
+        x[3] = mask
+        x[4] = x[4] + np.float32(-2e4)
+        for rule in (dict(), dict(top_k=20, top_p=0.9), dict(top_k=3000), dict(top_p=0.95), dict(min_p=0.1)):
+            check(sampling, x, rng.random(5), **rule)
+            if mask == -65504.0:
+                check(sampling, np.maximum(x, mask), rng.random(5), "f16", **rule)
+
+
+def test_answers_over_settings(sampling):
+    """Tokens written where k was, shares where the temperature was: each row's settings have been read by then."""
+    from llamd_rs_b200 import backend
+
+    rng = np.random.default_rng(14)
+    rows, n = 24, 50000
+    x, u, t = logits(rng, rows, n), rng.random(rows).astype(np.float32), rng.choice([0.0, 0.7, 1.5], rows).astype(np.float32)
+    k = rng.choice([0, 1, 30, 2000], rows).astype(np.int32)
+    dx, du, dt, dk = dev(x), dev(u), dev(t), dev(k)
+    sampling.sample(dx, du, dk, temperature=dt, top_k=dk, prob=dt, rows=rows, n_vocab=n)
+    backend.sync()
+    want = [plain.sample(x[r], u[r], t[r], k[r])[0] for r in range(rows)]
+    assert dk.download(np.int32, rows).tolist() == want
+
+
 def test_settings_beyond_their_ranges(sampling):
     rng = np.random.default_rng(12)
     x, u = logits(rng, 6, 5000), rng.random(6)
