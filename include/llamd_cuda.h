@@ -460,7 +460,8 @@ void *llamd_cuda_paged_new(int n_head, int n_head_kv, int hd, int page_size, int
 #define LLAMD_PAGED_I8 3
 #define LLAMD_PAGED_E4M3 4
 /* As above; type is q_out's and out's, cache one of the two. Set and freed as above; goes with append8 and attention8 only, as a batch of the former with
- * append and attention only. */
+ * append and attention only. Where sequences have many new tokens, llamd_cuda_paged_set also takes device memory for the pages that those read in 16 bits, 4 hd n_head_kv
+ * page_size bytes each, for one layer at a time; it fails where there is none. */
 void *llamd_cuda_paged_new8(int n_head, int n_head_kv, int hd, int page_size, int type, int cache);
 /* Launches that read the batch may still be under way, a graph may be captured meanwhile: nothing is waited for. The library keeps the batch's memory (up to
  * 512 MB on the device, 256 MB pinned) for the next ones. Any thread. */

@@ -203,7 +203,7 @@ void launch_types(AppendParams &p, const Append8 &a, int cache, bool interleaved
 
 }  // namespace
 
-// One launch while its warps run all at once; beyond that the queries, which need half the registers, by themselves: 8511 tokens of f16, 32 heads over 4 of
+// One launch while its warps run all at once; beyond that the queries, which need half the registers, by themselves: 8450 tokens of f16, 32 heads over 4 of
 // 128, 42 us in two launches (the queries 28), 52 in one, 45 in one with twice as many heads to a warp, 45 in two at the same time on two streams.
 bool paged_append8_apart(const AppendParams &p, const Append8 &a) {
     return (long long)p.b.tokens * p.b.n_head / 8 + 2LL * a.n_blocks * p.b.n_head_kv > 16LL * kAppend8Ctas * p.sms;
