@@ -73,6 +73,22 @@ def _stream_of(*buffers):
     return None
 
 
+def _one_device(*buffers):
+    """Refuses tensors that are not all on the current device: the library has that one, and another's memory may be out of a kernel's reach."""
+    here = None
+    for x in buffers:
+        if hasattr(x, "get_device"):
+            if here is None:
+                here = x.get_device()
+            if x.get_device() != here:
+                raise ShapeError(f"tensors on devices {here} and {x.get_device()}")
+    if here is not None:
+        torch = sys.modules["torch"]
+        current = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)()
+        if here != current:
+            raise ShapeError(f"tensors on device {here} where {current} is the current one")
+
+
 def _refuse(what):
     """The last call's own refusal as an error, read so that the next call starts clean."""
     why = backend._last_error() or what
@@ -272,7 +288,7 @@ class Batch:
             rope_rows = _int(rope_rows, "rope_rows")
         D, T, t, c = self.head_dim, self.tokens, self.type, self.cache
         nq, nk = self.n_head * D, self.n_head_kv * D
-        scales = () if c == t and k_scales is None and v_scales is None else self._scales_of(k_scales, v_scales)
+        scales = () if c == t and k_scales is None and v_scales is None else self._scales_of(k_scales, v_scales, q, k, v, q_out, k_pages, v_pages, rope, q_norm, k_norm)
         if rot and q_norm is not None and k_norm is not None:
             plain = self._tensors((q, it, T * nq, T), (k, it, T * nk, T), (v, it, T * nk, T), (q_norm, 2, D, None), (k_norm, 2, D, None),
                                   (rope, 2, rope_rows * rot, None), (q_out, t, T * nq, T), (k_pages, c, self._pool, None), (v_pages, c, self._pool, None))
@@ -289,14 +305,15 @@ class Batch:
                    self._whole(rope, 2, rope_rows * rot, "rope") if rot else None, rope_rows, rot, interleaved, op, os_,
                    self._whole(k_pages, c, self._pool, "k_pages"), self._whole(v_pages, c, self._pool, "v_pages"), *scales)
 
-    def _scales_of(self, k_scales, v_scales):
-        """The addresses of a cache's scales where it is in 8 bits."""
+    def _scales_of(self, k_scales, v_scales, *others):
+        """The addresses of a cache's scales where it is in 8 bits; they and the call's other buffers are then looked at for their device."""
         if self.cache == self.type:
             if k_scales is not None or v_scales is not None:
                 raise Malformed("scales of a cache that is not in 8 bits")
             return ()
         if k_scales is None or v_scales is None:
             raise Malformed("a cache in 8 bits without its scales")
+        _one_device(k_scales, v_scales, *others)
         n = self._pool // (SCALE_BLOCK * self.head_dim)
         return self._tensors((k_scales, _SCALES, n, None), (v_scales, _SCALES, n, None)) or (self._whole(k_scales, _SCALES, n, "k_scales"), self._whole(v_scales, _SCALES, n, "v_scales"))
 
@@ -307,7 +324,7 @@ class Batch:
         n = self.n_head * self.head_dim
         scale = self.scale if scale is None else scale
         c = self.cache
-        scales = () if c == self.type and k_scales is None and v_scales is None else self._scales_of(k_scales, v_scales)
+        scales = () if c == self.type and k_scales is None and v_scales is None else self._scales_of(k_scales, v_scales, q, k_pages, v_pages, out)
         plain = self._tensors((q, self.type, self.tokens * n, self.tokens), (k_pages, c, self._pool, None), (v_pages, c, self._pool, None),
                               (out, 2 if out_f32 else self.type, self.tokens * n, self.tokens))
         if plain:

@@ -50,6 +50,50 @@ def test_scales_of_a_batch(built):
         b._scales_of(1 << 20, 1 << 20)
 
 
+class OnDevice:
+    """As much of a tensor as is looked at before an address is taken."""
+
+    is_cuda = True
+
+    def __init__(self, x, device):
+        self.x, self.device = x, device
+
+    def get_device(self):
+        return self.device
+
+    def __getattr__(self, name):
+        return getattr(self.x, name)
+
+
+def test_one_device(built):
+    """Tensors of two devices, or of one that is not the current one, are refused before anything is enqueued."""
+    backend, paged, sampling = built
+    torch = pytest.importorskip("torch")
+    f, i = (lambda n, d: OnDevice(torch.zeros(n), d)), (lambda n, d: OnDevice(torch.zeros(n, dtype=torch.int32), d))
+    rows = OnDevice(torch.zeros(2, 10), 0)
+    for kw in (dict(uniform=f(2, 1), token=i(2, 0)), dict(uniform=f(2, 0), token=i(2, 1)), dict(uniform=f(2, 0), token=i(2, 0), top_k=i(2, 1)),
+               dict(uniform=f(2, 0), token=i(2, 0), prob=f(2, 1))):
+        with pytest.raises(backend.ShapeError, match="devices 0 and 1"):
+            sampling.sample(rows, **kw)
+    b = paged.Batch.__new__(paged.Batch)
+    b.ptr, b.type, b.cache, b._pool, b.head_dim = None, 0, 3, 4 * 2 * 16 * 64, 64
+    scales = lambda d: OnDevice(torch.zeros(4, 2, 1, dtype=torch.uint8), d)  # noqa: E731
+    with pytest.raises(backend.ShapeError, match="devices 0 and 1"):
+        b._scales_of(scales(0), scales(1))
+    with pytest.raises(backend.ShapeError, match="devices 0 and 1"):
+        b._scales_of(scales(0), scales(0), None, f(8, 1))
+    paged._one_device(None, 1 << 20)  # (addresses are the caller's word)
+
+
+def test_current_device(built, monkeypatch):
+    backend, paged, _ = built
+    torch = pytest.importorskip("torch")
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    paged._one_device(OnDevice(torch.zeros(2), 0))
+    with pytest.raises(backend.ShapeError, match="device 1 where 0"):
+        paged._one_device(OnDevice(torch.zeros(2), 1), OnDevice(torch.zeros(2), 1))
+
+
 def test_refused_without_a_device(built):
     backend, paged, _ = built
     if backend.available():
