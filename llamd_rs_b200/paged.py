@@ -77,16 +77,29 @@ def _one_device(*buffers):
     """Refuses tensors that are not all on the current device: the library has that one, and another's memory may be out of a kernel's reach."""
     here = None
     for x in buffers:
-        if hasattr(x, "get_device"):
-            if here is None:
-                here = x.get_device()
-            if x.get_device() != here:
-                raise ShapeError(f"tensors on devices {here} and {x.get_device()}")
+        if x is not None and hasattr(x, "get_device"):
+            at = x.get_device()
+            if at != here:
+                if here is not None:
+                    raise ShapeError(f"tensors on devices {here} and {at}")
+                here = at
     if here is not None:
         torch = sys.modules["torch"]
         current = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)()
         if here != current:
             raise ShapeError(f"tensors on device {here} where {current} is the current one")
+
+
+def _stream_here(x):
+    """_stream_of a tensor that is to be on the current device."""
+    c, at = sys.modules["torch"]._C, x.get_device()
+    try:
+        if at == c._cuda_getDevice():
+            return c._cuda_getCurrentRawStream(at)
+    except AttributeError:
+        pass
+    _one_device(x)
+    return _stream_of(x)
 
 
 def _refuse(what):
@@ -214,11 +227,13 @@ class Batch:
 
     @staticmethod
     def _tensors(*wanted):
-        """The addresses of (tensor, type, values at least, rows) that are all as plain as can be, or None: then each is looked at for itself."""
-        found = []
+        """The addresses of (tensor, type, values at least, rows) that are all as plain as can be and on one device, or None: then each is looked at for itself."""
+        found, device = [], wanted[0][0].get_device() if hasattr(wanted[0][0], "get_device") else -1
+        if device < 0:
+            return None
         try:
             for x, type_, n, rows in wanted:
-                if _seen.get(x.dtype) != type_ or not x.is_cuda or not x.is_contiguous() or x.numel() < n or (rows is not None and (x.shape[0] != rows or x.numel() != n)):
+                if _seen.get(x.dtype) != type_ or x.get_device() != device or not x.is_contiguous() or x.numel() < n or (rows is not None and (x.shape[0] != rows or x.numel() != n)):
                     return None
                 found.append(x.data_ptr())
         except (AttributeError, IndexError):
@@ -288,14 +303,27 @@ class Batch:
             rope_rows = _int(rope_rows, "rope_rows")
         D, T, t, c = self.head_dim, self.tokens, self.type, self.cache
         nq, nk = self.n_head * D, self.n_head_kv * D
-        scales = () if c == t and k_scales is None and v_scales is None else self._scales_of(k_scales, v_scales, q, k, v, q_out, k_pages, v_pages, rope, q_norm, k_norm)
+        eight = c != t or k_scales is not None or v_scales is not None
+        if eight:
+            n_scales = self._scales_given(k_scales, v_scales)
         if rot and q_norm is not None and k_norm is not None:
-            plain = self._tensors((q, it, T * nq, T), (k, it, T * nk, T), (v, it, T * nk, T), (q_norm, 2, D, None), (k_norm, 2, D, None),
-                                  (rope, 2, rope_rows * rot, None), (q_out, t, T * nq, T), (k_pages, c, self._pool, None), (v_pages, c, self._pool, None))
+            plain = (self._tensors((q, it, T * nq, T), (k, it, T * nk, T), (v, it, T * nk, T), (q_norm, 2, D, None), (k_norm, 2, D, None),
+                                   (rope, 2, rope_rows * rot, None), (q_out, t, T * nq, T), (k_pages, t, self._pool, None), (v_pages, t, self._pool, None)) if not eight else
+                     self._tensors((q, it, T * nq, T), (k, it, T * nk, T), (v, it, T * nk, T), (q_norm, 2, D, None), (k_norm, 2, D, None),
+                                   (rope, 2, rope_rows * rot, None), (q_out, t, T * nq, T), (k_pages, c, self._pool, None), (v_pages, c, self._pool, None),
+                                   (k_scales, _SCALES, n_scales, None), (v_scales, _SCALES, n_scales, None)))
+            if plain and eight:
+                self._call("append", self._append, _stream_here(q), plain[0], plain[1], plain[2], it, nq, nk, nk, plain[3], plain[4], eps, plain[5], rope_rows, rot,
+                           interleaved, plain[6], nq, plain[7], plain[8], plain[9], plain[10])
+                return
             if plain:
                 self._call("append", self._append, _stream_of(q), plain[0], plain[1], plain[2], it, nq, nk, nk, plain[3], plain[4], eps, plain[5], rope_rows, rot,
-                           interleaved, plain[6], nq, plain[7], plain[8], *scales)
+                           interleaved, plain[6], nq, plain[7], plain[8])
                 return
+        scales = ()
+        if eight:
+            _one_device(q, k, v, q_out, k_pages, v_pages, rope, q_norm, k_norm, k_scales, v_scales)
+            scales = self._scales_of(k_scales, v_scales)
         qp, qs = self._rows(q, nq, it, "q", strides[0])
         kp, ks = self._rows(k, nk, it, "k", strides[1])
         vp, vs = self._rows(v, nk, it, "v", strides[2])
@@ -305,17 +333,20 @@ class Batch:
                    self._whole(rope, 2, rope_rows * rot, "rope") if rot else None, rope_rows, rot, interleaved, op, os_,
                    self._whole(k_pages, c, self._pool, "k_pages"), self._whole(v_pages, c, self._pool, "v_pages"), *scales)
 
-    def _scales_of(self, k_scales, v_scales, *others):
-        """The addresses of a cache's scales where it is in 8 bits; they and the call's other buffers are then looked at for their device."""
+    def _scales_given(self, k_scales, v_scales):
+        """How many scales a pool has of a cache in 8 bits; refused where they are missing, or the cache is not."""
         if self.cache == self.type:
-            if k_scales is not None or v_scales is not None:
-                raise Malformed("scales of a cache that is not in 8 bits")
-            return ()
+            raise Malformed("scales of a cache that is not in 8 bits")
         if k_scales is None or v_scales is None:
             raise Malformed("a cache in 8 bits without its scales")
-        _one_device(k_scales, v_scales, *others)
-        n = self._pool // (SCALE_BLOCK * self.head_dim)
-        return self._tensors((k_scales, _SCALES, n, None), (v_scales, _SCALES, n, None)) or (self._whole(k_scales, _SCALES, n, "k_scales"), self._whole(v_scales, _SCALES, n, "v_scales"))
+        return self._pool // (SCALE_BLOCK * self.head_dim)
+
+    def _scales_of(self, k_scales, v_scales):
+        """The scales' addresses where the cache is in 8 bits."""
+        if self.cache == self.type and k_scales is None and v_scales is None:
+            return ()
+        n = self._scales_given(k_scales, v_scales)
+        return self._whole(k_scales, _SCALES, n, "k_scales"), self._whole(v_scales, _SCALES, n, "v_scales")
 
     def attention(self, q, k_pages, v_pages, out, scale: float | None = None, out_f32: bool | None = None, k_scales=None, v_scales=None) -> None:
         """llamd_fwd_paged_attention, or _attention8 with the scales of a cache in 8 bits. ``out_f32`` says of an address that it takes f32; a tensor's type says so itself."""
@@ -324,12 +355,22 @@ class Batch:
         n = self.n_head * self.head_dim
         scale = self.scale if scale is None else scale
         c = self.cache
-        scales = () if c == self.type and k_scales is None and v_scales is None else self._scales_of(k_scales, v_scales, q, k_pages, v_pages, out)
-        plain = self._tensors((q, self.type, self.tokens * n, self.tokens), (k_pages, c, self._pool, None), (v_pages, c, self._pool, None),
-                              (out, 2 if out_f32 else self.type, self.tokens * n, self.tokens))
-        if plain:
-            self._call("attention", self._attention, _stream_of(q), plain[0], n, plain[1], plain[2], *scales, plain[3], n, out_f32, scale)
-            return
+        if c != self.type or k_scales is not None or v_scales is not None:
+            n_scales = self._scales_given(k_scales, v_scales)
+            plain = self._tensors((q, self.type, self.tokens * n, self.tokens), (k_pages, c, self._pool, None), (v_pages, c, self._pool, None),
+                                  (out, 2 if out_f32 else self.type, self.tokens * n, self.tokens), (k_scales, _SCALES, n_scales, None), (v_scales, _SCALES, n_scales, None))
+            if plain:
+                self._call("attention", self._attention, _stream_here(q), plain[0], n, plain[1], plain[2], plain[4], plain[5], plain[3], n, out_f32, scale)
+                return
+            _one_device(q, k_pages, v_pages, out, k_scales, v_scales)
+            scales = self._scales_of(k_scales, v_scales)
+        else:
+            plain = self._tensors((q, self.type, self.tokens * n, self.tokens), (k_pages, self.type, self._pool, None), (v_pages, self.type, self._pool, None),
+                                  (out, 2 if out_f32 else self.type, self.tokens * n, self.tokens))
+            if plain:
+                self._call("attention", self._attention, _stream_of(q), plain[0], n, plain[1], plain[2], plain[3], n, out_f32, scale)
+                return
+            scales = ()
         qp, qs = self._rows(q, n, self.type, "q")
         op, os_ = self._rows(out, n, 2 if out_f32 else self.type, "out")
         kp, vp = self._whole(k_pages, c, self._pool, "k_pages"), self._whole(v_pages, c, self._pool, "v_pages")

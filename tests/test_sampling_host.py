@@ -78,10 +78,21 @@ def test_one_device(built):
     b = paged.Batch.__new__(paged.Batch)
     b.ptr, b.type, b.cache, b._pool, b.head_dim = None, 0, 3, 4 * 2 * 16 * 64, 64
     scales = lambda d: OnDevice(torch.zeros(4, 2, 1, dtype=torch.uint8), d)  # noqa: E731
-    with pytest.raises(backend.ShapeError, match="devices 0 and 1"):
-        b._scales_of(scales(0), scales(1))
-    with pytest.raises(backend.ShapeError, match="devices 0 and 1"):
-        b._scales_of(scales(0), scales(0), None, f(8, 1))
+    b.tokens, b.n_head, b.n_head_kv, b.scale = 1, 8, 2, 0.125
+    b._wait = b._ready = b._attention = b._append = None  # (nothing is called)
+    codes = lambda d: OnDevice(torch.zeros(b._pool, dtype=torch.int8), d)  # noqa: E731
+    paged._type_of(codes(0)), paged._type_of(scales(0))
+    wanted = lambda d: ((codes(0), 3, b._pool, None), (codes(d), 3, b._pool, None))  # noqa: E731
+    assert len(paged.Batch._tensors(*wanted(0))) == 2 and paged.Batch._tensors(*wanted(1)) is None
+    for d in range(1, 64):
+        q, kp, vp, out, ks, vs = (make(d >> i & 1) for i, make in enumerate((lambda d: OnDevice(torch.zeros(1, 512, dtype=torch.float16), d), codes, codes,
+                                                                             lambda d: OnDevice(torch.zeros(1, 512), d), scales, scales)))
+        if d < 63:
+            with pytest.raises(backend.ShapeError, match="devices [01] and [01]"):
+                b.attention(q, kp, vp, out, k_scales=ks, v_scales=vs)
+        if d & 55 not in (0, 55):  # (all but `out`)
+            with pytest.raises(backend.ShapeError, match="devices [01] and [01]"):
+                b.append(q, q, q, q, kp, vp, k_scales=ks, v_scales=vs, inputs="f16")
     paged._one_device(None, 1 << 20)  # (addresses are the caller's word)
 
 
