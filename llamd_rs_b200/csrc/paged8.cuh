@@ -1,6 +1,6 @@
 // K/V caches in 8 bits: a page's rows are codes, and each 16 neighbouring positions of a page and kv head have one scale 2^e, kept as the byte e + 127
 // ([n_pages][n_head_kv][page / 16]). A value is its code times the scale. With powers of two every value is exact in f16 and bf16, and codes that are
-// taken to a larger scale are rounded once, whatever their history; they cost at most one of an i8 code's 8 bits, and nothing of e4m3's.
+// taken to a larger scale lose bits at their end only (e4m3 none but of what becomes subnormal); they cost at most one of an i8 code's 8 bits, and nothing of e4m3's.
 #pragma once
 #include "paged.cuh"
 
