@@ -49,19 +49,28 @@ struct SampleParams {
     float *prob;
 };
 
-// What the cluster's CTAs tell one another; what is the row's own is read from CTA 0.
+// What the cluster's CTAs tell one another; what is the row's own is read from CTA 0. A field that others read is written again only behind a join of the cluster that
+// comes after their reads:
+//   first, part_least, part_count   written once, in front of the first join
+//   hist, digit, list               CTA 0 reads all CTAs', between two joins
+//   part_low, part_high, mass       read between two joins
+//   n_list                          every warp reads all CTAs', from the join behind a look on; written in front of the next look, joins later
+//   bin, before, total              read from the join that ends find to the one behind the look that follows; CTA 0's own from there to the next find
+//   cut                             read from a round's last join on; written behind the next look's
 struct Shared {
+    // the CTA's own
     u64 scratch[kMostWarps];
     u64 low[kMostWarps], high[kMostWarps];
     int count[kMostWarps];
     float least[kMostWarps];
-    // of this CTA
+    int n_few, n_left;  // n_left: CTA 0's list while it narrows it, where late warps of the row may still be reading n_list
+    // what others read of every CTA
     u64 first, mass, part_low, part_high;
     float part_least;
-    int part_count;
+    int part_count, n_list;
     // of the row (CTA 0)
     u64 total, before, cut;
-    int bin, n_list, n_few;
+    int bin;
     alignas(16) uint32_t hist[kBins];
     union {
         alignas(16) uint32_t digit[2][kBins];  // the bins' weights: the sums' low 32 bits, and what is above them
@@ -685,7 +694,7 @@ __global__ void __launch_bounds__(CACHED ? kOneThreads : kManyThreads, CACHED ? 
                     for (int j = 0; j < kPer; j++)
                         if (threadIdx.x < kBins / kPer) c[j] = sh.hist[threadIdx.x * kPer + j], w[j] = counting ? c[j] : low_words[threadIdx.x * kPer + j] | (u64)high_words[threadIdx.x * kPer + j] << 32, m += w[j];
                     m = block_prefix<kThreads>(m, sh.scratch, all);
-                    if (threadIdx.x == 0) sh.n_list = 0;
+                    if (threadIdx.x == 0) sh.n_left = 0;
 #pragma unroll
                     for (int j = 0; j < kPer; j++) {
                         const bool here = counting ? ahead_here + m < (u64)k && ahead_here + m + c[j] >= (u64)k
@@ -698,9 +707,9 @@ __global__ void __launch_bounds__(CACHED ? kOneThreads : kManyThreads, CACHED ? 
                     ahead_here = sh.before;
 #pragma unroll
                     for (int j = 0; j < kEach; j++)
-                        if (threadIdx.x + j * kThreads < n && (int)((o[j] - lo) >> shift) == b) sh.list[atomicAdd(&sh.n_list, 1)] = o[j];
+                        if (threadIdx.x + j * kThreads < n && (int)((o[j] - lo) >> shift) == b) sh.list[atomicAdd(&sh.n_left, 1)] = o[j];
                     __syncthreads();
-                    n = sh.n_list;
+                    n = sh.n_left;
                     __syncthreads();
                 }
                 if (!counting)
