@@ -4,8 +4,11 @@
 //
 // Half the bytes bound it: 2 hd + 2 / 16 per position and kv head. Codes become f16 in registers, exactly, so both products are f16 whatever the batch's type; a bf16
 // row of q is brought to f16 by a power of two of its own (what falls into the subnormals is below 2^-30 of the row's largest). A scale block's K scale multiplies its
-// scores. Its V scale goes into the weights: with lV = eV and m about the maximum of s + lV so far, sums of w cV, w = 2^(s + lV - m), are the numerator and sums of
-// w 2^-eV the denominator, in f32, whatever the scales.
+// scores, its V scale the codes: 2^eV cV is in f16 too, with every scale of an append's, so that an output is off by the rounding of the weights 2^(s - m) alone, whatever other
+// blocks' scales are. In i8 the bias that is taken off a code goes times the scale in the same instruction; 1152 2^e is in f16 up to e = 5, and the up to 2^4 above go
+// into the block's weights, as whatever a scale has beyond an append's does: m is about the maximum of s + r, r that rest of log2 of the V scale, and the
+// denominator sums 2^(s + r - m) 2^-r in f32. (The whole scale in the weights was as fast, 148 sequences of 4096 positions 102 to 105 us either way, 256 behind 4096
+// shared ones 56.2 and 57.4, but a block with one large element then cost the other blocks' weights their bits, from 2^26 between scales on.)
 //
 // Which codes a lane holds as the products' first operand is free as long as the second follows. K: 16 bytes of rows g and g + 8 (g = lane / 4, t = lane % 4) are the
 // contraction's elements of four steps; q is read in the same order. V: hd / 8 bytes of rows 2t, 2t + 1, 2t + 8, 2t + 9; bytes of two rows
@@ -179,6 +182,7 @@ __global__ void __launch_bounds__(kWarps * 32, kDecode8Ctas) paged_decode8_kerne
                 e_k[b] = __shfl_sync(0xffffffffu, (i >> 4) == newest ? k_scale : k_before, (i & 15) * 2 + b);
                 e_v[b] = __shfl_sync(0xffffffffu, (i >> 4) == newest ? v_scale : v_before, (i & 15) * 2 + b);
             }
+            const Times<C> of_v[kBlocks] = {Times<C>(e_v[0]), Times<C>(e_v[1])};
             fetch(i + kStages - 1);  // into the stage that the slice before this one has left
             const uint32_t kt = my_ring + (uint32_t)(i % kStages) * Tl::kBytes, vt = kt + Tl::kK;
             float s[kBlocks][NT][4];
@@ -213,7 +217,7 @@ __global__ void __launch_bounds__(kWarps * 32, kDecode8Ctas) paged_decode8_kerne
                     top[n][e] = -INFINITY;
 #pragma unroll
                     for (int b = 0; b < kBlocks; b++) {
-                        const float by = scale[n][e] * scale_of(e_k[b]), l_v = (float)(e_v[b] - 127);
+                        const float by = scale[n][e] * scale_of(e_k[b]), l_v = (float)(of_v[b].rest - 127);
                         s[b][n][e] = pos + b * kScaleBlock < last[n][e] ? fmaf(s[b][n][e], by, l_v) : -INFINITY;
                         s[b][n][e + 2] = pos + b * kScaleBlock + 8 < last[n][e] ? fmaf(s[b][n][e + 2], by, l_v) : -INFINITY;
                         top[n][e] = fmaxf(top[n][e], fmaxf(s[b][n][e], s[b][n][e + 2]));
@@ -238,7 +242,7 @@ __global__ void __launch_bounds__(kWarps * 32, kDecode8Ctas) paged_decode8_kerne
             uint32_t w[kBlocks][NT][2];
 #pragma unroll
             for (int b = 0; b < kBlocks; b++) {
-                const float by_v = scale_inverse(e_v[b]);
+                const float by_v = scale_inverse(of_v[b].rest);
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
                     float x[4];
@@ -248,7 +252,7 @@ __global__ void __launch_bounds__(kWarps * 32, kDecode8Ctas) paged_decode8_kerne
                         x[e] = exp2_fast(s[b][n][e] - at), x[e + 2] = exp2_fast(s[b][n][e + 2] - at);
                         sum[n][e] = fmaf(x[e] + x[e + 2], by_v, sum[n][e]);
                     }
-                    // rounded to f16 for the second product: relative 2^-12, no more than the output itself will be
+                    // rounded to f16 for the second product: relative 2^-11 at most down to 2^-26 of the largest weight, by 2^-37 of that below (i8 with scales above 2^5: 2^-22, 2^-33)
                     w[b][n][0] = transpose8(Half16<__half>::pack(x[0], x[1]));
                     w[b][n][1] = transpose8(Half16<__half>::pack(x[2], x[3]));
                 }
@@ -272,7 +276,7 @@ __global__ void __launch_bounds__(kWarps * 32, kDecode8Ctas) paged_decode8_kerne
 #pragma unroll
                     for (int h = 0; h < 2; h++) {  // bytes 2h, 2h + 1: this lane's two rows of product 2x + h
                         const uint32_t lo = __byte_perm(v[0][x], v[1][x], h ? 0x7362 : 0x5140), hi = __byte_perm(v[2][x], v[3][x], h ? 0x7362 : 0x5140);
-                        const uint32_t a[4] = {Cv::template f16x2<0>(lo), Cv::template f16x2<1>(lo), Cv::template f16x2<0>(hi), Cv::template f16x2<1>(hi)};
+                        const uint32_t a[4] = {Cv::template f16x2<0>(lo, of_v[b]), Cv::template f16x2<1>(lo, of_v[b]), Cv::template f16x2<0>(hi, of_v[b]), Cv::template f16x2<1>(hi, of_v[b])};
 #pragma unroll
                         for (int n = 0; n < NT; n++) mma16816<__half>(o[2 * x + h][n], a, w[b][n][0], w[b][n][1]);
                     }
