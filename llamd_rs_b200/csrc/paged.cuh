@@ -30,7 +30,7 @@ void paged_decode_launch(const PagedAttn &p, int type, int n_items, int max_rows
 void paged_decode8_launch(const PagedAttn &p, int type, int cache, const int32_t *begin, int n_ctas, int max_rows, cudaStream_t to);  // begin: each CTA's pieces, of every kv head
 bool paged_gave_up();       // a wait of an earlier attention has run out, and the host has not read it yet
 bool paged_prompt_ready();  // what its launches need beside the batch: false and an error where it cannot be had
-// The pages of a cache in 8 bits that paged_prompt.cu reads, and where their 16-bit values go: page i of the list is page i of k_out and v_out.
+// The pages of a cache in 8 bits that paged_prompt.cu reads, and where their 16-bit values go: page i of the list is page i of k_out, in the batch's type, and v_out, in f16.
 struct PagedWiden {
     const PagedWide *page;
     int n_pages, page_size, rows, chunks;  // rows (heads x positions) of a page, 16-byte pieces of a row of codes

@@ -90,3 +90,13 @@ def test_scales_far_apart(paged, cache, dtype, H, K, D, q_len, kv_len, n_shared)
     """Few query rows; V's scales as far apart as an append makes them, in different elements: an element's error is in proportion to what that element is made of."""
     for ahead in (0.0, 5.0, 10.0):
         compare(paged, cache, H, K, D, dtype, q_len, kv_len, far_apart(cache, dtype, ahead), FEW[cache], n_shared)
+
+
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("H,K,D,q_len,kv_len,n_shared", [(8, 1, 128, [70], [300], 0), (4, 2, 64, [257, 60], [257, 1000], 0), (32, 4, 128, [600], [600], 0), (8, 1, 64, [100], [9000], 0),
+                                                         (32, 4, 128, [1] * 40, [1700 + i for i in range(40)], 1696)])
+def test_many_rows(paged, cache, dtype, H, K, D, q_len, kv_len, n_shared):
+    """The kernel of many query rows, of either type: weights and V in f16, as in that of few."""
+    for edit in (None, far_apart(cache, dtype, 0.0), far_apart(cache, dtype, 5.0)):
+        compare(paged, cache, H, K, D, dtype, q_len, kv_len, edit, max(2.0 ** -32, FEW[cache]), n_shared)
