@@ -277,7 +277,8 @@ void llamd_fwd_argmax(const float *x, int n, float *scratch_v, int32_t *scratch_
  * first top_k (0 and less: all), of those the ones whose predecessors weigh less than top_p times the k's together (1 and more: all; the first always is), of those the ones
  * that weigh min_p of the first's or more. token[r]: by rising index the first at which the kept weights up to it are more than uniform times all of
  * them; prob[r] (may be NULL): its share of them. A temperature that is not above 0: the first token, share 1. NaN logits count as -inf; a row with nothing else: -1
- * and 0. Weights are taken in whole multiples of 2^-40 of the first's and summed exactly: the same token every time. n_vocab up to 393216. Numbers outside their range are
+ * and 0. Weights, right to 2^-36 of themselves, are taken in whole multiples of 2^-40 of the first's and summed exactly: the same token every time, and another than the exact
+ * one only where uniform is that near to a border, n 2^-41 for n kept tokens included. n_vocab up to 393216. Numbers outside their range are
  * brought to its ends (a NaN limits nothing, and as a uniform number is 0). Enqueues; 0, or -1 and a message where refused, and nothing was launched. */
 int llamd_fwd_sample(const void *logits, int type, size_t stride, int rows, int n_vocab, const float *temperature, const int32_t *top_k,
                      const float *top_p, const float *min_p, const float *uniform, int32_t *token, float *prob);

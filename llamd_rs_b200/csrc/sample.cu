@@ -4,8 +4,9 @@
 //   kept: the first k; of those the ones whose predecessors weigh less than p times the k's; of those the ones with w_i >= m
 //   token: by rising index the first at which the kept weights up to it are more than u times all of them
 //
-// Every weight is a whole multiple of 2^-40 (from an exponential in 64 bits, off by 2^-37 of itself), so that sums are exact and the same in whatever order they are made, and a
-// token is another than in exact arithmetic only where u falls within some 2^-40 of a border.
+// Every weight is a whole multiple of 2^-40 of the first's (from an exponential in 64 bits, off by 2^-36.6 of itself), so that sums are exact and the same in whatever order
+// they are made. n kept weights of W first ones in all are off by 2^-36.6 W + n 2^-41 at most together: a token is another than in exact arithmetic only where u is within
+// 2^-36.6 + n 2^-41 / W of a border, 2^-23.8 for 151936 tokens beside one that outweighs them all. Where top_p's share ends, the same.
 //
 // A row belongs to a cluster of 1 to 8 CTAs. The first look at it finds its top, and every thread's largest logit. With a small k: what is at least the k-th largest of those is
 // k tokens and little more; they are gathered in a second look, and one CTA sorts them and settles the row. Else, or where they are too many, a histogram of all logits (kBins
@@ -95,7 +96,8 @@ __device__ __forceinline__ float logit_of(u64 order) {
     return __uint_as_float(b & 0x80000000u ? b : ~b & 0x7FFFFFFFu);
 }
 
-// 2^y for y <= 0 in units of 2^-40, rounded, and as it is: y = n + f, |f| <= 1/2, the exponential's series up to f^9 (the next term is below 2^-37)
+// 2^y for y <= 0 in units of 2^-40, rounded, and as it is: y = n + f, |f| <= 1/2, the exponential's series up to f^9 (off by 2^-36.6 of the weight at
+// f = -1/2, where the next term is 2^-37.1 and its sum 2^-1/2)
 struct Weigher {
     double max, per;  // log2 e / T
     float top, per32;

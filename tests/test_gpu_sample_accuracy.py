@@ -1,0 +1,48 @@
+"""Sampling against a softmax whose weights are not rounded: how near to a border a number has to be for another token to come out, and weights over the whole range of
+temperatures and logits."""
+import numpy as np
+import pytest
+
+import sample_plain as plain
+from test_gpu_sample import logits, run, sampling  # noqa: F401  (sampling: the fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+def near(sampling, x, u, **settings):
+    """The token's own stretch of [0, 1), in 80 bits, is no further from u than what the weights' errors move its ends, and its share no further from the exact one. A
+    weight is off by 2^-36.6 of itself (the series up to f^9, |f| <= 1/2: (ln 2 / 2)^10 / 10! 2^(1/2)) and by a rounding to multiples of 2^-40 of the first's, 2^-41. With n weights of W in all, in
+    units of the first's, a sum of some of them and of all are off by e = 2^-36.6 W + n 2^-41 at most, together, so their quotient by e / (W - e)."""
+    got, share = run(sampling, x, u, **settings)
+    for r, row in enumerate(x):
+        T = np.longdouble(np.float32(settings.get("temperature", 1.0)))
+        order = np.argsort(-row.astype(np.float64), kind="stable")
+        order = np.sort(order[:settings["top_k"]]) if settings.get("top_k", 0) > 0 else np.arange(len(row))
+        w = np.exp((row[order].astype(np.longdouble) - np.longdouble(row.max())) / T)
+        W, n = w.sum(), len(w)
+        e = 2.0 ** -36.6 * W + n * 2.0 ** -41
+        e = float(e / (W - e)) + n * 2.0 ** -63
+        at = int(np.flatnonzero(order == got[r])[0])
+        end = w[:at + 1].sum() / W
+        begin = end - w[at] / W
+        assert begin - e <= u[r] < end + e, (r, float(begin), float(end), u[r], e)
+        assert abs(share[r] - w[at] / W) <= 2.0 ** -23 * w[at] / W + e
+    return got
+
+
+@pytest.mark.parametrize("n", [40, 5000, 151936])
+def test_near_a_border(sampling, n):  # noqa: F811
+    rng = np.random.default_rng(n)
+    for spread in (0.01, 2.0, 8.0):
+        x = logits(rng, 12, n, spread)
+        for rule in (dict(), dict(temperature=0.3), dict(top_k=30, temperature=1.7), dict(top_k=n // 3)):
+            near(sampling, x, rng.random(12).astype(np.float32), **rule)
+
+
+def test_weights_below_a_unit(sampling):  # noqa: F811
+    """One token far above all others, each of which weighs less than half of 2^-40 of it, or just more: all of them together are what rounding may lose, or add."""
+    for n in (151936, 393216):
+        for weight in (2.0 ** -41.2, 2.0 ** -40.8, 2.0 ** -39.5):
+            x = np.full((3, n), np.log(weight), np.float32)
+            x[:, 0] = 0.0
+            near(sampling, x, np.array([0.5, 1 - 2.0 ** -23, 1 - 2.0 ** -24], np.float32))
