@@ -100,11 +100,11 @@ __device__ __forceinline__ float logit_of(u64 order) {
 // f = -1/2, where the next term is 2^-37.1 and its sum 2^-1/2)
 struct Weigher {
     double max, per;  // log2 e / T
-    float top, per32;
+    float top;
     __device__ __forceinline__ double exact(float x) const {
-        const bool far = !((x - top) * per32 >= -100.0f);  // (also where x or T is infinite: weight 0)
-        const double y = far ? 0.0 : ((double)x - max) * per, magic = 6755399441055744.0;  // 1.5 * 2^52
-        const double t = y + magic, f = y - (t - magic);
+        const double at = ((double)x - max) * per, magic = 6755399441055744.0;  // 1.5 * 2^52
+        const bool far = !(at >= -100.0);  // (also where x or T is infinite: weight 0)
+        const double y = far ? 0.0 : at, t = y + magic, f = y - (t - magic);
         const int n = (int)(uint32_t)__double2loint(t);
         double p = 1.01780860092396999e-07;  // ln 2^k / k! for k = 9 to 0
         p = fma(p, f, 1.32154867901443095e-06);
@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(CACHED ? kOneThreads : kManyThreads, CACHED ? 
         return;
     }
     const double per_logit = 1.4426950408889634 / (double)temperature;
-    const Weigher weigh = {(double)top, per_logit, top, (float)fmin(per_logit, 1e38)};
+    const Weigher weigh = {(double)top, per_logit, top};
 
     // the whole part of u times `total`, exactly
     auto target = [&](u64 total) -> u64 {

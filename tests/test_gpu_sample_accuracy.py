@@ -46,3 +46,18 @@ def test_weights_below_a_unit(sampling):  # noqa: F811
             x = np.full((3, n), np.log(weight), np.float32)
             x[:, 0] = 0.0
             near(sampling, x, np.array([0.5, 1 - 2.0 ** -23, 1 - 2.0 ** -24], np.float32))
+
+
+def test_ends_of_the_range(sampling):  # noqa: F811
+    """Logits further apart than f32 reaches, with a temperature as large; and temperatures among f32's smallest, with logits nearer than a normal number to one another."""
+    u = np.array([0.0, 0.3, 0.9, 0.999, 1 - 2.0 ** -24], np.float32)
+    for n in (3, 700, 40000):
+        x = np.tile(np.linspace(3.3e38, -3.3e38, n).astype(np.float32), (5, 1))
+        for T in (1e38, 3e38, 4e37):
+            for rule in (dict(), dict(top_k=2), dict(top_k=n // 2 + 1)):
+                near(sampling, x, u, temperature=T, **rule)
+        x = (-1e-39 * np.arange(n)).astype(np.float32)
+        for T in (1e-44, 1e-41, 3e-39, 1e-38):
+            for rule in (dict(), dict(top_k=2), dict(top_k=n // 2 + 1)):
+                near(sampling, np.tile(x, (5, 1)), u, temperature=T, **rule)
+                assert plain.sample(x, 0.0, T)[0] == 0
