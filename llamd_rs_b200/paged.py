@@ -317,13 +317,11 @@ class Batch:
                            interleaved, plain[6], nq, plain[7], plain[8], plain[9], plain[10])
                 return
             if plain:
-                self._call("append", self._append, _stream_of(q), plain[0], plain[1], plain[2], it, nq, nk, nk, plain[3], plain[4], eps, plain[5], rope_rows, rot,
+                self._call("append", self._append, _stream_here(q), plain[0], plain[1], plain[2], it, nq, nk, nk, plain[3], plain[4], eps, plain[5], rope_rows, rot,
                            interleaved, plain[6], nq, plain[7], plain[8])
                 return
-        scales = ()
-        if eight:
-            _one_device(q, k, v, q_out, k_pages, v_pages, rope, q_norm, k_norm, k_scales, v_scales)
-            scales = self._scales_of(k_scales, v_scales)
+        _one_device(q, k, v, q_out, k_pages, v_pages, rope, q_norm, k_norm, k_scales, v_scales)
+        scales = self._scales_of(k_scales, v_scales) if eight else ()
         qp, qs = self._rows(q, nq, it, "q", strides[0])
         kp, ks = self._rows(k, nk, it, "k", strides[1])
         vp, vs = self._rows(v, nk, it, "v", strides[2])
@@ -362,15 +360,15 @@ class Batch:
             if plain:
                 self._call("attention", self._attention, _stream_here(q), plain[0], n, plain[1], plain[2], plain[4], plain[5], plain[3], n, out_f32, scale)
                 return
-            _one_device(q, k_pages, v_pages, out, k_scales, v_scales)
             scales = self._scales_of(k_scales, v_scales)
         else:
             plain = self._tensors((q, self.type, self.tokens * n, self.tokens), (k_pages, self.type, self._pool, None), (v_pages, self.type, self._pool, None),
                                   (out, 2 if out_f32 else self.type, self.tokens * n, self.tokens))
             if plain:
-                self._call("attention", self._attention, _stream_of(q), plain[0], n, plain[1], plain[2], plain[3], n, out_f32, scale)
+                self._call("attention", self._attention, _stream_here(q), plain[0], n, plain[1], plain[2], plain[3], n, out_f32, scale)
                 return
             scales = ()
+        _one_device(q, k_pages, v_pages, out, k_scales, v_scales)
         qp, qs = self._rows(q, n, self.type, "q")
         op, os_ = self._rows(out, n, 2 if out_f32 else self.type, "out")
         kp, vp = self._whole(k_pages, c, self._pool, "k_pages"), self._whole(v_pages, c, self._pool, "v_pages")
