@@ -35,7 +35,8 @@ inline int decode_piece(long long positions, int n_head_kv, int sms) {
 }
 
 // paged_decode8.cu runs kDecode8Ctas CTAs to an SM. A piece costs about as much as kDecode8Piece positions to begin and end (a pipeline's filling and the join of four
-// warps), the launch that joins cut pieces as much as kDecode8Join; a piece has kDecode8Least positions at least (one step of each warp).
+// warps), the launch that joins cut pieces as much as kDecode8Join; a CTA's share has room for a piece of kDecode8Least positions at least (one step of each warp). A run that is
+// cut leaves pieces of 64 positions and more, its last of 32 and more: at a list's end half the warps may have nothing to do.
 constexpr int kDecode8Piece = 64, kDecode8Join = 256, kDecode8Least = 128;
 
 // A stretch's positions for some tokens, and the cuts that deal it out: pieces [first, first + n) of CTA cta.
