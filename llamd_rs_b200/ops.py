@@ -263,7 +263,11 @@ def sample(x, uniform, temperature=None, top_k=None, top_p=None, min_p=None):
     x = _f32(x)
     x2 = x.reshape(-1, x.shape[-1])
     rows, n = x2.shape
-    per_row = lambda a, t: None if a is None else DevBuf.from_array(np.ascontiguousarray(np.broadcast_to(np.asarray(a, dtype=t), (rows,))))  # noqa: E731
+    if top_k is not None:
+        k = np.asarray(top_k)
+        if k.dtype.kind not in "iuf" or not np.all((k >= -2 ** 31) & (k < 2 ** 31) & (k == np.floor(k))):
+            raise Malformed(f"sample: top_k {top_k!r} is not whole numbers of 32 bits")
+    per_row = lambda a, t: None if a is None else DevBuf.from_array(np.ascontiguousarray(np.broadcast_to(np.asarray(a).astype(t), (rows,))))  # noqa: E731
     dx, token, prob = DevBuf.from_array(x2), DevBuf(4 * rows), DevBuf(4 * rows)
     du, dt, dk, dp, dm = (per_row(a, t) for a, t in ((uniform, np.float32), (temperature, np.float32), (top_k, np.int32), (top_p, np.float32), (min_p, np.float32)))
     sampling.sample(dx, du, token, dt, dk, dp, dm, prob, rows=rows, n_vocab=n)
