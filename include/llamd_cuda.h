@@ -489,9 +489,9 @@ int llamd_fwd_paged_append(const void *batch, const void *q, const void *k, cons
                            int rope_rows, int rot, int interleaved, void *q_out, size_t out_stride, void *k_pages, void *v_pages);
 /* The same into a cache in 8 bits. A block's scale is the least power of two with which its new values fit (between 2^-24 and 2^9 for I8, 2^-15 and 2^7 for
  * E4M3: every value is then exact in f16), and no less than it was where the block holds older positions of the sequence: their codes are rounded
- * again when it grows. Values are rounded to even; larger ones than the largest scale takes (65024, 57344), infinities among them, become the largest; a NaN
- * counts for nothing in a scale, and becomes 0 in I8. Rows and scales
- * without new tokens, and rows behind a sequence's last, stay as they are. A page that new tokens go to belongs to one
+ * again when it grows. (The scales of such blocks are an append8's: with a byte of 255, e8m0's NaN, the block's codes become anything.) Values are rounded to
+ * even; larger ones than the largest scale takes (65024, 57344), infinities among them, become the largest; a NaN counts for nothing in a scale, and becomes 0
+ * in I8. Rows and scales without new tokens, and rows behind a sequence's last, stay as they are. A page that new tokens go to belongs to one
  * sequence: refused where two of the batch's would write to one. */
 int llamd_fwd_paged_append8(const void *batch, const void *q, const void *k, const void *v, int in_type, size_t q_stride,
                             size_t k_stride, size_t v_stride, const float *wq, const float *wk, float eps, const float *rope_tab,
