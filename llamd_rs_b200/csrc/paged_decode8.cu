@@ -7,8 +7,8 @@
 // scores, its V scale the codes: 2^eV cV is in f16 too, with every scale of an append's, so that an output is off by the rounding of the weights 2^(s - m) alone, whatever other
 // blocks' scales are. In i8 the bias that is taken off a code goes times the scale in the same instruction; 1152 2^e is in f16 up to e = 5, and the up to 2^4 above go
 // into the block's weights, as whatever a scale has beyond an append's does: m is about the maximum of s + r, r that rest of log2 of the V scale, and the
-// denominator sums 2^(s + r - m) 2^-r in f32. (The whole scale in the weights was as fast, 148 sequences of 4096 positions 102 to 105 us either way, 256 behind 4096
-// shared ones 56.2 and 57.4, but a block with one large element then cost the other blocks' weights their bits, from 2^26 between scales on.)
+// denominator sums 2^(s + r - m) 2^-r in f32. (The whole scale in the weights was as fast, 148 sequences of 4096 positions in the same time, 256 behind 4096
+// shared ones 56.2 us for 57.4, but a block with one large element then cost the other blocks' weights their bits, from 2^26 between scales on.)
 //
 // Which codes a lane holds as the products' first operand is free as long as the second follows. K: 16 bytes of rows g and g + 8 (g = lane / 4, t = lane % 4) are the
 // contraction's elements of four steps; q is read in the same order. V: hd / 8 bytes of rows 2t, 2t + 1, 2t + 8, 2t + 9; bytes of two rows
@@ -17,7 +17,7 @@
 //
 // Halved bytes leave a slice's chain of steps (codes, scores, maximum, weights, values) as what is waited for: a warp takes two scale blocks at a time, and the maximum is
 // taken over the warp's lanes only where a score is more than 2^3 above m (weights are at most 2^3, and 2^12 times that in f16 until the end). Three slices of a
-// warp on their way and two CTAs to an SM; two slices and three CTAs: 148 sequences of 4096 positions 131 us where these take 100 (6.2 TB/s).
+// warp on their way and two CTAs to an SM; two slices and three CTAs: 148 sequences of 4096 positions 131 us where these take 102 to 105 (6.0 TB/s).
 #include "paged8.cuh"
 #include "paged_mma.cuh"
 

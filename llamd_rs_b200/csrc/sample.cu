@@ -14,12 +14,14 @@
 // is cut in bins again, of (logit, index) compared as one number, until kList or fewer are in it, which are sorted. What is kept then, or where min-p is the only limit, is
 // weighed tile by tile of 128 neighbours, and the tile that u falls on looked through.
 // Few rows are kept in shared memory, each looked at there; of many, parts are read again, from L2.
-// What bounds it: one row, the joins of the cluster one behind the other, three with a small k (151936 tokens, k 20: 13.6 us, 31k cycles: the first look 5k, the top 5k, the second look
-// 10k, CTA 0 for itself 11k), some ten in the long way. Many rows without a k, an exponential in 64 bits for each token, some 20 operations at 64 a clock and SM and a conversion at 16, for
-// the histogram and, where more than the lists' are kept, for the tiles: 64 rows of 16 bits with tens of thousands kept 116 us, of whose 175k cycles the histogram takes 50k and the
-// tiles 40k. 128 rows of 151936 f32, each with its own limits, a fifth with k 5000 and a fifth without: 107 us; those with a small k alone are the least of it.
-// CTAs of 256 threads, four to an SM: a batch's rows wait for one another's joins less than with 512 and two (163 us where 246 were). Counting instead of sorting up to a thread to
-// a token, and lists in place of the row once few matter, took 130 to 107.
+// What bounds it: one row, the joins of the cluster one behind the other, three with a small k (151936 tokens, k 20: 13.7 us, 31k cycles: the first look 5k, the top 5k, the second look
+// 10k, CTA 0 for itself 11k), some ten in the long way. Many rows, no pipe: latency and joins, with issue slots busy in 43 to 48 of 100 cycles, the fp64 pipe in 6 to 16 and HBM in 2 to 10.
+// Every instance is held at 64 registers, for four CTAs (or 1024 threads) to an SM, and spills (280 to 296 bytes a thread). Without a small k each token takes an
+// exponential in 64 bits, some 20 operations, for the histogram and, where more than the lists' are kept, for the tiles: 64 rows of 16 bits with tens of thousands kept 115 us, of whose
+// 175k cycles the histogram takes 50k and the tiles 40k. 128 rows of 151936 f32, us: k 20 49, min-p alone 80, no limit 80, top-p alone 168, each with its own limits, a fifth
+// with k 5000 and a fifth without, 108. One row: 13.7, 15.5, 15.6, 43.
+// CTAs of 256 threads, four to an SM: a batch's rows wait for one another's joins less than with 512 and two (163 us where 246 were). Histograms by carry and lists in place of the row
+// once few matter took that to 130, counting instead of sorting up to a thread to a token to 121, weights four at a time and one atomic a warp for the lists to 107.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
