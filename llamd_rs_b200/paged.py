@@ -63,43 +63,49 @@ def _int(x, what, below=2 ** 31):
     return n
 
 
-def _stream_of(*buffers):
-    """torch's current stream (a cudaStream_t) where one of the buffers is a tensor, else None."""
-    for x in buffers:
-        if hasattr(x, "data_ptr") and x.is_cuda:
-            torch = sys.modules["torch"]
-            raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # (0.1 us; the public way makes an object of it, 2.4 us)
-            return raw(x.get_device()) if raw else torch.cuda.current_stream(x.device).cuda_stream
-    return None
-
-
 def _one_device(*buffers):
-    """Refuses tensors that are not all on the current device: the library has that one, and another's memory may be out of a kernel's reach."""
+    """Refuses tensors that are not all on the current device: the library has that one, and another's memory may be out of a kernel's reach. -> the device, None
+    where no buffer is a tensor."""
     here = None
     for x in buffers:
-        if x is not None and hasattr(x, "get_device"):
+        if x is None:
+            continue
+        try:
             at = x.get_device()
-            if at != here:
-                if here is not None:
-                    raise ShapeError(f"tensors on devices {here} and {at}")
-                here = at
+        except AttributeError:  # (an address, a DevBuf)
+            continue
+        if at != here:
+            if here is not None:
+                raise ShapeError(f"tensors on devices {here} and {at}")
+            here = at
     if here is not None:
+        if here < 0:
+            raise ShapeError("a tensor that is not on a device")
         torch = sys.modules["torch"]
         current = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)()
         if here != current:
             raise ShapeError(f"tensors on device {here} where {current} is the current one")
+    return here
+
+
+def _stream_at(device):
+    """torch's current stream (a cudaStream_t) on _one_device's device."""
+    if device is None:
+        return None
+    torch = sys.modules["torch"]
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # (0.1 us; the public way makes an object of it, 2.4 us)
+    return raw(device) if raw else torch.cuda.current_stream(device).cuda_stream
 
 
 def _stream_here(x):
-    """_stream_of a tensor that is to be on the current device."""
+    """The same of one tensor that is to be on the current device."""
     c, at = sys.modules["torch"]._C, x.get_device()
     try:
         if at == c._cuda_getDevice():
             return c._cuda_getCurrentRawStream(at)
     except AttributeError:
         pass
-    _one_device(x)
-    return _stream_of(x)
+    return _stream_at(_one_device(x))
 
 
 def _refuse(what):
@@ -228,10 +234,11 @@ class Batch:
     @staticmethod
     def _tensors(*wanted):
         """The addresses of (tensor, type, values at least, rows) that are all as plain as can be and on one device, or None: then each is looked at for itself."""
-        found, device = [], wanted[0][0].get_device() if hasattr(wanted[0][0], "get_device") else -1
-        if device < 0:
-            return None
+        found = []
         try:
+            device = wanted[0][0].get_device()
+            if device < 0:
+                return None
             for x, type_, n, rows in wanted:
                 if _seen.get(x.dtype) != type_ or x.get_device() != device or not x.is_contiguous() or x.numel() < n or (rows is not None and (x.shape[0] != rows or x.numel() != n)):
                     return None
@@ -251,8 +258,8 @@ class Batch:
                     raise ShapeError(f"{what}: {x.nbytes} bytes for {self.tokens} tokens") from None
                 return x.ptr, stride
             return x, stride
-        if _type_of(x) != type_ or not x.is_cuda:
-            raise ShapeError(f"{what}: {x.dtype} on {x.device}")
+        if _seen.get(x.dtype) != type_ and _type_of(x) != type_:
+            raise ShapeError(f"{what}: {x.dtype}")
         if x.numel() == self.tokens * n:
             if x.is_contiguous() and (not self.tokens or x.shape[0] == self.tokens):
                 return ptr, n
@@ -271,7 +278,7 @@ class Batch:
                     raise ShapeError(f"{what}: {x.nbytes} bytes for {n} values") from None
                 return x.ptr
             return x
-        if _type_of(x) != type_ or x.numel() < n or not x.is_contiguous() or not x.is_cuda:
+        if (_seen.get(x.dtype) != type_ and _type_of(x) != type_) or x.numel() < n or not x.is_contiguous():
             raise ShapeError(f"{what}: {x.dtype}, {tuple(x.shape)} on {x.device} for {n} values")
         return ptr
 
@@ -320,13 +327,13 @@ class Batch:
                 self._call("append", self._append, _stream_here(q), plain[0], plain[1], plain[2], it, nq, nk, nk, plain[3], plain[4], eps, plain[5], rope_rows, rot,
                            interleaved, plain[6], nq, plain[7], plain[8])
                 return
-        _one_device(q, k, v, q_out, k_pages, v_pages, rope, q_norm, k_norm, k_scales, v_scales)
+        stream = _stream_at(_one_device(q, k, v, q_out, k_pages, v_pages, rope, q_norm, k_norm, k_scales, v_scales))
         scales = self._scales_of(k_scales, v_scales) if eight else ()
         qp, qs = self._rows(q, nq, it, "q", strides[0])
         kp, ks = self._rows(k, nk, it, "k", strides[1])
         vp, vs = self._rows(v, nk, it, "v", strides[2])
         op, os_ = self._rows(q_out, nq, self.type, "q_out")
-        self._call("append", self._append, _stream_of(q, k, v, q_out, k_pages, v_pages, rope, q_norm, k_norm, k_scales, v_scales), qp, kp, vp, it, qs, ks, vs,
+        self._call("append", self._append, stream, qp, kp, vp, it, qs, ks, vs,
                    None if q_norm is None else self._whole(q_norm, 2, D, "q_norm"), None if k_norm is None else self._whole(k_norm, 2, D, "k_norm"), eps,
                    self._whole(rope, 2, rope_rows * rot, "rope") if rot else None, rope_rows, rot, interleaved, op, os_,
                    self._whole(k_pages, c, self._pool, "k_pages"), self._whole(v_pages, c, self._pool, "v_pages"), *scales)
@@ -360,19 +367,18 @@ class Batch:
             if plain:
                 self._call("attention", self._attention, _stream_here(q), plain[0], n, plain[1], plain[2], plain[4], plain[5], plain[3], n, out_f32, scale)
                 return
-            scales = self._scales_of(k_scales, v_scales)
         else:
             plain = self._tensors((q, self.type, self.tokens * n, self.tokens), (k_pages, self.type, self._pool, None), (v_pages, self.type, self._pool, None),
                                   (out, 2 if out_f32 else self.type, self.tokens * n, self.tokens))
             if plain:
                 self._call("attention", self._attention, _stream_here(q), plain[0], n, plain[1], plain[2], plain[3], n, out_f32, scale)
                 return
-            scales = ()
-        _one_device(q, k_pages, v_pages, out, k_scales, v_scales)
+        stream = _stream_at(_one_device(q, k_pages, v_pages, out, k_scales, v_scales))
+        scales = self._scales_of(k_scales, v_scales)
         qp, qs = self._rows(q, n, self.type, "q")
         op, os_ = self._rows(out, n, 2 if out_f32 else self.type, "out")
         kp, vp = self._whole(k_pages, c, self._pool, "k_pages"), self._whole(v_pages, c, self._pool, "v_pages")
-        self._call("attention", self._attention, _stream_of(q, k_pages, v_pages, out, k_scales, v_scales), qp, qs, kp, vp, *scales, op, os_, out_f32, scale)
+        self._call("attention", self._attention, stream, qp, qs, kp, vp, *scales, op, os_, out_f32, scale)
 
     def free(self) -> None:
         if self.ptr:

@@ -8,7 +8,7 @@ from __future__ import annotations
 
 from ._lib import lib
 from .backend import DevBuf, Malformed, ShapeError, Unsupported
-from .paged import TYPES, _int, _one_device, _refuse, _stream_of, _type_of
+from .paged import TYPES, _int, _one_device, _refuse, _stream_at, _type_of
 
 MOST_TOKENS = 393216
 _SIZE = {0: 2, 1: 2, 2: 4}
@@ -60,9 +60,7 @@ def sample(logits, uniform, token, temperature=None, top_k=None, top_p=None, min
     at = [_of_rows(x, rows, d, what) for x, d, what in ((temperature, "torch.float32", "temperature"), (top_k, "torch.int32", "top_k"), (top_p, "torch.float32", "top_p"),
                                                         (min_p, "torch.float32", "min_p"), (uniform, "torch.float32", "uniform"), (token, "torch.int32", "token"),
                                                         (prob, "torch.float32", "prob"))]
-    _one_device(logits, uniform, token, temperature, top_k, top_p, min_p, prob)
-    L = lib()
-    stream = _stream_of(logits, uniform, token, temperature, top_k, top_p, min_p, prob)
+    stream, L = _stream_at(_one_device(logits, uniform, token, temperature, top_k, top_p, min_p, prob)), lib()
     if stream is not None and L.llamd_fwd_wait_stream(stream) != 0:
         _refuse("sample")
     if L.llamd_fwd_sample(ptr, t, stride, rows, n_vocab, *at) != 0:
