@@ -534,10 +534,12 @@ __global__ void __launch_bounds__(CACHED ? kOneThreads : kManyThreads, CACHED ? 
                 const u64 w = Weigher::units(exact);
                 u64 all, kept;
                 u64 before = block_prefix<kThreads>(w, sh.scratch, all);
-                const bool keep = of_k && (!i || !by_mass || (double)before < (double)p_in * (double)all) && exact >= least_weight;
+                // (the first so many: weights fall with the order, but for the exponential's last bit)
+                const int n_kept = __syncthreads_count(of_k && (!i || !by_mass || (double)before < (double)p_in * (double)all) && exact >= least_weight);
+                const bool keep = i < n_kept;
                 block_prefix<kThreads>(keep ? w : 0, sh.scratch, kept);
                 if (keep) sh.list[i] = (uint32_t)o, sh.weight[i] = w;
-                const int n_kept = __syncthreads_count(keep);
+                __syncthreads();
                 if (keep) {
                     in_front(n_kept, (uint32_t)o, before);
                     const u64 want = target(kept);
@@ -566,21 +568,18 @@ __global__ void __launch_bounds__(CACHED ? kOneThreads : kManyThreads, CACHED ? 
                     const u64 w = sh.weight[i];
                     const bool keep = i < kept_k && (!i || !by_mass || (double)before < limit) && weigh.exact(logit_of(sh.list[i])) >= least_weight;
                     before += w;
-                    if (!keep) sh.weight[i] = 0;
-                    part += keep ? w + (1ull << 52) : 0;  // (in the top bits: how many; weights are 2^50 at most in all)
+                    part += keep;
                 }
-                u64 kept;
-                block_prefix<kThreads>(part, sh.scratch, kept);
-                // the kept ones are the first of the list: by rising index, (index, place in order) sorted
-                const int n_kept = (int)(kept >> 52), size_kept = padded(n_kept);
-                kept &= (1ull << 52) - 1;
+                block_prefix<kThreads>(part, sh.scratch, all);
+                // the kept ones are the first so many of the list (weights fall with it, but for the exponential's last bit): by rising index, (index, place in order) sorted
+                const int n_kept = (int)all, size_kept = padded(n_kept);
                 __syncthreads();
                 for (int i = threadIdx.x; i < size_kept; i += kThreads) sh.list[i] = i < n_kept ? (sh.list[i] & 0xFFFFFFFFull) << 32 | (uint32_t)i : ~0ull;
                 sort_list<kThreads>(sh.list, size_kept);
                 part = 0;
                 const int last = min(end, n_kept);
                 for (int i = begin; i < last; i++) part += sh.weight[(uint32_t)sh.list[i]];
-                u64 run = block_prefix<kThreads>(part, sh.scratch, all);
+                u64 kept, run = block_prefix<kThreads>(part, sh.scratch, kept);
                 const u64 want = target(kept);
                 for (int i = begin; i < last; i++) {
                     const u64 w = sh.weight[(uint32_t)sh.list[i]];

@@ -61,3 +61,25 @@ def test_ends_of_the_range(sampling):  # noqa: F811
             for rule in (dict(), dict(top_k=2), dict(top_k=n // 2 + 1)):
                 near(sampling, np.tile(x, (5, 1)), u, temperature=T, **rule)
                 assert plain.sample(x, 0.0, T)[0] == 0
+
+
+# The largest logit, temperature, min_p and j: logits (j - 1) 2^-53 and j 2^-53 have weights that are min_p and the number of 64 bits just below, in this order: the smaller logit's is the larger (a last
+# bit of the series). Found by trying some 10^10.
+TURNED = [("0x1.4e471cp-1", "0x1.085846p+1", "0x1.753a18p-1", 50), ("0x1.92d2fep-1", "0x1.3319cp+1", "0x1.70da7ap-1", -54), ("0x1.3bd1b8p-1", "0x1.2973ep+1", "0x1.88a354p-1", -45),
+          ("0x1.97fa18p-1", "0x1.2a6efap+1", "0x1.6bc89cp-1", 62), ("0x1.4d82d4p-1", "0x1.0de482p+1", "0x1.77ed56p-1", -4)]
+
+
+@pytest.mark.parametrize("k,n,rows", [(3, 9, 4), (3, 20000, 4), (40, 5000, 300), (400, 5000, 300), (300, 40000, 64)])
+def test_a_last_bit_at_min_p(sampling, k, n, rows):  # noqa: F811
+    """Two logits at min_p whose weights are in the wrong order: two tokens are kept, the largest and one of these, and every number falls on one of them."""
+    u = ((np.arange(rows) + 0.5) / rows).astype(np.float32)
+    for top, T, m, j in TURNED:
+        top, T, m = (np.float32(float.fromhex(v)) for v in (top, T, m))
+        x = np.tile(np.linspace(-3, -5, n).astype(np.float32), (rows, 1))
+        x[:, :3] = [(j - 1) * 2.0 ** -53, top, j * 2.0 ** -53]
+        got, share = run(sampling, x, u, temperature=T, top_k=k, min_p=m)
+        assert set(got.tolist()) <= {0, 1, 2} and {0, 2} - set(got.tolist())
+        assert np.allclose(share, np.where(got == 1, 1 / (1 + m), m / (1 + m)), rtol=1e-6)
+        near_top = np.sum(got == 1) / rows
+        assert abs(near_top - 1 / (1 + m)) <= 1.001 / rows
+        assert np.array_equal(got, run(sampling, x, u, temperature=T, top_k=k, min_p=m)[0])
