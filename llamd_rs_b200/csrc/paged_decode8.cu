@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(kWarps * 32, kDecode8Ctas) paged_decode8_kerne
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 // the largest to [2^8, 2^9): sums of 128 products with codes stay far below f32's limits; a row of nothing, or with an infinity, as it is
                 const int e = (__float_as_int(top) >> 23) - (127 + 8);
-                const bool fits = e > -126 && e < 119;
+                const bool fits = e > -126 && e < 120;  // (120: an infinity)
                 const float by = fits ? __int_as_float((127 - e) << 23) : 1.0f;
                 down = fits ? __int_as_float((127 + e) << 23) : 1.0f;
 #pragma unroll

@@ -4,6 +4,7 @@ import pytest
 
 import paged8_plain as plain8
 import paged_plain as plain
+from test_gpu_paged import close
 from test_gpu_paged8 import run_attention8
 
 pytestmark = pytest.mark.gpu
@@ -100,3 +101,15 @@ def test_many_rows(paged, cache, dtype, H, K, D, q_len, kv_len, n_shared):
     """The kernel of many query rows, of either type: weights and V in f16, as in that of few."""
     for edit in (None, far_apart(cache, dtype, 0.0), far_apart(cache, dtype, 5.0)):
         compare(paged, cache, H, K, D, dtype, q_len, kv_len, edit, max(2.0 ** -32, FEW[cache]), n_shared)
+
+
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("D", [64, 128])
+def test_the_largest_queries(paged, cache, D):
+    """bf16 rows of which each element is near the type's largest: finite scores, by a small scale, in both kernels."""
+    def largest(q, k, v, tables):
+        sign = np.random.default_rng(1).choice([-1.0, 1.0], q.shape)
+        q[:] = plain.to_bits((sign * np.linspace(1.5e38, 3.3e38, q.size).reshape(q.shape)).astype(np.float32), "bf16")
+
+    for q_len, kv_len in (([1, 2], [90, 40]), ([1], [2000]), ([60], [200])):
+        close(*run_attention8(paged, cache, 8, 2, D, 16, "bf16", q_len, kv_len, edit=largest, scale=1.3e-38, low=-12, high=-8))
